@@ -331,6 +331,46 @@ int ttt_layer_qk_conv_backward(const ttt_dims* d, const void* grad_q, const void
                                float* grad_q_params, float* grad_k_params, void* workspace, size_t workspace_bytes,
                                void* stream);
 
+/* ---- gated linear recurrence ---------------------------------------------------------------------------------
+ * An inner model beside TTT-Linear whose update is linear in the state (no counterpart in the reference):
+ *     W_t = exp(log_decay_t) W_{t-1} + beta_t k_t^T v_t,      o_t = q_t W_t
+ * for every (batch, head) stream: a gradient step per token on -<k W, v> with weight decay.  Of `d`, batch, heads, seq_len (any
+ * length), head_dim (64 or 32; any number of heads) and dtype are read.
+ *   xq, xk, xv    T [B,H,T,F] with rows of F contiguous elements; `strides`: for each of them the strides of batch, head and token
+ *                 in elements, positive multiples of 16 bytes (null: contiguous [B,H,T,F]); strides of dimensions of size 1 are not read
+ *   log_decay     float32 [B,H,T], not above 0 for a state that does not grow; -infinity (anything below -111) forgets everything
+ *                 before the token: sequences may follow one another in one row
+ *   beta          float32 [B,H,T], or null: ones
+ *   weight        float32 [B,H,F,F] state before the first token, W[k][v], or null: zeros
+ *   output        T [B,H,T,F] (out);  weight_out  float32 [B,H,F,F] (out) state behind the last token
+ *   saved         (out) ttt_linear_gated_saved_bytes(d) bytes for the backward: the state before every 64 tokens, opaque; null
+ *                 (with 0 bytes) for inference
+ *   workspace     ttt_linear_gated_*_workspace_bytes(d) bytes (0 for many streams; null then)
+ * The state is float32 throughout, and what results of type float32 depend on is not rounded to bf16 on the way.  A NaN or an
+ * infinity in a token reaches the outputs of the 64 tokens around it, those before it among them.
+ *
+ * ttt_linear_gated_backward: gradients for loss = <grad_output, output> + <grad_weight_out, weight_out> (grad_weight_out null:
+ * zero).  `strides`: of xq, xk, xv and grad_output.  grad_xq, grad_xk, grad_xv T [B,H,T,F] contiguous, grad_log_decay, grad_beta
+ * (null exactly where beta is) float32 [B,H,T], grad_weight float32 [B,H,F,F]; all written.  grad_log_decay is 0 where exp(log_decay) is.
+ *
+ * ttt_linear_gated_step: the forward over 1 to 16 tokens (token-by-token generation); weight_out may be weight.
+ */
+size_t ttt_linear_gated_saved_bytes(const ttt_dims* d);
+size_t ttt_linear_gated_forward_workspace_bytes(const ttt_dims* d);
+int ttt_linear_gated_forward(const ttt_dims* d, const void* xq, const void* xk, const void* xv, const int64_t* strides,
+                             const float* log_decay, const float* beta, const float* weight, void* output,
+                             float* weight_out, void* saved, size_t saved_bytes, void* workspace,
+                             size_t workspace_bytes, void* status, void* stream);
+size_t ttt_linear_gated_backward_workspace_bytes(const ttt_dims* d);
+int ttt_linear_gated_backward(const ttt_dims* d, const void* xq, const void* xk, const void* xv,
+                              const void* grad_output, const int64_t* strides, const float* log_decay,
+                              const float* beta, const void* saved, size_t saved_bytes, const float* grad_weight_out,
+                              void* grad_xq, void* grad_xk, void* grad_xv, float* grad_log_decay, float* grad_beta,
+                              float* grad_weight, void* workspace, size_t workspace_bytes, void* status, void* stream);
+int ttt_linear_gated_step(const ttt_dims* d, const void* xq, const void* xk, const void* xv, const int64_t* strides,
+                          const float* log_decay, const float* beta, const float* weight, void* output,
+                          float* weight_out, void* stream);
+
 /* Backward without a caller workspace.  (No counterpart in the reference: its host wrapper always allocates its
  * scratch itself, backward/launch.rs:389-392.)
  *

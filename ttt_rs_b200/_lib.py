@@ -77,6 +77,12 @@ SYMBOLS = {
                                         _P, _P, _P, _P, _P, _P, _P]),
     "ttt_layer_qk_conv": (C.c_int, [_DP, _P, C.c_int64, _P, _P, _P, _P, _P, _P, _P]),
     "ttt_layer_qk_conv_backward_workspace_bytes": (C.c_size_t, [_DP]),
+    "ttt_linear_gated_saved_bytes": (C.c_size_t, [_DP]),
+    "ttt_linear_gated_forward_workspace_bytes": (C.c_size_t, [_DP]),
+    "ttt_linear_gated_forward": (C.c_int, [_DP] + [_P] * 9 + [_P, C.c_size_t, _P, C.c_size_t, _P, _P]),
+    "ttt_linear_gated_backward_workspace_bytes": (C.c_size_t, [_DP]),
+    "ttt_linear_gated_backward": (C.c_int, [_DP] + [_P] * 8 + [C.c_size_t] + [_P] * 8 + [C.c_size_t, _P, _P]),
+    "ttt_linear_gated_step": (C.c_int, [_DP] + [_P] * 10),
     "ttt_layer_qk_conv_backward": (C.c_int, [_DP, _P, _P, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
 }
 # entry points of this package alone (csrc/ttt_internal.h)

@@ -1230,3 +1230,261 @@ extern "C" int ttt_internal_mlp_backward(const ttt_dims* d, const void* xq, cons
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "MLP backward launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;
 }
+
+// ---- gated linear recurrence -------------------------------------------------------------------------------------------
+namespace {
+
+constexpr int kGatedChunk = 64;
+
+int check_gated_dims(const ttt_dims* d) {
+  if (d == nullptr) return fail(TTT_ERR_NULL, "dims is null");
+  if (d->batch <= 0 || d->heads <= 0 || d->seq_len <= 0)
+    return fail(TTT_ERR_SHAPE, "batch, heads and seq_len must be positive");
+  if (d->dtype != TTT_F32 && d->dtype != TTT_BF16) return fail(TTT_ERR_UNSUPPORTED, "unknown dtype %d", d->dtype);
+  if (d->head_dim != 64 && d->head_dim != 32)
+    return fail(TTT_ERR_UNSUPPORTED, "Unsupported head_dim=%d (supported: 64, 32)", d->head_dim);
+  if ((int64_t)d->batch * d->heads * 64 >= (int64_t)1 << 31 || d->seq_len >= (1 << 30))
+    return fail(TTT_ERR_SHAPE, "batch*heads must be below 2^25, seq_len below 2^30");
+  return TTT_OK;
+}
+
+// Strides (batch, head, token; in elements) of tensor number `i` of a call; null: contiguous [B,H,T,F]
+struct GatedStrides {
+  int64_t s[3];
+};
+int gated_strides(GatedStrides* out, const ttt_dims* d, const int64_t* strides, int i, const char* name) {
+  const int64_t F = d->head_dim, T = d->seq_len;
+  const int64_t size[3] = {d->batch, d->heads, T}, dense[3] = {d->heads * T * F, T * F, F};
+  for (int k = 0; k < 3; ++k) {
+    const int64_t v = strides != nullptr && size[k] > 1 ? strides[3 * i + k] : dense[k];
+    if (v <= 0 || v * (d->dtype == TTT_BF16 ? 2 : 4) % 16 != 0 || v >= (int64_t)1 << 37)
+      return fail(TTT_ERR_ALIGN, "the strides of %s must be positive multiples of 16 bytes", name);
+    out->s[k] = v;
+  }
+  return TTT_OK;
+}
+// 4-D view (features, tokens, heads, batch) of a [B,H,T,F] tensor with any strides; box = the rows of one chunk.  A box that
+// reaches behind the sequence reads zeros there.  bf16 rows are swizzled over their whole length, float32 rows are not.
+int make_gated_map(CUtensorMap* m, const void* base, const ttt_dims* d, const int64_t* strides, int i, const char* name) {
+  GatedStrides s;
+  const int rc = gated_strides(&s, d, strides, i, name);
+  if (rc != TTT_OK) return rc;
+  EncodeFn enc = get_encode_fn();
+  if (enc == nullptr) return fail(TTT_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available");
+  const bool bf = d->dtype == TTT_BF16;
+  const cuuint64_t es = bf ? 2 : 4, F = (cuuint64_t)d->head_dim;
+  const cuuint64_t dims[4] = {F, (cuuint64_t)d->seq_len, (cuuint64_t)d->heads, (cuuint64_t)d->batch};
+  const cuuint64_t pitch[3] = {(cuuint64_t)s.s[2] * es, (cuuint64_t)s.s[1] * es, (cuuint64_t)s.s[0] * es};
+  const cuuint32_t box[4] = {(cuuint32_t)F, kGatedChunk, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapSwizzle sw = !bf ? CU_TENSOR_MAP_SWIZZLE_NONE : F == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  const CUresult r = encode_tiled(enc, m, bf ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
+                                  const_cast<void*>(base), dims, pitch, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TTT_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return TTT_OK;
+}
+
+// How a call's streams are cut: segments per stream, chunks per segment
+struct GatedCut {
+  int chunks, nseg, seg_chunks;
+  size_t state_floats, total_bytes;  // workspace: a state per segment, then a decay per segment
+};
+GatedCut gated_cut(const ttt_dims* d, bool backward) {
+  GatedCut c;
+  c.chunks = (d->seq_len + kGatedChunk - 1) / kGatedChunk;
+  const int64_t streams = (int64_t)d->batch * d->heads;
+  c.nseg = ttt::gated_segments(streams, c.chunks, backward);
+  c.seg_chunks = (c.chunks + c.nseg - 1) / c.nseg;
+  c.nseg = (c.chunks + c.seg_chunks - 1) / c.seg_chunks;
+  c.state_floats = c.nseg > 1 ? (size_t)streams * c.nseg * d->head_dim * d->head_dim : 0;
+  c.total_bytes = c.nseg > 1 ? (c.state_floats + (size_t)streams * c.nseg) * sizeof(float) : 0;
+  return c;
+}
+int check_gated_workspace(const GatedCut& c, const void* workspace, size_t bytes) {
+  if (c.total_bytes == 0) return TTT_OK;
+  if (workspace == nullptr || bytes < c.total_bytes)
+    return fail(TTT_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", workspace == nullptr ? (size_t)0 : bytes, c.total_bytes);
+  if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return fail(TTT_ERR_ALIGN, "workspace is not 16-byte aligned");
+  return TTT_OK;
+}
+int check_optional(const char* name, const void* p, unsigned align) {
+  if ((reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0) return fail(TTT_ERR_ALIGN, "%s is not %u-byte aligned", name, align);
+  return TTT_OK;
+}
+size_t gated_saved_bytes(const ttt_dims* d) {
+  return (size_t)d->batch * d->heads * ((d->seq_len + kGatedChunk - 1) / kGatedChunk) * d->head_dim * d->head_dim * 4;
+}
+
+}  // namespace
+
+extern "C" size_t ttt_linear_gated_saved_bytes(const ttt_dims* d) {
+  return check_gated_dims(d) == TTT_OK ? gated_saved_bytes(d) : 0;
+}
+extern "C" size_t ttt_linear_gated_forward_workspace_bytes(const ttt_dims* d) {
+  return check_gated_dims(d) == TTT_OK ? gated_cut(d, false).total_bytes : 0;
+}
+extern "C" size_t ttt_linear_gated_backward_workspace_bytes(const ttt_dims* d) {
+  return check_gated_dims(d) == TTT_OK ? gated_cut(d, true).total_bytes : 0;
+}
+
+extern "C" int ttt_linear_gated_forward(const ttt_dims* d, const void* xq, const void* xk, const void* xv,
+                                        const int64_t* strides, const float* log_decay, const float* beta,
+                                        const float* weight, void* output, float* weight_out, void* saved,
+                                        size_t saved_bytes, void* workspace, size_t workspace_bytes, void* status,
+                                        void* stream) {
+  int rc = check_gated_dims(d);
+  if (rc != TTT_OK) return rc;
+  const NamedPtr ptrs[] = {{"xq", xq}, {"xk", xk}, {"xv", xv}, {"output", output}, {"weight_out", weight_out}};
+  if ((rc = check_ptrs(ptrs, 5)) != TTT_OK) return rc;
+  if (log_decay == nullptr) return fail(TTT_ERR_NULL, "log_decay is null");
+  if ((rc = check_optional("log_decay", log_decay, 4)) != TTT_OK || (rc = check_optional("beta", beta, 4)) != TTT_OK ||
+      (rc = check_optional("weight", weight, 16)) != TTT_OK || (rc = check_optional("saved", saved, 16)) != TTT_OK ||
+      (rc = check_optional("status", status, 4)) != TTT_OK)
+    return rc;
+  if (saved != nullptr && saved_bytes < gated_saved_bytes(d))
+    return fail(TTT_ERR_WORKSPACE, "saved has %zu bytes, %zu needed", saved_bytes, gated_saved_bytes(d));
+  const GatedCut cut = gated_cut(d, false);
+  if ((rc = check_gated_workspace(cut, workspace, workspace_bytes)) != TTT_OK) return rc;
+  ttt::GatedMaps maps{};
+  const void* bases[3] = {xq, xk, xv};
+  const char* names[3] = {"xq", "xk", "xv"};
+  GatedStrides checked;
+  for (int i = 0; i < 3; ++i)
+    if ((rc = gated_strides(&checked, d, strides, i, names[i])) != TTT_OK) return rc;
+  for (int i = 0; i < 3; ++i)
+    if ((rc = make_gated_map(&maps.m[i], bases[i], d, strides, i, names[i])) != TTT_OK) return rc;
+  ttt::GatedParams p{};
+  p.w0 = weight;
+  p.g = log_decay;
+  p.beta = beta;
+  p.seg_state = static_cast<float*>(workspace);
+  p.seg_decay = p.seg_state + cut.state_floats;
+  p.saved = static_cast<uint8_t*>(saved);
+  p.out = output;
+  p.w_out = weight_out;
+  p.status = static_cast<uint32_t*>(status);
+  p.T = d->seq_len;
+  p.H = d->heads;
+  p.NC = cut.chunks;
+  p.nstreams = d->batch * d->heads;
+  p.nseg = cut.nseg;
+  p.seg_chunks = cut.seg_chunks;
+  const cudaError_t e = ttt::launch_gated_fwd(d->dtype, d->head_dim, maps, p, saved != nullptr, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated forward launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}
+
+extern "C" int ttt_linear_gated_backward(const ttt_dims* d, const void* xq, const void* xk, const void* xv,
+                                         const void* grad_output, const int64_t* strides, const float* log_decay,
+                                         const float* beta, const void* saved, size_t saved_bytes,
+                                         const float* grad_weight_out, void* grad_xq, void* grad_xk, void* grad_xv,
+                                         float* grad_log_decay, float* grad_beta, float* grad_weight, void* workspace,
+                                         size_t workspace_bytes, void* status, void* stream) {
+  int rc = check_gated_dims(d);
+  if (rc != TTT_OK) return rc;
+  const NamedPtr ptrs[] = {{"xq", xq}, {"xk", xk}, {"xv", xv}, {"grad_output", grad_output}, {"saved", saved},
+                           {"grad_xq", grad_xq}, {"grad_xk", grad_xk}, {"grad_xv", grad_xv}, {"grad_weight", grad_weight}};
+  if ((rc = check_ptrs(ptrs, 9)) != TTT_OK) return rc;
+  if (log_decay == nullptr) return fail(TTT_ERR_NULL, "log_decay is null");
+  if (grad_log_decay == nullptr) return fail(TTT_ERR_NULL, "grad_log_decay is null");
+  if ((grad_beta != nullptr) != (beta != nullptr)) return fail(TTT_ERR_NULL, "beta and grad_beta must be given together");
+  if ((rc = check_optional("log_decay", log_decay, 4)) != TTT_OK || (rc = check_optional("beta", beta, 4)) != TTT_OK ||
+      (rc = check_optional("grad_log_decay", grad_log_decay, 4)) != TTT_OK ||
+      (rc = check_optional("grad_beta", grad_beta, 4)) != TTT_OK ||
+      (rc = check_optional("grad_weight_out", grad_weight_out, 16)) != TTT_OK ||
+      (rc = check_optional("status", status, 4)) != TTT_OK)
+    return rc;
+  if (saved_bytes < gated_saved_bytes(d))
+    return fail(TTT_ERR_WORKSPACE, "saved has %zu bytes, %zu needed", saved_bytes, gated_saved_bytes(d));
+  const GatedCut cut = gated_cut(d, true);
+  if ((rc = check_gated_workspace(cut, workspace, workspace_bytes)) != TTT_OK) return rc;
+  ttt::GatedMaps maps{};
+  const void* bases[4] = {xq, xk, xv, grad_output};
+  const char* names[4] = {"xq", "xk", "xv", "grad_output"};
+  GatedStrides checked;
+  for (int i = 0; i < 4; ++i)
+    if ((rc = gated_strides(&checked, d, strides, i, names[i])) != TTT_OK) return rc;
+  for (int i = 0; i < 4; ++i)
+    if ((rc = make_gated_map(&maps.m[i], bases[i], d, strides, i, names[i])) != TTT_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float* seg = static_cast<float*>(workspace);
+  if (cut.nseg > 1) {
+    ttt::GatedParams r{};
+    r.w0 = grad_weight_out;
+    r.g = log_decay;
+    r.seg_state = seg;
+    r.seg_decay = seg + cut.state_floats;
+    r.status = static_cast<uint32_t*>(status);
+    r.T = d->seq_len;
+    r.H = d->heads;
+    r.NC = cut.chunks;
+    r.nstreams = d->batch * d->heads;
+    r.nseg = cut.nseg;
+    r.seg_chunks = cut.seg_chunks;
+    ttt::GatedMaps rev = maps;
+    rev.m[1] = maps.m[0];
+    rev.m[2] = maps.m[3];
+    const cudaError_t e = ttt::launch_gated_segments_rev(d->dtype, d->head_dim, rev, r, st);
+    if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated backward launch failed: %s", cudaGetErrorString(e));
+  }
+  ttt::GatedBwdParams p{};
+  p.g = log_decay;
+  p.beta = beta;
+  p.saved = static_cast<const uint8_t*>(saved);
+  p.dw_out = grad_weight_out;
+  p.seg_state = seg;
+  p.dq = grad_xq;
+  p.dk = grad_xk;
+  p.dv = grad_xv;
+  p.dg = grad_log_decay;
+  p.dbeta = grad_beta;
+  p.dw0 = grad_weight;
+  p.status = static_cast<uint32_t*>(status);
+  p.T = d->seq_len;
+  p.H = d->heads;
+  p.NC = cut.chunks;
+  p.nstreams = d->batch * d->heads;
+  p.nseg = cut.nseg;
+  p.seg_chunks = cut.seg_chunks;
+  const cudaError_t e = ttt::launch_gated_bwd(d->dtype, d->head_dim, maps, p, st);
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated backward launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}
+
+extern "C" int ttt_linear_gated_step(const ttt_dims* d, const void* xq, const void* xk, const void* xv, const int64_t* strides,
+                                     const float* log_decay, const float* beta, const float* weight, void* output,
+                                     float* weight_out, void* stream) {
+  int rc = check_gated_dims(d);
+  if (rc != TTT_OK) return rc;
+  if (d->seq_len > 16) return fail(TTT_ERR_SHAPE, "a step has 1..16 tokens (got seq_len=%d)", d->seq_len);
+  const NamedPtr ptrs[] = {{"xq", xq}, {"xk", xk}, {"xv", xv}, {"output", output}, {"weight_out", weight_out}};
+  if ((rc = check_ptrs(ptrs, 5)) != TTT_OK) return rc;
+  if (log_decay == nullptr) return fail(TTT_ERR_NULL, "log_decay is null");
+  if ((rc = check_optional("log_decay", log_decay, 4)) != TTT_OK || (rc = check_optional("beta", beta, 4)) != TTT_OK ||
+      (rc = check_optional("weight", weight, 16)) != TTT_OK)
+    return rc;
+  ttt::GatedStepParams p{};
+  GatedStrides s[3];
+  const char* names[3] = {"xq", "xk", "xv"};
+  for (int i = 0; i < 3; ++i)
+    if ((rc = gated_strides(&s[i], d, strides, i, names[i])) != TTT_OK) return rc;
+  for (int k = 0; k < 3; ++k) {
+    p.sq[k] = (long)s[0].s[k];
+    p.sk[k] = (long)s[1].s[k];
+    p.sv[k] = (long)s[2].s[k];
+  }
+  p.q = xq;
+  p.k = xk;
+  p.v = xv;
+  p.g = log_decay;
+  p.beta = beta;
+  p.w = weight;
+  p.out = output;
+  p.w_out = weight_out;
+  p.H = d->heads;
+  p.R = d->seq_len;
+  const cudaError_t e = ttt::launch_gated_step(d->dtype, d->head_dim, p, d->batch * d->heads, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated step launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}

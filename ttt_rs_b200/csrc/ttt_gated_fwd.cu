@@ -1,0 +1,321 @@
+// Gated linear recurrence, forward (the mathematics and its chunked form: ttt_gated.cuh).
+//
+// One CTA of four warps per stream (or per segment of one) walks its chunks; warp w owns 16 queries of the chunk and 16 rows of
+// the float32 state, both in accumulator layout.  Per chunk, for each block of 16 tokens: their keys against the queries at or
+// behind them, the decayed products as the A operand of the product with their values, and the same values, still in registers,
+// under the transposed and scaled keys for the state.  The state goes to shared memory once per chunk as the operand of the next
+// chunk's q W (double-buffered: one barrier per chunk); the next two chunks are on their way meanwhile (TMA, rows behind the
+// sequence read as zeros).
+//
+// Few streams are cut into segments: a first launch leaves every segment's own state (as if it began with none) and its decay, a
+// second one joins them along the sequence, and the third is this kernel with a CTA per segment.
+#include "ttt_kernels.h"
+#include "ttt_gated.cuh"
+#include "ttt_stage.cuh"
+
+namespace ttt {
+
+constexpr int GF_THREADS = 32 * GATED_WARPS;
+
+// STATE: only the state at the end of the segment is wanted (REV: of the gradient's walk, from the last token to the first)
+template <typename T, int F, bool STATE>
+struct GatedFwdSmem {
+  static constexpr bool BF = sizeof(T) == 2;
+  static constexpr int NP = BF ? 1 : 3, NIN = STATE ? 2 : 3;
+  static constexpr uint32_t PLANE = GTile<F>::BYTES, TILE = NP * PLANE;
+  static constexpr uint32_t RAW = GC * F * 4;                                 // float32 rows as they arrive
+  static constexpr uint32_t STAGES = BF ? 2 : 1;
+  static constexpr uint32_t TILES = 0, RAWS = TILES + STAGES * NIN * TILE;
+  static constexpr uint32_t W = RAWS + (BF ? 0 : NIN * RAW);
+  static constexpr uint32_t GATES = W + (STATE ? 0 : 2 * NP * GTile<F>::STATE_BYTES);
+  static constexpr uint32_t BAR = GATES + 2 * sizeof(ChunkGates), BYTES = BAR + 16 + 1024;  // (1024: the base is aligned by hand)
+};
+
+template <typename T, int F, bool SAVE, bool STATE, bool REV>
+__global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
+    ttt_gated_fwd_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+  using SM = GatedFwdSmem<T, F, STATE>;
+  using SH = StateShare<F>;
+  constexpr bool BF = SM::BF;
+  constexpr int NP = SM::NP, NS = BF ? 2 : 3;  // planes of inputs, of scaled keys
+  constexpr int KS = F / 16;
+  extern __shared__ uint8_t gated_smem[];
+  const uint32_t raw = smem_u32(gated_smem), base = (raw + 1023) & ~1023u;
+  uint8_t* const mem = gated_smem + (base - raw);
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  const int stream = blockIdx.x / p.nseg, seg = blockIdx.x - stream * p.nseg;
+  const int c_lo = seg * p.seg_chunks, c_hi = min(p.NC, c_lo + p.seg_chunks), n = c_hi - c_lo;
+  const int h = stream % p.H, b = stream / p.H;
+  if (STATE && seg == (REV ? 0 : p.nseg - 1)) return;  // nothing follows it
+  const uint32_t bar = base + SM::BAR;
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    mbar_init(bar + 8, 1);
+    fence_mbar_init();
+  }
+  pdl_join();
+  __syncthreads();
+  auto chunk_of = [&](int i) { return REV ? c_hi - 1 - i : c_lo + i; };
+  auto fetch = [&](int i) {  // thread 0
+    const int slot = BF ? i & 1 : 0;
+    const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * SM::NIN * SM::TILE : SM::RAWS);
+    constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
+    mbar_expect_tx(at, SM::NIN * bytes);
+#pragma unroll
+    for (int m = 0; m < SM::NIN; ++m) tma_load_4d(dst + m * bytes, &maps.m[(STATE ? 1 : 0) + m], chunk_of(i) * GC, h, b, at);
+  };
+  if (tid == 0) {
+    fetch(0);
+    if (BF && n > 1) fetch(1);
+  }
+  const float* gp = p.g + (size_t)stream * p.T;
+  const float* bp = p.beta != nullptr ? p.beta + (size_t)stream * p.T : nullptr;
+  ChunkGates* const gates = reinterpret_cast<ChunkGates*>(mem + SM::GATES);
+  // the gates of walk step i by warp i % 4, a step ahead
+  auto make_gates = [&](int i) {
+    const int t0 = chunk_of(i) * GC;
+    make_chunk_gates(gates[i & 1], lane, load_gates(gp, t0, p.T, lane, 0.f), load_gates(bp, t0, p.T, lane, 1.f));
+  };
+  if (w == 0) make_gates(0);
+
+  // this warp's share of the state
+  const int row0 = 16 * (w % SH::SLABS), part = w / SH::SLABS, col0 = part * SH::COLS;
+  float W[SH::NT][4];
+  {
+    const float* w0 = nullptr;
+    if (!STATE) w0 = seg > 0 ? p.seg_state + ((size_t)stream * p.nseg + seg) * F * F : p.w0 != nullptr ? p.w0 + (size_t)stream * F * F : nullptr;
+    load_state<F>(W, w0, row0, col0, lane);
+  }
+  float total = 1.f;  // what is left of the state before the segment after it
+  uint8_t* const saved = SAVE ? p.saved + (size_t)stream * p.NC * F * F * 4 : nullptr;
+  auto publish = [&](int i) {  // the state before walk step i: operand of its q W, and what the backward reads back
+    if constexpr (!STATE) {
+      const uint32_t dst = base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES;
+      uint8_t* image = SAVE && i < n ? saved + (size_t)(c_lo + i) * F * F * 4 : nullptr;
+      if constexpr (BF && SAVE) {
+        float hi[SH::NT][4], lo[SH::NT][4];
+#pragma unroll
+        for (int k = 0; k < SH::NT; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            hi[k][e] = __bfloat162float(__float2bfloat16_rn(W[k][e]));
+            lo[k][e] = W[k][e] - hi[k][e];
+          }
+        put_state<F, 1>(hi, row0, col0, dst, image, lane);
+        if (image != nullptr) put_state<F, 1>(lo, row0, col0, 0, image + GTile<F>::STATE_BYTES, lane);
+      } else {
+        put_state<F, NP>(W, row0, col0, dst, nullptr, lane);
+        if (SAVE && image != nullptr) store_state<F>(reinterpret_cast<float*>(image), W, row0, col0, lane);
+      }
+    }
+  };
+  publish(0);
+  __syncthreads();
+
+  for (int i = 0; i < n; ++i) {
+    const int slot = BF ? i & 1 : 0, t0 = chunk_of(i) * GC;
+    const bool ahead = w == ((i + 1) & 3) && i + 1 < n;
+    float2 g_next, b_next;
+    if (ahead) {
+      g_next = load_gates(gp, chunk_of(i + 1) * GC, p.T, lane, 0.f);
+      b_next = load_gates(bp, chunk_of(i + 1) * GC, p.T, lane, 1.f);
+    }
+    if (!mbar_wait_bounded(bar + 8 * slot, (BF ? i >> 1 : i) & 1)) {
+      if (tid == 0) report_timeout(p.status, 20, (uint32_t)i);
+      return;
+    }
+    const uint32_t tiles = base + SM::TILES + slot * SM::NIN * SM::TILE;
+    if constexpr (!BF) {
+#pragma unroll
+      for (int m = 0; m < SM::NIN; ++m)
+        split_rows<F>(tiles + m * SM::TILE, SM::PLANE, reinterpret_cast<const float*>(mem + SM::RAWS + m * SM::RAW), GC, tid, GF_THREADS);
+      __syncthreads();
+      if (tid == 0 && i + 1 < n) fetch(i + 1);
+    }
+    const uint32_t tq = tiles, tk = tiles + (STATE ? 0 : SM::TILE), tv = tk + SM::TILE;
+    const ChunkGates& cg = gates[i & 1];
+
+    float o[STATE ? 1 : F / 8][4];
+    Pk<NP> q[STATE ? 1 : KS][4];
+    if constexpr (!STATE) {
+      // o = e^{G_i} q_i W
+      const uint32_t tw = base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) ldsm_np<NP>(q[k], tq + GTile<F>::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
+#pragma unroll
+      for (int k = 0; k < F / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int m = 0; m < KS; ++m) {
+          Pk<NP> f[4];
+          ldsm_np<NP>(f, tw + GTile<F>::b_kn(lane, 16 * m, 16 * k), GTile<F>::STATE_BYTES, true);
+          mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], q[k], f);
+        }
+      const float fa = cg.from[16 * w + g], fb = cg.from[16 * w + g + 8];
+#pragma unroll
+      for (int k = 0; k < F / 8; ++k) {
+        o[k][0] *= fa;
+        o[k][1] *= fa;
+        o[k][2] *= fb;
+        o[k][3] *= fb;
+      }
+    }
+    const float all = cg.all;
+    total *= all;
+#pragma unroll
+    for (int k = 0; k < SH::NT; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) W[k][e] *= all;
+
+#pragma unroll
+    for (int jt = 0; jt < GC / 16; ++jt) {
+      // queries of this warp against the keys of tokens 16 jt .. 16 jt + 15, decayed; an operand of the inputs' planes
+      Pk<NP> a[4];
+      const bool here = !STATE && jt <= w;
+      if (!STATE && here) {
+        float s0[4] = {}, s1[4] = {};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          Pk<NP> f[4];
+          ldsm_np<NP>(f, tk + GTile<F>::b_nk(lane, 16 * jt, 16 * k), SM::PLANE, false);
+          mma_planes<NP, NP>(s0, s1, q[STATE ? 0 : k], f);
+        }
+        const int ia = 16 * w + g, j0 = 16 * jt + 2 * t4;
+        const float ha = cg.hi[ia], la = cg.lo[ia], hb = cg.hi[ia + 8], lb = cg.lo[ia + 8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // columns j0, j0 + 1, j0 + 8, j0 + 9
+          const int j = j0 + (e & 1) + 8 * (e >> 1);
+          const float hj = cg.hi[j], lj = cg.lo[j], bj = cg.beta[j];
+          float* s = e < 2 ? s0 : s1;
+          const float da = j <= ia ? exp2f((ha - hj) + (la - lj)) * bj : 0.f;
+          const float db = j <= ia + 8 ? exp2f((hb - hj) + (lb - lj)) * bj : 0.f;
+          s[e & 1] = j <= ia ? s[e & 1] * da : 0.f;
+          s[2 + (e & 1)] = j <= ia + 8 ? s[2 + (e & 1)] * db : 0.f;
+        }
+        a[0] = split_pack<NP>(s0[0], s0[1]);
+        a[1] = split_pack<NP>(s0[2], s0[3]);
+        a[2] = split_pack<NP>(s1[0], s1[1]);
+        a[3] = split_pack<NP>(s1[2], s1[3]);
+      }
+      // keys of these tokens, transposed: rows of the state
+      Pk<NS> kt[4];
+      {
+        Pk<NP> f[4];
+        ldsm_np<NP>(f, tk + GTile<F>::a_km(lane, row0, 16 * jt), SM::PLANE, true);
+        const int j0 = 16 * jt + 2 * t4;
+        float2 lo, hi;
+        if constexpr (REV) {  // (the gradient's walk: what is left at the token of the state before the chunk)
+          lo = *reinterpret_cast<const float2*>(&cg.from[j0]);
+          hi = *reinterpret_cast<const float2*>(&cg.from[j0 + 8]);
+        } else {
+          lo = f2mul(*reinterpret_cast<const float2*>(&cg.to[j0]), *reinterpret_cast<const float2*>(&cg.beta[j0]));
+          hi = f2mul(*reinterpret_cast<const float2*>(&cg.to[j0 + 8]), *reinterpret_cast<const float2*>(&cg.beta[j0 + 8]));
+        }
+        scale_a_cols<NS, NP>(kt, f, lo, hi);
+      }
+#pragma unroll
+      for (int m = 0; m < KS; ++m) {
+        const bool mine = SH::PARTS == 1 || m == part;
+        if (!mine && !here) continue;
+        Pk<NP> f[4];
+        ldsm_np<NP>(f, tv + GTile<F>::b_kn(lane, 16 * m, 16 * jt), SM::PLANE, true);
+        if constexpr (!STATE) {
+          if (here) mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], a, f);
+        }
+        if (mine) {
+          const int at = SH::PARTS == 1 ? 2 * m : 0;
+          mma_planes<NS, NP>(W[at], W[at + 1], kt, f);
+        }
+      }
+    }
+    if constexpr (!STATE)
+      store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)stream * p.T + t0) * F, 16 * w, p.T - t0, o, lane);
+    if (i + 1 < n) publish(i + 1);
+    if (ahead) make_chunk_gates(gates[(i + 1) & 1], lane, g_next, b_next);
+    __syncthreads();  // the tiles and this chunk's state and gates are free, the next one's are there
+    if (BF && tid == 0 && i + 2 < n) fetch(i + 2);
+  }
+  if constexpr (STATE) {
+    store_state<F>(p.seg_state + ((size_t)stream * p.nseg + seg) * F * F, W, row0, col0, lane);
+    if (tid == 0) p.seg_decay[(size_t)stream * p.nseg + seg] = total;
+  } else if (seg == p.nseg - 1) {
+    store_state<F>(p.w_out + (size_t)stream * F * F, W, row0, col0, lane);
+  }
+}
+
+// The segments' own states to the states before them, along the sequence (REV: gradients, from the last segment to the first):
+// state[s] <- W_s, W_{s+1} = decay[s] W_s + own[s].  Every thread carries one float4 of a stream's state.
+template <int F, bool REV>
+__global__ void __launch_bounds__(256) ttt_gated_join_kernel(const GatedParams p) {
+  pdl_join();
+  constexpr int Q = F * F / 4;
+  const long e = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= (long)p.nstreams * Q) return;
+  const long stream = e / Q;
+  const int at = (int)(e - stream * Q);
+  float4* s = reinterpret_cast<float4*>(p.seg_state) + stream * p.nseg * Q + at;
+  const float* d = p.seg_decay + stream * p.nseg;
+  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.w0 != nullptr) w = reinterpret_cast<const float4*>(p.w0)[stream * Q + at];
+  for (int k = 0; k < p.nseg; ++k) {
+    const int i = REV ? p.nseg - 1 - k : k;
+    const float4 own = s[(long)i * Q];
+    s[(long)i * Q] = w;
+    const float f = d[i];
+    w = make_float4(fmaf(f, w.x, own.x), fmaf(f, w.y, own.y), fmaf(f, w.z, own.z), fmaf(f, w.w, own.w));
+  }
+}
+
+// Streams that do not fill the card are cut until they do.
+int gated_segments(int64_t streams, int chunks, bool backward) {
+  constexpr int SMS = 148, LEAST = 4;  // (chunks per segment: a segment's states and its second reading must be worth it)
+  if (streams >= SMS) return 1;
+  const int64_t want = ((backward ? 2 : 3) * SMS) / streams;
+  const int64_t most = chunks / LEAST;
+  return (int)(want < most ? want : most > 1 ? most : 1);
+}
+
+template <typename T, int F, bool SAVE, bool STATE, bool REV>
+static cudaError_t launch_one(const GatedMaps& maps, const GatedParams& p, int grid, cudaStream_t st) {
+  auto kfn = ttt_gated_fwd_kernel<T, F, SAVE, STATE, REV>;
+  constexpr size_t smem = GatedFwdSmem<T, F, STATE>::BYTES;
+  static DeviceValue ready;
+  int unused;
+  cudaError_t e = ready.get(0, &unused, [&](int* v) {
+    *v = 0;
+    return cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  });
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kfn, grid, GF_THREADS, smem, st, maps, p);
+}
+
+template <typename T, int F>
+static cudaError_t launch_gated(const GatedMaps& maps, GatedParams p, bool save, cudaStream_t st) {
+  if (p.nseg > 1) {
+    cudaError_t e = launch_one<T, F, false, true, false>(maps, p, p.nstreams * p.nseg, st);
+    if (e != cudaSuccess) return e;
+    e = launch_dependent(ttt_gated_join_kernel<F, false>, (int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st, p);
+    if (e != cudaSuccess) return e;
+  }
+  if (save) return launch_one<T, F, true, false, false>(maps, p, p.nstreams * p.nseg, st);
+  return launch_one<T, F, false, false, false>(maps, p, p.nstreams * p.nseg, st);
+}
+cudaError_t launch_gated_fwd(int dtype, int F, const GatedMaps& maps, const GatedParams& p, bool save, cudaStream_t st) {
+  if (F == 64) return dtype == 1 ? launch_gated<__nv_bfloat16, 64>(maps, p, save, st) : launch_gated<float, 64>(maps, p, save, st);
+  return dtype == 1 ? launch_gated<__nv_bfloat16, 32>(maps, p, save, st) : launch_gated<float, 32>(maps, p, save, st);
+}
+
+// The gradient's states behind every segment: maps 1 and 2 are the queries and the output's gradient
+template <typename T, int F>
+static cudaError_t launch_rev(const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
+  cudaError_t e = launch_one<T, F, false, true, true>(maps, p, p.nstreams * p.nseg, st);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(ttt_gated_join_kernel<F, true>, (int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st, p);
+}
+cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
+  if (F == 64) return dtype == 1 ? launch_rev<__nv_bfloat16, 64>(maps, p, st) : launch_rev<float, 64>(maps, p, st);
+  return dtype == 1 ? launch_rev<__nv_bfloat16, 32>(maps, p, st) : launch_rev<float, 32>(maps, p, st);
+}
+
+}  // namespace ttt

@@ -259,6 +259,96 @@ struct MlpFn : torch::autograd::Function<MlpFn> {
   }
 };
 
+// ---- gated linear recurrence ---------------------------------------------------------------------------------------------
+// [B,H,T,F] with any strides that the kernels take (rows contiguous, the other strides positive multiples of 16 bytes)
+bool rows_of_16_bytes(const Tensor& t) {
+  if (t.layout() != c10::kStrided || t.stride(3) != 1 || !on_16_bytes(t)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) * (int64_t)t.element_size() % 16 != 0)) return false;
+  return true;
+}
+struct Gated {
+  Dims m;
+  bool plain(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& w) {
+    if (!m.set(q, q.dim() == 4 ? q.size(3) : -1, 1, 1, 0) || !m.status.defined()) return false;
+    const c10::IntArrayRef four = q.sizes();
+    for (const Tensor* t : {&q, &k, &v})
+      if (t->scalar_type() != m.dt || t->device() != m.dev || t->sizes() != four || !rows_of_16_bytes(*t)) return false;
+    if (!is(g, at::kFloat, m.dev, {m.B, m.H, m.T})) return false;
+    if (beta.defined() && !is(beta, at::kFloat, m.dev, {m.B, m.H, m.T})) return false;
+    if (w.defined() && (!is(w, at::kFloat, m.dev, {m.B, m.H, m.F, m.F}) || !on_16_bytes(w))) return false;
+    return ttt_linear_gated_saved_bytes(&m.d) != 0;
+  }
+  static const float* f32(const Tensor& t) { return t.defined() ? static_cast<const float*>(t.const_data_ptr()) : nullptr; }
+  template <size_t N>
+  static std::array<int64_t, 3 * N> strides(const std::array<const Tensor*, N>& ts) {
+    std::array<int64_t, 3 * N> s;
+    for (size_t i = 0; i < N; ++i)
+      for (int k = 0; k < 3; ++k) s[3 * i + k] = ts[i]->stride(k);
+    return s;
+  }
+  int forward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& w, bool save,
+              Tensor& out, Tensor& w_out, Tensor& saved) {
+    c10::cuda::CUDAGuard guard(m.dev);
+    out = at::empty({m.B, m.H, m.T, m.F}, m.opt());
+    w_out = at::empty({m.B, m.H, m.F, m.F}, m.opt(at::kFloat));
+    const auto s = strides<3>({&q, &k, &v});
+    if (!save && m.T <= 16)
+      return ttt_linear_gated_step(&m.d, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), s.data(), f32(g), f32(beta),
+                                   f32(w), out.data_ptr(), static_cast<float*>(w_out.data_ptr()), m.stream());
+    const size_t wsb = ttt_linear_gated_forward_workspace_bytes(&m.d), sb = save ? ttt_linear_gated_saved_bytes(&m.d) : 0;
+    Tensor ws;
+    if (wsb != 0) ws = at::empty({(int64_t)wsb}, m.opt(at::kByte));
+    if (save) saved = at::empty({(int64_t)sb}, m.opt(at::kByte));
+    return ttt_linear_gated_forward(&m.d, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), s.data(), f32(g), f32(beta),
+                                    f32(w), out.data_ptr(), static_cast<float*>(w_out.data_ptr()), save ? saved.data_ptr() : nullptr,
+                                    sb, wsb != 0 ? ws.data_ptr() : nullptr, wsb, m.status.data_ptr(), m.stream());
+  }
+};
+
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                               const Tensor& beta, const Tensor& w, bool has_beta, bool has_w) {
+    Gated call;
+    Tensor out, w_out, saved;
+    call.m.set(q, q.size(3), 1, 1, 0);
+    const int rc = call.forward(q, k, v, g, has_beta ? beta : Tensor(), has_w ? w : Tensor(), true, out, w_out, saved);
+    if (rc != TTT_OK) throw_error(rc);
+    ctx->save_for_backward({q, k, v, g, beta});
+    ctx->saved_data["has"] = std::vector<int64_t>{has_beta, has_w};
+    ctx->saved_data["s"] = saved;
+    ctx->set_materialize_grads(false);
+    return {out, w_out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const variable_list t = ctx->get_saved_variables();
+    const std::vector<int64_t> has = ctx->saved_data["has"].toIntVector();
+    const Tensor &q = t[0], &k = t[1], &v = t[2], &g = t[3], beta = has[0] ? t[4] : Tensor();
+    const Tensor saved = ctx->saved_data["s"].toTensor();
+    if (!go[0].defined() && !go[1].defined()) return variable_list(8);
+    Gated call;
+    call.m.set(q, q.size(3), 1, 1, 0);
+    const Dims& m = call.m;
+    c10::cuda::CUDAGuard guard(m.dev);
+    Tensor u = go[0].defined() ? go[0] : at::zeros({m.B, m.H, m.T, m.F}, m.opt()), dw_out = go[1];
+    if (!rows_of_16_bytes(u)) u = u.clone(at::MemoryFormat::Contiguous);
+    if (dw_out.defined() && (!dw_out.is_contiguous() || !on_16_bytes(dw_out))) dw_out = dw_out.clone(at::MemoryFormat::Contiguous);
+    Tensor dq = at::empty({m.B, m.H, m.T, m.F}, m.opt()), dk = at::empty_like(dq), dv = at::empty_like(dq);
+    Tensor dg = at::empty({m.B, m.H, m.T}, m.opt(at::kFloat)), db, dw = at::empty({m.B, m.H, m.F, m.F}, m.opt(at::kFloat)), ws;
+    if (beta.defined()) db = at::empty_like(dg);
+    const size_t wsb = ttt_linear_gated_backward_workspace_bytes(&m.d);
+    if (wsb != 0) ws = at::empty({(int64_t)wsb}, m.opt(at::kByte));
+    const auto s = Gated::strides<4>({&q, &k, &v, &u});
+    const int rc = ttt_linear_gated_backward(
+        &m.d, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), u.const_data_ptr(), s.data(), Gated::f32(g), Gated::f32(beta),
+        saved.const_data_ptr(), (size_t)saved.numel(), Gated::f32(dw_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        static_cast<float*>(dg.data_ptr()), beta.defined() ? static_cast<float*>(db.data_ptr()) : nullptr,
+        static_cast<float*>(dw.data_ptr()), wsb != 0 ? ws.data_ptr() : nullptr, wsb, m.status.data_ptr(), m.stream());
+    if (rc != TTT_OK) throw_error(rc);
+    return {dq, dk, dv, dg, db, has[1] ? dw : Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ---- Python functions ----------------------------------------------------------------------------------------------
 // tensors args[0..n), false when one is not a tensor
 template <int N>
@@ -849,6 +939,35 @@ PyObject* py_layer_train(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// optional tensor: None, or a tensor (false: neither)
+bool optional_tensor(PyObject* o, Tensor& t) {
+  if (o == Py_None) return true;
+  if (!THPVariable_Check(o)) return false;
+  t = THPVariable_Unpack(o);
+  return true;
+}
+// gated(q, k, v, log_decay, beta | None, weight | None) -> (out, weight), recorded for autograd where that is on and asked for | None
+PyObject* py_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 6)) return nullptr;
+  Tensor t[4], beta, w;
+  NONE_IF(!tensors(args, t) || !optional_tensor(args[4], beta) || !optional_tensor(args[5], w));
+  Gated call;
+  NONE_IF(!call.plain(t[0], t[1], t[2], t[3], beta, w));
+  bool grad = false;
+  if (at::GradMode::is_enabled())
+    for (const Tensor* x : {&t[0], &t[1], &t[2], &t[3], &beta, &w}) grad = grad || (x->defined() && x->requires_grad());
+  if (grad) {  // (a node's arguments are defined tensors)
+    const bool has_beta = beta.defined(), has_w = w.defined();
+    return wrap(GatedFn::apply(t[0], t[1], t[2], t[3], has_beta ? beta : at::empty({0}), has_w ? w : at::empty({0}), has_beta, has_w));
+  }
+  Tensor out, w_out, saved;
+  const int rc = call.forward(t[0], t[1], t[2], t[3], beta, w, false, out, w_out, saved);
+  if (rc != TTT_OK) throw_error(rc);
+  return wrap({out, w_out});
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(set_status),
@@ -862,6 +981,7 @@ PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(stream_key),
                          FAST(layer_infer),
                          FAST(layer_train),
+                         FAST(gated),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -407,4 +407,52 @@ cudaError_t launch_linear_bwd(int dtype, int seg, int mb, const CUtensorMap* map
 cudaError_t launch_linear_bwd_f32(int seg, int mb, const CUtensorMap* maps, LinBwdParams& p, int nstreams, cudaStream_t st);
 cudaError_t launch_linear_bwd_reduce(const ReduceParams& p, cudaStream_t st);
 
+// ---- gated linear recurrence (ttt_gated_fwd.cu, ttt_gated_bwd.cu, ttt_gated_step.cu) -------------------------------
+// maps, 4-D (features, tokens, heads, batch), boxes of 64 tokens: q, k, v, and the output's gradient
+struct GatedMaps {
+  CUtensorMap m[4];
+};
+struct GatedParams {
+  const float* w0;    // [B,H,F,F] state before the sequence (backwards walk: gradient of the one behind it), or null: zeros
+  const float* g;     // [B,H,T] logarithms of the decays
+  const float* beta;  // [B,H,T] or null: ones
+  float* seg_state;   // [streams][nseg][F*F], nseg > 1 only
+  float* seg_decay;   // [streams][nseg]
+  uint8_t* saved;     // [streams][NC][F*F*4] states before every chunk, for the backward (save)
+  void* out;          // [B,H,T,F]
+  float* w_out;       // [B,H,F,F]
+  uint32_t* status;
+  int T, H, NC;       // NC: chunks of 64 tokens
+  int nstreams, nseg, seg_chunks;
+};
+struct GatedBwdParams {
+  const float* g;
+  const float* beta;
+  const uint8_t* saved;
+  const float* dw_out;     // [B,H,F,F] or null: zeros
+  const float* seg_state;  // gradients of the states behind each segment
+  void *dq, *dk, *dv;      // [B,H,T,F]
+  float* dg;               // [B,H,T]
+  float* dbeta;            // [B,H,T] or null
+  float* dw0;              // [B,H,F,F]
+  uint32_t* status;
+  int T, H, NC;
+  int nstreams, nseg, seg_chunks;
+};
+struct GatedStepParams {
+  const void *q, *k, *v;
+  long sq[3], sk[3], sv[3];  // strides of batch, head and token, in elements
+  const float *g, *beta, *w;
+  void* out;
+  float* w_out;  // may be w
+  int H, R;      // tokens, 1..16
+};
+// Segments per stream (ttt_gated_fwd.cu)
+int gated_segments(int64_t streams, int chunks, bool backward);
+cudaError_t launch_gated_fwd(int dtype, int F, const GatedMaps& maps, const GatedParams& p, bool save, cudaStream_t st);
+// maps.m[1], m[2]: queries, gradient of the output
+cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, const GatedParams& p, cudaStream_t st);
+cudaError_t launch_gated_bwd(int dtype, int F, const GatedMaps& maps, const GatedBwdParams& p, cudaStream_t st);
+cudaError_t launch_gated_step(int dtype, int F, const GatedStepParams& p, int nstreams, cudaStream_t st);
+
 }  // namespace ttt

@@ -22,7 +22,7 @@ BEGIN = "<!-- generated by include/gen_rust_ffi.py: begin -->"
 END = "<!-- generated by include/gen_rust_ffi.py: end -->"
 
 _TYPES = {
-    "const ttt_dims*": "*const TttDims", "const void*": "*const c_void", "void*": "*mut c_void",
+    "const ttt_dims*": "*const TttDims", "const ttt_rotation*": "*const TttRotation", "const void*": "*const c_void", "void*": "*mut c_void",
     "const float*": "*const f32", "const int64_t*": "*const i64", "float*": "*mut f32", "const char*": "*const c_char",
     "size_t": "usize", "int64_t": "i64", "int32_t": "i32", "uint32_t": "u32", "int": "c_int", "float": "f32",
 }

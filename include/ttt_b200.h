@@ -66,6 +66,19 @@ typedef struct ttt_dims {
   int32_t dtype;               /* enum ttt_dtype */
 } ttt_dims;
 
+/* Rotary positions of ttt_layer_rotary and ttt_layer_qk_norm_rotary: pair p of a row's first `rotary_dim` features is turned by
+ * 2 pi * position * turns[p] / 2^64, and scaled by `size`; the features behind are left as they are. */
+typedef struct ttt_rotation {
+  const uint64_t* turns;      /* device, [rotary_dim / 2]: turns per position as a fraction of 2^64, exact at any position */
+  const int64_t* positions;   /* device, [T] or [B][T] with rows positions_stride apart (0: one row for all); null: start_idx + t */
+  int64_t positions_stride;
+  int64_t start_idx;
+  int32_t rotary_dim;         /* even, 2..head_dim */
+  int32_t half;               /* pairs: 0 features (2p, 2p + 1), 1 features (p, p + rotary_dim / 2) */
+  int32_t wrap;               /* > 0: positions modulo this */
+  float size;
+} ttt_rotation;
+
 int ttt_b200_abi_version(void);
 const char* ttt_b200_status_string(int status);
 const char* ttt_b200_last_error(void);
@@ -370,6 +383,34 @@ int ttt_linear_gated_backward(const ttt_dims* d, const void* xq, const void* xk,
 int ttt_linear_gated_step(const ttt_dims* d, const void* xq, const void* xk, const void* xv, const int64_t* strides,
                           const float* log_decay, const float* beta, const float* weight, void* output,
                           float* weight_out, void* stream);
+
+/* ---- rotary positions; norm and rotation of queries and keys ---------------------------------------------------
+ * For layers that place their queries and keys otherwise than ttt_layer_prologue (neighbouring pairs over the whole head, unscaled):
+ * pairs of either layout, a part of the head, angles scaled for long contexts, any positions; and with a root-mean-square norm of
+ * every head in the same pass (no counterpart in the reference).  Of `d`, batch, heads (queries), seq_len, head_dim (even, 2..256),
+ * dtype and, for the norm, epsilon are read; k_heads may differ from heads.
+ * `strides`: for each tensor in the order of the arguments the strides of batch, head and token in elements (null: contiguous
+ * [B,H,T,F]); rows are F contiguous elements at any address (on 16 bytes, with F and rotary_dim multiples of 8, they are read 16
+ * bytes at a time).  Results may be the inputs themselves, and must not overlap them otherwise.
+ *
+ * ttt_layer_rotary: y = the rows of x rotated (inverse != 0: by the angles' negatives, the gradient).
+ * ttt_layer_qk_norm_rotary: rows x / sqrt(mean(x^2) + epsilon) * weight, rotated (rotation null: not).  q_weight, k_weight: T [F]
+ *   or null (ones).
+ * ttt_layer_qk_norm_rotary_backward: `strides` of q, k, grad_q_out, grad_k_out (gradients of the results), `grad_strides` of grad_q,
+ *   grad_k; grad_q_weight, grad_k_weight T [F] (out) or null, summed in float32 in a fixed order; workspace of
+ *   ttt_layer_qk_norm_rotary_backward_workspace_bytes bytes where one of them is given.
+ */
+int ttt_layer_rotary(const ttt_dims* d, const void* x, const int64_t* strides, const ttt_rotation* rotation, int inverse,
+                     void* y, const int64_t* y_strides, void* stream);
+int ttt_layer_qk_norm_rotary(const ttt_dims* d, int k_heads, const void* q, const void* k, const int64_t* strides,
+                             const void* q_weight, const void* k_weight, const ttt_rotation* rotation, void* q_out,
+                             void* k_out, const int64_t* out_strides, void* stream);
+size_t ttt_layer_qk_norm_rotary_backward_workspace_bytes(const ttt_dims* d, int k_heads);
+int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads, const void* q, const void* k,
+                                      const void* grad_q_out, const void* grad_k_out, const int64_t* strides,
+                                      const void* q_weight, const void* k_weight, const ttt_rotation* rotation,
+                                      void* grad_q, void* grad_k, const int64_t* grad_strides, void* grad_q_weight,
+                                      void* grad_k_weight, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Backward without a caller workspace.  (No counterpart in the reference: its host wrapper always allocates its
  * scratch itself, backward/launch.rs:389-392.)

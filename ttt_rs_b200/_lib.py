@@ -35,6 +35,14 @@ class TttDims(C.Structure):
     ]
 
 
+class TttRotation(C.Structure):
+    """struct ttt_rotation"""
+    _fields_ = [
+        ("turns", C.c_void_p), ("positions", C.c_void_p), ("positions_stride", C.c_int64), ("start_idx", C.c_int64),
+        ("rotary_dim", C.c_int32), ("half", C.c_int32), ("wrap", C.c_int32), ("size", C.c_float),
+    ]
+
+
 class TttError(RuntimeError):
     """Raised where the reference would panic (bad shapes, unsupported tile configuration, launch failure)."""
 
@@ -46,6 +54,7 @@ class TttError(RuntimeError):
 # every symbol include/ttt_b200.h declares: name -> (restype, argtypes)
 _P = C.c_void_p
 _DP = C.POINTER(TttDims)
+_RP = C.POINTER(TttRotation)
 SYMBOLS = {
     "ttt_b200_abi_version": (C.c_int, []),
     "ttt_b200_status_string": (C.c_char_p, [C.c_int]),
@@ -83,6 +92,10 @@ SYMBOLS = {
     "ttt_linear_gated_backward_workspace_bytes": (C.c_size_t, [_DP]),
     "ttt_linear_gated_backward": (C.c_int, [_DP] + [_P] * 8 + [C.c_size_t] + [_P] * 8 + [C.c_size_t, _P, _P]),
     "ttt_linear_gated_step": (C.c_int, [_DP] + [_P] * 10),
+    "ttt_layer_rotary": (C.c_int, [_DP, _P, _P, _RP, C.c_int, _P, _P, _P]),
+    "ttt_layer_qk_norm_rotary": (C.c_int, [_DP, C.c_int, _P, _P, _P, _P, _P, _RP, _P, _P, _P, _P]),
+    "ttt_layer_qk_norm_rotary_backward_workspace_bytes": (C.c_size_t, [_DP, C.c_int]),
+    "ttt_layer_qk_norm_rotary_backward": (C.c_int, [_DP, C.c_int] + [_P] * 7 + [_RP] + [_P] * 6 + [C.c_size_t, _P]),
     "ttt_layer_qk_conv_backward": (C.c_int, [_DP, _P, _P, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
 }
 # entry points of this package alone (csrc/ttt_internal.h)

@@ -19,7 +19,7 @@ LIB = PKG / "libttt_b200.so"
 PROBE_SRC = CSRC / "probe_chain_latency.cu"      # stand-alone measurement program (bench.py --workload chain-latency)
 PROBE_BIN = PKG / "build" / "probe_chain_latency"
 SOURCES = ["ttt_abi.cu", "ttt_linear_fwd.cu", "ttt_linear_fwd_roles.cu", "ttt_linear_bwd.cu", "ttt_linear_bwd_f32.cu", "ttt_mlp_fwd.cu", "ttt_layer.cu", "ttt_layer_small.cu", "ttt_linear_partial.cu", "ttt_mlp_bwd.cu", "ttt_gemm.cu",
-           "ttt_gated_fwd.cu", "ttt_gated_bwd.cu", "ttt_gated_step.cu"]
+           "ttt_gated_fwd.cu", "ttt_gated_bwd.cu", "ttt_gated_step.cu", "ttt_rotary.cu"]
 HOST_SRC = CSRC / "ttt_host.cpp"                 # native host path of the Python operator, linked against LIB
 HOST_LIB = PKG / "_host.so"
 HOST_TAG = PKG / "build" / "_host.tag"           # what HOST_LIB was built against

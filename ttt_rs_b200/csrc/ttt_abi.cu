@@ -1488,3 +1488,168 @@ extern "C" int ttt_linear_gated_step(const ttt_dims* d, const void* xq, const vo
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated step launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;
 }
+
+// ---- rotary positions, norm and rotation of queries and keys -----------------------------------------------------------
+namespace {
+
+int check_head_dims(const ttt_dims* d, int k_heads) {
+  if (d == nullptr) return fail(TTT_ERR_NULL, "dims is null");
+  if (d->batch <= 0 || d->heads <= 0 || d->seq_len <= 0 || k_heads < 0)
+    return fail(TTT_ERR_SHAPE, "batch, heads and seq_len must be positive");
+  if (d->dtype != TTT_F32 && d->dtype != TTT_BF16) return fail(TTT_ERR_UNSUPPORTED, "unknown dtype %d", d->dtype);
+  if (d->head_dim < 2 || d->head_dim > 256 || d->head_dim % 2 != 0)
+    return fail(TTT_ERR_UNSUPPORTED, "Unsupported head_dim=%d (supported: even, 2..256)", d->head_dim);
+  if ((int64_t)d->heads + k_heads > 65535) return fail(TTT_ERR_UNSUPPORTED, "at most 65535 heads");
+  if ((int64_t)d->batch * d->seq_len >= (int64_t)1 << 31) return fail(TTT_ERR_SHAPE, "batch*seq_len must be below 2^31");
+  return TTT_OK;
+}
+int set_rotation(ttt::RotaryParams* p, const ttt_dims* d, const ttt_rotation* rot, bool needed) {
+  p->size = 1.f;
+  if (rot == nullptr) return needed ? fail(TTT_ERR_NULL, "rotation is null") : TTT_OK;
+  if (rot->rotary_dim < 2 || rot->rotary_dim > d->head_dim || rot->rotary_dim % 2 != 0)
+    return fail(TTT_ERR_SHAPE, "rotary_dim=%d must be even, 2..head_dim", rot->rotary_dim);
+  if (rot->half != 0 && rot->half != 1) return fail(TTT_ERR_UNSUPPORTED, "half=%d (0: neighbouring pairs, 1: halves)", rot->half);
+  if (rot->turns == nullptr) return fail(TTT_ERR_NULL, "turns is null");
+  if ((reinterpret_cast<uintptr_t>(rot->turns) & 7u) != 0 || (reinterpret_cast<uintptr_t>(rot->positions) & 7u) != 0)
+    return fail(TTT_ERR_ALIGN, "turns / positions is not 8-byte aligned");
+  if (rot->wrap < 0) return fail(TTT_ERR_SHAPE, "wrap must be >= 0");
+  if (rot->positions != nullptr && rot->positions_stride != 0 && rot->positions_stride < d->seq_len)
+    return fail(TTT_ERR_SHAPE, "positions_stride must be 0 or at least seq_len");
+  if (!(rot->size > 0.f)) return fail(TTT_ERR_SHAPE, "size must be positive");
+  p->turns = rot->turns;
+  p->positions = rot->positions;
+  p->pos_stride = rot->positions_stride;
+  p->start = rot->start_idx;
+  p->wrap = rot->wrap;
+  p->rdim = rot->rotary_dim;
+  p->size = rot->size;
+  return TTT_OK;
+}
+// strides of tensor number `i` of a call (null: contiguous [B,H,T,F]); *vec: false where rows are not on 16 bytes
+int set_rows(int64_t (&out)[3], const ttt_dims* d, int heads, const void* base, const int64_t* strides, int i, bool written,
+             const char* name, bool* vec) {
+  const int64_t F = d->head_dim, T = d->seq_len, es = d->dtype == TTT_BF16 ? 2 : 4;
+  const int64_t dense[3] = {heads * T * F, T * F, F}, size[3] = {d->batch, heads, T};
+  if (base == nullptr) return fail(TTT_ERR_NULL, "%s is null", name);
+  if (reinterpret_cast<uintptr_t>(base) % es != 0) return fail(TTT_ERR_ALIGN, "%s is not aligned to its elements", name);
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0) *vec = false;
+  for (int k = 0; k < 3; ++k) {
+    out[k] = size[k] == 1 ? 0 : strides != nullptr ? strides[3 * i + k] : dense[k];
+    if (size[k] > 1 && (written ? out[k] < F : out[k] < 0))
+      return fail(TTT_ERR_SHAPE, written ? "rows of %s overlap" : "the strides of %s must not be negative", name);
+    if (out[k] * es % 16 != 0) *vec = false;
+  }
+  return TTT_OK;
+}
+
+}  // namespace
+
+extern "C" int ttt_layer_rotary(const ttt_dims* d, const void* x, const int64_t* strides, const ttt_rotation* rotation, int inverse,
+                                void* y, const int64_t* y_strides, void* stream) {
+  int rc = check_head_dims(d, 0);
+  if (rc != TTT_OK) return rc;
+  ttt::RotaryParams p{};
+  bool vec = d->head_dim % 8 == 0;
+  if ((rc = set_rotation(&p, d, rotation, true)) != TTT_OK ||
+      (rc = set_rows(p.xs[0], d, d->heads, x, strides, 0, false, "x", &vec)) != TTT_OK ||
+      (rc = set_rows(p.ys[0], d, d->heads, y, y_strides, 0, true, "y", &vec)) != TTT_OK)
+    return rc;
+  p.x[0] = x;
+  p.y[0] = y;
+  p.heads[0] = d->heads;
+  p.T = d->seq_len;
+  p.F = d->head_dim;
+  p.tokens = (int64_t)d->batch * d->seq_len;
+  p.sign = inverse != 0 ? -1.f : 1.f;
+  const cudaError_t e = ttt::launch_rotary(d->dtype, p, vec && p.rdim % 8 == 0, rotation->half != 0, false, false,
+                                           static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "rotary launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}
+
+namespace {
+int qk_params(ttt::RotaryParams* p, const ttt_dims* d, int k_heads, const ttt_rotation* rotation, const void* q, const void* k,
+              const int64_t* strides, void* q_out, void* k_out, const int64_t* out_strides, const char* q_name, const char* k_name,
+              const void* q_weight, const void* k_weight, bool* vec) {
+  int rc = check_head_dims(d, k_heads);
+  if (rc != TTT_OK) return rc;
+  if (k_heads < 1) return fail(TTT_ERR_SHAPE, "k_heads must be positive");
+  if (!(d->epsilon >= 0.f)) return fail(TTT_ERR_SHAPE, "epsilon must be >= 0");
+  *vec = d->head_dim % 8 == 0;
+  if ((rc = set_rotation(p, d, rotation, false)) != TTT_OK ||
+      (rc = set_rows(p->xs[0], d, d->heads, q, strides, 0, false, "q", vec)) != TTT_OK ||
+      (rc = set_rows(p->xs[1], d, k_heads, k, strides, 1, false, "k", vec)) != TTT_OK ||
+      (rc = set_rows(p->ys[0], d, d->heads, q_out, out_strides, 0, true, q_name, vec)) != TTT_OK ||
+      (rc = set_rows(p->ys[1], d, k_heads, k_out, out_strides, 1, true, k_name, vec)) != TTT_OK)
+    return rc;
+  const unsigned es = d->dtype == TTT_BF16 ? 2 : 4;
+  if ((rc = check_optional("q_weight", q_weight, es)) != TTT_OK || (rc = check_optional("k_weight", k_weight, es)) != TTT_OK) return rc;
+  if (p->rdim % 8 != 0) *vec = false;
+  p->x[0] = q;
+  p->x[1] = k;
+  p->y[0] = q_out;
+  p->y[1] = k_out;
+  p->w[0] = q_weight;
+  p->w[1] = k_weight;
+  p->heads[0] = d->heads;
+  p->heads[1] = k_heads;
+  p->T = d->seq_len;
+  p->F = d->head_dim;
+  p->tokens = (int64_t)d->batch * d->seq_len;
+  p->eps = d->epsilon;
+  return TTT_OK;
+}
+}  // namespace
+
+extern "C" int ttt_layer_qk_norm_rotary(const ttt_dims* d, int k_heads, const void* q, const void* k, const int64_t* strides,
+                                        const void* q_weight, const void* k_weight, const ttt_rotation* rotation, void* q_out,
+                                        void* k_out, const int64_t* out_strides, void* stream) {
+  ttt::RotaryParams p{};
+  bool vec;
+  const int rc = qk_params(&p, d, k_heads, rotation, q, k, strides, q_out, k_out, out_strides, "q_out", "k_out", q_weight, k_weight, &vec);
+  if (rc != TTT_OK) return rc;
+  p.sign = 1.f;
+  const cudaError_t e = ttt::launch_rotary(d->dtype, p, vec, rotation != nullptr && rotation->half != 0, true, false,
+                                           static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "norm and rotation launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}
+
+extern "C" size_t ttt_layer_qk_norm_rotary_backward_workspace_bytes(const ttt_dims* d, int k_heads) {
+  if (check_head_dims(d, k_heads) != TTT_OK || k_heads < 1) return 0;
+  return sizeof(float) * ttt::rotary_partial_floats((int64_t)d->batch * d->seq_len, d->heads + k_heads, d->head_dim);
+}
+
+extern "C" int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads, const void* q, const void* k, const void* grad_q_out,
+                                                 const void* grad_k_out, const int64_t* strides, const void* q_weight,
+                                                 const void* k_weight, const ttt_rotation* rotation, void* grad_q, void* grad_k,
+                                                 const int64_t* grad_strides, void* grad_q_weight, void* grad_k_weight,
+                                                 void* workspace, size_t workspace_bytes, void* stream) {
+  ttt::RotaryParams p{};
+  bool vec;
+  int rc = qk_params(&p, d, k_heads, rotation, q, k, strides, grad_q, grad_k, grad_strides, "grad_q", "grad_k", q_weight, k_weight, &vec);
+  if (rc != TTT_OK) return rc;
+  if ((rc = set_rows(p.gs[0], d, d->heads, grad_q_out, strides, 2, false, "grad_q_out", &vec)) != TTT_OK ||
+      (rc = set_rows(p.gs[1], d, k_heads, grad_k_out, strides, 3, false, "grad_k_out", &vec)) != TTT_OK)
+    return rc;
+  const unsigned es = d->dtype == TTT_BF16 ? 2 : 4;
+  if ((rc = check_optional("grad_q_weight", grad_q_weight, es)) != TTT_OK ||
+      (rc = check_optional("grad_k_weight", grad_k_weight, es)) != TTT_OK)
+    return rc;
+  p.g[0] = grad_q_out;
+  p.g[1] = grad_k_out;
+  p.dw[0] = grad_q_weight;
+  p.dw[1] = grad_k_weight;
+  p.sign = -1.f;
+  if (grad_q_weight != nullptr || grad_k_weight != nullptr) {
+    const size_t need = ttt_layer_qk_norm_rotary_backward_workspace_bytes(d, k_heads);
+    if (workspace == nullptr || workspace_bytes < need)
+      return fail(TTT_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", workspace == nullptr ? (size_t)0 : workspace_bytes, need);
+    if ((rc = check_optional("workspace", workspace, 4)) != TTT_OK) return rc;
+    p.partials = static_cast<float*>(workspace);
+  }
+  const cudaError_t e = ttt::launch_rotary(d->dtype, p, vec, rotation != nullptr && rotation->half != 0, true, true,
+                                           static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "norm and rotation backward launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}

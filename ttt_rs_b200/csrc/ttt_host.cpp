@@ -349,6 +349,161 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   }
 };
 
+// ---- rotary positions, norm and rotation of queries and keys -----------------------------------------------------------------
+// [B,H,T,F] on a GPU with contiguous rows
+bool head_rows(const Tensor& t, const c10::Device& dev, at::ScalarType dt) {
+  return t.defined() && t.is_cuda() && t.device() == dev && t.scalar_type() == dt && t.layout() == c10::kStrided && t.dim() == 4 &&
+         (t.stride(3) == 1 || t.size(3) == 1);
+}
+struct Rotation {
+  Tensor turns, positions;
+  int64_t rdim = 0, half = 0, wrap = 0, start = 0;
+  double size = 1.0;
+  ttt_rotation r;
+  bool set(const Dims& m) {
+    r = ttt_rotation{};
+    if (!turns.defined()) return true;
+    if (rdim < 2 || rdim > m.F || !is(turns, at::kLong, m.dev, {rdim / 2}) || wrap < 0 || wrap > INT32_MAX) return false;
+    if (positions.defined()) {
+      const bool rows = positions.dim() == 2;
+      if (!positions.is_cuda() || positions.device() != m.dev || positions.scalar_type() != at::kLong || !positions.is_contiguous() ||
+          (!rows && positions.dim() != 1) || positions.size(-1) != m.T || (rows && positions.size(0) != m.B && positions.size(0) != 1))
+        return false;
+      r.positions_stride = rows && positions.size(0) > 1 ? m.T : 0;
+      r.positions = static_cast<const int64_t*>(positions.const_data_ptr());
+    }
+    r.turns = static_cast<const uint64_t*>(turns.const_data_ptr());
+    r.start_idx = start;
+    r.rotary_dim = (int32_t)rdim;
+    r.half = (int32_t)half;
+    r.wrap = (int32_t)wrap;
+    r.size = (float)size;
+    return true;
+  }
+  const ttt_rotation* get() const { return turns.defined() ? &r : nullptr; }
+  std::vector<int64_t> ints() const { return {rdim, half, wrap, start, turns.defined(), positions.defined()}; }
+  void from(const std::vector<int64_t>& v, double sz, const Tensor& t, const Tensor& p) {
+    rdim = v[0], half = v[1], wrap = v[2], start = v[3], size = sz;
+    if (v[4]) turns = t;
+    if (v[5]) positions = p;
+  }
+};
+Tensor given(const Tensor& t) { return t.defined() ? t : at::empty({0}); }  // (a node's arguments are defined tensors)
+
+bool head_dims(Dims& m, const Tensor& x, double eps) {
+  if (!x.defined() || x.dim() != 4 || !m.set(x, x.size(3), 1, 1, 0) || !head_rows(x, m.dev, m.dt)) return false;
+  m.d.epsilon = (float)eps;
+  return m.B > 0 && m.H > 0 && m.T > 0 && m.F >= 2;
+}
+int rotary(const Dims& m, const Tensor& x, const Rotation& rot, bool inverse, Tensor& y) {
+  c10::cuda::CUDAGuard guard(m.dev);
+  if (!y.defined()) y = at::empty({m.B, m.H, m.T, m.F}, m.opt());
+  return ttt_layer_rotary(&m.d, x.const_data_ptr(), Gated::strides<1>({&x}).data(), rot.get(), inverse, y.data_ptr(),
+                          Gated::strides<1>({&y}).data(), m.stream());
+}
+const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& turns, const Tensor& positions, std::vector<int64_t> ints,
+                        double size) {
+    Dims m;
+    Rotation rot;
+    Tensor y;
+    head_dims(m, x, 0.0);
+    rot.from(ints, size, turns, positions);
+    rot.set(m);
+    const int rc = rotary(m, x, rot, false, y);
+    if (rc != TTT_OK) throw_error(rc);
+    ctx->save_for_backward({turns, positions});
+    ctx->saved_data["i"] = ints;
+    ctx->saved_data["s"] = size;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const variable_list t = ctx->get_saved_variables();
+    Tensor g = go[0], y;
+    if (g.stride(3) != 1 && g.size(3) != 1) g = g.clone(at::MemoryFormat::Contiguous);
+    Dims m;
+    Rotation rot;
+    head_dims(m, g, 0.0);
+    rot.from(ctx->saved_data["i"].toIntVector(), ctx->saved_data["s"].toDouble(), t[0], t[1]);
+    rot.set(m);
+    const int rc = rotary(m, g, rot, true, y);
+    if (rc != TTT_OK) throw_error(rc);
+    return {y, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+struct QkNorm {
+  Dims m;
+  int64_t Hk = 0;
+  bool set(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, double eps) {
+    if (!head_dims(m, q, eps) || !head_rows(k, m.dev, m.dt)) return false;
+    Hk = k.size(1);
+    if (k.size(0) != m.B || k.size(2) != m.T || k.size(3) != m.F || Hk < 1 || Hk > INT32_MAX) return false;
+    for (const Tensor* w : {&wq, &wk})
+      if (w->defined() && !is(*w, m.dt, m.dev, {m.F})) return false;
+    return true;
+  }
+  int forward(const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk, const Rotation& rot, Tensor& yq, Tensor& yk) const {
+    c10::cuda::CUDAGuard guard(m.dev);
+    if (!yq.defined()) yq = at::empty({m.B, m.H, m.T, m.F}, m.opt());
+    if (!yk.defined()) yk = at::empty({m.B, Hk, m.T, m.F}, m.opt());
+    return ttt_layer_qk_norm_rotary(&m.d, (int)Hk, q.const_data_ptr(), k.const_data_ptr(), Gated::strides<2>({&q, &k}).data(), ptr(wq),
+                                    ptr(wk), rot.get(), yq.data_ptr(), yk.data_ptr(), Gated::strides<2>({&yq, &yk}).data(), m.stream());
+  }
+  int backward(const Tensor& q, const Tensor& k, const Tensor& gq, const Tensor& gk, const Tensor& wq, const Tensor& wk,
+               const Rotation& rot, Tensor& dq, Tensor& dk, Tensor& dwq, Tensor& dwk) const {
+    c10::cuda::CUDAGuard guard(m.dev);
+    if (!dq.defined()) dq = at::empty({m.B, m.H, m.T, m.F}, m.opt());
+    if (!dk.defined()) dk = at::empty({m.B, Hk, m.T, m.F}, m.opt());
+    if (wq.defined()) dwq = at::empty({m.F}, m.opt());
+    if (wk.defined()) dwk = at::empty({m.F}, m.opt());
+    const bool w = wq.defined() || wk.defined();
+    const size_t wsb = w ? ttt_layer_qk_norm_rotary_backward_workspace_bytes(&m.d, (int)Hk) : 0;
+    Tensor ws;
+    if (wsb != 0) ws = at::empty({(int64_t)wsb}, m.opt(at::kByte));
+    return ttt_layer_qk_norm_rotary_backward(
+        &m.d, (int)Hk, q.const_data_ptr(), k.const_data_ptr(), gq.const_data_ptr(), gk.const_data_ptr(),
+        Gated::strides<4>({&q, &k, &gq, &gk}).data(), ptr(wq), ptr(wk), rot.get(), dq.data_ptr(), dk.data_ptr(),
+        Gated::strides<2>({&dq, &dk}).data(), wq.defined() ? dwq.data_ptr() : nullptr, wk.defined() ? dwk.data_ptr() : nullptr,
+        wsb != 0 ? ws.data_ptr() : nullptr, wsb, m.stream());
+  }
+};
+struct QkNormFn : torch::autograd::Function<QkNormFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& wq, const Tensor& wk,
+                               const Tensor& turns, const Tensor& positions, std::vector<int64_t> ints, double size, double eps) {
+    QkNorm call;
+    Rotation rot;
+    Tensor yq, yk;
+    const Tensor w0 = ints[6] ? wq : Tensor(), w1 = ints[7] ? wk : Tensor();
+    call.set(q, k, w0, w1, eps);
+    rot.from(ints, size, turns, positions);
+    rot.set(call.m);
+    const int rc = call.forward(q, k, w0, w1, rot, yq, yk);
+    if (rc != TTT_OK) throw_error(rc);
+    ctx->save_for_backward({q, k, wq, wk, turns, positions});
+    ctx->saved_data["i"] = ints;
+    ctx->saved_data["s"] = size;
+    ctx->saved_data["e"] = eps;
+    return {yq, yk};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const variable_list t = ctx->get_saved_variables();
+    const std::vector<int64_t> ints = ctx->saved_data["i"].toIntVector();
+    for (Tensor& g : go)  // (undefined ones are zeros here)
+      if (g.stride(3) != 1 && g.size(3) != 1) g = g.clone(at::MemoryFormat::Contiguous);
+    QkNorm call;
+    Rotation rot;
+    const Tensor w0 = ints[6] ? t[2] : Tensor(), w1 = ints[7] ? t[3] : Tensor();
+    call.set(t[0], t[1], w0, w1, ctx->saved_data["e"].toDouble());
+    rot.from(ints, ctx->saved_data["s"].toDouble(), t[4], t[5]);
+    rot.set(call.m);
+    Tensor dq, dk, dwq, dwk;
+    const int rc = call.backward(t[0], t[1], go[0], go[1], w0, w1, rot, dq, dk, dwq, dwk);
+    if (rc != TTT_OK) throw_error(rc);
+    return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
 // ---- Python functions ----------------------------------------------------------------------------------------------
 // tensors args[0..n), false when one is not a tensor
 template <int N>
@@ -968,6 +1123,87 @@ PyObject* py_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A rotation's arguments: turns | None, rotary_dim, half, wrap, size, positions | None, start_idx
+bool rotation_args(PyObject* const* a, Rotation& rot) {
+  if (!optional_tensor(a[0], rot.turns) || !optional_tensor(a[5], rot.positions)) return false;
+  rot.rdim = as_int(a[1]), rot.half = as_int(a[2]), rot.wrap = as_int(a[3]), rot.size = PyFloat_AsDouble(a[4]), rot.start = as_int(a[6]);
+  return true;
+}
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+bool same_shape_result(const Tensor& y, const Tensor& x, const Dims& m) {
+  return !y.defined() || (head_rows(y, m.dev, m.dt) && y.sizes() == x.sizes());
+}
+// rotary(x, rotation (7), inverse, out | None) -> y, recorded for autograd where that is on and asked for | None
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 10)) return nullptr;
+  Tensor x[1], y;
+  Dims m;
+  Rotation rot;
+  NONE_IF(!tensors(args, x) || !rotation_args(args + 1, rot) || !optional_tensor(args[9], y));
+  const bool inverse = as_int(args[8]) != 0;
+  if (PyErr_Occurred()) return nullptr;
+  NONE_IF(!rot.turns.defined() || !head_dims(m, x[0], 0.0) || !rot.set(m) || !same_shape_result(y, x[0], m));
+  if (wants_grad({&x[0]})) {
+    NONE_IF(y.defined() || inverse);
+    return THPVariable_Wrap(RotaryFn::apply(x[0], rot.turns, given(rot.positions), rot.ints(), rot.size));
+  }
+  const int rc = rotary(m, x[0], rot, inverse, y);
+  if (rc != TTT_OK) throw_error(rc);
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+// qk_norm(q, k, q_weight | None, k_weight | None, rotation (7), eps, q_out | None, k_out | None) -> (q, k), recorded for autograd
+// where that is on and asked for | None
+PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 14)) return nullptr;
+  Tensor x[2], wq, wk, yq, yk;
+  QkNorm call;
+  Rotation rot;
+  NONE_IF(!tensors(args, x) || !optional_tensor(args[2], wq) || !optional_tensor(args[3], wk) || !rotation_args(args + 4, rot) ||
+          !optional_tensor(args[12], yq) || !optional_tensor(args[13], yk));
+  const double eps = PyFloat_AsDouble(args[11]);
+  if (PyErr_Occurred()) return nullptr;
+  NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m));
+  if (wants_grad({&x[0], &x[1], &wq, &wk})) {
+    NONE_IF(yq.defined() || yk.defined());
+    std::vector<int64_t> ints = rot.ints();
+    ints.push_back(wq.defined());
+    ints.push_back(wk.defined());
+    return wrap(QkNormFn::apply(x[0], x[1], given(wq), given(wk), given(rot.turns), given(rot.positions), ints, rot.size, eps));
+  }
+  const int rc = call.forward(x[0], x[1], wq, wk, rot, yq, yk);
+  if (rc != TTT_OK) throw_error(rc);
+  return wrap({yq, yk});
+  END_HANDLE_TH_ERRORS
+}
+// qk_norm_backward(q, k, grad_q_out, grad_k_out, q_weight | None, k_weight | None, rotation (7), eps, grad_q, grad_k) ->
+// (grad_q, grad_k, grad_q_weight | None, grad_k_weight | None): into the given tensors, for the layer's own node
+PyObject* py_qk_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 16)) return nullptr;
+  Tensor x[4], wq, wk, d[2], dwq, dwk;
+  QkNorm call;
+  Rotation rot;
+  NONE_IF(!tensors(args, x) || !optional_tensor(args[4], wq) || !optional_tensor(args[5], wk) || !rotation_args(args + 6, rot) ||
+          !tensors(args + 14, d));
+  const double eps = PyFloat_AsDouble(args[13]);
+  if (PyErr_Occurred()) return nullptr;
+  NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m));
+  for (int i = 0; i < 2; ++i)
+    NONE_IF(!head_rows(x[2 + i], call.m.dev, call.m.dt) || x[2 + i].sizes() != x[i].sizes() || !same_shape_result(d[i], x[i], call.m));
+  const int rc = call.backward(x[0], x[1], x[2], x[3], wq, wk, rot, d[0], d[1], dwq, dwk);
+  if (rc != TTT_OK) throw_error(rc);
+  return wrap({d[0], d[1], dwq, dwk});
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(set_status),
@@ -982,6 +1218,9 @@ PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(layer_infer),
                          FAST(layer_train),
                          FAST(gated),
+                         FAST(rotary),
+                         FAST(qk_norm),
+                         FAST(qk_norm_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

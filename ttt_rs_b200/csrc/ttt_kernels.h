@@ -455,4 +455,24 @@ cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, c
 cudaError_t launch_gated_bwd(int dtype, int F, const GatedMaps& maps, const GatedBwdParams& p, cudaStream_t st);
 cudaError_t launch_gated_step(int dtype, int F, const GatedStepParams& p, int nstreams, cudaStream_t st);
 
+// ---- rotary positions, norm of queries and keys (ttt_rotary.cu): tensors 0 (queries) and 1 (keys; heads[1] = 0: none) ----
+struct RotaryParams {
+  const void* x[2];
+  const void* g[2];  // gradients of the results (backward of the norm)
+  void* y[2];
+  int64_t xs[2][3], gs[2][3], ys[2][3];  // strides of batch, head and token, in elements
+  const void* w[2];                      // [F] or null: ones
+  void* dw[2];
+  float* partials;                       // rotary_partial_floats, or null: no gradients of weights are wanted
+  const uint64_t* turns;                 // [rdim / 2] turns per position, in 2^-64
+  const int64_t* positions;              // [B or 1][T] or null: start + t
+  int64_t pos_stride, start, tokens;     // tokens: B T
+  int heads[2], T, F, rdim, wrap;
+  float size, sign, eps;
+  int lanes, rows_each;                  // set by the launcher
+};
+size_t rotary_partial_floats(int64_t tokens, int rows, int F);
+// vec: F and rdim multiples of 8, all rows on 16 bytes
+cudaError_t launch_rotary(int dtype, const RotaryParams& p, bool vec, bool half, bool norm, bool bwd, cudaStream_t st);
+
 }  // namespace ttt

@@ -73,7 +73,6 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     mbar_init(bar_w, 1);
     fence_mbar_init();
   }
-  pdl_join();
   __syncthreads();
   auto chunk_of = [&](int i) { return c_hi - 1 - i; };
   // thread 0.  bf16: q, k, v, u of a chunk; float32: two of them at a time, through the same rows of shared memory
@@ -515,7 +514,8 @@ static cudaError_t launch_one(const GatedMaps& maps, const GatedBwdParams& p, cu
     return cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   });
   if (e != cudaSuccess) return e;
-  return launch_dependent(kfn, p.nstreams * p.nseg, GB_THREADS, smem, st, maps, p);
+  kfn<<<p.nstreams * p.nseg, GB_THREADS, smem, st>>>(maps, p);
+  return cudaGetLastError();
 }
 cudaError_t launch_gated_bwd(int dtype, int F, const GatedMaps& maps, const GatedBwdParams& p, cudaStream_t st) {
   if (F == 64) return dtype == 1 ? launch_one<__nv_bfloat16, 64>(maps, p, st) : launch_one<float, 64>(maps, p, st);

@@ -53,7 +53,6 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     mbar_init(bar + 8, 1);
     fence_mbar_init();
   }
-  pdl_join();
   __syncthreads();
   auto chunk_of = [&](int i) { return REV ? c_hi - 1 - i : c_lo + i; };
   auto fetch = [&](int i) {  // thread 0
@@ -248,7 +247,6 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
 // state[s] <- W_s, W_{s+1} = decay[s] W_s + own[s].  Every thread carries one float4 of a stream's state.
 template <int F, bool REV>
 __global__ void __launch_bounds__(256) ttt_gated_join_kernel(const GatedParams p) {
-  pdl_join();
   constexpr int Q = F * F / 4;
   const long e = (long)blockIdx.x * 256 + threadIdx.x;
   if (e >= (long)p.nstreams * Q) return;
@@ -287,7 +285,8 @@ static cudaError_t launch_one(const GatedMaps& maps, const GatedParams& p, int g
     return cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   });
   if (e != cudaSuccess) return e;
-  return launch_dependent(kfn, grid, GF_THREADS, smem, st, maps, p);
+  kfn<<<grid, GF_THREADS, smem, st>>>(maps, p);
+  return cudaGetLastError();
 }
 
 template <typename T, int F>
@@ -295,8 +294,8 @@ static cudaError_t launch_gated(const GatedMaps& maps, GatedParams p, bool save,
   if (p.nseg > 1) {
     cudaError_t e = launch_one<T, F, false, true, false>(maps, p, p.nstreams * p.nseg, st);
     if (e != cudaSuccess) return e;
-    e = launch_dependent(ttt_gated_join_kernel<F, false>, (int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st, p);
-    if (e != cudaSuccess) return e;
+    ttt_gated_join_kernel<F, false><<<(int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (save) return launch_one<T, F, true, false, false>(maps, p, p.nstreams * p.nseg, st);
   return launch_one<T, F, false, false, false>(maps, p, p.nstreams * p.nseg, st);
@@ -311,7 +310,8 @@ template <typename T, int F>
 static cudaError_t launch_rev(const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
   cudaError_t e = launch_one<T, F, false, true, true>(maps, p, p.nstreams * p.nseg, st);
   if (e != cudaSuccess) return e;
-  return launch_dependent(ttt_gated_join_kernel<F, true>, (int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st, p);
+  ttt_gated_join_kernel<F, true><<<(int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st>>>(p);
+  return cudaGetLastError();
 }
 cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
   if (F == 64) return dtype == 1 ? launch_rev<__nv_bfloat16, 64>(maps, p, st) : launch_rev<float, 64>(maps, p, st);

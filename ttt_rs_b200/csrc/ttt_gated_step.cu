@@ -19,7 +19,6 @@ __global__ void __launch_bounds__(GS_THREADS) ttt_gated_step_kernel(const GatedS
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = tid % QUADS, kg = tid / QUADS;
   const long stream = blockIdx.x;
   const long b = stream / p.H, h = stream - b * p.H;
-  pdl_join();
   float4 w[ROWS];
   const float4* src = reinterpret_cast<const float4*>(p.w) + stream * (F * QUADS);
 #pragma unroll
@@ -66,10 +65,11 @@ __global__ void __launch_bounds__(GS_THREADS) ttt_gated_step_kernel(const GatedS
 }
 
 cudaError_t launch_gated_step(int dtype, int F, const GatedStepParams& p, int nstreams, cudaStream_t st) {
-  if (F == 64) return dtype == 1 ? launch_dependent(ttt_gated_step_kernel<__nv_bfloat16, 64>, nstreams, GS_THREADS, 0, st, p)
-                                 : launch_dependent(ttt_gated_step_kernel<float, 64>, nstreams, GS_THREADS, 0, st, p);
-  return dtype == 1 ? launch_dependent(ttt_gated_step_kernel<__nv_bfloat16, 32>, nstreams, GS_THREADS, 0, st, p)
-                    : launch_dependent(ttt_gated_step_kernel<float, 32>, nstreams, GS_THREADS, 0, st, p);
+  if (F == 64 && dtype == 1) ttt_gated_step_kernel<__nv_bfloat16, 64><<<nstreams, GS_THREADS, 0, st>>>(p);
+  else if (F == 64) ttt_gated_step_kernel<float, 64><<<nstreams, GS_THREADS, 0, st>>>(p);
+  else if (dtype == 1) ttt_gated_step_kernel<__nv_bfloat16, 32><<<nstreams, GS_THREADS, 0, st>>>(p);
+  else ttt_gated_step_kernel<float, 32><<<nstreams, GS_THREADS, 0, st>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace ttt

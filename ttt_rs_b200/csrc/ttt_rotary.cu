@@ -146,7 +146,6 @@ __device__ __forceinline__ float group_sum(float v, int lanes) {
 // NORM: the norm before the rotation.  BWD (with NORM): its gradient.
 template <typename T, int V, int NU, bool HALF, bool NORM, bool BWD>
 __global__ void __launch_bounds__(ROT_THREADS) ttt_rotary_kernel(const RotaryParams p) {
-  pdl_join();
   const int lanes = p.lanes, tid = threadIdx.x, sub = tid & (lanes - 1), groups = ROT_THREADS / lanes;
   const int rows = p.heads[0] + p.heads[1];
   const int r_lo = (int)blockIdx.y * p.rows_each, r_hi = min(rows, r_lo + p.rows_each);
@@ -303,7 +302,6 @@ __global__ void __launch_bounds__(ROT_THREADS) ttt_rotary_kernel(const RotaryPar
 // The blocks' shares to the gradients of both weights: a warp per column, lanes over the blocks
 template <typename T>
 __global__ void __launch_bounds__(256) ttt_rotary_reduce_kernel(const float* partials, int blocks, int F, T* dq, T* dk) {
-  pdl_join();
   const int col = (int)blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (col >= 2 * F) return;
   float v = 0.f;
@@ -354,22 +352,16 @@ static cudaError_t launch_rot(RotaryParams p, bool norm, bool bwd, cudaStream_t 
   const RotaryGrid g = rotary_grid(p.tokens, p.heads[0] + p.heads[1], p.F, V == 4, bwd);
   p.rows_each = g.rows_each;
   p.lanes = g.lanes;
-  cudaLaunchAttribute at;
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(g.x, g.y);
-  cfg.blockDim = dim3(ROT_THREADS);
-  cfg.dynamicSmemBytes = bwd ? (ROT_THREADS / 32) * 2 * p.F * sizeof(float) : 0;
-  cfg.stream = st;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  if (!norm) return cudaLaunchKernelEx(&cfg, ttt_rotary_kernel<T, V, NU, HALF, false, false>, p);
-  if (!bwd) return cudaLaunchKernelEx(&cfg, ttt_rotary_kernel<T, V, NU, HALF, true, false>, p);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, ttt_rotary_kernel<T, V, NU, HALF, true, true>, p);
-  if (e != cudaSuccess || p.partials == nullptr) return e;
-  return launch_dependent(ttt_rotary_reduce_kernel<T>, (2 * p.F + 7) / 8, 256, 0, st, (const float*)p.partials, g.x * g.y, p.F,
-                          static_cast<T*>(p.dw[0]), static_cast<T*>(p.dw[1]));
+  const dim3 grid(g.x, g.y);
+  const size_t smem = bwd ? (ROT_THREADS / 32) * 2 * p.F * sizeof(float) : 0;
+  if (!norm) ttt_rotary_kernel<T, V, NU, HALF, false, false><<<grid, ROT_THREADS, 0, st>>>(p);
+  else if (!bwd) ttt_rotary_kernel<T, V, NU, HALF, true, false><<<grid, ROT_THREADS, 0, st>>>(p);
+  else ttt_rotary_kernel<T, V, NU, HALF, true, true><<<grid, ROT_THREADS, smem, st>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || !bwd || p.partials == nullptr) return e;
+  ttt_rotary_reduce_kernel<T><<<(2 * p.F + 7) / 8, 256, 0, st>>>(p.partials, g.x * g.y, p.F, static_cast<T*>(p.dw[0]),
+                                                                static_cast<T*>(p.dw[1]));
+  return cudaGetLastError();
 }
 template <typename T>
 static cudaError_t launch_rot_t(const RotaryParams& p, bool vec, bool half, bool norm, bool bwd, cudaStream_t st) {

@@ -28,7 +28,8 @@ template <>
 __device__ __forceinline__ Pk<2> split_pack<2>(float x, float y) {
   Pk<2> r;
   r.p[0] = pack_bf16(x, y);
-  r.p[1] = pack_bf16(x - bf16_lo(r.p[0]), y - bf16_hi(r.p[0]));
+  const float2 rest = __ffma2_rn(make_float2(bf16_lo(r.p[0]), bf16_hi(r.p[0])), make_float2(-1.f, -1.f), make_float2(x, y));
+  r.p[1] = pack_bf16(rest.x, rest.y);
   return r;
 }
 
@@ -40,23 +41,12 @@ struct GTile {
     const int x = F == 64 ? (row & 7) : ((row >> 1) & 3);
     return (uint32_t)(row * (int)ROW + (((col >> 3) ^ x) << 4) + ((col & 7) << 1));
   }
-  // lane addresses of ldmatrix.x4; row0 and col0 multiples of 8
-  // A operand [16 rows of the product][16 of its K], stored [row][k]
-  static __device__ __forceinline__ uint32_t a_mk(int lane, int row0, int k0) {
-    return off(row0 + (lane & 7) + ((lane >> 3) & 1) * 8, k0 + (lane >> 4) * 8);
-  }
-  // the same operand stored [k][row] (with .trans)
-  static __device__ __forceinline__ uint32_t a_km(int lane, int row0, int k0) {
-    return off(k0 + (lane & 7) + (lane >> 4) * 8, row0 + ((lane >> 3) & 1) * 8);
-  }
-  // B operand, two tiles of 8 of the product's columns, stored [n][k]
-  static __device__ __forceinline__ uint32_t b_nk(int lane, int n0, int k0) {
-    return off(n0 + (lane & 7) + (lane >> 4) * 8, k0 + ((lane >> 3) & 1) * 8);
-  }
-  // the same stored [k][n] (with .trans)
-  static __device__ __forceinline__ uint32_t b_kn(int lane, int n0, int k0) {
-    return off(k0 + (lane & 7) + ((lane >> 3) & 1) * 8, n0 + (lane >> 4) * 8);
-  }
+  // Lane addresses of ldmatrix.x4 within 16 rows: the address of a 16 x 16 block at row r (a multiple of 16) and column 16 c is
+  // (tile + r * ROW + lane part) ^ (c << 5), the tile on 128 bytes: the swizzle is an exclusive or with the row.
+  // low: matrices 0..3 at (0, 0), (8, 0), (0, 8), (8, 8): A operands stored [row][k], B operands stored [k][n] (.trans)
+  static __device__ __forceinline__ uint32_t low(int lane) { return off((lane & 7) + ((lane >> 3) & 1) * 8, (lane >> 4) * 8); }
+  // high: at (0, 0), (0, 8), (8, 0), (8, 8): B operands stored [n][k], A operands stored [k][row] (.trans)
+  static __device__ __forceinline__ uint32_t high(int lane) { return off((lane & 7) + (lane >> 4) * 8, ((lane >> 3) & 1) * 8); }
 };
 
 // c0 += a . b[0..1], c1 += a . b[2..3]: the products of planes whose weight is at least 2^-16 of the leading one
@@ -75,6 +65,31 @@ __device__ __forceinline__ void mma_planes(float (&c0)[4], float (&c1)[4], const
     }
   }
 }
+
+// rows g and g + 8 of an accumulator tile times a factor each; its column pair times a pair
+__device__ __forceinline__ void scale_rows(float (&c)[4], float a, float b) {
+  const F2 x = f2mul(make_float2(c[0], c[1]), f2(a)), y = f2mul(make_float2(c[2], c[3]), f2(b));
+  c[0] = x.x, c[1] = x.y, c[2] = y.x, c[3] = y.y;
+}
+__device__ __forceinline__ void scale_cols(float (&c)[4], F2 f) {
+  const F2 x = f2mul(make_float2(c[0], c[1]), f), y = f2mul(make_float2(c[2], c[3]), f);
+  c[0] = x.x, c[1] = x.y, c[2] = y.x, c[3] = y.y;
+}
+// d += rows of c times a factor each
+__device__ __forceinline__ void add_rows(float (&d)[4], const float (&c)[4], float a, float b) {
+  const F2 x = f2fma(make_float2(c[0], c[1]), f2(a), make_float2(d[0], d[1]));
+  const F2 y = f2fma(make_float2(c[2], c[3]), f2(b), make_float2(d[2], d[3]));
+  d[0] = x.x, d[1] = x.y, d[2] = y.x, d[3] = y.y;
+}
+// two accumulator tiles (16 rows x 16 columns) as an A operand
+template <int NP>
+__device__ __forceinline__ void as_operand(Pk<NP> (&a)[4], const float (&c0)[4], const float (&c1)[4]) {
+  a[0] = split_pack<NP>(c0[0], c0[1]);
+  a[1] = split_pack<NP>(c0[2], c0[3]);
+  a[2] = split_pack<NP>(c1[0], c1[1]);
+  a[3] = split_pack<NP>(c1[2], c1[3]);
+}
+__device__ __forceinline__ float2 ld2(const float* p) { return *reinterpret_cast<const float2*>(p); }
 
 template <int NP>
 __device__ __forceinline__ float pk_lo(const Pk<NP>& v) {
@@ -95,23 +110,28 @@ template <int NO, int NI>
 __device__ __forceinline__ void scale_a_cols(Pk<NO> (&o)[4], const Pk<NI> (&a)[4], float2 lo, float2 hi) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 s = i < 2 ? lo : hi;
-    o[i] = split_pack<NO>(pk_lo(a[i]) * s.x, pk_hi(a[i]) * s.y);
+    const float2 v = f2mul(make_float2(pk_lo(a[i]), pk_hi(a[i])), i < 2 ? lo : hi);
+    o[i] = split_pack<NO>(v.x, v.y);
   }
 }
 
-// The gates of a chunk, for all warps of a block
+// The gates of a chunk, for all warps of a block.  A decay between tokens of different blocks of 16 is the product of what is
+// left at the end of the first one's block, of the blocks between, and at the second one from the start of its block: factors
+// of rows, of pairs of blocks and of columns, none above 1 for g <= 0.  Only pairs within a block take an exponential each.
 struct ChunkGates {
   float hi[GC], lo[GC];  // G_i in units of log2, in two floats
   float from[GC];        // e^{G_i}: what is left at token i of the state before the chunk
-  float to[GC];          // e^{G_end - G_i}: what is left of token i after the chunk
+  float into[GC];        // the same of the state before i's block
+  float out[GC];         // what is left of token i behind its block
+  float out_b[GC];       // that times beta_i
+  float end_b[GC];       // what is left of token i behind the chunk, times beta_i
+  float end[GC];         // without beta_i
   float beta[GC];
+  float blocks[4][4];    // [a][b]: from the end of block a to the end of block b >= a
+  float starts[4];       // e^G before block a
   float all;             // e^{G_end}
   float pad[3];
 };
-__device__ __forceinline__ float gated_decay(const ChunkGates& s, int i, int j) {  // e^{G_i - G_j}
-  return exp2f((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
-}
 // One warp; lane l brings tokens 2l and 2l + 1 of the chunk.  Tokens behind the sequence: g = 0, beta = 0.
 __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2 g, float2 beta) {
   auto log2_of = [](float x) {
@@ -125,14 +145,55 @@ __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2
     const double up = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += up;
   }
-  const double end = __shfl_sync(0xffffffffu, sum, 31), G0 = sum - g1, G1 = sum;
+  const int blk = lane >> 3;
+  const double G0 = sum - g1, G1 = sum, end = __shfl_sync(0xffffffffu, sum, 31);
+  double ends[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) ends[k] = __shfl_sync(0xffffffffu, sum, 8 * k + 7);
+  const double mine = blk == 0 ? ends[0] : blk == 1 ? ends[1] : blk == 2 ? ends[2] : ends[3];
+  const double before = blk == 0 ? 0.0 : blk == 1 ? ends[0] : blk == 2 ? ends[1] : ends[2];
+  auto put = [&](float* a, float x, float y) { *reinterpret_cast<float2*>(a + 2 * lane) = make_float2(x, y); };
   const float h0 = (float)G0, h1 = (float)G1;
-  *reinterpret_cast<float2*>(&s.hi[2 * lane]) = make_float2(h0, h1);
-  *reinterpret_cast<float2*>(&s.lo[2 * lane]) = make_float2((float)(G0 - h0), (float)(G1 - h1));
-  *reinterpret_cast<float2*>(&s.from[2 * lane]) = make_float2(exp2f((float)G0), exp2f((float)G1));
-  *reinterpret_cast<float2*>(&s.to[2 * lane]) = make_float2(exp2f((float)(end - G0)), exp2f((float)(end - G1)));
-  *reinterpret_cast<float2*>(&s.beta[2 * lane]) = beta;
+  put(s.hi, h0, h1);
+  put(s.lo, (float)(G0 - h0), (float)(G1 - h1));
+  put(s.from, exp2f((float)G0), exp2f((float)G1));
+  put(s.into, exp2f((float)(G0 - before)), exp2f((float)(G1 - before)));
+  const float o0 = exp2f((float)(mine - G0)), o1 = exp2f((float)(mine - G1));
+  const float e0 = exp2f((float)(end - G0)), e1 = exp2f((float)(end - G1));
+  put(s.out, o0, o1);
+  put(s.out_b, o0 * beta.x, o1 * beta.y);
+  put(s.end, e0, e1);
+  put(s.end_b, e0 * beta.x, e1 * beta.y);
+  put(s.beta, beta.x, beta.y);
+  if (lane < 16) {
+    const int a = lane >> 2, b = lane & 3;
+    double ga = ends[0], gb = ends[0];
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+      if (a == k) ga = ends[k];
+      if (b == k) gb = ends[k];
+    }
+    s.blocks[a][b] = b >= a ? exp2f((float)(gb - ga)) : 0.f;
+    if (b == 0) s.starts[a] = a == 0 ? 1.f : exp2f((float)(a == 1 ? ends[0] : a == 2 ? ends[1] : ends[2]));
+  }
   if (lane == 0) s.all = exp2f((float)end);
+}
+// Decays e^{G_i - G_j} of the 16 x 16 pairs of block `blk` with row r (g, g + 8) and column c (2t, 2t + 1, 2t + 8, 2t + 9) of a
+// lane's accumulators: [row half][column]; rows are i (ROWS_LATE) or j.  Zero where i < j.
+template <bool ROWS_LATE>
+__device__ __forceinline__ void block_decays(float (&d)[2][4], const ChunkGates& s, int blk, int g, int t4) {
+  const int r0 = 16 * blk + g, c0 = 16 * blk + 2 * t4;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = r0 + 8 * half;
+    const float hr = s.hi[r], lr = s.lo[r];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = c0 + (e & 1) + 8 * (e >> 1);
+      const float x = (hr - s.hi[c]) + (lr - s.lo[c]);
+      d[half][e] = (ROWS_LATE ? c <= r : c >= r) ? exp2f(ROWS_LATE ? x : -x) : 0.f;
+    }
+  }
 }
 // what lane `lane` brings for the chunk that starts at token t0
 __device__ __forceinline__ float2 load_gates(const float* x, int t0, int T, int lane, float none) {
@@ -222,44 +283,33 @@ struct StateShare {
   static constexpr int SLABS = F / 16, PARTS = GATED_WARPS / SLABS, COLS = F / PARTS, NT = COLS / 8;
 };
 
-// A warp's share of the state (rows row0.., columns col0..) as NP bf16 planes in the tile layout: to shared memory (planes
-// STATE_BYTES apart) and, where `image` is given, the same bytes to global memory.
+// A warp's share of the state (rows row0.., columns col0..) as NP bf16 planes (STATE_BYTES apart) in the tile layout of shared
+// memory
 template <int F, int NP>
-__device__ __forceinline__ void put_state(const float (&w)[StateShare<F>::NT][4], int row0, int col0, uint32_t smem, uint8_t* image,
-                                          int lane) {
-  using S = StateShare<F>;
-  const int g = lane >> 2, t = lane & 3;
-  auto put = [&](uint32_t (&r)[4], int plane, int row, int col) {
-    quad_transpose(r, lane);
-    const uint32_t at = plane * GTile<F>::STATE_BYTES + GTile<F>::off(row, col);
-    if (smem != 0)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(smem + at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-    if (image != nullptr) *reinterpret_cast<uint4*>(image + at) = make_uint4(r[0], r[1], r[2], r[3]);
-  };
-  if constexpr (S::NT % 4 == 0) {
+__device__ __forceinline__ void put_state(const float (&w)[StateShare<F>::NT][4], int row0, int col0, uint32_t smem, int lane) {
+  const uint32_t at = smem + row0 * GTile<F>::ROW + GTile<F>::low(lane);
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
-#pragma unroll
-      for (int n = 0; n < S::NT; n += 4) {
-        Pk<NP> v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = split_pack<NP>(w[n + k][2 * half], w[n + k][2 * half + 1]);
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-          uint32_t r[4] = {v[0].p[i], v[1].p[i], v[2].p[i], v[3].p[i]};
-          put(r, i, row0 + g + 8 * half, col0 + 8 * (n + t));
-        }
-      }
-  } else {
-    static_assert(S::NT == 2, "two tiles of eight columns");
+  for (int n = 0; n < StateShare<F>::NT; n += 2) {
     Pk<NP> v[4];
+    as_operand<NP>(v, w[n], w[n + 1]);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = split_pack<NP>(w[k & 1][k & 2], w[k & 1][(k & 2) + 1]);
+    for (int i = 0; i < NP; ++i)
+      stsm_x4((at ^ ((col0 + 8 * n) << 1)) + i * GTile<F>::STATE_BYTES, v[0].p[i], v[1].p[i], v[2].p[i], v[3].p[i]);
+  }
+}
+// The same share as the threads hold it, 16 bytes a thread side by side (what the forward saves for the backward)
+template <int F>
+__device__ __forceinline__ void put_fragments(float4* m, const float (&w)[StateShare<F>::NT][4], int warp, int lane) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      uint32_t r[4] = {v[0].p[i], v[1].p[i], v[2].p[i], v[3].p[i]};
-      put(r, i, row0 + g + 8 * (t >> 1), col0 + 8 * (t & 1));
-    }
+  for (int n = 0; n < StateShare<F>::NT; ++n)
+    m[(warp * StateShare<F>::NT + n) * 32 + lane] = make_float4(w[n][0], w[n][1], w[n][2], w[n][3]);
+}
+template <int F>
+__device__ __forceinline__ void get_fragments(float (&w)[StateShare<F>::NT][4], const float4* m, int warp, int lane) {
+#pragma unroll
+  for (int n = 0; n < StateShare<F>::NT; ++n) {
+    const float4 v = m[(warp * StateShare<F>::NT + n) * 32 + lane];
+    w[n][0] = v.x, w[n][1] = v.y, w[n][2] = v.z, w[n][3] = v.w;
   }
 }
 // The same share to and from a float32 matrix [F][F]

@@ -17,6 +17,8 @@
 // float32 dW in their registers with its update.  Warps 4-7 own 16 keys each: dk, dv and the gates' sums.  Per chunk two
 // barriers: all warps at its end, and the second group once more before it reads dW, which the first publishes after the first
 // barrier.
+#include <type_traits>
+
 #include "ttt_kernels.h"
 #include "ttt_gated.cuh"
 #include "ttt_stage.cuh"
@@ -24,6 +26,7 @@
 namespace ttt {
 
 constexpr int GB_THREADS = 2 * 32 * GATED_WARPS;
+__device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0, %0;" ::"n"(GB_THREADS) : "memory"); }
 
 struct ChunkSums {
   float r[GC], s[GC];               // r_i; beta_j s_j
@@ -42,11 +45,11 @@ struct GatedBwdSmem {
   static constexpr uint32_t STATE = NS * GTile<F>::STATE_BYTES;
   static constexpr uint32_t STAGES = BF ? 2 : 1;
   static constexpr uint32_t TILES = 0, RAWS = TILES + STAGES * 4 * TILE;
-  static constexpr uint32_t WSAVED = RAWS + (BF ? 0 : 2 * RAW);  // as it was saved (bf16: the planes themselves)
+  static constexpr uint32_t WSAVED = RAWS + (BF ? 0 : 2 * RAW);  // as it was saved; bf16: its planes take the same bytes
   static constexpr uint32_t W = BF ? WSAVED : WSAVED + WRAW, DW = W + STATE;
   static constexpr uint32_t GATES = DW + STATE;
   static constexpr uint32_t SUMS = GATES + 2 * sizeof(ChunkGates);
-  static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 32 + 1024;
+  static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 32 + 1024;  // (BAR + 24: a wait has run out)
   static_assert(!BF || STATE == WRAW, "two planes of bf16 are as long as the float32 state");
 };
 
@@ -102,14 +105,11 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     make_chunk_gates(gates[0], lane, load_gates(gp, t0, p.T, lane, 0.f), load_gates(bp, t0, p.T, lane, 1.f));
   }
   const int row0 = 16 * (w % SH::SLABS), part = w / SH::SLABS, col0 = part * SH::COLS;
-  float dW[SH::NT][4];
-  if (queries) {
-    const float* d0 = seg < p.nseg - 1 ? p.seg_state + ((size_t)stream * p.nseg + seg) * F * F
-                      : p.dw_out != nullptr ? p.dw_out + (size_t)stream * F * F : nullptr;
-    load_state<F>(dW, d0, row0, col0, lane);
-  }
+  volatile int* const failed = reinterpret_cast<volatile int*>(mem + SM::BAR + 24);
+  if (tid == 0) *failed = 0;
   __syncthreads();
 
+  const uint32_t low = TL::low(lane), high = TL::high(lane);
   // the gradients of the gates of walk step i, from the sums its warps left (one warp)
   auto finish_gates = [&](int i) {
     const ChunkSums& cs = sums[i & 1];
@@ -163,9 +163,19 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     }
   };
 
+  // One walk per group, so that neither carries the other's registers; the groups meet at barriers by number.
+  auto walk = [&](auto group) {
+  constexpr bool QUERIES = decltype(group)::value;
+  float dW[QUERIES ? SH::NT : 1][4];
+  if constexpr (QUERIES) {
+    const float* d0 = seg < p.nseg - 1 ? p.seg_state + ((size_t)stream * p.nseg + seg) * F * F
+                      : p.dw_out != nullptr ? p.dw_out + (size_t)stream * F * F : nullptr;
+    load_state<F>(dW, d0, row0, col0, lane);
+  }
+#pragma unroll 1
   for (int i = 0; i < n; ++i) {
     const int slot = BF ? i & 1 : 0, t0 = chunk_of(i) * GC, rows = p.T - t0;
-    const bool ahead = tid < 32 && i + 1 < n;
+    const bool ahead = QUERIES && w == 0 && i + 1 < n;
     float2 g_next, b_next;
     if (ahead) {
       g_next = load_gates(gp, chunk_of(i + 1) * GC, p.T, lane, 0.f);
@@ -176,8 +186,8 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     const uint32_t tw = base + SM::W, tdw = base + SM::DW;
     const ChunkGates& cg = gates[i & 1];
     ChunkSums& cs = sums[i & 1];
-    if (queries) {  // dW behind this chunk, for the other group
-      put_state<F, NS>(dW, row0, col0, tdw, nullptr, lane);
+    if constexpr (QUERIES) {  // dW behind this chunk, for the other group
+      put_state<F, NS>(dW, row0, col0, tdw, lane);
       asm volatile("bar.arrive 1, %0;" ::"n"(GB_THREADS) : "memory");
     }
     bool ok = mbar_wait_bounded(bar + 8 * slot, BF ? (i >> 1) & 1 : 0);
@@ -187,319 +197,342 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
           split_rows<F>(dst + m * SM::TILE, SM::PLANE, reinterpret_cast<const float*>(mem + SM::RAWS + m * SM::RAW), GC, tid, GB_THREADS);
       };
       split2(tq);
-      __syncthreads();
+      block_sync();
       if (tid == 0 && ok) fetch(i, 2, 2);
-      ok = ok && mbar_wait_bounded(bar, 1) && mbar_wait_bounded(bar_w, i & 1);
+      ok = ok && mbar_wait_bounded(bar, 1);
       split2(tv);
-      split_rows<F>(tw, TL::STATE_BYTES, reinterpret_cast<const float*>(mem + SM::WSAVED), F, tid, GB_THREADS);
-      __syncthreads();
-      if (tid == 0 && ok && i + 1 < n) {
-        fetch(i + 1, 0, 2);
-        fetch_w(i + 1);
-      }
+      block_sync();
+      if (tid == 0 && ok && i + 1 < n) fetch(i + 1, 0, 2);
     }
     if (!ok) {
       if (tid == 0) report_timeout(p.status, 21, (uint32_t)i);
       return;
     }
-    if (queries) {
+    if constexpr (QUERIES) {
       const int ia = 16 * w + g;
       float dq[F / 8][4];
 #pragma unroll
       for (int k = 0; k < F / 8; ++k) dq[k][0] = dq[k][1] = dq[k][2] = dq[k][3] = 0.f;
-      Pk<NP> u[KS][4];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(u[k], tu + TL::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
-      // inside the chunk
-      const float ha = cg.hi[ia], la = cg.lo[ia], hb = cg.hi[ia + 8], lb = cg.lo[ia + 8];
-#pragma unroll
-      for (int jt = 0; jt < GC / 16; ++jt) {
-        if (jt > w) break;
+      const uint32_t uq = tu + 16 * w * TL::ROW + low;
+      // inside the chunk: the blocks before this warp's, then its own
+      const float ra = cg.into[ia], rb = cg.into[ia + 8];
+#pragma unroll 1
+      for (int jt = 0; jt <= w; ++jt) {
         float s0[4] = {}, s1[4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          Pk<NP> f[4];
-          ldsm_np<NP>(f, tv + TL::b_nk(lane, 16 * jt, 16 * k), SM::PLANE, false);
-          mma_planes<NP, NP>(s0, s1, u[k], f);
+          Pk<NP> u[4], f[4];
+          ldsm_np<NP>(u, uq ^ (k << 5), SM::PLANE, false);
+          ldsm_np<NP>(f, (tv + 16 * jt * TL::ROW + high) ^ (k << 5), SM::PLANE, false);
+          mma_planes<NP, NP>(s0, s1, u, f);
         }
         const int j0 = 16 * jt + 2 * t4;
+        if (jt < w) {
+          const F2 between = f2(cg.blocks[jt][w - 1]);
+          scale_cols(s0, f2mul(ld2(&cg.out_b[j0]), between));
+          scale_cols(s1, f2mul(ld2(&cg.out_b[j0 + 8]), between));
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + (e & 1) + 8 * (e >> 1);
-          const float hj = cg.hi[j], lj = cg.lo[j], bj = cg.beta[j];
-          float* s = e < 2 ? s0 : s1;
-          s[e & 1] = j <= ia ? s[e & 1] * (exp2f((ha - hj) + (la - lj)) * bj) : 0.f;
-          s[2 + (e & 1)] = j <= ia + 8 ? s[2 + (e & 1)] * (exp2f((hb - hj) + (lb - lj)) * bj) : 0.f;
+          for (int k = 0; k < F / 8; ++k) scale_rows(dq[k], ra, rb);
+          float d[2][4];
+          block_decays<true>(d, cg, w, g, t4);
+          const float2 b0 = ld2(&cg.beta[j0]), b1 = ld2(&cg.beta[j0 + 8]);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            s0[2 * half] = d[half][0] > 0.f ? s0[2 * half] * (d[half][0] * b0.x) : 0.f;
+            s0[2 * half + 1] = d[half][1] > 0.f ? s0[2 * half + 1] * (d[half][1] * b0.y) : 0.f;
+            s1[2 * half] = d[half][2] > 0.f ? s1[2 * half] * (d[half][2] * b1.x) : 0.f;
+            s1[2 * half + 1] = d[half][3] > 0.f ? s1[2 * half + 1] * (d[half][3] * b1.y) : 0.f;
+          }
         }
-        const Pk<NP> a[4] = {split_pack<NP>(s0[0], s0[1]), split_pack<NP>(s0[2], s0[3]), split_pack<NP>(s1[0], s1[1]),
-                             split_pack<NP>(s1[2], s1[3])};
+        Pk<NP> a[4];
+        as_operand<NP>(a, s0, s1);
 #pragma unroll
         for (int m = 0; m < KS; ++m) {
           Pk<NP> f[4];
-          ldsm_np<NP>(f, tk + TL::b_kn(lane, 16 * m, 16 * jt), SM::PLANE, true);
+          ldsm_np<NP>(f, (tk + 16 * jt * TL::ROW + low) ^ (m << 5), SM::PLANE, true);
           mma_planes<NP, NP>(dq[2 * m], dq[2 * m + 1], a, f);
         }
       }
-      // from the state before the chunk
-      if constexpr (BF) {
-        if (!mbar_wait_bounded(bar_w, i & 1)) {
-          if (tid == 0) report_timeout(p.status, 22, (uint32_t)i);
-          ok = false;
-        }
+      // from the state before the chunk: this thread's share as it was saved, for the ways that cross the whole chunk, and its
+      // planes as an operand for all four warps
+      const float all = cg.all;
+      if (!mbar_wait_bounded(bar_w, i & 1)) {
+        if (tid == 0) report_timeout(p.status, 22, (uint32_t)i);
+        ok = false;
       }
+      {
+        float W[SH::NT][4];
+        get_fragments<F>(W, reinterpret_cast<const float4*>(mem + SM::WSAVED), w, lane);
+        F2 cross = f2(0.f);
+#pragma unroll
+        for (int k = 0; k < SH::NT; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) cross = f2fma(pr(W[k], half), pr(dW[k], half), cross);
+        float through = f2hsum(cross);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) through += __shfl_xor_sync(0xffffffffu, through, o);
+        if (lane == 0) cs.through[w] = through * all;
+        asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+        put_state<F, NS>(W, row0, col0, tw, lane);
+        asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+      }
+      Pk<NP> u[KS][4];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) ldsm_np<NP>(u[k], uq ^ (k << 5), SM::PLANE, false);
       const float fa = cg.from[ia], fb = cg.from[ia + 8];
-      float ra = 0.f, rb = 0.f;
+      F2 sa = f2(0.f), sb = f2(0.f);
 #pragma unroll
       for (int m = 0; m < KS; ++m) {
         float c0[4] = {}, c1[4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           Pk<NS> f[4];
-          ldsm_np<NS>(f, tw + TL::b_nk(lane, 16 * m, 16 * k), TL::STATE_BYTES, false);
+          ldsm_np<NS>(f, (tw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
           mma_planes<NP, NS>(c0, c1, u[k], f);
         }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float* c = e ? c1 : c0;
-          const int col = 16 * m + 8 * e + 2 * t4;
-          Pk<NP> qa, qb;
-#pragma unroll
-          for (int pl = 0; pl < NP; ++pl) {
-            qa.p[pl] = ld_shared_b32(tq + pl * SM::PLANE + TL::off(ia, col));
-            qb.p[pl] = ld_shared_b32(tq + pl * SM::PLANE + TL::off(ia + 8, col));
-          }
-          c[0] *= fa;
-          c[1] *= fa;
-          c[2] *= fb;
-          c[3] *= fb;
-          ra = fmaf(c[0], pk_lo(qa), fmaf(c[1], pk_hi(qa), ra));
-          rb = fmaf(c[2], pk_lo(qb), fmaf(c[3], pk_hi(qb), rb));
-#pragma unroll
-          for (int x = 0; x < 4; ++x) dq[2 * m + e][x] += c[x];
-        }
+        Pk<NP> q[4];
+        ldsm_np<NP>(q, (tq + 16 * w * TL::ROW + low) ^ (m << 5), SM::PLANE, false);  // (an A fragment is two accumulator tiles)
+        sa = f2fma(make_float2(c0[0], c0[1]), make_float2(pk_lo(q[0]), pk_hi(q[0])), sa);
+        sb = f2fma(make_float2(c0[2], c0[3]), make_float2(pk_lo(q[1]), pk_hi(q[1])), sb);
+        sa = f2fma(make_float2(c1[0], c1[1]), make_float2(pk_lo(q[2]), pk_hi(q[2])), sa);
+        sb = f2fma(make_float2(c1[2], c1[3]), make_float2(pk_lo(q[3]), pk_hi(q[3])), sb);
+        add_rows(dq[2 * m], c0, fa, fb);
+        add_rows(dq[2 * m + 1], c1, fa, fb);
       }
-      ra = quad_sum(ra);
-      rb = quad_sum(rb);
+      const float r0 = quad_sum(f2hsum(sa)) * fa, r1 = quad_sum(f2hsum(sb)) * fb;
       if (t4 == 0) {
-        cs.r[ia] = ra;
-        cs.r[ia + 8] = rb;
+        cs.r[ia] = r0;
+        cs.r[ia + 8] = r1;
       }
       store_rows<T, F>(static_cast<T*>(p.dq) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dq, lane);
-      // ways that cross the whole chunk
-      float through = 0.f;
-#pragma unroll
-      for (int k = 0; k < SH::NT; ++k)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          Pk<NS> s;
-#pragma unroll
-          for (int pl = 0; pl < NS; ++pl)
-            s.p[pl] = ld_shared_b32(tw + pl * TL::STATE_BYTES + TL::off(row0 + g + 8 * half, col0 + 8 * k + 2 * t4));
-          through = fmaf(pk_lo(s), dW[k][2 * half], fmaf(pk_hi(s), dW[k][2 * half + 1], through));
-        }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) through += __shfl_xor_sync(0xffffffffu, through, o);
-      const float all = cg.all;
-      if (lane == 0) cs.through[w] = through * all;
       // dW before the chunk
 #pragma unroll
-      for (int k = 0; k < SH::NT; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dW[k][e] *= all;
-#pragma unroll
+      for (int k = 0; k < SH::NT; ++k) scale_rows(dW[k], all, all);
+#pragma unroll 1
       for (int it = 0; it < GC / 16; ++it) {
         Pk<NS> qt[4];
         {
           Pk<NP> f[4];
-          ldsm_np<NP>(f, tq + TL::a_km(lane, row0, 16 * it), SM::PLANE, true);
-          scale_a_cols<NS, NP>(qt, f, *reinterpret_cast<const float2*>(&cg.from[16 * it + 2 * t4]),
-                               *reinterpret_cast<const float2*>(&cg.from[16 * it + 2 * t4 + 8]));
+          ldsm_np<NP>(f, (tq + 16 * it * TL::ROW + high) ^ (row0 << 1), SM::PLANE, true);
+          scale_a_cols<NS, NP>(qt, f, ld2(&cg.from[16 * it + 2 * t4]), ld2(&cg.from[16 * it + 2 * t4 + 8]));
         }
 #pragma unroll
         for (int k = 0; k < SH::NT / 2; ++k) {
           Pk<NP> f[4];
-          ldsm_np<NP>(f, tu + TL::b_kn(lane, col0 + 16 * k, 16 * it), SM::PLANE, true);
+          ldsm_np<NP>(f, (tu + 16 * it * TL::ROW + low) ^ ((col0 + 16 * k) << 1), SM::PLANE, true);
           mma_planes<NS, NP>(dW[2 * k], dW[2 * k + 1], qt, f);
         }
       }
     } else {
       const int ja = 16 * w + g;
-      float dk[F / 8][4], dv[F / 8][4];
+      const float oa = cg.out[ja], ob = cg.out[ja + 8], ba = cg.beta[ja], bb = cg.beta[ja + 8];
+      const float wa = cg.out_b[ja], wb = cg.out_b[ja + 8];
+      const uint32_t kq = tk + 16 * w * TL::ROW + low, vq = tv + 16 * w * TL::ROW + low;
+      Pk<NP> k_[KS][4];
 #pragma unroll
-      for (int k = 0; k < F / 8; ++k)
+      for (int k = 0; k < KS; ++k) ldsm_np<NP>(k_[k], kq ^ (k << 5), SM::PLANE, false);
+      // keys . queries and values . u of this warp's 16 tokens against those of block `it`
+      auto products = [&](int it, float (&s0)[4], float (&s1)[4], float (&v0)[4], float (&v1)[4]) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) dk[k][x] = dv[k][x] = 0.f;
-      const float ha = cg.hi[ja], la = cg.lo[ja], hb = cg.hi[ja + 8], lb = cg.lo[ja + 8];
-      const float ba = cg.beta[ja], bb = cg.beta[ja + 8];
-      float na = 0.f, nb = 0.f, ca = 0.f, cb = 0.f;  // sums of N over i >= j and over the blocks behind
-#pragma unroll
-      for (int it = 0; it < GC / 16; ++it) {
-        if (it < w) continue;
-        float s0[4] = {}, s1[4] = {}, v0[4] = {}, v1[4] = {};
+        for (int x = 0; x < 4; ++x) s0[x] = s1[x] = v0[x] = v1[x] = 0.f;
+        const uint32_t q = tq + 16 * it * TL::ROW + high, u = tu + 16 * it * TL::ROW + high;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           Pk<NP> a[4], f[4];
-          ldsm_np<NP>(a, tk + TL::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
-          ldsm_np<NP>(f, tq + TL::b_nk(lane, 16 * it, 16 * k), SM::PLANE, false);
-          mma_planes<NP, NP>(s0, s1, a, f);
-          ldsm_np<NP>(a, tv + TL::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
-          ldsm_np<NP>(f, tu + TL::b_nk(lane, 16 * it, 16 * k), SM::PLANE, false);
+          ldsm_np<NP>(f, q ^ (k << 5), SM::PLANE, false);
+          mma_planes<NP, NP>(s0, s1, k_[k], f);
+          ldsm_np<NP>(a, vq ^ (k << 5), SM::PLANE, false);
+          ldsm_np<NP>(f, u ^ (k << 5), SM::PLANE, false);
           mma_planes<NP, NP>(v0, v1, a, f);
         }
-        const int i0 = 16 * it + 2 * t4;
-        float col[4];  // sums over this warp's j of beta_j N_ij, columns i0, i0 + 1, i0 + 8, i0 + 9
-        float Ma[4], Mb[4];
+      };
+      // sums over the eight row pairs of the warp: halve the columns that a lane carries with each exchange
+      auto column_sums = [&](const float (&col)[4], float* to) {
+        const bool up4 = lane & 4, up8 = lane & 8;
+        float k0 = up4 ? col[2] : col[0], k1 = up4 ? col[3] : col[1];
+        k0 += __shfl_xor_sync(0xffffffffu, up4 ? col[0] : col[2], 4);
+        k1 += __shfl_xor_sync(0xffffffffu, up4 ? col[1] : col[3], 4);
+        float k = up8 ? k1 : k0;
+        k += __shfl_xor_sync(0xffffffffu, up8 ? k0 : k1, 8);
+        k += __shfl_xor_sync(0xffffffffu, k, 16);
+        if (lane < 16) to[2 * t4 + (up4 ? 8 : 0) + (up8 ? 1 : 0)] = k;
+      };
+      // sums of N: over the blocks behind j's without what is left of j behind its own block (na, nb), and within the block
+      float na = 0.f, nb = 0.f, own_a = 0.f, own_b = 0.f;
+      Pk<NP> as[4][4], av[4][4];  // the operands of dv and dk: 0 the own block, d the one d blocks behind it
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int ii = i0 + (e & 1) + 8 * (e >> 1);
-          const float hi = cg.hi[ii], li = cg.lo[ii];
-          float *s = e < 2 ? s0 : s1, *v = e < 2 ? v0 : v1;
-          const int x = e & 1;
-          const float da = ii >= ja ? exp2f((hi - ha) + (li - la)) : 0.f, db = ii >= ja + 8 ? exp2f((hi - hb) + (li - lb)) : 0.f;
-          const float Na = ii >= ja ? s[x] * v[x] * da : 0.f, Nb = ii >= ja + 8 ? s[2 + x] * v[2 + x] * db : 0.f;
-          na += Na;
-          nb += Nb;
-          if (it > w) {
-            ca += Na;
-            cb += Nb;
-            col[e] = fmaf(ba, Na, bb * Nb);
-          } else {
-            Ma[e] = ii > ja ? ba * Na : 0.f;
-            Mb[e] = ii > ja + 8 ? bb * Nb : 0.f;
-          }
-          s[x] = ii >= ja ? s[x] * (da * ba) : 0.f;
-          v[x] = ii >= ja ? v[x] * (da * ba) : 0.f;
-          s[2 + x] = ii >= ja + 8 ? s[2 + x] * (db * bb) : 0.f;
-          v[2 + x] = ii >= ja + 8 ? v[2 + x] * (db * bb) : 0.f;
+      for (int d = 1; d < 4; ++d) {
+        const int it = w + d;
+        if (it < 4) {
+          float s0[4], s1[4], v0[4], v1[4];
+          products(it, s0, s1, v0, v1);
+          const F2 between = f2(cg.blocks[w][it - 1]);
+          const F2 f0 = f2mul(ld2(&cg.into[16 * it + 2 * t4]), between), f1 = f2mul(ld2(&cg.into[16 * it + 2 * t4 + 8]), between);
+          scale_cols(s0, f0);
+          scale_cols(s1, f1);
+          const F2 p0 = f2mul(pr(s0, 0), pr(v0, 0)), p1 = f2mul(pr(s0, 1), pr(v0, 1));
+          const F2 p2 = f2mul(pr(s1, 0), pr(v1, 0)), p3 = f2mul(pr(s1, 1), pr(v1, 1));
+          na += f2hsum(f2add(p0, p2));
+          nb += f2hsum(f2add(p1, p3));
+          const F2 x0 = f2fma(p0, f2(wa), f2mul(p1, f2(wb))), x1 = f2fma(p2, f2(wa), f2mul(p3, f2(wb)));
+          const float col[4] = {x0.x, x0.y, x1.x, x1.y};
+          column_sums(col, cs.rows[w] + 16 * it);
+          scale_cols(v0, f0);
+          scale_cols(v1, f1);
+          as_operand<NP>(as[d], s0, s1);
+          as_operand<NP>(av[d], v0, v1);
         }
-        if (it == w) {  // the ways within the block across token t: over j < t the sums of i >= t
-          auto behind = [&](float (&m)[4]) {
-            float lo = m[0] + m[1], hi = m[2] + m[3];
+      }
+      {
+        float s0[4], s1[4], v0[4], v1[4], d[2][4], M[2][4], col[4];
+        products(w, s0, s1, v0, v1);
+        block_decays<false>(d, cg, w, g, t4);
 #pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-              const float l = __shfl_down_sync(0xffffffffu, lo, o, 4), u = __shfl_down_sync(0xffffffffu, hi, o, 4);
-              if (t4 + o < 4) {
-                lo += l;
-                hi += u;
-              }
-            }
-            const float l = __shfl_down_sync(0xffffffffu, lo, 1, 4), u = __shfl_down_sync(0xffffffffu, hi, 1, 4);
-            const float upper = __shfl_sync(0xffffffffu, hi, 0, 4), lo1 = t4 == 3 ? 0.f : l, hi1 = t4 == 3 ? 0.f : u;
-            m[3] += hi1;
-            m[2] += m[3];
-            m[1] += lo1 + upper;
-            m[0] += m[1];
-          };
-          behind(Ma);
-          behind(Mb);
+        for (int half = 0; half < 2; ++half) {
+          const float beta = half ? bb : ba;
+          float sum = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int t = i0 + (e & 1) + 8 * (e >> 1);
-            col[e] = (t > ja ? Ma[e] : 0.f) + (t > ja + 8 ? Mb[e] : 0.f);
+            float &s = (e < 2 ? s0 : s1)[2 * half + (e & 1)], &v = (e < 2 ? v0 : v1)[2 * half + (e & 1)];
+            const float x = d[half][e];
+            const float n_ij = x > 0.f ? s * v * x : 0.f;
+            sum += n_ij;
+            M[half][e] = 2 * t4 + (e & 1) + 8 * (e >> 1) > g + 8 * half ? beta * n_ij : 0.f;
+            s = x > 0.f ? s * (x * beta) : 0.f;
+            v = x > 0.f ? v * (x * beta) : 0.f;
           }
+          (half ? own_b : own_a) = sum;
         }
-        {  // over the eight row pairs of the warp: halve the columns that a lane carries with each exchange
-          const bool up4 = lane & 4, up8 = lane & 8;
-          float k0 = up4 ? col[2] : col[0], k1 = up4 ? col[3] : col[1];
-          k0 += __shfl_xor_sync(0xffffffffu, up4 ? col[0] : col[2], 4);
-          k1 += __shfl_xor_sync(0xffffffffu, up4 ? col[1] : col[3], 4);
-          float k = up8 ? k1 : k0;
-          k += __shfl_xor_sync(0xffffffffu, up8 ? k0 : k1, 8);
-          k += __shfl_xor_sync(0xffffffffu, k, 16);
-          if (lane < 16) (it > w ? cs.rows[w] : cs.block)[i0 + (up4 ? 8 : 0) + (up8 ? 1 : 0)] = k;
-        }
-        const Pk<NP> as[4] = {split_pack<NP>(s0[0], s0[1]), split_pack<NP>(s0[2], s0[3]), split_pack<NP>(s1[0], s1[1]),
-                              split_pack<NP>(s1[2], s1[3])};
-        const Pk<NP> av[4] = {split_pack<NP>(v0[0], v0[1]), split_pack<NP>(v0[2], v0[3]), split_pack<NP>(v1[0], v1[1]),
-                              split_pack<NP>(v1[2], v1[3])};
+        as_operand<NP>(as[0], s0, s1);
+        as_operand<NP>(av[0], v0, v1);
+        // the ways within the block across token t: over j < t the sums of i >= t
 #pragma unroll
-        for (int m = 0; m < KS; ++m) {
-          Pk<NP> f[4];
-          ldsm_np<NP>(f, tu + TL::b_kn(lane, 16 * m, 16 * it), SM::PLANE, true);
-          mma_planes<NP, NP>(dv[2 * m], dv[2 * m + 1], as, f);
-          ldsm_np<NP>(f, tq + TL::b_kn(lane, 16 * m, 16 * it), SM::PLANE, true);
-          mma_planes<NP, NP>(dk[2 * m], dk[2 * m + 1], av, f);
+        for (int half = 0; half < 2; ++half) {
+          float(&m)[4] = M[half];
+          float lo = m[0] + m[1], hi = m[2] + m[3];
+#pragma unroll
+          for (int o = 1; o < 4; o <<= 1) {
+            const float l = __shfl_down_sync(0xffffffffu, lo, o, 4), h = __shfl_down_sync(0xffffffffu, hi, o, 4);
+            if (t4 + o < 4) {
+              lo += l;
+              hi += h;
+            }
+          }
+          const float l = __shfl_down_sync(0xffffffffu, lo, 1, 4), h = __shfl_down_sync(0xffffffffu, hi, 1, 4);
+          const float upper = __shfl_sync(0xffffffffu, hi, 0, 4);
+          m[3] += t4 == 3 ? 0.f : h;
+          m[2] += m[3];
+          m[1] += (t4 == 3 ? 0.f : l) + upper;
+          m[0] += m[1];
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = 2 * t4 + (e & 1) + 8 * (e >> 1);
+          col[e] = (t > g ? M[0][e] : 0.f) + (t > g + 8 ? M[1][e] : 0.f);
+        }
+        column_sums(col, cs.block + 16 * w);
       }
       na = quad_sum(na);
       nb = quad_sum(nb);
-      ca = quad_sum(ca);
-      cb = quad_sum(cb);
-      // from the state's gradient behind the chunk
-      asm volatile("bar.sync 1, %0;" ::"n"(GB_THREADS) : "memory");
-      const float ta = cg.to[ja], tb = cg.to[ja + 8], wa = ta * ba, wb = tb * bb;
-      Pk<NP> fr[KS][4];
+      own_a = quad_sum(own_a);
+      own_b = quad_sum(own_b);
+      // rows of sum over the blocks of operand . tile: the blocks behind, what is left of the row behind its own block, the own one
+      auto gather = [&](float (&r)[F / 8][4], const Pk<NP> (&a)[4][4], uint32_t tile) {
 #pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(fr[k], tk + TL::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
+        for (int k = 0; k < F / 8; ++k) r[k][0] = r[k][1] = r[k][2] = r[k][3] = 0.f;
 #pragma unroll
-      for (int m = 0; m < KS; ++m) {
-        float c0[4] = {}, c1[4] = {};
+        for (int d = 3; d >= 0; --d) {
+          if (d == 0) {
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {  // (dv is a result of the inputs' type: bf16 takes the leading plane of dW)
-          Pk<NP> f[4];
-          ldsm_np<NP>(f, tdw + TL::b_kn(lane, 16 * m, 16 * k), TL::STATE_BYTES, true);
-          mma_planes<NP, NP>(c0, c1, fr[k], f);
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          dv[2 * m][x] = fmaf(x < 2 ? wa : wb, c0[x], dv[2 * m][x]);
-          dv[2 * m + 1][x] = fmaf(x < 2 ? wa : wb, c1[x], dv[2 * m + 1][x]);
-        }
-      }
-      store_rows<T, F>(static_cast<T*>(p.dv) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dv, lane);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(fr[k], tv + TL::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
-      float sa = 0.f, sb = 0.f;
-#pragma unroll
-      for (int m = 0; m < KS; ++m) {
-        float c0[4] = {}, c1[4] = {};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          Pk<NS> f[4];
-          ldsm_np<NS>(f, tdw + TL::b_nk(lane, 16 * m, 16 * k), TL::STATE_BYTES, false);
-          mma_planes<NP, NS>(c0, c1, fr[k], f);
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float* c = e ? c1 : c0;
-          const int col = 16 * m + 8 * e + 2 * t4;
-          Pk<NP> ka, kb;
-#pragma unroll
-          for (int pl = 0; pl < NP; ++pl) {
-            ka.p[pl] = ld_shared_b32(tk + pl * SM::PLANE + TL::off(ja, col));
-            kb.p[pl] = ld_shared_b32(tk + pl * SM::PLANE + TL::off(ja + 8, col));
+            for (int k = 0; k < F / 8; ++k) scale_rows(r[k], wa, wb);
           }
-          sa = fmaf(c[0], pk_lo(ka), fmaf(c[1], pk_hi(ka), sa));
-          sb = fmaf(c[2], pk_lo(kb), fmaf(c[3], pk_hi(kb), sb));
+          if (w + d < 4) {
+            const uint32_t at = tile + 16 * (w + d) * TL::ROW + low;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) dk[2 * m + e][x] = fmaf(x < 2 ? wa : wb, c[x], dk[2 * m + e][x]);
+            for (int m = 0; m < KS; ++m) {
+              Pk<NP> f[4];
+              ldsm_np<NP>(f, at ^ (m << 5), SM::PLANE, true);
+              mma_planes<NP, NP>(r[2 * m], r[2 * m + 1], a[d], f);
+            }
+          }
         }
+      };
+      const float ea = cg.end[ja], eb = cg.end[ja + 8], eba = cg.end_b[ja], ebb = cg.end_b[ja + 8];
+      {
+        float dv[F / 8][4];
+        gather(dv, as, tu);
+        // from the state's gradient behind the chunk
+        asm volatile("bar.sync 1, %0;" ::"n"(GB_THREADS) : "memory");
+#pragma unroll
+        for (int m = 0; m < KS; ++m) {
+          float c0[4] = {}, c1[4] = {};
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {  // (dv is a result of the inputs' type: bf16 takes the leading plane of dW)
+            Pk<NP> f[4];
+            ldsm_np<NP>(f, (tdw + 16 * k * TL::ROW + low) ^ (m << 5), TL::STATE_BYTES, true);
+            mma_planes<NP, NP>(c0, c1, k_[k], f);
+          }
+          add_rows(dv[2 * m], c0, eba, ebb);
+          add_rows(dv[2 * m + 1], c1, eba, ebb);
+        }
+        store_rows<T, F>(static_cast<T*>(p.dv) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dv, lane);
       }
-      store_rows<T, F>(static_cast<T*>(p.dk) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dk, lane);
-      sa = quad_sum(sa) * ta;
-      sb = quad_sum(sb) * tb;
+      F2 sa = f2(0.f), sb = f2(0.f);
+      {
+        float dk[F / 8][4];
+        gather(dk, av, tq);
+        Pk<NP> v_[KS][4];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) ldsm_np<NP>(v_[k], vq ^ (k << 5), SM::PLANE, false);
+#pragma unroll
+        for (int m = 0; m < KS; ++m) {
+          float c0[4] = {}, c1[4] = {};
+#pragma unroll
+          for (int k = 0; k < KS; ++k) {
+            Pk<NS> f[4];
+            ldsm_np<NS>(f, (tdw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
+            mma_planes<NP, NS>(c0, c1, v_[k], f);
+          }
+          // (an A fragment is two accumulator tiles)
+          sa = f2fma(make_float2(c0[0], c0[1]), make_float2(pk_lo(k_[m][0]), pk_hi(k_[m][0])), sa);
+          sb = f2fma(make_float2(c0[2], c0[3]), make_float2(pk_lo(k_[m][1]), pk_hi(k_[m][1])), sb);
+          sa = f2fma(make_float2(c1[0], c1[1]), make_float2(pk_lo(k_[m][2]), pk_hi(k_[m][2])), sa);
+          sb = f2fma(make_float2(c1[2], c1[3]), make_float2(pk_lo(k_[m][3]), pk_hi(k_[m][3])), sb);
+          add_rows(dk[2 * m], c0, eba, ebb);
+          add_rows(dk[2 * m + 1], c1, eba, ebb);
+        }
+        store_rows<T, F>(static_cast<T*>(p.dk) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dk, lane);
+      }
+      const float s0 = quad_sum(f2hsum(sa)) * ea, s1 = quad_sum(f2hsum(sb)) * eb;
       if (t4 == 0) {
-        cs.s[ja] = sa * ba;
-        cs.s[ja + 8] = sb * bb;
-        cs.c[ja] = ca * ba;
-        cs.c[ja + 8] = cb * bb;
+        cs.s[ja] = s0 * ba;
+        cs.s[ja + 8] = s1 * bb;
+        cs.c[ja] = na * wa;
+        cs.c[ja + 8] = nb * wb;
         if (p.dbeta != nullptr) {
           float* d = p.dbeta + (size_t)stream * p.T + t0;
-          if (ja < rows) d[ja] = na + sa;
-          if (ja + 8 < rows) d[ja + 8] = nb + sb;
+          if (ja < rows) d[ja] = fmaf(na, oa, own_a) + s0;
+          if (ja + 8 < rows) d[ja + 8] = fmaf(nb, ob, own_b) + s1;
         }
       }
     }
     if (ahead) make_chunk_gates(gates[(i + 1) & 1], lane, g_next, b_next);
-    ok = __syncthreads_and(ok);  // this chunk's tiles, states and sums are complete and free
-    if (!ok) return;
-    if (BF && tid == 0) {
-      if (i + 2 < n) fetch(i + 2, 0, 4);
+    if (!ok) *failed = 1;
+    block_sync();  // this chunk's tiles, states and sums are complete and free
+    if (*failed) return;
+    if (QUERIES && tid == 0) {
+      if (BF && i + 2 < n) fetch(i + 2, 0, 4);
       if (i + 1 < n) fetch_w(i + 1);
     }
-    if (tid >= GB_THREADS - 32) finish_gates(i);
+    if (!QUERIES && w == GATED_WARPS - 1) finish_gates(i);
   }
-  if (queries && seg == 0) store_state<F>(p.dw0 + (size_t)stream * F * F, dW, row0, col0, lane);
+  if constexpr (QUERIES) {
+    if (seg == 0) store_state<F>(p.dw0 + (size_t)stream * F * F, dW, row0, col0, lane);
+  }
+  };
+  if (queries) walk(std::true_type{});
+  else walk(std::false_type{});
 }
 
 template <typename T, int F>

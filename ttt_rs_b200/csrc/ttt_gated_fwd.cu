@@ -90,26 +90,13 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   auto publish = [&](int i) {  // the state before walk step i: operand of its q W, and what the backward reads back
     if constexpr (!STATE) {
       const uint32_t dst = base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES;
-      uint8_t* image = SAVE && i < n ? saved + (size_t)(c_lo + i) * F * F * 4 : nullptr;
-      if constexpr (BF && SAVE) {
-        float hi[SH::NT][4], lo[SH::NT][4];
-#pragma unroll
-        for (int k = 0; k < SH::NT; ++k)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            hi[k][e] = __bfloat162float(__float2bfloat16_rn(W[k][e]));
-            lo[k][e] = W[k][e] - hi[k][e];
-          }
-        put_state<F, 1>(hi, row0, col0, dst, image, lane);
-        if (image != nullptr) put_state<F, 1>(lo, row0, col0, 0, image + GTile<F>::STATE_BYTES, lane);
-      } else {
-        put_state<F, NP>(W, row0, col0, dst, nullptr, lane);
-        if (SAVE && image != nullptr) store_state<F>(reinterpret_cast<float*>(image), W, row0, col0, lane);
-      }
+      put_state<F, NP>(W, row0, col0, dst, lane);
+      if (SAVE && i < n) put_fragments<F>(reinterpret_cast<float4*>(saved + (size_t)(c_lo + i) * F * F * 4), W, w, lane);
     }
   };
   publish(0);
   __syncthreads();
+  const uint32_t low = GTile<F>::low(lane), high = GTile<F>::high(lane);
 
   for (int i = 0; i < n; ++i) {
     const int slot = BF ? i & 1 : 0, t0 = chunk_of(i) * GC;
@@ -137,10 +124,10 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     float o[STATE ? 1 : F / 8][4];
     Pk<NP> q[STATE ? 1 : KS][4];
     if constexpr (!STATE) {
-      // o = e^{G_i} q_i W
+      // q_i W, from the start of this warp's block on
       const uint32_t tw = base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES;
 #pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(q[k], tq + GTile<F>::a_mk(lane, 16 * w, 16 * k), SM::PLANE, false);
+      for (int k = 0; k < KS; ++k) ldsm_np<NP>(q[k], (tq + 16 * w * GTile<F>::ROW + low) ^ (k << 5), SM::PLANE, false);
 #pragma unroll
       for (int k = 0; k < F / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
 #pragma unroll
@@ -148,77 +135,70 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
 #pragma unroll
         for (int m = 0; m < KS; ++m) {
           Pk<NP> f[4];
-          ldsm_np<NP>(f, tw + GTile<F>::b_kn(lane, 16 * m, 16 * k), GTile<F>::STATE_BYTES, true);
+          ldsm_np<NP>(f, (tw + 16 * k * GTile<F>::ROW + low) ^ (m << 5), GTile<F>::STATE_BYTES, true);
           mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], q[k], f);
         }
-      const float fa = cg.from[16 * w + g], fb = cg.from[16 * w + g + 8];
+      const float first = cg.starts[w];
 #pragma unroll
-      for (int k = 0; k < F / 8; ++k) {
-        o[k][0] *= fa;
-        o[k][1] *= fa;
-        o[k][2] *= fb;
-        o[k][3] *= fb;
-      }
+      for (int k = 0; k < F / 8; ++k) scale_rows(o[k], first, first);
     }
     const float all = cg.all;
     total *= all;
 #pragma unroll
-    for (int k = 0; k < SH::NT; ++k)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) W[k][e] *= all;
+    for (int k = 0; k < SH::NT; ++k) scale_rows(W[k], all, all);
 
-#pragma unroll
+#pragma unroll 1
     for (int jt = 0; jt < GC / 16; ++jt) {
-      // queries of this warp against the keys of tokens 16 jt .. 16 jt + 15, decayed; an operand of the inputs' planes
+      const int j0 = 16 * jt + 2 * t4;
+      // queries of this warp against the keys of the block, decayed, as an operand of the inputs' planes
       Pk<NP> a[4];
       const bool here = !STATE && jt <= w;
-      if (!STATE && here) {
-        float s0[4] = {}, s1[4] = {};
+      if constexpr (!STATE) {
+        if (here) {
+          float s0[4] = {}, s1[4] = {};
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          Pk<NP> f[4];
-          ldsm_np<NP>(f, tk + GTile<F>::b_nk(lane, 16 * jt, 16 * k), SM::PLANE, false);
-          mma_planes<NP, NP>(s0, s1, q[STATE ? 0 : k], f);
-        }
-        const int ia = 16 * w + g, j0 = 16 * jt + 2 * t4;
-        const float ha = cg.hi[ia], la = cg.lo[ia], hb = cg.hi[ia + 8], lb = cg.lo[ia + 8];
+          for (int k = 0; k < KS; ++k) {
+            Pk<NP> f[4];
+            ldsm_np<NP>(f, (tk + 16 * jt * GTile<F>::ROW + high) ^ (k << 5), SM::PLANE, false);
+            mma_planes<NP, NP>(s0, s1, q[k], f);
+          }
+          if (jt < w) {
+            const F2 between = f2(cg.blocks[jt][w - 1]);
+            scale_cols(s0, f2mul(ld2(&cg.out_b[j0]), between));
+            scale_cols(s1, f2mul(ld2(&cg.out_b[j0 + 8]), between));
+          } else {
+            // what came from before the block, to each of its tokens; then the block itself
+            const float ra = cg.into[16 * w + g], rb = cg.into[16 * w + g + 8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // columns j0, j0 + 1, j0 + 8, j0 + 9
-          const int j = j0 + (e & 1) + 8 * (e >> 1);
-          const float hj = cg.hi[j], lj = cg.lo[j], bj = cg.beta[j];
-          float* s = e < 2 ? s0 : s1;
-          const float da = j <= ia ? exp2f((ha - hj) + (la - lj)) * bj : 0.f;
-          const float db = j <= ia + 8 ? exp2f((hb - hj) + (lb - lj)) * bj : 0.f;
-          s[e & 1] = j <= ia ? s[e & 1] * da : 0.f;
-          s[2 + (e & 1)] = j <= ia + 8 ? s[2 + (e & 1)] * db : 0.f;
+            for (int k = 0; k < F / 8; ++k) scale_rows(o[k], ra, rb);
+            float d[2][4];
+            block_decays<true>(d, cg, w, g, t4);
+            const float2 b0 = ld2(&cg.beta[j0]), b1 = ld2(&cg.beta[j0 + 8]);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {  // (a select, not a product: what is not there may be infinite)
+              s0[2 * half] = d[half][0] > 0.f ? s0[2 * half] * (d[half][0] * b0.x) : 0.f;
+              s0[2 * half + 1] = d[half][1] > 0.f ? s0[2 * half + 1] * (d[half][1] * b0.y) : 0.f;
+              s1[2 * half] = d[half][2] > 0.f ? s1[2 * half] * (d[half][2] * b1.x) : 0.f;
+              s1[2 * half + 1] = d[half][3] > 0.f ? s1[2 * half + 1] * (d[half][3] * b1.y) : 0.f;
+            }
+          }
+          as_operand<NP>(a, s0, s1);
         }
-        a[0] = split_pack<NP>(s0[0], s0[1]);
-        a[1] = split_pack<NP>(s0[2], s0[3]);
-        a[2] = split_pack<NP>(s1[0], s1[1]);
-        a[3] = split_pack<NP>(s1[2], s1[3]);
       }
-      // keys of these tokens, transposed: rows of the state
+      // keys of the block, transposed: rows of the state
       Pk<NS> kt[4];
       {
         Pk<NP> f[4];
-        ldsm_np<NP>(f, tk + GTile<F>::a_km(lane, row0, 16 * jt), SM::PLANE, true);
-        const int j0 = 16 * jt + 2 * t4;
-        float2 lo, hi;
-        if constexpr (REV) {  // (the gradient's walk: what is left at the token of the state before the chunk)
-          lo = *reinterpret_cast<const float2*>(&cg.from[j0]);
-          hi = *reinterpret_cast<const float2*>(&cg.from[j0 + 8]);
-        } else {
-          lo = f2mul(*reinterpret_cast<const float2*>(&cg.to[j0]), *reinterpret_cast<const float2*>(&cg.beta[j0]));
-          hi = f2mul(*reinterpret_cast<const float2*>(&cg.to[j0 + 8]), *reinterpret_cast<const float2*>(&cg.beta[j0 + 8]));
-        }
-        scale_a_cols<NS, NP>(kt, f, lo, hi);
+        ldsm_np<NP>(f, (tk + 16 * jt * GTile<F>::ROW + high) ^ (row0 << 1), SM::PLANE, true);
+        const float* scale = REV ? cg.from : cg.end_b;  // (REV: what is left at the token of the state before the chunk)
+        scale_a_cols<NS, NP>(kt, f, ld2(scale + j0), ld2(scale + j0 + 8));
       }
 #pragma unroll
       for (int m = 0; m < KS; ++m) {
         const bool mine = SH::PARTS == 1 || m == part;
         if (!mine && !here) continue;
         Pk<NP> f[4];
-        ldsm_np<NP>(f, tv + GTile<F>::b_kn(lane, 16 * m, 16 * jt), SM::PLANE, true);
+        ldsm_np<NP>(f, (tv + 16 * jt * GTile<F>::ROW + low) ^ (m << 5), SM::PLANE, true);
         if constexpr (!STATE) {
           if (here) mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], a, f);
         }

@@ -214,6 +214,62 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
 #pragma unroll
       for (int k = 0; k < F / 8; ++k) dq[k][0] = dq[k][1] = dq[k][2] = dq[k][3] = 0.f;
       const uint32_t uq = tu + 16 * w * TL::ROW + low;
+      // from the state before the chunk: this thread's share as it was saved, for the ways that cross the whole chunk, and its
+      // planes as an operand for all four warps
+      const float all = cg.all;
+      if (!mbar_wait_bounded(bar_w, i & 1)) {
+        if (tid == 0) report_timeout(p.status, 22, (uint32_t)i);
+        ok = false;
+      }
+      {
+        float W[SH::NT][4];
+        get_fragments<F>(W, reinterpret_cast<const float4*>(mem + SM::WSAVED), w, lane);
+        F2 cross = f2(0.f);
+#pragma unroll
+        for (int k = 0; k < SH::NT; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) cross = f2fma(pr(W[k], half), pr(dW[k], half), cross);
+        float through = f2hsum(cross);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) through += __shfl_xor_sync(0xffffffffu, through, o);
+        if (lane == 0) cs.through[w] = through * all;
+        asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+        put_state<F, NS>(W, row0, col0, tw, lane);
+        asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+      }
+      // W u, for r and, from the start of this warp's block on, for dq
+      Pk<NP> u[KS][4];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        ldsm_np<NP>(u[k], uq ^ (k << 5), SM::PLANE, false);
+#pragma unroll
+        for (int m = 0; m < KS; ++m) {
+          Pk<NS> f[4];
+          ldsm_np<NS>(f, (tw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
+          mma_planes<NP, NS>(dq[2 * m], dq[2 * m + 1], u[k], f);
+        }
+      }
+      asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+      if (tid == 0 && i + 1 < n) fetch_w(i + 1);
+      F2 sa = f2(0.f), sb = f2(0.f);
+#pragma unroll
+      for (int m = 0; m < KS; ++m) {  // (an A fragment is two accumulator tiles)
+        Pk<NP> q[4];
+        ldsm_np<NP>(q, (tq + 16 * w * TL::ROW + low) ^ (m << 5), SM::PLANE, false);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          sa = f2fma(pr(dq[2 * m + e], 0), make_float2(pk_lo(q[2 * e]), pk_hi(q[2 * e])), sa);
+          sb = f2fma(pr(dq[2 * m + e], 1), make_float2(pk_lo(q[2 * e + 1]), pk_hi(q[2 * e + 1])), sb);
+        }
+      }
+      const float r0 = quad_sum(f2hsum(sa)) * cg.from[ia], r1 = quad_sum(f2hsum(sb)) * cg.from[ia + 8];
+      if (t4 == 0) {
+        cs.r[ia] = r0;
+        cs.r[ia + 8] = r1;
+      }
+      const float first = cg.starts[w];
+#pragma unroll
+      for (int k = 0; k < F / 8; ++k) scale_rows(dq[k], first, first);
       // inside the chunk: the blocks before this warp's, then its own
       const float ra = cg.into[ia], rb = cg.into[ia + 8];
 #pragma unroll 1
@@ -221,10 +277,9 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         float s0[4] = {}, s1[4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          Pk<NP> u[4], f[4];
-          ldsm_np<NP>(u, uq ^ (k << 5), SM::PLANE, false);
+          Pk<NP> f[4];
           ldsm_np<NP>(f, (tv + 16 * jt * TL::ROW + high) ^ (k << 5), SM::PLANE, false);
-          mma_planes<NP, NP>(s0, s1, u, f);
+          mma_planes<NP, NP>(s0, s1, u[k], f);
         }
         const int j0 = 16 * jt + 2 * t4;
         if (jt < w) {
@@ -253,57 +308,6 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
           ldsm_np<NP>(f, (tk + 16 * jt * TL::ROW + low) ^ (m << 5), SM::PLANE, true);
           mma_planes<NP, NP>(dq[2 * m], dq[2 * m + 1], a, f);
         }
-      }
-      // from the state before the chunk: this thread's share as it was saved, for the ways that cross the whole chunk, and its
-      // planes as an operand for all four warps
-      const float all = cg.all;
-      if (!mbar_wait_bounded(bar_w, i & 1)) {
-        if (tid == 0) report_timeout(p.status, 22, (uint32_t)i);
-        ok = false;
-      }
-      {
-        float W[SH::NT][4];
-        get_fragments<F>(W, reinterpret_cast<const float4*>(mem + SM::WSAVED), w, lane);
-        F2 cross = f2(0.f);
-#pragma unroll
-        for (int k = 0; k < SH::NT; ++k)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) cross = f2fma(pr(W[k], half), pr(dW[k], half), cross);
-        float through = f2hsum(cross);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) through += __shfl_xor_sync(0xffffffffu, through, o);
-        if (lane == 0) cs.through[w] = through * all;
-        asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
-        put_state<F, NS>(W, row0, col0, tw, lane);
-        asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
-      }
-      Pk<NP> u[KS][4];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(u[k], uq ^ (k << 5), SM::PLANE, false);
-      const float fa = cg.from[ia], fb = cg.from[ia + 8];
-      F2 sa = f2(0.f), sb = f2(0.f);
-#pragma unroll
-      for (int m = 0; m < KS; ++m) {
-        float c0[4] = {}, c1[4] = {};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          Pk<NS> f[4];
-          ldsm_np<NS>(f, (tw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
-          mma_planes<NP, NS>(c0, c1, u[k], f);
-        }
-        Pk<NP> q[4];
-        ldsm_np<NP>(q, (tq + 16 * w * TL::ROW + low) ^ (m << 5), SM::PLANE, false);  // (an A fragment is two accumulator tiles)
-        sa = f2fma(make_float2(c0[0], c0[1]), make_float2(pk_lo(q[0]), pk_hi(q[0])), sa);
-        sb = f2fma(make_float2(c0[2], c0[3]), make_float2(pk_lo(q[1]), pk_hi(q[1])), sb);
-        sa = f2fma(make_float2(c1[0], c1[1]), make_float2(pk_lo(q[2]), pk_hi(q[2])), sa);
-        sb = f2fma(make_float2(c1[2], c1[3]), make_float2(pk_lo(q[3]), pk_hi(q[3])), sb);
-        add_rows(dq[2 * m], c0, fa, fb);
-        add_rows(dq[2 * m + 1], c1, fa, fb);
-      }
-      const float r0 = quad_sum(f2hsum(sa)) * fa, r1 = quad_sum(f2hsum(sb)) * fb;
-      if (t4 == 0) {
-        cs.r[ia] = r0;
-        cs.r[ia + 8] = r1;
       }
       store_rows<T, F>(static_cast<T*>(p.dq) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dq, lane);
       // dW before the chunk
@@ -437,10 +441,12 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       nb = quad_sum(nb);
       own_a = quad_sum(own_a);
       own_b = quad_sum(own_b);
-      // rows of sum over the blocks of operand . tile: the blocks behind, what is left of the row behind its own block, the own one
+      // adds to rows that hold what comes from behind the chunk: up to the end of this block, the sums over the blocks behind of
+      // operand . tile; what is left of the row's token there; the own block
       auto gather = [&](float (&r)[F / 8][4], const Pk<NP> (&a)[4][4], uint32_t tile) {
+        const float last = cg.blocks[w][3];
 #pragma unroll
-        for (int k = 0; k < F / 8; ++k) r[k][0] = r[k][1] = r[k][2] = r[k][3] = 0.f;
+        for (int k = 0; k < F / 8; ++k) scale_rows(r[k], last, last);
 #pragma unroll
         for (int d = 3; d >= 0; --d) {
           if (d == 0) {
@@ -458,52 +464,49 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
           }
         }
       };
-      const float ea = cg.end[ja], eb = cg.end[ja + 8], eba = cg.end_b[ja], ebb = cg.end_b[ja + 8];
+      asm volatile("bar.sync 1, %0;" ::"n"(GB_THREADS) : "memory");
       {
         float dv[F / 8][4];
-        gather(dv, as, tu);
-        // from the state's gradient behind the chunk
-        asm volatile("bar.sync 1, %0;" ::"n"(GB_THREADS) : "memory");
 #pragma unroll
-        for (int m = 0; m < KS; ++m) {
-          float c0[4] = {}, c1[4] = {};
+        for (int k = 0; k < F / 8; ++k) dv[k][0] = dv[k][1] = dv[k][2] = dv[k][3] = 0.f;
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {  // (dv is a result of the inputs' type: bf16 takes the leading plane of dW)
+        for (int k = 0; k < KS; ++k)  // (dv is a result of the inputs' type: bf16 takes the leading plane of dW)
+#pragma unroll
+          for (int m = 0; m < KS; ++m) {
             Pk<NP> f[4];
             ldsm_np<NP>(f, (tdw + 16 * k * TL::ROW + low) ^ (m << 5), TL::STATE_BYTES, true);
-            mma_planes<NP, NP>(c0, c1, k_[k], f);
+            mma_planes<NP, NP>(dv[2 * m], dv[2 * m + 1], k_[k], f);
           }
-          add_rows(dv[2 * m], c0, eba, ebb);
-          add_rows(dv[2 * m + 1], c1, eba, ebb);
-        }
+        gather(dv, as, tu);
         store_rows<T, F>(static_cast<T*>(p.dv) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dv, lane);
       }
       F2 sa = f2(0.f), sb = f2(0.f);
       {
         float dk[F / 8][4];
-        gather(dk, av, tq);
-        Pk<NP> v_[KS][4];
 #pragma unroll
-        for (int k = 0; k < KS; ++k) ldsm_np<NP>(v_[k], vq ^ (k << 5), SM::PLANE, false);
+        for (int k = 0; k < F / 8; ++k) dk[k][0] = dk[k][1] = dk[k][2] = dk[k][3] = 0.f;
 #pragma unroll
-        for (int m = 0; m < KS; ++m) {
-          float c0[4] = {}, c1[4] = {};
+        for (int k = 0; k < KS; ++k) {
+          Pk<NP> v[4];
+          ldsm_np<NP>(v, vq ^ (k << 5), SM::PLANE, false);
 #pragma unroll
-          for (int k = 0; k < KS; ++k) {
+          for (int m = 0; m < KS; ++m) {
             Pk<NS> f[4];
             ldsm_np<NS>(f, (tdw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
-            mma_planes<NP, NS>(c0, c1, v_[k], f);
+            mma_planes<NP, NS>(dk[2 * m], dk[2 * m + 1], v, f);
           }
-          // (an A fragment is two accumulator tiles)
-          sa = f2fma(make_float2(c0[0], c0[1]), make_float2(pk_lo(k_[m][0]), pk_hi(k_[m][0])), sa);
-          sb = f2fma(make_float2(c0[2], c0[3]), make_float2(pk_lo(k_[m][1]), pk_hi(k_[m][1])), sb);
-          sa = f2fma(make_float2(c1[0], c1[1]), make_float2(pk_lo(k_[m][2]), pk_hi(k_[m][2])), sa);
-          sb = f2fma(make_float2(c1[2], c1[3]), make_float2(pk_lo(k_[m][3]), pk_hi(k_[m][3])), sb);
-          add_rows(dk[2 * m], c0, eba, ebb);
-          add_rows(dk[2 * m + 1], c1, eba, ebb);
         }
+#pragma unroll
+        for (int m = 0; m < KS; ++m)  // (an A fragment is two accumulator tiles)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sa = f2fma(pr(dk[2 * m + e], 0), make_float2(pk_lo(k_[m][2 * e]), pk_hi(k_[m][2 * e])), sa);
+            sb = f2fma(pr(dk[2 * m + e], 1), make_float2(pk_lo(k_[m][2 * e + 1]), pk_hi(k_[m][2 * e + 1])), sb);
+          }
+        gather(dk, av, tq);
         store_rows<T, F>(static_cast<T*>(p.dk) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dk, lane);
       }
+      const float ea = cg.end[ja], eb = cg.end[ja + 8];
       const float s0 = quad_sum(f2hsum(sa)) * ea, s1 = quad_sum(f2hsum(sb)) * eb;
       if (t4 == 0) {
         cs.s[ja] = s0 * ba;
@@ -523,7 +526,6 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     if (*failed) return;
     if (QUERIES && tid == 0) {
       if (BF && i + 2 < n) fetch(i + 2, 0, 4);
-      if (i + 1 < n) fetch_w(i + 1);
     }
     if (!QUERIES && w == GATED_WARPS - 1) finish_gates(i);
   }

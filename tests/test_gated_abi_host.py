@@ -37,7 +37,9 @@ def test_sizes(lib):
     assert lib.ttt_linear_gated_saved_bytes(C.byref(dims(head_dim=32, seq_len=64))) == 6 * 32 * 32 * 4
     many = dims(batch=32, heads=12, seq_len=2048)
     assert lib.ttt_linear_gated_forward_workspace_bytes(C.byref(many)) == 0
-    assert lib.ttt_linear_gated_backward_workspace_bytes(C.byref(many)) == 0
+    # more streams than blocks are resident: a state and a flag per range, and the counter
+    assert lib.ttt_linear_gated_backward_workspace_bytes(C.byref(many)) == 296 * (64 * 64 + 1) * 4 + 4
+    assert lib.ttt_linear_gated_backward_workspace_bytes(C.byref(dims(batch=16, heads=16, seq_len=2048))) == 0
     few = lib.ttt_linear_gated_forward_workspace_bytes(C.byref(dims(batch=1, heads=1, seq_len=8192)))
     assert few > 0 and few % (64 * 64 * 4 + 4) == 0  # a state and a decay per segment
     for bad in (dict(head_dim=48), dict(batch=0), dict(seq_len=0), dict(dtype=3)):

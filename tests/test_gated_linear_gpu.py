@@ -122,6 +122,19 @@ def test_few_streams_in_segments(T):
         assert all(torch.equal(x[0], x[i]) for i in (1, 77, 159))
 
 
+@pytest.mark.parametrize("B,H,T,F,dtype", [(41, 11, 200, 64, torch.bfloat16), (30, 10, 65, 32, torch.bfloat16), (17, 9, 130, 64, torch.float32),
+                                           (149, 1, 10, 32, torch.float32), (99, 9, 70, 64, torch.bfloat16)])
+def test_more_streams_than_resident_blocks(B, H, T, F, dtype):
+    """Streams cut into ranges, a stream's state handed from one block to the next."""
+    ins, d_out, d_w = make(B, H, T, F, dtype, seed=B)
+    args = (*f64(ins), d_out.double(), d_w.double())
+    want, mag = O.gated_grads(*args), O.gated_magnitudes(*args)
+    got = run(ins, d_out, d_w)
+    check(got, want, mag, dtype)
+    check(run(ins)[:2], want, mag, dtype)
+    assert all(torch.equal(x, y) for x, y in zip(got, run(ins, d_out, d_w)))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strided_inputs(dtype):
     """[B,T,H,F] turned, columns of a projection, rows that cannot be read in place, expanded gradients."""

@@ -1285,20 +1285,22 @@ int make_gated_map(CUtensorMap* m, const void* base, const ttt_dims* d, const in
   return TTT_OK;
 }
 
-// How a call's streams are cut: segments per stream, chunks per segment
+// How a call's streams are cut: segments per stream, chunks per segment; ranges
 struct GatedCut {
-  int chunks, nseg, seg_chunks;
-  size_t state_floats, total_bytes;  // workspace: a state per segment, then a decay per segment
+  int chunks, nseg, seg_chunks, slots;
+  size_t state_floats, total_bytes;  // workspace: a state per segment (or range), then a decay per segment (flag per range, counter)
 };
 GatedCut gated_cut(const ttt_dims* d, bool backward) {
   GatedCut c;
   c.chunks = (d->seq_len + kGatedChunk - 1) / kGatedChunk;
   const int64_t streams = (int64_t)d->batch * d->heads;
-  c.nseg = ttt::gated_segments(streams, c.chunks, backward);
+  ttt::gated_split(streams, c.chunks, d->dtype, backward, &c.nseg, &c.slots);
   c.seg_chunks = (c.chunks + c.nseg - 1) / c.nseg;
   c.nseg = (c.chunks + c.seg_chunks - 1) / c.seg_chunks;
-  c.state_floats = c.nseg > 1 ? (size_t)streams * c.nseg * d->head_dim * d->head_dim : 0;
-  c.total_bytes = c.nseg > 1 ? (c.state_floats + (size_t)streams * c.nseg) * sizeof(float) : 0;
+  const size_t state = (size_t)d->head_dim * d->head_dim, segments = (size_t)streams * c.nseg;
+  c.state_floats = c.nseg > 1 ? segments * state : c.slots * state;
+  c.total_bytes = c.nseg > 1 ? (c.state_floats + segments) * sizeof(float)
+                  : c.slots > 0 ? (c.state_floats + c.slots + 1) * sizeof(float) : 0;
   return c;
 }
 int check_gated_workspace(const GatedCut& c, const void* workspace, size_t bytes) {
@@ -1370,6 +1372,9 @@ extern "C" int ttt_linear_gated_forward(const ttt_dims* d, const void* xq, const
   p.nstreams = d->batch * d->heads;
   p.nseg = cut.nseg;
   p.seg_chunks = cut.seg_chunks;
+  p.slots = cut.slots;
+  p.records = p.seg_state;
+  p.flags = reinterpret_cast<int*>(p.seg_decay);
   const cudaError_t e = ttt::launch_gated_fwd(d->dtype, d->head_dim, maps, p, saved != nullptr, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated forward launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;
@@ -1447,6 +1452,9 @@ extern "C" int ttt_linear_gated_backward(const ttt_dims* d, const void* xq, cons
   p.nstreams = d->batch * d->heads;
   p.nseg = cut.nseg;
   p.seg_chunks = cut.seg_chunks;
+  p.slots = cut.slots;
+  p.records = seg;
+  p.flags = reinterpret_cast<int*>(seg + cut.state_floats);
   const cudaError_t e = ttt::launch_gated_bwd(d->dtype, d->head_dim, maps, p, st);
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated backward launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;

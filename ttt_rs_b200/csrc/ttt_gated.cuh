@@ -277,6 +277,84 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
       : "memory");
 }
 
+// What a block walks: steps of one chunk each.  A stream's chunks are numbered in walk order (`pos`; the backward walks from the
+// last chunk).  With p.slots = 0 a block has one segment of one stream.  Else (more streams than blocks are resident) all steps
+// of all streams, stream after stream, are cut into p.slots equal ranges, of at least a stream's length each: a block's range is
+// the end of one stream, whole streams, and the beginning of another.  It begins with that beginning, whose state it hands on
+// to the block of the next range, and ends with the end of the first stream, whose state it gets from the block of the range before:
+// by then that block is long past it.  Ranges are numbered in the order in which blocks start, so that what a block waits for
+// has always started.
+struct GatedWalk {
+  int slot, n;            // range; steps
+  int head, head_n;       // stream and steps of the beginning
+  int mid, mid_n;         // first whole stream, steps of all of them
+  int tail, tail_pos;     // stream and first chunk of the end
+  int NC;
+  struct Step {
+    int i, stream, pos;
+    bool starts, ends;  // a stream or a part of one starts, ends with this step
+  };
+  template <class P>
+  __device__ __forceinline__ void set(const P& p, int slot_, bool rev) {
+    slot = slot_;
+    NC = p.NC;
+    head = mid = tail = head_n = mid_n = tail_pos = 0;
+    if (p.slots == 0) {
+      tail = slot / p.nseg;
+      const int seg = slot - tail * p.nseg, lo = seg * p.seg_chunks, hi = min(NC, lo + p.seg_chunks);
+      tail_pos = rev ? NC - hi : lo;
+      n = hi - lo;
+      return;
+    }
+    const long long total = (long long)p.nstreams * NC;
+    const long long a = total * slot / p.slots, b = total * (slot + 1) / p.slots;
+    const int sa = (int)(a / NC), pa = (int)(a - (long long)sa * NC), sb = (int)(b / NC), pb = (int)(b - (long long)sb * NC);
+    n = (int)(b - a);
+    tail = sa;
+    tail_pos = pa;
+    head = sb;
+    head_n = pb;
+    mid = pa > 0 ? sa + 1 : sa;
+    mid_n = (sb - mid) * NC;
+  }
+  __device__ __forceinline__ Step part(int i) const {  // the step that a part starts with
+    Step s;
+    s.i = i;
+    s.starts = true;
+    s.stream = i < head_n ? head : tail;
+    s.pos = i < head_n ? 0 : tail_pos;
+    if (i >= head_n && i < head_n + mid_n) {
+      s.stream = mid + (i - head_n) / NC;
+      s.pos = 0;
+    }
+    s.ends = last(s);
+    return s;
+  }
+  __device__ __forceinline__ bool last(const Step& s) const { return s.pos + 1 == NC || s.i + 1 == head_n || s.i + 1 == n; }
+  __device__ __forceinline__ Step next(const Step& s) const {  // (behind the last step: one that is not used)
+    if (s.ends) return part(s.i + 1);
+    Step t = s;
+    ++t.i;
+    ++t.pos;
+    t.starts = false;
+    t.ends = last(t);
+    return t;
+  }
+};
+// One thread: the record of range `slot` has been handed on (false: the wait ran out)
+__device__ __forceinline__ bool wait_record(const int* flags, int slot) {
+  for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(flags + slot) : "memory");
+    if (v != 0) return true;
+    __nanosleep(100);
+  }
+  return false;
+}
+__device__ __forceinline__ void set_record(int* flags, int slot) {
+  asm volatile("st.release.gpu.global.s32 [%0], %1;" ::"l"(flags + slot), "r"(1) : "memory");
+}
+
 // How the F x F state lies in the registers of four warps: warp w holds rows 16 (w % SLABS).. and the columns of its part
 template <int F>
 struct StateShare {

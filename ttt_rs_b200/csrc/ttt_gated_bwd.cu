@@ -49,7 +49,7 @@ struct GatedBwdSmem {
   static constexpr uint32_t W = BF ? WSAVED : WSAVED + WRAW, DW = W + STATE;
   static constexpr uint32_t GATES = DW + STATE;
   static constexpr uint32_t SUMS = GATES + 2 * sizeof(ChunkGates);
-  static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 32 + 1024;  // (BAR + 24: a wait has run out)
+  static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 32 + 1024;  
   static_assert(!BF || STATE == WRAW, "two planes of bf16 are as long as the float32 state");
 };
 
@@ -66,54 +66,63 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   uint8_t* const mem = gated_smem + (base - raw);
   const int tid = threadIdx.x, lane = tid & 31, w = (tid >> 5) & 3, g = lane >> 2, t4 = lane & 3;
   const bool queries = tid < GB_THREADS / 2;
-  const int stream = blockIdx.x / p.nseg, seg = blockIdx.x - stream * p.nseg;
-  const int c_lo = seg * p.seg_chunks, c_hi = min(p.NC, c_lo + p.seg_chunks), n = c_hi - c_lo;
-  const int h = stream % p.H, b = stream / p.H;
   const uint32_t bar = base + SM::BAR, bar_w = bar + 16;
+  volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 24);  // a wait has run out; this block's range
   if (tid == 0) {
+    shared[0] = 0;
+    shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
     mbar_init(bar, 1);
     mbar_init(bar + 8, 1);
     mbar_init(bar_w, 1);
     fence_mbar_init();
   }
   __syncthreads();
-  auto chunk_of = [&](int i) { return c_hi - 1 - i; };
+  GatedWalk walk_{};
+  walk_.set(p, shared[1], true);
+  const int n = walk_.n;
+  const GatedWalk::Step first = walk_.part(0);
+  auto chunk_of = [&](const GatedWalk::Step& s) { return p.NC - 1 - s.pos; };
   // thread 0.  bf16: q, k, v, u of a chunk; float32: two of them at a time, through the same rows of shared memory
-  auto fetch = [&](int i, int first, int count) {
+  auto fetch = [&](const GatedWalk::Step& s, int first, int count) {
+    const int i = s.i;
     const int slot = BF ? i & 1 : 0;
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * 4 * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
     mbar_expect_tx(at, count * bytes);
-    for (int m = 0; m < count; ++m) tma_load_4d(dst + m * bytes, &maps.m[first + m], chunk_of(i) * GC, h, b, at);
+    const int b = s.stream / p.H, h = s.stream - b * p.H;
+    for (int m = 0; m < count; ++m) tma_load_4d(dst + m * bytes, &maps.m[first + m], chunk_of(s) * GC, h, b, at);
   };
-  const uint8_t* saved = p.saved + (size_t)stream * p.NC * SM::WRAW;
-  auto fetch_w = [&](int i) {
+  auto fetch_w = [&](const GatedWalk::Step& s) {
     mbar_expect_tx(bar_w, SM::WRAW);
-    bulk_load_1d(base + SM::WSAVED, saved + (size_t)chunk_of(i) * SM::WRAW, SM::WRAW, bar_w);
+    bulk_load_1d(base + SM::WSAVED, p.saved + ((size_t)s.stream * p.NC + chunk_of(s)) * SM::WRAW, SM::WRAW, bar_w);
   };
   if (tid == 0) {
-    fetch(0, 0, BF ? 4 : 2);
-    if (BF && n > 1) fetch(1, 0, 4);
-    fetch_w(0);
+    fetch(first, 0, BF ? 4 : 2);
+    if (BF && n > 1) fetch(walk_.next(first), 0, 4);
+    fetch_w(first);
   }
-  const float* gp = p.g + (size_t)stream * p.T;
-  const float* bp = p.beta != nullptr ? p.beta + (size_t)stream * p.T : nullptr;
+  auto gates_of = [&](const GatedWalk::Step& s, float2& g, float2& beta) {
+    const size_t row = (size_t)s.stream * p.T;
+    g = load_gates(p.g + row, chunk_of(s) * GC, p.T, lane, 0.f);
+    beta = load_gates(p.beta != nullptr ? p.beta + row : nullptr, chunk_of(s) * GC, p.T, lane, 1.f);
+  };
   ChunkGates* const gates = reinterpret_cast<ChunkGates*>(mem + SM::GATES);
   ChunkSums* const sums = reinterpret_cast<ChunkSums*>(mem + SM::SUMS);
   if (tid < 32) {
-    const int t0 = chunk_of(0) * GC;
-    make_chunk_gates(gates[0], lane, load_gates(gp, t0, p.T, lane, 0.f), load_gates(bp, t0, p.T, lane, 1.f));
+    float2 g0, b0;
+    gates_of(first, g0, b0);
+    make_chunk_gates(gates[0], lane, g0, b0);
   }
   const int row0 = 16 * (w % SH::SLABS), part = w / SH::SLABS, col0 = part * SH::COLS;
-  volatile int* const failed = reinterpret_cast<volatile int*>(mem + SM::BAR + 24);
-  if (tid == 0) *failed = 0;
   __syncthreads();
 
   const uint32_t low = TL::low(lane), high = TL::high(lane);
   // the gradients of the gates of walk step i, from the sums its warps left (one warp)
-  auto finish_gates = [&](int i) {
+  auto finish_gates = [&](const GatedWalk::Step& st) {
+    const int i = st.i;
     const ChunkSums& cs = sums[i & 1];
-    const int t0 = chunk_of(i) * GC, a = 2 * lane;
+    const size_t row = (size_t)st.stream * p.T;
+    const int t0 = chunk_of(st) * GC, a = 2 * lane;
     const float through = (cs.through[0] + cs.through[1]) + (cs.through[2] + cs.through[3]);
     const int blk = lane >> 3;
     float x[2], far1 = 0.f, far2 = 0.f;
@@ -159,7 +168,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int t = t0 + a + e;
-      if (t < p.T) p.dg[(size_t)stream * p.T + t] = expf(gp[t]) == 0.f ? 0.f : d[e];
+      if (t < p.T) p.dg[row + t] = expf(p.g[row + t]) == 0.f ? 0.f : d[e];
     }
   };
 
@@ -167,19 +176,33 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   auto walk = [&](auto group) {
   constexpr bool QUERIES = decltype(group)::value;
   float dW[QUERIES ? SH::NT : 1][4];
-  if constexpr (QUERIES) {
-    const float* d0 = seg < p.nseg - 1 ? p.seg_state + ((size_t)stream * p.nseg + seg) * F * F
-                      : p.dw_out != nullptr ? p.dw_out + (size_t)stream * F * F : nullptr;
-    load_state<F>(dW, d0, row0, col0, lane);
-  }
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) {
-    const int slot = BF ? i & 1 : 0, t0 = chunk_of(i) * GC, rows = p.T - t0;
+  for (GatedWalk::Step st = first, nx; st.i < n; st = nx) {
+    nx = walk_.next(st);
+    const int i = st.i;
+    const int stream = st.stream;
+    const int slot = BF ? i & 1 : 0, t0 = chunk_of(st) * GC, rows = p.T - t0;
     const bool ahead = QUERIES && w == 0 && i + 1 < n;
     float2 g_next, b_next;
-    if (ahead) {
-      g_next = load_gates(gp, chunk_of(i + 1) * GC, p.T, lane, 0.f);
-      b_next = load_gates(bp, chunk_of(i + 1) * GC, p.T, lane, 1.f);
+    if (ahead) gates_of(nx, g_next, b_next);
+    bool ok = true;
+    if constexpr (QUERIES) {
+      if (st.starts) {  // the gradient of the state behind this stream, or behind this part of it
+        const float* d0 = p.dw_out != nullptr ? p.dw_out + (size_t)stream * F * F : nullptr;
+        if (st.pos > 0) {
+          if (p.slots > 0) {
+            if (tid == 0 && !wait_record(p.flags, walk_.slot - 1)) {
+              report_timeout(p.status, 23, (uint32_t)i);
+              ok = false;
+            }
+            asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+            d0 = p.records + (size_t)(walk_.slot - 1) * F * F;
+          } else {
+            d0 = p.seg_state + (size_t)walk_.slot * F * F;
+          }
+        }
+        load_state<F>(dW, d0, row0, col0, lane);
+      }
     }
     const uint32_t tiles = base + SM::TILES + slot * 4 * SM::TILE;
     const uint32_t tq = tiles, tk = tq + SM::TILE, tv = tk + SM::TILE, tu = tv + SM::TILE;
@@ -190,7 +213,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       put_state<F, NS>(dW, row0, col0, tdw, lane);
       asm volatile("bar.arrive 1, %0;" ::"n"(GB_THREADS) : "memory");
     }
-    bool ok = mbar_wait_bounded(bar + 8 * slot, BF ? (i >> 1) & 1 : 0);
+    bool arrived = mbar_wait_bounded(bar + 8 * slot, BF ? (i >> 1) & 1 : 0);
     if constexpr (!BF) {
       auto split2 = [&](uint32_t dst) {
         for (int m = 0; m < 2; ++m)
@@ -198,13 +221,13 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       };
       split2(tq);
       block_sync();
-      if (tid == 0 && ok) fetch(i, 2, 2);
-      ok = ok && mbar_wait_bounded(bar, 1);
+      if (tid == 0 && arrived) fetch(st, 2, 2);
+      arrived = arrived && mbar_wait_bounded(bar, 1);
       split2(tv);
       block_sync();
-      if (tid == 0 && ok && i + 1 < n) fetch(i + 1, 0, 2);
+      if (tid == 0 && arrived && i + 1 < n) fetch(nx, 0, 2);
     }
-    if (!ok) {
+    if (!arrived) {
       if (tid == 0) report_timeout(p.status, 21, (uint32_t)i);
       return;
     }
@@ -250,7 +273,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         }
       }
       asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
-      if (tid == 0 && i + 1 < n) fetch_w(i + 1);
+      if (tid == 0 && i + 1 < n) fetch_w(nx);
       F2 sa = f2(0.f), sb = f2(0.f);
 #pragma unroll
       for (int m = 0; m < KS; ++m) {  // (an A fragment is two accumulator tiles)
@@ -521,16 +544,25 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       }
     }
     if (ahead) make_chunk_gates(gates[(i + 1) & 1], lane, g_next, b_next);
-    if (!ok) *failed = 1;
-    block_sync();  // this chunk's tiles, states and sums are complete and free
-    if (*failed) return;
-    if (QUERIES && tid == 0) {
-      if (BF && i + 2 < n) fetch(i + 2, 0, 4);
+    if constexpr (QUERIES) {
+      if (st.ends) {
+        if (st.pos == p.NC - 1) {
+          store_state<F>(p.dw0 + (size_t)stream * F * F, dW, row0, col0, lane);
+        } else if (p.slots > 0) {
+          store_state<F>(p.records + (size_t)walk_.slot * F * F, dW, row0, col0, lane);
+          __threadfence();
+          asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
+          if (tid == 0) set_record(p.flags, walk_.slot);
+        }
+      }
     }
-    if (!QUERIES && w == GATED_WARPS - 1) finish_gates(i);
-  }
-  if constexpr (QUERIES) {
-    if (seg == 0) store_state<F>(p.dw0 + (size_t)stream * F * F, dW, row0, col0, lane);
+    if (!ok) shared[0] = 1;
+    block_sync();  // this chunk's tiles, states and sums are complete and free
+    if (shared[0]) return;
+    if (QUERIES && tid == 0) {
+      if (BF && i + 2 < n) fetch(walk_.next(nx), 0, 4);
+    }
+    if (!QUERIES && w == GATED_WARPS - 1) finish_gates(st);
   }
   };
   if (queries) walk(std::true_type{});
@@ -549,7 +581,8 @@ static cudaError_t launch_one(const GatedMaps& maps, const GatedBwdParams& p, cu
     return cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   });
   if (e != cudaSuccess) return e;
-  kfn<<<p.nstreams * p.nseg, GB_THREADS, smem, st>>>(maps, p);
+  if (p.slots > 0 && (e = cudaMemsetAsync(p.flags, 0, (p.slots + 1) * sizeof(int), st)) != cudaSuccess) return e;
+  kfn<<<p.slots > 0 ? p.slots : p.nstreams * p.nseg, GB_THREADS, smem, st>>>(maps, p);
   return cudaGetLastError();
 }
 cudaError_t launch_gated_bwd(int dtype, int F, const GatedMaps& maps, const GatedBwdParams& p, cudaStream_t st) {

@@ -28,7 +28,7 @@ struct GatedFwdSmem {
   static constexpr uint32_t TILES = 0, RAWS = TILES + STAGES * NIN * TILE;
   static constexpr uint32_t W = RAWS + (BF ? 0 : NIN * RAW);
   static constexpr uint32_t GATES = W + (STATE ? 0 : 2 * NP * GTile<F>::STATE_BYTES);
-  static constexpr uint32_t BAR = GATES + 2 * sizeof(ChunkGates), BYTES = BAR + 16 + 1024;  // (1024: the base is aligned by hand)
+  static constexpr uint32_t BAR = GATES + 2 * sizeof(ChunkGates), BYTES = BAR + 32 + 1024;  // (1024: the base is aligned by hand)
 };
 
 template <typename T, int F, bool SAVE, bool STATE, bool REV>
@@ -43,68 +43,93 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   const uint32_t raw = smem_u32(gated_smem), base = (raw + 1023) & ~1023u;
   uint8_t* const mem = gated_smem + (base - raw);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  const int stream = blockIdx.x / p.nseg, seg = blockIdx.x - stream * p.nseg;
-  const int c_lo = seg * p.seg_chunks, c_hi = min(p.NC, c_lo + p.seg_chunks), n = c_hi - c_lo;
-  const int h = stream % p.H, b = stream / p.H;
-  if (STATE && seg == (REV ? 0 : p.nseg - 1)) return;  // nothing follows it
+  if (STATE && (int)blockIdx.x % p.nseg == (REV ? 0 : p.nseg - 1)) return;  // nothing follows it
   const uint32_t bar = base + SM::BAR;
+  volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 16);  // a wait has run out; this block's range
   if (tid == 0) {
+    shared[0] = 0;
+    shared[1] = !STATE && p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
     mbar_init(bar, 1);
     mbar_init(bar + 8, 1);
     fence_mbar_init();
   }
   __syncthreads();
-  auto chunk_of = [&](int i) { return REV ? c_hi - 1 - i : c_lo + i; };
-  auto fetch = [&](int i) {  // thread 0
+  GatedWalk walk{};
+  walk.set(p, shared[1], REV);
+  const int n = walk.n;
+  const GatedWalk::Step first = walk.part(0);
+  auto chunk_of = [&](const GatedWalk::Step& s) { return REV ? p.NC - 1 - s.pos : s.pos; };
+  auto fetch = [&](const GatedWalk::Step& s) {  // thread 0
+    const int i = s.i;
     const int slot = BF ? i & 1 : 0;
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * SM::NIN * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
+    const int b = s.stream / p.H, h = s.stream - b * p.H;
     mbar_expect_tx(at, SM::NIN * bytes);
 #pragma unroll
-    for (int m = 0; m < SM::NIN; ++m) tma_load_4d(dst + m * bytes, &maps.m[(STATE ? 1 : 0) + m], chunk_of(i) * GC, h, b, at);
+    for (int m = 0; m < SM::NIN; ++m) tma_load_4d(dst + m * bytes, &maps.m[(STATE ? 1 : 0) + m], chunk_of(s) * GC, h, b, at);
   };
   if (tid == 0) {
-    fetch(0);
-    if (BF && n > 1) fetch(1);
+    fetch(first);
+    if (BF && n > 1) fetch(walk.next(first));
   }
-  const float* gp = p.g + (size_t)stream * p.T;
-  const float* bp = p.beta != nullptr ? p.beta + (size_t)stream * p.T : nullptr;
   ChunkGates* const gates = reinterpret_cast<ChunkGates*>(mem + SM::GATES);
-  // the gates of walk step i by warp i % 4, a step ahead
-  auto make_gates = [&](int i) {
-    const int t0 = chunk_of(i) * GC;
-    make_chunk_gates(gates[i & 1], lane, load_gates(gp, t0, p.T, lane, 0.f), load_gates(bp, t0, p.T, lane, 1.f));
+  auto gates_of = [&](const GatedWalk::Step& s, float2& g, float2& beta) {
+    const size_t row = (size_t)s.stream * p.T;
+    g = load_gates(p.g + row, chunk_of(s) * GC, p.T, lane, 0.f);
+    beta = load_gates(p.beta != nullptr ? p.beta + row : nullptr, chunk_of(s) * GC, p.T, lane, 1.f);
   };
-  if (w == 0) make_gates(0);
+  if (w == 0) {
+    float2 g0, b0;
+    gates_of(first, g0, b0);
+    make_chunk_gates(gates[0], lane, g0, b0);
+  }
 
   // this warp's share of the state
   const int row0 = 16 * (w % SH::SLABS), part = w / SH::SLABS, col0 = part * SH::COLS;
   float W[SH::NT][4];
-  {
-    const float* w0 = nullptr;
-    if (!STATE) w0 = seg > 0 ? p.seg_state + ((size_t)stream * p.nseg + seg) * F * F : p.w0 != nullptr ? p.w0 + (size_t)stream * F * F : nullptr;
-    load_state<F>(W, w0, row0, col0, lane);
-  }
-  float total = 1.f;  // what is left of the state before the segment after it
-  uint8_t* const saved = SAVE ? p.saved + (size_t)stream * p.NC * F * F * 4 : nullptr;
-  auto publish = [&](int i) {  // the state before walk step i: operand of its q W, and what the backward reads back
-    if constexpr (!STATE) {
-      const uint32_t dst = base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES;
-      put_state<F, NP>(W, row0, col0, dst, lane);
-      if (SAVE && i < n) put_fragments<F>(reinterpret_cast<float4*>(saved + (size_t)(c_lo + i) * F * F * 4), W, w, lane);
+  // the state before walk step i: operand of its q W, and what the backward reads back.  Where a stream or a part of one starts,
+  // from memory; false: the wait for it ran out
+  auto publish = [&](const GatedWalk::Step& s) {
+    const int i = s.i;
+    if constexpr (STATE) {
+      if (i == 0) load_state<F>(W, nullptr, row0, col0, lane);
+    } else {
+        bool ok = true;
+      if (s.starts) {
+        const float* w0 = p.w0 != nullptr ? p.w0 + (size_t)s.stream * F * F : nullptr;
+        if (s.pos > 0) {
+          if (p.slots > 0) {
+            if (lane == 0) ok = wait_record(p.flags, walk.slot - 1);
+            ok = __shfl_sync(0xffffffffu, ok, 0);
+            w0 = p.records + (size_t)(walk.slot - 1) * F * F;
+          } else {
+            w0 = p.seg_state + (size_t)walk.slot * F * F;
+          }
+        }
+        load_state<F>(W, w0, row0, col0, lane);
+      }
+      put_state<F, NP>(W, row0, col0, base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES, lane);
+      if (SAVE) put_fragments<F>(reinterpret_cast<float4*>(p.saved + ((size_t)s.stream * p.NC + s.pos) * F * F * 4), W, w, lane);
+      return ok;
     }
+    return true;
   };
-  publish(0);
+  float total = 1.f;  // what is left of the state before the segment after it
+  if (!publish(first)) shared[0] = 1;
   __syncthreads();
   const uint32_t low = GTile<F>::low(lane), high = GTile<F>::high(lane);
 
-  for (int i = 0; i < n; ++i) {
-    const int slot = BF ? i & 1 : 0, t0 = chunk_of(i) * GC;
+  for (GatedWalk::Step st = first, nx; st.i < n; st = nx) {
+    nx = walk.next(st);
+    const int i = st.i;
+    const int slot = BF ? i & 1 : 0, t0 = chunk_of(st) * GC;
     const bool ahead = w == ((i + 1) & 3) && i + 1 < n;
     float2 g_next, b_next;
-    if (ahead) {
-      g_next = load_gates(gp, chunk_of(i + 1) * GC, p.T, lane, 0.f);
-      b_next = load_gates(bp, chunk_of(i + 1) * GC, p.T, lane, 1.f);
+    if (ahead) gates_of(nx, g_next, b_next);
+    if (!STATE && shared[0]) {
+      if (tid == 0) report_timeout(p.status, 24, (uint32_t)i);
+      return;
     }
     if (!mbar_wait_bounded(bar + 8 * slot, (BF ? i >> 1 : i) & 1)) {
       if (tid == 0) report_timeout(p.status, 20, (uint32_t)i);
@@ -116,7 +141,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       for (int m = 0; m < SM::NIN; ++m)
         split_rows<F>(tiles + m * SM::TILE, SM::PLANE, reinterpret_cast<const float*>(mem + SM::RAWS + m * SM::RAW), GC, tid, GF_THREADS);
       __syncthreads();
-      if (tid == 0 && i + 1 < n) fetch(i + 1);
+      if (tid == 0 && i + 1 < n) fetch(nx);
     }
     const uint32_t tq = tiles, tk = tiles + (STATE ? 0 : SM::TILE), tv = tk + SM::TILE;
     const ChunkGates& cg = gates[i & 1];
@@ -209,49 +234,76 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       }
     }
     if constexpr (!STATE)
-      store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)stream * p.T + t0) * F, 16 * w, p.T - t0, o, lane);
-    if (i + 1 < n) publish(i + 1);
+      store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F, 16 * w, p.T - t0, o, lane);
+    if constexpr (!STATE) {
+      if (st.ends) {
+        if (st.pos == p.NC - 1) {
+          store_state<F>(p.w_out + (size_t)st.stream * F * F, W, row0, col0, lane);
+        } else if (p.slots > 0) {
+          store_state<F>(p.records + (size_t)walk.slot * F * F, W, row0, col0, lane);
+          __threadfence();
+          __syncthreads();
+          if (tid == 0) set_record(p.flags, walk.slot);
+        }
+      }
+    }
+    if (i + 1 < n && !publish(nx)) shared[0] = 1;
     if (ahead) make_chunk_gates(gates[(i + 1) & 1], lane, g_next, b_next);
     __syncthreads();  // the tiles and this chunk's state and gates are free, the next one's are there
-    if (BF && tid == 0 && i + 2 < n) fetch(i + 2);
+    if (BF && tid == 0 && i + 2 < n) fetch(walk.next(nx));
   }
   if constexpr (STATE) {
-    store_state<F>(p.seg_state + ((size_t)stream * p.nseg + seg) * F * F, W, row0, col0, lane);
-    if (tid == 0) p.seg_decay[(size_t)stream * p.nseg + seg] = total;
-  } else if (seg == p.nseg - 1) {
-    store_state<F>(p.w_out + (size_t)stream * F * F, W, row0, col0, lane);
+    store_state<F>(p.seg_state + (size_t)walk.slot * F * F, W, row0, col0, lane);
+    if (tid == 0) p.seg_decay[walk.slot] = total;
   }
 }
 
 // The segments' own states to the states before them, along the sequence (REV: gradients, from the last segment to the first):
-// state[s] <- W_s, W_{s+1} = decay[s] W_s + own[s].  Every thread carries one float4 of a stream's state.
+// state[s] <- W_s, W_{s+1} = decay[s] W_s + own[s].  Every thread carries one float2 of a stream's state; the loads of JOIN_AHEAD
+// segments are on their way at once (one after the other, 37 segments of 12 streams took 60 us).
+constexpr int JOIN_AHEAD = 12, JOIN_THREADS = 128;
 template <int F, bool REV>
-__global__ void __launch_bounds__(256) ttt_gated_join_kernel(const GatedParams p) {
-  constexpr int Q = F * F / 4;
-  const long e = (long)blockIdx.x * 256 + threadIdx.x;
-  if (e >= (long)p.nstreams * Q) return;
+__global__ void __launch_bounds__(JOIN_THREADS) ttt_gated_join_kernel(const GatedParams p) {
+  constexpr int Q = F * F / 2;
+  const long e = (long)blockIdx.x * JOIN_THREADS + threadIdx.x;  // (a multiple of the threads)
   const long stream = e / Q;
   const int at = (int)(e - stream * Q);
-  float4* s = reinterpret_cast<float4*>(p.seg_state) + stream * p.nseg * Q + at;
+  float2* s = reinterpret_cast<float2*>(p.seg_state) + stream * p.nseg * Q + at;
   const float* d = p.seg_decay + stream * p.nseg;
-  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (p.w0 != nullptr) w = reinterpret_cast<const float4*>(p.w0)[stream * Q + at];
-  for (int k = 0; k < p.nseg; ++k) {
-    const int i = REV ? p.nseg - 1 - k : k;
-    const float4 own = s[(long)i * Q];
-    s[(long)i * Q] = w;
-    const float f = d[i];
-    w = make_float4(fmaf(f, w.x, own.x), fmaf(f, w.y, own.y), fmaf(f, w.z, own.z), fmaf(f, w.w, own.w));
+  float2 w = make_float2(0.f, 0.f);
+  if (p.w0 != nullptr) w = reinterpret_cast<const float2*>(p.w0)[stream * Q + at];
+  for (int k0 = 0; k0 < p.nseg; k0 += JOIN_AHEAD) {
+    float2 own[JOIN_AHEAD];
+    float f[JOIN_AHEAD];
+#pragma unroll
+    for (int k = 0; k < JOIN_AHEAD; ++k) {
+      const int i = REV ? p.nseg - 1 - (k0 + k) : k0 + k;
+      if (k0 + k < p.nseg - 1) {  // (nothing follows the last: it has no state of its own)
+        own[k] = s[(long)i * Q];
+        f[k] = d[i];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < JOIN_AHEAD; ++k) {
+      const int i = REV ? p.nseg - 1 - (k0 + k) : k0 + k;
+      if (k0 + k < p.nseg) s[(long)i * Q] = w;
+      if (k0 + k < p.nseg - 1) w = make_float2(fmaf(f[k], w.x, own[k].x), fmaf(f[k], w.y, own[k].y));
+    }
   }
 }
+static_assert(32 * 32 / 2 % JOIN_THREADS == 0, "whole blocks per stream");
 
-// Streams that do not fill the card are cut until they do.
-int gated_segments(int64_t streams, int chunks, bool backward) {
+// Streams that do not fill the card are cut into segments until they do; more streams than blocks are resident are cut into as
+// many ranges as blocks are.
+void gated_split(int64_t streams, int chunks, int dtype, bool backward, int* nseg, int* slots) {
   constexpr int SMS = 148, LEAST = 4;  // (chunks per segment: a segment's states and its second reading must be worth it)
-  if (streams >= SMS) return 1;
-  const int64_t want = ((backward ? 2 : 3) * SMS) / streams;
-  const int64_t most = chunks / LEAST;
-  return (int)(want < most ? want : most > 1 ? most : 1);
+  const int resident = dtype == 1 ? (backward ? 2 : 3) : 1;
+  *nseg = 1;
+  *slots = 0;
+  if (streams > (int64_t)SMS * resident) *slots = SMS * resident;
+  if (streams >= SMS) return;
+  const int64_t want = ((backward ? 2 : 3) * SMS) / streams, most = chunks / LEAST;
+  *nseg = (int)(want < most ? want : most > 1 ? most : 1);
 }
 
 template <typename T, int F, bool SAVE, bool STATE, bool REV>
@@ -274,11 +326,16 @@ static cudaError_t launch_gated(const GatedMaps& maps, GatedParams p, bool save,
   if (p.nseg > 1) {
     cudaError_t e = launch_one<T, F, false, true, false>(maps, p, p.nstreams * p.nseg, st);
     if (e != cudaSuccess) return e;
-    ttt_gated_join_kernel<F, false><<<(int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st>>>(p);
+    ttt_gated_join_kernel<F, false><<<(int)((long)p.nstreams * (F * F / 2) / JOIN_THREADS), JOIN_THREADS, 0, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
-  if (save) return launch_one<T, F, true, false, false>(maps, p, p.nstreams * p.nseg, st);
-  return launch_one<T, F, false, false, false>(maps, p, p.nstreams * p.nseg, st);
+  const int grid = p.slots > 0 ? p.slots : p.nstreams * p.nseg;
+  if (p.slots > 0) {
+    const cudaError_t e = cudaMemsetAsync(p.flags, 0, (p.slots + 1) * sizeof(int), st);
+    if (e != cudaSuccess) return e;
+  }
+  if (save) return launch_one<T, F, true, false, false>(maps, p, grid, st);
+  return launch_one<T, F, false, false, false>(maps, p, grid, st);
 }
 cudaError_t launch_gated_fwd(int dtype, int F, const GatedMaps& maps, const GatedParams& p, bool save, cudaStream_t st) {
   if (F == 64) return dtype == 1 ? launch_gated<__nv_bfloat16, 64>(maps, p, save, st) : launch_gated<float, 64>(maps, p, save, st);
@@ -290,7 +347,7 @@ template <typename T, int F>
 static cudaError_t launch_rev(const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
   cudaError_t e = launch_one<T, F, false, true, true>(maps, p, p.nstreams * p.nseg, st);
   if (e != cudaSuccess) return e;
-  ttt_gated_join_kernel<F, true><<<(int)(((long)p.nstreams * (F * F / 4) + 255) / 256), 256, 0, st>>>(p);
+  ttt_gated_join_kernel<F, true><<<(int)((long)p.nstreams * (F * F / 2) / JOIN_THREADS), JOIN_THREADS, 0, st>>>(p);
   return cudaGetLastError();
 }
 cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {

@@ -424,6 +424,9 @@ struct GatedParams {
   uint32_t* status;
   int T, H, NC;       // NC: chunks of 64 tokens
   int nstreams, nseg, seg_chunks;
+  int slots;          // > 0: ranges of the streams' chunks (GatedWalk); their records and flags, and the counter that numbers them
+  float* records;     // [slots][F*F]
+  int* flags;         // [slots], then the counter; zero before the launch
 };
 struct GatedBwdParams {
   const float* g;
@@ -438,6 +441,9 @@ struct GatedBwdParams {
   uint32_t* status;
   int T, H, NC;
   int nstreams, nseg, seg_chunks;
+  int slots;
+  float* records;
+  int* flags;
 };
 struct GatedStepParams {
   const void *q, *k, *v;
@@ -447,8 +453,8 @@ struct GatedStepParams {
   float* w_out;  // may be w
   int H, R;      // tokens, 1..16
 };
-// Segments per stream (ttt_gated_fwd.cu)
-int gated_segments(int64_t streams, int chunks, bool backward);
+// How many streams are cut: segments per stream, or (more streams than resident blocks) ranges of all of them (ttt_gated_fwd.cu)
+void gated_split(int64_t streams, int chunks, int dtype, bool backward, int* nseg, int* slots);
 cudaError_t launch_gated_fwd(int dtype, int F, const GatedMaps& maps, const GatedParams& p, bool save, cudaStream_t st);
 // maps.m[1], m[2]: queries, gradient of the output
 cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, const GatedParams& p, cudaStream_t st);

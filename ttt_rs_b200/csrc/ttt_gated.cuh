@@ -277,6 +277,10 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* tm,
       : "memory");
 }
 
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // What a block walks: steps of one chunk each.  A stream's chunks are numbered in walk order (`pos`; the backward walks from the
 // last chunk).  With p.slots = 0 a block has one segment of one stream.  Else (more streams than blocks are resident) all steps
 // of all streams, stream after stream, are cut into p.slots equal ranges, of at least a stream's length each: a block's range is

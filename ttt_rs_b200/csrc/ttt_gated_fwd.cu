@@ -1,11 +1,12 @@
 // Gated linear recurrence, forward (the mathematics and its chunked form: ttt_gated.cuh).
 //
-// One CTA of four warps per stream (or per segment of one) walks its chunks; warp w owns 16 queries of the chunk and 16 rows of
-// the float32 state, both in accumulator layout.  Per chunk, for each block of 16 tokens: their keys against the queries at or
-// behind them, the decayed products as the A operand of the product with their values, and the same values, still in registers,
-// under the transposed and scaled keys for the state.  The state goes to shared memory once per chunk as the operand of the next
-// chunk's q W (double-buffered: one barrier per chunk); the next two chunks are on their way meanwhile (TMA, rows behind the
-// sequence read as zeros).
+// One CTA of four warps per stream (or segment, or range of streams) walks its chunks.  A warp owns 16 rows of the float32 state,
+// in accumulator layout, and updates them with the transposed and scaled keys of every chunk; and 16 queries of the chunk, another
+// 16 in every chunk, since the last ones meet four blocks of keys and the first ones one: for each block of 16 tokens the
+// decayed products of queries and keys become, in registers, the A operand of the product with the block's values.  q W comes
+// last: the state before the chunk is there once all warps have left the chunk before, and until then a warp works on what needs only
+// this chunk's inputs, so that no warp waits for the others of its chunk.  The next two chunks are on their way meanwhile (TMA,
+// rows behind the sequence read as zeros).
 //
 // Few streams are cut into segments: a first launch leaves every segment's own state (as if it began with none) and its decay, a
 // second one joins them along the sequence, and the third is this kernel with a CTA per segment.
@@ -17,245 +18,323 @@ namespace ttt {
 
 constexpr int GF_THREADS = 32 * GATED_WARPS;
 
-// STATE: only the state at the end of the segment is wanted (REV: of the gradient's walk, from the last token to the first)
+// STATE: only keys and values (or queries and gradients) come in, and no state goes out before the end
 template <typename T, int F, bool STATE>
 struct GatedFwdSmem {
   static constexpr bool BF = sizeof(T) == 2;
   static constexpr int NP = BF ? 1 : 3, NIN = STATE ? 2 : 3;
   static constexpr uint32_t PLANE = GTile<F>::BYTES, TILE = NP * PLANE;
-  static constexpr uint32_t RAW = GC * F * 4;                                 // float32 rows as they arrive
+  static constexpr uint32_t RAW = GC * F * 4;  // float32 rows as they arrive
   static constexpr uint32_t STAGES = BF ? 2 : 1;
   static constexpr uint32_t TILES = 0, RAWS = TILES + STAGES * NIN * TILE;
   static constexpr uint32_t W = RAWS + (BF ? 0 : NIN * RAW);
   static constexpr uint32_t GATES = W + (STATE ? 0 : 2 * NP * GTile<F>::STATE_BYTES);
-  static constexpr uint32_t BAR = GATES + 2 * sizeof(ChunkGates), BYTES = BAR + 32 + 1024;  // (1024: the base is aligned by hand)
+  static constexpr int NG = STATE ? 2 : 3;  // chunks whose gates are held
+  static constexpr uint32_t BAR = GATES + NG * sizeof(ChunkGates), BYTES = BAR + 48 + 1024;  // (1024: the base is aligned by hand)
 };
 
-template <typename T, int F, bool SAVE, bool STATE, bool REV>
-__global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
-    ttt_gated_fwd_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+// What both kernels do with a chunk's inputs, gates and the state's update
+template <typename T, int F, bool STATE, bool REV, int THREADS>
+struct GatedFwdBlock {
   using SM = GatedFwdSmem<T, F, STATE>;
   using SH = StateShare<F>;
-  constexpr bool BF = SM::BF;
-  constexpr int NP = SM::NP, NS = BF ? 2 : 3;  // planes of inputs, of scaled keys
-  constexpr int KS = F / 16;
-  extern __shared__ uint8_t gated_smem[];
-  const uint32_t raw = smem_u32(gated_smem), base = (raw + 1023) & ~1023u;
-  uint8_t* const mem = gated_smem + (base - raw);
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
-  if (STATE && (int)blockIdx.x % p.nseg == (REV ? 0 : p.nseg - 1)) return;  // nothing follows it
-  const uint32_t bar = base + SM::BAR;
-  volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 16);  // a wait has run out; this block's range
-  if (tid == 0) {
-    shared[0] = 0;
-    shared[1] = !STATE && p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
-    mbar_init(bar, 1);
-    mbar_init(bar + 8, 1);
-    fence_mbar_init();
-  }
-  __syncthreads();
-  GatedWalk walk{};
-  walk.set(p, shared[1], REV);
-  const int n = walk.n;
-  const GatedWalk::Step first = walk.part(0);
-  auto chunk_of = [&](const GatedWalk::Step& s) { return REV ? p.NC - 1 - s.pos : s.pos; };
-  auto fetch = [&](const GatedWalk::Step& s) {  // thread 0
-    const int i = s.i;
-    const int slot = BF ? i & 1 : 0;
+  using TL = GTile<F>;
+  static constexpr bool BF = SM::BF;
+  static constexpr int NP = SM::NP, NS = BF ? 2 : 3, KS = F / 16;  // planes of inputs, of scaled keys
+  const GatedMaps& maps;
+  const GatedParams& p;
+  uint8_t* mem;
+  uint32_t base, bar;
+  ChunkGates* gates;
+  int tid, lane, w;  // w: warp of its group
+  GatedWalk walk;
+
+  __device__ __forceinline__ int chunk_of(const GatedWalk::Step& s) const { return REV ? p.NC - 1 - s.pos : s.pos; }
+  __device__ __forceinline__ void fetch(const GatedWalk::Step& s) const {  // one thread
+    const int slot = BF ? s.i & 1 : 0;
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * SM::NIN * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
     const int b = s.stream / p.H, h = s.stream - b * p.H;
     mbar_expect_tx(at, SM::NIN * bytes);
 #pragma unroll
     for (int m = 0; m < SM::NIN; ++m) tma_load_4d(dst + m * bytes, &maps.m[(STATE ? 1 : 0) + m], chunk_of(s) * GC, h, b, at);
-  };
-  if (tid == 0) {
-    fetch(first);
-    if (BF && n > 1) fetch(walk.next(first));
   }
-  ChunkGates* const gates = reinterpret_cast<ChunkGates*>(mem + SM::GATES);
-  auto gates_of = [&](const GatedWalk::Step& s, float2& g, float2& beta) {
+  __device__ __forceinline__ void gates_of(const GatedWalk::Step& s, float2& g, float2& beta) const {  // one warp
     const size_t row = (size_t)s.stream * p.T;
     g = load_gates(p.g + row, chunk_of(s) * GC, p.T, lane, 0.f);
     beta = load_gates(p.beta != nullptr ? p.beta + row : nullptr, chunk_of(s) * GC, p.T, lane, 1.f);
-  };
-  if (w == 0) {
-    float2 g0, b0;
-    gates_of(first, g0, b0);
-    make_chunk_gates(gates[0], lane, g0, b0);
   }
-
-  // this warp's share of the state
-  const int row0 = 16 * (w % SH::SLABS), part = w / SH::SLABS, col0 = part * SH::COLS;
-  float W[SH::NT][4];
-  // the state before walk step i: operand of its q W, and what the backward reads back.  Where a stream or a part of one starts,
-  // from memory; false: the wait for it ran out
-  auto publish = [&](const GatedWalk::Step& s) {
-    const int i = s.i;
-    if constexpr (STATE) {
-      if (i == 0) load_state<F>(W, nullptr, row0, col0, lane);
-    } else {
-        bool ok = true;
-      if (s.starts) {
-        const float* w0 = p.w0 != nullptr ? p.w0 + (size_t)s.stream * F * F : nullptr;
-        if (s.pos > 0) {
-          if (p.slots > 0) {
-            if (lane == 0) ok = wait_record(p.flags, walk.slot - 1);
-            ok = __shfl_sync(0xffffffffu, ok, 0);
-            w0 = p.records + (size_t)(walk.slot - 1) * F * F;
-          } else {
-            w0 = p.seg_state + (size_t)walk.slot * F * F;
-          }
-        }
-        load_state<F>(W, w0, row0, col0, lane);
-      }
-      put_state<F, NP>(W, row0, col0, base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES, lane);
-      if (SAVE) put_fragments<F>(reinterpret_cast<float4*>(p.saved + ((size_t)s.stream * p.NC + s.pos) * F * F * 4), W, w, lane);
-      return ok;
+  // this chunk's tiles in their planes; false: the wait ran out
+  __device__ __forceinline__ bool tiles(const GatedWalk::Step& st, const GatedWalk::Step& nx, uint32_t& at) const {
+    const int slot = BF ? st.i & 1 : 0;
+    at = base + SM::TILES + slot * SM::NIN * SM::TILE;
+    if (!mbar_wait_bounded(bar + 8 * slot, (BF ? st.i >> 1 : st.i) & 1)) {
+      if (tid == 0) report_timeout(p.status, 20, (uint32_t)st.i);
+      return false;
     }
-    return true;
-  };
-  float total = 1.f;  // what is left of the state before the segment after it
-  if (!publish(first)) shared[0] = 1;
-  __syncthreads();
-  const uint32_t low = GTile<F>::low(lane), high = GTile<F>::high(lane);
-
-  for (GatedWalk::Step st = first, nx; st.i < n; st = nx) {
-    nx = walk.next(st);
-    const int i = st.i;
-    const int slot = BF ? i & 1 : 0, t0 = chunk_of(st) * GC;
-    const bool ahead = w == ((i + 1) & 3) && i + 1 < n;
-    float2 g_next, b_next;
-    if (ahead) gates_of(nx, g_next, b_next);
-    if (!STATE && shared[0]) {
-      if (tid == 0) report_timeout(p.status, 24, (uint32_t)i);
-      return;
-    }
-    if (!mbar_wait_bounded(bar + 8 * slot, (BF ? i >> 1 : i) & 1)) {
-      if (tid == 0) report_timeout(p.status, 20, (uint32_t)i);
-      return;
-    }
-    const uint32_t tiles = base + SM::TILES + slot * SM::NIN * SM::TILE;
     if constexpr (!BF) {
 #pragma unroll
       for (int m = 0; m < SM::NIN; ++m)
-        split_rows<F>(tiles + m * SM::TILE, SM::PLANE, reinterpret_cast<const float*>(mem + SM::RAWS + m * SM::RAW), GC, tid, GF_THREADS);
-      __syncthreads();
-      if (tid == 0 && i + 1 < n) fetch(nx);
+        split_rows<F>(at + m * SM::TILE, SM::PLANE, reinterpret_cast<const float*>(mem + SM::RAWS + m * SM::RAW), GC, tid, THREADS);
+      block_sync();
+      if (tid == 0 && nx.i < walk.n) fetch(nx);
     }
-    const uint32_t tq = tiles, tk = tiles + (STATE ? 0 : SM::TILE), tv = tk + SM::TILE;
-    const ChunkGates& cg = gates[i & 1];
-
-    float o[STATE ? 1 : F / 8][4];
-    Pk<NP> q[STATE ? 1 : KS][4];
-    if constexpr (!STATE) {
-      // q_i W, from the start of this warp's block on
-      const uint32_t tw = base + SM::W + (i & 1) * NP * GTile<F>::STATE_BYTES;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(q[k], (tq + 16 * w * GTile<F>::ROW + low) ^ (k << 5), SM::PLANE, false);
-#pragma unroll
-      for (int k = 0; k < F / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int m = 0; m < KS; ++m) {
-          Pk<NP> f[4];
-          ldsm_np<NP>(f, (tw + 16 * k * GTile<F>::ROW + low) ^ (m << 5), GTile<F>::STATE_BYTES, true);
-          mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], q[k], f);
-        }
-      const float first = cg.starts[w];
-#pragma unroll
-      for (int k = 0; k < F / 8; ++k) scale_rows(o[k], first, first);
-    }
+    return true;
+  }
+  static __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0, %0;" ::"n"(THREADS) : "memory"); }
+  // W <- e^{G_end} W + sum of scaled keys^T values (REV: queries^T gradients, scaled by what is left at the token)
+  __device__ __forceinline__ void update(float (&W)[SH::NT][4], uint32_t tk, uint32_t tv, const ChunkGates& cg, int row0, int col0) const {
+    const uint32_t low = TL::low(lane), high = TL::high(lane);
     const float all = cg.all;
-    total *= all;
 #pragma unroll
     for (int k = 0; k < SH::NT; ++k) scale_rows(W[k], all, all);
-
+    const float* scale = REV ? cg.from : cg.end_b;
 #pragma unroll 1
     for (int jt = 0; jt < GC / 16; ++jt) {
-      const int j0 = 16 * jt + 2 * t4;
-      // queries of this warp against the keys of the block, decayed, as an operand of the inputs' planes
-      Pk<NP> a[4];
-      const bool here = !STATE && jt <= w;
-      if constexpr (!STATE) {
-        if (here) {
-          float s0[4] = {}, s1[4] = {};
-#pragma unroll
-          for (int k = 0; k < KS; ++k) {
-            Pk<NP> f[4];
-            ldsm_np<NP>(f, (tk + 16 * jt * GTile<F>::ROW + high) ^ (k << 5), SM::PLANE, false);
-            mma_planes<NP, NP>(s0, s1, q[k], f);
-          }
-          if (jt < w) {
-            const F2 between = f2(cg.blocks[jt][w - 1]);
-            scale_cols(s0, f2mul(ld2(&cg.out_b[j0]), between));
-            scale_cols(s1, f2mul(ld2(&cg.out_b[j0 + 8]), between));
-          } else {
-            // what came from before the block, to each of its tokens; then the block itself
-            const float ra = cg.into[16 * w + g], rb = cg.into[16 * w + g + 8];
-#pragma unroll
-            for (int k = 0; k < F / 8; ++k) scale_rows(o[k], ra, rb);
-            float d[2][4];
-            block_decays<true>(d, cg, w, g, t4);
-            const float2 b0 = ld2(&cg.beta[j0]), b1 = ld2(&cg.beta[j0 + 8]);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {  // (a select, not a product: what is not there may be infinite)
-              s0[2 * half] = d[half][0] > 0.f ? s0[2 * half] * (d[half][0] * b0.x) : 0.f;
-              s0[2 * half + 1] = d[half][1] > 0.f ? s0[2 * half + 1] * (d[half][1] * b0.y) : 0.f;
-              s1[2 * half] = d[half][2] > 0.f ? s1[2 * half] * (d[half][2] * b1.x) : 0.f;
-              s1[2 * half + 1] = d[half][3] > 0.f ? s1[2 * half + 1] * (d[half][3] * b1.y) : 0.f;
-            }
-          }
-          as_operand<NP>(a, s0, s1);
-        }
-      }
-      // keys of the block, transposed: rows of the state
+      const int j0 = 16 * jt + 2 * (lane & 3);
       Pk<NS> kt[4];
       {
         Pk<NP> f[4];
-        ldsm_np<NP>(f, (tk + 16 * jt * GTile<F>::ROW + high) ^ (row0 << 1), SM::PLANE, true);
-        const float* scale = REV ? cg.from : cg.end_b;  // (REV: what is left at the token of the state before the chunk)
+        ldsm_np<NP>(f, (tk + 16 * jt * TL::ROW + high) ^ (row0 << 1), SM::PLANE, true);
         scale_a_cols<NS, NP>(kt, f, ld2(scale + j0), ld2(scale + j0 + 8));
       }
+      const uint32_t v = tv + 16 * jt * TL::ROW + low;
+#pragma unroll
+      for (int m = 0; m < SH::NT / 2; ++m) {
+        Pk<NP> f[4];
+        ldsm_np<NP>(f, v ^ ((col0 << 1) + (m << 5)), SM::PLANE, true);
+        mma_planes<NS, NP>(W[2 * m], W[2 * m + 1], kt, f);
+      }
+    }
+  }
+};
+
+template <typename T, int F, bool SAVE>
+__global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
+    ttt_gated_fwd_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+  using BK = GatedFwdBlock<T, F, false, false, GF_THREADS>;
+  using SM = typename BK::SM;
+  using SH = StateShare<F>;
+  using TL = GTile<F>;
+  constexpr bool BF = BK::BF;
+  constexpr int NP = BK::NP, KS = BK::KS;
+  extern __shared__ uint8_t gated_smem[];
+  const uint32_t raw = smem_u32(gated_smem), base = (raw + 1023) & ~1023u;
+  uint8_t* const mem = gated_smem + (base - raw);
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
+  volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 32);  // a wait has run out; this block's range
+  BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), tid, lane, w, {}};
+  const uint32_t left = bk.bar + 16;  // the warps have left an even, an odd chunk
+  if (tid == 0) {
+    shared[0] = 0;
+    shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
+    mbar_init(bk.bar, 1);
+    mbar_init(bk.bar + 8, 1);
+    mbar_init(left, GATED_WARPS);
+    mbar_init(left + 8, GATED_WARPS);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  bk.walk.set(p, shared[1], false);
+  const int n = bk.walk.n;
+  const GatedWalk::Step first = bk.walk.part(0), second = bk.walk.next(first);
+  if (tid == 0) {
+    bk.fetch(first);
+    if (BF && n > 1) bk.fetch(second);
+  }
+  if (w < 2 && w < n) {
+    float2 g0, b0;
+    bk.gates_of(w == 0 ? first : second, g0, b0);
+    make_chunk_gates(bk.gates[w], lane, g0, b0);
+  }
+  const uint32_t low = TL::low(lane), high = TL::high(lane);
+  const int row0 = 16 * (w % SH::SLABS), col0 = w / SH::SLABS * SH::COLS;
+  float W[SH::NT][4];
+  // the state before a step: operand of its q W, and what the backward reads back.  Where a stream or a part of one starts, from
+  // memory
+  auto publish = [&](const GatedWalk::Step& s) {
+    if (s.starts) {
+      const float* w0 = p.w0 != nullptr ? p.w0 + (size_t)s.stream * F * F : nullptr;
+      if (s.pos > 0) {
+        if (p.slots > 0) {
+          int ok = 1;
+          if (lane == 0) ok = wait_record(p.flags, bk.walk.slot - 1);
+          if (!__shfl_sync(0xffffffffu, ok, 0)) {
+            if (lane == 0) report_timeout(p.status, 24, (uint32_t)s.i);
+            shared[0] = 1;
+          }
+          w0 = p.records + (size_t)(bk.walk.slot - 1) * F * F;
+        } else {
+          w0 = p.seg_state + (size_t)bk.walk.slot * F * F;
+        }
+      }
+      load_state<F>(W, w0, row0, col0, lane);
+    }
+    put_state<F, NP>(W, row0, col0, base + SM::W + (s.i & 1) * NP * TL::STATE_BYTES, lane);
+    if (SAVE) put_fragments<F>(reinterpret_cast<float4*>(p.saved + ((size_t)s.stream * p.NC + s.pos) * F * F * 4), W, w, lane);
+  };
+  publish(first);
+  __syncthreads();
+  if (shared[0]) return;
+  // all warps have left the chunk before step i: its tiles, gates and the state before it are free, the state behind it is complete
+  auto settled = [&](int i) {
+    if (i == 0) return true;
+    if (!mbar_wait_bounded(left + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1)) {
+      if (tid == 0) report_timeout(p.status, 25, (uint32_t)i);
+      return false;
+    }
+    return shared[0] == 0;
+  };
+  int slot3 = 0;  // i modulo 3
+#pragma unroll 1
+  for (GatedWalk::Step st = first, nx = second, fa; st.i < n; st = nx, nx = fa) {
+    fa = bk.walk.next(nx);
+    const int i = st.i, r = (w + i) & 3, slot3n = slot3 == 0 ? 2 : slot3 - 1;  // r: this warp's queries; (i + 2) modulo 3
+    const bool ahead = r == 0 && fa.i < n;  // (the warp with one block)
+    float2 g_next, b_next;
+    if (ahead) bk.gates_of(fa, g_next, b_next);
+    if (!BF && !settled(i)) return;  // (one set of planes)
+    uint32_t tq;
+    if (!bk.tiles(st, nx, tq)) return;
+    const uint32_t tk = tq + SM::TILE, tv = tk + SM::TILE, tw = base + SM::W + (i & 1) * NP * TL::STATE_BYTES;
+    const ChunkGates& cg = bk.gates[slot3];
+    float o[F / 8][4];
+    Pk<NP> q[KS][4];
+#pragma unroll
+    for (int k = 0; k < F / 8; ++k) o[k][0] = o[k][1] = o[k][2] = o[k][3] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ldsm_np<NP>(q[k], (tq + 16 * r * TL::ROW + low) ^ (k << 5), SM::PLANE, false);
+#pragma unroll 1
+    for (int jt = 0; jt <= r; ++jt) {
+      const int j0 = 16 * jt + 2 * t4;
+      float s0[4] = {}, s1[4] = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        Pk<NP> f[4];
+        ldsm_np<NP>(f, (tk + 16 * jt * TL::ROW + high) ^ (k << 5), SM::PLANE, false);
+        mma_planes<NP, NP>(s0, s1, q[k], f);
+      }
+      if (jt < r) {
+        const F2 between = f2(cg.blocks[jt][r - 1]);
+        scale_cols(s0, f2mul(ld2(&cg.out_b[j0]), between));
+        scale_cols(s1, f2mul(ld2(&cg.out_b[j0 + 8]), between));
+      } else {
+        // what came from the blocks before, to each token of this one; then the block itself
+        const float ra = cg.into[16 * r + g], rb = cg.into[16 * r + g + 8];
+#pragma unroll
+        for (int k = 0; k < F / 8; ++k) scale_rows(o[k], ra, rb);
+        float d[2][4];
+        block_decays<true>(d, cg, r, g, t4);
+        const float2 b0 = ld2(&cg.beta[j0]), b1 = ld2(&cg.beta[j0 + 8]);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {  // (a select, not a product: what is not there may be infinite)
+          s0[2 * half] = d[half][0] > 0.f ? s0[2 * half] * (d[half][0] * b0.x) : 0.f;
+          s0[2 * half + 1] = d[half][1] > 0.f ? s0[2 * half + 1] * (d[half][1] * b0.y) : 0.f;
+          s1[2 * half] = d[half][2] > 0.f ? s1[2 * half] * (d[half][2] * b1.x) : 0.f;
+          s1[2 * half + 1] = d[half][3] > 0.f ? s1[2 * half + 1] * (d[half][3] * b1.y) : 0.f;
+        }
+      }
+      Pk<NP> a[4];
+      as_operand<NP>(a, s0, s1);
 #pragma unroll
       for (int m = 0; m < KS; ++m) {
-        const bool mine = SH::PARTS == 1 || m == part;
-        if (!mine && !here) continue;
         Pk<NP> f[4];
-        ldsm_np<NP>(f, (tv + 16 * jt * GTile<F>::ROW + low) ^ (m << 5), SM::PLANE, true);
-        if constexpr (!STATE) {
-          if (here) mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], a, f);
-        }
-        if (mine) {
-          const int at = SH::PARTS == 1 ? 2 * m : 0;
-          mma_planes<NS, NP>(W[at], W[at + 1], kt, f);
-        }
+        ldsm_np<NP>(f, (tv + 16 * jt * TL::ROW + low) ^ (m << 5), SM::PLANE, true);
+        mma_planes<NP, NP>(o[2 * m], o[2 * m + 1], a, f);
       }
     }
-    if constexpr (!STATE)
-      store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F, 16 * w, p.T - t0, o, lane);
-    if constexpr (!STATE) {
-      if (st.ends) {
-        if (st.pos == p.NC - 1) {
-          store_state<F>(p.w_out + (size_t)st.stream * F * F, W, row0, col0, lane);
-        } else if (p.slots > 0) {
-          store_state<F>(p.records + (size_t)walk.slot * F * F, W, row0, col0, lane);
-          __threadfence();
-          __syncthreads();
-          if (tid == 0) set_record(p.flags, walk.slot);
+    bk.update(W, tk, tv, cg, row0, col0);
+    if (BF && !settled(i)) return;
+    if (BF && r == 0 && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
+    if (ahead) make_chunk_gates(bk.gates[slot3n], lane, g_next, b_next);
+    const float fra = cg.from[16 * r + g], frb = cg.from[16 * r + g + 8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {  // (columns in two halves, for the registers)
+      float c[F / 16][4];
+#pragma unroll
+      for (int k = 0; k < F / 16; ++k) c[k][0] = c[k][1] = c[k][2] = c[k][3] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int m = 0; m < KS / 2; ++m) {
+          Pk<NP> f[4];
+          ldsm_np<NP>(f, (tw + 16 * k * TL::ROW + low) ^ ((half * (KS / 2) + m) << 5), TL::STATE_BYTES, true);
+          mma_planes<NP, NP>(c[2 * m], c[2 * m + 1], q[k], f);
         }
+#pragma unroll
+      for (int k = 0; k < F / 16; ++k) add_rows(o[half * (F / 16) + k], c[k], fra, frb);
+    }
+    if (st.ends) {
+      if (st.pos == p.NC - 1) {
+        store_state<F>(p.w_out + (size_t)st.stream * F * F, W, row0, col0, lane);
+      } else if (p.slots > 0) {
+        store_state<F>(p.records + (size_t)bk.walk.slot * F * F, W, row0, col0, lane);
+        __threadfence();
+        asm volatile("bar.sync 1, %0;" ::"n"(GF_THREADS) : "memory");
+        if (tid == 0) set_record(p.flags, bk.walk.slot);
       }
     }
-    if (i + 1 < n && !publish(nx)) shared[0] = 1;
-    if (ahead) make_chunk_gates(gates[(i + 1) & 1], lane, g_next, b_next);
-    __syncthreads();  // the tiles and this chunk's state and gates are free, the next one's are there
-    if (BF && tid == 0 && i + 2 < n) fetch(walk.next(nx));
+    if (nx.i < n) publish(nx);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(left + 8 * (i & 1));
+    const int t0 = st.pos * GC;
+    store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F, 16 * r, p.T - t0, o, lane);
+    slot3 = slot3 == 2 ? 0 : slot3 + 1;
   }
-  if constexpr (STATE) {
-    store_state<F>(p.seg_state + (size_t)walk.slot * F * F, W, row0, col0, lane);
-    if (tid == 0) p.seg_decay[walk.slot] = total;
+}
+
+// Every segment's own state, and what is left behind it of the state before it
+template <typename T, int F, bool REV>
+__global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 6 : F == 64 ? 2 : 4)
+    ttt_gated_state_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
+  using BK = GatedFwdBlock<T, F, true, REV, GF_THREADS>;
+  using SM = typename BK::SM;
+  using SH = StateShare<F>;
+  constexpr bool BF = BK::BF;
+  if ((int)blockIdx.x % p.nseg == (REV ? 0 : p.nseg - 1)) return;  // nothing follows it
+  extern __shared__ uint8_t gated_smem[];
+  const uint32_t raw = smem_u32(gated_smem), base = (raw + 1023) & ~1023u;
+  uint8_t* const mem = gated_smem + (base - raw);
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), tid, lane, w, {}};
+  if (tid == 0) {
+    mbar_init(bk.bar, 1);
+    mbar_init(bk.bar + 8, 1);
+    fence_mbar_init();
   }
+  bk.walk.set(p, (int)blockIdx.x, REV);
+  const int n = bk.walk.n;
+  const GatedWalk::Step first = bk.walk.part(0);
+  if (w == 0) {
+    float2 g0, b0;
+    bk.gates_of(first, g0, b0);
+    make_chunk_gates(bk.gates[0], lane, g0, b0);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    bk.fetch(first);
+    if (BF && n > 1) bk.fetch(bk.walk.next(first));
+  }
+  const int row0 = 16 * (w % SH::SLABS), col0 = w / SH::SLABS * SH::COLS;
+  float W[SH::NT][4], total = 1.f;
+  load_state<F>(W, nullptr, row0, col0, lane);
+#pragma unroll 1
+  for (GatedWalk::Step st = first, nx; st.i < n; st = nx) {
+    nx = bk.walk.next(st);
+    const bool ahead = w == (nx.i & 3) && nx.i < n;
+    float2 g_next, b_next;
+    if (ahead) bk.gates_of(nx, g_next, b_next);
+    uint32_t tk;
+    if (!bk.tiles(st, nx, tk)) return;
+    const ChunkGates& cg = bk.gates[st.i & 1];
+    total *= cg.all;
+    bk.update(W, tk, tk + SM::TILE, cg, row0, col0);
+    if (ahead) make_chunk_gates(bk.gates[nx.i & 1], lane, g_next, b_next);
+    BK::block_sync();
+    if (BF && tid == 0 && nx.i + 1 < n) bk.fetch(bk.walk.next(nx));
+  }
+  store_state<F>(p.seg_state + (size_t)bk.walk.slot * F * F, W, row0, col0, lane);
+  if (tid == 0) p.seg_decay[bk.walk.slot] = total;
 }
 
 // The segments' own states to the states before them, along the sequence (REV: gradients, from the last segment to the first):
@@ -306,36 +385,40 @@ void gated_split(int64_t streams, int chunks, int dtype, bool backward, int* nse
   *nseg = (int)(want < most ? want : most > 1 ? most : 1);
 }
 
-template <typename T, int F, bool SAVE, bool STATE, bool REV>
-static cudaError_t launch_one(const GatedMaps& maps, const GatedParams& p, int grid, cudaStream_t st) {
-  auto kfn = ttt_gated_fwd_kernel<T, F, SAVE, STATE, REV>;
-  constexpr size_t smem = GatedFwdSmem<T, F, STATE>::BYTES;
-  static DeviceValue ready;
+template <typename Fn>
+static cudaError_t launch_one(Fn kfn, DeviceValue& ready, const GatedMaps& maps, const GatedParams& p, int grid, int threads, size_t smem,
+                              cudaStream_t st) {
   int unused;
-  cudaError_t e = ready.get(0, &unused, [&](int* v) {
+  const cudaError_t e = ready.get(0, &unused, [&](int* v) {
     *v = 0;
     return cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   });
   if (e != cudaSuccess) return e;
-  kfn<<<grid, GF_THREADS, smem, st>>>(maps, p);
+  kfn<<<grid, threads, smem, st>>>(maps, p);
+  return cudaGetLastError();
+}
+// The states before every segment (REV: the gradients of those behind)
+template <typename T, int F, bool REV>
+static cudaError_t launch_states(const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
+  static DeviceValue ready;
+  const cudaError_t e = launch_one(ttt_gated_state_kernel<T, F, REV>, ready, maps, p, p.nstreams * p.nseg, GF_THREADS,
+                                   GatedFwdSmem<T, F, true>::BYTES, st);
+  if (e != cudaSuccess) return e;
+  ttt_gated_join_kernel<F, REV><<<(int)((long)p.nstreams * (F * F / 2) / JOIN_THREADS), JOIN_THREADS, 0, st>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T, int F>
-static cudaError_t launch_gated(const GatedMaps& maps, GatedParams p, bool save, cudaStream_t st) {
-  if (p.nseg > 1) {
-    cudaError_t e = launch_one<T, F, false, true, false>(maps, p, p.nstreams * p.nseg, st);
-    if (e != cudaSuccess) return e;
-    ttt_gated_join_kernel<F, false><<<(int)((long)p.nstreams * (F * F / 2) / JOIN_THREADS), JOIN_THREADS, 0, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  }
+static cudaError_t launch_gated(const GatedMaps& maps, const GatedParams& p, bool save, cudaStream_t st) {
+  cudaError_t e = cudaSuccess;
+  if (p.nseg > 1) e = launch_states<T, F, false>(maps, p, st);
+  else if (p.slots > 0) e = cudaMemsetAsync(p.flags, 0, (p.slots + 1) * sizeof(int), st);
+  if (e != cudaSuccess) return e;
+  static DeviceValue ready_save, ready;
   const int grid = p.slots > 0 ? p.slots : p.nstreams * p.nseg;
-  if (p.slots > 0) {
-    const cudaError_t e = cudaMemsetAsync(p.flags, 0, (p.slots + 1) * sizeof(int), st);
-    if (e != cudaSuccess) return e;
-  }
-  if (save) return launch_one<T, F, true, false, false>(maps, p, grid, st);
-  return launch_one<T, F, false, false, false>(maps, p, grid, st);
+  constexpr size_t smem = GatedFwdSmem<T, F, false>::BYTES;
+  return save ? launch_one(ttt_gated_fwd_kernel<T, F, true>, ready_save, maps, p, grid, GF_THREADS, smem, st)
+              : launch_one(ttt_gated_fwd_kernel<T, F, false>, ready, maps, p, grid, GF_THREADS, smem, st);
 }
 cudaError_t launch_gated_fwd(int dtype, int F, const GatedMaps& maps, const GatedParams& p, bool save, cudaStream_t st) {
   if (F == 64) return dtype == 1 ? launch_gated<__nv_bfloat16, 64>(maps, p, save, st) : launch_gated<float, 64>(maps, p, save, st);
@@ -343,16 +426,9 @@ cudaError_t launch_gated_fwd(int dtype, int F, const GatedMaps& maps, const Gate
 }
 
 // The gradient's states behind every segment: maps 1 and 2 are the queries and the output's gradient
-template <typename T, int F>
-static cudaError_t launch_rev(const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
-  cudaError_t e = launch_one<T, F, false, true, true>(maps, p, p.nstreams * p.nseg, st);
-  if (e != cudaSuccess) return e;
-  ttt_gated_join_kernel<F, true><<<(int)((long)p.nstreams * (F * F / 2) / JOIN_THREADS), JOIN_THREADS, 0, st>>>(p);
-  return cudaGetLastError();
-}
 cudaError_t launch_gated_segments_rev(int dtype, int F, const GatedMaps& maps, const GatedParams& p, cudaStream_t st) {
-  if (F == 64) return dtype == 1 ? launch_rev<__nv_bfloat16, 64>(maps, p, st) : launch_rev<float, 64>(maps, p, st);
-  return dtype == 1 ? launch_rev<__nv_bfloat16, 32>(maps, p, st) : launch_rev<float, 32>(maps, p, st);
+  if (F == 64) return dtype == 1 ? launch_states<__nv_bfloat16, 64, true>(maps, p, st) : launch_states<float, 64, true>(maps, p, st);
+  return dtype == 1 ? launch_states<__nv_bfloat16, 32, true>(maps, p, st) : launch_states<float, 32, true>(maps, p, st);
 }
 
 }  // namespace ttt

@@ -29,8 +29,7 @@ struct GatedFwdSmem {
   static constexpr uint32_t TILES = 0, RAWS = TILES + STAGES * NIN * TILE;
   static constexpr uint32_t W = RAWS + (BF ? 0 : NIN * RAW);
   static constexpr uint32_t GATES = W + (STATE ? 0 : 2 * NP * GTile<F>::STATE_BYTES);
-  static constexpr int NG = STATE ? 2 : 3;  // chunks whose gates are held
-  static constexpr uint32_t BAR = GATES + NG * sizeof(ChunkGates), BYTES = BAR + 48 + 1024;  // (1024: the base is aligned by hand)
+  static constexpr uint32_t BAR = GATES + 3 * sizeof(ChunkGates), BYTES = BAR + 48 + 1024;  // (1024: the base is aligned by hand)
 };
 
 // What both kernels do with a chunk's inputs, gates and the state's update
@@ -81,6 +80,19 @@ struct GatedFwdBlock {
     }
     return true;
   }
+  // a warp has left step i; all warps have left the step before i (its tiles and gates are free, what it wrote is complete)
+  __device__ __forceinline__ void leave(int i) const {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar + 16 + 8 * (i & 1));
+  }
+  __device__ __forceinline__ bool settled(int i) const {
+    if (i <= 0) return true;
+    if (!mbar_wait_bounded(bar + 16 + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1)) {
+      if (tid == 0) report_timeout(p.status, 25, (uint32_t)i);
+      return false;
+    }
+    return reinterpret_cast<volatile int*>(mem + SM::BAR + 32)[0] == 0;
+  }
   static __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0, %0;" ::"n"(THREADS) : "memory"); }
   // W <- e^{G_end} W + sum of scaled keys^T values (REV: queries^T gradients, scaled by what is left at the token)
   __device__ __forceinline__ void update(float (&W)[SH::NT][4], uint32_t tk, uint32_t tv, const ChunkGates& cg, int row0, int col0) const {
@@ -124,14 +136,13 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
   volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 32);  // a wait has run out; this block's range
   BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), tid, lane, w, {}};
-  const uint32_t left = bk.bar + 16;  // the warps have left an even, an odd chunk
   if (tid == 0) {
     shared[0] = 0;
     shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
     mbar_init(bk.bar, 1);
     mbar_init(bk.bar + 8, 1);
-    mbar_init(left, GATED_WARPS);
-    mbar_init(left + 8, GATED_WARPS);
+    mbar_init(bk.bar + 16, GATED_WARPS);
+    mbar_init(bk.bar + 24, GATED_WARPS);
     fence_mbar_init();
   }
   __syncthreads();
@@ -176,15 +187,6 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   publish(first);
   __syncthreads();
   if (shared[0]) return;
-  // all warps have left the chunk before step i: its tiles, gates and the state before it are free, the state behind it is complete
-  auto settled = [&](int i) {
-    if (i == 0) return true;
-    if (!mbar_wait_bounded(left + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1)) {
-      if (tid == 0) report_timeout(p.status, 25, (uint32_t)i);
-      return false;
-    }
-    return shared[0] == 0;
-  };
   int slot3 = 0;  // i modulo 3
 #pragma unroll 1
   for (GatedWalk::Step st = first, nx = second, fa; st.i < n; st = nx, nx = fa) {
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     const bool ahead = r == 0 && fa.i < n;  // (the warp with one block)
     float2 g_next, b_next;
     if (ahead) bk.gates_of(fa, g_next, b_next);
-    if (!BF && !settled(i)) return;  // (one set of planes)
+    if (!BF && !bk.settled(i)) return;  // (one set of planes)
     uint32_t tq;
     if (!bk.tiles(st, nx, tq)) return;
     const uint32_t tk = tq + SM::TILE, tv = tk + SM::TILE, tw = base + SM::W + (i & 1) * NP * TL::STATE_BYTES;
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       }
     }
     bk.update(W, tk, tv, cg, row0, col0);
-    if (BF && !settled(i)) return;
+    if (BF && !bk.settled(i)) return;
     if (BF && r == 0 && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
     if (ahead) make_chunk_gates(bk.gates[slot3n], lane, g_next, b_next);
     const float fra = cg.from[16 * r + g], frb = cg.from[16 * r + g + 8];
@@ -275,17 +277,17 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       }
     }
     if (nx.i < n) publish(nx);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(left + 8 * (i & 1));
+    bk.leave(i);
     const int t0 = st.pos * GC;
     store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F, 16 * r, p.T - t0, o, lane);
     slot3 = slot3 == 2 ? 0 : slot3 + 1;
   }
 }
 
-// Every segment's own state, and what is left behind it of the state before it
+// Every segment's own state, and what is left behind it of the state before it.  No warp needs another's rows: they share the tiles
+// and the gates, made two chunks ahead.
 template <typename T, int F, bool REV>
-__global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 6 : F == 64 ? 2 : 4)
+__global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 : 4)
     ttt_gated_state_kernel(const __grid_constant__ GatedMaps maps, const GatedParams p) {
   using BK = GatedFwdBlock<T, F, true, REV, GF_THREADS>;
   using SM = typename BK::SM;
@@ -298,40 +300,50 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 6 : F == 64 ? 2 :
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), tid, lane, w, {}};
   if (tid == 0) {
+    *reinterpret_cast<volatile int*>(mem + SM::BAR + 32) = 0;
     mbar_init(bk.bar, 1);
     mbar_init(bk.bar + 8, 1);
+    mbar_init(bk.bar + 16, GATED_WARPS);
+    mbar_init(bk.bar + 24, GATED_WARPS);
     fence_mbar_init();
   }
   bk.walk.set(p, (int)blockIdx.x, REV);
   const int n = bk.walk.n;
-  const GatedWalk::Step first = bk.walk.part(0);
-  if (w == 0) {
-    float2 g0, b0;
-    bk.gates_of(first, g0, b0);
-    make_chunk_gates(bk.gates[0], lane, g0, b0);
-  }
-  __syncthreads();
+  const GatedWalk::Step first = bk.walk.part(0), second = bk.walk.next(first);
   if (tid == 0) {
     bk.fetch(first);
-    if (BF && n > 1) bk.fetch(bk.walk.next(first));
+    if (BF && n > 1) bk.fetch(second);
   }
+  if (w < 2 && w < n) {
+    float2 g0, b0;
+    bk.gates_of(w == 0 ? first : second, g0, b0);
+    make_chunk_gates(bk.gates[w], lane, g0, b0);
+  }
+  __syncthreads();
   const int row0 = 16 * (w % SH::SLABS), col0 = w / SH::SLABS * SH::COLS;
   float W[SH::NT][4], total = 1.f;
   load_state<F>(W, nullptr, row0, col0, lane);
+  int slot3 = 0;  // i modulo 3
 #pragma unroll 1
-  for (GatedWalk::Step st = first, nx; st.i < n; st = nx) {
-    nx = bk.walk.next(st);
-    const bool ahead = w == (nx.i & 3) && nx.i < n;
+  for (GatedWalk::Step st = first, nx = second, fa; st.i < n; st = nx, nx = fa) {
+    fa = bk.walk.next(nx);
+    const int i = st.i;
+    const bool turn = w == (i & 3), ahead = turn && fa.i < n;
     float2 g_next, b_next;
-    if (ahead) bk.gates_of(nx, g_next, b_next);
+    if (ahead) bk.gates_of(fa, g_next, b_next);
+    if (!bk.settled(BF ? i - 1 : i)) return;  // (float32: one set of planes)
     uint32_t tk;
     if (!bk.tiles(st, nx, tk)) return;
-    const ChunkGates& cg = bk.gates[st.i & 1];
+    const ChunkGates& cg = bk.gates[slot3];
     total *= cg.all;
     bk.update(W, tk, tk + SM::TILE, cg, row0, col0);
-    if (ahead) make_chunk_gates(bk.gates[nx.i & 1], lane, g_next, b_next);
-    BK::block_sync();
-    if (BF && tid == 0 && nx.i + 1 < n) bk.fetch(bk.walk.next(nx));
+    if (turn) {
+      if (BF && !bk.settled(i)) return;
+      if (BF && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
+      if (ahead) make_chunk_gates(bk.gates[slot3 == 0 ? 2 : slot3 - 1], lane, g_next, b_next);
+    }
+    bk.leave(i);
+    slot3 = slot3 == 2 ? 0 : slot3 + 1;
   }
   store_state<F>(p.seg_state + (size_t)bk.walk.slot * F * F, W, row0, col0, lane);
   if (tid == 0) p.seg_decay[bk.walk.slot] = total;

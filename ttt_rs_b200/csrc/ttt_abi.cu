@@ -1625,7 +1625,7 @@ extern "C" int ttt_layer_qk_norm_rotary(const ttt_dims* d, int k_heads, const vo
 
 extern "C" size_t ttt_layer_qk_norm_rotary_backward_workspace_bytes(const ttt_dims* d, int k_heads) {
   if (check_head_dims(d, k_heads) != TTT_OK || k_heads < 1) return 0;
-  return sizeof(float) * ttt::rotary_partial_floats((int64_t)d->batch * d->seq_len, d->heads + k_heads, d->head_dim);
+  return sizeof(float) * ttt::rotary_partial_floats((int64_t)d->batch * d->seq_len, d->heads + k_heads, d->head_dim, d->dtype == TTT_F32);
 }
 
 extern "C" int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads, const void* q, const void* k, const void* grad_q_out,

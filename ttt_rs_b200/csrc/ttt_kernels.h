@@ -475,9 +475,9 @@ struct RotaryParams {
   int64_t pos_stride, start, tokens;     // tokens: B T
   int heads[2], T, F, rdim, wrap;
   float size, sign, eps;
-  int lanes, rows_each;                  // set by the launcher
+  int rows_each;                         // set by the launcher
 };
-size_t rotary_partial_floats(int64_t tokens, int rows, int F);
+size_t rotary_partial_floats(int64_t tokens, int rows, int F, bool f32);
 // vec: F and rdim multiples of 8, all rows on 16 bytes
 cudaError_t launch_rotary(int dtype, const RotaryParams& p, bool vec, bool half, bool norm, bool bwd, cudaStream_t st);
 

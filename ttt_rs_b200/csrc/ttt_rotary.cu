@@ -12,6 +12,8 @@
 // Memory-bound: 16 bytes per lane and row both ways.  A group of lanes that covers a row owns one token: it makes the token's
 // sines and cosines once and walks the heads of queries and keys with them, a few rows in flight.  Rows of a token's heads are
 // neighbours in [B,T,H,F], rows of neighbouring tokens (the other groups of the warp) in [B,H,T,F]: whole lines in both.
+#include <type_traits>
+
 #include "ttt_kernels.h"
 #include "ttt_common.cuh"
 
@@ -20,117 +22,89 @@ namespace ttt {
 constexpr int ROT_THREADS = 256;
 constexpr int ROT_ROWS = 4;  // rows in flight
 
-// V pairs of a row, NU times per lane (stride: the group).  V = 4: vectors of 4 or 8 elements; V = 1: any alignment.
-template <typename T, int V>
-struct PairIo;
-template <typename T>
-struct PairIo<T, 1> {
-  T a, b;
-  __device__ __forceinline__ void load(const T* p, int i, int j) { a = p[i], b = p[j]; }
-  __device__ __forceinline__ void unpack(float (&x)[1], float (&y)[1]) const { x[0] = (float)a, y[0] = (float)b; }
-  static __device__ __forceinline__ void store(T* p, int i, int j, const float (&x)[1], const float (&y)[1]) {
-    p[i] = (T)x[0];
-    p[j] = (T)y[0];
-  }
-};
-template <>
-struct PairIo<float, 4> {
-  float4 a, b;
-  __device__ __forceinline__ void load(const float* p, int i, int j) {
-    a = *reinterpret_cast<const float4*>(p + i);
-    b = *reinterpret_cast<const float4*>(p + j);
-  }
-  __device__ __forceinline__ void unpack(float (&x)[4], float (&y)[4]) const {
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, y[0] = b.x, y[1] = b.y, y[2] = b.z, y[3] = b.w;
-  }
-  static __device__ __forceinline__ void store(float* p, int i, int j, const float (&x)[4], const float (&y)[4]) {
-    *reinterpret_cast<float4*>(p + i) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(p + j) = make_float4(y[0], y[1], y[2], y[3]);
-  }
-};
-template <>
-struct PairIo<__nv_bfloat16, 4> {
-  uint2 a, b;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p, int i, int j) {
-    if (j == i + 4) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + i);
-      a = make_uint2(v.x, v.y);
-      b = make_uint2(v.z, v.w);
-    } else {
-      a = *reinterpret_cast<const uint2*>(p + i);
-      b = *reinterpret_cast<const uint2*>(p + j);
-    }
-  }
-  __device__ __forceinline__ void unpack(float (&x)[4], float (&y)[4]) const {
-    x[0] = bf16_lo(a.x), x[1] = bf16_hi(a.x), x[2] = bf16_lo(a.y), x[3] = bf16_hi(a.y);
-    y[0] = bf16_lo(b.x), y[1] = bf16_hi(b.x), y[2] = bf16_lo(b.y), y[3] = bf16_hi(b.y);
-  }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, int i, int j, const float (&x)[4], const float (&y)[4]) {
-    const uint2 a = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])), b = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-    if (j == i + 4) {
-      *reinterpret_cast<uint4*>(p + i) = make_uint4(a.x, a.y, b.x, b.y);
-    } else {
-      *reinterpret_cast<uint2*>(p + i) = a;
-      *reinterpret_cast<uint2*>(p + j) = b;
-    }
-  }
-};
-
-// Where the elements of a lane's unit lie in the row, and which of them belong to a pair: with x = elements at i.., y = at j..,
-// pairs are (x[k], y[k]) if `split` (halves) and (x[0], x[1]), (x[2], x[3]), (y[0], y[1]), .. if not (V = 1: (x, y) always)
+constexpr int rotary_resident(bool f32, bool norm, bool bwd) {  // blocks per SM that the kernels' registers are bounded for
+  return bwd ? (f32 ? 1 : 2) : f32 ? (norm ? 2 : 3) : norm ? 3 : 4;
+}
+// A unit is V pairs of a row, NU of them per lane (a group's lanes apart): x[k] and y[k] are the two features of pair k (V = 4: of
+// two pairs (x[0], x[1]) and (y[0], y[1]) side by side in registers, for the packed float32 operations).  Features behind the rotated
+// part come in units too, as pairs that are not turned.  V = 4 takes 16 bytes at a time, V = 1 single features at any address.
 template <int V, bool HALF>
 struct Unit {
-  int i, j, pair;  // pair: first pair, or -1: not rotated
+  int i, j, pair;  // elements of the row: V from i on and V from j on; first pair, or -1: not rotated
   bool live;
   __device__ __forceinline__ Unit(int u, int F, int r) {
     live = 2 * V * u < F;
     const bool rotated = 2 * V * u < r;
     pair = rotated ? V * u : -1;
-    if (HALF && rotated) {
-      i = V * u;
-      j = r / 2 + V * u;
+    i = HALF && rotated ? V * u : 2 * V * u;
+    j = HALF && rotated ? r / 2 + V * u : i + V;
+  }
+};
+template <typename T, int V, bool HALF>
+struct Pairs;
+template <typename T, bool HALF>
+struct Pairs<T, 1, HALF> {
+  T a, b;
+  __device__ __forceinline__ void load(const T* p, const Unit<1, HALF>& u) { a = p[u.i], b = p[u.j]; }
+  __device__ __forceinline__ void unpack(F2 (&x)[1], F2 (&y)[1]) const { x[0] = f2((float)a, 0.f), y[0] = f2((float)b, 0.f); }
+  static __device__ __forceinline__ void store(T* p, const Unit<1, HALF>& u, const F2 (&x)[1], const F2 (&y)[1]) {
+    p[u.i] = (T)x[0].x;
+    p[u.j] = (T)y[0].x;
+  }
+};
+template <bool HALF>
+struct Pairs<float, 4, HALF> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p, const Unit<4, HALF>& u) {
+    a = *reinterpret_cast<const float4*>(p + u.i);
+    b = *reinterpret_cast<const float4*>(p + u.j);
+  }
+  __device__ __forceinline__ void unpack(F2 (&x)[2], F2 (&y)[2]) const {
+    if constexpr (HALF) x[0] = f2(a.x, a.y), x[1] = f2(a.z, a.w), y[0] = f2(b.x, b.y), y[1] = f2(b.z, b.w);
+    else x[0] = f2(a.x, a.z), y[0] = f2(a.y, a.w), x[1] = f2(b.x, b.z), y[1] = f2(b.y, b.w);
+  }
+  static __device__ __forceinline__ void store(float* p, const Unit<4, HALF>& u, const F2 (&x)[2], const F2 (&y)[2]) {
+    float4 a, b;
+    if constexpr (HALF) a = make_float4(x[0].x, x[0].y, x[1].x, x[1].y), b = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+    else a = make_float4(x[0].x, y[0].x, x[0].y, y[0].y), b = make_float4(x[1].x, y[1].x, x[1].y, y[1].y);
+    *reinterpret_cast<float4*>(p + u.i) = a;
+    *reinterpret_cast<float4*>(p + u.j) = b;
+  }
+};
+template <bool HALF>
+struct Pairs<__nv_bfloat16, 4, HALF> {
+  uint2 a, b;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, const Unit<4, HALF>& u) {
+    if constexpr (HALF) {
+      a = *reinterpret_cast<const uint2*>(p + u.i);
+      b = *reinterpret_cast<const uint2*>(p + u.j);
     } else {
-      i = 2 * V * u;
-      j = i + V;
+      const uint4 v = *reinterpret_cast<const uint4*>(p + u.i);
+      a = make_uint2(v.x, v.y);
+      b = make_uint2(v.z, v.w);
+    }
+  }
+  __device__ __forceinline__ void unpack(F2 (&x)[2], F2 (&y)[2]) const {
+    if constexpr (HALF) {
+      x[0] = f2(bf16_lo(a.x), bf16_hi(a.x)), x[1] = f2(bf16_lo(a.y), bf16_hi(a.y));
+      y[0] = f2(bf16_lo(b.x), bf16_hi(b.x)), y[1] = f2(bf16_lo(b.y), bf16_hi(b.y));
+    } else {
+      x[0] = f2(bf16_lo(a.x), bf16_lo(a.y)), y[0] = f2(bf16_hi(a.x), bf16_hi(a.y));
+      x[1] = f2(bf16_lo(b.x), bf16_lo(b.y)), y[1] = f2(bf16_hi(b.x), bf16_hi(b.y));
+    }
+  }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, const Unit<4, HALF>& u, const F2 (&x)[2], const F2 (&y)[2]) {
+    if constexpr (HALF) {
+      *reinterpret_cast<uint2*>(p + u.i) = make_uint2(pack_bf16(x[0].x, x[0].y), pack_bf16(x[1].x, x[1].y));
+      *reinterpret_cast<uint2*>(p + u.j) = make_uint2(pack_bf16(y[0].x, y[0].y), pack_bf16(y[1].x, y[1].y));
+    } else {
+      *reinterpret_cast<uint4*>(p + u.i) = make_uint4(pack_bf16(x[0].x, y[0].x), pack_bf16(x[0].y, y[0].y), pack_bf16(x[1].x, y[1].x),
+                                                      pack_bf16(x[1].y, y[1].y));
     }
   }
 };
-template <int V, bool HALF>
-__device__ __forceinline__ void rotate(float (&x)[V], float (&y)[V], const float (&c)[V], const float (&s)[V]) {
-  if constexpr (HALF || V == 1) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float a = x[k], b = y[k];
-      x[k] = a * c[k] - b * s[k];
-      y[k] = b * c[k] + a * s[k];
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < V; k += 2) {
-      const float a = x[k], b = x[k + 1], d = y[k], e = y[k + 1];
-      x[k] = a * c[k / 2] - b * s[k / 2];
-      x[k + 1] = b * c[k / 2] + a * s[k / 2];
-      y[k] = d * c[V / 2 + k / 2] - e * s[V / 2 + k / 2];
-      y[k + 1] = e * c[V / 2 + k / 2] + d * s[V / 2 + k / 2];
-    }
-  }
-}
-template <int V>
-__device__ __forceinline__ void sines(float (&c)[V], float (&s)[V], const RotaryParams& p, int64_t pos, int pair) {
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    c[k] = 1.f;
-    s[k] = 0.f;
-    if (pair >= 0) {
-      const uint64_t turn = (uint64_t)pos * p.turns[pair + k];
-      sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s[k], &c[k]);
-      c[k] *= p.size;
-      s[k] *= p.sign * p.size;
-    }
-  }
-}
-__device__ __forceinline__ int64_t position(const RotaryParams& p, int64_t token, int T) {
-  const int64_t b = token / T, t = token - b * T;
+
+__device__ __forceinline__ int64_t position(const RotaryParams& p, int64_t b, int64_t t) {
   int64_t pos = p.positions != nullptr ? p.positions[b * p.pos_stride + t] : p.start + t;
   if (p.wrap > 0) {
     pos %= p.wrap;
@@ -138,29 +112,53 @@ __device__ __forceinline__ int64_t position(const RotaryParams& p, int64_t token
   }
   return pos;
 }
-__device__ __forceinline__ float group_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+__device__ __forceinline__ float2 turn(const RotaryParams& p, int64_t pos, int pair) {  // cosine and sine, of the results' size
+  const uint64_t t = (uint64_t)pos * p.turns[pair];
+  float c, s;
+  sincospif((float)(int32_t)(t >> 32) * 0x1p-31f, &s, &c);
+  return make_float2(c * p.size, s * p.sign * p.size);
+}
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
 // NORM: the norm before the rotation.  BWD (with NORM): its gradient.
-template <typename T, int V, int NU, bool HALF, bool NORM, bool BWD>
-__global__ void __launch_bounds__(ROT_THREADS) ttt_rotary_kernel(const RotaryParams p) {
-  const int lanes = p.lanes, tid = threadIdx.x, sub = tid & (lanes - 1), groups = ROT_THREADS / lanes;
-  const int rows = p.heads[0] + p.heads[1];
-  const int r_lo = (int)blockIdx.y * p.rows_each, r_hi = min(rows, r_lo + p.rows_each);
+template <typename T, int V, int NU, int LANES, bool HALF, bool NORM, bool BWD>
+__global__ void __launch_bounds__(ROT_THREADS, rotary_resident(sizeof(T) == 4, NORM, BWD))
+    ttt_rotary_kernel(const RotaryParams p) {
+  constexpr int H = V == 1 ? 1 : V / 2;  // pairs of pairs
+  using Io = Pairs<T, V, HALF>;
+  using Un = Unit<V, HALF>;
+  constexpr int groups = ROT_THREADS / LANES;
+  const int tid = threadIdx.x, sub = tid & (LANES - 1);
+  const int r_lo = (int)blockIdx.y * p.rows_each, r_hi = min(p.heads[0] + p.heads[1], r_lo + p.rows_each);
   const float inv_f = 1.f / p.F;
-  float wgt[NORM ? 2 : 1][NU][2 * V], dw[BWD ? 2 : 1][NU][2 * V];
+  F2 wx[NORM ? 2 : 1][NU][H], wy[NORM ? 2 : 1][NU][H], dx[BWD ? 2 : 1][NU][H], dy[BWD ? 2 : 1][NU][H];
   if constexpr (NORM) {
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int n = 0; n < NU; ++n) {
-        const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
+        const Un u(sub + LANES * n, p.F, p.rdim);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          wgt[m][n][k] = u.live && p.w[m] != nullptr ? ld_as_float<T>(p.w[m], u.i + k) : 1.f;
-          wgt[m][n][V + k] = u.live && p.w[m] != nullptr ? ld_as_float<T>(p.w[m], u.j + k) : 1.f;
+        for (int k = 0; k < H; ++k) wx[m][n][k] = wy[m][n][k] = f2(1.f);
+        if (u.live && p.w[m] != nullptr) {
+          if constexpr (V == 1) {
+            wx[m][n][0].x = ld_as_float<T>(p.w[m], u.i);
+            wy[m][n][0].x = ld_as_float<T>(p.w[m], u.j);
+          } else {
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = ld_as_float<T>(p.w[m], u.i + k), e[4 + k] = ld_as_float<T>(p.w[m], u.j + k);
+            if constexpr (HALF) {
+              wx[m][n][0] = f2(e[0], e[1]), wx[m][n][H - 1] = f2(e[2], e[3]), wy[m][n][0] = f2(e[4], e[5]), wy[m][n][H - 1] = f2(e[6], e[7]);
+            } else {
+              wx[m][n][0] = f2(e[0], e[2]), wy[m][n][0] = f2(e[1], e[3]), wx[m][n][H - 1] = f2(e[4], e[6]), wy[m][n][H - 1] = f2(e[5], e[7]);
+            }
+          }
         }
       }
   }
@@ -170,122 +168,150 @@ __global__ void __launch_bounds__(ROT_THREADS) ttt_rotary_kernel(const RotaryPar
 #pragma unroll
       for (int n = 0; n < NU; ++n)
 #pragma unroll
-        for (int k = 0; k < 2 * V; ++k) dw[m][n][k] = 0.f;
+        for (int k = 0; k < H; ++k) dx[m][n][k] = dy[m][n][k] = f2(0.f);
   }
   // whole groups of a warp take part in its shuffles to the end: a group without a token works on the last one and stores nothing
   for (int64_t first = (int64_t)blockIdx.x * groups; first < p.tokens; first += (int64_t)gridDim.x * groups) {
-    const bool has = first + tid / lanes < p.tokens;
-    const int64_t token = has ? first + tid / lanes : p.tokens - 1;
+    const bool has = first + tid / LANES < p.tokens;
+    const int64_t token = has ? first + tid / LANES : p.tokens - 1;
     const int64_t b = token / p.T, t = token - b * p.T;
-    float c[NU][V], s[NU][V];
-    const int64_t pos = p.rdim > 0 ? position(p, token, p.T) : 0;
+    F2 c[NU][H], s[NU][H];
+    const int64_t pos = p.rdim > 0 ? position(p, b, t) : 0;
 #pragma unroll
-    for (int n = 0; n < NU; ++n) sines<V>(c[n], s[n], p, pos, Unit<V, HALF>(sub + lanes * n, p.F, p.rdim).pair);
-    for (int row0 = r_lo; row0 < r_hi; row0 += ROT_ROWS) {
-      PairIo<T, V> in[ROT_ROWS][NU], grad[BWD ? ROT_ROWS : 1][NU];
+    for (int n = 0; n < NU; ++n) {
+      const Un u(sub + LANES * n, p.F, p.rdim);
 #pragma unroll
-      for (int q = 0; q < ROT_ROWS; ++q) {
-        const int row = min(row0 + q, r_hi - 1), m = row >= p.heads[0], h = row - (m ? p.heads[0] : 0);
-        const T* src = static_cast<const T*>(p.x[m]) + (b * p.xs[m][0] + h * p.xs[m][1] + t * p.xs[m][2]);
-#pragma unroll
-        for (int n = 0; n < NU; ++n) {
-          const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
-          if (u.live) in[q][n].load(src, u.i, u.j);
-        }
-        if constexpr (BWD) {
-          const T* g = static_cast<const T*>(p.g[m]) + (b * p.gs[m][0] + h * p.gs[m][1] + t * p.gs[m][2]);
-#pragma unroll
-          for (int n = 0; n < NU; ++n) {
-            const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
-            if (u.live) grad[q][n].load(g, u.i, u.j);
-          }
+      for (int k = 0; k < H; ++k) {
+        c[n][k] = f2(1.f);
+        s[n][k] = f2(0.f);
+        if (u.pair >= 0) {
+          const float2 e = turn(p, pos, u.pair + 2 * k), f = V == 1 ? e : turn(p, pos, u.pair + 2 * k + 1);
+          c[n][k] = f2(e.x, f.x);
+          s[n][k] = f2(e.y, f.y);
         }
       }
+    }
 #pragma unroll
-      for (int q = 0; q < ROT_ROWS; ++q) {
-        if (row0 + q >= r_hi) break;
-        const int row = row0 + q, m = row >= p.heads[0], h = row - (m ? p.heads[0] : 0);
-        T* dst = static_cast<T*>(p.y[m]) + (b * p.ys[m][0] + h * p.ys[m][1] + t * p.ys[m][2]);
-        float x[NU][V], y[NU][V];
-        float sq = 0.f;
+    for (int m = 0; m < 2; ++m) {
+      const int off = m ? p.heads[0] : 0, h_lo = max(r_lo - off, 0), h_hi = min(r_hi - off, p.heads[m]);
+      if (h_lo >= h_hi) continue;
+      const T* src = static_cast<const T*>(p.x[m]) + (b * p.xs[m][0] + h_lo * p.xs[m][1] + t * p.xs[m][2]);
+      const T* grd = BWD ? static_cast<const T*>(p.g[m]) + (b * p.gs[m][0] + h_lo * p.gs[m][1] + t * p.gs[m][2]) : nullptr;
+      T* dst = static_cast<T*>(p.y[m]) + (b * p.ys[m][0] + h_lo * p.ys[m][1] + t * p.ys[m][2]);
+      auto rows = [&](auto count) {  // so many rows, all of them on their way before the first is worked on
+        constexpr int ROWS = decltype(count)::value;
+        Io in[ROWS][NU], grad[BWD ? ROWS : 1][NU];
 #pragma unroll
-        for (int n = 0; n < NU; ++n) {
-          const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
-          if (u.live) in[q][n].unpack(x[n], y[n]);
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            if (!u.live) x[n][k] = y[n][k] = 0.f;
-            if (NORM) sq = fmaf(x[n][k], x[n][k], fmaf(y[n][k], y[n][k], sq));
-          }
-        }
-        float r = 1.f;
-        if constexpr (NORM) r = rsqrtf(group_sum(sq, lanes) * inv_f + p.eps);
-        if constexpr (!BWD) {
+        for (int q = 0; q < ROWS; ++q) {
 #pragma unroll
           for (int n = 0; n < NU; ++n) {
-            const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
-            if constexpr (NORM) {
+            const Un u(sub + LANES * n, p.F, p.rdim);
+            if (u.live) in[q][n].load(src, u);
+            if constexpr (BWD) {
+              if (u.live) grad[q][n].load(grd, u);
+            }
+          }
+          src += p.xs[m][1];
+          if constexpr (BWD) grd += p.gs[m][1];
+        }
 #pragma unroll
-              for (int k = 0; k < V; ++k) {
-                x[n][k] *= r * (m ? wgt[1][n][k] : wgt[0][n][k]);
-                y[n][k] *= r * (m ? wgt[1][n][V + k] : wgt[0][n][V + k]);
+        for (int q = 0; q < ROWS; ++q) {
+          {
+            F2 x[NU][H], y[NU][H], sq = f2(0.f);
+#pragma unroll
+            for (int n = 0; n < NU; ++n) {
+              const Un u(sub + LANES * n, p.F, p.rdim);
+#pragma unroll
+              for (int k = 0; k < H; ++k) x[n][k] = y[n][k] = f2(0.f);
+              if (u.live) in[q][n].unpack(x[n], y[n]);
+              if constexpr (NORM) {
+#pragma unroll
+                for (int k = 0; k < H; ++k) sq = f2fma(x[n][k], x[n][k], f2fma(y[n][k], y[n][k], sq));
               }
             }
-            rotate<V, HALF>(x[n], y[n], c[n], s[n]);
-            if (u.live && has) PairIo<T, V>::store(dst, u.i, u.j, x[n], y[n]);
-          }
-        } else {
-          float gx[NU][V], gy[NU][V], dot = 0.f;
+            float r = 1.f;
+            if constexpr (NORM) r = rsqrtf(group_sum<LANES>(f2hsum(sq)) * inv_f + p.eps);
+            if constexpr (!BWD) {
 #pragma unroll
-          for (int n = 0; n < NU; ++n) {
-            const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
-            if (u.live) grad[q][n].unpack(gx[n], gy[n]);
+              for (int n = 0; n < NU; ++n) {
+                const Un u(sub + LANES * n, p.F, p.rdim);
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-              if (!u.live) gx[n][k] = gy[n][k] = 0.f;
-            rotate<V, HALF>(gx[n], gy[n], c[n], s[n]);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-              const float ax = gx[n][k] * x[n][k] * r, ay = gy[n][k] * y[n][k] * r;
-              if (has) {
-                dw[0][n][k] += m ? 0.f : ax;
-                dw[0][n][V + k] += m ? 0.f : ay;
-                dw[1][n][k] += m ? ax : 0.f;
-                dw[1][n][V + k] += m ? ay : 0.f;
+                for (int k = 0; k < H; ++k) {
+                  if constexpr (NORM) {
+                    x[n][k] = f2mul(x[n][k], f2mul(wx[m][n][k], f2(r)));
+                    y[n][k] = f2mul(y[n][k], f2mul(wy[m][n][k], f2(r)));
+                  }
+                  const F2 a = f2fma(x[n][k], c[n][k], f2neg(f2mul(y[n][k], s[n][k])));
+                  y[n][k] = f2fma(y[n][k], c[n][k], f2mul(x[n][k], s[n][k]));
+                  x[n][k] = a;
+                }
+                if (u.live && has) Io::store(dst, u, x[n], y[n]);
               }
-              gx[n][k] *= m ? wgt[1][n][k] : wgt[0][n][k];
-              gy[n][k] *= m ? wgt[1][n][V + k] : wgt[0][n][V + k];
-              dot = fmaf(gx[n][k], x[n][k], fmaf(gy[n][k], y[n][k], dot));
+            } else {
+              F2 gx[NU][H], gy[NU][H], dot = f2(0.f);
+#pragma unroll
+              for (int n = 0; n < NU; ++n) {
+                const Un u(sub + LANES * n, p.F, p.rdim);
+#pragma unroll
+                for (int k = 0; k < H; ++k) gx[n][k] = gy[n][k] = f2(0.f);
+                if (u.live && has) grad[q][n].unpack(gx[n], gy[n]);
+#pragma unroll
+                for (int k = 0; k < H; ++k) {
+                  const F2 a = f2fma(gx[n][k], c[n][k], f2neg(f2mul(gy[n][k], s[n][k])));
+                  const F2 e = f2fma(gy[n][k], c[n][k], f2mul(gx[n][k], s[n][k]));
+                  const F2 px = f2mul(a, x[n][k]), py = f2mul(e, y[n][k]);
+                  dx[m][n][k] = f2fma(px, f2(r), dx[m][n][k]);
+                  dy[m][n][k] = f2fma(py, f2(r), dy[m][n][k]);
+                  dot = f2fma(px, wx[m][n][k], f2fma(py, wy[m][n][k], dot));
+                  gx[n][k] = f2mul(a, wx[m][n][k]);
+                  gy[n][k] = f2mul(e, wy[m][n][k]);
+                }
+              }
+              const float f = -group_sum<LANES>(f2hsum(dot)) * inv_f * r * r * r;
+#pragma unroll
+              for (int n = 0; n < NU; ++n) {
+                const Un u(sub + LANES * n, p.F, p.rdim);
+#pragma unroll
+                for (int k = 0; k < H; ++k) {
+                  gx[n][k] = f2fma(gx[n][k], f2(r), f2mul(x[n][k], f2(f)));
+                  gy[n][k] = f2fma(gy[n][k], f2(r), f2mul(y[n][k], f2(f)));
+                }
+                if (u.live && has) Io::store(dst, u, gx[n], gy[n]);
+              }
             }
           }
-          const float f = group_sum(dot, lanes) * inv_f * r * r * r;
-#pragma unroll
-          for (int n = 0; n < NU; ++n) {
-            const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-              gx[n][k] = r * gx[n][k] - f * x[n][k];
-              gy[n][k] = r * gy[n][k] - f * y[n][k];
-            }
-            if (u.live && has) PairIo<T, V>::store(dst, u.i, u.j, gx[n], gy[n]);
-          }
+          dst += p.ys[m][1];
         }
-      }
+      };
+      int h = h_lo;
+      for (; h + ROT_ROWS <= h_hi; h += ROT_ROWS) rows(std::integral_constant<int, ROT_ROWS>{});
+      for (; h < h_hi; ++h) rows(std::integral_constant<int, 1>{});
     }
   }
   if constexpr (BWD) {  // this block's share of the weights' gradients, in a fixed order: groups of a warp, warps, blocks
     if (p.partials == nullptr) return;
     extern __shared__ float rot_smem[];  // [warps][2][F]
+    auto put = [&](int m, int at, float v, bool live) {
+#pragma unroll
+      for (int o = LANES; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (live && (tid & 31) < LANES) rot_smem[((tid >> 5) * 2 + m) * p.F + at] = v;
+    };
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
       for (int n = 0; n < NU; ++n) {
-        const Unit<V, HALF> u(sub + lanes * n, p.F, p.rdim);
+        const Un u(sub + LANES * n, p.F, p.rdim);
+        if constexpr (V == 1) {
+          put(m, u.i, dx[m][n][0].x, u.live);
+          put(m, u.j, dy[m][n][0].x, u.live);
+        } else {
 #pragma unroll
-        for (int k = 0; k < 2 * V; ++k) {
-          float v = dw[m][n][k];
-          for (int o = lanes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-          if (u.live && (tid & 31) < lanes) rot_smem[((tid >> 5) * 2 + m) * p.F + (k < V ? u.i + k : u.j + k - V)] = v;
+          for (int k = 0; k < 2; ++k) {
+            put(m, HALF ? u.i + 2 * k : (k ? u.j : u.i), dx[m][n][k].x, u.live);
+            put(m, HALF ? u.i + 2 * k + 1 : (k ? u.j : u.i) + 2, dx[m][n][k].y, u.live);
+            put(m, HALF ? u.j + 2 * k : (k ? u.j : u.i) + 1, dy[m][n][k].x, u.live);
+            put(m, HALF ? u.j + 2 * k + 1 : (k ? u.j : u.i) + 3, dy[m][n][k].y, u.live);
+          }
         }
       }
     __syncthreads();
@@ -313,63 +339,76 @@ __global__ void __launch_bounds__(256) ttt_rotary_reduce_kernel(const float* par
   if (out != nullptr) st_from_float<T>(out, col < F ? col : col - F, v);
 }
 
-// Blocks: tokens of groups of lanes, and the rows of a token in as many shares as it takes to fill the card
+// Lanes of a row: with vectors a lane per 8 features, else the whole warp
+static int rotary_lanes(int F, bool vec) {
+  if (!vec || F > 128) return 32;
+  return F > 64 ? 16 : F > 32 ? 8 : 4;
+}
+// Blocks of tokens (x) and shares of a token's rows (y).  More shares than one where the tokens do not fill the card, or where the
+// last round of blocks would run half empty: a share costs its rows and, for the sines, about ROT_SETUP more, and the rounds
+// count.  (32768 tokens of 32 rows: 2 shares in 3.5 rounds 57.8 us, 4 in 6.9 rounds less.)  The gradient's blocks are no more than are
+// resident, since each leaves a row of partial sums.
+constexpr int ROT_SETUP = 4;
 struct RotaryGrid {
-  int x, y, rows_each, lanes;
+  int x, y, rows_each;
 };
-static RotaryGrid rotary_grid(int64_t tokens, int rows, int F, bool vec, bool bwd) {
-  RotaryGrid g;
-  const int units = vec ? F / 8 : F / 2;
-  g.lanes = 1;
-  while (g.lanes < units && g.lanes < 32) g.lanes *= 2;
-  const int groups = ROT_THREADS / g.lanes;
-  const int64_t blocks = (tokens + groups - 1) / groups;
-  constexpr int FILL = 148 * 8;
-  int64_t shares = (FILL + blocks - 1) / blocks;
-  const int most = (rows + ROT_ROWS - 1) / ROT_ROWS;
-  if (shares > most) shares = most;
-  g.rows_each = (int)((rows + shares - 1) / shares);
-  g.y = (rows + g.rows_each - 1) / g.rows_each;
-  int64_t x = blocks;
-  const int64_t cap = bwd ? (FILL + g.y - 1) / g.y : (int64_t)1 << 30;
-  if (x > cap) x = cap;
-  g.x = (int)x;
+static RotaryGrid rotary_grid(int64_t tokens, int rows, int F, bool vec, int resident, bool bwd) {
+  RotaryGrid g{};
+  const int groups = ROT_THREADS / rotary_lanes(F, vec);
+  const int64_t blocks = (tokens + groups - 1) / groups, most = 148 * resident;
+  int64_t least = -1;
+  for (int each = rows; each >= 1; each = each > ROT_ROWS ? (each - 1) / ROT_ROWS * ROT_ROWS : each > 1 ? 1 : 0) {
+    const int64_t shares = (rows + each - 1) / each;
+    if (bwd && shares > most) break;
+    const int64_t cost = (blocks * shares + most - 1) / most * (each + ROT_SETUP);
+    if (least >= 0 && cost >= least) continue;
+    least = cost;
+    g.rows_each = each;
+    g.y = (int)shares;
+  }
+  const int64_t cap = bwd ? most / g.y : (int64_t)1 << 30;
+  g.x = (int)(blocks < cap ? blocks : cap);
   return g;
 }
-size_t rotary_partial_floats(int64_t tokens, int rows, int F) {
+size_t rotary_partial_floats(int64_t tokens, int rows, int F, bool f32) {
   size_t most = 0;
   for (bool vec : {false, true}) {  // (which of them runs depends on addresses)
     if (vec && F % 8 != 0) continue;
-    const RotaryGrid g = rotary_grid(tokens, rows, F, vec, true);
+    const RotaryGrid g = rotary_grid(tokens, rows, F, vec, rotary_resident(f32, true, true), true);
     const size_t n = (size_t)g.x * g.y * 2 * F;
     if (n > most) most = n;
   }
   return most;
 }
 
-template <typename T, int V, int NU, bool HALF>
+template <typename T, int V, int NU, int LANES, bool HALF>
 static cudaError_t launch_rot(RotaryParams p, bool norm, bool bwd, cudaStream_t st) {
-  const RotaryGrid g = rotary_grid(p.tokens, p.heads[0] + p.heads[1], p.F, V == 4, bwd);
+  const RotaryGrid g = rotary_grid(p.tokens, p.heads[0] + p.heads[1], p.F, V == 4, rotary_resident(sizeof(T) == 4, norm, bwd), bwd);
   p.rows_each = g.rows_each;
-  p.lanes = g.lanes;
   const dim3 grid(g.x, g.y);
   const size_t smem = bwd ? (ROT_THREADS / 32) * 2 * p.F * sizeof(float) : 0;
-  if (!norm) ttt_rotary_kernel<T, V, NU, HALF, false, false><<<grid, ROT_THREADS, 0, st>>>(p);
-  else if (!bwd) ttt_rotary_kernel<T, V, NU, HALF, true, false><<<grid, ROT_THREADS, 0, st>>>(p);
-  else ttt_rotary_kernel<T, V, NU, HALF, true, true><<<grid, ROT_THREADS, smem, st>>>(p);
+  if (!norm) ttt_rotary_kernel<T, V, NU, LANES, HALF, false, false><<<grid, ROT_THREADS, 0, st>>>(p);
+  else if (!bwd) ttt_rotary_kernel<T, V, NU, LANES, HALF, true, false><<<grid, ROT_THREADS, 0, st>>>(p);
+  else ttt_rotary_kernel<T, V, NU, LANES, HALF, true, true><<<grid, ROT_THREADS, smem, st>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !bwd || p.partials == nullptr) return e;
   ttt_rotary_reduce_kernel<T><<<(2 * p.F + 7) / 8, 256, 0, st>>>(p.partials, g.x * g.y, p.F, static_cast<T*>(p.dw[0]),
                                                                 static_cast<T*>(p.dw[1]));
   return cudaGetLastError();
 }
-template <typename T>
-static cudaError_t launch_rot_t(const RotaryParams& p, bool vec, bool half, bool norm, bool bwd, cudaStream_t st) {
-  if (vec) return half ? launch_rot<T, 4, 1, true>(p, norm, bwd, st) : launch_rot<T, 4, 1, false>(p, norm, bwd, st);
-  return half ? launch_rot<T, 1, 4, true>(p, norm, bwd, st) : launch_rot<T, 1, 4, false>(p, norm, bwd, st);
+template <typename T, bool HALF>
+static cudaError_t launch_rot_t(const RotaryParams& p, bool vec, bool norm, bool bwd, cudaStream_t st) {
+  if (!vec) return launch_rot<T, 1, 4, 32, HALF>(p, norm, bwd, st);
+  switch (rotary_lanes(p.F, true)) {
+    case 4: return launch_rot<T, 4, 1, 4, HALF>(p, norm, bwd, st);
+    case 8: return launch_rot<T, 4, 1, 8, HALF>(p, norm, bwd, st);
+    case 16: return launch_rot<T, 4, 1, 16, HALF>(p, norm, bwd, st);
+    default: return launch_rot<T, 4, 1, 32, HALF>(p, norm, bwd, st);
+  }
 }
 cudaError_t launch_rotary(int dtype, const RotaryParams& p, bool vec, bool half, bool norm, bool bwd, cudaStream_t st) {
-  return dtype == 1 ? launch_rot_t<__nv_bfloat16>(p, vec, half, norm, bwd, st) : launch_rot_t<float>(p, vec, half, norm, bwd, st);
+  if (half) return dtype == 1 ? launch_rot_t<__nv_bfloat16, true>(p, vec, norm, bwd, st) : launch_rot_t<float, true>(p, vec, norm, bwd, st);
+  return dtype == 1 ? launch_rot_t<__nv_bfloat16, false>(p, vec, norm, bwd, st) : launch_rot_t<float, false>(p, vec, norm, bwd, st);
 }
 
 }  // namespace ttt

@@ -103,6 +103,8 @@ INTERNAL = {
     "ttt_internal_layer_projections": (C.c_int, [_DP, _P, C.c_int64, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int64,
                                                  C.c_int64, C.c_int64, C.c_int64, C.c_int64, _P, C.c_int, C.c_int,
                                                  C.c_float, C.c_float, C.c_int] + [_P] * 10),
+    "ttt_internal_layer_values": (C.c_int, [_DP, _P, C.c_int64, _P, C.c_int64, _P, C.c_float, _P, _P, _P]),
+    "ttt_internal_layer_values_backward": (C.c_int, [_DP, _P, _P, _P, C.c_float, _P, C.c_int64, _P, C.c_int64, C.c_int, _P]),
 }
 
 NOALLOC_SCRATCH_BYTES = 32 << 20  # TTT_NOALLOC_SCRATCH_BYTES

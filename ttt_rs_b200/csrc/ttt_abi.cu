@@ -1661,3 +1661,67 @@ extern "C" int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads,
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "norm and rotation backward launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;
 }
+
+extern "C" int ttt_internal_layer_values(const ttt_dims* d, const void* v_src, int64_t src_ld, const void* lr_logits, int64_t lr_ld,
+                                         const void* lr_bias, float base_lr, void* xv, void* ttt_lr_eta, void* stream) {
+  int rc = check_layer_dims(d);
+  if (rc != TTT_OK) return rc;
+  if (src_ld < (int64_t)d->heads * d->head_dim || (src_ld & 7) != 0)
+    return fail(TTT_ERR_SHAPE, "src_ld (%lld) must be >= heads*head_dim and a multiple of 8", (long long)src_ld);
+  if (lr_ld < d->heads) return fail(TTT_ERR_SHAPE, "lr_ld (%lld) must be >= heads", (long long)lr_ld);
+  const NamedPtr ptrs[] = {{"v_src", v_src}, {"xv", xv}};
+  if ((rc = check_ptrs(ptrs, 2)) != TTT_OK) return rc;
+  if (lr_logits == nullptr || ttt_lr_eta == nullptr) return fail(TTT_ERR_NULL, "lr_logits / ttt_lr_eta is null");
+  ttt::LayerProParams p{};
+  p.v_src = v_src;
+  p.ld_src = (long)src_ld;
+  p.lr_logits = lr_logits;
+  p.ld_lr = (long)lr_ld;
+  p.lr_bias = lr_bias;
+  p.xv = xv;
+  p.lr_out = ttt_lr_eta;
+  p.lr_ld_out = d->seq_len;
+  p.B = d->batch;
+  p.H = d->heads;
+  p.T = d->seq_len;
+  p.pos_mod = 1;
+  p.rope_theta = 1.f;
+  p.base_lr = base_lr;
+  const cudaError_t e = ttt::launch_layer_prologue(d->dtype, d->head_dim, p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "layer values launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}
+
+extern "C" int ttt_internal_layer_values_backward(const ttt_dims* d, const void* grad_xv, const void* grad_ttt_lr_eta,
+                                                  const void* ttt_lr_eta, float base_lr, void* grad_v_dst, int64_t dst_ld,
+                                                  void* grad_lr_logits, int64_t lr_ld, int lr_cols, void* stream) {
+  int rc = check_layer_dims(d);
+  if (rc != TTT_OK) return rc;
+  if (!(base_lr != 0.f)) return fail(TTT_ERR_SHAPE, "base_lr must be non-zero");
+  if (dst_ld < (int64_t)d->heads * d->head_dim || (dst_ld & 7) != 0)
+    return fail(TTT_ERR_SHAPE, "dst_ld (%lld) must be >= heads*head_dim and a multiple of 8", (long long)dst_ld);
+  if (lr_cols < d->heads || lr_ld < lr_cols)
+    return fail(TTT_ERR_SHAPE, "need heads <= lr_cols <= lr_ld (got lr_cols=%d, lr_ld=%lld)", lr_cols, (long long)lr_ld);
+  const NamedPtr ptrs[] = {{"grad_xv", grad_xv}, {"grad_v_dst", grad_v_dst}};
+  if ((rc = check_ptrs(ptrs, 2)) != TTT_OK) return rc;
+  if (grad_ttt_lr_eta == nullptr || ttt_lr_eta == nullptr || grad_lr_logits == nullptr)
+    return fail(TTT_ERR_NULL, "grad_ttt_lr_eta / ttt_lr_eta / grad_lr_logits is null");
+  ttt::LayerProBwdParams p{};
+  p.dxv = grad_xv;
+  p.dlr = grad_ttt_lr_eta;
+  p.lr = ttt_lr_eta;
+  p.dv_dst = grad_v_dst;
+  p.ld_dst = (long)dst_ld;
+  p.dlogits_dst = grad_lr_logits;
+  p.ld_dlr = (long)lr_ld;
+  p.lr_cols = lr_cols;
+  p.B = d->batch;
+  p.H = d->heads;
+  p.T = d->seq_len;
+  p.pos_mod = 1;
+  p.rope_theta = 1.f;
+  p.base_lr = base_lr;
+  const cudaError_t e = ttt::launch_layer_prologue_bwd(d->dtype, d->head_dim, p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "layer values backward launch failed: %s", cudaGetErrorString(e));
+  return TTT_OK;
+}

@@ -77,4 +77,12 @@ int ttt_internal_layer_small_out(const ttt_dims* d, const void* inner_out, const
                                  const void* post_norm_weight, const void* post_norm_bias, float eps, const void* o_proj,
                                  int64_t o_ld, void* y, void* stream);
 
+// ttt_layer_prologue's values and learning rates alone, and their gradients: for a layer whose queries and keys go through
+// ttt_layer_qk_norm_rotary or ttt_layer_rotary.
+int ttt_internal_layer_values(const ttt_dims* d, const void* v_src, int64_t src_ld, const void* lr_logits, int64_t lr_ld,
+                              const void* lr_bias, float base_lr, void* xv, void* ttt_lr_eta, void* stream);
+int ttt_internal_layer_values_backward(const ttt_dims* d, const void* grad_xv, const void* grad_ttt_lr_eta, const void* ttt_lr_eta,
+                                       float base_lr, void* grad_v_dst, int64_t dst_ld, void* grad_lr_logits, int64_t lr_ld,
+                                       int lr_cols, void* stream);
+
 }  // extern "C"

@@ -80,7 +80,8 @@ constexpr int PRO_MAXPOS = 64;   // rotary table rows (positions modulo the mini
 // used (memory-level parallelism).
 constexpr int PRO_TG = 4;
 
-template <typename T, bool CONV, int FD>
+// QK false: values and learning rates only (queries and keys go through the norm and rotation of ttt_rotary.cu).
+template <typename T, bool CONV, int FD, bool QK>
 __global__ void __launch_bounds__(PRO_THREADS, (CONV || sizeof(T) == 4) ? 1 : 3) ttt_layer_prologue_kernel(const LayerProParams p) {
   __shared__ float2 rope_tab[PRO_MAXPOS][32];  // (cos, sin) per position and pair (the first FD/2 pairs are used)
   constexpr int F = FD, SUBS = FD / 8, HPW = 32 / SUBS;
@@ -157,8 +158,8 @@ __global__ void __launch_bounds__(PRO_THREADS, (CONV || sizeof(T) == 4) ? 1 : 3)
       for (int u = 0; u < PRO_TG; ++u) {
         if (tb + u < t1) {
           const size_t srow = ((size_t)b * NT + tb + u) * p.ld_src + col;
-          vq[u].load(static_cast<const T*>(p.q_src) + srow);
-          if constexpr (!CONV) vk[u].load(static_cast<const T*>(p.k_src) + srow);
+          if constexpr (QK) vq[u].load(static_cast<const T*>(p.q_src) + srow);
+          if constexpr (QK && !CONV) vk[u].load(static_cast<const T*>(p.k_src) + srow);
           vv[u].load(static_cast<const T*>(p.v_src) + srow);
         }
       }
@@ -187,11 +188,11 @@ __global__ void __launch_bounds__(PRO_THREADS, (CONV || sizeof(T) == 4) ? 1 : 3)
               for (int c = 0; c < 8; ++c) hist[j][c] = hist[j + 1][c];
 #pragma unroll
             for (int c = 0; c < 8; ++c) hist[PRO_MAXK - 2][c] = cur[c];
-          } else {
+          } else if constexpr (QK) {
             vq[u].unpack(fq);
             vk[u].unpack(fk);
           }
-          if (rope) {
+          if (QK && rope) {
             const int pos = p.start_idx + t;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -209,13 +210,15 @@ __global__ void __launch_bounds__(PRO_THREADS, (CONV || sizeof(T) == 4) ? 1 : 3)
               fk[2 * j + 1] = k1 * cs.x + k0 * cs.y;
             }
           }
-          if (CONV || rope) {
+          if (QK && (CONV || rope)) {
             vq[u].pack(fq);
             vk[u].pack(fk);
           }
           const size_t drow = (((size_t)b * H + h) * NT + t) * F + 8 * sub;
-          vq[u].store(static_cast<T*>(p.xq) + drow);
-          vk[u].store(static_cast<T*>(p.xk) + drow);
+          if constexpr (QK) {
+            vq[u].store(static_cast<T*>(p.xq) + drow);
+            vk[u].store(static_cast<T*>(p.xk) + drow);
+          }
           vv[u].store(static_cast<T*>(p.xv) + drow);
         }
       }
@@ -414,8 +417,10 @@ static int prologue_grid(int B, int H, int T, int head_dim, int first_chunk, int
 template <typename T, int FD>
 static cudaError_t launch_pro_t(const LayerProParams& p, int grid, cudaStream_t st) {
   if (p.conv_q_w != nullptr)
-    return launch_dependent(ttt_layer_prologue_kernel<T, true, FD>, grid, PRO_THREADS, 0, st, p);
-  return launch_dependent(ttt_layer_prologue_kernel<T, false, FD>, grid, PRO_THREADS, 0, st, p);
+    return launch_dependent(ttt_layer_prologue_kernel<T, true, FD, true>, grid, PRO_THREADS, 0, st, p);
+  if (p.xq == nullptr)
+    return launch_dependent(ttt_layer_prologue_kernel<T, false, FD, false>, grid, PRO_THREADS, 0, st, p);
+  return launch_dependent(ttt_layer_prologue_kernel<T, false, FD, true>, grid, PRO_THREADS, 0, st, p);
 }
 
 cudaError_t launch_layer_prologue(int dtype, int head_dim, const LayerProParams& p0, cudaStream_t st) {
@@ -490,7 +495,7 @@ namespace ttt {
 // to the projection layout [B*T, ld] with the inverse rotation applied to q and k; the gradient of ttt_lr_eta goes
 // back through the sigmoid to the logits' columns (lr = c sigma(z), c = base_lr / F  =>  dz = dlr * lr * (1 - lr/c));
 // padding columns after the H logit columns are zeroed.
-template <typename T, int FD>
+template <typename T, int FD, bool QK>
 __global__ void __launch_bounds__(PRO_THREADS, sizeof(T) == 2 ? 3 : 1) ttt_layer_prologue_bwd_kernel(const LayerProBwdParams p) {
   __shared__ float2 rope_tab[PRO_MAXPOS][32];
   constexpr int F = FD, SUBS = FD / 8, HPW = 32 / SUBS;
@@ -524,8 +529,10 @@ __global__ void __launch_bounds__(PRO_THREADS, sizeof(T) == 2 ? 3 : 1) ttt_layer
       for (int u = 0; u < PRO_TG; ++u) {
         if (tb + u < t1) {
           const size_t srow = (((size_t)b * H + h) * NT + tb + u) * F + 8 * sub;
-          vq[u].load(static_cast<const T*>(p.dxq) + srow);
-          vk[u].load(static_cast<const T*>(p.dxk) + srow);
+          if constexpr (QK) {
+            vq[u].load(static_cast<const T*>(p.dxq) + srow);
+            vk[u].load(static_cast<const T*>(p.dxk) + srow);
+          }
           vv[u].load(static_cast<const T*>(p.dxv) + srow);
         }
       }
@@ -533,7 +540,7 @@ __global__ void __launch_bounds__(PRO_THREADS, sizeof(T) == 2 ? 3 : 1) ttt_layer
       for (int u = 0; u < PRO_TG; ++u) {
         const int t = tb + u;
         if (t < t1) {
-          if (rope) {
+          if (QK && rope) {
             float fq[8], fk[8];
             vq[u].unpack(fq);
             vk[u].unpack(fk);
@@ -557,8 +564,10 @@ __global__ void __launch_bounds__(PRO_THREADS, sizeof(T) == 2 ? 3 : 1) ttt_layer
             vk[u].pack(fk);
           }
           const size_t drow = ((size_t)b * NT + t) * p.ld_dst + col;
-          vq[u].store_once(static_cast<T*>(p.dq_dst) + drow);
-          vk[u].store_once(static_cast<T*>(p.dk_dst) + drow);
+          if constexpr (QK) {
+            vq[u].store_once(static_cast<T*>(p.dq_dst) + drow);
+            vk[u].store_once(static_cast<T*>(p.dk_dst) + drow);
+          }
           vv[u].store_once(static_cast<T*>(p.dv_dst) + drow);
         }
       }
@@ -837,12 +846,17 @@ cudaError_t launch_layer_prologue_bwd(int dtype, int head_dim, const LayerProBwd
   // as many blocks as are resident, each warp several short tasks: a task per warp was 1.7 rounds of them at 65536 tokens x 768
   // (130 us; 107 with two blocks of eight warps per SM, head groups of the same tokens side by side and streaming stores)
   const int grid = prologue_grid(p.B, p.H, p.T, head_dim, PRO_TG, 2, &p.tchunk);
+  const bool qk = p.dxq != nullptr;
   if (head_dim == 32) {
-    if (dtype == 1) ttt_layer_prologue_bwd_kernel<__nv_bfloat16, 32><<<grid, PRO_THREADS, 0, st>>>(p);
-    else ttt_layer_prologue_bwd_kernel<float, 32><<<grid, PRO_THREADS, 0, st>>>(p);
+    if (dtype == 1 && qk) ttt_layer_prologue_bwd_kernel<__nv_bfloat16, 32, true><<<grid, PRO_THREADS, 0, st>>>(p);
+    else if (dtype == 1) ttt_layer_prologue_bwd_kernel<__nv_bfloat16, 32, false><<<grid, PRO_THREADS, 0, st>>>(p);
+    else if (qk) ttt_layer_prologue_bwd_kernel<float, 32, true><<<grid, PRO_THREADS, 0, st>>>(p);
+    else ttt_layer_prologue_bwd_kernel<float, 32, false><<<grid, PRO_THREADS, 0, st>>>(p);
   } else {
-    if (dtype == 1) ttt_layer_prologue_bwd_kernel<__nv_bfloat16, 64><<<grid, PRO_THREADS, 0, st>>>(p);
-    else ttt_layer_prologue_bwd_kernel<float, 64><<<grid, PRO_THREADS, 0, st>>>(p);
+    if (dtype == 1 && qk) ttt_layer_prologue_bwd_kernel<__nv_bfloat16, 64, true><<<grid, PRO_THREADS, 0, st>>>(p);
+    else if (dtype == 1) ttt_layer_prologue_bwd_kernel<__nv_bfloat16, 64, false><<<grid, PRO_THREADS, 0, st>>>(p);
+    else if (qk) ttt_layer_prologue_bwd_kernel<float, 64, true><<<grid, PRO_THREADS, 0, st>>>(p);
+    else ttt_layer_prologue_bwd_kernel<float, 64, false><<<grid, PRO_THREADS, 0, st>>>(p);
   }
   return cudaGetLastError();
 }

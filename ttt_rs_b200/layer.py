@@ -16,6 +16,9 @@ Under autograd the same kernels run with their gradient kernels (`ttt_layer_prol
 `ttt_layer_epilogue_backward`) joined by torch autograd, so the layer trains end to end; the output projection and the
 products of the gradients are library GEMMs there.  With the shared-QK layout the two convolutions are a step of their own
 (`ttt_layer_qk_conv`, `ttt_layer_qk_conv_backward`) instead of being applied inside the prologue kernel.
+With a norm of queries and keys, or another rotation than the reference's, both go through `qk_norm_rotary` / `rotary` on the
+projection's columns, and the prologue makes values and learning rates only.  The inner model may be any with the
+`forward(state, inputs)` interface: TTT-Linear, TTT-MLP, the gated linear recurrence.
 There is no PyTorch fallback for the layer kernels: without the CUDA library the calls raise.
 """
 
@@ -31,6 +34,8 @@ import torch
 from . import _lib
 from ._lib import TttDims
 from .fused import FusedTileMultiTTTLinear, FusedTttConfig, Qkv, TTTInputsInner, TTTLinear, TTTLinearState
+from .gated import FusedGatedLinear, GatedLinear
+from .rope import _NO_ROTATION, Rotary, RotaryConfig, qk_norm_rotary, rotary
 
 ROPE_NONE, ROPE_WRAPPED, ROPE_GLOBAL = 0, 1, 2
 _NO_CONV = (None, None, None, None)
@@ -50,10 +55,31 @@ class TTTLayerConfig:
     conv_kernel_size: int = 4
     use_gate: bool = False
     share_qk: bool = False
+    # beyond the reference: queries and keys normed per head (root mean square, weights q_norm_weight and k_norm_weight), and
+    # rotated otherwise than in neighbouring pairs over the whole head with unscaled angles (see RotaryConfig)
+    qk_norm: bool = False
+    rope_layout: str = "interleaved"
+    rotary_dim: Optional[int] = None
+    rope_scaling: str = "none"
+    rope_factor: float = 1.0
+    rope_original_length: int = 0
 
     @property
     def head_dim(self) -> int:
         return self.hidden_size // self.num_heads
+
+    @property
+    def own_heads(self) -> bool:
+        """Queries and keys go through the norm and rotation of `qk_norm_rotary` / `rotary`, not through the prologue."""
+        plain = self.rope_layout == "interleaved" and self.rotary_dim in (None, self.head_dim) and self.rope_scaling == "none"
+        return self.qk_norm or (self.pos_encoding != "none" and not plain)
+
+    def rotary_config(self) -> Optional[RotaryConfig]:
+        """The rotation of `pos_encoding` and the fields above (None: none)."""
+        if self.pos_encoding == "none":
+            return None
+        return RotaryConfig(self.head_dim, self.rotary_dim, self.rope_theta, self.rope_layout, self.rope_scaling, self.rope_factor,
+                            self.rope_original_length, wrap=self.mini_batch_size if _POS[self.pos_encoding] == ROPE_WRAPPED else 0)
 
 
 @functools.lru_cache(maxsize=64)
@@ -218,6 +244,94 @@ def _prologue_backward(dproj, cols, cfg, start_idx, lr, dxq, dxk, dxv, dlr):
             _ptr(dlr), _ptr(lr), start_idx, _POS[cfg.pos_encoding], cfg.rope_theta, cfg.base_lr,
             col(cols["q"]), col(cols["k"]), col(cols["v"]), N, col(cols["lr"]), N, N - cols["lr"], stream))
     return dproj[..., cols["lr"]:cols["lr"] + H].sum(dim=(0, 1), dtype=torch.float32).to(dt).reshape(H, 1)
+
+
+@functools.lru_cache(maxsize=64)
+def _rotary_on(config: RotaryConfig, device: torch.device) -> Rotary:
+    return Rotary(config, device)
+
+
+def _layer_rotary(cfg: TTTLayerConfig, device) -> Optional[Rotary]:
+    rc = cfg.rotary_config()
+    return None if rc is None else _rotary_on(rc, device)
+
+
+def _head_columns(proj: torch.Tensor, col: int, cfg: TTTLayerConfig) -> torch.Tensor:
+    """A column block of proj [B,T,N] as [B,H,T,F], where it lies."""
+    return proj[..., col:col + cfg.num_heads * cfg.head_dim].unflatten(-1, (cfg.num_heads, cfg.head_dim)).transpose(1, 2)
+
+
+def layer_values(proj: torch.Tensor, cfg: TTTLayerConfig, *, v_col: int, lr_col: int, lr_bias: Optional[torch.Tensor]):
+    """XV [B,H,T,F] and ttt_lr_eta [B,H,T] from a projection output: `layer_prologue` without queries and keys."""
+    lib = _lib.load()
+    B, T, N = proj.shape
+    H, F = cfg.num_heads, cfg.head_dim
+    dt, dev, esz = proj.dtype, proj.device, proj.element_size()
+    if not proj.is_cuda or not proj.is_contiguous():
+        raise ValueError("proj must be a contiguous CUDA tensor")
+    d = TttDims(B, H, T, F, cfg.mini_batch_size, 1, 0.0, _dtype_code(dt))
+    xv, lr = torch.empty(B, H, T, F, dtype=dt, device=dev), torch.empty(B, H, T, dtype=dt, device=dev)
+    bias = None if lr_bias is None else lr_bias.detach().to(dt).reshape(-1).contiguous()
+    stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    with torch.cuda.device(dev):
+        _lib.check(lib.ttt_internal_layer_values(C.byref(d), C.c_void_p(proj.data_ptr() + v_col * esz), N,
+                                                 C.c_void_p(proj.data_ptr() + lr_col * esz), N, _ptr(bias), cfg.base_lr, _ptr(xv),
+                                                 _ptr(lr), stream))
+    return xv, lr
+
+
+def _normed_heads(q, k, q_weight, k_weight, cfg: TTTLayerConfig, start_idx: int):
+    """Queries and keys [B,H,T,F] of any strides as the layer's config wants them for the inner loop."""
+    rot = _layer_rotary(cfg, q.device)
+    if cfg.qk_norm:
+        return qk_norm_rotary(q, k, q_weight, k_weight, rot, eps=1e-6, start_idx=start_idx)
+    return rotary(q, rot, start_idx), rotary(k, rot, start_idx)
+
+
+class _HeadsFn(torch.autograd.Function):
+    """proj [B,T,N] -> XQ, XK (normed, rotated), XV and ttt_lr_eta, for the configs with `own_heads`; every column of proj's
+    gradient is written by one kernel."""
+
+    @staticmethod
+    def forward(ctx, proj, q_weight, k_weight, lr_bias, cfg, cols, start_idx):
+        xq, xk = _normed_heads(_head_columns(proj, cols["q"], cfg), _head_columns(proj, cols["k"], cfg), q_weight, k_weight, cfg,
+                               start_idx)
+        xv, lr = layer_values(proj, cfg, v_col=cols["v"], lr_col=cols["lr"], lr_bias=lr_bias)
+        ctx.save_for_backward(proj, q_weight, k_weight, lr)
+        ctx.meta = (cfg, cols, start_idx)
+        return xq, xk, xv, lr
+
+    @staticmethod
+    def backward(ctx, dxq, dxk, dxv, dlr):
+        proj, q_weight, k_weight, lr = ctx.saved_tensors
+        cfg, cols, start_idx = ctx.meta
+        lib, host = _lib.load(), _lib.host()
+        B, T, N = proj.shape
+        H, dt, dev, esz = cfg.num_heads, proj.dtype, proj.device, proj.element_size()
+        dproj = torch.empty_like(proj)
+        rot = _layer_rotary(cfg, dev)
+        args = _NO_ROTATION if rot is None else rot._args
+        q, k, dq, dk = (_head_columns(t, cols[n], cfg) for t in (proj, dproj) for n in ("q", "k"))
+        dxq, dxk, dxv, dlr = (t.contiguous() for t in (dxq, dxk, dxv, dlr))  # named: copies must outlive the launch
+        dwq = dwk = None
+        if cfg.qk_norm:
+            done = host.qk_norm_backward(q, k, dxq, dxk, q_weight, k_weight, *args, None, start_idx, 1e-6, dq, dk)
+            if done is not None:
+                dwq, dwk = done[2:]
+        else:
+            done = host.rotary(dxq, *args, None, start_idx, 1, dq)
+            if done is not None:
+                done = host.rotary(dxk, *args, None, start_idx, 1, dk)
+        if done is None:
+            raise _lib.TttError(_lib.TTT_ERR_SHAPE, "gradients of other shape or type than the layer's queries and keys")
+        d = TttDims(B, H, T, cfg.head_dim, cfg.mini_batch_size, 1, 0.0, _dtype_code(dt))
+        stream = C.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(dev):
+            _lib.check(lib.ttt_internal_layer_values_backward(
+                C.byref(d), _ptr(dxv), _ptr(dlr), _ptr(lr), cfg.base_lr, C.c_void_p(dproj.data_ptr() + cols["v"] * esz), N,
+                C.c_void_p(dproj.data_ptr() + cols["lr"] * esz), N, N - cols["lr"], stream))
+        dbias = dproj[..., cols["lr"]:cols["lr"] + H].sum(dim=(0, 1), dtype=torch.float32).to(dt).reshape(H, 1)
+        return dproj, dwq, dwk, dbias, None, None, None
 
 
 class _ProjectionsFn(torch.autograd.Function):
@@ -432,6 +546,9 @@ class TTT(torch.nn.Module):
         self.learnable_token_idx = torch.nn.Parameter(torch.zeros(c.mini_batch_size, **kw))
         self.post_norm_weight = torch.nn.Parameter(torch.ones(hs, **kw))
         self.post_norm_bias = torch.nn.Parameter(torch.zeros(hs, **kw))
+        self.q_norm_weight = torch.nn.Parameter(torch.ones(c.head_dim, **kw)) if c.qk_norm else None
+        self.k_norm_weight = torch.nn.Parameter(torch.ones(c.head_dim, **kw)) if c.qk_norm else None
+        c.rotary_config()  # (refuses what it cannot rotate)
         self._stack = None
 
     def __getstate__(self):  # (copies and pickles stack their own)
@@ -504,7 +621,7 @@ class TTT(torch.nn.Module):
         projections, wrapped or no rotary positions with a mini-batch of at most 16 tokens, and column blocks that
         start on multiples of 64."""
         c = self.config
-        return (x.dtype == torch.bfloat16 and x.is_cuda and x.shape[1] % 128 == 0 and not c.share_qk
+        return (x.dtype == torch.bfloat16 and x.is_cuda and x.shape[1] % 128 == 0 and not c.share_qk and not c.own_heads
                 and c.head_dim == 64 and c.hidden_size % 8 == 0 and c.num_heads <= 64
                 and c.pos_encoding in ("none", "rope") and c.mini_batch_size <= 16
                 and all(v % 64 == 0 for v in cols.values()))
@@ -521,18 +638,26 @@ class TTT(torch.nn.Module):
             xq, xk, xv, lr, gate = layer_projections(x, wcat, cols, c, self.learnable_ttt_lr_bias, start_idx)
             return TTTInputsInner(Qkv(xq, xk, xv), token_eta, lr, start_idx), gate, c.num_heads * c.head_dim
         proj = self._project(x, wcat)  # [B, T, N]: every projection of the token in one product
+        gate = proj.reshape(B * T, -1)[:, cols["g"]:] if c.use_gate else None
+        if c.own_heads:
+            q, k = _head_columns(proj, cols["q"], c), _head_columns(proj, cols["k"], c)
+            if c.share_qk:
+                q, k = (_head_columns(t, 0, c) for t in _QkConvFn.apply(
+                    proj, cols["q"], c.hidden_size, self.q_conv_weight, self.q_conv_bias, self.k_conv_weight, self.k_conv_bias, c))
+            xq, xk = _normed_heads(q, k, self.q_norm_weight, self.k_norm_weight, c, start_idx)
+            xv, lr = layer_values(proj, c, v_col=cols["v"], lr_col=cols["lr"], lr_bias=self.learnable_ttt_lr_bias)
+            return TTTInputsInner(Qkv(xq, xk, xv), token_eta, lr, start_idx), gate, proj.shape[-1]
         conv = None
         if c.share_qk:
             conv = (self.q_conv_weight, self.q_conv_bias, self.k_conv_weight, self.k_conv_bias)
         xq, xk, xv, lr = layer_prologue(proj, c, q_col=cols["q"], k_col=cols["k"], v_col=cols["v"], lr_col=cols["lr"],
                                         lr_bias=self.learnable_ttt_lr_bias, conv=conv, start_idx=start_idx)
-        gate = proj.reshape(B * T, -1)[:, cols["g"]:] if c.use_gate else None
         return TTTInputsInner(Qkv(xq, xk, xv), token_eta, lr, start_idx), gate, proj.shape[-1]
 
     def _infer_native(self, x: torch.Tensor, inner, state, start_idx: int) -> Optional[torch.Tensor]:
         """The whole inference forward as one native call (bf16; None: not a case it takes, nothing was done)."""
         c = self.config
-        if type(inner) is not FusedTileMultiTTTLinear or not x.is_cuda:
+        if type(inner) is not FusedTileMultiTTTLinear or not x.is_cuda or c.own_heads:
             return None
         # (modules and parameters through the dictionaries: attribute access on a module costs a multiple of it, and this
         # call runs once per generated token and layer)
@@ -577,7 +702,7 @@ class TTT(torch.nn.Module):
 def _train_native(self, x, inner, state, start_idx):
     """The whole layer as one native autograd node (None: not a case it takes, nothing was done)."""
     c = self.config
-    if type(inner) is not FusedTileMultiTTTLinear or not x.is_cuda:
+    if type(inner) is not FusedTileMultiTTTLinear or not x.is_cuda or c.own_heads:
         return None
     i = inner._modules["inner"]
     if type(i) is not TTTLinear or i.mini_batch_size != c.mini_batch_size:
@@ -643,7 +768,10 @@ def _train_forward(self, x, inner, state, start_idx):
             blocks.append(torch.zeros(pad, hs, dtype=x.dtype, device=x.device))
         proj = torch.matmul(x, torch.cat(blocks, dim=0).t())
     cols = {"q": 0, "k": hs, "v": 2 * hs, "lr": 3 * hs}
-    xq, xk, xv, lr = _PrologueFn.apply(proj, self.learnable_ttt_lr_bias, c, cols, start_idx)
+    if c.own_heads:
+        xq, xk, xv, lr = _HeadsFn.apply(proj, self.q_norm_weight, self.k_norm_weight, self.learnable_ttt_lr_bias, c, cols, start_idx)
+    else:
+        xq, xk, xv, lr = _PrologueFn.apply(proj, self.learnable_ttt_lr_bias, c, cols, start_idx)
     out = inner.forward(state, TTTInputsInner(Qkv(xq, xk, xv), token_eta, lr, start_idx))
     gate = torch.matmul(x, self.g_proj.t()) if c.use_gate else None
     y = _EpilogueFn.apply(out, gate, self.post_norm_weight, self.post_norm_bias, 1e-6)
@@ -660,6 +788,12 @@ def new_inner(config: TTTLayerConfig, checkpoint_interval: int = 1, device=None,
     return FusedTileMultiTTTLinear(TTTLinear(config.num_heads, config.head_dim, config.mini_batch_size, 1e-6,
                                              checkpoint_interval, device=device, dtype=dtype), allow_partial,
                                    partial_in_place)
+
+
+def new_gated_inner(config: TTTLayerConfig, device=None) -> FusedGatedLinear:
+    """The gated linear recurrence as the inner model of a layer with this config (any sequence length, single tokens included;
+    state and decays in float32 whatever the layer's type)."""
+    return FusedGatedLinear(GatedLinear(config.num_heads, config.head_dim, config.base_lr, device=device))
 
 
 class DecodeGraphs:
@@ -681,8 +815,8 @@ class DecodeGraphs:
         c = layer.config
         if c.pos_encoding == "rope_global":
             raise ValueError("rope_global positions never repeat: the step cannot be captured once per phase")
-        if not (inner.allow_partial and inner.partial_in_place):
-            raise ValueError("the inner model must be built with allow_partial=True, partial_in_place=True")
+        if not (getattr(inner, "allow_partial", False) and inner.partial_in_place):
+            raise ValueError("the inner model must be a TTT-Linear one, built with allow_partial=True, partial_in_place=True")
         self.layer, self.inner, self.state = layer, inner, state
         p = layer.q_proj
         self.x = torch.zeros(batch, 1, c.hidden_size, dtype=p.dtype, device=p.device)

@@ -11,9 +11,12 @@
 // floats, because a decay of zero (g = -inf: a new sequence begins) counts as one of 2^-160 (zero in float32), after which G is
 // large and its differences would keep few digits.
 //
-// Operands.  bf16 inputs go to the tensor cores as they are.  What a float32 result depends on (the state, the gradients of the
-// gates) must not be rounded to bf16 on the way: the state and the scaled keys enter products as two bf16 planes (16 bits of
-// mantissa: 2^-17 of a term at most).  float32 inputs are carried as three planes throughout, as in the other float32 kernels.
+// Operands.  bf16 inputs go to the tensor cores as they are; what a result of the inputs' type alone depends on is rounded to bf16 where
+// it becomes an operand (the decayed products, the state in q W).  What float32 results depend on is not: the scaled keys and
+// queries whose products make up the state and its gradient are carried as three bf16 planes (24 bits of mantissa, as float32; two
+// planes left 2.5e-6 of the state, three 5e-7, for 4 % of the forward's time), the state and its gradient in the sums for the gates'
+// gradients as two (2^-17 of a term; a third plane of both does not fit beside the tiles of two chunks).  float32
+// inputs are carried as three planes throughout, as in the other float32 kernels.
 #pragma once
 
 #include "ttt_common.cuh"
@@ -56,10 +59,10 @@ __device__ __forceinline__ void mma_planes(float (&c0)[4], float (&c1)[4], const
     const Pk<3> b0[2] = {b[0], b[1]}, b1[2] = {b[2], b[3]};
     mma_np2<3>(c0, a, b0, c1, a, b1);
   } else {
-    static_assert(NA * NB <= 2, "planes");
+    static_assert(NA == 1 || NB == 1, "planes");
 #pragma unroll
-    for (int i = NA * NB - 1; i >= 0; --i) {  // the small plane first
-      const int pa = NA == 2 ? i : 0, pb = NB == 2 ? i : 0;
+    for (int i = NA * NB - 1; i >= 0; --i) {  // the small planes first
+      const int pa = NA > 1 ? i : 0, pb = NB > 1 ? i : 0;
       mma_bf16(c0, a[0].p[pa], a[1].p[pa], a[2].p[pa], a[3].p[pa], b[0].p[pb], b[1].p[pb]);
       mma_bf16(c1, a[0].p[pa], a[1].p[pa], a[2].p[pa], a[3].p[pa], b[2].p[pb], b[3].p[pb]);
     }

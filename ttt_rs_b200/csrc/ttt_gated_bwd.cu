@@ -338,17 +338,17 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       for (int k = 0; k < SH::NT; ++k) scale_rows(dW[k], all, all);
 #pragma unroll 1
       for (int it = 0; it < GC / 16; ++it) {
-        Pk<NS> qt[4];
+        Pk<3> qt[4];
         {
           Pk<NP> f[4];
           ldsm_np<NP>(f, (tq + 16 * it * TL::ROW + high) ^ (row0 << 1), SM::PLANE, true);
-          scale_a_cols<NS, NP>(qt, f, ld2(&cg.from[16 * it + 2 * t4]), ld2(&cg.from[16 * it + 2 * t4 + 8]));
+          scale_a_cols<3, NP>(qt, f, ld2(&cg.from[16 * it + 2 * t4]), ld2(&cg.from[16 * it + 2 * t4 + 8]));
         }
 #pragma unroll
         for (int k = 0; k < SH::NT / 2; ++k) {
           Pk<NP> f[4];
           ldsm_np<NP>(f, (tu + 16 * it * TL::ROW + low) ^ ((col0 + 16 * k) << 1), SM::PLANE, true);
-          mma_planes<NS, NP>(dW[2 * k], dW[2 * k + 1], qt, f);
+          mma_planes<3, NP>(dW[2 * k], dW[2 * k + 1], qt, f);
         }
       }
     } else {

@@ -39,7 +39,7 @@ struct GatedFwdBlock {
   using SH = StateShare<F>;
   using TL = GTile<F>;
   static constexpr bool BF = SM::BF;
-  static constexpr int NP = SM::NP, NS = BF ? 2 : 3, KS = F / 16;  // planes of inputs, of scaled keys
+  static constexpr int NP = SM::NP, NS = 3, KS = F / 16;  // planes of inputs, of scaled keys
   const GatedMaps& maps;
   const GatedParams& p;
   uint8_t* mem;

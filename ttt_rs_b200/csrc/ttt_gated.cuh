@@ -36,6 +36,13 @@ __device__ __forceinline__ Pk<2> split_pack<2>(float x, float y) {
   return r;
 }
 
+// 2^x; results below 2^-126 are zero (exp2f spends three instructions more on those)
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // A bf16 tile of rows of F elements (128 or 64 bytes) in the swizzle of TMA: rows 0..63, any multiple of 8 columns
 template <int F>
 struct GTile {
@@ -159,10 +166,10 @@ __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2
   const float h0 = (float)G0, h1 = (float)G1;
   put(s.hi, h0, h1);
   put(s.lo, (float)(G0 - h0), (float)(G1 - h1));
-  put(s.from, exp2f((float)G0), exp2f((float)G1));
-  put(s.into, exp2f((float)(G0 - before)), exp2f((float)(G1 - before)));
-  const float o0 = exp2f((float)(mine - G0)), o1 = exp2f((float)(mine - G1));
-  const float e0 = exp2f((float)(end - G0)), e1 = exp2f((float)(end - G1));
+  put(s.from, pow2((float)G0), pow2((float)G1));
+  put(s.into, pow2((float)(G0 - before)), pow2((float)(G1 - before)));
+  const float o0 = pow2((float)(mine - G0)), o1 = pow2((float)(mine - G1));
+  const float e0 = pow2((float)(end - G0)), e1 = pow2((float)(end - G1));
   put(s.out, o0, o1);
   put(s.out_b, o0 * beta.x, o1 * beta.y);
   put(s.end, e0, e1);
@@ -176,10 +183,10 @@ __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2
       if (a == k) ga = ends[k];
       if (b == k) gb = ends[k];
     }
-    s.blocks[a][b] = b >= a ? exp2f((float)(gb - ga)) : 0.f;
-    if (b == 0) s.starts[a] = a == 0 ? 1.f : exp2f((float)(a == 1 ? ends[0] : a == 2 ? ends[1] : ends[2]));
+    s.blocks[a][b] = b >= a ? pow2((float)(gb - ga)) : 0.f;
+    if (b == 0) s.starts[a] = a == 0 ? 1.f : pow2((float)(a == 1 ? ends[0] : a == 2 ? ends[1] : ends[2]));
   }
-  if (lane == 0) s.all = exp2f((float)end);
+  if (lane == 0) s.all = pow2((float)end);
 }
 // Decays e^{G_i - G_j} of the 16 x 16 pairs of block `blk` with row r (g, g + 8) and column c (2t, 2t + 1, 2t + 8, 2t + 9) of a
 // lane's accumulators: [row half][column]; rows are i (ROWS_LATE) or j.  Zero where i < j.
@@ -194,7 +201,7 @@ __device__ __forceinline__ void block_decays(float (&d)[2][4], const ChunkGates&
     for (int e = 0; e < 4; ++e) {
       const int c = c0 + (e & 1) + 8 * (e >> 1);
       const float x = (hr - s.hi[c]) + (lr - s.lo[c]);
-      d[half][e] = (ROWS_LATE ? c <= r : c >= r) ? exp2f(ROWS_LATE ? x : -x) : 0.f;
+      d[half][e] = (ROWS_LATE ? c <= r : c >= r) ? pow2(ROWS_LATE ? x : -x) : 0.f;
     }
   }
 }

@@ -89,7 +89,8 @@ const char* ttt_b200_last_error(void);
  * write {TTT_ERR_TIMEOUT, 15, block, stage} to `status` and return.  `poll_limit` replaces the limit (0 restores the
  * default, 2^24 polls of about 100 ns); `first_item` > 0 makes the launch skip that many work items, which -- set to
  * batch*heads -- leaves every remaining item waiting for a hand-off nobody publishes, so that a test can watch the
- * wait give up.  Process-wide; affects launches issued after the call.  Leave at (0, 0) in production. */
+ * wait give up.  The gated linear recurrence, where its streams outnumber resident blocks, takes both for the blocks' waits for
+ * one another's states (`first_item` = 1: the first block's state never comes).  Process-wide; affects launches issued after the call.  Leave at (0, 0) in production. */
 void ttt_b200_debug_handoff(uint32_t poll_limit, int32_t first_item);
 
 /* Number of checkpoints per (batch, head) stream: ceil((T / CS) / K)  (forward/launch.rs:221-223). */
@@ -358,13 +359,17 @@ int ttt_layer_qk_conv_backward(const ttt_dims* d, const void* grad_q, const void
  *   output        T [B,H,T,F] (out);  weight_out  float32 [B,H,F,F] (out) state behind the last token
  *   saved         (out) ttt_linear_gated_saved_bytes(d) bytes for the backward: the state before every 64 tokens, opaque; null
  *                 (with 0 bytes) for inference
- *   workspace     ttt_linear_gated_*_workspace_bytes(d) bytes (0 for many streams; null then)
+ *   workspace     ttt_linear_gated_forward_workspace_bytes(d) (backward: ..._backward_workspace_bytes(d)) bytes, 16-byte aligned;
+ *                 may be 0 (null then): a state per segment where streams are few, or per block where they outnumber the blocks
  * The state is float32 throughout, and what results of type float32 depend on is not rounded to bf16 on the way.  A NaN or an
  * infinity in a token reaches the outputs of the 64 tokens around it, those before it among them.
  *
  * ttt_linear_gated_backward: gradients for loss = <grad_output, output> + <grad_weight_out, weight_out> (grad_weight_out null:
  * zero).  `strides`: of xq, xk, xv and grad_output.  grad_xq, grad_xk, grad_xv T [B,H,T,F] contiguous, grad_log_decay, grad_beta
  * (null exactly where beta is) float32 [B,H,T], grad_weight float32 [B,H,F,F]; all written.  grad_log_decay is 0 where exp(log_decay) is.
+ *
+ * Blocks hand a stream's state to one another where streams outnumber resident blocks (by the order in which blocks start, through
+ * `workspace`), and every kernel waits for copies of its own; all waits have a limit, see `status`.
  *
  * ttt_linear_gated_step: the forward over 1 to 16 tokens (token-by-token generation); weight_out may be weight.
  */

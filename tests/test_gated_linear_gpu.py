@@ -226,6 +226,85 @@ def test_two_runs_are_the_same():
     assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def test_a_state_that_is_never_handed_on_ends_the_launch():
+    """The first block's range is taken by nobody: the block of the next one gives up its wait, reports it, and everything ends."""
+    import ttt_rs_b200 as tb
+    from ttt_rs_b200 import _lib
+    lib = _lib.load()
+    B, H = 50, 10
+    # 500 streams of 10 chunks on 444 (backward: 296) blocks: the first one's 11 (16) steps end within a stream, which the second finishes
+    ins, d_out, d_w = make(B, H, 640, 64, torch.bfloat16, seed=12)
+    want = run(ins, d_out, d_w)
+    tb.check_status()
+    try:
+        lib.ttt_b200_debug_handoff(2000, 1)
+        with torch.no_grad():
+            tb.fused_gated_linear(*[t.cuda() for t in ins])
+        with pytest.raises(tb.TttError) as e:
+            tb.check_status()
+        assert e.value.code == _lib.TTT_ERR_TIMEOUT
+        dev = [t.cuda().requires_grad_() for t in ins]
+        lib.ttt_b200_debug_handoff(0, 0)
+        out, _ = tb.fused_gated_linear(*dev)
+        lib.ttt_b200_debug_handoff(2000, 1)
+        torch.autograd.grad(out, dev, d_out.cuda())
+        with pytest.raises(tb.TttError):
+            tb.check_status()
+    finally:
+        lib.ttt_b200_debug_handoff(0, 0)
+    assert all(torch.equal(x, y) for x, y in zip(run(ins, d_out, d_w), want))
+    tb.check_status()
+
+
+def test_captured_with_its_backward_and_replayed():
+    """Forward and backward in one graph, replayed with other inputs in the captured buffers; few streams (segments) and many."""
+    import ttt_rs_b200 as tb
+    for B, H, T in ((1, 2, 700), (40, 12, 70)):
+        ins, d_out, _ = make(B, H, T, 64, torch.bfloat16, seed=13)
+        other, _, _ = make(B, H, T, 64, torch.bfloat16, seed=14)
+        want = run(other, d_out)
+        dev = [t.cuda() for t in ins]
+        u = d_out.cuda()
+
+        def step():
+            leaves = [t.detach().requires_grad_() for t in dev]
+            out, w = tb.fused_gated_linear(*leaves)
+            return [out.detach(), w.detach(), *torch.autograd.grad(out, leaves, u)]
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        for d, o in zip(dev, other):
+            d.copy_(o)
+        for _ in range(2):
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        tb.check_status()
+
+
+def test_two_calls_at_once_on_two_streams():
+    import ttt_rs_b200 as tb
+    calls = []
+    for seed, (B, H, T) in enumerate(((40, 12, 70), (40, 12, 70), (1, 3, 900), (1, 3, 900))):
+        ins, _, _ = make(B, H, T, 64, torch.bfloat16, seed=20 + seed)
+        calls.append(([t.cuda() for t in ins], run(ins)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    with torch.no_grad():
+        for _ in range(3):
+            got = []
+            for (dev, _), s in zip(calls, streams):
+                with torch.cuda.stream(s):
+                    got.append(tb.fused_gated_linear(*dev))
+    torch.cuda.synchronize()
+    for (_, want), g in zip(calls, got):
+        assert all(torch.equal(x, y) for x, y in zip(g, want))
+    tb.check_status()
+
+
 def test_refusals():
     import ttt_rs_b200 as tb
     ins, _, _ = make(1, 2, 8, 64, torch.bfloat16)

@@ -1375,6 +1375,8 @@ extern "C" int ttt_linear_gated_forward(const ttt_dims* d, const void* xq, const
   p.slots = cut.slots;
   p.records = p.seg_state;
   p.flags = reinterpret_cast<int*>(p.seg_decay);
+  p.polls = g_handoff_polls.load();
+  p.first_slot = g_item_base.load();
   const cudaError_t e = ttt::launch_gated_fwd(d->dtype, d->head_dim, maps, p, saved != nullptr, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated forward launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;
@@ -1455,6 +1457,8 @@ extern "C" int ttt_linear_gated_backward(const ttt_dims* d, const void* xq, cons
   p.slots = cut.slots;
   p.records = seg;
   p.flags = reinterpret_cast<int*>(seg + cut.state_floats);
+  p.polls = g_handoff_polls.load();
+  p.first_slot = g_item_base.load();
   const cudaError_t e = ttt::launch_gated_bwd(d->dtype, d->head_dim, maps, p, st);
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "gated backward launch failed: %s", cudaGetErrorString(e));
   return TTT_OK;

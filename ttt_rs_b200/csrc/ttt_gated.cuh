@@ -20,6 +20,7 @@
 #pragma once
 
 #include "ttt_common.cuh"
+#include "ttt_stage.cuh"
 
 namespace ttt {
 
@@ -355,9 +356,24 @@ struct GatedWalk {
     return t;
   }
 };
+// Waits of a block.  One that runs out is reported, and from then on no wait waits and no copy starts: every warp still passes all the
+// barriers that the others meet it at, on its way to the end, and what the launch writes is not valid.
+struct GatedWaits {
+  volatile int* failed;  // shared memory
+  uint32_t* status;
+  __device__ __forceinline__ bool ok() const { return *failed == 0; }
+  __device__ __forceinline__ void fail(uint32_t where, int step) const {
+    report_timeout(status, where, (uint32_t)step);
+    *failed = 1;
+  }
+  __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, uint32_t where, int step) const {
+    if (ok() && !mbar_wait_bounded(bar, parity)) fail(where, step);
+  }
+};
+
 // One thread: the record of range `slot` has been handed on (false: the wait ran out)
-__device__ __forceinline__ bool wait_record(const int* flags, int slot) {
-  for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+__device__ __forceinline__ bool wait_record(const int* flags, int slot, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i) {
     int v;
     asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(flags + slot) : "memory");
     if (v != 0) return true;

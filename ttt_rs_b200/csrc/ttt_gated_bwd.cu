@@ -68,15 +68,17 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   const bool queries = tid < GB_THREADS / 2;
   const uint32_t bar = base + SM::BAR, bar_w = bar + 16;
   volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 24);  // a wait has run out; this block's range
+  const GatedWaits waits{shared, p.status};
   if (tid == 0) {
     shared[0] = 0;
-    shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
+    shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) + p.first_slot : (int)blockIdx.x;
     mbar_init(bar, 1);
     mbar_init(bar + 8, 1);
     mbar_init(bar_w, 1);
     fence_mbar_init();
   }
   __syncthreads();
+  if (p.slots > 0 && shared[1] >= p.slots) return;  // (first_slot)
   GatedWalk walk_{};
   walk_.set(p, shared[1], true);
   const int n = walk_.n;
@@ -84,8 +86,8 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   auto chunk_of = [&](const GatedWalk::Step& s) { return p.NC - 1 - s.pos; };
   // thread 0.  bf16: q, k, v, u of a chunk; float32: two of them at a time, through the same rows of shared memory
   auto fetch = [&](const GatedWalk::Step& s, int first, int count) {
-    const int i = s.i;
-    const int slot = BF ? i & 1 : 0;
+    if (!waits.ok()) return;
+    const int slot = BF ? s.i & 1 : 0;
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * 4 * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
     mbar_expect_tx(at, count * bytes);
@@ -93,6 +95,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     for (int m = 0; m < count; ++m) tma_load_4d(dst + m * bytes, &maps.m[first + m], chunk_of(s) * GC, h, b, at);
   };
   auto fetch_w = [&](const GatedWalk::Step& s) {
+    if (!waits.ok()) return;
     mbar_expect_tx(bar_w, SM::WRAW);
     bulk_load_1d(base + SM::WSAVED, p.saved + ((size_t)s.stream * p.NC + chunk_of(s)) * SM::WRAW, SM::WRAW, bar_w);
   };
@@ -185,16 +188,12 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     const bool ahead = QUERIES && w == 0 && i + 1 < n;
     float2 g_next, b_next;
     if (ahead) gates_of(nx, g_next, b_next);
-    bool ok = true;
     if constexpr (QUERIES) {
       if (st.starts) {  // the gradient of the state behind this stream, or behind this part of it
         const float* d0 = p.dw_out != nullptr ? p.dw_out + (size_t)stream * F * F : nullptr;
         if (st.pos > 0) {
           if (p.slots > 0) {
-            if (tid == 0 && !wait_record(p.flags, walk_.slot - 1)) {
-              report_timeout(p.status, 23, (uint32_t)i);
-              ok = false;
-            }
+            if (tid == 0 && waits.ok() && !wait_record(p.flags, walk_.slot - 1, p.polls)) waits.fail(23, i);
             asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
             d0 = p.records + (size_t)(walk_.slot - 1) * F * F;
           } else {
@@ -213,7 +212,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       put_state<F, NS>(dW, row0, col0, tdw, lane);
       asm volatile("bar.arrive 1, %0;" ::"n"(GB_THREADS) : "memory");
     }
-    bool arrived = mbar_wait_bounded(bar + 8 * slot, BF ? (i >> 1) & 1 : 0);
+    waits.wait(bar + 8 * slot, BF ? (i >> 1) & 1 : 0, 21, i);
     if constexpr (!BF) {
       auto split2 = [&](uint32_t dst) {
         for (int m = 0; m < 2; ++m)
@@ -221,15 +220,11 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       };
       split2(tq);
       block_sync();
-      if (tid == 0 && arrived) fetch(st, 2, 2);
-      arrived = arrived && mbar_wait_bounded(bar, 1);
+      if (tid == 0) fetch(st, 2, 2);
+      waits.wait(bar, 1, 21, i);
       split2(tv);
       block_sync();
-      if (tid == 0 && arrived && i + 1 < n) fetch(nx, 0, 2);
-    }
-    if (!arrived) {
-      if (tid == 0) report_timeout(p.status, 21, (uint32_t)i);
-      return;
+      if (tid == 0 && i + 1 < n) fetch(nx, 0, 2);
     }
     if constexpr (QUERIES) {
       const int ia = 16 * w + g;
@@ -240,10 +235,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       // from the state before the chunk: this thread's share as it was saved, for the ways that cross the whole chunk, and its
       // planes as an operand for all four warps
       const float all = cg.all;
-      if (!mbar_wait_bounded(bar_w, i & 1)) {
-        if (tid == 0) report_timeout(p.status, 22, (uint32_t)i);
-        ok = false;
-      }
+      waits.wait(bar_w, i & 1, 22, i);
       {
         float W[SH::NT][4];
         get_fragments<F>(W, reinterpret_cast<const float4*>(mem + SM::WSAVED), w, lane);
@@ -556,9 +548,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         }
       }
     }
-    if (!ok) shared[0] = 1;
     block_sync();  // this chunk's tiles, states and sums are complete and free
-    if (shared[0]) return;
     if (QUERIES && tid == 0) {
       if (BF && i + 2 < n) fetch(walk_.next(nx), 0, 4);
     }
@@ -567,6 +557,9 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   };
   if (queries) walk(std::true_type{});
   else walk(std::false_type{});
+  if (!waits.ok()) {  // copies that may still be on their way
+    for (int k = 0; k < 3; ++k) mbar_wait_bounded(bar + 8 * k, 0);
+  }
 }
 
 template <typename T, int F>

@@ -45,11 +45,13 @@ struct GatedFwdBlock {
   uint8_t* mem;
   uint32_t base, bar;
   ChunkGates* gates;
-  int tid, lane, w;  // w: warp of its group
+  GatedWaits waits;
+  int tid, lane, w;
   GatedWalk walk;
 
   __device__ __forceinline__ int chunk_of(const GatedWalk::Step& s) const { return REV ? p.NC - 1 - s.pos : s.pos; }
   __device__ __forceinline__ void fetch(const GatedWalk::Step& s) const {  // one thread
+    if (!waits.ok()) return;
     const int slot = BF ? s.i & 1 : 0;
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * SM::NIN * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
@@ -63,14 +65,11 @@ struct GatedFwdBlock {
     g = load_gates(p.g + row, chunk_of(s) * GC, p.T, lane, 0.f);
     beta = load_gates(p.beta != nullptr ? p.beta + row : nullptr, chunk_of(s) * GC, p.T, lane, 1.f);
   }
-  // this chunk's tiles in their planes; false: the wait ran out
-  __device__ __forceinline__ bool tiles(const GatedWalk::Step& st, const GatedWalk::Step& nx, uint32_t& at) const {
+  // this chunk's tiles, in their planes
+  __device__ __forceinline__ uint32_t tiles(const GatedWalk::Step& st, const GatedWalk::Step& nx) const {
     const int slot = BF ? st.i & 1 : 0;
-    at = base + SM::TILES + slot * SM::NIN * SM::TILE;
-    if (!mbar_wait_bounded(bar + 8 * slot, (BF ? st.i >> 1 : st.i) & 1)) {
-      if (tid == 0) report_timeout(p.status, 20, (uint32_t)st.i);
-      return false;
-    }
+    const uint32_t at = base + SM::TILES + slot * SM::NIN * SM::TILE;
+    waits.wait(bar + 8 * slot, (BF ? st.i >> 1 : st.i) & 1, 20, st.i);
     if constexpr (!BF) {
 #pragma unroll
       for (int m = 0; m < SM::NIN; ++m)
@@ -78,20 +77,21 @@ struct GatedFwdBlock {
       block_sync();
       if (tid == 0 && nx.i < walk.n) fetch(nx);
     }
-    return true;
+    return at;
   }
   // a warp has left step i; all warps have left the step before i (its tiles and gates are free, what it wrote is complete)
   __device__ __forceinline__ void leave(int i) const {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar + 16 + 8 * (i & 1));
   }
-  __device__ __forceinline__ bool settled(int i) const {
-    if (i <= 0) return true;
-    if (!mbar_wait_bounded(bar + 16 + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1)) {
-      if (tid == 0) report_timeout(p.status, 25, (uint32_t)i);
-      return false;
+  __device__ __forceinline__ void settled(int i) const {
+    if (i > 0) waits.wait(bar + 16 + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1, 25, i);
+  }
+  __device__ __forceinline__ void drain() const {  // copies that may still be on their way
+    if (!waits.ok()) {
+      mbar_wait_bounded(bar, 0);
+      mbar_wait_bounded(bar + 8, 0);
     }
-    return reinterpret_cast<volatile int*>(mem + SM::BAR + 32)[0] == 0;
   }
   static __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0, %0;" ::"n"(THREADS) : "memory"); }
   // W <- e^{G_end} W + sum of scaled keys^T values (REV: queries^T gradients, scaled by what is left at the token)
@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   uint8_t* const mem = gated_smem + (base - raw);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t4 = lane & 3;
   volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 32);  // a wait has run out; this block's range
-  BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), tid, lane, w, {}};
+  BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), {shared, p.status}, tid, lane, w, {}};
   if (tid == 0) {
     shared[0] = 0;
-    shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) : (int)blockIdx.x;
+    shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) + p.first_slot : (int)blockIdx.x;
     mbar_init(bk.bar, 1);
     mbar_init(bk.bar + 8, 1);
     mbar_init(bk.bar + 16, GATED_WARPS);
@@ -146,6 +146,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     fence_mbar_init();
   }
   __syncthreads();
+  if (p.slots > 0 && shared[1] >= p.slots) return;  // (first_slot)
   bk.walk.set(p, shared[1], false);
   const int n = bk.walk.n;
   const GatedWalk::Step first = bk.walk.part(0), second = bk.walk.next(first);
@@ -168,12 +169,8 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       const float* w0 = p.w0 != nullptr ? p.w0 + (size_t)s.stream * F * F : nullptr;
       if (s.pos > 0) {
         if (p.slots > 0) {
-          int ok = 1;
-          if (lane == 0) ok = wait_record(p.flags, bk.walk.slot - 1);
-          if (!__shfl_sync(0xffffffffu, ok, 0)) {
-            if (lane == 0) report_timeout(p.status, 24, (uint32_t)s.i);
-            shared[0] = 1;
-          }
+          if (lane == 0 && bk.waits.ok() && !wait_record(p.flags, bk.walk.slot - 1, p.polls)) bk.waits.fail(24, s.i);
+          __syncwarp();
           w0 = p.records + (size_t)(bk.walk.slot - 1) * F * F;
         } else {
           w0 = p.seg_state + (size_t)bk.walk.slot * F * F;
@@ -186,7 +183,6 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   };
   publish(first);
   __syncthreads();
-  if (shared[0]) return;
   int slot3 = 0;  // i modulo 3
 #pragma unroll 1
   for (GatedWalk::Step st = first, nx = second, fa; st.i < n; st = nx, nx = fa) {
@@ -195,10 +191,8 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     const bool ahead = r == 0 && fa.i < n;  // (the warp with one block)
     float2 g_next, b_next;
     if (ahead) bk.gates_of(fa, g_next, b_next);
-    if (!BF && !bk.settled(i)) return;  // (one set of planes)
-    uint32_t tq;
-    if (!bk.tiles(st, nx, tq)) return;
-    const uint32_t tk = tq + SM::TILE, tv = tk + SM::TILE, tw = base + SM::W + (i & 1) * NP * TL::STATE_BYTES;
+    if (!BF) bk.settled(i);  // (one set of planes)
+    const uint32_t tq = bk.tiles(st, nx), tk = tq + SM::TILE, tv = tk + SM::TILE, tw = base + SM::W + (i & 1) * NP * TL::STATE_BYTES;
     const ChunkGates& cg = bk.gates[slot3];
     float o[F / 8][4];
     Pk<NP> q[KS][4];
@@ -246,7 +240,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       }
     }
     bk.update(W, tk, tv, cg, row0, col0);
-    if (BF && !bk.settled(i)) return;
+    if (BF) bk.settled(i);
     if (BF && r == 0 && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
     if (ahead) make_chunk_gates(bk.gates[slot3n], lane, g_next, b_next);
     const float fra = cg.from[16 * r + g], frb = cg.from[16 * r + g + 8];
@@ -282,6 +276,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F, 16 * r, p.T - t0, o, lane);
     slot3 = slot3 == 2 ? 0 : slot3 + 1;
   }
+  bk.drain();
 }
 
 // Every segment's own state, and what is left behind it of the state before it.  No warp needs another's rows: they share the tiles
@@ -298,9 +293,10 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 :
   const uint32_t raw = smem_u32(gated_smem), base = (raw + 1023) & ~1023u;
   uint8_t* const mem = gated_smem + (base - raw);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), tid, lane, w, {}};
+  volatile int* const failed = reinterpret_cast<volatile int*>(mem + SM::BAR + 32);
+  BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), {failed, p.status}, tid, lane, w, {}};
   if (tid == 0) {
-    *reinterpret_cast<volatile int*>(mem + SM::BAR + 32) = 0;
+    *failed = 0;
     mbar_init(bk.bar, 1);
     mbar_init(bk.bar + 8, 1);
     mbar_init(bk.bar + 16, GATED_WARPS);
@@ -331,14 +327,13 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 :
     const bool turn = w == (i & 3), ahead = turn && fa.i < n;
     float2 g_next, b_next;
     if (ahead) bk.gates_of(fa, g_next, b_next);
-    if (!bk.settled(BF ? i - 1 : i)) return;  // (float32: one set of planes)
-    uint32_t tk;
-    if (!bk.tiles(st, nx, tk)) return;
+    bk.settled(BF ? i - 1 : i);  // (float32: one set of planes)
+    const uint32_t tk = bk.tiles(st, nx);
     const ChunkGates& cg = bk.gates[slot3];
     total *= cg.all;
     bk.update(W, tk, tk + SM::TILE, cg, row0, col0);
     if (turn) {
-      if (BF && !bk.settled(i)) return;
+      if (BF) bk.settled(i);
       if (BF && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
       if (ahead) make_chunk_gates(bk.gates[slot3 == 0 ? 2 : slot3 - 1], lane, g_next, b_next);
     }
@@ -347,6 +342,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 :
   }
   store_state<F>(p.seg_state + (size_t)bk.walk.slot * F * F, W, row0, col0, lane);
   if (tid == 0) p.seg_decay[bk.walk.slot] = total;
+  bk.drain();
 }
 
 // The segments' own states to the states before them, along the sequence (REV: gradients, from the last segment to the first):

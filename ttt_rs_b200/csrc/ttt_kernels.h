@@ -427,6 +427,8 @@ struct GatedParams {
   int slots;          // > 0: ranges of the streams' chunks (GatedWalk); their records and flags, and the counter that numbers them
   float* records;     // [slots][F*F]
   int* flags;         // [slots], then the counter; zero before the launch
+  uint32_t polls;     // limit of a block's wait for another's record
+  int first_slot;     // ranges that nobody takes (diagnostic)
 };
 struct GatedBwdParams {
   const float* g;
@@ -444,6 +446,8 @@ struct GatedBwdParams {
   int slots;
   float* records;
   int* flags;
+  uint32_t polls;
+  int first_slot;
 };
 struct GatedStepParams {
   const void *q, *k, *v;

@@ -383,7 +383,7 @@ static_assert(32 * 32 / 2 % JOIN_THREADS == 0, "whole blocks per stream");
 // Streams that do not fill the card are cut into segments until they do; more streams than blocks are resident are cut into as
 // many ranges as blocks are.
 void gated_split(int64_t streams, int chunks, int dtype, bool backward, int* nseg, int* slots) {
-  constexpr int SMS = 148, LEAST = 4;  // (chunks per segment: a segment's states and its second reading must be worth it)
+  constexpr int SMS = 148, LEAST = 2;  // (chunks per segment: a segment's states and its second reading must be worth it)
   const int resident = dtype == 1 ? (backward ? 2 : 3) : 1;
   *nseg = 1;
   *slots = 0;

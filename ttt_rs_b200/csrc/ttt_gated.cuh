@@ -369,6 +369,14 @@ struct GatedWaits {
   __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, uint32_t where, int step) const {
     if (ok() && !mbar_wait_bounded(bar, parity)) fail(where, step);
   }
+  // The last copy that was started on barrier k of `copies`: its parity, and 2.  Written before the copy starts, by the thread that
+  // starts it.
+  __device__ __forceinline__ void started(volatile int* copies, int k, uint32_t parity) const { copies[k] = (int)parity | 2; }
+  // One thread, behind a barrier of all threads after a wait has run out: the block ends only with its copies complete
+  __device__ __forceinline__ void drain(volatile const int* copies, int count, uint32_t bar) const {
+    for (int k = 0; k < count; ++k)
+      if (copies[k] != 0) mbar_wait_bounded(bar + 8 * k, copies[k] & 1);
+  }
 };
 
 // One thread: the record of range `slot` has been handed on (false: the wait ran out)

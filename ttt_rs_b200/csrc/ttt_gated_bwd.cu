@@ -49,7 +49,7 @@ struct GatedBwdSmem {
   static constexpr uint32_t W = BF ? WSAVED : WSAVED + WRAW, DW = W + STATE;
   static constexpr uint32_t GATES = DW + STATE;
   static constexpr uint32_t SUMS = GATES + 2 * sizeof(ChunkGates);
-  static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 32 + 1024;  
+  static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 48 + 1024;
   static_assert(!BF || STATE == WRAW, "two planes of bf16 are as long as the float32 state");
 };
 
@@ -68,9 +68,10 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   const bool queries = tid < GB_THREADS / 2;
   const uint32_t bar = base + SM::BAR, bar_w = bar + 16;
   volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 24);  // a wait has run out; this block's range
+  volatile int* const copies = shared + 2;  // (three barriers)
   const GatedWaits waits{shared, p.status};
   if (tid == 0) {
-    shared[0] = 0;
+    shared[0] = copies[0] = copies[1] = copies[2] = 0;
     shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) + p.first_slot : (int)blockIdx.x;
     mbar_init(bar, 1);
     mbar_init(bar + 8, 1);
@@ -90,12 +91,14 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     const int slot = BF ? s.i & 1 : 0;
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * 4 * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
+    waits.started(copies, slot, BF ? (s.i >> 1) & 1 : first != 0);
     mbar_expect_tx(at, count * bytes);
     const int b = s.stream / p.H, h = s.stream - b * p.H;
     for (int m = 0; m < count; ++m) tma_load_4d(dst + m * bytes, &maps.m[first + m], chunk_of(s) * GC, h, b, at);
   };
   auto fetch_w = [&](const GatedWalk::Step& s) {
     if (!waits.ok()) return;
+    waits.started(copies, 2, s.i & 1);
     mbar_expect_tx(bar_w, SM::WRAW);
     bulk_load_1d(base + SM::WSAVED, p.saved + ((size_t)s.stream * p.NC + chunk_of(s)) * SM::WRAW, SM::WRAW, bar_w);
   };
@@ -557,9 +560,8 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   };
   if (queries) walk(std::true_type{});
   else walk(std::false_type{});
-  if (!waits.ok()) {  // copies that may still be on their way
-    for (int k = 0; k < 3; ++k) mbar_wait_bounded(bar + 8 * k, 0);
-  }
+  // copies that may still be on their way (the walk ends with a barrier, and thread 0 starts them all)
+  if (tid == 0 && !waits.ok()) waits.drain(copies, 3, bar);
 }
 
 template <typename T, int F>

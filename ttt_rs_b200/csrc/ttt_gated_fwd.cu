@@ -5,8 +5,8 @@
 // 16 in every chunk, since the last ones meet four blocks of keys and the first ones one: for each block of 16 tokens the
 // decayed products of queries and keys become, in registers, the A operand of the product with the block's values.  q W comes
 // last: the state before the chunk is there once all warps have left the chunk before, and until then a warp works on what needs only
-// this chunk's inputs, so that no warp waits for the others of its chunk.  The next two chunks are on their way meanwhile (TMA,
-// rows behind the sequence read as zeros).
+// this chunk's inputs, so that no warp waits for the others of its chunk.  The next chunk is on its way meanwhile (TMA, rows
+// behind the sequence read as zeros), fetched when all warps have left the chunk before.
 //
 // Few streams are cut into segments: a first launch leaves every segment's own state (as if it began with none) and its decay, a
 // second one joins them along the sequence, and the third is this kernel with a CTA per segment.
@@ -56,6 +56,7 @@ struct GatedFwdBlock {
     const uint32_t at = bar + 8 * slot, dst = base + (BF ? SM::TILES + slot * SM::NIN * SM::TILE : SM::RAWS);
     constexpr uint32_t bytes = BF ? SM::TILE : SM::RAW;
     const int b = s.stream / p.H, h = s.stream - b * p.H;
+    waits.started(copies(), slot, (BF ? s.i >> 1 : s.i) & 1);
     mbar_expect_tx(at, SM::NIN * bytes);
 #pragma unroll
     for (int m = 0; m < SM::NIN; ++m) tma_load_4d(dst + m * bytes, &maps.m[(STATE ? 1 : 0) + m], chunk_of(s) * GC, h, b, at);
@@ -87,11 +88,10 @@ struct GatedFwdBlock {
   __device__ __forceinline__ void settled(int i) const {
     if (i > 0) waits.wait(bar + 16 + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1, 25, i);
   }
+  __device__ __forceinline__ volatile int* copies() const { return reinterpret_cast<volatile int*>(mem + SM::BAR + 40); }
   __device__ __forceinline__ void drain() const {  // copies that may still be on their way
-    if (!waits.ok()) {
-      mbar_wait_bounded(bar, 0);
-      mbar_wait_bounded(bar + 8, 0);
-    }
+    block_sync();
+    if (tid == 0 && !waits.ok()) waits.drain(copies(), 2, bar);
   }
   static __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0, %0;" ::"n"(THREADS) : "memory"); }
   // W <- e^{G_end} W + sum of scaled keys^T values (REV: queries^T gradients, scaled by what is left at the token)
@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   volatile int* const shared = reinterpret_cast<volatile int*>(mem + SM::BAR + 32);  // a wait has run out; this block's range
   BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), {shared, p.status}, tid, lane, w, {}};
   if (tid == 0) {
-    shared[0] = 0;
+    shared[0] = bk.copies()[0] = bk.copies()[1] = 0;
     shared[1] = p.slots > 0 ? atomicAdd(p.flags + p.slots, 1) + p.first_slot : (int)blockIdx.x;
     mbar_init(bk.bar, 1);
     mbar_init(bk.bar + 8, 1);
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 :
   volatile int* const failed = reinterpret_cast<volatile int*>(mem + SM::BAR + 32);
   BK bk{maps, p, mem, base, base + SM::BAR, reinterpret_cast<ChunkGates*>(mem + SM::GATES), {failed, p.status}, tid, lane, w, {}};
   if (tid == 0) {
-    *failed = 0;
+    *failed = bk.copies()[0] = bk.copies()[1] = 0;
     mbar_init(bk.bar, 1);
     mbar_init(bk.bar + 8, 1);
     mbar_init(bk.bar + 16, GATED_WARPS);

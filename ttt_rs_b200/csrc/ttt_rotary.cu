@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(ROT_THREADS, rotary_resident(sizeof(T) == 4, N
       T* dst = static_cast<T*>(p.y[m]) + (b * p.ys[m][0] + h_lo * p.ys[m][1] + t * p.ys[m][2]);
       auto rows = [&](auto count) {  // so many rows, all of them on their way before the first is worked on
         constexpr int ROWS = decltype(count)::value;
-        Io in[ROWS][NU], grad[BWD ? ROWS : 1][NU];
+        Io in[ROWS][NU];
+        [[maybe_unused]] Io grad[BWD ? ROWS : 1][NU];
 #pragma unroll
         for (int q = 0; q < ROWS; ++q) {
 #pragma unroll
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(ROT_THREADS, rotary_resident(sizeof(T) == 4, N
                 for (int k = 0; k < H; ++k) sq = f2fma(x[n][k], x[n][k], f2fma(y[n][k], y[n][k], sq));
               }
             }
-            float r = 1.f;
+            [[maybe_unused]] float r = 1.f;
             if constexpr (NORM) r = rsqrtf(group_sum<LANES>(f2hsum(sq)) * inv_f + p.eps);
             if constexpr (!BWD) {
 #pragma unroll

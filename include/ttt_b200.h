@@ -352,7 +352,7 @@ int ttt_layer_qk_conv_backward(const ttt_dims* d, const void* grad_q, const void
  * length), head_dim (64 or 32; any number of heads) and dtype are read.
  *   xq, xk, xv    T [B,H,T,F] with rows of F contiguous elements; `strides`: for each of them the strides of batch, head and token
  *                 in elements, positive multiples of 16 bytes (null: contiguous [B,H,T,F]); strides of dimensions of size 1 are not read
- *   log_decay     float32 [B,H,T], not above 0 for a state that does not grow; -infinity (anything below -111) forgets everything
+ *   log_decay     float32 [B,H,T], at most 0; -infinity (anything below -111) forgets everything
  *                 before the token: sequences may follow one another in one row
  *   beta          float32 [B,H,T], or null: ones
  *   weight        float32 [B,H,F,F] state before the first token, W[k][v], or null: zeros

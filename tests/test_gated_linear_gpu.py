@@ -328,3 +328,69 @@ def test_refusals():
     refused(L.TTT_ERR_UNSUPPORTED, q=dev[0].half())
     refused(L.TTT_ERR_UNSUPPORTED, q=dev[0][..., :48], k=dev[1][..., :48], v=dev[2][..., :48])
     refused(L.TTT_ERR_CUDA, q=ins[0])
+
+
+def test_saved_states_go_with_the_backward():
+    """What the forward saves is freed by the backward, also while the results are kept."""
+    import ttt_rs_b200 as tb
+    ins, d_out, _ = make(4, 8, 1024, 64, torch.bfloat16)
+    dev = [t.cuda().requires_grad_() for t in ins]
+    torch.cuda.synchronize()
+    out, w = tb.fused_gated_linear(*dev)
+    before = torch.cuda.memory_allocated()
+    grads = torch.autograd.grad(out, dev, d_out.cuda())
+    held = torch.cuda.memory_allocated() - sum(t.numel() * t.element_size() for t in grads)
+    assert held <= before - 4 * 8 * 16 * 64 * 64 * 4 + 65536
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(w, dev, torch.ones_like(w))
+
+
+def test_gradients_of_gradients_are_refused():
+    import ttt_rs_b200 as tb
+    ins, _, _ = make(1, 2, 20, 64, torch.float32)
+    dev = [t.cuda().requires_grad_() for t in ins]
+    out, _ = tb.fused_gated_linear(*dev)
+    want = torch.autograd.grad(out.sum(), dev, retain_graph=True)
+    got = torch.autograd.grad(out.sum(), dev, create_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        sum(x.square().sum() for x in got).backward()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_what_is_not_finite_stays_in_its_stream_and_behind_its_chunk(bad):
+    import ttt_rs_b200 as tb
+    ins, _, _ = make(2, 2, 200, 64, torch.bfloat16, seed=6)
+    want = run(ins)
+    for x in ins[:3]:
+        x[1, 0, 130] = bad
+    got = run(ins)
+    rest = torch.ones(2, 2, 200, dtype=torch.bool)
+    rest[1, 0, 128:] = False
+    assert torch.equal(got[0].cpu()[rest], want[0].cpu()[rest])
+    assert not torch.isfinite(got[0][1, 0, 130:]).all(-1).any()
+    others = torch.tensor([[True, True], [False, True]])
+    assert torch.equal(got[1].cpu()[others], want[1].cpu()[others])
+    tb.check_status()
+
+
+def test_offsets_behind_32_bits():
+    """9 sequences of 2^20 tokens and 4 heads as views of [B,T,H,F], 2.4e9 elements a tensor: the last tokens of the last stream against
+    a call on those alone from the state before them."""
+    import ttt_rs_b200 as tb
+    B, H, T, F, last = 9, 4, 1 << 20, 64, 100
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(3, 1, T, H, F, generator=gen, device="cuda", dtype=torch.bfloat16)
+    q, k, v = (t.expand(B, T, H, F).contiguous().transpose(1, 2) for t in x)
+    decay = -0.3 * torch.rand(B, H, T, generator=gen, device="cuda")
+    with torch.no_grad():
+        out, _ = tb.fused_gated_linear(q, k, v, decay)
+        cut = T - last
+        _, state = tb.fused_gated_linear(q[-1:, :, :cut], k[-1:, :, :cut], v[-1:, :, :cut], decay[-1:, :, :cut])
+        del q
+        tail = [t[0].transpose(0, 1)[None, :, cut:].float() for t in x]
+        want, _ = tb.fused_gated_linear(*tail, decay[-1:, :, cut:], None, state)
+    tb.check_status()
+    # bf16 results against float32 ones of the same inputs and (up to the order of their sums) the same state: three roundings
+    mag, _ = tb.fused_gated_linear(*[t.abs() for t in tail], decay[-1:, :, cut:], None, state.abs())
+    assert ((out[-1:, :, cut:].float() - want).abs() <= 3 * 2 ** -8 * mag + F32 * mag).all()

@@ -193,3 +193,9 @@ def test_refused_configurations():
         with pytest.raises(ValueError):
             tb.TTT(tb.TTTLayerConfig(hidden_size=128, num_heads=2, **kw), device="cuda")
     assert math.isclose(tb.TTTLayerConfig(128, 2, rope_scaling="by_parts", rope_factor=math.e, rope_original_length=64).rotary_config().size, 1.1)
+
+
+def test_base_lr_of_the_recurrence_is_positive():
+    import ttt_rs_b200 as tb
+    with pytest.raises(ValueError):
+        tb.GatedLinear(2, 64, base_lr=0.0)

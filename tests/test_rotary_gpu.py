@@ -287,3 +287,51 @@ def test_refusals():
     refused(L.TTT_ERR_SHAPE, lambda: tb.qk_norm_rotary(x, x[:, :, :4], rot=rot))
     refused(L.TTT_ERR_SHAPE, lambda: tb.qk_norm_rotary(x, x, torch.ones(64, device="cuda", dtype=torch.bfloat16), rot=rot))
     refused(L.TTT_ERR_SHAPE, lambda: tb.qk_norm_rotary(x, x, eps=-1.0))
+
+
+def test_results_that_lie_over_another_tensor_are_refused():
+    import ttt_rs_b200 as tb
+    from ttt_rs_b200 import _lib as L
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    flat = torch.zeros(2 * 3 * 8 * 64 + 64, device="cuda")
+    x, moved = flat[:-64].view(2, 3, 8, 64), flat[64:].view(2, 3, 8, 64)
+    q, k = torch.zeros(2, 2, 3, 8, 64, device="cuda")
+
+    def refused(call):
+        with pytest.raises(tb.TttError) as e:
+            call()
+        assert e.value.code == L.TTT_ERR_SHAPE
+
+    refused(lambda: tb.rotary(x, rot, out=moved))
+    refused(lambda: tb.rotary(x, rot, out=flat.as_strided((2, 3, 8, 64), (3 * 64, 64, 64, 1))))
+    refused(lambda: tb.qk_norm_rotary(q, k, rot=rot, out=(k, q)))
+    refused(lambda: tb.qk_norm_rotary(q, k, rot=rot, out=(q, q)))
+    refused(lambda: tb.qk_norm_rotary(x, k, rot=rot, out=(moved, k)))
+    both = torch.zeros(2, 8, 2, 3, 64, device="cuda")  # columns of one projection, each normed where it lies
+    cols = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    got = tb.qk_norm_rotary(*cols, rot=rot, out=cols)
+    assert got[0].data_ptr() == cols[0].data_ptr()
+
+
+def test_gradients_of_gradients_are_refused():
+    import ttt_rs_b200 as tb
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    x, w = torch.randn(2, 3, 8, 64, device="cuda").requires_grad_(), torch.ones(64, device="cuda").requires_grad_()
+    for y in (tb.rotary(x, rot), tb.qk_norm_rotary(x, x, w, w, rot)[0]):
+        (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            dx.sum().backward()
+
+
+def test_rotary_offsets_behind_32_bits():
+    import ttt_rs_b200 as tb
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    B, T, H, F = 9, 1 << 20, 4, 64
+    x = torch.zeros(B, T, H, F, device="cuda", dtype=torch.bfloat16)
+    x[-1, -5:] = torch.randn(5, H, F, device="cuda")
+    y = tb.rotary(x.transpose(1, 2), rot)
+    want = tb.rotary(x[-1:, -5:].transpose(1, 2).contiguous(), rot, start_idx=T - 5)
+    assert torch.equal(y[-1:, :, -5:], want)
+    n, _ = tb.qk_norm_rotary(x.transpose(1, 2), x.transpose(1, 2), rot=rot)
+    want, _ = tb.qk_norm_rotary(x[-1:, -5:].transpose(1, 2), x[-1:, -5:].transpose(1, 2), rot=rot, start_idx=T - 5)
+    assert torch.equal(n[-1:, :, -5:], want)

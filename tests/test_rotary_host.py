@@ -106,3 +106,10 @@ def test_qk_norm_refuses(lib):
     assert backward(ws_bytes=need - 4) == backward(ws=None) == _lib.TTT_ERR_WORKSPACE
     assert backward(gq=None) == backward(dk=None) == _lib.TTT_ERR_NULL
     assert backward(dwq=C.c_void_p(0x1001)) == _lib.TTT_ERR_ALIGN
+
+
+@pytest.mark.parametrize("strides", [(192, 64, 64), (640, 640, 64), (1920, 640, 1), (1919, 640, 64), (128, 256, 800), (1 << 61, 640, 64)])
+def test_rows_of_a_result_must_not_overlap(lib, strides):
+    rot = rotation()
+    ys = (C.c_int64 * 3)(*strides)
+    assert lib.ttt_layer_rotary(C.byref(dims(batch=3)), FAKE, None, C.byref(rot), 0, FAKE, ys, None) == _lib.TTT_ERR_SHAPE

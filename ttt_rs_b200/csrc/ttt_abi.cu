@@ -1,5 +1,6 @@
 // C ABI of the fused TTT inner loop: argument validation, TMA descriptor set-up and kernel launches.
 // Signatures and their reference counterparts are documented in include/ttt_b200.h.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <atomic>
@@ -1547,9 +1548,19 @@ int set_rows(int64_t (&out)[3], const ttt_dims* d, int heads, const void* base, 
   if (reinterpret_cast<uintptr_t>(base) % 16 != 0) *vec = false;
   for (int k = 0; k < 3; ++k) {
     out[k] = size[k] == 1 ? 0 : strides != nullptr ? strides[3 * i + k] : dense[k];
-    if (size[k] > 1 && (written ? out[k] < F : out[k] < 0))
-      return fail(TTT_ERR_SHAPE, written ? "rows of %s overlap" : "the strides of %s must not be negative", name);
+    if (out[k] < 0) return fail(TTT_ERR_SHAPE, "the strides of %s must not be negative", name);
     if (out[k] * es % 16 != 0) *vec = false;
+  }
+  if (written) {  // every stride is at least as long as what the smaller ones reach over
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int a, int b) { return out[a] < out[b]; });
+    int64_t extent = F;
+    for (int k : order) {
+      if (size[k] == 1) continue;
+      if (out[k] < extent) return fail(TTT_ERR_SHAPE, "rows of %s overlap", name);
+      if (out[k] > ((int64_t)1 << 62) / size[k]) return fail(TTT_ERR_SHAPE, "the strides of %s are out of range", name);
+      extent += out[k] * (size[k] - 1);
+    }
   }
   return TTT_OK;
 }

@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/autocast_mode.h>
 #include <torch/csrc/Exceptions.h>
@@ -306,6 +307,15 @@ struct Gated {
   }
 };
 
+// What a node's backward returns where it is itself recorded (create_graph): gradients that say so when they are differentiated, since
+// the kernels' gradients are not functions that autograd knows.
+variable_list only_once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_();
+  return torch::autograd::DelayedError("the gradients of this operator are not differentiable", (int64_t)grads.size())(std::move(grads));
+}
+
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
                                const Tensor& beta, const Tensor& w, bool has_beta, bool has_w) {
@@ -314,9 +324,8 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     call.m.set(q, q.size(3), 1, 1, 0);
     const int rc = call.forward(q, k, v, g, has_beta ? beta : Tensor(), has_w ? w : Tensor(), true, out, w_out, saved);
     if (rc != TTT_OK) throw_error(rc);
-    ctx->save_for_backward({q, k, v, g, beta});
+    ctx->save_for_backward({q, k, v, g, beta, saved});
     ctx->saved_data["has"] = std::vector<int64_t>{has_beta, has_w};
-    ctx->saved_data["s"] = saved;
     ctx->set_materialize_grads(false);
     return {out, w_out};
   }
@@ -324,7 +333,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     const variable_list t = ctx->get_saved_variables();
     const std::vector<int64_t> has = ctx->saved_data["has"].toIntVector();
     const Tensor &q = t[0], &k = t[1], &v = t[2], &g = t[3], beta = has[0] ? t[4] : Tensor();
-    const Tensor saved = ctx->saved_data["s"].toTensor();
+    const Tensor& saved = t[5];
     if (!go[0].defined() && !go[1].defined()) return variable_list(8);
     Gated call;
     call.m.set(q, q.size(3), 1, 1, 0);
@@ -345,7 +354,7 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
         static_cast<float*>(dg.data_ptr()), beta.defined() ? static_cast<float*>(db.data_ptr()) : nullptr,
         static_cast<float*>(dw.data_ptr()), wsb != 0 ? ws.data_ptr() : nullptr, wsb, m.status.data_ptr(), m.stream());
     if (rc != TTT_OK) throw_error(rc);
-    return {dq, dk, dv, dg, db, has[1] ? dw : Tensor(), Tensor(), Tensor()};
+    return only_once({dq, dk, dv, dg, db, has[1] ? dw : Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -429,7 +438,7 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     rot.set(m);
     const int rc = rotary(m, g, rot, true, y);
     if (rc != TTT_OK) throw_error(rc);
-    return {y, Tensor(), Tensor(), Tensor(), Tensor()};
+    return only_once({y, Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 struct QkNorm {
@@ -500,7 +509,7 @@ struct QkNormFn : torch::autograd::Function<QkNormFn> {
     Tensor dq, dk, dwq, dwk;
     const int rc = call.backward(t[0], t[1], go[0], go[1], w0, w1, rot, dq, dk, dwq, dwk);
     if (rc != TTT_OK) throw_error(rc);
-    return {dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return only_once({dq, dk, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
   }
 };
 
@@ -1135,8 +1144,14 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// (a result may be the input itself; two tensors that lie over one another otherwise are left to the caller's check)
+bool apart(const Tensor& y, const Tensor& x, bool or_same) {
+  if (!y.defined() || !x.defined()) return true;
+  const at::MemOverlapStatus s = at::get_overlap_status(y, x);
+  return s != at::MemOverlapStatus::Partial && (s != at::MemOverlapStatus::Full || (or_same && y.strides() == x.strides()));
+}
 bool same_shape_result(const Tensor& y, const Tensor& x, const Dims& m) {
-  return !y.defined() || (head_rows(y, m.dev, m.dt) && y.sizes() == x.sizes());
+  return !y.defined() || (head_rows(y, m.dev, m.dt) && y.sizes() == x.sizes() && apart(y, x, true));
 }
 // rotary(x, rotation (7), inverse, out | None) -> y, recorded for autograd where that is on and asked for | None
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -1170,7 +1185,8 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
           !optional_tensor(args[12], yq) || !optional_tensor(args[13], yk));
   const double eps = PyFloat_AsDouble(args[11]);
   if (PyErr_Occurred()) return nullptr;
-  NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m));
+  NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m) ||
+          !apart(yq, x[1], false) || !apart(yk, x[0], false) || !apart(yq, yk, false));
   if (wants_grad({&x[0], &x[1], &wq, &wk})) {
     NONE_IF(yq.defined() || yk.defined());
     std::vector<int64_t> ints = rot.ints();

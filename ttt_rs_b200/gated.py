@@ -39,7 +39,8 @@ def fused_gated_linear(xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, log
     bfloat16, head_dim 64 or 32; views of [B,T,H,F] or of a projection are read where they lie), from the state `weight`
     [B,H,F,F] float32 (None: zeros).  log_decay [B,H,T] float32, at most 0; -inf forgets everything before the token, so that
     sequences may follow one another in one row.  beta [B,H,T] float32 (None: ones).  Differentiable with respect to all six,
-    through both results; without gradients a call of up to 16 tokens runs as a decode step."""
+    through both results (once: gradients of gradients are refused); without gradients a call of up to 16 tokens runs as a decode
+    step.  A NaN or an infinity in a token reaches results of the 64 tokens around it, and no reset forgets one in the state."""
     native = _lib.host().gated(xq, xk, xv, log_decay, beta, weight)
     if native is not None:
         return native
@@ -82,6 +83,8 @@ class GatedLinear(torch.nn.Module):
 
     def __init__(self, num_heads: int, head_dim: int, base_lr: float = 1.0, device=None):
         super().__init__()
+        if not base_lr > 0.0:
+            raise ValueError(f"base_lr must be positive (got {base_lr})")
         self.num_heads, self.head_dim, self.base_lr = num_heads, head_dim, base_lr
         kw = dict(device=device, dtype=torch.float32)
         self.weight_init = torch.nn.Parameter(torch.randn(num_heads, head_dim, head_dim, **kw) * 0.02)

@@ -302,6 +302,7 @@ class _HeadsFn(torch.autograd.Function):
         return xq, xk, xv, lr
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dxq, dxk, dxv, dlr):
         proj, q_weight, k_weight, lr = ctx.saved_tensors
         cfg, cols, start_idx = ctx.meta

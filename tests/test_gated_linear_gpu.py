@@ -394,3 +394,28 @@ def test_offsets_behind_32_bits():
     # bf16 results against float32 ones of the same inputs and (up to the order of their sums) the same state: three roundings
     mag, _ = tb.fused_gated_linear(*[t.abs() for t in tail], decay[-1:, :, cut:], None, state.abs())
     assert ((out[-1:, :, cut:].float() - want).abs() <= 3 * 2 ** -8 * mag + F32 * mag).all()
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_a_long_memory_keeps_its_digits(reverse):
+    """128 chunks through a decay close to one, of as many streams as run without segments: the state (reverse: its gradient) as a
+    whole.  It is rounded once per chunk, to nearest: at most 2^-24 of the largest state on the way each, 128 * 2^-24 = 2^-17 in all, the
+    last of the states being the largest; a chunk's own part, of truncated sums of 12 products, 12 * 2^-23 of it, less than 2^-19.
+    Together below 2^-16.  (Sums truncated onto the state itself lose 12 * 2^-24 of it per chunk on average, 2^-14 or half of that
+    over a growing state.)"""
+    import ttt_rs_b200 as tb
+    B, H, T = 4, 37, 128 * 64
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    q, k, v, u = torch.randn(4, B, H, T, 64, generator=gen, device="cuda").bfloat16()
+    decay = torch.full((B, H, T), -2.0 ** -17, device="cuda")
+    sums = torch.cumsum(decay.double(), -1)
+    if reverse:
+        w = torch.zeros(B, H, 64, 64, device="cuda").requires_grad_()
+        out, _ = tb.fused_gated_linear(q, k, v, decay, None, w)
+        (got,) = torch.autograd.grad(out, w, u)
+        want = (q.double() * torch.exp(sums)[..., None]).transpose(2, 3) @ u.double()
+    else:
+        with torch.no_grad():
+            _, got = tb.fused_gated_linear(q, k, v, decay)
+        want = (k.double() * torch.exp(sums[..., -1:] - sums)[..., None]).transpose(2, 3) @ v.double()
+    assert (got.double() - want).norm() <= 2 ** -16 * want.norm()

@@ -14,9 +14,10 @@
 // Operands.  bf16 inputs go to the tensor cores as they are; what a result of the inputs' type alone depends on is rounded to bf16 where
 // it becomes an operand (the decayed products, the state in q W).  What float32 results depend on is not: the scaled keys and
 // queries whose products make up the state and its gradient are carried as three bf16 planes (24 bits of mantissa, as float32; two
-// planes left 2.5e-6 of the state, three 5e-7, for 4 % of the forward's time), the state and its gradient in the sums for the gates'
-// gradients as two (2^-17 of a term; a third plane of both does not fit beside the tiles of two chunks).  float32
-// inputs are carried as three planes throughout, as in the other float32 kernels.
+// planes left 2.5e-6 of the state, three 5e-7, for 4 % of the forward's time), and so are the state and its gradient in the sums for
+// the gates' gradients (two planes: 1.9e-6 of those, three 4e-7, for 8 % of the training pass).  float32 inputs are carried as three planes
+// throughout, as in the other float32 kernels.  A chunk's part of the state is a sum of its own, added to the decayed state by a fused
+// multiply-add: the tensor cores truncate as they add, and onto the state itself that lost 2e-5 of it in 128 chunks of weak decay.
 #pragma once
 
 #include "ttt_common.cuh"
@@ -86,6 +87,12 @@ __device__ __forceinline__ void scale_cols(float (&c)[4], F2 f) {
   const F2 x = f2mul(make_float2(c[0], c[1]), f), y = f2mul(make_float2(c[2], c[3]), f);
   c[0] = x.x, c[1] = x.y, c[2] = y.x, c[3] = y.y;
 }
+// c = c times a factor + d
+__device__ __forceinline__ void scale_add(float (&c)[4], float a, const float (&d)[4]) {
+  const F2 x = f2fma(make_float2(c[0], c[1]), f2(a), make_float2(d[0], d[1]));
+  const F2 y = f2fma(make_float2(c[2], c[3]), f2(a), make_float2(d[2], d[3]));
+  c[0] = x.x, c[1] = x.y, c[2] = y.x, c[3] = y.y;
+}
 // d += rows of c times a factor each
 __device__ __forceinline__ void add_rows(float (&d)[4], const float (&c)[4], float a, float b) {
   const F2 x = f2fma(make_float2(c[0], c[1]), f2(a), make_float2(d[0], d[1]));
@@ -135,15 +142,15 @@ struct ChunkGates {
   float into[GC];        // the same of the state before i's block
   float out[GC];         // what is left of token i behind its block
   float out_b[GC];       // that times beta_i
-  float end_b[GC];       // what is left of token i behind the chunk, times beta_i
-  float end[GC];         // without beta_i
+  float end[GC];         // what is left of token i behind the chunk (forward: times beta_i)
   float beta[GC];
   float blocks[4][4];    // [a][b]: from the end of block a to the end of block b >= a
   float starts[4];       // e^G before block a
   float all;             // e^{G_end}
   float pad[3];
 };
-// One warp; lane l brings tokens 2l and 2l + 1 of the chunk.  Tokens behind the sequence: g = 0, beta = 0.
+// FORWARD: `end` comes with the factor beta.  One warp; lane l brings tokens 2l and 2l + 1 of the chunk.  Tokens behind the sequence: g = 0, beta = 0.
+template <bool FORWARD>
 __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2 g, float2 beta) {
   auto log2_of = [](float x) {
     const double v = (double)x * 1.4426950408889634;
@@ -173,8 +180,7 @@ __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2
   const float e0 = pow2((float)(end - G0)), e1 = pow2((float)(end - G1));
   put(s.out, o0, o1);
   put(s.out_b, o0 * beta.x, o1 * beta.y);
-  put(s.end, e0, e1);
-  put(s.end_b, e0 * beta.x, e1 * beta.y);
+  put(s.end, FORWARD ? e0 * beta.x : e0, FORWARD ? e1 * beta.y : e1);
   put(s.beta, beta.x, beta.y);
   if (lane < 16) {
     const int a = lane >> 2, b = lane & 3;
@@ -215,24 +221,8 @@ __device__ __forceinline__ float2 load_gates(const float* x, int t0, int T, int 
   return v;
 }
 
-// Four registers of the four lanes of a quad, turned: lane t gets register t of lanes 0..3, in their order
-__device__ __forceinline__ void quad_transpose(uint32_t (&r)[4], int lane) {
-  const bool odd = lane & 1, high = lane & 2;
-#pragma unroll
-  for (int k = 0; k < 4; k += 2) {
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? r[k] : r[k + 1], 1);
-    if (odd) r[k] = got;
-    else r[k + 1] = got;
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? r[k] : r[k + 2], 2);
-    if (high) r[k] = got;
-    else r[k + 2] = got;
-  }
-}
-// Accumulators of 16 rows x F columns to global rows base[row * F], rows below `rows`.  bf16: 64 contiguous bytes per row and
-// store (four lanes of 16), float32: 32.
+// Accumulators of 16 rows x F columns to global rows base[row * F], rows below `rows`: the four lanes of a row store
+// 32 bytes side by side (bf16 in 64, after more shuffles: 1 % of the training pass slower).
 template <typename T, int F>
 __device__ __forceinline__ void store_rows(T* base, int row0, int rows, const float (&c)[F / 8][4], int lane) {
   const int g = lane >> 2, t = lane & 3;
@@ -241,12 +231,12 @@ __device__ __forceinline__ void store_rows(T* base, int row0, int rows, const fl
     const int row = row0 + g + 8 * half;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int n = 0; n < F / 8; n += 4) {
-        uint32_t r[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) r[k] = pack_bf16(c[n + k][2 * half], c[n + k][2 * half + 1]);
-        quad_transpose(r, lane);
-        if (row < rows) *reinterpret_cast<uint4*>(base + (size_t)row * F + 8 * (n + t)) = make_uint4(r[0], r[1], r[2], r[3]);
+      for (int n = 0; n < F / 8; n += 2) {  // two lanes swap halves of two tiles: 8 bytes each, whole sectors of 32
+        const uint32_t x = pack_bf16(c[n][2 * half], c[n][2 * half + 1]), y = pack_bf16(c[n + 1][2 * half], c[n + 1][2 * half + 1]);
+        const bool odd = lane & 1;
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? x : y, 1);
+        if (row < rows)
+          *reinterpret_cast<uint2*>(base + (size_t)row * F + 8 * (n + (t & 1)) + 4 * (t >> 1)) = odd ? make_uint2(got, y) : make_uint2(x, got);
       }
     } else if (row < rows) {
 #pragma unroll
@@ -271,12 +261,9 @@ __device__ __forceinline__ void split_rows(uint32_t planes, uint32_t plane_strid
                    : "memory");
   }
 }
-__device__ __forceinline__ void st_shared_b32(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t ld_shared_b32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
 
@@ -399,10 +386,11 @@ struct StateShare {
   static constexpr int SLABS = F / 16, PARTS = GATED_WARPS / SLABS, COLS = F / PARTS, NT = COLS / 8;
 };
 
-// A warp's share of the state (rows row0.., columns col0..) as NP bf16 planes (STATE_BYTES apart) in the tile layout of shared
+// A warp's share of the state (rows row0.., columns col0..) as NP bf16 planes (`stride` bytes apart) in the tile layout of shared
 // memory
 template <int F, int NP>
-__device__ __forceinline__ void put_state(const float (&w)[StateShare<F>::NT][4], int row0, int col0, uint32_t smem, int lane) {
+__device__ __forceinline__ void put_state(const float (&w)[StateShare<F>::NT][4], int row0, int col0, uint32_t smem, int lane,
+                                          uint32_t stride = GTile<F>::STATE_BYTES) {
   const uint32_t at = smem + row0 * GTile<F>::ROW + GTile<F>::low(lane);
 #pragma unroll
   for (int n = 0; n < StateShare<F>::NT; n += 2) {
@@ -410,7 +398,7 @@ __device__ __forceinline__ void put_state(const float (&w)[StateShare<F>::NT][4]
     as_operand<NP>(v, w[n], w[n + 1]);
 #pragma unroll
     for (int i = 0; i < NP; ++i)
-      stsm_x4((at ^ ((col0 + 8 * n) << 1)) + i * GTile<F>::STATE_BYTES, v[0].p[i], v[1].p[i], v[2].p[i], v[3].p[i]);
+      stsm_x4((at ^ ((col0 + 8 * n) << 1)) + i * stride, v[0].p[i], v[1].p[i], v[2].p[i], v[3].p[i]);
   }
 }
 // The same share as the threads hold it, 16 bytes a thread side by side (what the forward saves for the backward)

@@ -15,8 +15,8 @@
 //
 // One CTA of eight warps per stream (or segment) walks the chunks from the last.  Warps 0-3 own 16 queries each: dq, and the
 // float32 dW in their registers with its update.  Warps 4-7 own 16 keys each: dk, dv and the gates' sums.  Per chunk two
-// barriers: all warps at its end, and the second group once more before it reads dW, which the first publishes after the first
-// barrier.
+// barriers: all warps at its end, and the second group once more before it reads dW, which the first publishes when it has
+// read the state (their third planes share their bytes).
 #include <type_traits>
 
 #include "ttt_kernels.h"
@@ -32,7 +32,7 @@ struct ChunkSums {
   float r[GC], s[GC];               // r_i; beta_j s_j
   // the ways inside the chunk, from the block of 16 tokens that they start in to the one they end in:
   float c[GC];                      // sum over the blocks behind j's of beta_j N_ij
-  float rows[GATED_WARPS][GC];      // sum over the j of a block (= a warp) before i's of beta_j N_ij
+  float rows[GATED_WARPS - 1][GC];  // sum over the j of a block (= a warp) before i's of beta_j N_ij
   float block[GC];                  // those within a block that lead across token t
   float through[GATED_WARPS];       // e^{G_end} <W, dW>, by warp
 };
@@ -40,17 +40,19 @@ struct ChunkSums {
 template <typename T, int F>
 struct GatedBwdSmem {
   static constexpr bool BF = sizeof(T) == 2;
-  static constexpr int NP = BF ? 1 : 3, NS = BF ? 2 : 3;
+  static constexpr int NP = BF ? 1 : 3, NS = 3;
   static constexpr uint32_t PLANE = GTile<F>::BYTES, TILE = NP * PLANE, RAW = GC * F * 4, WRAW = F * F * 4;
-  static constexpr uint32_t STATE = NS * GTile<F>::STATE_BYTES;
+  static constexpr uint32_t SP = GTile<F>::STATE_BYTES;
   static constexpr uint32_t STAGES = BF ? 2 : 1;
   static constexpr uint32_t TILES = 0, RAWS = TILES + STAGES * 4 * TILE;
   static constexpr uint32_t WSAVED = RAWS + (BF ? 0 : 2 * RAW);  // as it was saved; bf16: its planes take the same bytes
-  static constexpr uint32_t W = BF ? WSAVED : WSAVED + WRAW, DW = W + STATE;
-  static constexpr uint32_t GATES = DW + STATE;
+  // planes of W upwards from W, of dW from DW in steps of DWS.  bf16: the third ones take the same bytes one after the other (both do
+  // not fit beside the tiles of two chunks, two blocks per SM), dW from the last plane down
+  static constexpr uint32_t W = BF ? WSAVED : WSAVED + WRAW, DW = W + (BF ? 4 : 3) * SP, DWS = BF ? 0u - SP : SP;
+  static constexpr uint32_t GATES = W + (BF ? 5 : 6) * SP;
   static constexpr uint32_t SUMS = GATES + 2 * sizeof(ChunkGates);
   static constexpr uint32_t BAR = SUMS + 2 * sizeof(ChunkSums), BYTES = BAR + 48 + 1024;
-  static_assert(!BF || STATE == WRAW, "two planes of bf16 are as long as the float32 state");
+  static_assert(!BF || 2 * SP == WRAW, "two planes of bf16 are as long as the float32 state");
 };
 
 template <typename T, int F>
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
   if (tid < 32) {
     float2 g0, b0;
     gates_of(first, g0, b0);
-    make_chunk_gates(gates[0], lane, g0, b0);
+    make_chunk_gates<false>(gates[0], lane, g0, b0);
   }
   const int row0 = 16 * (w % SH::SLABS), part = w / SH::SLABS, col0 = part * SH::COLS;
   __syncthreads();
@@ -211,10 +213,6 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
     const uint32_t tw = base + SM::W, tdw = base + SM::DW;
     const ChunkGates& cg = gates[i & 1];
     ChunkSums& cs = sums[i & 1];
-    if constexpr (QUERIES) {  // dW behind this chunk, for the other group
-      put_state<F, NS>(dW, row0, col0, tdw, lane);
-      asm volatile("bar.arrive 1, %0;" ::"n"(GB_THREADS) : "memory");
-    }
     waits.wait(bar + 8 * slot, BF ? (i >> 1) & 1 : 0, 21, i);
     if constexpr (!BF) {
       auto split2 = [&](uint32_t dst) {
@@ -256,19 +254,21 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
       }
       // W u, for r and, from the start of this warp's block on, for dq
-      Pk<NP> u[KS][4];
-#pragma unroll
+#pragma unroll 1
       for (int k = 0; k < KS; ++k) {
-        ldsm_np<NP>(u[k], uq ^ (k << 5), SM::PLANE, false);
+        Pk<NP> v[4];
+        ldsm_np<NP>(v, uq ^ (k << 5), SM::PLANE, false);
 #pragma unroll
         for (int m = 0; m < KS; ++m) {
           Pk<NS> f[4];
           ldsm_np<NS>(f, (tw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
-          mma_planes<NP, NS>(dq[2 * m], dq[2 * m + 1], u[k], f);
+          mma_planes<NP, NS>(dq[2 * m], dq[2 * m + 1], v, f);
         }
       }
       asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
       if (tid == 0 && i + 1 < n) fetch_w(nx);
+      put_state<F, NS>(dW, row0, col0, tdw, lane, SM::DWS);  // dW behind this chunk, for the other group
+      asm volatile("bar.arrive 1, %0;" ::"n"(GB_THREADS) : "memory");
       F2 sa = f2(0.f), sb = f2(0.f);
 #pragma unroll
       for (int m = 0; m < KS; ++m) {  // (an A fragment is two accumulator tiles)
@@ -285,6 +285,9 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         cs.r[ia] = r0;
         cs.r[ia + 8] = r1;
       }
+      Pk<NP> u[KS][4];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) ldsm_np<NP>(u[k], uq ^ (k << 5), SM::PLANE, false);
       const float first = cg.starts[w];
 #pragma unroll
       for (int k = 0; k < F / 8; ++k) scale_rows(dq[k], first, first);
@@ -329,8 +332,9 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       }
       store_rows<T, F>(static_cast<T*>(p.dq) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dq, lane);
       // dW before the chunk
+      float sum[SH::NT][4];  // (the tensor cores truncate as they add: not onto dW)
 #pragma unroll
-      for (int k = 0; k < SH::NT; ++k) scale_rows(dW[k], all, all);
+      for (int k = 0; k < SH::NT; ++k) sum[k][0] = sum[k][1] = sum[k][2] = sum[k][3] = 0.f;
 #pragma unroll 1
       for (int it = 0; it < GC / 16; ++it) {
         Pk<3> qt[4];
@@ -343,9 +347,11 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         for (int k = 0; k < SH::NT / 2; ++k) {
           Pk<NP> f[4];
           ldsm_np<NP>(f, (tu + 16 * it * TL::ROW + low) ^ ((col0 + 16 * k) << 1), SM::PLANE, true);
-          mma_planes<3, NP>(dW[2 * k], dW[2 * k + 1], qt, f);
+          mma_planes<3, NP>(sum[2 * k], sum[2 * k + 1], qt, f);
         }
       }
+#pragma unroll
+      for (int k = 0; k < SH::NT; ++k) scale_add(dW[k], all, sum[k]);
     } else {
       const int ja = 16 * w + g;
       const float oa = cg.out[ja], ob = cg.out[ja + 8], ba = cg.beta[ja], bb = cg.beta[ja + 8];
@@ -487,14 +493,17 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         float dv[F / 8][4];
 #pragma unroll
         for (int k = 0; k < F / 8; ++k) dv[k][0] = dv[k][1] = dv[k][2] = dv[k][3] = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)  // (dv is a result of the inputs' type: bf16 takes the leading plane of dW)
+#pragma unroll 1
+        for (int k = 0; k < KS; ++k) {  // (dv is a result of the inputs' type: bf16 takes the leading plane of dW)
+          Pk<NP> a[4];
+          ldsm_np<NP>(a, kq ^ (k << 5), SM::PLANE, false);
 #pragma unroll
           for (int m = 0; m < KS; ++m) {
             Pk<NP> f[4];
-            ldsm_np<NP>(f, (tdw + 16 * k * TL::ROW + low) ^ (m << 5), TL::STATE_BYTES, true);
-            mma_planes<NP, NP>(dv[2 * m], dv[2 * m + 1], k_[k], f);
+            ldsm_np<NP>(f, (tdw + 16 * k * TL::ROW + low) ^ (m << 5), SM::DWS, true);
+            mma_planes<NP, NP>(dv[2 * m], dv[2 * m + 1], a, f);
           }
+        }
         gather(dv, as, tu);
         store_rows<T, F>(static_cast<T*>(p.dv) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dv, lane);
       }
@@ -503,14 +512,14 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         float dk[F / 8][4];
 #pragma unroll
         for (int k = 0; k < F / 8; ++k) dk[k][0] = dk[k][1] = dk[k][2] = dk[k][3] = 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int k = 0; k < KS; ++k) {
           Pk<NP> v[4];
           ldsm_np<NP>(v, vq ^ (k << 5), SM::PLANE, false);
 #pragma unroll
           for (int m = 0; m < KS; ++m) {
             Pk<NS> f[4];
-            ldsm_np<NS>(f, (tdw + 16 * m * TL::ROW + high) ^ (k << 5), TL::STATE_BYTES, false);
+            ldsm_np<NS>(f, (tdw + 16 * m * TL::ROW + high) ^ (k << 5), SM::DWS, false);
             mma_planes<NP, NS>(dk[2 * m], dk[2 * m + 1], v, f);
           }
         }
@@ -538,7 +547,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         }
       }
     }
-    if (ahead) make_chunk_gates(gates[(i + 1) & 1], lane, g_next, b_next);
+    if (ahead) make_chunk_gates<false>(gates[(i + 1) & 1], lane, g_next, b_next);
     if constexpr (QUERIES) {
       if (st.ends) {
         if (st.pos == p.NC - 1) {

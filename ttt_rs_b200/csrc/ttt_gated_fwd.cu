@@ -97,10 +97,10 @@ struct GatedFwdBlock {
   // W <- e^{G_end} W + sum of scaled keys^T values (REV: queries^T gradients, scaled by what is left at the token)
   __device__ __forceinline__ void update(float (&W)[SH::NT][4], uint32_t tk, uint32_t tv, const ChunkGates& cg, int row0, int col0) const {
     const uint32_t low = TL::low(lane), high = TL::high(lane);
-    const float all = cg.all;
+    float sum[SH::NT][4];  // (the tensor cores truncate as they add: not onto the state)
 #pragma unroll
-    for (int k = 0; k < SH::NT; ++k) scale_rows(W[k], all, all);
-    const float* scale = REV ? cg.from : cg.end_b;
+    for (int k = 0; k < SH::NT; ++k) sum[k][0] = sum[k][1] = sum[k][2] = sum[k][3] = 0.f;
+    const float* scale = REV ? cg.from : cg.end;
 #pragma unroll 1
     for (int jt = 0; jt < GC / 16; ++jt) {
       const int j0 = 16 * jt + 2 * (lane & 3);
@@ -115,9 +115,12 @@ struct GatedFwdBlock {
       for (int m = 0; m < SH::NT / 2; ++m) {
         Pk<NP> f[4];
         ldsm_np<NP>(f, v ^ ((col0 << 1) + (m << 5)), SM::PLANE, true);
-        mma_planes<NS, NP>(W[2 * m], W[2 * m + 1], kt, f);
+        mma_planes<NS, NP>(sum[2 * m], sum[2 * m + 1], kt, f);
       }
     }
+    const float all = cg.all;
+#pragma unroll
+    for (int k = 0; k < SH::NT; ++k) scale_add(W[k], all, sum[k]);
   }
 };
 
@@ -157,7 +160,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
   if (w < 2 && w < n) {
     float2 g0, b0;
     bk.gates_of(w == 0 ? first : second, g0, b0);
-    make_chunk_gates(bk.gates[w], lane, g0, b0);
+    make_chunk_gates<true>(bk.gates[w], lane, g0, b0);
   }
   const uint32_t low = TL::low(lane), high = TL::high(lane);
   const int row0 = 16 * (w % SH::SLABS), col0 = w / SH::SLABS * SH::COLS;
@@ -242,8 +245,10 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
     bk.update(W, tk, tv, cg, row0, col0);
     if (BF) bk.settled(i);
     if (BF && r == 0 && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
-    if (ahead) make_chunk_gates(bk.gates[slot3n], lane, g_next, b_next);
+    if (ahead) make_chunk_gates<true>(bk.gates[slot3n], lane, g_next, b_next);
     const float fra = cg.from[16 * r + g], frb = cg.from[16 * r + g + 8];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ldsm_np<NP>(q[k], (tq + 16 * r * TL::ROW + low) ^ (k << 5), SM::PLANE, false);  // (again: the registers)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {  // (columns in two halves, for the registers)
       float c[F / 16][4];
@@ -271,9 +276,29 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       }
     }
     if (nx.i < n) publish(nx);
-    bk.leave(i);
     const int t0 = st.pos * GC;
-    store_rows<T, F>(static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F, 16 * r, p.T - t0, o, lane);
+    T* const out = static_cast<T*>(p.out) + ((size_t)st.stream * p.T + t0) * F;
+    if constexpr (BF) {  // through this warp's rows of the queries' tile, which no other warp reads: whole lines at a time
+      constexpr int VEC = F / 8, AT_ONCE = 32 / VEC;  // 16-byte pieces of a row; rows per store
+      const uint32_t mine = tq + 16 * r * TL::ROW;
+#pragma unroll
+      for (int k = 0; k < F / 8; k += 2)
+        stsm_x4((mine + low) ^ (k << 4), pack_bf16(o[k][0], o[k][1]), pack_bf16(o[k][2], o[k][3]), pack_bf16(o[k + 1][0], o[k + 1][1]),
+                pack_bf16(o[k + 1][2], o[k + 1][3]));
+      __syncwarp();
+      uint4 v[16 / AT_ONCE];
+#pragma unroll
+      for (int k = 0; k < 16 / AT_ONCE; ++k) v[k] = ld_shared_v4(mine + TL::off(AT_ONCE * k + lane / VEC, lane % VEC * 8));
+      bk.leave(i);
+#pragma unroll
+      for (int k = 0; k < 16 / AT_ONCE; ++k) {
+        const int row = 16 * r + AT_ONCE * k + lane / VEC;
+        if (row < p.T - t0) *reinterpret_cast<uint4*>(out + (size_t)row * F + lane % VEC * 8) = v[k];
+      }
+    } else {
+      bk.leave(i);
+      store_rows<T, F>(out, 16 * r, p.T - t0, o, lane);
+    }
     slot3 = slot3 == 2 ? 0 : slot3 + 1;
   }
   bk.drain();
@@ -313,7 +338,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 :
   if (w < 2 && w < n) {
     float2 g0, b0;
     bk.gates_of(w == 0 ? first : second, g0, b0);
-    make_chunk_gates(bk.gates[w], lane, g0, b0);
+    make_chunk_gates<true>(bk.gates[w], lane, g0, b0);
   }
   __syncthreads();
   const int row0 = 16 * (w % SH::SLABS), col0 = w / SH::SLABS * SH::COLS;
@@ -335,7 +360,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 5 : F == 64 ? 2 :
     if (turn) {
       if (BF) bk.settled(i);
       if (BF && lane == 0 && i > 0 && nx.i < n) bk.fetch(nx);
-      if (ahead) make_chunk_gates(bk.gates[slot3 == 0 ? 2 : slot3 - 1], lane, g_next, b_next);
+      if (ahead) make_chunk_gates<true>(bk.gates[slot3 == 0 ? 2 : slot3 - 1], lane, g_next, b_next);
     }
     bk.leave(i);
     slot3 = slot3 == 2 ? 0 : slot3 + 1;

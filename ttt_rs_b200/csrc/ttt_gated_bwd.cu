@@ -13,6 +13,9 @@
 // summed way by way: no sum is taken as the difference of two others.  (g's gradient as a running sum of q dq - k dk leaves the
 // rounding of the whole sequence behind, and where nothing leads across a token, noise instead of zero.)
 //
+// What an operand holds is read from its tile again where it is used (keys, values, u): registers are short, and with fragments kept
+// from use to use the training of 384 streams of 2048 tokens took 573 us, not 540.
+//
 // One CTA of eight warps per stream (or segment) walks the chunks from the last.  Warps 0-3 own 16 queries each: dq, and the
 // float32 dW in their registers with its update.  Warps 4-7 own 16 keys each: dk, dv and the gates' sums.  Per chunk two
 // barriers: all warps at its end, and the second group once more before it reads dW, which the first publishes when it has
@@ -285,9 +288,6 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         cs.r[ia] = r0;
         cs.r[ia + 8] = r1;
       }
-      Pk<NP> u[KS][4];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(u[k], uq ^ (k << 5), SM::PLANE, false);
       const float first = cg.starts[w];
 #pragma unroll
       for (int k = 0; k < F / 8; ++k) scale_rows(dq[k], first, first);
@@ -298,9 +298,10 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
         float s0[4] = {}, s1[4] = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          Pk<NP> f[4];
+          Pk<NP> u[4], f[4];
+          ldsm_np<NP>(u, uq ^ (k << 5), SM::PLANE, false);
           ldsm_np<NP>(f, (tv + 16 * jt * TL::ROW + high) ^ (k << 5), SM::PLANE, false);
-          mma_planes<NP, NP>(s0, s1, u[k], f);
+          mma_planes<NP, NP>(s0, s1, u, f);
         }
         const int j0 = 16 * jt + 2 * t4;
         if (jt < w) {
@@ -357,9 +358,6 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
       const float oa = cg.out[ja], ob = cg.out[ja + 8], ba = cg.beta[ja], bb = cg.beta[ja + 8];
       const float wa = cg.out_b[ja], wb = cg.out_b[ja + 8];
       const uint32_t kq = tk + 16 * w * TL::ROW + low, vq = tv + 16 * w * TL::ROW + low;
-      Pk<NP> k_[KS][4];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) ldsm_np<NP>(k_[k], kq ^ (k << 5), SM::PLANE, false);
       // keys . queries and values . u of this warp's 16 tokens against those of block `it`
       auto products = [&](int it, float (&s0)[4], float (&s1)[4], float (&v0)[4], float (&v1)[4]) {
 #pragma unroll
@@ -368,8 +366,9 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
           Pk<NP> a[4], f[4];
+          ldsm_np<NP>(a, kq ^ (k << 5), SM::PLANE, false);
           ldsm_np<NP>(f, q ^ (k << 5), SM::PLANE, false);
-          mma_planes<NP, NP>(s0, s1, k_[k], f);
+          mma_planes<NP, NP>(s0, s1, a, f);
           ldsm_np<NP>(a, vq ^ (k << 5), SM::PLANE, false);
           ldsm_np<NP>(f, u ^ (k << 5), SM::PLANE, false);
           mma_planes<NP, NP>(v0, v1, a, f);
@@ -524,12 +523,15 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
           }
         }
 #pragma unroll
-        for (int m = 0; m < KS; ++m)  // (an A fragment is two accumulator tiles)
+        for (int m = 0; m < KS; ++m) {  // (an A fragment is two accumulator tiles)
+          Pk<NP> a[4];
+          ldsm_np<NP>(a, kq ^ (m << 5), SM::PLANE, false);
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            sa = f2fma(pr(dk[2 * m + e], 0), make_float2(pk_lo(k_[m][2 * e]), pk_hi(k_[m][2 * e])), sa);
-            sb = f2fma(pr(dk[2 * m + e], 1), make_float2(pk_lo(k_[m][2 * e + 1]), pk_hi(k_[m][2 * e + 1])), sb);
+            sa = f2fma(pr(dk[2 * m + e], 0), make_float2(pk_lo(a[2 * e]), pk_hi(a[2 * e])), sa);
+            sb = f2fma(pr(dk[2 * m + e], 1), make_float2(pk_lo(a[2 * e + 1]), pk_hi(a[2 * e + 1])), sb);
           }
+        }
         gather(dk, av, tq);
         store_rows<T, F>(static_cast<T*>(p.dk) + ((size_t)stream * p.T + t0) * F, 16 * w, rows, dk, lane);
       }

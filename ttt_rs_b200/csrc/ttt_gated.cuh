@@ -149,7 +149,8 @@ struct ChunkGates {
   float all;             // e^{G_end}
   float pad[3];
 };
-// FORWARD: `end` comes with the factor beta.  One warp; lane l brings tokens 2l and 2l + 1 of the chunk.  Tokens behind the sequence: g = 0, beta = 0.
+// FORWARD: `end` comes with the factor beta.  One warp; lane l brings tokens 2l and 2l + 1 of the chunk.  Tokens behind the sequence:
+// g = 0, beta = 0.
 template <bool FORWARD>
 __device__ __forceinline__ void make_chunk_gates(ChunkGates& s, int lane, float2 g, float2 beta) {
   auto log2_of = [](float x) {

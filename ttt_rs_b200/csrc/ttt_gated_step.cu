@@ -1,5 +1,6 @@
 // Gated linear recurrence, a step of 1 to 16 tokens against the resident state (definitions: ttt_gated.cuh): token-by-token
-// generation.  Bound by reading and writing the float32 state once (32 KB per stream of 64 features), or by the launch.
+// generation.  Bound by reading and writing the float32 state once (32 KB per stream of 64 features), or by the launch:
+// 2048 streams 13 us (5.2 TB/s, 0.8 of a copy), 96 streams 4 us.
 //
 // A CTA of four warps per stream.  Every thread holds four columns of the state's rows kg, kg + GROUPS, ...; a token is a
 // multiply-add per element for the state and one for the output, whose partial sums over the rows meet once, behind the last

@@ -270,6 +270,7 @@ __global__ void __launch_bounds__(GB_THREADS, sizeof(T) == 2 ? 2 : 1)
           mma_planes<NP, NS>(dq[2 * m], dq[2 * m + 1], v, f);
         }
       }
+      if (BF) fence_proxy_async_smem();  // (the next saved state lands where this one's planes were written)
       asm volatile("bar.sync 2, %0;" ::"n"(GB_THREADS / 2) : "memory");
       if (tid == 0 && i + 1 < n) fetch_w(nx);
       put_state<F, NS>(dW, row0, col0, tdw, lane, SM::DWS);  // dW behind this chunk, for the other group

@@ -41,3 +41,20 @@ def test_backwards_of_many_chunks_repeat(B, H, T, F):
     args = (*G.f64(one), d_out[:1, :1].double(), d_w[:1, :1].double())
     G.check([t[:1, :1] for t in want], O.gated_grads(*args), O.gated_magnitudes(*args), torch.bfloat16)
     tb.check_status()
+
+
+@pytest.mark.parametrize("B,H,T,F", SHAPES)
+def test_forwards_of_many_chunks_repeat(B, H, T, F):
+    import ttt_rs_b200 as tb
+    ins, _, _ = G.make(B, H, T, F, torch.bfloat16, seed=32)
+    dev = [t.cuda() for t in ins]
+
+    def call():
+        with torch.no_grad():
+            return tb.fused_gated_linear(*dev)
+
+    want = call()
+    assert all(torch.equal(x, y) for got in on_three_streams(call) for x, y in zip(got, want))
+    one = G.f64([t[:1, :1] for t in ins])
+    G.check([t[:1, :1] for t in want], O.gated_forward(*one), O.gated_magnitudes(*one), torch.bfloat16)
+    tb.check_status()

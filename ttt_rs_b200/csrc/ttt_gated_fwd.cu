@@ -293,6 +293,7 @@ __global__ void __launch_bounds__(GF_THREADS, sizeof(T) == 2 ? 3 : 1)
       uint4 v[16 / AT_ONCE];
 #pragma unroll
       for (int k = 0; k < 16 / AT_ONCE; ++k) v[k] = ld_shared_v4(mine + TL::off(AT_ONCE * k + lane / VEC, lane % VEC * 8));
+      fence_proxy_async_smem();  // (a later chunk's queries land where these rows were written)
       bk.leave(i);
 #pragma unroll
       for (int k = 0; k < 16 / AT_ONCE; ++k) {

@@ -396,7 +396,8 @@ int ttt_linear_gated_step(const ttt_dims* d, const void* xq, const void* xk, con
  * dtype and, for the norm, epsilon are read; k_heads may differ from heads.
  * `strides`: for each tensor in the order of the arguments the strides of batch, head and token in elements (null: contiguous
  * [B,H,T,F]); rows are F contiguous elements at any address (on 16 bytes, with F and rotary_dim multiples of 8, they are read 16
- * bytes at a time).  Results may be the inputs themselves, and must not overlap them otherwise.
+ * bytes at a time).  Results may be the inputs themselves; results that lie over another tensor otherwise, and be it in one element,
+ * are refused (TTT_ERR_SHAPE).  Column blocks of one buffer that share none are apart, however they interleave.
  *
  * ttt_layer_rotary: y = the rows of x rotated (inverse != 0: by the angles' negatives, the gradient).
  * ttt_layer_qk_norm_rotary: rows x / sqrt(mean(x^2) + epsilon) * weight, rotated (rotation null: not).  q_weight, k_weight: T [F]

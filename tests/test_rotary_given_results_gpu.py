@@ -1,0 +1,40 @@
+"""Results of the rotary operators that are given: where they may lie, and what autograd knows of them."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def refused(code, call):
+    import ttt_rs_b200 as tb
+    with pytest.raises(tb.TttError) as e:
+        call()
+    assert e.value.code == code
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_views_that_share_elements_are_refused(dtype):
+    """Views that are not dense: shifted by a token of a padded cache, by features of a projection."""
+    import ttt_rs_b200 as tb
+    from ttt_rs_b200 import _lib as L
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    cache = torch.randn(2, 3, 50, 64, device="cuda").to(dtype)
+    proj = torch.randn(2, 40, 4 * 3 * 64, device="cuda").to(dtype)
+    was = cache.clone(), proj.clone()
+    cols = lambda at: proj[..., at:at + 192].unflatten(-1, (3, 64)).transpose(1, 2)  # noqa: E731
+    refused(L.TTT_ERR_SHAPE, lambda: tb.rotary(cache[:, :, :40], rot, out=cache[:, :, 1:41]))
+    refused(L.TTT_ERR_SHAPE, lambda: tb.rotary(cache[:, :, 1:41], rot, out=cache[:, :, :40]))
+    refused(L.TTT_ERR_SHAPE, lambda: tb.rotary(cols(0), rot, out=cols(8)))
+    refused(L.TTT_ERR_SHAPE, lambda: tb.qk_norm_rotary(cols(0), cols(192), rot=rot, out=(cols(384), cols(384 + 8))))
+    refused(L.TTT_ERR_SHAPE, lambda: tb.qk_norm_rotary(cols(0), cols(192), rot=rot, out=(cols(192), cols(384))))
+    assert torch.equal(cache, was[0]) and torch.equal(proj, was[1])
+    # columns that share none, and the same rows: as apart from one another
+    want = tb.qk_norm_rotary(cols(0), cols(192), rot=rot)
+    tb.qk_norm_rotary(cols(0), cols(192), rot=rot, out=(cols(384), cols(576)))
+    assert torch.equal(cols(384), want[0]) and torch.equal(cols(576), want[1])
+    tb.qk_norm_rotary(cols(0), cols(192), rot=rot, out=(cols(0), cols(192)))
+    assert torch.equal(cols(0), want[0]) and torch.equal(cols(192), want[1])
+    want = tb.rotary(cache[:, :, 40:], rot)
+    tb.rotary(cache[:, :, 40:], rot, out=cache[:, :, 5:15])
+    assert torch.equal(cache[:, :, 5:15], want)

@@ -105,6 +105,7 @@ INTERNAL = {
                                                  C.c_float, C.c_float, C.c_int] + [_P] * 10),
     "ttt_internal_layer_values": (C.c_int, [_DP, _P, C.c_int64, _P, C.c_int64, _P, C.c_float, _P, _P, _P]),
     "ttt_internal_layer_values_backward": (C.c_int, [_DP, _P, _P, _P, C.c_float, _P, C.c_int64, _P, C.c_int64, C.c_int, _P]),
+    "ttt_internal_rows_meet": (C.c_int, [C.c_int, C.c_int] + [_P] * 6),
 }
 
 NOALLOC_SCRATCH_BYTES = 32 << 20  # TTT_NOALLOC_SCRATCH_BYTES

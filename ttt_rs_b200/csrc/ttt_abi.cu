@@ -1565,7 +1565,82 @@ int set_rows(int64_t (&out)[3], const ttt_dims* d, int heads, const void* base, 
   return TTT_OK;
 }
 
+// A tensor's rows of F elements: where the first one is, how many there are, and their strides in elements (0 where one only)
+struct HeadRows {
+  const void* at;
+  int64_t size[3], stride[3];
+};
+HeadRows head_rows(const ttt_dims* d, int heads, const void* at, const int64_t (&strides)[3]) {
+  return {at, {d->batch, heads, d->seq_len}, {strides[0], strides[1], strides[2]}};
+}
+// Whether two tensors of rows share an element.  An element of b less one of a is offset + sum of stride * c + f elements: c counts b's
+// indices up and a's down (strides that both have: from -(n_a - 1) to n_b - 1), |f| < F.  Zero is looked for from the largest stride
+// down, among the counts that the smaller strides can make up for: one or two each where strides are nested as tensors' are.
+// Strides that make it a long search (no tensor of a layer) count as sharing.
+class RowsMeet {
+  using Wide = __int128;
+  struct Term {
+    Wide stride, lo, hi, rest_lo, rest_hi;
+  };
+  Term terms[7];
+  int count = 0, steps = 0;
+  bool find(int k, Wide target) {
+    if (++steps > 1 << 14) return true;
+    const Term& t = terms[k];
+    if (k + 1 == count) return t.lo <= target && target <= t.hi;  // (the elements of a row)
+    const auto floor_div = [](Wide a, Wide b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };
+    const Wide first = std::max(t.lo, -floor_div(t.rest_hi - target, t.stride)), last = std::min(t.hi, floor_div(target - t.rest_lo, t.stride));
+    for (Wide c = first; c <= last; ++c)
+      if (find(k + 1, target - c * t.stride)) return true;
+    return false;
+  }
+  void add(int64_t stride, int64_t lo, int64_t hi) {
+    if (stride == 0 || lo == hi) return;
+    for (int k = 0; k < count; ++k)
+      if (terms[k].stride == stride) {
+        terms[k].lo += lo;
+        terms[k].hi += hi;
+        return;
+      }
+    terms[count++] = {stride, lo, hi, 0, 0};
+  }
+
+ public:
+  bool operator()(const HeadRows& a, const HeadRows& b, int F, int element) {
+    const Wide offset = ((Wide)(intptr_t)b.at - (Wide)(intptr_t)a.at) / element;
+    for (int k = 0; k < 3; ++k) {
+      add(a.stride[k], -(a.size[k] - 1), 0);
+      add(b.stride[k], 0, b.size[k] - 1);
+    }
+    std::sort(terms, terms + count, [](const Term& x, const Term& y) { return x.stride > y.stride; });
+    terms[count++] = {1, -(F - 1), F - 1, 0, 0};
+    for (int k = count - 2; k >= 0; --k) {
+      terms[k].rest_lo = terms[k + 1].rest_lo + terms[k + 1].stride * terms[k + 1].lo;
+      terms[k].rest_hi = terms[k + 1].rest_hi + terms[k + 1].stride * terms[k + 1].hi;
+    }
+    const Wide lo = terms[0].rest_lo + terms[0].stride * terms[0].lo, hi = terms[0].rest_hi + terms[0].stride * terms[0].hi;
+    return lo <= -offset && -offset <= hi && find(0, -offset);
+  }
+};
+// A result must not lie over another tensor of the call; over its own input it may, row for row
+int check_apart(const ttt_dims* d, const char* name, const HeadRows& out, const char* other_name, const HeadRows& other, bool or_same) {
+  if (or_same && out.at == other.at && std::equal(out.size, out.size + 3, other.size) && std::equal(out.stride, out.stride + 3, other.stride))
+    return TTT_OK;
+  if (RowsMeet()(out, other, d->head_dim, d->dtype == TTT_BF16 ? 2 : 4)) return fail(TTT_ERR_SHAPE, "%s lies over %s", name, other_name);
+  return TTT_OK;
+}
+
 }  // namespace
+
+extern "C" int ttt_internal_rows_meet(int head_dim, int element_bytes, const void* a, const int64_t* a_sizes, const int64_t* a_strides,
+                                      const void* b, const int64_t* b_sizes, const int64_t* b_strides) {
+  HeadRows r[2] = {{a, {}, {}}, {b, {}, {}}};
+  for (int k = 0; k < 3; ++k) {
+    r[0].size[k] = a_sizes[k], r[0].stride[k] = a_strides[k];
+    r[1].size[k] = b_sizes[k], r[1].stride[k] = b_strides[k];
+  }
+  return RowsMeet()(r[0], r[1], head_dim, element_bytes);
+}
 
 extern "C" int ttt_layer_rotary(const ttt_dims* d, const void* x, const int64_t* strides, const ttt_rotation* rotation, int inverse,
                                 void* y, const int64_t* y_strides, void* stream) {
@@ -1575,7 +1650,8 @@ extern "C" int ttt_layer_rotary(const ttt_dims* d, const void* x, const int64_t*
   bool vec = d->head_dim % 8 == 0;
   if ((rc = set_rotation(&p, d, rotation, true)) != TTT_OK ||
       (rc = set_rows(p.xs[0], d, d->heads, x, strides, 0, false, "x", &vec)) != TTT_OK ||
-      (rc = set_rows(p.ys[0], d, d->heads, y, y_strides, 0, true, "y", &vec)) != TTT_OK)
+      (rc = set_rows(p.ys[0], d, d->heads, y, y_strides, 0, true, "y", &vec)) != TTT_OK ||
+      (rc = check_apart(d, "y", head_rows(d, d->heads, y, p.ys[0]), "x", head_rows(d, d->heads, x, p.xs[0]), true)) != TTT_OK)
     return rc;
   p.x[0] = x;
   p.y[0] = y;
@@ -1622,6 +1698,19 @@ int qk_params(ttt::RotaryParams* p, const ttt_dims* d, int k_heads, const ttt_ro
   p->eps = d->epsilon;
   return TTT_OK;
 }
+// the results of a call against each other and against what it reads
+int qk_apart(const ttt::RotaryParams& p, const ttt_dims* d, const char* q_name, const char* k_name) {
+  const char *out_names[2] = {q_name, k_name}, *in_names[2] = {"q", "k"}, *grad_names[2] = {"grad_q_out", "grad_k_out"};
+  const HeadRows out[2] = {head_rows(d, p.heads[0], p.y[0], p.ys[0]), head_rows(d, p.heads[1], p.y[1], p.ys[1])};
+  int rc = check_apart(d, q_name, out[0], k_name, out[1], false);
+  for (int m = 0; m < 2; ++m)
+    for (int n = 0; n < 2; ++n) {
+      if (rc == TTT_OK) rc = check_apart(d, out_names[m], out[m], in_names[n], head_rows(d, p.heads[n], p.x[n], p.xs[n]), m == n);
+      if (rc == TTT_OK && p.g[n] != nullptr)
+        rc = check_apart(d, out_names[m], out[m], grad_names[n], head_rows(d, p.heads[n], p.g[n], p.gs[n]), m == n);
+    }
+  return rc;
+}
 }  // namespace
 
 extern "C" int ttt_layer_qk_norm_rotary(const ttt_dims* d, int k_heads, const void* q, const void* k, const int64_t* strides,
@@ -1629,8 +1718,8 @@ extern "C" int ttt_layer_qk_norm_rotary(const ttt_dims* d, int k_heads, const vo
                                         void* k_out, const int64_t* out_strides, void* stream) {
   ttt::RotaryParams p{};
   bool vec;
-  const int rc = qk_params(&p, d, k_heads, rotation, q, k, strides, q_out, k_out, out_strides, "q_out", "k_out", q_weight, k_weight, &vec);
-  if (rc != TTT_OK) return rc;
+  int rc = qk_params(&p, d, k_heads, rotation, q, k, strides, q_out, k_out, out_strides, "q_out", "k_out", q_weight, k_weight, &vec);
+  if (rc != TTT_OK || (rc = qk_apart(p, d, "q_out", "k_out")) != TTT_OK) return rc;
   p.sign = 1.f;
   const cudaError_t e = ttt::launch_rotary(d->dtype, p, vec, rotation != nullptr && rotation->half != 0, true, false,
                                            static_cast<cudaStream_t>(stream));
@@ -1671,6 +1760,7 @@ extern "C" int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads,
     if ((rc = check_optional("workspace", workspace, 4)) != TTT_OK) return rc;
     p.partials = static_cast<float*>(workspace);
   }
+  if ((rc = qk_apart(p, d, "grad_q", "grad_k")) != TTT_OK) return rc;
   const cudaError_t e = ttt::launch_rotary(d->dtype, p, vec, rotation != nullptr && rotation->half != 0, true, true,
                                            static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail(TTT_ERR_CUDA, "norm and rotation backward launch failed: %s", cudaGetErrorString(e));

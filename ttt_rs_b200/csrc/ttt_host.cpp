@@ -1144,14 +1144,8 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
-// (a result may be the input itself; two tensors that lie over one another otherwise are left to the caller's check)
-bool apart(const Tensor& y, const Tensor& x, bool or_same) {
-  if (!y.defined() || !x.defined()) return true;
-  const at::MemOverlapStatus s = at::get_overlap_status(y, x);
-  return s != at::MemOverlapStatus::Partial && (s != at::MemOverlapStatus::Full || (or_same && y.strides() == x.strides()));
-}
 bool same_shape_result(const Tensor& y, const Tensor& x, const Dims& m) {
-  return !y.defined() || (head_rows(y, m.dev, m.dt) && y.sizes() == x.sizes() && apart(y, x, true));
+  return !y.defined() || (head_rows(y, m.dev, m.dt) && y.sizes() == x.sizes());
 }
 // rotary(x, rotation (7), inverse, out | None) -> y, recorded for autograd where that is on and asked for | None
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -1185,8 +1179,7 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
           !optional_tensor(args[12], yq) || !optional_tensor(args[13], yk));
   const double eps = PyFloat_AsDouble(args[11]);
   if (PyErr_Occurred()) return nullptr;
-  NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m) ||
-          !apart(yq, x[1], false) || !apart(yk, x[0], false) || !apart(yq, yk, false));
+  NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m));
   if (wants_grad({&x[0], &x[1], &wq, &wk})) {
     NONE_IF(yq.defined() || yk.defined());
     std::vector<int64_t> ints = rot.ints();

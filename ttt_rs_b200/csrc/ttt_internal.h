@@ -85,4 +85,9 @@ int ttt_internal_layer_values_backward(const ttt_dims* d, const void* grad_xv, c
                                        float base_lr, void* grad_v_dst, int64_t dst_ld, void* grad_lr_logits, int64_t lr_ld,
                                        int lr_cols, void* stream);
 
+// Whether two tensors [B,H,T,head_dim] with contiguous rows share an element: sizes and strides (elements) of batch, head and token.
+// (What ttt_layer_rotary and ttt_layer_qk_norm_rotary refuse results by; host only.)
+int ttt_internal_rows_meet(int head_dim, int element_bytes, const void* a, const int64_t* a_sizes, const int64_t* a_strides, const void* b,
+                           const int64_t* b_sizes, const int64_t* b_strides);
+
 }  // extern "C"

@@ -129,38 +129,12 @@ def _check_positions(positions: Optional[torch.Tensor], B: int, T: int, device):
     return positions.long().contiguous()
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the addresses that both reach over meet (columns of one projection do, without sharing an element)."""
-    def reach(t):
-        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    (a0, a1), (b0, b1) = reach(a), reach(b)
-    return a0 < b1 and b0 < a1
-
-
-def _dense(t: torch.Tensor) -> bool:
-    reach = 1
-    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
-        if s != reach:
-            return False
-        reach *= n
-    return True
-
-
-def _apart(a, b, what: str, or_same: bool = False):
-    """Refuses two tensors of which one lies over the other: a result may be its input itself, not part of it."""
-    if a is None or b is None or (or_same and a.data_ptr() == b.data_ptr() and a.stride() == b.stride()):
-        return
-    if _overlap(a, b) and _dense(a) and _dense(b):
-        raise TttError(_lib.TTT_ERR_SHAPE, f"{what} overlap")
-
-
 def _check_out(out, like, name: str):
     if out is None:
         return
     _expect(name, out, like.shape, like.dtype, like.device)
     if out.shape[3] > 1 and out.stride(3) != 1:
         raise TttError(_lib.TTT_ERR_SHAPE, f"rows of {name} must be contiguous")
-    _apart(out, like, f"{name} and its input", or_same=True)
     if torch.is_grad_enabled() and (like.requires_grad or out.requires_grad):
         raise TttError(_lib.TTT_ERR_UNSUPPORTED, "results that are given are not recorded for autograd")
 
@@ -220,9 +194,6 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
         _check_table(rot, q.device)
     _check_out(oq, q, "out[0]")
     _check_out(ok, k, "out[1]")
-    _apart(oq, k, "out[0] and k")
-    _apart(ok, q, "out[1] and q")
-    _apart(oq, ok, "out[0] and out[1]")
     positions = _check_positions(positions, B, T, q.device)
     device_status(q.device)
     native = _lib.host().qk_norm(_rows(q), _rows(k), None if q_weight is None else q_weight.contiguous(),

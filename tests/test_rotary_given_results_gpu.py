@@ -38,3 +38,23 @@ def test_views_that_share_elements_are_refused(dtype):
     want = tb.rotary(cache[:, :, 40:], rot)
     tb.rotary(cache[:, :, 40:], rot, out=cache[:, :, 5:15])
     assert torch.equal(cache[:, :, 5:15], want)
+
+
+def test_results_that_require_gradients_are_refused():
+    """As those of inputs and weights that do: nothing given is recorded."""
+    import ttt_rs_b200 as tb
+    from ttt_rs_b200 import _lib as L
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    x, k, leaf = torch.randn(3, 2, 3, 8, 64, device="cuda")
+    leaf = leaf.clone().requires_grad_()
+    part, was, w = leaf * 1.0, leaf.detach().clone(), torch.ones(64, device="cuda").requires_grad_()
+    for out in (leaf, part):
+        refused(L.TTT_ERR_UNSUPPORTED, lambda: tb.rotary(x, rot, out=out))
+        refused(L.TTT_ERR_UNSUPPORTED, lambda: tb.qk_norm_rotary(x, k, rot=rot, out=(out, torch.empty_like(k))))
+        refused(L.TTT_ERR_UNSUPPORTED, lambda: tb.qk_norm_rotary(x, k, rot=rot, out=(torch.empty_like(x), out)))
+    refused(L.TTT_ERR_UNSUPPORTED, lambda: tb.qk_norm_rotary(x, k, w, None, rot=rot, out=(torch.empty_like(x), torch.empty_like(k))))
+    refused(L.TTT_ERR_UNSUPPORTED, lambda: tb.qk_norm_rotary(x, leaf, rot=rot, out=(torch.empty_like(x), torch.empty_like(k))))
+    assert torch.equal(leaf.detach(), was) and torch.equal(part.detach(), was)
+    with torch.no_grad():  # (as torch's own operations into a leaf)
+        tb.rotary(x, rot, out=leaf)
+        assert torch.equal(leaf, tb.rotary(x, rot))

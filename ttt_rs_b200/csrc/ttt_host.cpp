@@ -1158,7 +1158,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const bool inverse = as_int(args[8]) != 0;
   if (PyErr_Occurred()) return nullptr;
   NONE_IF(!rot.turns.defined() || !head_dims(m, x[0], 0.0) || !rot.set(m) || !same_shape_result(y, x[0], m));
-  if (wants_grad({&x[0]})) {
+  if (wants_grad({&x[0], &y})) {  // (a given result is not recorded: the caller's check refuses it)
     NONE_IF(y.defined() || inverse);
     return THPVariable_Wrap(RotaryFn::apply(x[0], rot.turns, given(rot.positions), rot.ints(), rot.size));
   }
@@ -1180,7 +1180,7 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const double eps = PyFloat_AsDouble(args[11]);
   if (PyErr_Occurred()) return nullptr;
   NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m));
-  if (wants_grad({&x[0], &x[1], &wq, &wk})) {
+  if (wants_grad({&x[0], &x[1], &wq, &wk, &yq, &yk})) {
     NONE_IF(yq.defined() || yk.defined());
     std::vector<int64_t> ints = rot.ints();
     ints.push_back(wq.defined());

@@ -129,13 +129,14 @@ def _check_positions(positions: Optional[torch.Tensor], B: int, T: int, device):
     return positions.long().contiguous()
 
 
-def _check_out(out, like, name: str):
+def _check_out(out, like, name: str, *others: Optional[torch.Tensor]):
+    """`others`: what else the call reads or writes."""
     if out is None:
         return
     _expect(name, out, like.shape, like.dtype, like.device)
     if out.shape[3] > 1 and out.stride(3) != 1:
         raise TttError(_lib.TTT_ERR_SHAPE, f"rows of {name} must be contiguous")
-    if torch.is_grad_enabled() and (like.requires_grad or out.requires_grad):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (out, like, *others)):
         raise TttError(_lib.TTT_ERR_UNSUPPORTED, "results that are given are not recorded for autograd")
 
 
@@ -192,8 +193,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
             _expect(name, w, (F,), q.dtype, q.device)
     if rot is not None:
         _check_table(rot, q.device)
-    _check_out(oq, q, "out[0]")
-    _check_out(ok, k, "out[1]")
+    _check_out(oq, q, "out[0]", k, q_weight, k_weight)
+    _check_out(ok, k, "out[1]", q, q_weight, k_weight)
     positions = _check_positions(positions, B, T, q.device)
     device_status(q.device)
     native = _lib.host().qk_norm(_rows(q), _rows(k), None if q_weight is None else q_weight.contiguous(),

@@ -58,3 +58,29 @@ def test_results_that_require_gradients_are_refused():
     with torch.no_grad():  # (as torch's own operations into a leaf)
         tb.rotary(x, rot, out=leaf)
         assert torch.equal(leaf, tb.rotary(x, rot))
+
+
+def test_what_was_saved_and_is_overwritten_has_no_gradients():
+    """Results written over a tensor that a graph has saved: its backward refuses, as it does after torch's own operations."""
+    import ttt_rs_b200 as tb
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    x, k, leaf = torch.randn(3, 2, 3, 8, 64, device="cuda")
+    leaf.requires_grad_()
+    calls = [lambda a: tb.rotary(a, rot, out=a), lambda a: tb.rotary(x, rot, out=a), lambda a: tb.rotary(x[:, :, :4], rot, out=a[:, :, 4:]),
+             lambda a: tb.qk_norm_rotary(a, k, rot=rot, out=(a, k)), lambda a: tb.qk_norm_rotary(k, a, rot=rot, out=(k, a))]
+    for call in calls:
+        a = leaf.exp()  # (saves its result)
+        before = a._version
+        with torch.no_grad():
+            call(a)
+        assert a._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(a.sum(), leaf)
+    a = leaf.exp()
+    with torch.no_grad():
+        y = tb.rotary(a, rot)
+    assert y._version == 0 and torch.equal(torch.autograd.grad(a.sum(), leaf)[0], a.detach())
+    with torch.inference_mode():
+        b = torch.empty_like(x)
+    with torch.no_grad():  # (counts no versions)
+        assert torch.equal(tb.rotary(x, rot, out=b), tb.rotary(x, rot))

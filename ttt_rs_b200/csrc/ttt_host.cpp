@@ -1147,6 +1147,11 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
 bool same_shape_result(const Tensor& y, const Tensor& x, const Dims& m) {
   return !y.defined() || (head_rows(y, m.dev, m.dt) && y.sizes() == x.sizes());
 }
+// A tensor that a kernel has overwritten: autograd refuses what was computed from its former values, as after torch's own operations
+// (inference tensors count no versions, and nothing saves them)
+void overwritten(const Tensor& y) {
+  if (!y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
+}
 // rotary(x, rotation (7), inverse, out | None) -> y, recorded for autograd where that is on and asked for | None
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1162,8 +1167,10 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     NONE_IF(y.defined() || inverse);
     return THPVariable_Wrap(RotaryFn::apply(x[0], rot.turns, given(rot.positions), rot.ints(), rot.size));
   }
+  const bool given_y = y.defined();
   const int rc = rotary(m, x[0], rot, inverse, y);
   if (rc != TTT_OK) throw_error(rc);
+  if (given_y) overwritten(y);
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS
 }
@@ -1187,8 +1194,11 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     ints.push_back(wk.defined());
     return wrap(QkNormFn::apply(x[0], x[1], given(wq), given(wk), given(rot.turns), given(rot.positions), ints, rot.size, eps));
   }
+  const bool given_q = yq.defined(), given_k = yk.defined();
   const int rc = call.forward(x[0], x[1], wq, wk, rot, yq, yk);
   if (rc != TTT_OK) throw_error(rc);
+  if (given_q) overwritten(yq);
+  if (given_k) overwritten(yk);
   return wrap({yq, yk});
   END_HANDLE_TH_ERRORS
 }
@@ -1209,6 +1219,7 @@ PyObject* py_qk_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
     NONE_IF(!head_rows(x[2 + i], call.m.dev, call.m.dt) || x[2 + i].sizes() != x[i].sizes() || !same_shape_result(d[i], x[i], call.m));
   const int rc = call.backward(x[0], x[1], x[2], x[3], wq, wk, rot, d[0], d[1], dwq, dwk);
   if (rc != TTT_OK) throw_error(rc);
+  for (const Tensor& t : d) overwritten(t);
   return wrap({d[0], d[1], dwq, dwk});
   END_HANDLE_TH_ERRORS
 }

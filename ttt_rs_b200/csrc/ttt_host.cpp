@@ -32,9 +32,9 @@ constexpr int kMaxDevices = 64;
 Tensor g_status[kMaxDevices];   // the status words of each device, handed over by the Python side when it creates them
 PyObject* g_error_type = nullptr;  // TttError(code, message)
 
-[[noreturn]] void throw_error(int rc) {
+[[noreturn]] void throw_error(int rc, const char* message = nullptr) {
   pybind11::gil_scoped_acquire gil;
-  PyObject* args = Py_BuildValue("(is)", rc, ttt_b200_last_error());
+  PyObject* args = Py_BuildValue("(is)", rc, message != nullptr ? message : ttt_b200_last_error());
   PyObject* exc = args ? PyObject_CallObject(g_error_type, args) : nullptr;
   Py_XDECREF(args);
   if (exc) {
@@ -1110,6 +1110,13 @@ bool optional_tensor(PyObject* o, Tensor& t) {
   t = THPVariable_Unpack(o);
   return true;
 }
+// Tensors that carry a tangent (forward-mode differentiation, with or without gradients): no operator here continues one, and its
+// result would silently have none
+void refuse_tangents(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw_error(TTT_ERR_UNSUPPORTED, "derivatives in forward mode are not computed by this operator");
+}
 // gated(q, k, v, log_decay, beta | None, weight | None) -> (out, weight), recorded for autograd where that is on and asked for | None
 PyObject* py_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1117,6 +1124,7 @@ PyObject* py_gated(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Tensor t[4], beta, w;
   NONE_IF(!tensors(args, t) || !optional_tensor(args[4], beta) || !optional_tensor(args[5], w));
   Gated call;
+  refuse_tangents({&t[0], &t[1], &t[2], &t[3], &beta, &w});
   NONE_IF(!call.plain(t[0], t[1], t[2], t[3], beta, w));
   bool grad = false;
   if (at::GradMode::is_enabled())
@@ -1162,6 +1170,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   NONE_IF(!tensors(args, x) || !rotation_args(args + 1, rot) || !optional_tensor(args[9], y));
   const bool inverse = as_int(args[8]) != 0;
   if (PyErr_Occurred()) return nullptr;
+  refuse_tangents({&x[0], &y});
   NONE_IF(!rot.turns.defined() || !head_dims(m, x[0], 0.0) || !rot.set(m) || !same_shape_result(y, x[0], m));
   if (wants_grad({&x[0], &y})) {  // (a given result is not recorded: the caller's check refuses it)
     NONE_IF(y.defined() || inverse);
@@ -1186,6 +1195,7 @@ PyObject* py_qk_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
           !optional_tensor(args[12], yq) || !optional_tensor(args[13], yk));
   const double eps = PyFloat_AsDouble(args[11]);
   if (PyErr_Occurred()) return nullptr;
+  refuse_tangents({&x[0], &x[1], &wq, &wk, &yq, &yk});
   NONE_IF(!call.set(x[0], x[1], wq, wk, eps) || !rot.set(call.m) || !same_shape_result(yq, x[0], call.m) || !same_shape_result(yk, x[1], call.m));
   if (wants_grad({&x[0], &x[1], &wq, &wk, &yq, &yk})) {
     NONE_IF(yq.defined() || yk.defined());

@@ -549,7 +549,8 @@ class TTT(torch.nn.Module):
         self.post_norm_bias = torch.nn.Parameter(torch.zeros(hs, **kw))
         self.q_norm_weight = torch.nn.Parameter(torch.ones(c.head_dim, **kw)) if c.qk_norm else None
         self.k_norm_weight = torch.nn.Parameter(torch.ones(c.head_dim, **kw)) if c.qk_norm else None
-        c.rotary_config()  # (refuses what it cannot rotate)
+        if c.own_heads:
+            c.rotary_config()  # (refuses what it cannot rotate; the prologue has limits of its own)
         self._stack = None
 
     def __getstate__(self):  # (copies and pickles stack their own)

@@ -84,3 +84,12 @@ def test_what_was_saved_and_is_overwritten_has_no_gradients():
         b = torch.empty_like(x)
     with torch.no_grad():  # (counts no versions)
         assert torch.equal(tb.rotary(x, rot, out=b), tb.rotary(x, rot))
+
+
+def test_a_rotation_made_in_inference_mode_can_be_differentiated():
+    import ttt_rs_b200 as tb
+    with torch.inference_mode():
+        rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    x, w = torch.randn(1, 2, 8, 64, device="cuda").requires_grad_(), torch.ones(64, device="cuda").requires_grad_()
+    (dx,) = torch.autograd.grad(tb.rotary(x, rot).sum(), x)
+    assert torch.isfinite(dx).all() and all(torch.isfinite(t).all() for t in torch.autograd.grad(tb.qk_norm_rotary(x, x, w, w, rot)[0].sum(), (x, w)))

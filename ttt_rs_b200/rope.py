@@ -97,7 +97,8 @@ class Rotary:
         self.device = torch.device("cuda" if device is None else device)
         # turns per position in 2^-64, as the kernels multiply them (modulo one turn, so that sign does not matter)
         turns = [round(f / (2.0 * math.pi) * 2.0 ** 64) for f in config.frequencies()]
-        self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=self.device)
+        with torch.inference_mode(False):  # (a table made while serving is saved for the backward of a later call)
+            self.turns = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turns], dtype=torch.int64, device=self.device)
         self._args = (self.turns, config.width, int(config.layout == "half"), config.wrap, config.size)
 
 

@@ -246,7 +246,7 @@ def _prologue_backward(dproj, cols, cfg, start_idx, lr, dxq, dxk, dxv, dlr):
     return dproj[..., cols["lr"]:cols["lr"] + H].sum(dim=(0, 1), dtype=torch.float32).to(dt).reshape(H, 1)
 
 
-@functools.lru_cache(maxsize=64)
+@functools.lru_cache(maxsize=None)  # (never dropped: a captured graph reads the table where it lies)
 def _rotary_on(config: RotaryConfig, device: torch.device) -> Rotary:
     return Rotary(config, device)
 

@@ -71,8 +71,12 @@ class TTTLayerConfig:
     @property
     def own_heads(self) -> bool:
         """Queries and keys go through the norm and rotation of `qk_norm_rotary` / `rotary`, not through the prologue."""
+        if self.qk_norm:
+            return True
+        if self.rotary_dim is None and self.rope_layout == "interleaved" and self.rope_scaling == "none":
+            return False  # (first: asked for once per generated token and layer)
         plain = self.rope_layout == "interleaved" and self.rotary_dim in (None, self.head_dim) and self.rope_scaling == "none"
-        return self.qk_norm or (self.pos_encoding != "none" and not plain)
+        return self.pos_encoding != "none" and not plain
 
     def rotary_config(self) -> Optional[RotaryConfig]:
         """The rotation of `pos_encoding` and the fields above (None: none)."""

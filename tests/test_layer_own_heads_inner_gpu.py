@@ -84,3 +84,25 @@ def test_training(kind, dtype, kw):
         else:
             e = ((a.detach().double().cpu().reshape(b.shape) - b).norm() / b.norm()).item()
             assert e <= 5e-2, (name, e)
+
+
+def test_captured_tokens_of_the_recurrence():
+    """A token's step in a graph: the new state copied to where the captured one is read, between replays."""
+    import ttt_rs_b200 as tb
+    cfg = tb.TTTLayerConfig(hidden_size=256, num_heads=4, qk_norm=True, pos_encoding="none")
+    layer, inner = tb.TTT(cfg, device="cuda", dtype=torch.bfloat16), tb.new_gated_inner(cfg, device="cuda")
+    x = torch.randn(3, 12, 256, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():
+        eager = inner.init_state(3)
+        want = [layer(x[:, t:t + 1].contiguous(), inner, eager) for t in range(12)]
+        state, token = inner.init_state(3), x[:, :1].clone()
+        held, graph = state.weight, torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out = layer(token, inner, state)
+        for t in range(12):
+            token.copy_(x[:, t:t + 1])
+            graph.replay()
+            assert torch.equal(out, want[t])
+            held.copy_(state.weight)
+    assert torch.equal(held, eager.weight)

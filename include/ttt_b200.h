@@ -69,7 +69,7 @@ typedef struct ttt_dims {
 /* Rotary positions of ttt_layer_rotary and ttt_layer_qk_norm_rotary: pair p of a row's first `rotary_dim` features is turned by
  * 2 pi * position * turns[p] / 2^64, and scaled by `size`; the features behind are left as they are. */
 typedef struct ttt_rotation {
-  const uint64_t* turns;      /* device, [rotary_dim / 2]: turns per position as a fraction of 2^64, exact at any position */
+  const uint64_t* turns;      /* device, [rotary_dim / 2]: turns per position as a fraction of 2^64 (its product with a position is exact) */
   const int64_t* positions;   /* device, [T] or [B][T] with rows positions_stride apart (0: one row for all); null: start_idx + t */
   int64_t positions_stride;
   int64_t start_idx;

@@ -13,8 +13,8 @@
 // summed way by way: no sum is taken as the difference of two others.  (g's gradient as a running sum of q dq - k dk leaves the
 // rounding of the whole sequence behind, and where nothing leads across a token, noise instead of zero.)
 //
-// 384 streams of 2048 tokens, F = 64, bf16: 385 us, 2.3 TB/s; 1680 instructions per warp and chunk at 41 % of the issue slots (two
-// blocks per SM, for registers and shared memory), shared-memory pipe 71 %, tensor pipe 43 %.
+// 384 streams of 2048 tokens, F = 64, bf16: 385 us, 2.3 TB/s, in passes back to back (alone with cold caches, under the profiler, 411).
+// 1680 instructions per warp and chunk at 41 % of the issue slots (two blocks per SM, for registers and shared memory), shared-memory pipe 71 %, tensor pipe 43 %.
 // What an operand holds is read from its tile again where it is used (keys, values, u): registers are short, and with fragments kept
 // from use to use the training of 384 streams of 2048 tokens took 573 us, not 540.
 //

@@ -8,8 +8,8 @@
 // this chunk's inputs, so that no warp waits for the others of its chunk.  The next chunk is on its way meanwhile (TMA, rows
 // behind the sequence read as zeros), fetched when all warps have left the chunk before.
 //
-// 384 streams of 2048 tokens, F = 64, bf16, with the states saved: 155 us, 3.7 TB/s; 1170 instructions per warp and chunk at 41 % of the
-// issue slots (three blocks per SM, for the registers), tensor pipe 47 %, shared-memory pipe 54 %: bound by the latencies of a
+// 384 streams of 2048 tokens, F = 64, bf16, with the states saved: 155 us, 3.7 TB/s, in passes back to back (alone with cold caches, under the
+// profiler, 158); float32, without saved states, 616 us.  1170 instructions per warp and chunk at 41 % of the issue slots (three blocks per SM, for the registers), tensor pipe 47 %, shared-memory pipe 54 %: bound by the latencies of a
 // warp's own chain of products and changes of form, which stay in registers because every way through memory is longer.
 //
 // Few streams are cut into segments: a first launch leaves every segment's own state (as if it began with none) and its decay, a
@@ -412,9 +412,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) ttt_gated_join_kernel(const Gate
 }
 static_assert(32 * 32 / 2 % JOIN_THREADS == 0, "whole blocks per stream");
 
-// Streams that do not fill the card are cut into segments until they do; more streams than blocks are resident are cut into as
-// many ranges as blocks are.  Segments of at least LEAST chunks (2 against 4: 36 streams of 1201 tokens 28.7 and 32.8 us), no more of
-// them than blocks run at once (twice as many: 12 streams of 32768 tokens 12 % slower).  Ranges against a block per stream: training of
+// Fewer streams than SMs are cut into segments; more streams than blocks are resident are cut into as many ranges as blocks are; between
+// the two (148 to 444, backward 296; float32 none) there is a block per stream, whatever room that leaves.  Segments of at least LEAST
+// chunks (2 against 4: 36 streams of 1201 tokens 28.7 and 32.8 us), in bf16 no more of them than blocks run at once (twice as many: 12
+// streams of 32768 tokens 12 % slower).  float32 is cut into as many, of which one per SM runs at a time with F = 64 (178 KB of shared
+// memory forward): two or three rounds; its ranges are counted for one block per SM, though the forward of F = 32 has room for two.  Ranges against a block per stream: training of
 // 384 streams of 32 chunks 17 % faster, as no last round runs half empty.
 void gated_split(int64_t streams, int chunks, int dtype, bool backward, int* nseg, int* slots) {
   constexpr int SMS = 148, LEAST = 2;  // (chunks per segment: a segment's states and its second reading must be worth it)

@@ -7,13 +7,18 @@
 //   dx = r (w u - x r^2 mean(w u x)),   dw = sum over rows of u x r,      r = 1 / sqrt(mean(x^2) + eps)
 //
 // Angles are integers: a frequency is held in turns per position as a 64-bit fraction, so position * frequency modulo one turn
-// is one 64-bit product, exact to 2^-33 of a turn at any position, where a float32 angle of position 10^6 would be off by 0.03.
+// is one 64-bit product, exact at any position, where a float32 angle of position 10^6 would be off by 0.03.  What is off is the
+// float32 that the sine takes, by 2^-26 of a turn at most (half a last place near half a turn), and the table, made of frequencies of 53
+// bits: about 2^-55 of a turn per position for the fastest pair, 2^-24 at position 2^31.
 //
 // Memory-bound: 16 bytes per lane and row both ways.  A group of lanes that covers a row owns one token: it makes the token's
 // sines and cosines once and walks the heads of queries and keys with them, a few rows in flight.  Rows of a token's heads are
 // neighbours in [B,T,H,F], rows of neighbouring tokens (the other groups of the warp) in [B,H,T,F]: whole lines in both.  bf16,
 // F = 64: rotation of 32768 tokens of 32 rows 45 us (6.0 TB/s, 0.91 of a copy), norm and rotation of 65536 tokens of 24 rows 72 us, its
-// gradient 108 us (5.6 TB/s both, 0.85).
+// gradient 108 us (5.6 TB/s both, 0.85); float32 calls of the latter sizes 131 and 201 us (0.94 and 0.92), though the gradient's registers
+// leave one block per SM.  Rows off the 16 bytes, and rotated parts that are no multiple of 8, go feature by feature with a warp per row,
+// in instances that spill: bf16, 32768 tokens of 16 + 16 rows of 80 features, 20 of them rotated against 24, the call: norm and rotation
+// 301 to 393 us against 90 to 96, its gradient 850 to 968 against 145 to 152; rotation alone (16 rows) 94 to 123 against 39 to 45.
 #include <type_traits>
 
 #include "ttt_kernels.h"

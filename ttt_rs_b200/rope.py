@@ -154,8 +154,8 @@ def rotary(x: torch.Tensor, rot: Rotary, start_idx: int = 0, positions: Optional
            out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x [B,H,T,F] (float32 or bfloat16, head_dim even up to 256; any strides with contiguous rows: [B,T,H,F] and columns of a
     projection as views) with its rows rotated to positions start_idx + t, or to `positions` ([T] or [B,T], int32 or int64, of
-    either sign).  The result is contiguous [B,H,T,F], or `out` (which may be x itself; not under autograd).  Differentiable
-    with respect to x."""
+    either sign).  The result is contiguous [B,H,T,F], or `out` (which may be x itself but share no other element with it; not recorded
+    for autograd, and refused where that asks for gradients).  Differentiable with respect to x, once and not in forward mode."""
     native = _lib.host().rotary(x, *rot._args, positions, start_idx, 0, out) if isinstance(x, torch.Tensor) and \
         x.dim() == 4 and x.shape[3] == rot.config.head_dim else None
     if native is not None:
@@ -177,7 +177,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Te
                    out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Every head's query and key divided by its root mean square, sqrt(mean(x^2) + eps), multiplied by the weight ([F], of the
     inputs' type; None: ones) and rotated (`rot` None: not), in one pass over both.  q [B,H,T,F] and k [B,Hk,T,F] as in `rotary`,
-    Hk of any number; results contiguous [B,H,T,F], [B,Hk,T,F], or `out`.  Differentiable with respect to q, k and the weights."""
+    Hk of any number; results contiguous [B,H,T,F], [B,Hk,T,F], or `out` as in `rotary` (each may be its own input; neither may share
+    elements with the other's or with the other result).  Differentiable with respect to q, k and the weights, as `rotary` is."""
     args = _NO_ROTATION if rot is None else rot._args
     oq, ok = (None, None) if out is None else out
     fits = rot is None or (isinstance(q, torch.Tensor) and q.dim() == 4 and q.shape[3] == rot.config.head_dim)

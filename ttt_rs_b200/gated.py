@@ -46,7 +46,8 @@ def fused_gated_linear(xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, log
     The state, log_decay, beta, weight and their gradients are float32 throughout (3e-7 of their norm, from bfloat16 inputs too), and so are all
     results of float32 inputs (1e-7).  bfloat16 results are rounded more than once, each time by 2^-8 at most: the decayed products of
     queries and keys (of output gradients and values) and the state (its gradient) become bfloat16 operands.  output, grad_xq, grad_xk and
-    grad_xv are off by 2.3e-3 to 2.4e-3 of their norm, where one rounding of exact results leaves 1.7e-3."""
+    grad_xv are off by 2.3e-3 to 2.4e-3 of their norm, where one rounding of exact results leaves 1.7e-3.  (float32 inputs take three times
+    as long.)"""
     native = _lib.host().gated(xq, xk, xv, log_decay, beta, weight)
     if native is not None:
         return native
@@ -83,7 +84,8 @@ class GatedLinearState:
 
 
 class GatedLinear(torch.nn.Module):
-    """Parameter holder: weight_init [H,F,F] float32 ~ N(0, 0.02) and, per head, the logit of the weight decay.  With the
+    """Parameter holder: weight_init [H,F,F] float32 ~ N(0, 0.02) and, per head, the logit of the weight decay (of another type after
+    `.to(dtype)` of a whole model; states and gates are float32 all the same).  With the
     layer's learning rate eta_t = base_lr sigmoid(.) / F of a token, head h writes with beta_t = eta_t and keeps
     1 - sigmoid(decay_logit_h) sigmoid(.) of its state; the heads' strongest decays start spread from 2^-1 to 2^-7."""
 
@@ -98,7 +100,7 @@ class GatedLinear(torch.nn.Module):
         self.decay_logit = torch.nn.Parameter(torch.log(most) - torch.log1p(-most))
 
     def init_state(self, batch_size: int) -> GatedLinearState:
-        return GatedLinearState(_per_sequence(self.weight_init, batch_size))
+        return GatedLinearState(_per_sequence(self.weight_init.float(), batch_size))
 
     def gates(self, ttt_lr_eta: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         """(log_decay, beta) [B,H,T] float32 from the layer's learning rates."""

@@ -93,3 +93,19 @@ def test_a_rotation_made_in_inference_mode_can_be_differentiated():
     x, w = torch.randn(1, 2, 8, 64, device="cuda").requires_grad_(), torch.ones(64, device="cuda").requires_grad_()
     (dx,) = torch.autograd.grad(tb.rotary(x, rot).sum(), x)
     assert torch.isfinite(dx).all() and all(torch.isfinite(t).all() for t in torch.autograd.grad(tb.qk_norm_rotary(x, x, w, w, rot)[0].sum(), (x, w)))
+
+
+def test_given_results_in_inference_mode():
+    import ttt_rs_b200 as tb
+    rot = tb.Rotary(tb.RotaryConfig(head_dim=64), device="cuda")
+    x, out = torch.randn(2, 2, 3, 8, 64, device="cuda")
+    leaf = torch.randn(2, 3, 8, 64, device="cuda").requires_grad_()
+    a = leaf.exp()
+    with torch.inference_mode():
+        want = tb.rotary(x, rot)
+        assert torch.equal(tb.rotary(x, rot, out=out), want)  # (an ordinary tensor, written while serving)
+        made = torch.empty_like(x)
+        assert torch.equal(tb.rotary(x, rot, out=made), want)
+        tb.rotary(x, rot, out=a)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(a.sum(), leaf)

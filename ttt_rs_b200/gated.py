@@ -43,11 +43,11 @@ def fused_gated_linear(xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, log
     step.  Derivatives in forward mode are refused.  A NaN or an infinity in a token reaches results of the 64 tokens around it, and no
     reset forgets one in the state.
 
-    The state, log_decay, beta, weight and their gradients are float32 throughout (3e-7 of their norm, from bfloat16 inputs too), and so are all
+    The state, log_decay, beta, weight and their gradients are float32 throughout (4e-7 of their norm, from bfloat16 inputs too), and so are all
     results of float32 inputs (1e-7).  bfloat16 results are rounded more than once, each time by 2^-8 at most: the decayed products of
     queries and keys (of output gradients and values) and the state (its gradient) become bfloat16 operands.  output, grad_xq, grad_xk and
-    grad_xv are off by 2.3e-3 to 2.4e-3 of their norm, where one rounding of exact results leaves 1.7e-3.  (float32 inputs take three times
-    as long.)"""
+    grad_xv are off by 2.3e-3 to 2.4e-3 of their norm, where one rounding of exact results leaves 1.7e-3.  (float32 inputs take three to
+    four times as long.)"""
     native = _lib.host().gated(xq, xk, xv, log_decay, beta, weight)
     if native is not None:
         return native

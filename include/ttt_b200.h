@@ -418,6 +418,49 @@ int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads, const void
                                       void* grad_q, void* grad_k, const int64_t* grad_strides, void* grad_q_weight,
                                       void* grad_k_weight, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- causal depthwise convolution; group norm with channels last ---------------------------------------------------
+ * Steps of a layer that remembers through a selective state space scan (no counterpart in the reference, whose convolutions of 1 to 4
+ * taps carry nothing from call to call).  Tensors are T [batch, seq_len, channels] with contiguous channels; `strides`: for each
+ * of the tensors named there the strides of batch and token in elements, not negative (null: contiguous; not read where there is one
+ * row).  Any address that is a multiple of an element is taken; on 16 bytes throughout, the kernels read 16 bytes at a time.  Results are
+ * contiguous.  batch*seq_len < 2^31, channels <= 2^20.
+ *
+ * ttt_layer_causal_conv: y_t = act(bias + sum_j weight_j x_{t-taps+1+j}) channel by channel, taps 2 to 4, activation 0 (none) or 1
+ *   (SiLU).  weight T [channels, taps]; bias T [channels] or null; state T [batch, taps-1, channels] or null (zeros): the inputs before
+ *   the first token; state_out likewise, the last inputs (it may be state, and lies over no other tensor of the call, as y lies over none
+ *   of x and state).  starts uint8 [batch, seq_len] or null: a token with a nonzero start, and those behind it, see no input before it.
+ * ttt_layer_causal_conv_backward: `strides` of x, grad_y; grad_state_out, grad_state T [batch, taps-1, channels] or null; grad_weight,
+ *   grad_bias T or null, summed in float32 in a fixed order; with either, the workspace (16-byte aligned).
+ *
+ * ttt_layer_group_norm: `groups` groups of neighbouring channels; over 0: of every token (up to 4096 channels per group), 1: of every
+ *   sequence (batch row).  u = (x - mean) / sqrt(var + epsilon) * weight + bias; y = act(u) without a gate, u * act(gate) with one;
+ *   activation 0, 1 or 2 (GELU, tanh form).  `strides` of x, gate.  weight, bias T [channels] or null (ones, zeros).  stats float32
+ *   [batch, groups, 2] (out, over 1 only): for the backward, or null.  Variances come from differences, also across blocks.
+ * ttt_layer_group_norm_backward: `strides` of x, gate, grad_y; grad_gate exactly with a gate; grad_weight, grad_bias T or null, summed in
+ *   float32 in a fixed order; workspace where one of them is given, and always over 1.
+ */
+enum ttt_over { TTT_OVER_TOKEN = 0, TTT_OVER_SEQUENCE = 1 };
+int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype, int activation, const void* x,
+                          const int64_t* x_strides, const void* weight, const void* bias, const void* state,
+                          const void* starts, void* y, void* state_out, void* stream);
+size_t ttt_layer_causal_conv_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype);
+int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype, int activation,
+                                   const void* x, const void* grad_y, const int64_t* strides, const void* weight,
+                                   const void* bias, const void* state, const void* starts, const void* grad_state_out,
+                                   void* grad_x, void* grad_weight, void* grad_bias, void* grad_state, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+size_t ttt_layer_group_norm_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype);
+int ttt_layer_group_norm(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype, int activation,
+                         float epsilon, const void* x, const void* gate, const int64_t* strides, const void* weight,
+                         const void* bias, void* y, float* stats, void* workspace, size_t workspace_bytes, void* stream);
+size_t ttt_layer_group_norm_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over,
+                                                     int dtype);
+int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype,
+                                  int activation, float epsilon, const void* x, const void* gate, const void* grad_y,
+                                  const int64_t* strides, const void* weight, const void* bias, const float* stats,
+                                  void* grad_x, void* grad_gate, void* grad_weight, void* grad_bias, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 /* Backward without a caller workspace.  (No counterpart in the reference: its host wrapper always allocates its
  * scratch itself, backward/launch.rs:389-392.)
  *

@@ -53,6 +53,7 @@ class TttError(RuntimeError):
 
 # every symbol include/ttt_b200.h declares: name -> (restype, argtypes)
 _P = C.c_void_p
+_L = C.c_int64
 _DP = C.POINTER(TttDims)
 _RP = C.POINTER(TttRotation)
 SYMBOLS = {
@@ -96,6 +97,13 @@ SYMBOLS = {
     "ttt_layer_qk_norm_rotary": (C.c_int, [_DP, C.c_int, _P, _P, _P, _P, _P, _RP, _P, _P, _P, _P]),
     "ttt_layer_qk_norm_rotary_backward_workspace_bytes": (C.c_size_t, [_DP, C.c_int]),
     "ttt_layer_qk_norm_rotary_backward": (C.c_int, [_DP, C.c_int] + [_P] * 7 + [_RP] + [_P] * 6 + [C.c_size_t, _P]),
+    "ttt_layer_causal_conv": (C.c_int, [_L] * 3 + [C.c_int] * 3 + [_P] * 9),
+    "ttt_layer_causal_conv_backward_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 2),
+    "ttt_layer_causal_conv_backward": (C.c_int, [_L] * 3 + [C.c_int] * 3 + [_P] * 13 + [C.c_size_t, _P]),
+    "ttt_layer_group_norm_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),
+    "ttt_layer_group_norm": (C.c_int, [_L] * 3 + [C.c_int] * 4 + [C.c_float] + [_P] * 8 + [C.c_size_t, _P]),
+    "ttt_layer_group_norm_backward_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),
+    "ttt_layer_group_norm_backward": (C.c_int, [_L] * 3 + [C.c_int] * 4 + [C.c_float] + [_P] * 12 + [C.c_size_t, _P]),
     "ttt_layer_qk_conv_backward": (C.c_int, [_DP, _P, _P, _P, C.c_int64, _P, _P, _P, _P, _P, _P, C.c_size_t, _P]),
 }
 # entry points of this package alone (csrc/ttt_internal.h)

@@ -30,6 +30,12 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+}  // namespace
+namespace ttt {
+int abi_error(int code, const char* message) { return fail(code, "%s", message); }
+}  // namespace ttt
+namespace {
+
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                               const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

@@ -1,0 +1,256 @@
+// C ABI of the operators of a selective state space layer (include/ttt_b200.h): causal convolution, group norm with channels last.
+// Argument checks and launches.
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/ttt_b200.h"
+#include "ttt_kernels.h"
+
+namespace ttt {
+int abi_error(int code, const char* message);  // ttt_abi.cu: the thread's last error
+}
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char message[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(message, sizeof(message), fmt, ap);
+  va_end(ap);
+  return ttt::abi_error(code, message);
+}
+int launched(cudaError_t e, const char* what) {
+  return e == cudaSuccess ? TTT_OK : fail(TTT_ERR_CUDA, "%s launch failed: %s", what, cudaGetErrorString(e));
+}
+
+constexpr int64_t kMostChannels = 1 << 20;
+
+int check_sizes(int64_t B, int64_t T, int64_t C, int dtype) {
+  if (B <= 0 || T <= 0 || C <= 0) return fail(TTT_ERR_SHAPE, "batch, seq_len and channels must be positive");
+  if (dtype != TTT_F32 && dtype != TTT_BF16) return fail(TTT_ERR_UNSUPPORTED, "unknown dtype %d", dtype);
+  if (C > kMostChannels) return fail(TTT_ERR_UNSUPPORTED, "at most %lld channels", (long long)kMostChannels);
+  if (B >= (int64_t)1 << 31 || T >= (int64_t)1 << 31 || B * T >= (int64_t)1 << 31) return fail(TTT_ERR_SHAPE, "batch*seq_len must be below 2^31");
+  return TTT_OK;
+}
+int check_bytes(size_t have, size_t need, const void* p, const char* name) {
+  if (need == 0) return TTT_OK;
+  if (p == nullptr || have < need) return fail(TTT_ERR_WORKSPACE, "%s has %zu bytes, %zu needed", name, p == nullptr ? (size_t)0 : have, need);
+  if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return fail(TTT_ERR_ALIGN, "%s is not 16-byte aligned", name);
+  return TTT_OK;
+}
+
+// Tensors [B,T,C] (or shorter) with contiguous channels: widest vector of channels that all of them allow, and the bytes they span.
+struct Spans {
+  int64_t B, T, C;
+  int es;
+  uintptr_t low = 0;  // OR of the addresses and strides in bytes: what they are multiples of
+  int rc = TTT_OK;
+  void align(const char* name, const void* p) {
+    if (rc != TTT_OK || p == nullptr) return;
+    if (reinterpret_cast<uintptr_t>(p) % es != 0) rc = fail(TTT_ERR_ALIGN, "%s is not aligned to its elements", name);
+    low |= reinterpret_cast<uintptr_t>(p);
+  }
+  void need(const char* name, const void* p) {
+    if (rc == TTT_OK && p == nullptr) rc = fail(TTT_ERR_NULL, "%s is null", name);
+    align(name, p);
+  }
+  // strides of batch and token of tensor `i` (null: contiguous), 0 where there is one row only
+  void rows(const char* name, const void* p, const int64_t* strides, int i, int64_t (&out)[2], bool optional = false) {
+    out[0] = out[1] = 0;
+    if (optional && p == nullptr) return;
+    need(name, p);
+    const int64_t dense[2] = {T * C, C}, size[2] = {B, T};
+    for (int k = 0; k < 2; ++k) {
+      out[k] = size[k] == 1 ? 0 : strides != nullptr ? strides[2 * i + k] : dense[k];
+      low |= (uintptr_t)(out[k] * es);
+      if (rc == TTT_OK && out[k] < 0) rc = fail(TTT_ERR_SHAPE, "the strides of %s must not be negative", name);
+      if (rc == TTT_OK && out[k] > ((int64_t)1 << 60) / size[k]) rc = fail(TTT_ERR_SHAPE, "the strides of %s are out of range", name);
+    }
+  }
+  int64_t bytes(const int64_t (&s)[2]) const { return ((B - 1) * s[0] + (T - 1) * s[1] + C) * es; }
+};
+// A result (contiguous, `size` bytes) must share nothing with another tensor of the call; `same`: it may be that tensor itself
+int check_apart(const char* name, const void* out, int64_t size, const char* other_name, const void* other, int64_t other_size, bool same) {
+  if (out == nullptr || other == nullptr || (same && out == other && size == other_size)) return TTT_OK;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(other);
+  if (a < b + (uintptr_t)other_size && b < a + (uintptr_t)size) return fail(TTT_ERR_SHAPE, "%s lies over %s", name, other_name);
+  return TTT_OK;
+}
+
+int check_conv(int64_t B, int64_t T, int64_t C, int taps, int dtype, int activation) {
+  const int rc = check_sizes(B, T, C, dtype);
+  if (rc != TTT_OK) return rc;
+  if (taps < 2 || taps > 4) return fail(TTT_ERR_UNSUPPORTED, "Unsupported taps=%d (supported: 2, 3, 4)", taps);
+  if (activation != ttt::ACT_NONE && activation != ttt::ACT_SILU)
+    return fail(TTT_ERR_UNSUPPORTED, "unknown activation %d (0: none, 1: SiLU)", activation);
+  return TTT_OK;
+}
+
+}  // namespace
+
+extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype, int activation, const void* x,
+                                     const int64_t* x_strides, const void* weight, const void* bias, const void* state,
+                                     const void* starts, void* y, void* state_out, void* stream) {
+  int rc = check_conv(batch, seq_len, channels, taps, dtype, activation);
+  if (rc != TTT_OK) return rc;
+  const int es = dtype == TTT_BF16 ? 2 : 4;
+  ttt::ConvParams p{};
+  Spans s{batch, seq_len, channels, es};
+  s.rows("x", x, x_strides, 0, p.xs);
+  s.need("y", y);
+  s.need("state_out", state_out);
+  s.align("state", state);
+  const bool vec = s.low % 16 == 0 && channels * es % 16 == 0;
+  s.need("weight", weight);
+  s.align("bias", bias);
+  if (s.rc != TTT_OK) return s.rc;
+  const int64_t held = batch * (taps - 1) * channels * es, n = batch * seq_len * channels * es;
+  if ((rc = check_apart("state_out", state_out, held, "state", state, held, true)) != TTT_OK ||
+      (rc = check_apart("state_out", state_out, held, "x", x, s.bytes(p.xs), false)) != TTT_OK ||
+      (rc = check_apart("state_out", state_out, held, "y", y, n, false)) != TTT_OK ||
+      (rc = check_apart("state_out", state_out, held, "weight", weight, channels * taps * es, false)) != TTT_OK ||
+      (rc = check_apart("state_out", state_out, held, "bias", bias, channels * es, false)) != TTT_OK ||
+      (rc = check_apart("state_out", state_out, held, "starts", starts, batch * seq_len, false)) != TTT_OK ||
+      (rc = check_apart("y", y, n, "x", x, s.bytes(p.xs), false)) != TTT_OK ||
+      (rc = check_apart("y", y, n, "state", state, held, false)) != TTT_OK)
+    return rc;
+  p.x = x, p.w = weight, p.bias = bias, p.state = state, p.starts = static_cast<const uint8_t*>(starts);
+  p.y = y, p.state_out = state_out;
+  p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
+  return launched(ttt::launch_conv(dtype, p, taps, vec, static_cast<cudaStream_t>(stream)), "causal convolution");
+}
+
+extern "C" size_t ttt_layer_causal_conv_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype) {
+  if (check_conv(batch, seq_len, channels, taps, dtype, 0) != TTT_OK) return 0;
+  return sizeof(float) * ttt::conv_partial_floats(batch, seq_len, (int)channels, taps);
+}
+
+extern "C" int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype, int activation,
+                                              const void* x, const void* grad_y, const int64_t* strides, const void* weight,
+                                              const void* bias, const void* state, const void* starts, const void* grad_state_out,
+                                              void* grad_x, void* grad_weight, void* grad_bias, void* grad_state, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+  int rc = check_conv(batch, seq_len, channels, taps, dtype, activation);
+  if (rc != TTT_OK) return rc;
+  const int es = dtype == TTT_BF16 ? 2 : 4;
+  ttt::ConvParams p{};
+  Spans s{batch, seq_len, channels, es};
+  s.rows("x", x, strides, 0, p.xs);
+  s.rows("grad_y", grad_y, strides, 1, p.gs);
+  s.need("grad_x", grad_x);
+  s.align("state", state);
+  s.align("grad_state_out", grad_state_out);
+  s.align("grad_state", grad_state);
+  const bool vec = s.low % 16 == 0 && channels * es % 16 == 0;
+  s.need("weight", weight);
+  s.align("bias", bias);
+  s.align("grad_weight", grad_weight);
+  s.align("grad_bias", grad_bias);
+  if (s.rc != TTT_OK) return s.rc;
+  const bool sums = grad_weight != nullptr || grad_bias != nullptr;
+  if (sums && (rc = check_bytes(workspace_bytes, ttt_layer_causal_conv_backward_workspace_bytes(batch, seq_len, channels, taps, dtype), workspace,
+                                "workspace")) != TTT_OK)
+    return rc;
+  p.x = x, p.w = weight, p.bias = bias, p.state = state, p.starts = static_cast<const uint8_t*>(starts);
+  p.gy = grad_y, p.gstate_out = grad_state_out, p.gx = grad_x, p.gstate = grad_state, p.gw = grad_weight, p.gbias = grad_bias;
+  p.partials = sums ? static_cast<float*>(workspace) : nullptr;
+  p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
+  return launched(ttt::launch_conv_bwd(dtype, p, taps, vec, static_cast<cudaStream_t>(stream)), "causal convolution backward");
+}
+
+namespace {
+
+int check_norm(int64_t B, int64_t T, int64_t C, int G, int over, int dtype, int activation, float eps) {
+  const int rc = check_sizes(B, T, C, dtype);
+  if (rc != TTT_OK) return rc;
+  if (G <= 0 || C % G != 0) return fail(TTT_ERR_SHAPE, "channels=%lld are not a multiple of groups=%d", (long long)C, G);
+  if (over != TTT_OVER_TOKEN && over != TTT_OVER_SEQUENCE) return fail(TTT_ERR_UNSUPPORTED, "over=%d (0: tokens, 1: sequences)", over);
+  if (over == TTT_OVER_TOKEN && C / G > ttt::NORM_TOKEN_CHANNELS)
+    return fail(TTT_ERR_UNSUPPORTED, "groups of up to %d channels are normed token by token (got %lld)", ttt::NORM_TOKEN_CHANNELS, (long long)(C / G));
+  if (activation < ttt::ACT_NONE || activation > ttt::ACT_GELU)
+    return fail(TTT_ERR_UNSUPPORTED, "unknown activation %d (0: none, 1: SiLU, 2: GELU)", activation);
+  if (!(eps >= 0.f)) return fail(TTT_ERR_SHAPE, "epsilon must be >= 0");
+  return TTT_OK;
+}
+void norm_dims(ttt::NormParams* p, int64_t B, int64_t T, int64_t C, int G, int activation, float eps) {
+  p->B = B, p->T = T, p->tokens = B * T, p->C = (int)C, p->G = G, p->c = (int)(C / G), p->act = activation, p->eps = eps;
+  p->inv_c = 1.f / (float)p->c;
+}
+bool flat_rows(const int64_t (&s)[2], int64_t B, int64_t T) { return B == 1 || (T > 1 && s[0] == T * s[1]); }
+int norm_width(uintptr_t low, int c, int es) {
+  if (low % 16 == 0 && c % (16 / es) == 0) return 16 / es;
+  return low % (2 * es) == 0 && c % 2 == 0 ? 2 : 1;
+}
+
+}  // namespace
+
+extern "C" size_t ttt_layer_group_norm_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype) {
+  if (check_norm(batch, seq_len, channels, groups, over, dtype, 0, 0.f) != TTT_OK) return 0;
+  return sizeof(float) * ttt::norm_forward_floats(batch, seq_len, (int)channels, groups, over == TTT_OVER_SEQUENCE, dtype == TTT_BF16 ? 2 : 4);
+}
+extern "C" size_t ttt_layer_group_norm_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype) {
+  if (check_norm(batch, seq_len, channels, groups, over, dtype, 0, 0.f) != TTT_OK) return 0;
+  return sizeof(float) * ttt::norm_backward_floats(batch, seq_len, (int)channels, groups, over == TTT_OVER_SEQUENCE, dtype == TTT_BF16 ? 2 : 4);
+}
+
+extern "C" int ttt_layer_group_norm(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype, int activation,
+                                    float epsilon, const void* x, const void* gate, const int64_t* strides, const void* weight,
+                                    const void* bias, void* y, float* stats, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_norm(batch, seq_len, channels, groups, over, dtype, activation, epsilon);
+  if (rc != TTT_OK) return rc;
+  ttt::NormParams p{};
+  norm_dims(&p, batch, seq_len, channels, groups, activation, epsilon);
+  const int es = dtype == TTT_BF16 ? 2 : 4;
+  Spans s{batch, seq_len, channels, es};
+  s.rows("x", x, strides, 0, p.xs);
+  s.rows("gate", gate, strides, 1, p.gates, true);
+  s.need("y", y);
+  s.align("weight", weight);
+  s.align("bias", bias);
+  if (s.rc != TTT_OK) return s.rc;
+  if ((reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return fail(TTT_ERR_ALIGN, "stats is not aligned to its elements");
+  if ((rc = check_bytes(workspace_bytes, ttt_layer_group_norm_workspace_bytes(batch, seq_len, channels, groups, over, dtype), workspace,
+                        "workspace")) != TTT_OK)
+    return rc;
+  p.flat = flat_rows(p.xs, batch, seq_len) && (gate == nullptr || flat_rows(p.gates, batch, seq_len));
+  p.x = x, p.gate = gate, p.w = weight, p.bias = bias, p.y = y, p.stats = stats, p.moments = static_cast<float*>(workspace);
+  return launched(ttt::launch_norm(dtype, p, norm_width(s.low, p.c, es), over == TTT_OVER_SEQUENCE, false, static_cast<cudaStream_t>(stream)),
+                  "group norm");
+}
+
+extern "C" int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int over, int dtype,
+                                             int activation, float epsilon, const void* x, const void* gate, const void* grad_y,
+                                             const int64_t* strides, const void* weight, const void* bias, const float* stats,
+                                             void* grad_x, void* grad_gate, void* grad_weight, void* grad_bias, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+  int rc = check_norm(batch, seq_len, channels, groups, over, dtype, activation, epsilon);
+  if (rc != TTT_OK) return rc;
+  ttt::NormParams p{};
+  norm_dims(&p, batch, seq_len, channels, groups, activation, epsilon);
+  const int es = dtype == TTT_BF16 ? 2 : 4;
+  const bool sequence = over == TTT_OVER_SEQUENCE;
+  Spans s{batch, seq_len, channels, es};
+  s.rows("x", x, strides, 0, p.xs);
+  s.rows("gate", gate, strides, 1, p.gates, true);
+  s.rows("grad_y", grad_y, strides, 2, p.gys);
+  s.need("grad_x", grad_x);
+  if (gate != nullptr) s.need("grad_gate", grad_gate);
+  s.align("weight", weight);
+  s.align("bias", bias);
+  const int width = norm_width(s.low, p.c, es);
+  s.align("grad_weight", grad_weight);
+  s.align("grad_bias", grad_bias);
+  if (s.rc != TTT_OK) return s.rc;
+  if (sequence && stats == nullptr) return fail(TTT_ERR_NULL, "stats is null");
+  if ((reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return fail(TTT_ERR_ALIGN, "stats is not aligned to its elements");
+  const bool sums = sequence || grad_weight != nullptr || grad_bias != nullptr;
+  if (sums && (rc = check_bytes(workspace_bytes, ttt_layer_group_norm_backward_workspace_bytes(batch, seq_len, channels, groups, over, dtype),
+                                workspace, "workspace")) != TTT_OK)
+    return rc;
+  p.flat = flat_rows(p.xs, batch, seq_len) && flat_rows(p.gys, batch, seq_len) && (gate == nullptr || flat_rows(p.gates, batch, seq_len));
+  p.x = x, p.gate = gate, p.gy = grad_y, p.w = weight, p.bias = bias, p.stats = const_cast<float*>(stats);
+  p.gx = grad_x, p.ggate = grad_gate, p.gw = grad_weight, p.gb = grad_bias;
+  p.partials = sums ? static_cast<float*>(workspace) : nullptr;
+  return launched(ttt::launch_norm(dtype, p, width, sequence, true, static_cast<cudaStream_t>(stream)), "group norm backward");
+}

@@ -513,6 +513,162 @@ struct QkNormFn : torch::autograd::Function<QkNormFn> {
   }
 };
 
+// ---- causal convolution, group norm: tensors [B,T,C] with contiguous channels -------------------------------------------------
+bool channel_rows(const Tensor& t, const c10::Device& dev, at::ScalarType dt) {
+  if (!t.defined() || !t.is_cuda() || t.device() != dev || t.scalar_type() != dt || t.layout() != c10::kStrided || t.dim() != 3) return false;
+  return (t.stride(2) == 1 || t.size(2) == 1) && (t.stride(0) >= 0 || t.size(0) == 1) && (t.stride(1) >= 0 || t.size(1) == 1);
+}
+struct Rows {  // what [B,T,C] of a GPU operator is
+  int64_t B = 0, T = 0, C = 0;
+  int dtype = 0;
+  at::ScalarType dt = at::kFloat;
+  c10::Device dev = c10::Device(c10::kCPU);
+  bool set(const Tensor& x) {
+    if (!x.defined() || !x.is_cuda() || x.dim() != 3) return false;
+    dt = x.scalar_type(), dev = x.device();
+    if ((dt != at::kBFloat16 && dt != at::kFloat) || !channel_rows(x, dev, dt)) return false;
+    B = x.size(0), T = x.size(1), C = x.size(2);
+    dtype = dt == at::kBFloat16 ? TTT_BF16 : TTT_F32;
+    return B > 0 && T > 0 && C > 0;
+  }
+  at::TensorOptions opt() const { return at::TensorOptions().dtype(dt).device(dev); }
+  at::TensorOptions opt(at::ScalarType t) const { return at::TensorOptions().dtype(t).device(dev); }
+  void* stream() const { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+  Tensor empty() const { return at::empty({B, T, C}, opt()); }
+  bool vector(const Tensor& t, at::ScalarType of) const { return !t.defined() || is(t, of, dev, {C}); }
+  bool marks(const Tensor& t) const {
+    return !t.defined() || ((t.scalar_type() == at::kBool || t.scalar_type() == at::kByte) && is(t, t.scalar_type(), dev, {B, T}));
+  }
+};
+template <size_t N>
+std::array<int64_t, 2 * N> row_strides(const std::array<const Tensor*, N>& ts) {
+  std::array<int64_t, 2 * N> s{};
+  for (size_t i = 0; i < N; ++i)
+    if (ts[i]->defined()) s[2 * i] = ts[i]->stride(0), s[2 * i + 1] = ts[i]->stride(1);
+  return s;
+}
+Tensor workspace(const Rows& m, size_t bytes) { return bytes != 0 ? at::empty({(int64_t)bytes}, m.opt(at::kByte)) : Tensor(); }
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+// a gradient as the kernels read it
+Tensor rows_of(const Tensor& g, const Rows& m) { return channel_rows(g, m.dev, m.dt) ? g : g.clone(at::MemoryFormat::Contiguous); }
+
+struct Conv {
+  Rows m;
+  int64_t K = 0;
+  int act = 0;
+  bool set(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& state, const Tensor& starts, int64_t a) {
+    if (!m.set(x) || w.dim() != 2) return false;
+    K = w.size(1), act = (int)a;
+    return K >= 2 && K <= 4 && is(w, m.dt, m.dev, {m.C, K}) && m.vector(bias, m.dt) && held(state) && m.marks(starts);
+  }
+  bool held(const Tensor& s) const { return !s.defined() || is(s, m.dt, m.dev, {m.B, K - 1, m.C}); }
+  int forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& state, const Tensor& starts, Tensor& y, Tensor& out) const {
+    c10::cuda::CUDAGuard guard(m.dev);
+    y = m.empty();
+    if (!out.defined()) out = at::empty({m.B, K - 1, m.C}, m.opt());
+    return ttt_layer_causal_conv(m.B, m.T, m.C, (int)K, m.dtype, act, x.const_data_ptr(), row_strides<1>({&x}).data(), w.const_data_ptr(),
+                                 ptr(bias), ptr(state), ptr(starts), y.data_ptr(), out.data_ptr(), m.stream());
+  }
+};
+struct ConvFn : torch::autograd::Function<ConvFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& state,
+                               const Tensor& starts, std::vector<int64_t> has) {
+    Conv call;
+    Tensor y, out;
+    const Tensor b = has[0] ? bias : Tensor(), st = has[1] ? state : Tensor(), mk = has[2] ? starts : Tensor();
+    call.set(x, w, b, st, mk, has[3]);
+    const int rc = call.forward(x, w, b, st, mk, y, out);
+    if (rc != TTT_OK) throw_error(rc);
+    ctx->save_for_backward({x, w, bias, state, starts});
+    ctx->saved_data["has"] = has;
+    ctx->set_materialize_grads(false);
+    return {y, out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const variable_list t = ctx->get_saved_variables();
+    const std::vector<int64_t> has = ctx->saved_data["has"].toIntVector();
+    if (!go[0].defined() && !go[1].defined()) return variable_list(6);
+    Conv call;
+    const Tensor &x = t[0], &w = t[1], b = has[0] ? t[2] : Tensor(), st = has[1] ? t[3] : Tensor(), mk = has[2] ? t[4] : Tensor();
+    call.set(x, w, b, st, mk, has[3]);
+    const Rows& m = call.m;
+    c10::cuda::CUDAGuard guard(m.dev);
+    const Tensor gy = go[0].defined() ? rows_of(go[0], m) : at::zeros({m.B, m.T, m.C}, m.opt());
+    const Tensor gs = go[1].defined() ? go[1].contiguous() : Tensor();
+    Tensor gx = m.empty(), gw, gb, gst;
+    if (ctx->needs_input_grad(1)) gw = at::empty_like(w);
+    if (has[0] && ctx->needs_input_grad(2)) gb = at::empty_like(b);
+    if (has[1]) gst = at::empty_like(st);
+    const size_t wsb = gw.defined() || gb.defined() ? ttt_layer_causal_conv_backward_workspace_bytes(m.B, m.T, m.C, (int)call.K, m.dtype) : 0;
+    const Tensor ws = workspace(m, wsb);
+    const int rc = ttt_layer_causal_conv_backward(
+        m.B, m.T, m.C, (int)call.K, m.dtype, call.act, x.const_data_ptr(), gy.const_data_ptr(), row_strides<2>({&x, &gy}).data(),
+        w.const_data_ptr(), ptr(b), ptr(st), ptr(mk), ptr(gs), gx.data_ptr(), data(gw), data(gb), data(gst), data(ws), wsb, m.stream());
+    if (rc != TTT_OK) throw_error(rc);
+    return only_once({gx, gw, gb, gst, Tensor(), Tensor()});
+  }
+};
+
+struct Norm {
+  Rows m;
+  int64_t G = 0;
+  int act = 0, over = 0;
+  float eps = 0.f;
+  bool set(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& gate, int64_t groups, int64_t a, int64_t ov, double e) {
+    G = groups, act = (int)a, over = (int)ov, eps = (float)e;
+    return m.set(x) && G > 0 && G <= m.C && m.C % G == 0 && m.vector(w, m.dt) && m.vector(b, m.dt) &&
+           (!gate.defined() || (channel_rows(gate, m.dev, m.dt) && gate.sizes() == x.sizes()));
+  }
+  int forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& gate, bool save, Tensor& y, Tensor& stats) const {
+    c10::cuda::CUDAGuard guard(m.dev);
+    y = m.empty();
+    const size_t wsb = over == TTT_OVER_SEQUENCE ? ttt_layer_group_norm_workspace_bytes(m.B, m.T, m.C, (int)G, over, m.dtype) : 0;
+    const Tensor ws = workspace(m, wsb);
+    if (save && over == TTT_OVER_SEQUENCE) stats = at::empty({m.B, G, 2}, m.opt(at::kFloat));
+    return ttt_layer_group_norm(m.B, m.T, m.C, (int)G, over, m.dtype, act, eps, x.const_data_ptr(), ptr(gate),
+                                row_strides<2>({&x, &gate}).data(), ptr(w), ptr(b), y.data_ptr(), static_cast<float*>(data(stats)),
+                                data(ws), wsb, m.stream());
+  }
+};
+struct NormFn : torch::autograd::Function<NormFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& gate,
+                        std::vector<int64_t> has, double eps) {  // has: weight, bias, gate; groups, activation, over
+    Norm call;
+    Tensor y, stats;
+    const Tensor w0 = has[0] ? w : Tensor(), b0 = has[1] ? b : Tensor(), g0 = has[2] ? gate : Tensor();
+    call.set(x, w0, b0, g0, has[3], has[4], has[5], eps);
+    const int rc = call.forward(x, w0, b0, g0, true, y, stats);
+    if (rc != TTT_OK) throw_error(rc);
+    ctx->save_for_backward({x, w, b, gate, given(stats)});
+    ctx->saved_data["has"] = has;
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const variable_list t = ctx->get_saved_variables();
+    const std::vector<int64_t> has = ctx->saved_data["has"].toIntVector();
+    const Tensor &x = t[0], w = has[0] ? t[1] : Tensor(), b = has[1] ? t[2] : Tensor(), gate = has[2] ? t[3] : Tensor();
+    Norm call;
+    call.set(x, w, b, gate, has[3], has[4], has[5], ctx->saved_data["eps"].toDouble());
+    const Rows& m = call.m;
+    c10::cuda::CUDAGuard guard(m.dev);
+    const Tensor gy = rows_of(go[0], m);
+    Tensor gx = m.empty(), gw, gb, gg;
+    if (has[0] && ctx->needs_input_grad(1)) gw = at::empty_like(w);
+    if (has[1] && ctx->needs_input_grad(2)) gb = at::empty_like(b);
+    if (has[2]) gg = m.empty();
+    const bool sums = call.over == TTT_OVER_SEQUENCE || gw.defined() || gb.defined();
+    const size_t wsb = sums ? ttt_layer_group_norm_backward_workspace_bytes(m.B, m.T, m.C, (int)call.G, call.over, m.dtype) : 0;
+    const Tensor ws = workspace(m, wsb);
+    const int rc = ttt_layer_group_norm_backward(
+        m.B, m.T, m.C, (int)call.G, call.over, m.dtype, call.act, call.eps, x.const_data_ptr(), ptr(gate), gy.const_data_ptr(),
+        row_strides<3>({&x, &gate, &gy}).data(), ptr(w), ptr(b), call.over == TTT_OVER_SEQUENCE ? t[4].const_data_ptr<float>() : nullptr,
+        gx.data_ptr(), data(gg), data(gw), data(gb), data(ws), wsb, m.stream());
+    if (rc != TTT_OK) throw_error(rc);
+    return only_once({gx, gw, gb, gg, Tensor(), Tensor()});
+  }
+};
+
 // ---- Python functions ----------------------------------------------------------------------------------------------
 // tensors args[0..n), false when one is not a tensor
 template <int N>
@@ -1234,6 +1390,53 @@ PyObject* py_qk_norm_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// causal_conv(x, weight, bias | None, state | None, activation, starts | None, state_out | None) -> (y, state), recorded for autograd
+// where that is on and asked for | None
+PyObject* py_causal_conv(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 7)) return nullptr;
+  Tensor x[2], bias, state, starts, out, y;
+  NONE_IF(!tensors(args, x) || !optional_tensor(args[2], bias) || !optional_tensor(args[3], state) || !optional_tensor(args[5], starts) ||
+          !optional_tensor(args[6], out));
+  const int64_t act = as_int(args[4]);
+  if (PyErr_Occurred()) return nullptr;
+  refuse_tangents({&x[0], &x[1], &bias, &state, &out});
+  Conv call;
+  NONE_IF(!call.set(x[0], x[1], bias, state, starts, act) || !call.held(out));
+  if (wants_grad({&x[0], &x[1], &bias, &state, &out})) {  // (a given state is not recorded: the caller's check refuses it)
+    NONE_IF(out.defined());
+    return wrap(ConvFn::apply(x[0], x[1], given(bias), given(state), given(starts),
+                              std::vector<int64_t>{bias.defined(), state.defined(), starts.defined(), act}));
+  }
+  const bool given_out = out.defined();
+  const int rc = call.forward(x[0], x[1], bias, state, starts, y, out);
+  if (rc != TTT_OK) throw_error(rc);
+  if (given_out) overwritten(out);
+  return wrap({y, out});
+  END_HANDLE_TH_ERRORS
+}
+// group_norm(x, groups, weight | None, bias | None, gate | None, activation, eps, over) -> y, recorded for autograd where that is on
+// and asked for | None
+PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 8)) return nullptr;
+  Tensor x[1], w, b, gate, y, stats;
+  NONE_IF(!tensors(args, x) || !optional_tensor(args[2], w) || !optional_tensor(args[3], b) || !optional_tensor(args[4], gate));
+  const int64_t groups = as_int(args[1]), act = as_int(args[5]), over = as_int(args[7]);
+  const double eps = PyFloat_AsDouble(args[6]);
+  if (PyErr_Occurred()) return nullptr;
+  refuse_tangents({&x[0], &w, &b, &gate});
+  Norm call;
+  NONE_IF(groups > INT32_MAX || !call.set(x[0], w, b, gate, groups, act, over, eps));
+  if (wants_grad({&x[0], &w, &b, &gate}))
+    return THPVariable_Wrap(NormFn::apply(x[0], given(w), given(b), given(gate),
+                                          std::vector<int64_t>{w.defined(), b.defined(), gate.defined(), groups, act, over}, eps));
+  const int rc = call.forward(x[0], w, b, gate, false, y, stats);
+  if (rc != TTT_OK) throw_error(rc);
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(set_status),
@@ -1251,6 +1454,8 @@ PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(rotary),
                          FAST(qk_norm),
                          FAST(qk_norm_backward),
+                         FAST(causal_conv),
+                         FAST(group_norm),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

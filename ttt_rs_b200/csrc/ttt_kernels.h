@@ -485,4 +485,49 @@ size_t rotary_partial_floats(int64_t tokens, int rows, int F, bool f32);
 // vec: F and rdim multiples of 8, all rows on 16 bytes
 cudaError_t launch_rotary(int dtype, const RotaryParams& p, bool vec, bool half, bool norm, bool bwd, cudaStream_t st);
 
+
+// activations of the operators below (GELU: the tanh form)
+enum : int { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2 };
+
+// ---- causal depthwise convolution (ttt_conv.cu): tensors [B,T,C] with contiguous channels ------------------------------------------
+struct ConvParams {
+  const void *x, *w, *bias, *state;  // w [C][K]; bias [C] or null: zeros; state [B][K-1][C] or null: zeros
+  const uint8_t* starts;             // [B][T], nonzero: the token sees nothing before it; or null
+  void *y, *state_out;               // contiguous; state_out may be state
+  const void *gy, *gstate_out;       // backward: gradients of y and (or null) of state_out
+  void *gx, *gstate, *gw, *gbias;    // gstate, gw, gbias: or null
+  float* partials;                   // conv_partial_floats, or null: no gradients of weight and bias
+  int64_t xs[2], gs[2];              // strides of batch and token of x and gy, in elements
+  int64_t B, T;
+  int C, act;
+  int lanes_log, strip;              // set by the launch
+  int64_t strips;
+};
+size_t conv_partial_floats(int64_t B, int64_t T, int C, int K);
+cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, bool vec, cudaStream_t st);
+cudaError_t launch_conv_bwd(int dtype, const ConvParams& p, int taps, bool vec, cudaStream_t st);
+
+// ---- group norm (ttt_norm.cu): tensors [B,T,C] with contiguous channels ------------------------------------------------------------
+struct NormParams {
+  const void *x, *w, *bias, *gate;   // w, bias [C], gate [B,T,C], or null
+  void* y;
+  float* stats;                      // sequences: [B][G] mean and 1 / sqrt(var + eps), written by the forward (or null), read by the backward
+  float* moments;                    // sequences, forward: norm_forward_floats
+  const void* gy;
+  void *gx, *ggate, *gw, *gb;
+  float* partials;                   // backward: norm_backward_floats (a token's groups: or null, no gradients of weight and bias)
+  float* sums;                       // set by the launch, like all below G
+  int64_t xs[2], gates[2], gys[2];   // strides of batch and token, in elements
+  int64_t B, T, tokens;
+  bool flat;                         // rows of x, gate and gy are one token stride apart throughout
+  int C, G, c, act;
+  float eps, inv_c;
+  int lanes, cols, rows, per_block, spans, chunks;
+  int64_t chunk;
+};
+constexpr int NORM_TOKEN_CHANNELS = 4096;  // a token's groups: channels at most
+size_t norm_forward_floats(int64_t B, int64_t T, int C, int G, bool sequence, int element_bytes);
+size_t norm_backward_floats(int64_t B, int64_t T, int C, int G, bool sequence, int element_bytes);
+cudaError_t launch_norm(int dtype, const NormParams& p, int V, bool sequence, bool bwd, cudaStream_t st);
+
 }  // namespace ttt

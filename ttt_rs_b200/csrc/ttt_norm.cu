@@ -1,0 +1,763 @@
+// Group norm with channels last, [B,T,C], forward and backward, with an activation or a gate.
+//
+//   n = (x - mean) / sqrt(var + eps) over a group of c = C / G neighbouring channels, of one token or of a whole sequence
+//   u = n w + b;    y = act(u), or u act(gate)
+// Gradients, with du = dy act'(u) or dy act(gate), p = du w and means over the group:
+//   dx = (p - mean(p) - n mean(p n)) / sqrt(var + eps),  dw = sum du n,  db = sum du,  dgate = dy u act'(gate)
+// Variances are sums of squares of differences from the mean, never differences of sums.
+//
+// Memory-bound.
+//   A token's groups: eight channels per thread, a group to a power of two of lanes (several warps where it has more than 256
+//   channels), everything in registers between one read and one write.  A thread keeps its channels from token to token, so that
+//   weights and their gradients stay in registers; the backward's blocks leave a row of sums each, joined in a fixed order.
+//   A sequence's groups: a pass for the statistics (backward: for every channel's sums of du and du n) and one that applies them,
+//   which reads x again, from L2 where the tensors fit.  Chunks of tokens leave (mean, sum of squares) pairs that every block of the
+//   second pass joins in the same order.
+#include "ttt_kernels.h"
+#include "ttt_vec.cuh"
+
+namespace ttt {
+
+constexpr int NORM_THREADS = 256;
+constexpr int NORM_EACH = 8;  // channels per thread, a token's groups
+constexpr int NORM_WIDE = NORM_TOKEN_CHANNELS / NORM_EACH;  // threads at most, of groups that several warps share
+
+__device__ __forceinline__ int64_t norm_row(const NormParams& p, int64_t token, const int64_t (&s)[2]) {
+  if (p.flat) return token * s[1];
+  const int64_t b = token / p.T;
+  return b * s[0] + (token - b * p.T) * s[1];
+}
+
+// sum over the lanes of a group; wide: over its warps too (red: a float per warp, all threads of the block take part)
+template <bool WIDE>
+__device__ __forceinline__ float norm_sum(float v, int lanes, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (WIDE) {
+    const int warp = threadIdx.x >> 5, first = warp & ~((lanes >> 5) - 1);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int k = 0; k < (lanes >> 5); ++k) v += red[first + k];
+  }
+  return v;
+}
+
+template <typename T, int V>
+struct NormLane {  // a thread's channels
+  static constexpr int NV = NORM_EACH / V, P = Chan<T, V>::P;
+  int c0;           // first channel of the group
+  int at[NV];       // channels of the group: V from each on, or -1
+  F2 w[NV][P], b[NV][P];
+  __device__ __forceinline__ void set(const NormParams& p, int g, int l, bool live) {
+    c0 = g * p.c;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int e = (n * p.lanes + l) * V;
+      at[n] = live && e < p.c ? e : -1;
+#pragma unroll
+      for (int k = 0; k < P; ++k) w[n][k] = f2(1.f), b[n][k] = f2(0.f);
+      if (at[n] >= 0) {
+        Chan<T, V> r;
+        if (p.w != nullptr) r.load(static_cast<const T*>(p.w) + c0 + at[n]), r.unpack(w[n]);
+        if (p.bias != nullptr) r.load(static_cast<const T*>(p.bias) + c0 + at[n]), r.unpack(b[n]);
+      }
+    }
+  }
+};
+
+// difference from the mean and 1 / sqrt(var + eps) of a thread's channels (d: the channels on entry)
+template <typename T, int V, bool WIDE>
+__device__ __forceinline__ float norm_stats(F2 (&d)[NormLane<T, V>::NV][NormLane<T, V>::P], const NormLane<T, V>& me, const NormParams& p,
+                                            float* red) {
+  using L = NormLane<T, V>;
+  F2 s = f2(0.f);
+#pragma unroll
+  for (int n = 0; n < L::NV; ++n)
+#pragma unroll
+    for (int k = 0; k < L::P; ++k) s = f2add(s, d[n][k]);
+  const float mean = norm_sum<WIDE>(f2hsum(s), p.lanes, red) * p.inv_c;
+  F2 q = f2(0.f);
+#pragma unroll
+  for (int n = 0; n < L::NV; ++n)
+#pragma unroll
+    for (int k = 0; k < L::P; ++k) {
+      d[n][k] = me.at[n] < 0 ? f2(0.f) : f2(d[n][k].x - mean, V > 1 ? d[n][k].y - mean : 0.f);
+      q = f2fma(d[n][k], d[n][k], q);
+    }
+  return rsqrtf(norm_sum<WIDE>(f2hsum(q), p.lanes, red) * p.inv_c + p.eps);
+}
+
+template <typename T, int V, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_token_kernel(const NormParams p) {
+  using Ch = Chan<T, V>;
+  using L = NormLane<T, V>;
+  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE ? 1 : sizeof(T) == 2 ? 4 : 2;
+  __shared__ float red[32];
+  const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
+  const int g = gcol / p.lanes, l = gcol & (p.lanes - 1);
+  const bool live = row < p.rows && g < p.G;
+  L me;
+  me.set(p, g, l, live);
+  const T* x = static_cast<const T*>(p.x) + me.c0;
+  const T* gate = static_cast<const T*>(p.gate) + me.c0;
+  T* y = static_cast<T*>(p.y) + me.c0;
+  for (int64_t base = (int64_t)blockIdx.x * p.rows; base < p.tokens; base += (int64_t)gridDim.x * p.rows * AHEAD) {
+    Ch in[AHEAD][NV], gt[AHEAD][NV];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
+      const bool has = live && t < p.tokens;
+      const int64_t xo = has ? norm_row(p, t, p.xs) : 0, go = has && p.gate != nullptr ? norm_row(p, t, p.gates) : 0;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        in[u][n].zero();
+        gt[u][n].zero();
+        if (has && me.at[n] >= 0) {
+          in[u][n].load(x + xo + me.at[n]);
+          if (p.gate != nullptr) gt[u][n].load(gate + go + me.at[n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
+      if (base + (int64_t)u * gridDim.x * p.rows >= p.tokens) break;  // (the whole block)
+      F2 d[NV][P];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
+      const float r = norm_stats<T, V, WIDE>(d, me, p, red);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        F2 e[P];
+        gt[u][n].unpack(e);
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          const F2 v = f2fma(f2mul(d[n][k], f2(r)), me.w[n][k], me.b[n][k]);
+          if (p.gate != nullptr) d[n][k] = f2mul(v, f2(act_of(e[k].x, p.act), act_of(e[k].y, p.act)));
+          else d[n][k] = f2(act_of(v.x, p.act), act_of(v.y, p.act));
+        }
+        if (live && t < p.tokens && me.at[n] >= 0) {
+          Ch out;
+          out.pack(d[n]);
+          out.store(y + t * p.C + me.at[n]);
+        }
+      }
+    }
+  }
+}
+
+template <typename T, int V, bool WIDE>
+__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_token_bwd_kernel(const NormParams p) {
+  using Ch = Chan<T, V>;
+  using L = NormLane<T, V>;
+  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE ? 1 : sizeof(T) == 2 ? 2 : 1;
+  __shared__ float red[32];
+  const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
+  const int g = gcol / p.lanes, l = gcol & (p.lanes - 1);
+  const bool live = row < p.rows && g < p.G;
+  L me;
+  me.set(p, g, l, live);
+  const T* x = static_cast<const T*>(p.x) + me.c0;
+  const T* gate = static_cast<const T*>(p.gate) + me.c0;
+  const T* gy = static_cast<const T*>(p.gy) + me.c0;
+  T* gx = static_cast<T*>(p.gx) + me.c0;
+  T* ggate = static_cast<T*>(p.ggate) + me.c0;
+  F2 dw[NV][P], db[NV][P];
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int k = 0; k < P; ++k) dw[n][k] = db[n][k] = f2(0.f);
+  for (int64_t base = (int64_t)blockIdx.x * p.rows; base < p.tokens; base += (int64_t)gridDim.x * p.rows * AHEAD) {
+    Ch in[AHEAD][NV], gt[AHEAD][NV], gr[AHEAD][NV];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
+      const bool has = live && t < p.tokens;
+      const int64_t xo = has ? norm_row(p, t, p.xs) : 0, go = has && p.gate != nullptr ? norm_row(p, t, p.gates) : 0;
+      const int64_t yo = has ? norm_row(p, t, p.gys) : 0;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        in[u][n].zero();
+        gt[u][n].zero();
+        gr[u][n].zero();
+        if (has && me.at[n] >= 0) {
+          in[u][n].load(x + xo + me.at[n]);
+          gr[u][n].load(gy + yo + me.at[n]);
+          if (p.gate != nullptr) gt[u][n].load(gate + go + me.at[n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
+      if (base + (int64_t)u * gridDim.x * p.rows >= p.tokens) break;  // (the whole block)
+      const bool has = live && t < p.tokens;
+      F2 d[NV][P];
+#pragma unroll
+      for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
+      const float r = norm_stats<T, V, WIDE>(d, me, p, red);
+      F2 q[NV][P], s1 = f2(0.f), s2 = f2(0.f);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        F2 e[P], du[P], dg[P];
+        gr[u][n].unpack(du);
+        gt[u][n].unpack(e);
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          d[n][k] = f2mul(d[n][k], f2(r));  // n
+          const F2 v = f2fma(d[n][k], me.w[n][k], me.b[n][k]);
+          F2 a, slope;
+          if (p.gate != nullptr) {
+            a.x = act_and_slope(e[k].x, p.act, slope.x);
+            a.y = act_and_slope(e[k].y, p.act, slope.y);
+            dg[k] = f2mul(f2mul(du[k], v), slope);
+            du[k] = f2mul(du[k], a);
+          } else {
+            act_and_slope(v.x, p.act, slope.x);
+            act_and_slope(v.y, p.act, slope.y);
+            du[k] = f2mul(du[k], slope);
+          }
+          dw[n][k] = f2fma(du[k], d[n][k], dw[n][k]);
+          db[n][k] = f2add(db[n][k], du[k]);
+          q[n][k] = f2mul(du[k], me.w[n][k]);
+          s1 = f2add(s1, q[n][k]);
+          s2 = f2fma(q[n][k], d[n][k], s2);
+        }
+        if (p.gate != nullptr && has && me.at[n] >= 0) {
+          Ch out;
+          out.pack(dg);
+          out.store(ggate + t * p.C + me.at[n]);
+        }
+      }
+      const float m1 = norm_sum<WIDE>(f2hsum(s1), p.lanes, red) * p.inv_c, m2 = norm_sum<WIDE>(f2hsum(s2), p.lanes, red) * p.inv_c;
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) q[n][k] = f2mul(f2fma(d[n][k], f2(-m2), f2add(q[n][k], f2(-m1))), f2(r));
+        if (has && me.at[n] >= 0) {
+          Ch out;
+          out.pack(q[n]);
+          out.store(gx + t * p.C + me.at[n]);
+        }
+      }
+    }
+  }
+  if (p.partials == nullptr) return;
+  // this block's sums for the weights, over its rows in their order: [2][C]
+  extern __shared__ float norm_smem[];  // [2][rows][cols][8]; rows == 1: not used
+  float* out = p.partials + (int64_t)blockIdx.x * 2 * p.C;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+#pragma unroll
+    for (int k = 0; k < P; ++k)
+#pragma unroll
+      for (int h = 0; h < (V > 1 ? 2 : 1); ++h) {
+        const float a = h ? dw[n][k].y : dw[n][k].x, b = h ? db[n][k].y : db[n][k].x;
+        const int e = n * V + 2 * k + h;
+        if (p.rows > 1) {
+          if (row < p.rows) {
+            norm_smem[(row * p.cols + col) * NORM_EACH + e] = a;
+            norm_smem[((p.rows + row) * p.cols + col) * NORM_EACH + e] = b;
+          }
+        } else if (me.at[n] >= 0) {
+          out[me.c0 + me.at[n] + 2 * k + h] = a;
+          out[p.C + me.c0 + me.at[n] + 2 * k + h] = b;
+        }
+      }
+  if (p.rows == 1) return;
+  __syncthreads();
+  if (row != 0 || !live) return;
+#pragma unroll
+  for (int n = 0; n < NV; ++n)
+    if (me.at[n] >= 0)
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          float v = 0.f;
+          for (int q = 0; q < p.rows; ++q) v += norm_smem[((m * p.rows + q) * p.cols + col) * NORM_EACH + n * V + e];
+          out[m * p.C + me.c0 + me.at[n] + e] = v;
+        }
+}
+
+// rows of partial sums [rows][2][C] -> weight's and bias's gradients, in a fixed order
+template <typename T>
+__global__ void __launch_bounds__(256) ttt_norm_reduce_kernel(const float* partials, int rows, int C, T* gw, T* gb) {
+  __shared__ float part[8][33];
+  const int col = (int)blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
+  float v = 0.f;
+  if (col < 2 * C)
+    for (int r = share; r < rows; r += 8) v += partials[(int64_t)r * 2 * C + col];
+  part[share][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (share != 0 || col >= 2 * C) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x & 31];
+  if (col < C) {
+    if (gw != nullptr) st_from_float<T>(gw, col, v);
+  } else if (gb != nullptr) {
+    st_from_float<T>(gb, col - C, v);
+  }
+}
+
+// ---- whole sequences -----------------------------------------------------------------------------------------------
+// Numbers seen so far: how many, their mean, the sum of squares of differences from it.  Joined as by Chan, Golub and LeVeque
+// (1979), which does not cancel.
+struct Moments {
+  float n, mean, m2;
+  __device__ __forceinline__ void join(float bn, float bmean, float bm2) {
+    const float all = n + bn;
+    if (!(bn > 0.f)) return;
+    const float d = bmean - mean, f = bn / all;
+    mean = fmaf(d, f, mean);
+    m2 += bm2 + d * d * n * f;
+    n = all;
+  }
+  __device__ __forceinline__ void join_warp() {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float bn = __shfl_xor_sync(0xffffffffu, n, o), bm = __shfl_xor_sync(0xffffffffu, mean, o), b2 = __shfl_xor_sync(0xffffffffu, m2, o);
+      // (both lanes join in the same order, so that both have the same)
+      Moments lo = (threadIdx.x & o) ? Moments{bn, bm, b2} : *this, hi = (threadIdx.x & o) ? *this : Moments{bn, bm, b2};
+      if (lo.n > 0.f) lo.join(hi.n, hi.mean, hi.m2);
+      else lo = hi;
+      *this = lo;
+    }
+  }
+};
+
+// Where a block of the sequence kernels stands.  blockIdx.x: row of the batch and chunk of tokens; blockIdx.y: groups, or a part of
+// a group's channels.
+struct SeqPlace {
+  int64_t b, t_lo, t_hi;
+  int chunk, g0, groups, span;  // groups [g0, g0 + groups) or part `span` of group g0
+  int row, c;                   // this thread's row and first channel, c < 0: none
+  __device__ __forceinline__ SeqPlace(const NormParams& p, int V) {
+    b = blockIdx.x / p.chunks;
+    chunk = (int)(blockIdx.x - b * p.chunks);
+    t_lo = (int64_t)chunk * p.chunk;
+    t_hi = min(t_lo + p.chunk, p.T);
+    row = threadIdx.x / p.cols;
+    const int col = threadIdx.x - row * p.cols, vectors = p.c / V;
+    if (p.spans == 1) {
+      g0 = (int)blockIdx.y * p.per_block;
+      groups = min(p.per_block, p.G - g0);
+      span = 0;
+      c = row < p.rows && col < groups * vectors ? g0 * p.c + col * V : -1;
+    } else {
+      g0 = (int)blockIdx.y / p.spans;
+      groups = 1;
+      span = (int)blockIdx.y - g0 * p.spans;
+      const int v = span * p.cols + col;
+      c = row < p.rows && v < vectors ? g0 * p.c + v * V : -1;
+    }
+  }
+};
+
+template <typename T, int V>
+__global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_stats_kernel(const NormParams p) {
+  using Ch = Chan<T, V>;
+  constexpr int P = Ch::P, AHEAD = 4;
+  __shared__ float sm[3][NORM_THREADS];
+  const SeqPlace at(p, V);
+  Moments me{0.f, 0.f, 0.f};
+  if (at.c >= 0) {
+    const T* x = static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c;
+    for (int64_t t = at.t_lo + at.row; t < at.t_hi; t += (int64_t)AHEAD * p.rows) {
+      Ch in[AHEAD];
+      int have = 0;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        in[u].zero();
+        if (t + (int64_t)u * p.rows < at.t_hi) in[u].load(x + (t + (int64_t)u * p.rows) * p.xs[1]), ++have;
+      }
+      F2 v[AHEAD][P], s = f2(0.f), q = f2(0.f);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        in[u].unpack(v[u]);
+#pragma unroll
+        for (int k = 0; k < P; ++k) s = f2add(s, v[u][k]);
+      }
+      const float n = (float)(have * V), mean = f2hsum(s) / n;
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (u < have)
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            const F2 d = f2(v[u][k].x - mean, V > 1 ? v[u][k].y - mean : 0.f);
+            q = f2fma(d, d, q);
+          }
+      if (me.n > 0.f) me.join(n, mean, f2hsum(q));
+      else me = Moments{n, mean, f2hsum(q)};
+    }
+  }
+  sm[0][threadIdx.x] = me.n, sm[1][threadIdx.x] = me.mean, sm[2][threadIdx.x] = me.m2;
+  __syncthreads();
+  // a warp per group, lanes over its columns and rows
+  const int lane = threadIdx.x & 31, per_group = p.spans == 1 ? p.c / V : p.cols, entries = per_group * p.rows;
+  for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
+    Moments m{0.f, 0.f, 0.f};
+    for (int e = lane; e < entries; e += 32) {
+      const int r = e / per_group, i = r * p.cols + k * per_group + (e - r * per_group);
+      if (m.n > 0.f) m.join(sm[0][i], sm[1][i], sm[2][i]);
+      else m = Moments{sm[0][i], sm[1][i], sm[2][i]};
+    }
+    m.join_warp();
+    if (lane == 0) {
+      float* out = p.moments + (((at.b * p.G + at.g0 + k) * p.chunks + at.chunk) * p.spans + at.span) * 3;
+      out[0] = m.n, out[1] = m.mean, out[2] = m.m2;
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_apply_kernel(const NormParams p) {
+  using Ch = Chan<T, V>;
+  constexpr int P = Ch::P, AHEAD = 4;
+  __shared__ float stat[NORM_THREADS][2];
+  const SeqPlace at(p, V);
+  const int lane = threadIdx.x & 31;
+  for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
+    const float* m = p.moments + (at.b * p.G + at.g0 + k) * p.chunks * p.spans * 3;
+    Moments all{0.f, 0.f, 0.f};
+    for (int e = lane; e < p.chunks * p.spans; e += 32) {
+      if (all.n > 0.f) all.join(m[3 * e], m[3 * e + 1], m[3 * e + 2]);
+      else all = Moments{m[3 * e], m[3 * e + 1], m[3 * e + 2]};
+    }
+    all.join_warp();
+    if (lane == 0) {
+      stat[k][0] = all.mean;
+      stat[k][1] = rsqrtf(all.m2 / all.n + p.eps);
+      if (p.stats != nullptr && at.chunk == 0 && at.span == 0) {
+        p.stats[(at.b * p.G + at.g0 + k) * 2] = stat[k][0];
+        p.stats[(at.b * p.G + at.g0 + k) * 2 + 1] = stat[k][1];
+      }
+    }
+  }
+  __syncthreads();
+  if (at.c < 0) return;
+  const int k0 = at.c / p.c - at.g0;
+  const float mean = stat[k0][0], r = stat[k0][1];
+  F2 w[P], b[P];
+#pragma unroll
+  for (int k = 0; k < P; ++k) w[k] = f2(1.f), b[k] = f2(0.f);
+  Ch raw;
+  if (p.w != nullptr) raw.load(static_cast<const T*>(p.w) + at.c), raw.unpack(w);
+  if (p.bias != nullptr) raw.load(static_cast<const T*>(p.bias) + at.c), raw.unpack(b);
+  const T* x = static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c;
+  const T* gate = static_cast<const T*>(p.gate) + at.b * p.gates[0] + at.c;
+  T* y = static_cast<T*>(p.y) + at.b * p.T * p.C + at.c;
+  for (int64_t t = at.t_lo + at.row; t < at.t_hi; t += (int64_t)AHEAD * p.rows) {
+    Ch in[AHEAD], gt[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      gt[u].zero();
+      if (t + (int64_t)u * p.rows < at.t_hi) {
+        in[u].load(x + (t + (int64_t)u * p.rows) * p.xs[1]);
+        if (p.gate != nullptr) gt[u].load(gate + (t + (int64_t)u * p.rows) * p.gates[1]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      if (t + (int64_t)u * p.rows >= at.t_hi) break;
+      F2 v[P], e[P];
+      in[u].unpack(v);
+      gt[u].unpack(e);
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        v[k] = f2fma(f2mul(f2add(v[k], f2(-mean)), f2(r)), w[k], b[k]);
+        if (p.gate != nullptr) v[k] = f2mul(v[k], f2(act_of(e[k].x, p.act), act_of(e[k].y, p.act)));
+        else v[k] = f2(act_of(v[k].x, p.act), act_of(v[k].y, p.act));
+      }
+      Ch out;
+      out.pack(v);
+      out.store(y + (t + (int64_t)u * p.rows) * p.C);
+    }
+  }
+}
+
+// du and n of a thread's channels of one token, and the gate's gradient
+template <int P>
+__device__ __forceinline__ void norm_du(const NormParams& p, F2 (&n)[P], F2 (&du)[P], const F2 (&e)[P], F2 (&dg)[P], float mean, float r,
+                                        const F2 (&w)[P], const F2 (&b)[P]) {
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    n[k] = f2mul(f2add(n[k], f2(-mean)), f2(r));
+    const F2 v = f2fma(n[k], w[k], b[k]);
+    F2 a, slope;
+    if (p.gate != nullptr) {
+      a.x = act_and_slope(e[k].x, p.act, slope.x);
+      a.y = act_and_slope(e[k].y, p.act, slope.y);
+      dg[k] = f2mul(f2mul(du[k], v), slope);
+      du[k] = f2mul(du[k], a);
+    } else {
+      act_and_slope(v.x, p.act, slope.x);
+      act_and_slope(v.y, p.act, slope.y);
+      du[k] = f2mul(du[k], slope);
+    }
+  }
+}
+
+// APPLY false: every channel's sums of du and du n over the chunk.  true: the gradients of x and the gate.
+template <typename T, int V, bool APPLY>
+__global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_bwd_kernel(const NormParams p) {
+  using Ch = Chan<T, V>;
+  constexpr int P = Ch::P, AHEAD = 2;
+  __shared__ float mean_of[NORM_THREADS][2];
+  extern __shared__ float norm_smem[];  // APPLY false: [2][rows][cols][V]
+  const SeqPlace at(p, V);
+  if constexpr (APPLY) {  // the groups' means of p and p n, from the channels' sums
+    const int lane = threadIdx.x & 31;
+    const float inv = 1.f / ((float)p.c * (float)p.T);
+    for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
+      const int c0 = (at.g0 + k) * p.c;
+      const float* s = p.sums + at.b * 2 * p.C + c0;
+      float m1 = 0.f, m2 = 0.f;
+      for (int c = lane; c < p.c; c += 32) {
+        const float w = p.w != nullptr ? ld_as_float<T>(p.w, c0 + c) : 1.f;
+        m1 = fmaf(w, s[c], m1);
+        m2 = fmaf(w, s[p.C + c], m2);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        m1 += __shfl_xor_sync(0xffffffffu, m1, o);
+        m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+      }
+      if (lane == 0) mean_of[k][0] = m1 * inv, mean_of[k][1] = m2 * inv;
+    }
+    __syncthreads();
+  }
+  F2 s1[P], s2[P];
+#pragma unroll
+  for (int k = 0; k < P; ++k) s1[k] = s2[k] = f2(0.f);
+  if (at.c >= 0) {
+    const int g = at.c / p.c;
+    const float mean = p.stats[(at.b * p.G + g) * 2], r = p.stats[(at.b * p.G + g) * 2 + 1];
+    const float m1 = APPLY ? mean_of[g - at.g0][0] : 0.f, m2 = APPLY ? mean_of[g - at.g0][1] : 0.f;
+    F2 w[P], b[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) w[k] = f2(1.f), b[k] = f2(0.f);
+    Ch raw;
+    if (p.w != nullptr) raw.load(static_cast<const T*>(p.w) + at.c), raw.unpack(w);
+    if (p.bias != nullptr) raw.load(static_cast<const T*>(p.bias) + at.c), raw.unpack(b);
+    const T* x = static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c;
+    const T* gate = static_cast<const T*>(p.gate) + at.b * p.gates[0] + at.c;
+    const T* gy = static_cast<const T*>(p.gy) + at.b * p.gys[0] + at.c;
+    T* gx = static_cast<T*>(p.gx) + at.b * p.T * p.C + at.c;
+    T* ggate = static_cast<T*>(p.ggate) + at.b * p.T * p.C + at.c;
+    for (int64_t t = at.t_lo + at.row; t < at.t_hi; t += (int64_t)AHEAD * p.rows) {
+      Ch in[AHEAD], gt[AHEAD], gr[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t tu = t + (int64_t)u * p.rows;
+        gt[u].zero();
+        if (tu < at.t_hi) {
+          in[u].load(x + tu * p.xs[1]);
+          gr[u].load(gy + tu * p.gys[1]);
+          if (p.gate != nullptr) gt[u].load(gate + tu * p.gates[1]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int64_t tu = t + (int64_t)u * p.rows;
+        if (tu >= at.t_hi) break;
+        F2 n[P], du[P], e[P], dg[P];
+        in[u].unpack(n);
+        gr[u].unpack(du);
+        gt[u].unpack(e);
+        norm_du<P>(p, n, du, e, dg, mean, r, w, b);
+        if constexpr (APPLY) {
+          Ch out;
+#pragma unroll
+          for (int k = 0; k < P; ++k) du[k] = f2mul(f2fma(n[k], f2(-m2), f2fma(du[k], w[k], f2(-m1))), f2(r));
+          out.pack(du);
+          out.store(gx + tu * p.C);
+          if (p.gate != nullptr) {
+            out.pack(dg);
+            out.store(ggate + tu * p.C);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            s1[k] = f2add(s1[k], du[k]);
+            s2[k] = f2fma(du[k], n[k], s2[k]);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (!APPLY) {
+    const int width = p.cols * V, col = threadIdx.x - at.row * p.cols;
+    if (at.row < p.rows)
+#pragma unroll
+      for (int k = 0; k < P; ++k)
+#pragma unroll
+        for (int h = 0; h < (V > 1 ? 2 : 1); ++h) {
+          norm_smem[at.row * width + col * V + 2 * k + h] = h ? s1[k].y : s1[k].x;
+          norm_smem[(p.rows + at.row) * width + col * V + 2 * k + h] = h ? s2[k].y : s2[k].x;
+        }
+    __syncthreads();
+    // [2][C] per chunk: du n first, as the weight's gradient stands before the bias's
+    float* out = p.partials + (int64_t)blockIdx.x * 2 * p.C;
+    const int first = p.spans == 1 ? at.g0 * p.c : at.g0 * p.c + at.span * width;
+    const int have = p.spans == 1 ? at.groups * p.c : min(width, p.c - at.span * width);
+    for (int e = threadIdx.x; e < 2 * have; e += NORM_THREADS) {
+      const int m = e / have, c = e - m * have;
+      float v = 0.f;
+      for (int q = 0; q < p.rows; ++q) v += norm_smem[(m * p.rows + q) * width + c];
+      out[(1 - m) * p.C + first + c] = v;
+    }
+  }
+}
+
+// the chunks' sums [B][chunks][2][C] (du n, du) -> [B][2][C] (du, du n)
+__global__ void __launch_bounds__(256) ttt_norm_seq_sums_kernel(const float* partials, float* sums, int chunks, int C, int column_blocks) {
+  __shared__ float part[8][33];
+  const int64_t b = blockIdx.x / column_blocks;
+  const int col = (int)(blockIdx.x - b * column_blocks) * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
+  float v = 0.f;
+  if (col < 2 * C)
+    for (int r = share; r < chunks; r += 8) v += partials[(b * chunks + r) * 2 * C + col];
+  part[share][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (share != 0 || col >= 2 * C) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x & 31];
+  sums[b * 2 * C + (col < C ? C + col : col - C)] = v;
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------------
+struct NormCut {
+  int lanes, cols, rows, y, threads;      // a token's groups
+  int per_block, spans, chunks;           // sequences
+  int64_t chunk, x;
+};
+static NormCut norm_token_cut(int64_t tokens, int G, int c, bool bwd) {
+  NormCut k{};
+  k.lanes = 1;
+  while (k.lanes * NORM_EACH < c) k.lanes *= 2;
+  const int64_t total = (int64_t)G * k.lanes;
+  const int64_t blocks = (total + NORM_THREADS - 1) / NORM_THREADS;
+  const int64_t share = (total + blocks - 1) / blocks;
+  k.cols = (int)((share + k.lanes - 1) / k.lanes) * k.lanes;
+  k.rows = k.cols < NORM_THREADS ? NORM_THREADS / k.cols : 1;
+  k.threads = (k.cols * k.rows + 31) / 32 * 32;
+  k.y = (int)((total + k.cols - 1) / k.cols);
+  const int64_t need = (tokens + k.rows - 1) / k.rows, wanted = 148 * (bwd ? 3 : 6) / k.y, most = wanted > 1 ? wanted : 1;
+  k.x = need < most ? need : most;
+  return k;
+}
+static NormCut norm_seq_cut(int64_t B, int64_t T, int G, int c, int V) {
+  NormCut k{};
+  const int vectors = c / V;
+  if (vectors <= NORM_THREADS) {
+    const int fit = NORM_THREADS / vectors, blocks = (G + fit - 1) / fit;
+    k.spans = 1;
+    k.per_block = (G + blocks - 1) / blocks;
+    k.cols = k.per_block * vectors;
+    k.rows = NORM_THREADS / k.cols;
+    k.y = blocks;
+  } else {
+    k.spans = (vectors + NORM_THREADS - 1) / NORM_THREADS;
+    k.per_block = 1;
+    k.cols = NORM_THREADS;
+    k.rows = 1;
+    k.y = G * k.spans;
+  }
+  int64_t chunks = (148 * 4 + B * k.y - 1) / (B * k.y);
+  const int64_t most = (T + 4 * k.rows - 1) / (4 * k.rows);  // (four tokens per thread at least)
+  if (chunks > most) chunks = most;
+  k.chunk = (T + chunks - 1) / chunks;
+  k.chunks = (int)((T + k.chunk - 1) / k.chunk);
+  k.x = B * k.chunks;
+  return k;
+}
+static int norm_widths(int es, int c, int (&v)[3]) {  // the vector widths that a group of c channels allows; which runs depends on addresses
+  int n = 0;
+  for (int V : {16 / es, 2, 1})
+    if (c % V == 0) v[n++] = V;
+  return n;
+}
+size_t norm_forward_floats(int64_t B, int64_t T, int C, int G, bool sequence, int es) {
+  if (!sequence) return 0;
+  size_t most = 0;
+  int v[3];
+  for (int i = norm_widths(es, C / G, v); i-- > 0;) {
+    const NormCut k = norm_seq_cut(B, T, G, C / G, v[i]);
+    const size_t n = (size_t)B * G * k.chunks * k.spans * 3;
+    if (n > most) most = n;
+  }
+  return most;
+}
+size_t norm_backward_floats(int64_t B, int64_t T, int C, int G, bool sequence, int es) {
+  if (!sequence) return (size_t)norm_token_cut(B * T, G, C / G, true).x * 2 * C;
+  size_t most = 0;
+  int v[3];
+  for (int i = norm_widths(es, C / G, v); i-- > 0;) {
+    const NormCut k = norm_seq_cut(B, T, G, C / G, v[i]);
+    const size_t n = (size_t)B * (k.chunks + 1) * 2 * C;
+    if (n > most) most = n;
+  }
+  return most;
+}
+
+template <typename T>
+static cudaError_t reduce(const NormParams& p, int64_t rows, cudaStream_t st) {
+  ttt_norm_reduce_kernel<T><<<(2 * p.C + 31) / 32, 256, 0, st>>>(p.partials, (int)rows, p.C, static_cast<T*>(p.gw), static_cast<T*>(p.gb));
+  return cudaGetLastError();
+}
+template <typename T, int V>
+static cudaError_t launch_token(NormParams p, bool bwd, cudaStream_t st) {
+  const NormCut k = norm_token_cut(p.tokens, p.G, p.c, bwd);
+  p.lanes = k.lanes, p.cols = k.cols, p.rows = k.rows;
+  const dim3 grid((unsigned)k.x, k.y);
+  const bool wide = k.lanes > 32;
+  if (!bwd) {
+    if (wide) ttt_norm_token_kernel<T, V, true><<<grid, k.threads, 0, st>>>(p);
+    else ttt_norm_token_kernel<T, V, false><<<grid, k.threads, 0, st>>>(p);
+    return cudaGetLastError();
+  }
+  const size_t smem = k.rows > 1 ? sizeof(float) * 2 * k.rows * k.cols * NORM_EACH : 0;
+  if (wide) ttt_norm_token_bwd_kernel<T, V, true><<<grid, k.threads, smem, st>>>(p);
+  else ttt_norm_token_bwd_kernel<T, V, false><<<grid, k.threads, smem, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e != cudaSuccess || p.partials == nullptr ? e : reduce<T>(p, k.x, st);
+}
+template <typename T, int V>
+static cudaError_t launch_seq(NormParams p, bool bwd, cudaStream_t st) {
+  const NormCut k = norm_seq_cut(p.B, p.T, p.G, p.c, V);
+  p.cols = k.cols, p.rows = k.rows, p.per_block = k.per_block, p.spans = k.spans, p.chunks = k.chunks, p.chunk = k.chunk;
+  const dim3 grid((unsigned)k.x, k.y);
+  cudaError_t e;
+  if (!bwd) {
+    ttt_norm_seq_stats_kernel<T, V><<<grid, NORM_THREADS, 0, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    ttt_norm_seq_apply_kernel<T, V><<<grid, NORM_THREADS, 0, st>>>(p);
+    return cudaGetLastError();
+  }
+  p.sums = p.partials + (size_t)k.x * 2 * p.C;
+  ttt_norm_seq_bwd_kernel<T, V, false><<<grid, NORM_THREADS, sizeof(float) * 2 * k.rows * k.cols * V, st>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  const int column_blocks = (2 * p.C + 31) / 32;
+  ttt_norm_seq_sums_kernel<<<(unsigned)(p.B * column_blocks), 256, 0, st>>>(p.partials, p.sums, k.chunks, p.C, column_blocks);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  ttt_norm_seq_bwd_kernel<T, V, true><<<grid, NORM_THREADS, 0, st>>>(p);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  return p.gw == nullptr && p.gb == nullptr ? cudaSuccess : reduce<T>(p, k.x, st);
+}
+template <typename T, int V>
+static cudaError_t launch_v(const NormParams& p, bool sequence, bool bwd, cudaStream_t st) {
+  return sequence ? launch_seq<T, V>(p, bwd, st) : launch_token<T, V>(p, bwd, st);
+}
+// V: the widest vector that the group's channels and all addresses allow (16 bytes, 2 channels or 1)
+cudaError_t launch_norm(int dtype, const NormParams& p, int V, bool sequence, bool bwd, cudaStream_t st) {
+  if (dtype == 1)
+    return V == 8 ? launch_v<__nv_bfloat16, 8>(p, sequence, bwd, st) : V == 2 ? launch_v<__nv_bfloat16, 2>(p, sequence, bwd, st)
+                                                                              : launch_v<__nv_bfloat16, 1>(p, sequence, bwd, st);
+  return V == 4 ? launch_v<float, 4>(p, sequence, bwd, st) : V == 2 ? launch_v<float, 2>(p, sequence, bwd, st) : launch_v<float, 1>(p, sequence, bwd, st);
+}
+
+}  // namespace ttt

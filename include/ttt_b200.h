@@ -461,6 +461,47 @@ int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int64_t channe
                                   void* grad_x, void* grad_gate, void* grad_weight, void* grad_bias, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* ---- selective state space scan ---------------------------------------------------------------------------------------
+ * N = states per channel that decay at rates of their own, by steps that the token chooses (no counterpart in the reference):
+ *     d_t = softplus(dt_t + dt_bias)  (softplus 0: dt_t + dt_bias),   h_t = exp(d_t a) h_{t-1} + d_t x_t b_t,
+ *     y_t = (<c_t, h_t> + d_skip x_t), times SiLU(z_t)
+ *   x, dt, z      T [batch, seq_len, channels] with contiguous channels; z or null (no gate)
+ *   b, c          T [batch, seq_len, groups, states] with contiguous states, shared by channels / groups neighbouring channels
+ *   strides       of x, dt, z (backward: and grad_y) those of batch and token, then of b and c those of batch, token and group, in
+ *                 elements, not negative (null: all contiguous; not read where there is one row, or no z)
+ *   a             float32 [channels, states], at most 0 for states that do not grow; d_skip, dt_bias float32 [channels] or null (zeros)
+ *   state         float32 [batch, channels, states] before the first token, or null: zeros
+ *   starts        uint8 [batch, seq_len] or null: nonzero: the token finds a state of zero
+ *   y             T [batch, seq_len, channels] (out);  state_out  float32 like state (out; it may be state).  Results lie over no other
+ *                 tensor of the call.
+ *   saved         (out) ttt_linear_selective_saved_bytes bytes for the backward: the states before every 16 tokens, opaque; null for
+ *                 inference (1 to 16 tokens then are a decode step: one launch, no workspace)
+ *   workspace     ..._forward_workspace_bytes / ..._backward_workspace_bytes, 16-byte aligned; the forward's may be 0 (null then)
+ * states 1..64; batch*seq_len, batch*channels < 2^31.  a, state, state_out and their gradients on 16 bytes; all others at any multiple
+ * of an element.  Steps, decays, states and sums are float32; no result depends on the order in which blocks run.
+ *
+ * ttt_linear_selective_backward: gradients for loss = <grad_y, y> + <grad_state_out, state_out> (grad_state_out null: zero).  grad_x,
+ * grad_dt, grad_z (exactly with z) T, contiguous; grad_b, grad_c T [batch, seq_len, groups, states]; grad_a, grad_d, grad_dt_bias,
+ * grad_state float32, the last three or null.
+ */
+size_t ttt_linear_selective_saved_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype);
+size_t ttt_linear_selective_forward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,
+                                                    int dtype);
+int ttt_linear_selective_forward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype,
+                                 int softplus, const void* x, const void* dt, const float* a, const void* b, const void* c,
+                                 const float* d_skip, const void* z, const float* dt_bias, const float* state,
+                                 const void* starts, const int64_t* strides, void* y, float* state_out, void* saved,
+                                 size_t saved_bytes, void* workspace, size_t workspace_bytes, void* stream);
+size_t ttt_linear_selective_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,
+                                                     int dtype);
+int ttt_linear_selective_backward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype,
+                                  int softplus, const void* x, const void* dt, const float* a, const void* b, const void* c,
+                                  const float* d_skip, const void* z, const float* dt_bias, const void* starts,
+                                  const void* grad_y, const int64_t* strides, const void* saved, size_t saved_bytes,
+                                  const float* grad_state_out, void* grad_x, void* grad_dt, float* grad_a, void* grad_b,
+                                  void* grad_c, float* grad_d, void* grad_z, float* grad_dt_bias, float* grad_state,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+
 /* Backward without a caller workspace.  (No counterpart in the reference: its host wrapper always allocates its
  * scratch itself, backward/launch.rs:389-392.)
  *

@@ -81,9 +81,59 @@ def test_norm_refuses(lib):
     assert back(bytes_=8) == back(ws=None) == back(over=1, bytes_=8, grad_weight=None, grad_bias=None) == _lib.TTT_ERR_WORKSPACE
 
 
+def test_scan_refuses(lib):
+    def scan(B=2, T=40, Ch=32, G=2, N=16, dtype=1, strides=None, ws=None, bytes_=0, saved=None, saved_bytes=0, **p):
+        names = ("x", "dt", "a", "b", "c", "d", "z", "dt_bias", "state", "starts")
+        d = {n: 0x100000 * (i + 1) for i, n in enumerate(names)} | {"starts": None, "y": 0x2000000, "state_out": 0x3000000} | p
+        return lib.ttt_linear_selective_forward(B, T, Ch, G, N, dtype, 1, *[d[n] for n in names], strides, d["y"], d["state_out"], saved, saved_bytes,
+                                                ws, bytes_, None)
+    assert scan(G=5) == scan(G=0) == scan(T=0) == scan(B=0) == scan(B=1 << 11, Ch=1 << 20, G=1) == _lib.TTT_ERR_SHAPE
+    assert scan(N=0) == scan(N=65) == scan(dtype=3) == _lib.TTT_ERR_UNSUPPORTED
+    for n in ("x", "dt", "a", "b", "c", "y", "state_out"):
+        assert scan(**{n: None}) == _lib.TTT_ERR_NULL and n in _lib.last_error()
+    for n in ("x", "dt", "z", "b", "c", "y", "d", "dt_bias"):
+        assert scan(**{n: 0x4000001}) == _lib.TTT_ERR_ALIGN and n in _lib.last_error()
+    for n in ("a", "state", "state_out"):
+        assert scan(**{n: 0x4000008}) == _lib.TTT_ERR_ALIGN and n in _lib.last_error()
+    dense = [40 * 32, 32] * 3 + [40 * 32, 32, 16] * 2
+    for i, bad in ((0, -1), (3, 1 << 60), (8, -16)):
+        s = list(dense)
+        s[i] = bad
+        assert scan(strides=int64s(*s)) == _lib.TTT_ERR_SHAPE
+    assert scan(saved=FAKE, saved_bytes=8) == _lib.TTT_ERR_WORKSPACE
+    need = lib.ttt_linear_selective_forward_workspace_bytes(2, 40, 32, 2, 16, 1)
+    if need:
+        assert scan(ws=FAKE, bytes_=need - 1) == _lib.TTT_ERR_WORKSPACE and scan(ws=at(0x100008), bytes_=need) == _lib.TTT_ERR_ALIGN
+    # results over other tensors of the call
+    for n in (dict(state_out=0x900010), dict(state_out=0x100000), dict(state_out=0x300000), dict(state_out=0x2000000), dict(y=0x100000),
+              dict(y=0x900000), dict(y=0x400000)):
+        assert scan(**n) == _lib.TTT_ERR_SHAPE and "lies over" in _lib.last_error(), n
+
+
+def test_scan_backward_refuses(lib):
+    shape = (2, 40, 32, 2, 16, 1)
+    saved, need = lib.ttt_linear_selective_saved_bytes(*shape), lib.ttt_linear_selective_backward_workspace_bytes(*shape)
+    assert saved == 2 * 3 * 32 * 16 * 4 and need > 0
+    assert lib.ttt_linear_selective_saved_bytes(2, 40, 32, 5, 16, 1) == lib.ttt_linear_selective_backward_workspace_bytes(2, 40, 32, 2, 65, 1) == 0
+
+    def back(ws=FAKE, bytes_=need, saved_bytes=saved, **p):
+        first = ("x", "dt", "a", "b", "c", "d", "z", "dt_bias", "starts", "grad_y")
+        last = ("grad_state_out", "grad_x", "grad_dt", "grad_a", "grad_b", "grad_c", "grad_d", "grad_z", "grad_dt_bias", "grad_state")
+        d = {**{n: FAKE for n in first + last}, "saved": FAKE, **p}
+        return lib.ttt_linear_selective_backward(*shape, 1, *[d[n] for n in first], None, d["saved"], saved_bytes, *[d[n] for n in last], ws, bytes_,
+                                                 None)
+    assert back(bytes_=need - 1) == back(ws=None) == back(saved_bytes=16) == _lib.TTT_ERR_WORKSPACE
+    for n in ("grad_y", "grad_x", "grad_dt", "grad_z", "grad_a", "grad_b", "grad_c", "saved"):
+        assert back(**{n: None}) == _lib.TTT_ERR_NULL and n in _lib.last_error()
+    for n in ("grad_a", "grad_state", "grad_state_out"):
+        assert back(**{n: at(0x100008)}) == _lib.TTT_ERR_ALIGN and n in _lib.last_error()
+    assert back(ws=at(0x100004)) == back(grad_b=at(0x100001)) == back(grad_d=at(0x100002)) == _lib.TTT_ERR_ALIGN
+
+
 def test_host_refuses_cpu_tensors():
     x = torch.zeros(1, 4, 16)
-    for f in (lambda: tb.causal_conv(x, torch.zeros(16, 4)), lambda: tb.group_norm(x, 4)):
+    b = torch.zeros(1, 4, 8)
+    for f in (lambda: tb.causal_conv(x, torch.zeros(16, 4)), lambda: tb.group_norm(x, 4), lambda: tb.selective_scan(x, x, torch.zeros(16, 8), b, b)):
         with pytest.raises(tb.TttError):
             f()
 
@@ -95,3 +145,6 @@ def test_oracle_gradients_against_differences():
     assert torch.autograd.gradcheck(lambda *t: O.causal_conv(*t, activation="silu", starts=marks), [r(2, 5, 3), r(3, 4), r(3), r(2, 3, 3)])
     assert torch.autograd.gradcheck(lambda *t: O.group_norm(t[0], 2, t[1], t[2], gate=t[3], activation="silu"), [r(2, 3, 6), r(6), r(6), r(2, 3, 6)])
     assert torch.autograd.gradcheck(lambda *t: O.group_norm(t[0], 2, t[1], t[2], activation="gelu", over="sequence"), [r(2, 3, 6), r(6), r(6)])
+    assert torch.autograd.gradcheck(
+        lambda x, dt, A, B, C, D, z, bias, h: O.selective_scan(x, dt, A, B, C, D, z, bias, h, starts=marks),
+        [r(2, 5, 4), r(2, 5, 4), r(4, 3), r(2, 5, 2, 3), r(2, 5, 2, 3), r(4), r(2, 5, 4), r(4), r(2, 4, 3)])

@@ -29,4 +29,4 @@ from .fused import (  # noqa: F401
 from .layer import TTT, DecodeGraphs, TTTLayerConfig, gemm_bf16_tn, layer_epilogue, layer_projections, layer_prologue, layer_values, new_gated_inner, new_inner  # noqa: F401,E402
 from .gated import FusedGatedLinear, GatedLinear, GatedLinearState, fused_gated_linear  # noqa: F401,E402
 from .rope import Rotary, RotaryConfig, qk_norm_rotary, rotary  # noqa: F401,E402
-from .mixer import causal_conv, group_norm  # noqa: F401,E402
+from .mixer import causal_conv, group_norm, selective_scan  # noqa: F401,E402

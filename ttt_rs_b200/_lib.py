@@ -100,6 +100,11 @@ SYMBOLS = {
     "ttt_layer_causal_conv": (C.c_int, [_L] * 3 + [C.c_int] * 3 + [_P] * 9),
     "ttt_layer_causal_conv_backward_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 2),
     "ttt_layer_causal_conv_backward": (C.c_int, [_L] * 3 + [C.c_int] * 3 + [_P] * 13 + [C.c_size_t, _P]),
+    "ttt_linear_selective_saved_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),
+    "ttt_linear_selective_forward_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),
+    "ttt_linear_selective_forward": (C.c_int, [_L] * 3 + [C.c_int] * 4 + [_P] * 14 + [C.c_size_t, _P, C.c_size_t, _P]),
+    "ttt_linear_selective_backward_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),
+    "ttt_linear_selective_backward": (C.c_int, [_L] * 3 + [C.c_int] * 4 + [_P] * 12 + [C.c_size_t] + [_P] * 11 + [C.c_size_t, _P]),
     "ttt_layer_group_norm_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),
     "ttt_layer_group_norm": (C.c_int, [_L] * 3 + [C.c_int] * 4 + [C.c_float] + [_P] * 8 + [C.c_size_t, _P]),
     "ttt_layer_group_norm_backward_workspace_bytes": (C.c_size_t, [_L] * 3 + [C.c_int] * 3),

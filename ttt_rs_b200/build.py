@@ -20,7 +20,7 @@ PROBE_SRC = CSRC / "probe_chain_latency.cu"      # stand-alone measurement progr
 PROBE_BIN = PKG / "build" / "probe_chain_latency"
 SOURCES = ["ttt_abi.cu", "ttt_linear_fwd.cu", "ttt_linear_fwd_roles.cu", "ttt_linear_bwd.cu", "ttt_linear_bwd_f32.cu", "ttt_mlp_fwd.cu", "ttt_layer.cu", "ttt_layer_small.cu", "ttt_linear_partial.cu", "ttt_mlp_bwd.cu", "ttt_gemm.cu",
            "ttt_gated_fwd.cu", "ttt_gated_bwd.cu", "ttt_gated_step.cu", "ttt_rotary.cu",
-           "ttt_abi_mixer.cu", "ttt_conv.cu", "ttt_norm.cu"]
+           "ttt_abi_mixer.cu", "ttt_conv.cu", "ttt_norm.cu", "ttt_selective_fwd.cu", "ttt_selective_bwd.cu"]
 HOST_SRC = CSRC / "ttt_host.cpp"                 # native host path of the Python operator, linked against LIB
 HOST_LIB = PKG / "_host.so"
 HOST_TAG = PKG / "build" / "_host.tag"           # what HOST_LIB was built against

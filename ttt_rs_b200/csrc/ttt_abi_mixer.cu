@@ -1,4 +1,4 @@
-// C ABI of the operators of a selective state space layer (include/ttt_b200.h): causal convolution, group norm with channels last.
+// C ABI of the operators of a selective state space layer (include/ttt_b200.h): causal convolution, the scan, group norm with channels last.
 // Argument checks and launches.
 #include <cstdarg>
 #include <cstdio>
@@ -253,4 +253,199 @@ extern "C" int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int
   p.gx = grad_x, p.ggate = grad_gate, p.gw = grad_weight, p.gb = grad_bias;
   p.partials = sums ? static_cast<float*>(workspace) : nullptr;
   return launched(ttt::launch_norm(dtype, p, width, sequence, true, static_cast<cudaStream_t>(stream)), "group norm backward");
+}
+
+namespace {
+
+struct SelDims {
+  int64_t B, T, C;
+  int G, N, dtype;
+  int NP, es;
+  ttt::SelCut cut[2];  // forward, backward
+  int64_t tiles, blocks;
+};
+int sel_dims(SelDims* d, int64_t B, int64_t T, int64_t C, int G, int N, int dtype) {
+  const int rc = check_sizes(B, T, C, dtype);
+  if (rc != TTT_OK) return rc;
+  if (G <= 0 || C % G != 0) return fail(TTT_ERR_SHAPE, "channels=%lld are not a multiple of groups=%d", (long long)C, G);
+  if (N < 1 || N > ttt::SEL_STATES) return fail(TTT_ERR_UNSUPPORTED, "Unsupported states=%d (supported: 1..%d)", N, ttt::SEL_STATES);
+  if (B * C >= (int64_t)1 << 31) return fail(TTT_ERR_SHAPE, "batch*channels must be below 2^31");
+  if (B * T * G >= (int64_t)1 << 32) return fail(TTT_ERR_SHAPE, "batch*seq_len*groups must be below 2^32");
+  d->B = B, d->T = T, d->C = C, d->G = G, d->N = N, d->dtype = dtype;
+  d->NP = ttt::sel_padded(N);
+  d->es = dtype == TTT_BF16 ? 2 : 4;
+  for (int k = 0; k < 2; ++k) d->cut[k] = ttt::sel_cut(B, T, (int)C, G, N, k != 0);
+  d->tiles = (T + ttt::SEL_TILE - 1) / ttt::SEL_TILE;
+  d->blocks = d->cut[0].channel_blocks;
+  return TTT_OK;
+}
+int64_t up4(int64_t n) { return (n + 3) & ~(int64_t)3; }
+// floats of a cut's segment states (and the first one's start) and sums
+int64_t seg_floats(const SelDims& d, const ttt::SelCut& k) {
+  return k.nseg == 1 ? 0 : d.B * (k.nseg + 1) * d.C * d.NP + up4(d.B * k.nseg * d.C);
+}
+int64_t saved_floats(const SelDims& d) { return d.B * d.tiles * d.C * d.NP; }
+int64_t backward_floats(const SelDims& d) {
+  const int64_t rows = d.B * d.cut[1].nseg;
+  return d.B * d.G * d.blocks * d.T * 2 * d.NP + rows * d.C * d.NP + up4(rows * 2 * d.C) + seg_floats(d, d.cut[1]);
+}
+void set_segments(ttt::SelParams* p, const SelDims& d, const ttt::SelCut& k, float* at) {
+  p->nseg = k.nseg, p->seg_tiles = k.seg_tiles;
+  if (k.nseg > 1) p->seg_state = at, p->seg_sum = at + d.B * (k.nseg + 1) * d.C * d.NP;
+}
+
+// The tensors that both directions read.  strides: batch and token of x, dt, z and (backward) grad_y, then batch, token and group of b, c.
+int sel_inputs(ttt::SelParams* p, const SelDims& d, const void* x, const void* dt, const float* a, const void* b, const void* c, const float* skip,
+               const void* z, const float* bias, const float* state, const void* starts, const void* gy, bool backward, const int64_t* strides,
+               const void* y, const void* gx, const void* gdt, const void* gz) {
+  Spans s{d.B, d.T, d.C, d.es};
+  s.rows("x", x, strides, 0, p->xs);
+  s.rows("dt", dt, strides, 1, p->ds);
+  s.rows("z", z, strides, 2, p->zs, true);
+  if (backward) {
+    s.rows("grad_y", gy, strides, 3, p->gs);
+    s.need("grad_x", gx);
+    s.need("grad_dt", gdt);
+    if (z != nullptr) s.need("grad_z", gz);
+  } else {
+    s.need("y", y);
+  }
+  const int64_t each = d.C / d.G * d.es;
+  p->xg = s.low % 16 == 0 && each % 16 == 0 ? 16 : s.low % 4 == 0 && each % 4 == 0 ? 4 : d.es;
+  Spans m{d.B, d.T, (int64_t)d.G * d.N, d.es};
+  const int64_t* at = strides != nullptr ? strides + (backward ? 8 : 6) : nullptr;
+  const void* bases[2] = {b, c};
+  int64_t(*out[2])[3] = {&p->bs, &p->cs};
+  const char* names[2] = {"b", "c"};
+  for (int k = 0; k < 2; ++k) {
+    const int64_t two[2] = {at != nullptr ? at[3 * k] : d.T * d.G * d.N, at != nullptr ? at[3 * k + 1] : (int64_t)d.G * d.N};
+    int64_t rows[2];
+    m.rows(names[k], bases[k], two, 0, rows);
+    const int64_t group = d.G == 1 ? 0 : at != nullptr ? at[3 * k + 2] : d.N;
+    m.low |= (uintptr_t)(group * d.es);
+    if (m.rc == TTT_OK && (group < 0 || group > (int64_t)1 << 40)) m.rc = fail(TTT_ERR_SHAPE, "the strides of %s are out of range", names[k]);
+    (*out[k])[0] = rows[0], (*out[k])[1] = rows[1], (*out[k])[2] = group;
+  }
+  const int64_t wide = (int64_t)d.N * d.es;
+  p->bg = m.low % 16 == 0 && wide % 16 == 0 ? 16 : m.low % 4 == 0 && wide % 4 == 0 ? 4 : d.es;
+  if (s.rc != TTT_OK) return s.rc;
+  if (m.rc != TTT_OK) return m.rc;
+  const struct {
+    const char* name;
+    const void* p;
+    unsigned align;
+    bool needed;
+  } plain[] = {{"a", a, 16, true}, {"d", skip, 4, false}, {"dt_bias", bias, 4, false}, {"state", state, 16, false}};
+  for (const auto& q : plain) {
+    if (q.needed && q.p == nullptr) return fail(TTT_ERR_NULL, "%s is null", q.name);
+    if (reinterpret_cast<uintptr_t>(q.p) % q.align != 0) return fail(TTT_ERR_ALIGN, "%s is not %u-byte aligned", q.name, q.align);
+  }
+  p->x = x, p->dt = dt, p->z = z, p->b = b, p->c = c, p->A = a, p->D = skip, p->bias = bias, p->state = state;
+  p->starts = static_cast<const uint8_t*>(starts);
+  p->B = d.B, p->T = d.T, p->C = (int)d.C, p->G = d.G, p->N = d.N;
+  return TTT_OK;
+}
+int need16(const char* name, const void* p, bool optional) {
+  if (p == nullptr && !optional) return fail(TTT_ERR_NULL, "%s is null", name);
+  if ((reinterpret_cast<uintptr_t>(p) & 15u) != 0) return fail(TTT_ERR_ALIGN, "%s is not 16-byte aligned", name);
+  return TTT_OK;
+}
+
+}  // namespace
+
+extern "C" size_t ttt_linear_selective_saved_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype) {
+  SelDims d;
+  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * saved_floats(d) : 0;
+}
+extern "C" size_t ttt_linear_selective_forward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,
+                                                               int dtype) {
+  SelDims d;
+  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * seg_floats(d, d.cut[0]) : 0;
+}
+extern "C" size_t ttt_linear_selective_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,
+                                                                int dtype) {
+  SelDims d;
+  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * backward_floats(d) : 0;
+}
+
+extern "C" int ttt_linear_selective_forward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype, int softplus,
+                                            const void* x, const void* dt, const float* a, const void* b, const void* c, const float* d_skip,
+                                            const void* z, const float* dt_bias, const float* state, const void* starts,
+                                            const int64_t* strides, void* y, float* state_out, void* saved, size_t saved_bytes,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  SelDims d;
+  ttt::SelParams p{};
+  int rc = sel_dims(&d, batch, seq_len, channels, groups, states, dtype);
+  if (rc != TTT_OK ||
+      (rc = sel_inputs(&p, d, x, dt, a, b, c, d_skip, z, dt_bias, state, starts, nullptr, false, strides, y, nullptr, nullptr, nullptr)) != TTT_OK ||
+      (rc = need16("state_out", state_out, false)) != TTT_OK)
+    return rc;
+  const Spans s{d.B, d.T, d.C, d.es};
+  const Spans m{d.B, d.T, d.N, d.es};
+  const int64_t held = d.B * d.C * d.N * 4, n = d.B * d.T * d.C * d.es;
+  const int64_t bb[2] = {p.bs[0], p.bs[1]}, cb[2] = {p.cs[0], p.cs[1]};
+  const struct {
+    const char* name;
+    const void* p;
+    int64_t bytes;
+  } others[] = {{"x", x, s.bytes(p.xs)}, {"dt", dt, s.bytes(p.ds)}, {"z", z, s.bytes(p.zs)}, {"a", a, d.C * d.N * 4}, {"d", d_skip, d.C * 4},
+                {"dt_bias", dt_bias, d.C * 4}, {"b", b, m.bytes(bb) + p.bs[2] * (d.G - 1) * d.es}, {"c", c, m.bytes(cb) + p.cs[2] * (d.G - 1) * d.es},
+                {"starts", starts, d.B * d.T}, {"y", y, n}};
+  for (const auto& o : others) {
+    if ((rc = check_apart("state_out", state_out, held, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
+    if (o.p != y && (rc = check_apart("y", y, n, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
+  }
+  if ((rc = check_apart("state_out", state_out, held, "state", state, held, true)) != TTT_OK ||
+      (rc = check_apart("y", y, n, "state", state, held, false)) != TTT_OK)
+    return rc;
+  p.softplus = softplus != 0;
+  p.y = y, p.state_out = state_out;
+  if (saved == nullptr && seq_len <= 16) return launched(ttt::launch_selective_step(dtype, p, static_cast<cudaStream_t>(stream)), "selective step");
+  if (saved != nullptr && (rc = check_bytes(saved_bytes, sizeof(float) * saved_floats(d), saved, "saved")) != TTT_OK) return rc;
+  if ((rc = check_bytes(workspace_bytes, sizeof(float) * seg_floats(d, d.cut[0]), workspace, "workspace")) != TTT_OK) return rc;
+  p.saved = static_cast<float*>(saved);
+  set_segments(&p, d, d.cut[0], static_cast<float*>(workspace));
+  return launched(ttt::launch_selective(dtype, p, static_cast<cudaStream_t>(stream)), "selective scan");
+}
+
+extern "C" int ttt_linear_selective_backward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype, int softplus,
+                                             const void* x, const void* dt, const float* a, const void* b, const void* c, const float* d_skip,
+                                             const void* z, const float* dt_bias, const void* starts, const void* grad_y,
+                                             const int64_t* strides, const void* saved, size_t saved_bytes, const float* grad_state_out,
+                                             void* grad_x, void* grad_dt, float* grad_a, void* grad_b, void* grad_c, float* grad_d,
+                                             void* grad_z, float* grad_dt_bias, float* grad_state, void* workspace, size_t workspace_bytes,
+                                             void* stream) {
+  SelDims d;
+  ttt::SelParams p{};
+  int rc = sel_dims(&d, batch, seq_len, channels, groups, states, dtype);
+  if (rc != TTT_OK || (rc = sel_inputs(&p, d, x, dt, a, b, c, d_skip, z, dt_bias, nullptr, starts, grad_y, true, strides, nullptr, grad_x, grad_dt,
+                                       grad_z)) != TTT_OK)
+    return rc;
+  if (saved == nullptr) return fail(TTT_ERR_NULL, "saved is null");
+  if ((rc = check_bytes(saved_bytes, sizeof(float) * saved_floats(d), saved, "saved")) != TTT_OK ||
+      (rc = need16("grad_state_out", grad_state_out, true)) != TTT_OK || (rc = need16("grad_a", grad_a, false)) != TTT_OK ||
+      (rc = need16("grad_state", grad_state, true)) != TTT_OK)
+    return rc;
+  const struct {
+    const char* name;
+    const void* p;
+    unsigned align;
+    bool needed;
+  } plain[] = {{"grad_b", grad_b, (unsigned)d.es, true}, {"grad_c", grad_c, (unsigned)d.es, true}, {"grad_d", grad_d, 4, false}, {"grad_dt_bias", grad_dt_bias, 4, false}};
+  for (const auto& q : plain) {
+    if (q.needed && q.p == nullptr) return fail(TTT_ERR_NULL, "%s is null", q.name);
+    if (reinterpret_cast<uintptr_t>(q.p) % q.align != 0) return fail(TTT_ERR_ALIGN, "%s is not aligned to its elements", q.name);
+  }
+  if ((rc = check_bytes(workspace_bytes, sizeof(float) * backward_floats(d), workspace, "workspace")) != TTT_OK) return rc;
+  float* ws = static_cast<float*>(workspace);
+  const int64_t rows = d.B * d.cut[1].nseg;
+  p.part_bc = ws, ws += d.B * d.G * d.blocks * d.T * 2 * d.NP;
+  p.part_a = ws, ws += rows * d.C * d.NP;
+  p.part_d = ws, ws += up4(rows * 2 * d.C);
+  set_segments(&p, d, d.cut[1], ws);
+  p.softplus = softplus != 0;
+  p.saved = static_cast<float*>(const_cast<void*>(saved));
+  p.gy = grad_y, p.gstate_out = grad_state_out, p.gx = grad_x, p.gdt = grad_dt, p.gz = grad_z, p.ga = grad_a, p.gb = grad_b, p.gc = grad_c;
+  p.gd = grad_d, p.gbias = grad_dt_bias, p.gstate = grad_state;
+  return launched(ttt::launch_selective_bwd(dtype, p, static_cast<cudaStream_t>(stream)), "selective scan backward");
 }

@@ -669,6 +669,98 @@ struct NormFn : torch::autograd::Function<NormFn> {
   }
 };
 
+// x, dt, A, B, C, then D, z, dt_bias, state, starts (each or undefined)
+struct Selective {
+  Rows m;
+  int64_t G = 0, N = 0;
+  int softplus = 1;
+  static bool states(const Tensor& t, const Rows& m, int64_t G, int64_t N) {  // [B,T,G,N] with contiguous states
+    if (!t.defined() || !t.is_cuda() || t.device() != m.dev || t.scalar_type() != m.dt || t.layout() != c10::kStrided || t.dim() != 4) return false;
+    return t.size(0) == m.B && t.size(1) == m.T && t.size(2) == G && t.size(3) == N && (t.stride(3) == 1 || N == 1);
+  }
+  bool held(const Tensor& t) const { return !t.defined() || (is(t, at::kFloat, m.dev, {m.B, m.C, N}) && on_16_bytes(t)); }
+  bool set(const Tensor (&t)[5], const Tensor (&o)[5], int64_t sp) {
+    if (!m.set(t[0]) || !channel_rows(t[1], m.dev, m.dt) || t[1].sizes() != t[0].sizes() || t[3].dim() != 4) return false;
+    G = t[3].size(2), N = t[3].size(3), softplus = (int)sp;
+    if (G < 1 || N < 1 || m.C % G != 0 || N > INT32_MAX) return false;
+    return is(t[2], at::kFloat, m.dev, {m.C, N}) && on_16_bytes(t[2]) && states(t[3], m, G, N) && states(t[4], m, G, N) &&
+           m.vector(o[0], at::kFloat) && (!o[1].defined() || (channel_rows(o[1], m.dev, m.dt) && o[1].sizes() == t[0].sizes())) &&
+           m.vector(o[2], at::kFloat) && held(o[3]) && m.marks(o[4]);
+  }
+  std::vector<int64_t> strides(std::initializer_list<const Tensor*> rows, const Tensor& b, const Tensor& c) const {
+    std::vector<int64_t> s;
+    for (const Tensor* t : rows)
+      for (int k = 0; k < 2; ++k) s.push_back(t->defined() ? t->stride(k) : 0);
+    for (const Tensor* t : {&b, &c})
+      for (int k = 0; k < 3; ++k) s.push_back(t->stride(k));
+    return s;
+  }
+  static const float* f32(const Tensor& t) { return static_cast<const float*>(ptr(t)); }
+  int forward(const Tensor (&t)[5], const Tensor (&o)[5], bool save, Tensor& y, Tensor& out, Tensor& saved) const {
+    c10::cuda::CUDAGuard guard(m.dev);
+    y = m.empty();
+    if (!out.defined()) out = at::empty({m.B, m.C, N}, m.opt(at::kFloat));
+    size_t wsb = 0, sb = 0;
+    if (save || m.T > 16) wsb = ttt_linear_selective_forward_workspace_bytes(m.B, m.T, m.C, (int)G, (int)N, m.dtype);
+    if (save) {
+      sb = ttt_linear_selective_saved_bytes(m.B, m.T, m.C, (int)G, (int)N, m.dtype);
+      if (sb == 0) return TTT_ERR_UNSUPPORTED;
+      saved = at::empty({(int64_t)sb}, m.opt(at::kByte));
+    }
+    const Tensor ws = workspace(m, wsb);
+    return ttt_linear_selective_forward(m.B, m.T, m.C, (int)G, (int)N, m.dtype, softplus, ptr(t[0]), ptr(t[1]), f32(t[2]), ptr(t[3]), ptr(t[4]),
+                                        f32(o[0]), ptr(o[1]), f32(o[2]), f32(o[3]), ptr(o[4]), strides({&t[0], &t[1], &o[1]}, t[3], t[4]).data(),
+                                        y.data_ptr(), static_cast<float*>(out.data_ptr()), data(saved), sb, data(ws), wsb, m.stream());
+  }
+};
+struct SelectiveFn : torch::autograd::Function<SelectiveFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+                               const Tensor& D, const Tensor& z, const Tensor& bias, const Tensor& state, const Tensor& starts,
+                               std::vector<int64_t> has) {  // has: D, z, bias, state, starts; softplus
+    Selective call;
+    const Tensor t[5] = {x, dt, A, B, C}, o[5] = {has[0] ? D : Tensor(), has[1] ? z : Tensor(), has[2] ? bias : Tensor(), has[3] ? state : Tensor(),
+                                                  has[4] ? starts : Tensor()};
+    Tensor y, out, saved;
+    call.set(t, o, has[5]);
+    const int rc = call.forward(t, o, true, y, out, saved);
+    if (rc != TTT_OK) throw_error(rc);
+    ctx->save_for_backward({x, dt, A, B, C, D, z, bias, starts, saved});  // (of the state, what the tiles' states say)
+    ctx->saved_data["has"] = has;
+    ctx->set_materialize_grads(false);
+    return {y, out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list go) {
+    const variable_list s = ctx->get_saved_variables();
+    const std::vector<int64_t> has = ctx->saved_data["has"].toIntVector();
+    if (!go[0].defined() && !go[1].defined()) return variable_list(11);
+    Selective call;
+    const Tensor t[5] = {s[0], s[1], s[2], s[3], s[4]}, o[5] = {has[0] ? s[5] : Tensor(), has[1] ? s[6] : Tensor(), has[2] ? s[7] : Tensor(), Tensor(),
+                                                               has[4] ? s[8] : Tensor()};
+    call.set(t, o, has[5]);
+    const Rows& m = call.m;
+    c10::cuda::CUDAGuard guard(m.dev);
+    const Tensor gy = go[0].defined() ? rows_of(go[0], m) : at::zeros({m.B, m.T, m.C}, m.opt());
+    Tensor gs = go[1].defined() ? go[1].contiguous() : Tensor();
+    if (gs.defined() && !on_16_bytes(gs)) gs = gs.clone();
+    Tensor gx = m.empty(), gdt = m.empty(), gA = at::empty({m.C, call.N}, m.opt(at::kFloat)), gB = at::empty({m.B, m.T, call.G, call.N}, m.opt()),
+           gC = at::empty_like(gB), gD, gz, gbias, gstate;
+    if (has[0]) gD = at::empty({m.C}, m.opt(at::kFloat));
+    if (has[1]) gz = m.empty();
+    if (has[2]) gbias = at::empty({m.C}, m.opt(at::kFloat));
+    if (has[3]) gstate = at::empty({m.B, m.C, call.N}, m.opt(at::kFloat));
+    const size_t wsb = ttt_linear_selective_backward_workspace_bytes(m.B, m.T, m.C, (int)call.G, (int)call.N, m.dtype);
+    const Tensor ws = workspace(m, wsb);
+    auto f = [](const Tensor& v) { return static_cast<float*>(data(v)); };
+    const int rc = ttt_linear_selective_backward(
+        m.B, m.T, m.C, (int)call.G, (int)call.N, m.dtype, call.softplus, ptr(t[0]), ptr(t[1]), call.f32(t[2]), ptr(t[3]), ptr(t[4]), call.f32(o[0]),
+        ptr(o[1]), call.f32(o[2]), ptr(o[4]), gy.const_data_ptr(), call.strides({&t[0], &t[1], &o[1], &gy}, t[3], t[4]).data(),
+        s[9].const_data_ptr(), (size_t)s[9].numel(), call.f32(gs), gx.data_ptr(), gdt.data_ptr(), f(gA), gB.data_ptr(), gC.data_ptr(), f(gD), data(gz),
+        f(gbias), f(gstate), data(ws), wsb, m.stream());
+    if (rc != TTT_OK) throw_error(rc);
+    return only_once({gx, gdt, gA, gB, gC, gD, gz, gbias, gstate, Tensor(), Tensor()});
+  }
+};
+
 // ---- Python functions ----------------------------------------------------------------------------------------------
 // tensors args[0..n), false when one is not a tensor
 template <int N>
@@ -1437,6 +1529,33 @@ PyObject* py_group_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// selective(x, dt, A, B, C, D | None, z | None, dt_bias | None, state | None, starts | None, softplus, state_out | None) -> (y, state),
+// recorded for autograd where that is on and asked for | None
+PyObject* py_selective(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arity(n, 12)) return nullptr;
+  Tensor t[5], o[5], out, y, saved;
+  NONE_IF(!tensors(args, t));
+  for (int i = 0; i < 5; ++i) NONE_IF(!optional_tensor(args[5 + i], o[i]));
+  NONE_IF(!optional_tensor(args[11], out));
+  const int64_t softplus = as_int(args[10]);
+  if (PyErr_Occurred()) return nullptr;
+  refuse_tangents({&t[0], &t[1], &t[2], &t[3], &t[4], &o[0], &o[1], &o[2], &o[3], &out});
+  Selective call;
+  NONE_IF(!call.set(t, o, softplus) || !call.held(out));
+  if (wants_grad({&t[0], &t[1], &t[2], &t[3], &t[4], &o[0], &o[1], &o[2], &o[3], &out})) {
+    NONE_IF(out.defined());
+    return wrap(SelectiveFn::apply(t[0], t[1], t[2], t[3], t[4], given(o[0]), given(o[1]), given(o[2]), given(o[3]), given(o[4]),
+                                   std::vector<int64_t>{o[0].defined(), o[1].defined(), o[2].defined(), o[3].defined(), o[4].defined(), softplus}));
+  }
+  const bool given_out = out.defined();
+  const int rc = call.forward(t, o, false, y, out, saved);
+  if (rc != TTT_OK) throw_error(rc);
+  if (given_out) overwritten(out);
+  return wrap({y, out});
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(set_status),
@@ -1456,6 +1575,7 @@ PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST(qk_norm_backward),
                          FAST(causal_conv),
                          FAST(group_norm),
+                         FAST(selective),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -530,4 +530,44 @@ size_t norm_forward_floats(int64_t B, int64_t T, int C, int G, bool sequence, in
 size_t norm_backward_floats(int64_t B, int64_t T, int C, int G, bool sequence, int element_bytes);
 cudaError_t launch_norm(int dtype, const NormParams& p, int V, bool sequence, bool bwd, cudaStream_t st);
 
+
+// ---- selective state space scan (ttt_selective_fwd.cu, ttt_selective_bwd.cu) ---------------------------------------------------------
+// Tensors [B,T,C] (x, dt, z, gy) with contiguous channels, b and c [B,T,G,N] with contiguous states; N <= NP states, NP a power of two
+struct SelParams {
+  const void *x, *dt, *z, *b, *c;    // z or null
+  const float *A, *D, *bias, *state;  // A [C][N]; D, bias [C], state [B][C][N], or null: zeros
+  const uint8_t* starts;             // [B][T] or null
+  void* y;
+  float* state_out;                  // [B][C][N]; may be state
+  float* saved;                      // [B][tiles][C][NP] states before every SEL_TILE tokens, or null
+  float *seg_state, *seg_sum;        // nseg > 1: [B][nseg][C][NP] a segment's own state, then [B][C][NP] the first one's start; [B][nseg][C] its
+                                     // sum of steps (inf: a start in it)
+  int64_t xs[2], ds[2], zs[2], bs[3], cs[3];  // strides of batch and token (and group), in elements
+  int64_t B, T;
+  int C, G, N;
+  int softplus;
+  int xg, bg;                        // bytes that rows of channels, and of states, can be copied at a time
+  int nseg, seg_tiles;
+  // backward
+  const void* gy;
+  const float* gstate_out;           // or null: zeros
+  int64_t gs[2];
+  void *gx, *gdt, *gz;
+  float* part_bc;                    // [B][G][channel blocks][T][2][NP]
+  float* part_a;                     // [B nseg][C][NP]
+  float* part_d;                     // [B nseg][2][C]: D, bias
+  float *ga, *gd, *gbias, *gstate;   // gd, gbias, gstate: or null
+  void *gb, *gc;                     // contiguous [B,T,G,N]
+};
+constexpr int SEL_TILE = 16;         // tokens between saved states
+constexpr int SEL_STATES = 64;       // states per channel at most
+int sel_padded(int N);               // NP
+struct SelCut {
+  int nseg, seg_tiles, channel_blocks;  // channel blocks: of a group
+};
+SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd);
+cudaError_t launch_selective(int dtype, const SelParams& p, cudaStream_t st);
+cudaError_t launch_selective_step(int dtype, const SelParams& p, cudaStream_t st);
+cudaError_t launch_selective_bwd(int dtype, const SelParams& p, cudaStream_t st);
+
 }  // namespace ttt

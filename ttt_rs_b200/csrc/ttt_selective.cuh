@@ -1,0 +1,200 @@
+// Selective state space scan: definitions shared by its kernels.
+//
+//   d_t = softplus(dt_t + bias)  (or dt_t + bias),   h_t = exp(d_t A) h_{t-1} + d_t x_t B_t,   y_t = C_t h_t + D x_t,  times SiLU(z_t)
+// for every channel, with N states h and A [C][N], and with B_t, C_t [N] shared by a group's channels; a start at token t puts
+// h_{t-1} = 0.
+//
+// What bounds it is exponentials: one per state, channel and token, 16 per SM and clock, where memory would allow twice as many at
+// N = 16.  A thread holds SEL_EACH states of SEL_CH neighbouring channels (1 where N <= 4); NP / SEL_EACH lanes share a channel.
+// Tiles of SEL_TILE tokens are copied ahead (cp.async), turned into (step, step times x) pairs in float32 in shared memory, scanned
+// token by token, and written by pairs of channels.
+#pragma once
+
+#include "ttt_kernels.h"
+#include "ttt_vec.cuh"
+
+namespace ttt {
+
+constexpr int SEL_THREADS = 128;
+constexpr int SEL_EACH = 4;  // states per thread
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+template <int NP>
+struct SelShape {
+  static constexpr int SL = NP / SEL_EACH;         // lanes that share a channel
+  static constexpr int CL = 32 / SL;               // lanes with channels of their own
+  static constexpr int CC = SL == 1 ? 1 : 2;       // channels of a thread
+  static constexpr int WARP_CH = CL * CC;
+  static constexpr int CH = WARP_CH * (SEL_THREADS / 32);  // of a block: 128, 128, 64, 32, 16
+  static constexpr int PAIRS = CH / 2;
+  static constexpr int ROWS = SEL_THREADS / PAIRS;         // tokens that the block's threads cover, pair by pair
+  static constexpr int PITCH = CH + 16;            // floats between tokens of results: two tokens' channels in different banks
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ F2 ex2(F2 x) { return f2(ex2(x.x), ex2(x.y)); }
+
+// log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1], by log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: terms up
+// to s^15 leave 2^-27 of it.  sig: 1 / (1 + exp(-v)).
+__device__ __forceinline__ float softplus_of(float v, float& sig) {
+  const float e = __expf(-fabsf(v)), s = __fdividef(e, 2.f + e), q = s * s;
+  float r = fmaf(q, 1.f / 15.f, 1.f / 13.f);
+  r = fmaf(q, r, 1.f / 11.f);
+  r = fmaf(q, r, 1.f / 9.f);
+  r = fmaf(q, r, 1.f / 7.f);
+  r = fmaf(q, r, 1.f / 5.f);
+  r = fmaf(q, r, 1.f / 3.f);
+  r = fmaf(q * s, r, s);
+  sig = __fdividef(v >= 0.f ? 1.f : e, 1.f + e);
+  return v != v ? v : fmaf(2.f, r, fmaxf(v, 0.f));
+}
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async4(void* dst, const void* src, bool live) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// rows [t0, t0 + SEL_TILE) of `have` elements, at most WIDE, into dst [SEL_TILE][WIDE]; zeros beyond T and `have`.  bytes: 16, 4, or an
+// element's size, what addresses, strides and `have` are multiples of.
+template <typename T, int WIDE>
+__device__ __forceinline__ void copy_rows(T* dst, const T* src, int64_t stride, int64_t t0, int64_t t_end, int have, int bytes) {
+  constexpr int V16 = 16 / sizeof(T);
+  if (WIDE >= V16 && bytes == 16) {
+    constexpr int V = WIDE >= V16 ? V16 : 1, PER = WIDE / V;
+    for (int i = threadIdx.x; i < SEL_TILE * PER; i += SEL_THREADS) {
+      const int r = i / PER, e = (i - r * PER) * V;
+      const bool live = t0 + r < t_end && e < have;
+      copy_async16(dst + r * WIDE + e, live ? src + (t0 + r) * stride + e : src, live);
+    }
+  } else if (bytes >= 4) {
+    constexpr int V = 4 / sizeof(T), PER = WIDE / V;
+    for (int i = threadIdx.x; i < SEL_TILE * PER; i += SEL_THREADS) {
+      const int r = i / PER, e = (i - r * PER) * V;
+      const bool live = t0 + r < t_end && e < have;
+      copy_async4(dst + r * WIDE + e, live ? src + (t0 + r) * stride + e : src, live);
+    }
+  } else {
+    for (int i = threadIdx.x; i < SEL_TILE * WIDE; i += SEL_THREADS) {
+      const int r = i / WIDE, e = i - r * WIDE;
+      dst[i] = t0 + r < t_end && e < have ? src[(t0 + r) * stride + e] : T(0.f);
+    }
+  }
+}
+
+// Two neighbouring channels of a row, from shared memory and to global memory (whole: both exist and lie on a pair's address)
+__device__ __forceinline__ float2 pair_of(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 pair_of(const __nv_bfloat16* p) {
+  const uint32_t v = *reinterpret_cast<const uint32_t*>(p);
+  return make_float2(bf16_lo(v), bf16_hi(v));
+}
+template <typename T>
+__device__ __forceinline__ void put_pair(T* p, float2 v, int have, bool whole) {
+  if (whole) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = v;
+    else *reinterpret_cast<uint32_t*>(p) = pack_bf16(v.x, v.y);
+  } else {
+    if (have > 0) st_from_float<T>(p, 0, v.x);
+    if (have > 1) st_from_float<T>(p, 1, v.y);
+  }
+}
+
+// v[i] summed over the LANES lanes that differ in the lane bits STRIDE, 2 STRIDE, ...; the lane with number k among them gets v[k]
+// (COUNT = LANES), or v[k COUNT / LANES ...] in v[0 ...] (COUNT > LANES), or the one that k's high bits name (COUNT < LANES).
+template <int COUNT, int LANES, int STRIDE>
+__device__ __forceinline__ void sum_and_deal(float (&v)[COUNT], int lane) {
+  constexpr int STEPS = LANES == 1 ? 0 : LANES == 2 ? 1 : LANES == 4 ? 2 : LANES == 8 ? 3 : LANES == 16 ? 4 : 5;
+  int n = COUNT, o = LANES / 2;
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k) {
+    const bool up = (lane & (o * STRIDE)) != 0;
+    if (n > 1) {
+#pragma unroll
+      for (int i = 0; i < COUNT / 2; ++i)
+        if (i < n / 2) {
+          const float send = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o * STRIDE);
+        }
+      n /= 2;
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o * STRIDE);
+    }
+    o /= 2;
+  }
+}
+
+// Where a block stands: batch row, group, its channels, its segment of the tokens
+template <int NP>
+struct SelPlace {
+  using S = SelShape<NP>;
+  int64_t b;
+  int g, block, seg, c0, have;  // have: channels of the block that exist
+  int64_t t_lo, t_hi;           // tokens of the segment
+  // blocks of `segments` segments, from `first` on
+  __device__ __forceinline__ SelPlace(const SelParams& p, int first, int segments) {
+    const int each = p.C / p.G, blocks = (each + S::CH - 1) / S::CH;
+    int64_t i = blockIdx.x;
+    block = (int)(i % blocks), i /= blocks;
+    g = (int)(i % p.G), i /= p.G;
+    seg = first + (int)(i % segments), b = i / segments;
+    c0 = g * each + block * S::CH;
+    have = min(S::CH, each - block * S::CH);
+    t_lo = (int64_t)seg * p.seg_tiles * SEL_TILE;
+    t_hi = min(p.T, t_lo + (int64_t)p.seg_tiles * SEL_TILE);
+  }
+};
+
+// Rates of a thread's channels (times log2 e), and what is read and written as [C][N] or [C][NP] rows
+template <int NP>
+struct SelLane {
+  using S = SelShape<NP>;
+  int lane, sl, ch;  // ch: the first of the thread's channels, in the block
+  __device__ __forceinline__ SelLane() {
+    lane = threadIdx.x & 31;
+    sl = lane & (S::SL - 1);
+    ch = (threadIdx.x >> 5) * S::WARP_CH + (lane / S::SL) * S::CC;
+  }
+  // row of `n` states (N in memory) of channel c0 + ch + k, zeros beyond
+  __device__ __forceinline__ void load(F2 (&v)[S::CC][2], const float* rows, int n, int have) const {
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = rows != nullptr && ch + k < have && 4 * sl + i < n ? rows[(int64_t)(ch + k) * n + 4 * sl + i] : 0.f;
+      v[k][0] = f2(e[0], e[1]), v[k][1] = f2(e[2], e[3]);
+    }
+  }
+  __device__ __forceinline__ void store(const F2 (&v)[S::CC][2], float* rows, int n, int have) const {
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k) {
+      if (ch + k >= have) continue;
+      float* at = rows + (int64_t)(ch + k) * n + 4 * sl;
+      if (n == NP) {
+        *reinterpret_cast<float4*>(at) = make_float4(v[k][0].x, v[k][0].y, v[k][1].x, v[k][1].y);
+      } else {
+        if (4 * sl < n) at[0] = v[k][0].x;
+        if (4 * sl + 1 < n) at[1] = v[k][0].y;
+        if (4 * sl + 2 < n) at[2] = v[k][1].x;
+        if (4 * sl + 3 < n) at[3] = v[k][1].y;
+      }
+    }
+  }
+  // [C][NP] rows
+  __device__ __forceinline__ void load_padded(F2 (&v)[S::CC][2], const float* rows, int have) const {
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k) {
+      float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (ch + k < have) e = *reinterpret_cast<const float4*>(rows + (int64_t)(ch + k) * NP + 4 * sl);
+      v[k][0] = f2(e.x, e.y), v[k][1] = f2(e.z, e.w);
+    }
+  }
+};
+
+}  // namespace ttt

@@ -1,0 +1,338 @@
+// Selective state space scan, forward and decode step (definitions: ttt_selective.cuh).
+//
+// A block of four warps owns 64 channels (N = 16) of a sequence, or of a segment of it.  Segments, where channels are too few to fill
+// the card: every segment's own state first (from zero, with the sum of its steps, since exp(A sum d) is its whole decay), which the
+// scan's blocks join along the sequence before they begin.  For training the states before every SEL_TILE tokens are kept.
+#include "ttt_selective.cuh"
+
+namespace ttt {
+
+template <typename T, int NP, bool FULL>
+struct SelSmem {
+  using S = SelShape<NP>;
+  static constexpr int TENSORS = FULL ? 3 : 2;
+  alignas(16) T raw[2][TENSORS][SEL_TILE][S::CH];       // x, dt, z
+  alignas(16) T raw_bc[2][FULL ? 2 : 1][SEL_TILE][NP];
+  alignas(16) float4 du[SEL_TILE][S::PAIRS];            // (step, step x) of two channels
+  alignas(16) float bc[FULL ? 2 : 1][SEL_TILE][NP];
+  alignas(16) float y[FULL ? SEL_TILE : 1][S::PITCH];
+};
+
+template <typename T, int NP, bool FULL>
+__global__ void __launch_bounds__(SEL_THREADS) ttt_selective_kernel(const SelParams p) {
+  using S = SelShape<NP>;
+  using Smem = SelSmem<T, NP, FULL>;
+  extern __shared__ __align__(16) unsigned char sel_smem[];
+  Smem& sm = *reinterpret_cast<Smem*>(sel_smem);
+  const SelPlace<NP> at(p, 0, FULL ? p.nseg : p.nseg - 1);
+  const SelLane<NP> me;
+  const T* x = static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c0;
+  const T* dt = static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0;
+  const T* z = FULL && p.z != nullptr ? static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0 : nullptr;
+  const T* bm = static_cast<const T*>(p.b) + at.b * p.bs[0] + at.g * p.bs[2];
+  const T* cm = static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2];
+  const uint8_t* starts = p.starts != nullptr ? p.starts + at.b * p.T : nullptr;
+  auto fetch = [&](int64_t t0, int k) {
+    copy_rows<T, S::CH>(&sm.raw[k][0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH>(&sm.raw[k][1][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP>(&sm.raw_bc[k][0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
+    if constexpr (FULL) {
+      if (z != nullptr) copy_rows<T, S::CH>(&sm.raw[k][Smem::TENSORS - 1][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
+      copy_rows<T, NP>(&sm.raw_bc[k][FULL ? 1 : 0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
+    }
+    copy_commit();
+  };
+  fetch(at.t_lo, 0);
+
+  F2 A[S::CC][2], h[S::CC][2];
+  me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
+#pragma unroll
+  for (int k = 0; k < S::CC; ++k) A[k][0] = f2mul(A[k][0], f2(LOG2E)), A[k][1] = f2mul(A[k][1], f2(LOG2E));
+  if constexpr (FULL) {
+    if (p.nseg == 1) me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
+    else me.load_padded(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, at.have);
+    for (int j = 0; j < at.seg; ++j) {  // the segments before, in their order
+      const int64_t row = (at.b * p.nseg + j) * p.C + at.c0;
+      F2 own[S::CC][2];
+      me.load_padded(own, p.seg_state + row * NP, at.have);
+#pragma unroll
+      for (int k = 0; k < S::CC; ++k) {
+        const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
+        const bool cut = sum == INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) h[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), h[k][i], own[k][i]);
+      }
+    }
+  } else {
+    // (the given state may be where the new one goes, which other blocks of the scan write: the scan reads it from here)
+    if (at.seg == 0) {
+      me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
+      me.store(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, NP, at.have);
+    }
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k) h[k][0] = h[k][1] = f2(0.f);
+  }
+  // what an element-wise thread keeps: a pair of channels
+  const int pr = threadIdx.x % S::PAIRS, row0 = threadIdx.x / S::PAIRS, pair_have = at.have - 2 * pr;
+  float2 bias = make_float2(0.f, 0.f), skip = make_float2(0.f, 0.f);
+  if (p.bias != nullptr) {
+    if (pair_have > 0) bias.x = p.bias[at.c0 + 2 * pr];
+    if (pair_have > 1) bias.y = p.bias[at.c0 + 2 * pr + 1];
+  }
+  if (FULL && p.D != nullptr) {
+    if (pair_have > 0) skip.x = p.D[at.c0 + 2 * pr];
+    if (pair_have > 1) skip.y = p.D[at.c0 + 2 * pr + 1];
+  }
+  const bool whole = pair_have > 1 && p.xg >= 4 && (sizeof(T) == 2 || p.xg == 16);
+  float sum[2] = {0.f, 0.f};  // (FULL false: of the pair's steps over this thread's tokens)
+  bool any_start = false;
+
+  int buf = 0;
+  for (int64_t t0 = at.t_lo; t0 < at.t_hi; t0 += SEL_TILE, buf ^= 1) {
+    uint32_t mark = 0;
+    if (starts != nullptr) {
+      const int64_t t = t0 + (me.lane & (SEL_TILE - 1));
+      mark = __ballot_sync(0xffffffffu, t < at.t_hi && starts[t] != 0) & ((1u << SEL_TILE) - 1);
+      any_start = any_start || mark != 0;
+    }
+    copy_wait_all();
+    __syncthreads();
+    if (t0 + SEL_TILE < at.t_hi) fetch(t0 + SEL_TILE, buf ^ 1);
+#pragma unroll
+    for (int r = row0; r < SEL_TILE; r += S::ROWS) {
+      const float2 xv = pair_of(&sm.raw[buf][0][r][2 * pr]), dv = pair_of(&sm.raw[buf][1][r][2 * pr]);
+      float2 d = make_float2(dv.x + bias.x, dv.y + bias.y);
+      if (p.softplus) {
+        float sig;
+        d.x = softplus_of(d.x, sig), d.y = softplus_of(d.y, sig);
+      }
+      if (t0 + r >= at.t_hi || pair_have < 1) d.x = 0.f;
+      if (t0 + r >= at.t_hi || pair_have < 2) d.y = 0.f;
+      sm.du[r][pr] = make_float4(d.x, d.x * xv.x, d.y, d.y * xv.y);
+      if (!FULL) sum[0] += d.x, sum[1] += d.y;
+    }
+#pragma unroll
+    for (int i = threadIdx.x; i < (FULL ? 2 : 1) * SEL_TILE * NP; i += SEL_THREADS)
+      (&sm.bc[0][0][0])[i] = ld_as_float<T>(&sm.raw_bc[buf][0][0][0], i);
+    if (FULL && p.saved != nullptr)
+      me.store(h, p.saved + ((at.b * ((p.T + SEL_TILE - 1) / SEL_TILE) + t0 / SEL_TILE) * p.C + at.c0) * NP, NP, at.have);
+    __syncthreads();
+    constexpr int DEAL = S::SL > S::CC ? S::SL : S::CC, TOKENS = DEAL / S::CC;  // results dealt to the lanes of a channel
+#pragma unroll 4
+    for (int r0 = 0; r0 < SEL_TILE; r0 += TOKENS) {
+      float part[DEAL];
+#pragma unroll
+      for (int u = 0; u < TOKENS; ++u) {
+        const int r = r0 + u;
+        float4 q;
+        if constexpr (S::CC == 2) {
+          q = sm.du[r][me.ch / 2];
+        } else {
+          const float2 one = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(&sm.du[r][0]) + 2 * me.ch);
+          q = make_float4(one.x, one.y, 0.f, 0.f);
+        }
+        const float4 b = *reinterpret_cast<const float4*>(&sm.bc[0][r][4 * me.sl]);
+        if (mark >> r & 1) {
+#pragma unroll
+          for (int k = 0; k < S::CC; ++k) h[k][0] = h[k][1] = f2(0.f);
+        }
+        [[maybe_unused]] float4 c;
+        if constexpr (FULL) c = *reinterpret_cast<const float4*>(&sm.bc[FULL ? 1 : 0][r][4 * me.sl]);
+#pragma unroll
+        for (int k = 0; k < S::CC; ++k) {
+          const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
+          h[k][0] = f2fma(ex2(f2mul(A[k][0], d)), h[k][0], f2mul(v, f2(b.x, b.y)));
+          h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
+          if constexpr (FULL) part[u * S::CC + k] = f2hsum(f2fma(h[k][0], f2(c.x, c.y), f2mul(h[k][1], f2(c.z, c.w))));
+        }
+      }
+      if constexpr (FULL) {
+        sum_and_deal<DEAL, S::SL, 1>(part, me.lane);
+        // lane sl has result sl: channel sl % CC of token sl / CC (N <= 4: its only one)
+        if constexpr (S::SL == 1) sm.y[r0][me.ch] = part[0];
+        else sm.y[r0 + me.sl / S::CC][me.ch + me.sl % S::CC] = part[0];
+      }
+    }
+    if constexpr (FULL) {
+      __syncthreads();
+#pragma unroll
+      for (int r = row0; r < SEL_TILE; r += S::ROWS) {
+        if (t0 + r >= at.t_hi || pair_have < 1) continue;
+        const float2 xv = pair_of(&sm.raw[buf][0][r][2 * pr]);
+        float2 v = *reinterpret_cast<const float2*>(&sm.y[r][2 * pr]);
+        v.x = fmaf(skip.x, xv.x, v.x), v.y = fmaf(skip.y, xv.y, v.y);
+        if (z != nullptr) {
+          const float2 zv = pair_of(&sm.raw[buf][Smem::TENSORS - 1][r][2 * pr]);
+          v.x *= act_of(zv.x, ACT_SILU), v.y *= act_of(zv.y, ACT_SILU);
+        }
+        put_pair<T>(static_cast<T*>(p.y) + (at.b * p.T + t0 + r) * p.C + at.c0 + 2 * pr, v, pair_have, whole);
+      }
+    }
+  }
+  if constexpr (FULL) {
+    if (at.t_hi == p.T) me.store(h, p.state_out + (at.b * p.C + at.c0) * p.N, p.N, at.have);
+  } else {
+    const int64_t row = (at.b * p.nseg + at.seg) * p.C + at.c0;
+    me.store(h, p.seg_state + row * NP, NP, at.have);
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(&sm.du[0][0]);  // [ROWS][CH]
+    sums[row0 * S::CH + 2 * pr] = sum[0];
+    sums[row0 * S::CH + 2 * pr + 1] = sum[1];
+    __syncthreads();
+    for (int c = threadIdx.x; c < at.have; c += SEL_THREADS) {
+      float v = 0.f;
+      for (int r = 0; r < S::ROWS; ++r) v += sums[r * S::CH + c];
+      p.seg_sum[row + c] = any_start ? INFINITY : v;
+    }
+  }
+}
+
+// Up to 16 tokens against the resident state: a thread per channel and SEL_EACH states, no shared memory.  Bound by the state's read
+// and write where sequences are many, by the launch and one chain of loads where not.
+template <typename T, int SL>
+__global__ void __launch_bounds__(SEL_THREADS) ttt_selective_step_kernel(const SelParams p) {
+  const int64_t i = (int64_t)blockIdx.x * SEL_THREADS + threadIdx.x;
+  const int sl = (int)(i % SL);
+  const int64_t row = i / SL;  // b C + c
+  const bool live = row < p.B * p.C;
+  const int64_t b = live ? row / p.C : 0;
+  const int c = live ? (int)(row - b * p.C) : 0, g = c / (p.C / p.G);
+  const bool quads = p.N % 4 == 0;
+  float a[4], h[4];
+  const float* ap = p.A + (int64_t)c * p.N + 4 * sl;
+  const float* hp = p.state != nullptr ? p.state + (b * p.C + c) * p.N + 4 * sl : nullptr;
+  if (quads) {
+    const float4 av = 4 * sl < p.N ? *reinterpret_cast<const float4*>(ap) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 hv = hp != nullptr && 4 * sl < p.N ? *reinterpret_cast<const float4*>(hp) : make_float4(0.f, 0.f, 0.f, 0.f);
+    a[0] = av.x, a[1] = av.y, a[2] = av.z, a[3] = av.w;
+    h[0] = hv.x, h[1] = hv.y, h[2] = hv.z, h[3] = hv.w;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      a[k] = 4 * sl + k < p.N ? ap[k] : 0.f;
+      h[k] = hp != nullptr && 4 * sl + k < p.N ? hp[k] : 0.f;
+    }
+  }
+  const float bias = p.bias != nullptr ? p.bias[c] : 0.f, skip = p.D != nullptr ? p.D[c] : 0.f;
+  const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + c;
+  const T* dt = static_cast<const T*>(p.dt) + b * p.ds[0] + c;
+  const T* z = p.z != nullptr ? static_cast<const T*>(p.z) + b * p.zs[0] + c : nullptr;
+  const T* bm = static_cast<const T*>(p.b) + b * p.bs[0] + g * p.bs[2] + 4 * sl;
+  const T* cm = static_cast<const T*>(p.c) + b * p.cs[0] + g * p.cs[2] + 4 * sl;
+  T* y = static_cast<T*>(p.y) + b * p.T * p.C + c;
+  for (int t = 0; t < (int)p.T; ++t) {
+    const float xv = ld_as_float<T>(x, t * p.xs[1]);
+    float d = ld_as_float<T>(dt, t * p.ds[1]) + bias, sig;
+    const float zv = z != nullptr ? ld_as_float<T>(z, t * p.zs[1]) : 0.f;
+    float bv[4], cv[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const bool has = 4 * sl + k < p.N;
+      bv[k] = has ? ld_as_float<T>(bm, t * p.bs[1] + k) : 0.f;
+      cv[k] = has ? ld_as_float<T>(cm, t * p.cs[1] + k) : 0.f;
+    }
+    const bool start = p.starts != nullptr && p.starts[b * p.T + t] != 0;
+    if (p.softplus) d = softplus_of(d, sig);
+    const float u = d * xv;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[k] = fmaf(ex2(a[k] * LOG2E * d), start ? 0.f : h[k], u * bv[k]);
+      s = fmaf(h[k], cv[k], s);
+    }
+#pragma unroll
+    for (int o = 1; o < SL; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    s = fmaf(skip, xv, s);
+    if (z != nullptr) s *= act_of(zv, ACT_SILU);
+    if (live && sl == 0) st_from_float<T>(y, t * (int64_t)p.C, s);
+  }
+  if (!live) return;
+  float* out = p.state_out + (b * p.C + c) * p.N + 4 * sl;
+  if (quads) {
+    if (4 * sl < p.N) *reinterpret_cast<float4*>(out) = make_float4(h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (4 * sl + k < p.N) out[k] = h[k];
+  }
+}
+
+int sel_padded(int N) {
+  int n = SEL_EACH;
+  while (n < N) n *= 2;
+  return n;
+}
+SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd) {
+  const int NP = sel_padded(N), CH = NP <= 8 ? 128 : 1024 / NP, each = C / G;
+  SelCut k{};
+  k.channel_blocks = (each + CH - 1) / CH;
+  const int64_t blocks = B * G * k.channel_blocks, tiles = (T + SEL_TILE - 1) / SEL_TILE;
+  const int resident = bwd ? 2 : 4;
+  // As many segments as make the slowest SM's work least: tiles after one another, `resident` blocks of them for the price of about
+  // one and a half; the segments' own states cost about two thirds of the scan itself (backward: a third).
+  double least = 0.0;
+  k.nseg = 1;
+  for (int n = 1; n <= 64 && n <= tiles; ++n) {
+    const int64_t each_tiles = (tiles + n - 1) / n, total = blocks * ((tiles + each_tiles - 1) / each_tiles), per_sm = (total + 147) / 148;
+    const double rounds = (double)(per_sm / resident) * 1.0 + (per_sm % resident ? 0.6 + 0.4 * (per_sm % resident) / resident : 0.0);
+    const double cost = rounds * each_tiles * (n == 1 ? 1.0 : bwd ? 1.33 : 1.67) + (n == 1 ? 0.0 : 4.0 + 0.25 * n);
+    if (n > 1 && cost >= least) continue;
+    least = cost;
+    k.nseg = n;
+  }
+  k.seg_tiles = (int)((tiles + k.nseg - 1) / k.nseg);
+  k.nseg = (int)((tiles + k.seg_tiles - 1) / k.seg_tiles);
+  return k;
+}
+
+template <typename T, int NP, bool FULL>
+static cudaError_t run(const SelParams& p, int64_t blocks, cudaStream_t st) {
+  constexpr int bytes = sizeof(SelSmem<T, NP, FULL>);
+  if (bytes > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(ttt_selective_kernel<T, NP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+  }
+  ttt_selective_kernel<T, NP, FULL><<<(unsigned)blocks, SEL_THREADS, bytes, st>>>(p);
+  return cudaGetLastError();
+}
+template <typename T, int NP>
+static cudaError_t run_all(const SelParams& p, cudaStream_t st) {
+  const int each = p.C / p.G;
+  const int64_t blocks = p.B * p.G * ((each + SelShape<NP>::CH - 1) / SelShape<NP>::CH);
+  if (p.nseg > 1) {  // (the last segment's own state is nobody's)
+    const cudaError_t e = run<T, NP, false>(p, blocks * (p.nseg - 1), st);
+    if (e != cudaSuccess) return e;
+  }
+  return run<T, NP, true>(p, blocks * p.nseg, st);
+}
+template <typename T>
+static cudaError_t run_np(const SelParams& p, cudaStream_t st) {
+  switch (sel_padded(p.N)) {
+    case 4: return run_all<T, 4>(p, st);
+    case 8: return run_all<T, 8>(p, st);
+    case 16: return run_all<T, 16>(p, st);
+    case 32: return run_all<T, 32>(p, st);
+    default: return run_all<T, 64>(p, st);
+  }
+}
+cudaError_t launch_selective(int dtype, const SelParams& p, cudaStream_t st) {
+  return dtype == 1 ? run_np<__nv_bfloat16>(p, st) : run_np<float>(p, st);
+}
+template <typename T>
+static cudaError_t step_np(const SelParams& p, cudaStream_t st) {
+  const int SL = sel_padded(p.N) / SEL_EACH;
+  const unsigned blocks = (unsigned)((p.B * p.C * SL + SEL_THREADS - 1) / SEL_THREADS);
+  switch (SL) {
+    case 1: ttt_selective_step_kernel<T, 1><<<blocks, SEL_THREADS, 0, st>>>(p); break;
+    case 2: ttt_selective_step_kernel<T, 2><<<blocks, SEL_THREADS, 0, st>>>(p); break;
+    case 4: ttt_selective_step_kernel<T, 4><<<blocks, SEL_THREADS, 0, st>>>(p); break;
+    case 8: ttt_selective_step_kernel<T, 8><<<blocks, SEL_THREADS, 0, st>>>(p); break;
+    default: ttt_selective_step_kernel<T, 16><<<blocks, SEL_THREADS, 0, st>>>(p); break;
+  }
+  return cudaGetLastError();
+}
+cudaError_t launch_selective_step(int dtype, const SelParams& p, cudaStream_t st) {
+  return dtype == 1 ? step_np<__nv_bfloat16>(p, st) : step_np<float>(p, st);
+}
+
+}  // namespace ttt

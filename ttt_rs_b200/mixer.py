@@ -1,6 +1,6 @@
 """Operators of a layer that remembers through a selective state space scan, on [batch, seq_len, channels] with channels last:
-its short causal convolution (csrc/ttt_conv.cu) and the group norm with its gate (csrc/ttt_norm.cu).  (The reference has
-neither.)
+its short causal convolution (csrc/ttt_conv.cu), the scan (csrc/ttt_selective*.cu) and the group norm with its gate
+(csrc/ttt_norm.cu).  (The reference has none of them.)
 """
 
 from __future__ import annotations
@@ -41,6 +41,13 @@ def _rows(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def _dense(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return None if x is None else x.contiguous()
+
+
+def _aligned(x: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if x is None:
+        return None
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
 def _check_starts(starts: Optional[torch.Tensor], B: int, T: int, device):
@@ -91,6 +98,62 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     native = _lib.host().causal_conv(_rows(x), weight.contiguous(), _dense(bias), _dense(state), act, _dense(starts), state_out)
     if native is None:
         raise TttError(_lib.TTT_ERR_SHAPE, _lib.last_error() or "unsupported problem for the causal convolution")
+    return native
+
+
+def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, D: Optional[torch.Tensor] = None,
+                   z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+                   softplus: bool = True, starts: Optional[torch.Tensor] = None,
+                   state_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y [B,T,C], state behind the last token [B,C,N] float32) of the selective state space scan
+
+        d_t = softplus(dt_t + dt_bias),   h_t = exp(d_t A) h_{t-1} + d_t x_t B_t,   y_t = (<C_t, h_t> + D x_t) * SiLU(z_t)
+
+    for every channel, any number of tokens; without gradients a call of up to 16 tokens runs as a decode step.  x, dt and z (None: no
+    gate) [B,T,C], float32 or bfloat16, and B, C [B,T,G,N] or [B,T,N] (one group) of the same type, shared by the C / G neighbouring
+    channels of a group: strides that are not negative, with contiguous channels and states (columns of a projection are read where they
+    lie).  A [C,N], 1 to 64 states per channel, at most 0 for states that do not grow; D, dt_bias [C] (None: zeros); state [B,C,N], the
+    state before the first token (None: zeros): float32.  softplus=False: d_t = dt_t + dt_bias.  starts [B,T] (bool or uint8): such a token
+    finds a state of zero, so that sequences may follow one another in one row, or be padded on the left; nothing before it is seen, not
+    even a NaN.  The new state goes to `state_out` where given (it may be `state` itself but share nothing with another tensor; not
+    recorded for autograd, and refused where that asks for gradients).  Differentiable with respect to all nine, through both results,
+    once and not in forward mode.  Steps, decays, states and sums are float32, and results are rounded to bfloat16 once."""
+    one = isinstance(B, torch.Tensor) and isinstance(C, torch.Tensor) and B.dim() == 3 and C.dim() == 3
+    if one:
+        B, C = B.unsqueeze(2), C.unsqueeze(2)
+    native = _lib.host().selective(x, dt, A, B, C, D, z, dt_bias, state, starts, softplus, state_out)
+    if native is not None:
+        return native
+    _check_rows("x", x)
+    b, T, ch = x.shape
+    dev = x.device
+    _expect("dt", dt, x.shape, x.dtype, dev)
+    if B.dim() != 4 or ch % max(1, B.shape[2]) or B.numel() == 0:
+        raise TttError(_lib.TTT_ERR_SHAPE, f"B must be [batch, seq_len, groups, states] with groups that divide {ch} channels, got {tuple(B.shape)}")
+    G, N = B.shape[2:]
+    if N > 64:
+        raise TttError(_lib.TTT_ERR_UNSUPPORTED, f"Unsupported states={N} (supported: 1..64)")
+    _expect("B", B, (b, T, G, N), x.dtype, dev)
+    _expect("C", C, (b, T, G, N), x.dtype, dev)
+    _expect("A", A, (ch, N), torch.float32, dev)
+    for name, t in (("D", D), ("dt_bias", dt_bias)):
+        if t is not None:
+            _expect(name, t, (ch,), torch.float32, dev)
+    if z is not None:
+        _expect("z", z, x.shape, x.dtype, dev)
+    if state is not None:
+        _expect("state", state, (b, ch, N), torch.float32, dev)
+    _check_starts(starts, b, T, dev)
+    _check_state_out(state_out, (b, ch, N), torch.float32, dev, x, dt, A, B, C, D, z, dt_bias, state)
+    if state_out is not None and state_out.data_ptr() % 16:
+        raise TttError(_lib.TTT_ERR_ALIGN, "state_out is not 16-byte aligned")
+
+    def states(t):
+        return t if t.stride(3) == 1 or N == 1 else t.contiguous()
+    native = _lib.host().selective(_rows(x), _rows(dt), _aligned(A), states(B), states(C), _dense(D), _rows(z), _dense(dt_bias), _aligned(state),
+                                   _dense(starts), softplus, state_out)
+    if native is None:
+        raise TttError(_lib.TTT_ERR_SHAPE, _lib.last_error() or "unsupported problem for the selective scan")
     return native
 
 

@@ -390,12 +390,13 @@ extern "C" int ttt_linear_selective_forward(int64_t batch, int64_t seq_len, int6
     int64_t bytes;
   } others[] = {{"x", x, s.bytes(p.xs)}, {"dt", dt, s.bytes(p.ds)}, {"z", z, s.bytes(p.zs)}, {"a", a, d.C * d.N * 4}, {"d", d_skip, d.C * 4},
                 {"dt_bias", dt_bias, d.C * 4}, {"b", b, m.bytes(bb) + p.bs[2] * (d.G - 1) * d.es}, {"c", c, m.bytes(cb) + p.cs[2] * (d.G - 1) * d.es},
-                {"starts", starts, d.B * d.T}, {"y", y, n}};
+                {"starts", starts, d.B * d.T}};
   for (const auto& o : others) {
     if ((rc = check_apart("state_out", state_out, held, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
-    if (o.p != y && (rc = check_apart("y", y, n, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
+    if ((rc = check_apart("y", y, n, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
   }
-  if ((rc = check_apart("state_out", state_out, held, "state", state, held, true)) != TTT_OK ||
+  if ((rc = check_apart("state_out", state_out, held, "y", y, n, false)) != TTT_OK ||
+      (rc = check_apart("state_out", state_out, held, "state", state, held, true)) != TTT_OK ||
       (rc = check_apart("y", y, n, "state", state, held, false)) != TTT_OK)
     return rc;
   p.softplus = softplus != 0;

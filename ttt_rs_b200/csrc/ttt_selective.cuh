@@ -6,8 +6,9 @@
 //
 // What bounds it is exponentials: one per state, channel and token, 16 per SM and clock, where memory would allow twice as many at
 // N = 16.  A thread holds SEL_EACH states of SEL_CH neighbouring channels (1 where N <= 4); NP / SEL_EACH lanes share a channel.
-// Tiles of SEL_TILE tokens are copied ahead (cp.async), turned into (step, step times x) pairs in float32 in shared memory, scanned
-// token by token, and written by pairs of channels.
+// Four warps of a block scan; four others (SEL_THREADS each) do what is done once per token and channel: they copy tiles of SEL_TILE
+// tokens ahead (cp.async), turn them into (step, step times x) pairs in float32 in shared memory a tile before the scan, and write the
+// results a tile behind it, so that the two kinds of work hide one another's latency.  One barrier of the block per tile.
 #pragma once
 
 #include "ttt_kernels.h"
@@ -15,9 +16,9 @@
 
 namespace ttt {
 
-constexpr int SEL_THREADS = 128;
+constexpr int SEL_THREADS = 128;  // of each kind
+constexpr int SEL_STAGES = 3;     // tiles of inputs in shared memory
 constexpr int SEL_EACH = 4;  // states per thread
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 template <int NP>
 struct SelShape {
@@ -31,26 +32,20 @@ struct SelShape {
   static constexpr int PITCH = CH + 16;            // floats between tokens of results: two tokens' channels in different banks
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ F2 ex2(F2 x) { return f2(ex2(x.x), ex2(x.y)); }
-
-// log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1], by log(1 + e) = 2 artanh(s), s = e / (2 + e) <= 1/3: terms up
-// to s^15 leave 2^-27 of it.  sig: 1 / (1 + exp(-v)).
-__device__ __forceinline__ float softplus_of(float v, float& sig) {
-  const float e = __expf(-fabsf(v)), s = __fdividef(e, 2.f + e), q = s * s;
-  float r = fmaf(q, 1.f / 15.f, 1.f / 13.f);
-  r = fmaf(q, r, 1.f / 11.f);
-  r = fmaf(q, r, 1.f / 9.f);
-  r = fmaf(q, r, 1.f / 7.f);
-  r = fmaf(q, r, 1.f / 5.f);
-  r = fmaf(q, r, 1.f / 3.f);
-  r = fmaf(q * s, r, s);
-  sig = __fdividef(v >= 0.f ? 1.f : e, 1.f + e);
-  return v != v ? v : fmaf(2.f, r, fmaxf(v, 0.f));
+// log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1].  log(1 + e) / e is a polynomial of degree 8, fitted on [0, 1] for
+// the least largest relative error (3.0e-8): accurate relative to small steps too, which a logarithm of 1 + e is not, and without a
+// quotient, whose place among the exponentials it would take.  Two channels at once; a NaN stays one.
+__device__ __forceinline__ F2 softplus_of(F2 v) {
+  const F2 e = f2(ex2(-LOG2E * fabsf(v.x)), ex2(-LOG2E * fabsf(v.y)));
+  F2 r = f2fma(e, f2(0.005232690833508968f), f2(-0.029505228623747826f));
+  r = f2fma(e, r, f2(0.07822594791650772f));
+  r = f2fma(e, r, f2(-0.13663245737552643f));
+  r = f2fma(e, r, f2(0.19106008112430573f));
+  r = f2fma(e, r, f2(-0.2484298199415207f));
+  r = f2fma(e, r, f2(0.3331909775733948f));
+  r = f2fma(e, r, f2(-0.4999949336051941f));
+  r = f2fma(e, r, f2(0.9999999403953552f));
+  return f2fma(e, r, f2(v.x < 0.f ? 0.f : v.x, v.y < 0.f ? 0.f : v.y));
 }
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src, bool live) {
@@ -60,29 +55,31 @@ __device__ __forceinline__ void copy_async4(void* dst, const void* src, bool liv
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// the block's threads that do not scan
+__device__ __forceinline__ void helpers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SEL_THREADS) : "memory"); }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // rows [t0, t0 + SEL_TILE) of `have` elements, at most WIDE, into dst [SEL_TILE][WIDE]; zeros beyond T and `have`.  bytes: 16, 4, or an
 // element's size, what addresses, strides and `have` are multiples of.
 template <typename T, int WIDE>
-__device__ __forceinline__ void copy_rows(T* dst, const T* src, int64_t stride, int64_t t0, int64_t t_end, int have, int bytes) {
+__device__ __forceinline__ void copy_rows(int tid, T* dst, const T* src, int64_t stride, int64_t t0, int64_t t_end, int have, int bytes) {
   constexpr int V16 = 16 / sizeof(T);
   if (WIDE >= V16 && bytes == 16) {
     constexpr int V = WIDE >= V16 ? V16 : 1, PER = WIDE / V;
-    for (int i = threadIdx.x; i < SEL_TILE * PER; i += SEL_THREADS) {
+    for (int i = tid; i < SEL_TILE * PER; i += SEL_THREADS) {
       const int r = i / PER, e = (i - r * PER) * V;
       const bool live = t0 + r < t_end && e < have;
       copy_async16(dst + r * WIDE + e, live ? src + (t0 + r) * stride + e : src, live);
     }
   } else if (bytes >= 4) {
     constexpr int V = 4 / sizeof(T), PER = WIDE / V;
-    for (int i = threadIdx.x; i < SEL_TILE * PER; i += SEL_THREADS) {
+    for (int i = tid; i < SEL_TILE * PER; i += SEL_THREADS) {
       const int r = i / PER, e = (i - r * PER) * V;
       const bool live = t0 + r < t_end && e < have;
       copy_async4(dst + r * WIDE + e, live ? src + (t0 + r) * stride + e : src, live);
     }
   } else {
-    for (int i = threadIdx.x; i < SEL_TILE * WIDE; i += SEL_THREADS) {
+    for (int i = tid; i < SEL_TILE * WIDE; i += SEL_THREADS) {
       const int r = i / WIDE, e = i - r * WIDE;
       dst[i] = t0 + r < t_end && e < have ? src[(t0 + r) * stride + e] : T(0.f);
     }

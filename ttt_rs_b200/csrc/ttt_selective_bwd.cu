@@ -41,13 +41,13 @@ __global__ void __launch_bounds__(SEL_THREADS, FULL ? 2 : 4) ttt_selective_bwd_k
   const uint8_t* starts = MARKS ? p.starts + at.b * p.T : nullptr;
   const int64_t tiles = (p.T + SEL_TILE - 1) / SEL_TILE;
   auto fetch = [&](int64_t t0, int k) {
-    copy_rows<T, S::CH>(&sm.raw[k][0][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(&sm.raw[k][1][0][0], gy, p.gs[1], t0, at.t_hi, at.have, p.xg);
-    if (z != nullptr) copy_rows<T, S::CH>(&sm.raw[k][2][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, NP>(&sm.raw_bc[k][0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
+    copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][0][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][1][0][0], gy, p.gs[1], t0, at.t_hi, at.have, p.xg);
+    if (z != nullptr) copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][2][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP>(threadIdx.x, &sm.raw_bc[k][0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
     if constexpr (FULL) {
-      copy_rows<T, S::CH>(&sm.raw[k][FULL ? 3 : 0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
-      copy_rows<T, NP>(&sm.raw_bc[k][FULL ? 1 : 0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
+      copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][FULL ? 3 : 0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
+      copy_rows<T, NP>(threadIdx.x, &sm.raw_bc[k][FULL ? 1 : 0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
     }
     copy_commit();
   };
@@ -109,11 +109,8 @@ __global__ void __launch_bounds__(SEL_THREADS, FULL ? 2 : 4) ttt_selective_bwd_k
     for (int r = row0; r < SEL_TILE; r += S::ROWS) {
       const float2 dv = pair_of(&sm.raw[buf][0][r][2 * pr]);
       float2 gv = pair_of(&sm.raw[buf][1][r][2 * pr]);
-      float2 d = make_float2(dv.x + bias.x, dv.y + bias.y);
-      if (p.softplus) {
-        float sig;
-        d.x = softplus_of(d.x, sig), d.y = softplus_of(d.y, sig);
-      }
+      F2 d = f2add(dv, bias);
+      if (p.softplus) d = softplus_of(d);
       if (t0 + r >= at.t_hi || pair_have < 1) d.x = 0.f;
       if (t0 + r >= at.t_hi || pair_have < 2) d.y = 0.f;
       if (z != nullptr) {
@@ -239,7 +236,7 @@ __global__ void __launch_bounds__(SEL_THREADS, FULL ? 2 : 4) ttt_selective_bwd_k
         const float2 in = *reinterpret_cast<const float2*>(&sm.res[0][r][2 * pr]), ra = *reinterpret_cast<const float2*>(&sm.res[1][r][2 * pr]);
         const float4 q = sm.du[r][pr];
         float2 sig = make_float2(1.f, 1.f);
-        if (p.softplus) softplus_of(dv.x + bias.x, sig.x), softplus_of(dv.y + bias.y, sig.y);
+        if (p.softplus) sig = make_float2(sigmoid_of(dv.x + bias.x), sigmoid_of(dv.y + bias.y));
         const float2 dx = make_float2(fmaf(skip.x, gv.x, q.x * in.x), fmaf(skip.y, gv.y, q.z * in.y));
         const float2 dd = make_float2(fmaf(LN2, ra.x, in.x * xv.x) * sig.x, fmaf(LN2, ra.y, in.y * xv.y) * sig.y);
         s0.x = fmaf(gv.x, xv.x, s0.x), s0.y = fmaf(gv.y, xv.y, s0.y);

@@ -11,69 +11,127 @@ template <typename T, int NP, bool FULL>
 struct SelSmem {
   using S = SelShape<NP>;
   static constexpr int TENSORS = FULL ? 3 : 2;
-  alignas(16) T raw[2][TENSORS][SEL_TILE][S::CH];       // x, dt, z
-  alignas(16) T raw_bc[2][FULL ? 2 : 1][SEL_TILE][NP];
-  alignas(16) float4 du[SEL_TILE][S::PAIRS];            // (step, step x) of two channels
-  alignas(16) float bc[FULL ? 2 : 1][SEL_TILE][NP];
-  alignas(16) float y[FULL ? SEL_TILE : 1][S::PITCH];
+  alignas(16) T raw[SEL_STAGES][TENSORS][SEL_TILE][S::CH];  // x, dt, z
+  alignas(16) T raw_bc[SEL_STAGES][FULL ? 2 : 1][SEL_TILE][NP];
+  alignas(16) float4 du[2][SEL_TILE][S::PAIRS];             // (step, step x) of two channels
+  alignas(16) float bc[2][FULL ? 2 : 1][SEL_TILE][NP];
+  alignas(16) float y[2][FULL ? SEL_TILE : 1][S::SL * S::CH];  // shares of a result, as the scanning lanes lie
+  uint32_t mark[2];                                         // starts of a tile, bit by bit
 };
 
-template <typename T, int NP, bool FULL>
-__global__ void __launch_bounds__(SEL_THREADS) ttt_selective_kernel(const SelParams p) {
+// FULL false: a segment's own state, from zero, and its sum of steps.  MARKS: there are starts (else the kernel knows none).
+template <typename T, int NP, bool FULL, bool MARKS>
+__global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const SelParams p) {
   using S = SelShape<NP>;
   using Smem = SelSmem<T, NP, FULL>;
   extern __shared__ __align__(16) unsigned char sel_smem[];
   Smem& sm = *reinterpret_cast<Smem*>(sel_smem);
   const SelPlace<NP> at(p, 0, FULL ? p.nseg : p.nseg - 1);
-  const SelLane<NP> me;
+  const int tiles = (int)((at.t_hi - at.t_lo + SEL_TILE - 1) / SEL_TILE);
+  if (threadIdx.x < SEL_THREADS) {
+    // ---- scan
+    const SelLane<NP> me;
+    F2 A[S::CC][2], h[S::CC][2];
+    me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k) A[k][0] = f2mul(A[k][0], f2(LOG2E)), A[k][1] = f2mul(A[k][1], f2(LOG2E));
+    if constexpr (FULL) {
+      if (p.nseg == 1) me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
+      else me.load_padded(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, at.have);
+      for (int j = 0; j < at.seg; ++j) {  // the segments before, in their order
+        const int64_t row = (at.b * p.nseg + j) * p.C + at.c0;
+        F2 own[S::CC][2];
+        me.load_padded(own, p.seg_state + row * NP, at.have);
+#pragma unroll
+        for (int k = 0; k < S::CC; ++k) {
+          const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
+          const bool cut = sum == INFINITY;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) h[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), h[k][i], own[k][i]);
+        }
+      }
+    } else {
+      // (the given state may be where the new one goes, which other blocks of the scan write: the scan reads it from here)
+      if (at.seg == 0) {
+        me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
+        me.store(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, NP, at.have);
+      }
+#pragma unroll
+      for (int k = 0; k < S::CC; ++k) h[k][0] = h[k][1] = f2(0.f);
+    }
+    float* saved = nullptr;
+    if (FULL && p.saved != nullptr) saved = p.saved + ((at.b * ((p.T + SEL_TILE - 1) / SEL_TILE) + at.t_lo / SEL_TILE) * p.C + at.c0) * NP;
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      if (saved != nullptr) {
+        me.store(h, saved, NP, at.have);
+        saved += (int64_t)p.C * NP;
+      }
+      const uint32_t mark = MARKS ? sm.mark[i & 1] : 0;
+#pragma unroll 8
+      for (int r = 0; r < SEL_TILE; ++r) {
+        float4 q;
+        if constexpr (S::CC == 2) {
+          q = sm.du[i & 1][r][me.ch / 2];
+        } else {
+          const float2 one = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(&sm.du[i & 1][r][0]) + 2 * me.ch);
+          q = make_float4(one.x, one.y, 0.f, 0.f);
+        }
+        const float4 b = *reinterpret_cast<const float4*>(&sm.bc[i & 1][0][r][4 * me.sl]);
+        if (MARKS && mark >> r & 1) {
+#pragma unroll
+          for (int k = 0; k < S::CC; ++k) h[k][0] = h[k][1] = f2(0.f);
+        }
+        [[maybe_unused]] float4 c;
+        [[maybe_unused]] float part[2];
+        if constexpr (FULL) c = *reinterpret_cast<const float4*>(&sm.bc[i & 1][FULL ? 1 : 0][r][4 * me.sl]);
+#pragma unroll
+        for (int k = 0; k < S::CC; ++k) {
+          const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
+          h[k][0] = f2fma(ex2(f2mul(A[k][0], d)), h[k][0], f2mul(v, f2(b.x, b.y)));
+          h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
+          if constexpr (FULL) part[k] = f2hsum(f2fma(h[k][0], f2(c.x, c.y), f2mul(h[k][1], f2(c.z, c.w))));
+        }
+        if constexpr (FULL) {  // [pair][lane of its channels][channel]
+          if constexpr (S::CC == 2) *reinterpret_cast<float2*>(&sm.y[i & 1][r][2 * threadIdx.x]) = make_float2(part[0], part[1]);
+          else sm.y[i & 1][r][threadIdx.x] = part[0];
+        }
+      }
+      __syncthreads();
+    }
+    if constexpr (FULL) {
+      if (at.t_hi == p.T) me.store(h, p.state_out + (at.b * p.C + at.c0) * p.N, p.N, at.have);
+    } else {
+      me.store(h, p.seg_state + ((at.b * p.nseg + at.seg) * p.C + at.c0) * NP, NP, at.have);
+    }
+    return;
+  }
+  // ---- what is done once per token and channel, pair of channels by pair
+  const int tid = threadIdx.x - SEL_THREADS, pr = tid % S::PAIRS, row0 = tid / S::PAIRS, pair_have = at.have - 2 * pr;
   const T* x = static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c0;
   const T* dt = static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0;
   const T* z = FULL && p.z != nullptr ? static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0 : nullptr;
   const T* bm = static_cast<const T*>(p.b) + at.b * p.bs[0] + at.g * p.bs[2];
   const T* cm = static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2];
-  const uint8_t* starts = p.starts != nullptr ? p.starts + at.b * p.T : nullptr;
-  auto fetch = [&](int64_t t0, int k) {
-    copy_rows<T, S::CH>(&sm.raw[k][0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(&sm.raw[k][1][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, NP>(&sm.raw_bc[k][0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
+  const uint8_t* starts = MARKS ? p.starts + at.b * p.T : nullptr;
+  bool first[2] = {false, false};  // lane r of a warp: a start at token r of the next tile to be made ready, and of the one behind it
+  bool any_start = false;
+  auto fetch = [&](int i) {
+    const int k = i % SEL_STAGES;
+    const int64_t t0 = at.t_lo + (int64_t)i * SEL_TILE;
+    copy_rows<T, S::CH>(tid, &sm.raw[k][0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH>(tid, &sm.raw[k][1][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP>(tid, &sm.raw_bc[k][0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
     if constexpr (FULL) {
-      if (z != nullptr) copy_rows<T, S::CH>(&sm.raw[k][Smem::TENSORS - 1][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
-      copy_rows<T, NP>(&sm.raw_bc[k][FULL ? 1 : 0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
+      if (z != nullptr) copy_rows<T, S::CH>(tid, &sm.raw[k][Smem::TENSORS - 1][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
+      copy_rows<T, NP>(tid, &sm.raw_bc[k][FULL ? 1 : 0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
     }
     copy_commit();
+    if constexpr (MARKS) {
+      const int64_t t = t0 + (tid & 31);
+      first[1] = (tid & 31) < SEL_TILE && t < at.t_hi && starts[t] != 0;
+    }
   };
-  fetch(at.t_lo, 0);
-
-  F2 A[S::CC][2], h[S::CC][2];
-  me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
-#pragma unroll
-  for (int k = 0; k < S::CC; ++k) A[k][0] = f2mul(A[k][0], f2(LOG2E)), A[k][1] = f2mul(A[k][1], f2(LOG2E));
-  if constexpr (FULL) {
-    if (p.nseg == 1) me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
-    else me.load_padded(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, at.have);
-    for (int j = 0; j < at.seg; ++j) {  // the segments before, in their order
-      const int64_t row = (at.b * p.nseg + j) * p.C + at.c0;
-      F2 own[S::CC][2];
-      me.load_padded(own, p.seg_state + row * NP, at.have);
-#pragma unroll
-      for (int k = 0; k < S::CC; ++k) {
-        const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
-        const bool cut = sum == INFINITY;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) h[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), h[k][i], own[k][i]);
-      }
-    }
-  } else {
-    // (the given state may be where the new one goes, which other blocks of the scan write: the scan reads it from here)
-    if (at.seg == 0) {
-      me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
-      me.store(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, NP, at.have);
-    }
-#pragma unroll
-    for (int k = 0; k < S::CC; ++k) h[k][0] = h[k][1] = f2(0.f);
-  }
-  // what an element-wise thread keeps: a pair of channels
-  const int pr = threadIdx.x % S::PAIRS, row0 = threadIdx.x / S::PAIRS, pair_have = at.have - 2 * pr;
   float2 bias = make_float2(0.f, 0.f), skip = make_float2(0.f, 0.f);
   if (p.bias != nullptr) {
     if (pair_have > 0) bias.x = p.bias[at.c0 + 2 * pr];
@@ -84,105 +142,78 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_kernel(const SelPar
     if (pair_have > 1) skip.y = p.D[at.c0 + 2 * pr + 1];
   }
   const bool whole = pair_have > 1 && p.xg >= 4 && (sizeof(T) == 2 || p.xg == 16);
-  float sum[2] = {0.f, 0.f};  // (FULL false: of the pair's steps over this thread's tokens)
-  bool any_start = false;
-
-  int buf = 0;
-  for (int64_t t0 = at.t_lo; t0 < at.t_hi; t0 += SEL_TILE, buf ^= 1) {
-    uint32_t mark = 0;
-    if (starts != nullptr) {
-      const int64_t t = t0 + (me.lane & (SEL_TILE - 1));
-      mark = __ballot_sync(0xffffffffu, t < at.t_hi && starts[t] != 0) & ((1u << SEL_TILE) - 1);
-      any_start = any_start || mark != 0;
-    }
-    copy_wait_all();
-    __syncthreads();
-    if (t0 + SEL_TILE < at.t_hi) fetch(t0 + SEL_TILE, buf ^ 1);
+  float2 sum = make_float2(0.f, 0.f);  // (FULL false: of the pair's steps over this thread's tokens)
+  auto make_ready = [&](int i) {
+    const int k = i % SEL_STAGES, left = (int)(at.t_hi - at.t_lo) - i * SEL_TILE;
 #pragma unroll
     for (int r = row0; r < SEL_TILE; r += S::ROWS) {
-      const float2 xv = pair_of(&sm.raw[buf][0][r][2 * pr]), dv = pair_of(&sm.raw[buf][1][r][2 * pr]);
-      float2 d = make_float2(dv.x + bias.x, dv.y + bias.y);
-      if (p.softplus) {
-        float sig;
-        d.x = softplus_of(d.x, sig), d.y = softplus_of(d.y, sig);
-      }
-      if (t0 + r >= at.t_hi || pair_have < 1) d.x = 0.f;
-      if (t0 + r >= at.t_hi || pair_have < 2) d.y = 0.f;
-      sm.du[r][pr] = make_float4(d.x, d.x * xv.x, d.y, d.y * xv.y);
-      if (!FULL) sum[0] += d.x, sum[1] += d.y;
+      const float2 xv = pair_of(&sm.raw[k][0][r][2 * pr]), dv = pair_of(&sm.raw[k][1][r][2 * pr]);
+      F2 d = f2add(dv, bias);
+      if (p.softplus) d = softplus_of(d);
+      if (r >= left || pair_have < 1) d.x = 0.f;
+      if (r >= left || pair_have < 2) d.y = 0.f;
+      sm.du[i & 1][r][pr] = make_float4(d.x, d.x * xv.x, d.y, d.y * xv.y);
+      if (!FULL) sum = f2add(sum, d);
     }
 #pragma unroll
-    for (int i = threadIdx.x; i < (FULL ? 2 : 1) * SEL_TILE * NP; i += SEL_THREADS)
-      (&sm.bc[0][0][0])[i] = ld_as_float<T>(&sm.raw_bc[buf][0][0][0], i);
-    if (FULL && p.saved != nullptr)
-      me.store(h, p.saved + ((at.b * ((p.T + SEL_TILE - 1) / SEL_TILE) + t0 / SEL_TILE) * p.C + at.c0) * NP, NP, at.have);
+    for (int e = tid; e < (FULL ? 2 : 1) * SEL_TILE * NP; e += SEL_THREADS)
+      (&sm.bc[i & 1][0][0][0])[e] = ld_as_float<T>(&sm.raw_bc[k][0][0][0], e);
+    if constexpr (MARKS) {
+      const uint32_t mark = __ballot_sync(0xffffffffu, first[0]);
+      if (tid == 0) sm.mark[i & 1] = mark;
+      any_start = any_start || mark != 0;
+      first[0] = first[1];
+    }
+  };
+  auto finish = [&](int i) {
+    const int k = i % SEL_STAGES, left = (int)(at.t_hi - at.t_lo) - i * SEL_TILE;
+    if (pair_have < 1) return;
+    T* y = static_cast<T*>(p.y) + (at.b * p.T + at.t_lo + (int64_t)i * SEL_TILE + row0) * p.C + at.c0 + 2 * pr;
+#pragma unroll
+    for (int r = row0; r < SEL_TILE; r += S::ROWS, y += (int64_t)S::ROWS * p.C) {
+      if (r >= left) break;
+      F2 v = f2(0.f);
+      if constexpr (S::CC == 2) {
+#pragma unroll
+        for (int l = 0; l < S::SL; ++l) v = f2add(v, *reinterpret_cast<const float2*>(&sm.y[i & 1][r][2 * (pr * S::SL + l)]));
+      } else {
+        v = *reinterpret_cast<const float2*>(&sm.y[i & 1][r][2 * pr]);
+      }
+      v = f2fma(skip, pair_of(&sm.raw[k][0][r][2 * pr]), v);
+      if (z != nullptr) {
+        const float2 zv = pair_of(&sm.raw[k][Smem::TENSORS - 1][r][2 * pr]);
+        v = f2mul(v, f2(act_of(zv.x, ACT_SILU), act_of(zv.y, ACT_SILU)));
+      }
+      put_pair<T>(y, v, pair_have, whole);
+    }
+  };
+  fetch(0);
+  first[0] = first[1];
+  if (tiles > 1) fetch(1);
+  copy_wait_all();
+  helpers_sync();
+  make_ready(0);
+  __syncthreads();
+  for (int i = 0; i < tiles; ++i) {
+    if (FULL && i > 0) finish(i - 1);
+    copy_wait_all();
+    helpers_sync();  // the copies of tile i + 1 are everybody's, and nobody reads tile i - 1 any more
+    if (i + 2 < tiles) fetch(i + 2);
+    if (i + 1 < tiles) make_ready(i + 1);
     __syncthreads();
-    constexpr int DEAL = S::SL > S::CC ? S::SL : S::CC, TOKENS = DEAL / S::CC;  // results dealt to the lanes of a channel
-#pragma unroll 4
-    for (int r0 = 0; r0 < SEL_TILE; r0 += TOKENS) {
-      float part[DEAL];
-#pragma unroll
-      for (int u = 0; u < TOKENS; ++u) {
-        const int r = r0 + u;
-        float4 q;
-        if constexpr (S::CC == 2) {
-          q = sm.du[r][me.ch / 2];
-        } else {
-          const float2 one = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(&sm.du[r][0]) + 2 * me.ch);
-          q = make_float4(one.x, one.y, 0.f, 0.f);
-        }
-        const float4 b = *reinterpret_cast<const float4*>(&sm.bc[0][r][4 * me.sl]);
-        if (mark >> r & 1) {
-#pragma unroll
-          for (int k = 0; k < S::CC; ++k) h[k][0] = h[k][1] = f2(0.f);
-        }
-        [[maybe_unused]] float4 c;
-        if constexpr (FULL) c = *reinterpret_cast<const float4*>(&sm.bc[FULL ? 1 : 0][r][4 * me.sl]);
-#pragma unroll
-        for (int k = 0; k < S::CC; ++k) {
-          const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
-          h[k][0] = f2fma(ex2(f2mul(A[k][0], d)), h[k][0], f2mul(v, f2(b.x, b.y)));
-          h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
-          if constexpr (FULL) part[u * S::CC + k] = f2hsum(f2fma(h[k][0], f2(c.x, c.y), f2mul(h[k][1], f2(c.z, c.w))));
-        }
-      }
-      if constexpr (FULL) {
-        sum_and_deal<DEAL, S::SL, 1>(part, me.lane);
-        // lane sl has result sl: channel sl % CC of token sl / CC (N <= 4: its only one)
-        if constexpr (S::SL == 1) sm.y[r0][me.ch] = part[0];
-        else sm.y[r0 + me.sl / S::CC][me.ch + me.sl % S::CC] = part[0];
-      }
-    }
-    if constexpr (FULL) {
-      __syncthreads();
-#pragma unroll
-      for (int r = row0; r < SEL_TILE; r += S::ROWS) {
-        if (t0 + r >= at.t_hi || pair_have < 1) continue;
-        const float2 xv = pair_of(&sm.raw[buf][0][r][2 * pr]);
-        float2 v = *reinterpret_cast<const float2*>(&sm.y[r][2 * pr]);
-        v.x = fmaf(skip.x, xv.x, v.x), v.y = fmaf(skip.y, xv.y, v.y);
-        if (z != nullptr) {
-          const float2 zv = pair_of(&sm.raw[buf][Smem::TENSORS - 1][r][2 * pr]);
-          v.x *= act_of(zv.x, ACT_SILU), v.y *= act_of(zv.y, ACT_SILU);
-        }
-        put_pair<T>(static_cast<T*>(p.y) + (at.b * p.T + t0 + r) * p.C + at.c0 + 2 * pr, v, pair_have, whole);
-      }
-    }
   }
   if constexpr (FULL) {
-    if (at.t_hi == p.T) me.store(h, p.state_out + (at.b * p.C + at.c0) * p.N, p.N, at.have);
+    finish(tiles - 1);
   } else {
-    const int64_t row = (at.b * p.nseg + at.seg) * p.C + at.c0;
-    me.store(h, p.seg_state + row * NP, NP, at.have);
-    __syncthreads();
-    float* sums = reinterpret_cast<float*>(&sm.du[0][0]);  // [ROWS][CH]
-    sums[row0 * S::CH + 2 * pr] = sum[0];
-    sums[row0 * S::CH + 2 * pr + 1] = sum[1];
-    __syncthreads();
-    for (int c = threadIdx.x; c < at.have; c += SEL_THREADS) {
+    float* sums = reinterpret_cast<float*>(&sm.du[0][0][0]);  // [ROWS][CH]
+    helpers_sync();
+    sums[row0 * S::CH + 2 * pr] = sum.x;
+    sums[row0 * S::CH + 2 * pr + 1] = sum.y;
+    helpers_sync();
+    for (int c = tid; c < at.have; c += SEL_THREADS) {
       float v = 0.f;
       for (int r = 0; r < S::ROWS; ++r) v += sums[r * S::CH + c];
-      p.seg_sum[row + c] = any_start ? INFINITY : v;
+      p.seg_sum[(at.b * p.nseg + at.seg) * p.C + at.c0 + c] = any_start ? INFINITY : v;
     }
   }
 }
@@ -222,7 +253,7 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_step_kernel(const S
   T* y = static_cast<T*>(p.y) + b * p.T * p.C + c;
   for (int t = 0; t < (int)p.T; ++t) {
     const float xv = ld_as_float<T>(x, t * p.xs[1]);
-    float d = ld_as_float<T>(dt, t * p.ds[1]) + bias, sig;
+    float d = ld_as_float<T>(dt, t * p.ds[1]) + bias;
     const float zv = z != nullptr ? ld_as_float<T>(z, t * p.zs[1]) : 0.f;
     float bv[4], cv[4];
 #pragma unroll
@@ -232,7 +263,7 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_step_kernel(const S
       cv[k] = has ? ld_as_float<T>(cm, t * p.cs[1] + k) : 0.f;
     }
     const bool start = p.starts != nullptr && p.starts[b * p.T + t] != 0;
-    if (p.softplus) d = softplus_of(d, sig);
+    if (p.softplus) d = softplus_of(f2(d)).x;
     const float u = d * xv;
     float s = 0.f;
 #pragma unroll
@@ -288,11 +319,12 @@ SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd) {
 template <typename T, int NP, bool FULL>
 static cudaError_t run(const SelParams& p, int64_t blocks, cudaStream_t st) {
   constexpr int bytes = sizeof(SelSmem<T, NP, FULL>);
+  void (*kernel)(SelParams) = p.starts != nullptr ? ttt_selective_kernel<T, NP, FULL, true> : ttt_selective_kernel<T, NP, FULL, false>;
   if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(ttt_selective_kernel<T, NP, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
   }
-  ttt_selective_kernel<T, NP, FULL><<<(unsigned)blocks, SEL_THREADS, bytes, st>>>(p);
+  kernel<<<(unsigned)blocks, 2 * SEL_THREADS, bytes, st>>>(p);
   return cudaGetLastError();
 }
 template <typename T, int NP>

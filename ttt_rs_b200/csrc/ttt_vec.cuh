@@ -62,9 +62,22 @@ struct Chan {
   }
 };
 
-// Activations and their derivatives.  The quotients are approximate (2 units in the last place); 1 + exp(-v) beyond 2^126 gives 0,
-// as the limit is.
-__device__ __forceinline__ float sigmoid_of(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// 2^x and 1 / x, approximate (2 and 1 units in the last place), results below 2^-126 as zero
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ F2 ex2(F2 x) { return f2(ex2(x.x), ex2(x.y)); }
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// Activations and their derivatives.  (1 + exp(-v) that overflows has a reciprocal of 0, as the limit is.)
+__device__ __forceinline__ float sigmoid_of(float v) { return rcp(1.f + ex2(-LOG2E * v)); }
 __device__ __forceinline__ float act_of(float v, int act) {
   if (act == ACT_SILU) return v * sigmoid_of(v);
   if (act == ACT_GELU) {

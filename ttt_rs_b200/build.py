@@ -30,7 +30,7 @@ NVCC_FLAGS = [
 ]
 # Kernels whose groups of warps split the launch's registers among themselves (setmaxnreg): registers per thread that the
 # splits add up to.  With fewer at launch a group would wait for registers that do not exist.
-REGISTER_SPLITS = {"ttt_linear_bwd_f32.cu": ("ttt_linear_bwd_f32_kernel", 128)}
+REGISTER_SPLITS = {"ttt_linear_bwd_f32.cu": ("ttt_linear_bwd_f32_kernel", 128), "ttt_selective_bwd.cu": ("ttt_selective_bwd_kernel", 128)}
 
 
 def check_register_split(src: str, log: str) -> None:

@@ -11,174 +11,127 @@
 
 namespace ttt {
 
-template <typename T, int NP, bool FULL>
+template <typename T, int NP>
 struct SelBwdSmem {
   using S = SelShape<NP>;
-  alignas(16) T raw[2][FULL ? 4 : 3][SEL_TILE][S::CH];  // dt, gradient of y, z, x
-  alignas(16) T raw_bc[2][FULL ? 2 : 1][SEL_TILE][NP];  // c, b
-  alignas(16) float4 du[SEL_TILE][S::PAIRS];            // (step, step x) of two channels
-  alignas(16) float g[SEL_TILE][S::CH];
-  alignas(16) float bc[FULL ? 2 : 1][SEL_TILE][NP];     // c, b
-  alignas(16) float res[FULL ? 3 : 1][FULL ? SEL_TILE : 1][S::PITCH];  // <dh, B>, <e, A log2 e>, <C, h>
-  alignas(16) float part[FULL ? SEL_THREADS / 32 : 1][FULL ? SEL_TILE : 1][2 * NP];  // dB, dC
+  alignas(16) T raw[SEL_STAGES][4][SEL_TILE][S::CH];    // dt, gradient of y, z, x
+  alignas(16) T raw_bc[SEL_STAGES][2][SEL_TILE][NP];    // c, b
+  alignas(16) float4 du[2][SEL_TILE][S::PAIRS];         // (step, step x) of two channels
+  alignas(16) float g[2][SEL_TILE][S::CH];
+  alignas(16) float bc[2][2][SEL_TILE][NP];             // c, b
+  alignas(16) float res[2][3][SEL_TILE][S::PITCH];      // <dh, B>, <e, A log2 e>, <C, h>
+  alignas(16) float part[2][SEL_THREADS / 32][SEL_TILE][2 * NP];  // dB, dC
+  uint32_t mark[2];
 };
 
-// FULL false: a segment's gradient of its first state, from zero behind it.  MARKS: there are starts (else the kernel knows none).
-template <typename T, int NP, bool FULL, bool MARKS>
-__global__ void __launch_bounds__(SEL_THREADS, FULL ? 2 : 4) ttt_selective_bwd_kernel(const SelParams p) {
+// (step, step x) of a thread's channels, and their gradients, of a token in shared memory
+template <int NP>
+__device__ __forceinline__ float4 steps_of(const float4* row, const SelLane<NP>& me) {
+  if constexpr (SelShape<NP>::CC == 2) {
+    return row[me.ch / 2];
+  } else {
+    const float2 one = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(row) + 2 * me.ch);
+    return make_float4(one.x, one.y, 0.f, 0.f);
+  }
+}
+template <int NP>
+__device__ __forceinline__ float2 grads_of(const float* row, const SelLane<NP>& me) {
+  if constexpr (SelShape<NP>::CC == 2) return *reinterpret_cast<const float2*>(row + me.ch);
+  else return make_float2(row[me.ch], 0.f);
+}
+
+// The state's gradient behind a segment: the given one, and what the segments behind carry back, from the last
+template <int NP>
+__device__ __forceinline__ void gradient_behind(F2 (&dh)[SelShape<NP>::CC][2], const F2 (&A)[SelShape<NP>::CC][2], const SelLane<NP>& me,
+                                                const SelPlace<NP>& at, const SelParams& p) {
   using S = SelShape<NP>;
-  using Smem = SelBwdSmem<T, NP, FULL>;
+  me.load(dh, p.gstate_out != nullptr ? p.gstate_out + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
+  for (int j = p.nseg - 1; j > at.seg; --j) {
+    const int64_t row = (at.b * p.nseg + j) * p.C + at.c0;
+    F2 own[S::CC][2];
+    me.load_padded(own, p.seg_state + row * NP, at.have);
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k) {
+      const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
+      const bool cut = sum == INFINITY;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dh[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), dh[k][i], own[k][i]);
+    }
+  }
+}
+
+// The launch's 128 registers per thread are shared out: the scanning warps take 200, the others keep 56 (build.py checks the 128).
+// MARKS: there are starts (else the kernel knows none).
+template <typename T, int NP, bool MARKS>
+__global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(const SelParams p) {
+  using S = SelShape<NP>;
+  using Smem = SelBwdSmem<T, NP>;
   extern __shared__ __align__(16) unsigned char sel_smem[];
   Smem& sm = *reinterpret_cast<Smem*>(sel_smem);
-  const SelPlace<NP> at(p, FULL ? 0 : 1, FULL ? p.nseg : p.nseg - 1);
-  const SelLane<NP> me;
-  const T* x = static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c0;
-  const T* dt = static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0;
-  const T* gy = static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0;
-  const T* z = p.z != nullptr ? static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0 : nullptr;
-  const T* bm = static_cast<const T*>(p.b) + at.b * p.bs[0] + at.g * p.bs[2];
-  const T* cm = static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2];
-  const uint8_t* starts = MARKS ? p.starts + at.b * p.T : nullptr;
-  const int64_t tiles = (p.T + SEL_TILE - 1) / SEL_TILE;
-  auto fetch = [&](int64_t t0, int k) {
-    copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][0][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][1][0][0], gy, p.gs[1], t0, at.t_hi, at.have, p.xg);
-    if (z != nullptr) copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][2][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, NP>(threadIdx.x, &sm.raw_bc[k][0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
-    if constexpr (FULL) {
-      copy_rows<T, S::CH>(threadIdx.x, &sm.raw[k][FULL ? 3 : 0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
-      copy_rows<T, NP>(threadIdx.x, &sm.raw_bc[k][FULL ? 1 : 0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
-    }
-    copy_commit();
-  };
-  const int64_t t_last = at.t_lo + (at.t_hi - at.t_lo - 1) / SEL_TILE * SEL_TILE;
-  fetch(t_last, 0);
-
-  F2 A[S::CC][2], dh[S::CC][2];
-  [[maybe_unused]] F2 dA[S::CC][2];
-  me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
+  const SelPlace<NP> at(p, 0, p.nseg);
+  const int tiles = (int)((at.t_hi - at.t_lo + SEL_TILE - 1) / SEL_TILE);
+  if (threadIdx.x < SEL_THREADS) {
+    // ---- scan
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const SelLane<NP> me;
+    F2 A[S::CC][2], dh[S::CC][2], dA[S::CC][2];
+    me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
 #pragma unroll
-  for (int k = 0; k < S::CC; ++k)
+    for (int k = 0; k < S::CC; ++k)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) A[k][i] = f2mul(A[k][i], f2(LOG2E)), dh[k][i] = f2(0.f);
-  if constexpr (FULL) {
-#pragma unroll
-    for (int k = 0; k < S::CC; ++k) dA[k][0] = dA[k][1] = f2(0.f);
-    me.load(dh, p.gstate_out != nullptr ? p.gstate_out + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
-    for (int j = p.nseg - 1; j > at.seg; --j) {  // the segments behind, from the last
-      const int64_t row = (at.b * p.nseg + j) * p.C + at.c0;
-      F2 own[S::CC][2];
-      me.load_padded(own, p.seg_state + row * NP, at.have);
-#pragma unroll
-      for (int k = 0; k < S::CC; ++k) {
-        const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
-        const bool cut = sum == INFINITY;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) dh[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), dh[k][i], own[k][i]);
-      }
-    }
-  }
-  const int pr = threadIdx.x % S::PAIRS, row0 = threadIdx.x / S::PAIRS, pair_have = at.have - 2 * pr;
-  float2 bias = make_float2(0.f, 0.f), skip = make_float2(0.f, 0.f);
-  if (p.bias != nullptr) {
-    if (pair_have > 0) bias.x = p.bias[at.c0 + 2 * pr];
-    if (pair_have > 1) bias.y = p.bias[at.c0 + 2 * pr + 1];
-  }
-  if (FULL && p.D != nullptr) {
-    if (pair_have > 0) skip.x = p.D[at.c0 + 2 * pr];
-    if (pair_have > 1) skip.y = p.D[at.c0 + 2 * pr + 1];
-  }
-  const bool whole = pair_have > 1 && p.xg >= 4 && (sizeof(T) == 2 || p.xg == 16);
-  float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);  // FULL: of dD and the bias's gradient; else of steps
-  bool any_start = false;
-
-  int buf = 0;
-  for (int64_t t0 = t_last; t0 >= at.t_lo; t0 -= SEL_TILE, buf ^= 1) {
-    uint32_t mark = 0;
-    if constexpr (MARKS) {
-      const int64_t t = t0 + (me.lane & (SEL_TILE - 1));
-      mark = __ballot_sync(0xffffffffu, t < at.t_hi && starts[t] != 0) & ((1u << SEL_TILE) - 1);
-      any_start = any_start || mark != 0;
-    }
-    [[maybe_unused]] F2 h[S::CC][2];
-    if constexpr (FULL) me.load_padded(h, p.saved + ((at.b * tiles + t0 / SEL_TILE) * p.C + at.c0) * NP, at.have);
-    copy_wait_all();
+      for (int i = 0; i < 2; ++i) A[k][i] = f2mul(A[k][i], f2(LOG2E)), dA[k][i] = f2(0.f);
+    gradient_behind<NP>(dh, A, me, at, p);
+    const float* saved = p.saved + ((at.b * ((p.T + SEL_TILE - 1) / SEL_TILE) + at.t_lo / SEL_TILE + tiles - 1) * p.C + at.c0) * NP;
+    F2 next[S::CC][2];
+    me.load_padded(next, saved, at.have);
     __syncthreads();
-    if (t0 - SEL_TILE >= at.t_lo) fetch(t0 - SEL_TILE, buf ^ 1);
+    for (int i = 0; i < tiles; ++i) {
+      const int k2 = i & 1;
+      const uint32_t mark = MARKS ? sm.mark[k2] : 0;
+      F2 h[S::CC][2], before[SEL_TILE / 2][S::CC][2];  // the states that tokens 0, 2, 4, ... find
 #pragma unroll
-    for (int r = row0; r < SEL_TILE; r += S::ROWS) {
-      const float2 dv = pair_of(&sm.raw[buf][0][r][2 * pr]);
-      float2 gv = pair_of(&sm.raw[buf][1][r][2 * pr]);
-      F2 d = f2add(dv, bias);
-      if (p.softplus) d = softplus_of(d);
-      if (t0 + r >= at.t_hi || pair_have < 1) d.x = 0.f;
-      if (t0 + r >= at.t_hi || pair_have < 2) d.y = 0.f;
-      if (z != nullptr) {
-        const float2 zv = pair_of(&sm.raw[buf][2][r][2 * pr]);
-        gv.x *= act_of(zv.x, ACT_SILU), gv.y *= act_of(zv.y, ACT_SILU);
+      for (int k = 0; k < S::CC; ++k) h[k][0] = next[k][0], h[k][1] = next[k][1];
+      if (i + 1 < tiles) {
+        saved -= (int64_t)p.C * NP;
+        me.load_padded(next, saved, at.have);
       }
-      float2 xv = make_float2(0.f, 0.f);
-      if constexpr (FULL) xv = pair_of(&sm.raw[buf][FULL ? 3 : 0][r][2 * pr]);
-      else s0.x += d.x, s0.y += d.y;
-      sm.du[r][pr] = make_float4(d.x, d.x * xv.x, d.y, d.y * xv.y);
-      *reinterpret_cast<float2*>(&sm.g[r][2 * pr]) = gv;
-    }
-#pragma unroll
-    for (int i = threadIdx.x; i < (FULL ? 2 : 1) * SEL_TILE * NP; i += SEL_THREADS)
-      (&sm.bc[0][0][0])[i] = ld_as_float<T>(&sm.raw_bc[buf][0][0][0], i);
-    __syncthreads();
-    auto steps = [&](int r) {
-      if constexpr (S::CC == 2) {
-        return sm.du[r][me.ch / 2];
-      } else {
-        const float2 one = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(&sm.du[r][0]) + 2 * me.ch);
-        return make_float4(one.x, one.y, 0.f, 0.f);
-      }
-    };
-    auto grads = [&](int r) {
-      if constexpr (S::CC == 2) return *reinterpret_cast<const float2*>(&sm.g[r][me.ch]);
-      else return make_float2(sm.g[r][me.ch], 0.f);
-    };
-    if constexpr (!FULL) {
-#pragma unroll 4
-      for (int r = SEL_TILE - 1; r >= 0; --r) {
-        const float4 q = steps(r), c = *reinterpret_cast<const float4*>(&sm.bc[0][r][4 * me.sl]);
-        const float2 g = grads(r);
-#pragma unroll
-        for (int k = 0; k < S::CC; ++k) {
-          const F2 d = f2(k ? q.z : q.x), gk = f2(k ? g.y : g.x);
-          dh[k][0] = f2mul(f2fma(gk, f2(c.x, c.y), dh[k][0]), ex2(f2mul(A[k][0], d)));
-          dh[k][1] = f2mul(f2fma(gk, f2(c.z, c.w), dh[k][1]), ex2(f2mul(A[k][1], d)));
-        }
-        if (MARKS && mark >> r & 1) {
-#pragma unroll
-          for (int k = 0; k < S::CC; ++k) dh[k][0] = dh[k][1] = f2(0.f);
-        }
-      }
-    } else {
-      F2 before[SEL_TILE][S::CC][2];  // the state that token r finds
 #pragma unroll
       for (int r = 0; r < SEL_TILE; ++r) {
-        const float4 q = steps(r), b = *reinterpret_cast<const float4*>(&sm.bc[FULL ? 1 : 0][r][4 * me.sl]);
+        if (r % 4 == 0) asm volatile("" ::: "memory");
+        const float4 q = steps_of<NP>(sm.du[k2][r], me), b = *reinterpret_cast<const float4*>(&sm.bc[k2][1][r][4 * me.sl]);
 #pragma unroll
         for (int k = 0; k < S::CC; ++k) {
           const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
-          before[r][k][0] = h[k][0], before[r][k][1] = h[k][1];
+          if (r % 2 == 0) before[r / 2][k][0] = h[k][0], before[r / 2][k][1] = h[k][1];
           if (MARKS && mark >> r & 1) h[k][0] = h[k][1] = f2(0.f);
           h[k][0] = f2fma(ex2(f2mul(A[k][0], d)), h[k][0], f2mul(v, f2(b.x, b.y)));
           h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
         }
       }
-      constexpr int DEAL = S::SL > 4 ? 4 : S::SL > S::CC ? S::SL : S::CC, TOKENS = DEAL / S::CC;
 #pragma unroll
-      for (int r0 = SEL_TILE - TOKENS; r0 >= 0; r0 -= TOKENS) {
-        float into[DEAL], rate[DEAL], yd[DEAL];
+      for (int r0 = SEL_TILE - 2; r0 >= 0; r0 -= 2) {
+        asm volatile("" ::: "memory");  // (the loads of all pairs of tokens at once would not fit in the registers)
+        float into[2 * S::CC], rate[2 * S::CC], yd[2 * S::CC];
+        F2 decay[S::CC][2], mid[S::CC][2];  // of token r0; the state behind it
+        {
+          const float4 q = steps_of<NP>(sm.du[k2][r0], me), b = *reinterpret_cast<const float4*>(&sm.bc[k2][1][r0][4 * me.sl]);
 #pragma unroll
-        for (int u = TOKENS - 1; u >= 0; --u) {
+          for (int k = 0; k < S::CC; ++k) {
+            const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              decay[k][n] = ex2(f2mul(A[k][n], d));
+              mid[k][n] = f2mul(v, n ? f2(b.z, b.w) : f2(b.x, b.y));
+              if (!(MARKS && mark >> r0 & 1)) mid[k][n] = f2fma(decay[k][n], before[r0 / 2][k][n], mid[k][n]);
+            }
+          }
+        }
+#pragma unroll
+        for (int u = 1; u >= 0; --u) {
           const int r = r0 + u;
-          const float4 q = steps(r);
-          const float4 c = *reinterpret_cast<const float4*>(&sm.bc[0][r][4 * me.sl]), b = *reinterpret_cast<const float4*>(&sm.bc[FULL ? 1 : 0][r][4 * me.sl]);
-          const float2 g = grads(r);
+          const float4 q = steps_of<NP>(sm.du[k2][r], me);
+          const float4 c = *reinterpret_cast<const float4*>(&sm.bc[k2][0][r][4 * me.sl]), b = *reinterpret_cast<const float4*>(&sm.bc[k2][1][r][4 * me.sl]);
+          const float2 g = grads_of<NP>(sm.g[k2][r], me);
           const F2 cv[2] = {f2(c.x, c.y), f2(c.z, c.w)}, bv[2] = {f2(b.x, b.y), f2(b.z, b.w)};
           F2 db[2], dc[2];
 #pragma unroll
@@ -186,18 +139,18 @@ __global__ void __launch_bounds__(SEL_THREADS, FULL ? 2 : 4) ttt_selective_bwd_k
             const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y), gk = f2(k ? g.y : g.x);
             F2 in, ra, ys;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              dh[k][i] = f2fma(gk, cv[i], dh[k][i]);
-              db[i] = k ? f2fma(dh[k][i], v, db[i]) : f2mul(dh[k][i], v);
-              dc[i] = k ? f2fma(gk, h[k][i], dc[i]) : f2mul(gk, h[k][i]);
-              in = i ? f2fma(dh[k][i], bv[i], in) : f2mul(dh[k][i], bv[i]);
-              ys = i ? f2fma(h[k][i], cv[i], ys) : f2mul(h[k][i], cv[i]);
-              dh[k][i] = f2mul(dh[k][i], ex2(f2mul(A[k][i], d)));
-              h[k][i] = before[r][k][i];
-              F2 way = f2mul(dh[k][i], h[k][i]);
-              if (MARKS && mark >> r & 1) dh[k][i] = way = f2(0.f);
-              ra = i ? f2fma(way, A[k][i], ra) : f2mul(way, A[k][i]);
-              dA[k][i] = f2fma(way, d, dA[k][i]);
+            for (int n = 0; n < 2; ++n) {
+              dh[k][n] = f2fma(gk, cv[n], dh[k][n]);
+              db[n] = k ? f2fma(dh[k][n], v, db[n]) : f2mul(dh[k][n], v);
+              dc[n] = k ? f2fma(gk, h[k][n], dc[n]) : f2mul(gk, h[k][n]);
+              in = n ? f2fma(dh[k][n], bv[n], in) : f2mul(dh[k][n], bv[n]);
+              ys = n ? f2fma(h[k][n], cv[n], ys) : f2mul(h[k][n], cv[n]);
+              h[k][n] = u ? mid[k][n] : before[r0 / 2][k][n];
+              dh[k][n] = f2mul(dh[k][n], u ? ex2(f2mul(A[k][n], d)) : decay[k][n]);
+              F2 way = f2mul(dh[k][n], h[k][n]);
+              if (MARKS && mark >> r & 1) dh[k][n] = way = f2(0.f);
+              ra = n ? f2fma(way, A[k][n], ra) : f2mul(way, A[k][n]);
+              dA[k][n] = f2fma(way, d, dA[k][n]);
             }
             into[u * S::CC + k] = f2hsum(in);
             rate[u * S::CC + k] = f2hsum(ra);
@@ -210,81 +163,256 @@ __global__ void __launch_bounds__(SEL_THREADS, FULL ? 2 : 4) ttt_selective_bwd_k
           const int cl = me.lane / S::SL, first = S::CL >= 8 ? cl / SHARED : cl * GOT;
           if (SHARED == 1 || cl % SHARED == 0) {
 #pragma unroll
-            for (int i = 0; i < GOT; ++i) {
-              const int e = first + i;  // dB of states 4 sl .. 4 sl + 3, then dC of them
-              sm.part[threadIdx.x >> 5][r][(e >= 4 ? NP : 0) + 4 * me.sl + (e & 3)] = sums[i];
+            for (int e0 = 0; e0 < GOT; ++e0) {
+              const int e = first + e0;  // dB of states 4 sl .. 4 sl + 3, then dC of them
+              sm.part[k2][threadIdx.x >> 5][r][(e >= 4 ? NP : 0) + 4 * me.sl + (e & 3)] = sums[e0];
             }
           }
         }
-        sum_and_deal<DEAL, S::SL, 1>(into, me.lane);
-        sum_and_deal<DEAL, S::SL, 1>(rate, me.lane);
-        sum_and_deal<DEAL, S::SL, 1>(yd, me.lane);
+        // a channel's lanes share its sums out: (token, channel) by (token, channel)
         if constexpr (S::SL == 1) {
-          sm.res[0][r0][me.ch] = into[0], sm.res[1][r0][me.ch] = rate[0], sm.res[2][r0][me.ch] = yd[0];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) sm.res[k2][0][r0 + u][me.ch] = into[u], sm.res[k2][1][r0 + u][me.ch] = rate[u], sm.res[k2][2][r0 + u][me.ch] = yd[u];
         } else {
-          constexpr int EACH = S::SL / DEAL;  // lanes with the same result
-          const int e = me.sl / EACH, r = r0 + e / S::CC, c = me.ch + e % S::CC;
-          if (EACH == 1 || me.sl % EACH == 0) sm.res[0][r][c] = into[0], sm.res[1][r][c] = rate[0], sm.res[2][r][c] = yd[0];
+          sum_and_deal<4, S::SL, 1>(into, me.lane);
+          sum_and_deal<4, S::SL, 1>(rate, me.lane);
+          sum_and_deal<4, S::SL, 1>(yd, me.lane);
+          constexpr int GOT = S::SL >= 4 ? 1 : 4 / S::SL, SHARED = S::SL >= 4 ? S::SL / 4 : 1;
+          const int first = S::SL >= 4 ? me.sl / SHARED : me.sl * GOT;
+          if (SHARED == 1 || me.sl % SHARED == 0) {
+#pragma unroll
+            for (int e0 = 0; e0 < GOT; ++e0) {
+              const int r = r0 + (first + e0) / 2, c = me.ch + (first + e0) % 2;
+              sm.res[k2][0][r][c] = into[e0], sm.res[k2][1][r][c] = rate[e0], sm.res[k2][2][r][c] = yd[e0];
+            }
+          }
         }
       }
       __syncthreads();
+    }
+    me.store(dA, p.part_a + ((at.b * p.nseg + at.seg) * p.C + at.c0) * NP, NP, at.have);
+    if (at.seg == 0 && p.gstate != nullptr) me.store(dh, p.gstate + (at.b * p.C + at.c0) * p.N, p.N, at.have);
+    return;
+  }
+  // ---- what is done once per token and channel, pair of channels by pair
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+  const int tid = threadIdx.x - SEL_THREADS, pr = tid % S::PAIRS, row0 = tid / S::PAIRS, pair_have = at.have - 2 * pr;
+  bool first[2] = {false, false};  // lane r of a warp: a start at token r of the next tile to be made ready, and of the one behind it
+  auto fetch = [&](int i) {
+    const int k = i % SEL_STAGES;
+    const int64_t t0 = at.t_lo + (int64_t)(tiles - 1 - i) * SEL_TILE;
+    copy_rows<T, S::CH>(tid, &sm.raw[k][0][0][0], static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH>(tid, &sm.raw[k][1][0][0], static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0, p.gs[1], t0, at.t_hi, at.have, p.xg);
+    if (p.z != nullptr)
+      copy_rows<T, S::CH>(tid, &sm.raw[k][2][0][0], static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0, p.zs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH>(tid, &sm.raw[k][3][0][0], static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c0, p.xs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP>(tid, &sm.raw_bc[k][0][0][0], static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2], p.cs[1], t0, at.t_hi, p.N, p.bg);
+    copy_rows<T, NP>(tid, &sm.raw_bc[k][1][0][0], static_cast<const T*>(p.b) + at.b * p.bs[0] + at.g * p.bs[2], p.bs[1], t0, at.t_hi, p.N, p.bg);
+    copy_commit();
+    if constexpr (MARKS) {
+      const int64_t t = t0 + (tid & 31);
+      first[1] = (tid & 31) < SEL_TILE && t < at.t_hi && p.starts[at.b * p.T + t] != 0;
+    }
+  };
+  float2 bias = make_float2(0.f, 0.f), skip = make_float2(0.f, 0.f);
+  if (p.bias != nullptr) {
+    if (pair_have > 0) bias.x = p.bias[at.c0 + 2 * pr];
+    if (pair_have > 1) bias.y = p.bias[at.c0 + 2 * pr + 1];
+  }
+  if (p.D != nullptr) {
+    if (pair_have > 0) skip.x = p.D[at.c0 + 2 * pr];
+    if (pair_have > 1) skip.y = p.D[at.c0 + 2 * pr + 1];
+  }
+  const bool whole = pair_have > 1 && p.xg >= 4 && (sizeof(T) == 2 || p.xg == 16);
+  float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);  // of dD and of the bias's gradient
+  auto make_ready = [&](int i) {
+    const int k = i % SEL_STAGES, left = (int)(at.t_hi - at.t_lo) - (tiles - 1 - i) * SEL_TILE;
+#pragma unroll 2
+    for (int r = row0; r < SEL_TILE; r += S::ROWS) {
+      F2 d = f2add(pair_of(&sm.raw[k][0][r][2 * pr]), bias), gv = pair_of(&sm.raw[k][1][r][2 * pr]);
+      if (p.softplus) d = softplus_of(d);
+      if (r >= left || pair_have < 1) d.x = 0.f;
+      if (r >= left || pair_have < 2) d.y = 0.f;
+      if (p.z != nullptr) {
+        const float2 zv = pair_of(&sm.raw[k][2][r][2 * pr]);
+        gv = f2mul(gv, f2(act_of(zv.x, ACT_SILU), act_of(zv.y, ACT_SILU)));
+      }
+      const F2 v = f2mul(d, pair_of(&sm.raw[k][3][r][2 * pr]));
+      sm.du[i & 1][r][pr] = make_float4(d.x, v.x, d.y, v.y);
+      *reinterpret_cast<float2*>(&sm.g[i & 1][r][2 * pr]) = gv;
+    }
 #pragma unroll
+    for (int e = tid; e < 2 * SEL_TILE * NP; e += SEL_THREADS) (&sm.bc[i & 1][0][0][0])[e] = ld_as_float<T>(&sm.raw_bc[k][0][0][0], e);
+    if constexpr (MARKS) {
+      const uint32_t mark = __ballot_sync(0xffffffffu, first[0]);
+      if (tid == 0) sm.mark[i & 1] = mark;
+      first[0] = first[1];
+    }
+  };
+  auto finish = [&](int i) {
+    const int k = i % SEL_STAGES, k2 = i & 1;
+    const int64_t t0 = at.t_lo + (int64_t)(tiles - 1 - i) * SEL_TILE;
+    const int left = (int)min((int64_t)SEL_TILE, at.t_hi - t0);
+    if (pair_have > 0) {
+#pragma unroll 2
       for (int r = row0; r < SEL_TILE; r += S::ROWS) {
-        if (t0 + r >= at.t_hi || pair_have < 1) continue;
-        const float2 xv = pair_of(&sm.raw[buf][FULL ? 3 : 0][r][2 * pr]), dv = pair_of(&sm.raw[buf][0][r][2 * pr]);
-        const float2 go = pair_of(&sm.raw[buf][1][r][2 * pr]), gv = *reinterpret_cast<const float2*>(&sm.g[r][2 * pr]);
-        const float2 in = *reinterpret_cast<const float2*>(&sm.res[0][r][2 * pr]), ra = *reinterpret_cast<const float2*>(&sm.res[1][r][2 * pr]);
-        const float4 q = sm.du[r][pr];
-        float2 sig = make_float2(1.f, 1.f);
-        if (p.softplus) sig = make_float2(sigmoid_of(dv.x + bias.x), sigmoid_of(dv.y + bias.y));
-        const float2 dx = make_float2(fmaf(skip.x, gv.x, q.x * in.x), fmaf(skip.y, gv.y, q.z * in.y));
-        const float2 dd = make_float2(fmaf(LN2, ra.x, in.x * xv.x) * sig.x, fmaf(LN2, ra.y, in.y * xv.y) * sig.y);
-        s0.x = fmaf(gv.x, xv.x, s0.x), s0.y = fmaf(gv.y, xv.y, s0.y);
-        s1.x += dd.x, s1.y += dd.y;
+        if (r >= left) break;
+        const F2 xv = pair_of(&sm.raw[k][3][r][2 * pr]), gv = *reinterpret_cast<const float2*>(&sm.g[k2][r][2 * pr]);
+        const F2 in = *reinterpret_cast<const float2*>(&sm.res[k2][0][r][2 * pr]);
+        const float4 q = sm.du[k2][r][pr];
         const int64_t row = (at.b * p.T + t0 + r) * p.C + at.c0 + 2 * pr;
-        put_pair<T>(static_cast<T*>(p.gx) + row, dx, pair_have, whole);
+        put_pair<T>(static_cast<T*>(p.gx) + row, f2fma(f2(q.x, q.z), in, f2mul(skip, gv)), pair_have, whole);
+        F2 dd = f2fma(*reinterpret_cast<const float2*>(&sm.res[k2][1][r][2 * pr]), f2(LN2), f2mul(in, xv));
+        if (p.softplus) {
+          const F2 v = f2add(pair_of(&sm.raw[k][0][r][2 * pr]), bias);
+          dd = f2mul(dd, f2(sigmoid_of(v.x), sigmoid_of(v.y)));
+        }
         put_pair<T>(static_cast<T*>(p.gdt) + row, dd, pair_have, whole);
-        if (z != nullptr) {
-          const float2 zv = pair_of(&sm.raw[buf][2][r][2 * pr]), yv = *reinterpret_cast<const float2*>(&sm.res[2][r][2 * pr]);
-          float2 slope;
+        s0 = f2fma(gv, xv, s0);
+        s1 = f2add(s1, dd);
+        if (p.z != nullptr) {
+          const float2 zv = pair_of(&sm.raw[k][2][r][2 * pr]);
+          F2 slope;
           act_and_slope(zv.x, ACT_SILU, slope.x), act_and_slope(zv.y, ACT_SILU, slope.y);
-          put_pair<T>(static_cast<T*>(p.gz) + row, make_float2(go.x * fmaf(skip.x, xv.x, yv.x) * slope.x, go.y * fmaf(skip.y, xv.y, yv.y) * slope.y),
-                      pair_have, whole);
+          const F2 y = f2fma(skip, xv, *reinterpret_cast<const float2*>(&sm.res[k2][2][r][2 * pr]));
+          put_pair<T>(static_cast<T*>(p.gz) + row, f2mul(f2mul(pair_of(&sm.raw[k][1][r][2 * pr]), y), slope), pair_have, whole);
         }
       }
-      const int blocks = (p.C / p.G + S::CH - 1) / S::CH;
-      float* out = p.part_bc + (((at.b * p.G + at.g) * blocks + at.block) * p.T + t0) * 2 * NP;
+    }
+    const int blocks = (p.C / p.G + S::CH - 1) / S::CH;
+    float* out = p.part_bc + (((at.b * p.G + at.g) * blocks + at.block) * p.T + t0) * 2 * NP;
+#pragma unroll 4
+    for (int e = tid; e < left * 2 * NP; e += SEL_THREADS) {
+      float v = 0.f;
 #pragma unroll
-      for (int i = threadIdx.x; i < SEL_TILE * 2 * NP; i += SEL_THREADS) {
-        float v = 0.f;
+      for (int w = 0; w < SEL_THREADS / 32; ++w) v += (&sm.part[k2][w][0][0])[e];
+      out[e] = v;
+    }
+  };
+  fetch(0);
+  first[0] = first[1];
+  if (tiles > 1) fetch(1);
+  copy_wait_all();
+  helpers_sync();
+  make_ready(0);
+  __syncthreads();
+  for (int i = 0; i < tiles; ++i) {
+    if (i > 0) finish(i - 1);
+    copy_wait_all();
+    helpers_sync();  // the copies of tile i + 1 are everybody's, and nobody reads tile i - 1 any more
+    if (i + 2 < tiles) fetch(i + 2);
+    if (i + 1 < tiles) make_ready(i + 1);
+    __syncthreads();
+  }
+  finish(tiles - 1);
+  float* sums = reinterpret_cast<float*>(&sm.du[0][0][0]);  // [2][ROWS][CH]
+  helpers_sync();
+  sums[row0 * S::CH + 2 * pr] = s0.x;
+  sums[row0 * S::CH + 2 * pr + 1] = s0.y;
+  sums[(S::ROWS + row0) * S::CH + 2 * pr] = s1.x;
+  sums[(S::ROWS + row0) * S::CH + 2 * pr + 1] = s1.y;
+  helpers_sync();
+  for (int e = tid; e < 2 * at.have; e += SEL_THREADS) {
+    const int m = e / at.have, c = e - m * at.have;
+    float v = 0.f;
+    for (int r = 0; r < S::ROWS; ++r) v += sums[(m * S::ROWS + r) * S::CH + c];
+    p.part_d[((at.b * p.nseg + at.seg) * 2 + m) * p.C + at.c0 + c] = v;
+  }
+}
+
+// A segment's gradient of its first state, from zero behind it, and its sum of steps
+template <typename T, int NP>
+struct SelRevSmem {
+  using S = SelShape<NP>;
+  alignas(16) T raw[2][3][SEL_TILE][S::CH];  // dt, gradient of y, z
+  alignas(16) T raw_c[2][SEL_TILE][NP];
+  alignas(16) float2 d[SEL_TILE][S::PAIRS];  // steps
+  alignas(16) float g[SEL_TILE][S::CH];
+  alignas(16) float c[SEL_TILE][NP];
+};
+template <typename T, int NP, bool MARKS>
+__global__ void __launch_bounds__(SEL_THREADS) ttt_selective_rev_kernel(const SelParams p) {
+  using S = SelShape<NP>;
+  extern __shared__ __align__(16) unsigned char sel_smem[];
+  SelRevSmem<T, NP>& sm = *reinterpret_cast<SelRevSmem<T, NP>*>(sel_smem);
+  const SelPlace<NP> at(p, 1, p.nseg - 1);
+  const SelLane<NP> me;
+  const int tid = threadIdx.x;
+  auto fetch = [&](int64_t t0, int k) {
+    copy_rows<T, S::CH>(tid, &sm.raw[k][0][0][0], static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH>(tid, &sm.raw[k][1][0][0], static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0, p.gs[1], t0, at.t_hi, at.have, p.xg);
+    if (p.z != nullptr)
+      copy_rows<T, S::CH>(tid, &sm.raw[k][2][0][0], static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0, p.zs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP>(tid, &sm.raw_c[k][0][0], static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2], p.cs[1], t0, at.t_hi, p.N, p.bg);
+    copy_commit();
+  };
+  const int64_t t_last = at.t_lo + (at.t_hi - at.t_lo - 1) / SEL_TILE * SEL_TILE;
+  fetch(t_last, 0);
+  F2 A[S::CC][2], dh[S::CC][2];
+  me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
 #pragma unroll
-        for (int w = 0; w < SEL_THREADS / 32; ++w) v += (&sm.part[w][0][0])[i];
-        if (t0 + i / (2 * NP) < at.t_hi) out[i] = v;
+  for (int k = 0; k < S::CC; ++k)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) A[k][i] = f2mul(A[k][i], f2(LOG2E)), dh[k][i] = f2(0.f);
+  const int pr = tid % S::PAIRS, row0 = tid / S::PAIRS, pair_have = at.have - 2 * pr;
+  float2 bias = make_float2(0.f, 0.f), sum = make_float2(0.f, 0.f);
+  if (p.bias != nullptr) {
+    if (pair_have > 0) bias.x = p.bias[at.c0 + 2 * pr];
+    if (pair_have > 1) bias.y = p.bias[at.c0 + 2 * pr + 1];
+  }
+  bool any_start = false;
+  int buf = 0;
+  for (int64_t t0 = t_last; t0 >= at.t_lo; t0 -= SEL_TILE, buf ^= 1) {
+    uint32_t mark = 0;
+    if constexpr (MARKS) {
+      const int64_t t = t0 + (me.lane & (SEL_TILE - 1));
+      mark = __ballot_sync(0xffffffffu, t < at.t_hi && p.starts[at.b * p.T + t] != 0) & ((1u << SEL_TILE) - 1);
+      any_start = any_start || mark != 0;
+    }
+    copy_wait_all();
+    __syncthreads();
+    if (t0 - SEL_TILE >= at.t_lo) fetch(t0 - SEL_TILE, buf ^ 1);
+#pragma unroll
+    for (int r = row0; r < SEL_TILE; r += S::ROWS) {
+      F2 d = f2add(pair_of(&sm.raw[buf][0][r][2 * pr]), bias), gv = pair_of(&sm.raw[buf][1][r][2 * pr]);
+      if (p.softplus) d = softplus_of(d);
+      if (t0 + r >= at.t_hi || pair_have < 1) d.x = 0.f;
+      if (t0 + r >= at.t_hi || pair_have < 2) d.y = 0.f;
+      if (p.z != nullptr) {
+        const float2 zv = pair_of(&sm.raw[buf][2][r][2 * pr]);
+        gv = f2mul(gv, f2(act_of(zv.x, ACT_SILU), act_of(zv.y, ACT_SILU)));
+      }
+      sum = f2add(sum, d);
+      sm.d[r][pr] = d;
+      *reinterpret_cast<float2*>(&sm.g[r][2 * pr]) = gv;
+    }
+#pragma unroll
+    for (int e = tid; e < SEL_TILE * NP; e += SEL_THREADS) (&sm.c[0][0])[e] = ld_as_float<T>(&sm.raw_c[buf][0][0], e);
+    __syncthreads();
+#pragma unroll 8
+    for (int r = SEL_TILE - 1; r >= 0; --r) {
+      const float2 d = grads_of<NP>(reinterpret_cast<const float*>(&sm.d[r][0]), me), g = grads_of<NP>(sm.g[r], me);
+      const float4 c = *reinterpret_cast<const float4*>(&sm.c[r][4 * me.sl]);
+#pragma unroll
+      for (int k = 0; k < S::CC; ++k) {
+        const F2 dk = f2(k ? d.y : d.x), gk = f2(k ? g.y : g.x);
+        dh[k][0] = f2mul(f2fma(gk, f2(c.x, c.y), dh[k][0]), ex2(f2mul(A[k][0], dk)));
+        dh[k][1] = f2mul(f2fma(gk, f2(c.z, c.w), dh[k][1]), ex2(f2mul(A[k][1], dk)));
+        if (MARKS && mark >> r & 1) dh[k][0] = dh[k][1] = f2(0.f);
       }
     }
   }
-  float* sums = reinterpret_cast<float*>(&sm.du[0][0]);  // [2][ROWS][CH], or [ROWS][CH]
+  const int64_t row = (at.b * p.nseg + at.seg) * p.C + at.c0;
+  me.store(dh, p.seg_state + row * NP, NP, at.have);
+  float* sums = reinterpret_cast<float*>(&sm.g[0][0]);  // [ROWS][CH]
   __syncthreads();
-  sums[row0 * S::CH + 2 * pr] = s0.x;
-  sums[row0 * S::CH + 2 * pr + 1] = s0.y;
-  if constexpr (FULL) {
-    sums[(S::ROWS + row0) * S::CH + 2 * pr] = s1.x;
-    sums[(S::ROWS + row0) * S::CH + 2 * pr + 1] = s1.y;
-  }
+  sums[row0 * S::CH + 2 * pr] = sum.x;
+  sums[row0 * S::CH + 2 * pr + 1] = sum.y;
   __syncthreads();
-  const int64_t row = at.b * p.nseg + at.seg;
-  for (int i = threadIdx.x; i < (FULL ? 2 : 1) * at.have; i += SEL_THREADS) {
-    const int m = i / at.have, c = i - m * at.have;
+  for (int c = tid; c < at.have; c += SEL_THREADS) {
     float v = 0.f;
-    for (int r = 0; r < S::ROWS; ++r) v += sums[(m * S::ROWS + r) * S::CH + c];
-    if constexpr (FULL) p.part_d[(row * 2 + m) * p.C + at.c0 + c] = v;
-    else p.seg_sum[row * p.C + at.c0 + c] = any_start ? INFINITY : v;
-  }
-  if constexpr (FULL) {
-    me.store(dA, p.part_a + (row * p.C + at.c0) * NP, NP, at.have);
-    if (at.seg == 0 && p.gstate != nullptr) me.store(dh, p.gstate + (at.b * p.C + at.c0) * p.N, p.N, at.have);
-  } else {
-    me.store(dh, p.seg_state + (row * p.C + at.c0) * NP, NP, at.have);
+    for (int r = 0; r < S::ROWS; ++r) v += sums[r * S::CH + c];
+    p.seg_sum[row + c] = any_start ? INFINITY : v;
   }
 }
 
@@ -323,15 +451,13 @@ __global__ void __launch_bounds__(256) ttt_selective_rows_kernel(const float* pa
   if (s < N) out[c * N + s] = v;
 }
 
-template <typename T, int NP, bool FULL>
-static cudaError_t run(const SelParams& p, int64_t blocks, cudaStream_t st) {
-  constexpr int bytes = sizeof(SelBwdSmem<T, NP, FULL>);
-  void (*kernel)(SelParams) = p.starts != nullptr ? ttt_selective_bwd_kernel<T, NP, FULL, true> : ttt_selective_bwd_kernel<T, NP, FULL, false>;
+template <typename K>
+static cudaError_t run(K kernel, int bytes, int64_t blocks, int threads, const SelParams& p, cudaStream_t st) {
   if (bytes > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<(unsigned)blocks, SEL_THREADS, bytes, st>>>(p);
+  kernel<<<(unsigned)blocks, threads, bytes, st>>>(p);
   return cudaGetLastError();
 }
 template <typename T, int NP>
@@ -339,8 +465,14 @@ static cudaError_t run_all(const SelParams& p, cudaStream_t st) {
   const int each = p.C / p.G, channel_blocks = (each + SelShape<NP>::CH - 1) / SelShape<NP>::CH;
   const int64_t blocks = p.B * p.G * channel_blocks, rows = p.B * p.nseg;
   cudaError_t e;
-  if (p.nseg > 1 && (e = run<T, NP, false>(p, blocks * (p.nseg - 1), st)) != cudaSuccess) return e;
-  if ((e = run<T, NP, true>(p, blocks * p.nseg, st)) != cudaSuccess) return e;
+  const bool marks = p.starts != nullptr;
+  static_assert(sizeof(SelBwdSmem<T, NP>) <= 227 * 1024, "");
+  if (p.nseg > 1 && (e = run(marks ? ttt_selective_rev_kernel<T, NP, true> : ttt_selective_rev_kernel<T, NP, false>, sizeof(SelRevSmem<T, NP>),
+                             blocks * (p.nseg - 1), SEL_THREADS, p, st)) != cudaSuccess)
+    return e;
+  if ((e = run(marks ? ttt_selective_bwd_kernel<T, NP, true> : ttt_selective_bwd_kernel<T, NP, false>, sizeof(SelBwdSmem<T, NP>), blocks * p.nseg,
+               2 * SEL_THREADS, p, st)) != cudaSuccess)
+    return e;
   ttt_selective_bc_kernel<T><<<(unsigned)((p.B * p.G * p.T * 2 * NP + 255) / 256), 256, 0, st>>>(p, NP, channel_blocks);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int64_t n = (int64_t)p.C * NP;

@@ -5,7 +5,7 @@
 // h_{t-1} = 0.
 //
 // What bounds it is exponentials: one per state, channel and token, 16 per SM and clock, where memory would allow twice as many at
-// N = 16.  A thread holds SEL_EACH states of SEL_CH neighbouring channels (1 where N <= 4); NP / SEL_EACH lanes share a channel.
+// N = 16.  A thread holds SEL_EACH states of SEL_CH neighbouring channels (1 where N <= 8); NP / SEL_EACH lanes share a channel.
 // Four warps of a block scan; four others (SEL_THREADS each) do what is done once per token and channel: they copy tiles of SEL_TILE
 // tokens ahead (cp.async), turn them into (step, step times x) pairs in float32 in shared memory a tile before the scan, and write the
 // results a tile behind it, so that the two kinds of work hide one another's latency.  One barrier of the block per tile.
@@ -24,9 +24,9 @@ template <int NP>
 struct SelShape {
   static constexpr int SL = NP / SEL_EACH;         // lanes that share a channel
   static constexpr int CL = 32 / SL;               // lanes with channels of their own
-  static constexpr int CC = SL == 1 ? 1 : 2;       // channels of a thread
+  static constexpr int CC = SL >= 4 ? 2 : 1;       // channels of a thread
   static constexpr int WARP_CH = CL * CC;
-  static constexpr int CH = WARP_CH * (SEL_THREADS / 32);  // of a block: 128, 128, 64, 32, 16
+  static constexpr int CH = WARP_CH * (SEL_THREADS / 32);  // of a block: 128, 64, 64, 32, 16
   static constexpr int PAIRS = CH / 2;
   static constexpr int ROWS = SEL_THREADS / PAIRS;         // tokens that the block's threads cover, pair by pair
   static constexpr int PITCH = CH + 16;            // floats between tokens of results: two tokens' channels in different banks

@@ -3,42 +3,29 @@
 //   g = dout SiLU(z);   dh_t = C_t g_t + exp(d_{t+1} A) dh_{t+1};   e_t = dh_t exp(d_t A) h_{t-1}
 //   dx = d <dh, B> + D g,   dd = <e, A> + <dh, B> x,   dA = sum_t e d,   dB = sum_channels dh d x,   dC = sum_channels g h
 //   ddt = dd / (1 + exp(-dt - bias)),   dz = dout (<C, h> + D x) SiLU'(z)
-// A tile of SEL_TILE tokens at a time, from the last: its states again from the saved one before it, kept in registers, then the
-// gradients token by token.  Sums over a channel's states are dealt out over its lanes, sums over channels over the lanes with
+// Half a tile of SEL_TILE tokens at a time, from the last: its states again from the saved one before the tile, every second one
+// kept in registers, then the gradients token by token (whole tiles at once: twice the code, whose fetches cost more than the states
+// of the first half do once more).  Sums over a channel's states are dealt out over its lanes, sums over channels over the lanes with
 // channels of their own, then over the block's warps through shared memory; the blocks' shares of dB, dC, dA, dD and the bias's
 // gradient go to the workspace and are joined in a fixed order.  Segments: as in the forward, from the last token on.
 #include "ttt_selective.cuh"
 
 namespace ttt {
 
+constexpr int SEL_HALF = SEL_TILE / 2;
+
 template <typename T, int NP>
 struct SelBwdSmem {
   using S = SelShape<NP>;
   alignas(16) T raw[SEL_STAGES][4][SEL_TILE][S::CH];    // dt, gradient of y, z, x
   alignas(16) T raw_bc[SEL_STAGES][2][SEL_TILE][NP];    // c, b
-  alignas(16) float4 du[2][SEL_TILE][S::PAIRS];         // (step, step x) of two channels
-  alignas(16) float g[2][SEL_TILE][S::CH];
+  alignas(16) float4 du[2][SEL_TILE][S::CH];            // step and step x, twice each, as operands of packed operations
+  alignas(16) float2 g[2][SEL_TILE][S::CH];             // gradient of the result before the gate, twice
   alignas(16) float bc[2][2][SEL_TILE][NP];             // c, b
-  alignas(16) float res[2][3][SEL_TILE][S::PITCH];      // <dh, B>, <e, A log2 e>, <C, h>
-  alignas(16) float part[2][SEL_THREADS / 32][SEL_TILE][2 * NP];  // dB, dC
+  alignas(16) float res[2][3][SEL_HALF][S::PITCH];      // <dh, B>, <e, A log2 e>, <C, h>
+  alignas(16) float part[2][SEL_THREADS / 32][SEL_HALF][2 * NP];  // dB, dC
   uint32_t mark[2];
 };
-
-// (step, step x) of a thread's channels, and their gradients, of a token in shared memory
-template <int NP>
-__device__ __forceinline__ float4 steps_of(const float4* row, const SelLane<NP>& me) {
-  if constexpr (SelShape<NP>::CC == 2) {
-    return row[me.ch / 2];
-  } else {
-    const float2 one = *reinterpret_cast<const float2*>(reinterpret_cast<const float*>(row) + 2 * me.ch);
-    return make_float4(one.x, one.y, 0.f, 0.f);
-  }
-}
-template <int NP>
-__device__ __forceinline__ float2 grads_of(const float* row, const SelLane<NP>& me) {
-  if constexpr (SelShape<NP>::CC == 2) return *reinterpret_cast<const float2*>(row + me.ch);
-  else return make_float2(row[me.ch], 0.f);
-}
 
 // The state's gradient behind a segment: the given one, and what the segments behind carry back, from the last
 template <int NP>
@@ -86,109 +73,126 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
     me.load_padded(next, saved, at.have);
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
-      const int k2 = i & 1;
-      const uint32_t mark = MARKS ? sm.mark[k2] : 0;
-      F2 h[S::CC][2], before[SEL_TILE / 2][S::CC][2];  // the states that tokens 0, 2, 4, ... find
+      const uint32_t marks = MARKS ? sm.mark[i & 1] : 0;
+      F2 h0[S::CC][2];
 #pragma unroll
-      for (int k = 0; k < S::CC; ++k) h[k][0] = next[k][0], h[k][1] = next[k][1];
+      for (int k = 0; k < S::CC; ++k) h0[k][0] = next[k][0], h0[k][1] = next[k][1];
       if (i + 1 < tiles) {
         saved -= (int64_t)p.C * NP;
         me.load_padded(next, saved, at.have);
       }
+#pragma unroll 1
+      for (int half = 1; half >= 0; --half) {
+        const int k2 = half ^ 1;  // results alternate
+        F2 h[S::CC][2], before[SEL_HALF / 2][S::CC][2];  // the states that the half's tokens 0, 2, 4, 6 find
 #pragma unroll
-      for (int r = 0; r < SEL_TILE; ++r) {
-        if (r % 4 == 0) asm volatile("" ::: "memory");
-        const float4 q = steps_of<NP>(sm.du[k2][r], me), b = *reinterpret_cast<const float4*>(&sm.bc[k2][1][r][4 * me.sl]);
-#pragma unroll
-        for (int k = 0; k < S::CC; ++k) {
-          const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
-          if (r % 2 == 0) before[r / 2][k][0] = h[k][0], before[r / 2][k][1] = h[k][1];
-          if (MARKS && mark >> r & 1) h[k][0] = h[k][1] = f2(0.f);
-          h[k][0] = f2fma(ex2(f2mul(A[k][0], d)), h[k][0], f2mul(v, f2(b.x, b.y)));
-          h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
-        }
-      }
-#pragma unroll
-      for (int r0 = SEL_TILE - 2; r0 >= 0; r0 -= 2) {
-        asm volatile("" ::: "memory");  // (the loads of all pairs of tokens at once would not fit in the registers)
-        float into[2 * S::CC], rate[2 * S::CC], yd[2 * S::CC];
-        F2 decay[S::CC][2], mid[S::CC][2];  // of token r0; the state behind it
-        {
-          const float4 q = steps_of<NP>(sm.du[k2][r0], me), b = *reinterpret_cast<const float4*>(&sm.bc[k2][1][r0][4 * me.sl]);
+        for (int k = 0; k < S::CC; ++k) h[k][0] = h0[k][0], h[k][1] = h0[k][1];
+        const float4* du = &sm.du[i & 1][0][me.ch];
+        const float* bp = &sm.bc[i & 1][1][0][4 * me.sl];
+        uint32_t mark = marks;
+        auto step = [&](int r) {
+          const float4 b = *reinterpret_cast<const float4*>(bp + r * NP);
 #pragma unroll
           for (int k = 0; k < S::CC; ++k) {
-            const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              decay[k][n] = ex2(f2mul(A[k][n], d));
-              mid[k][n] = f2mul(v, n ? f2(b.z, b.w) : f2(b.x, b.y));
-              if (!(MARKS && mark >> r0 & 1)) mid[k][n] = f2fma(decay[k][n], before[r0 / 2][k][n], mid[k][n]);
-            }
+            const float4 q = du[r * S::CH + k];
+            if (MARKS && mark >> r & 1) h[k][0] = h[k][1] = f2(0.f);
+            h[k][0] = f2fma(ex2(f2mul(A[k][0], f2(q.x, q.y))), h[k][0], f2mul(f2(q.z, q.w), f2(b.x, b.y)));
+            h[k][1] = f2fma(ex2(f2mul(A[k][1], f2(q.x, q.y))), h[k][1], f2mul(f2(q.z, q.w), f2(b.z, b.w)));
           }
+        };
+        if (half) {
+#pragma unroll 4
+          for (int r = 0; r < SEL_HALF; ++r) step(r);
+          du += SEL_HALF * S::CH;
+          bp += SEL_HALF * NP;
+          mark >>= SEL_HALF;
+        }
+        const float* cp = bp - SEL_TILE * NP;
+        const float2* gp = &sm.g[i & 1][half * SEL_HALF][me.ch];
+#pragma unroll
+        for (int r = 0; r < SEL_HALF; ++r) {
+          if (r % 4 == 0) asm volatile("" ::: "memory");  // (the loads of all tokens at once would not fit in the registers)
+          if (r % 2 == 0)
+#pragma unroll
+            for (int k = 0; k < S::CC; ++k) before[r / 2][k][0] = h[k][0], before[r / 2][k][1] = h[k][1];
+          step(r);
         }
 #pragma unroll
-        for (int u = 1; u >= 0; --u) {
-          const int r = r0 + u;
-          const float4 q = steps_of<NP>(sm.du[k2][r], me);
-          const float4 c = *reinterpret_cast<const float4*>(&sm.bc[k2][0][r][4 * me.sl]), b = *reinterpret_cast<const float4*>(&sm.bc[k2][1][r][4 * me.sl]);
-          const float2 g = grads_of<NP>(sm.g[k2][r], me);
-          const F2 cv[2] = {f2(c.x, c.y), f2(c.z, c.w)}, bv[2] = {f2(b.x, b.y), f2(b.z, b.w)};
-          F2 db[2], dc[2];
+        for (int r0 = SEL_HALF - 2; r0 >= 0; r0 -= 2) {
+          asm volatile("" ::: "memory");
+          float into[2 * S::CC], rate[2 * S::CC], yd[2 * S::CC];
+          F2 decay[S::CC][2], mid[S::CC][2];  // of token r0; the state behind it
+          {
+            const float4 b = *reinterpret_cast<const float4*>(bp + r0 * NP);
 #pragma unroll
-          for (int k = 0; k < S::CC; ++k) {
-            const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y), gk = f2(k ? g.y : g.x);
-            F2 in, ra, ys;
+            for (int k = 0; k < S::CC; ++k) {
+              const float4 q = du[r0 * S::CH + k];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              dh[k][n] = f2fma(gk, cv[n], dh[k][n]);
-              db[n] = k ? f2fma(dh[k][n], v, db[n]) : f2mul(dh[k][n], v);
-              dc[n] = k ? f2fma(gk, h[k][n], dc[n]) : f2mul(gk, h[k][n]);
-              in = n ? f2fma(dh[k][n], bv[n], in) : f2mul(dh[k][n], bv[n]);
-              ys = n ? f2fma(h[k][n], cv[n], ys) : f2mul(h[k][n], cv[n]);
-              h[k][n] = u ? mid[k][n] : before[r0 / 2][k][n];
-              dh[k][n] = f2mul(dh[k][n], u ? ex2(f2mul(A[k][n], d)) : decay[k][n]);
-              F2 way = f2mul(dh[k][n], h[k][n]);
-              if (MARKS && mark >> r & 1) dh[k][n] = way = f2(0.f);
-              ra = n ? f2fma(way, A[k][n], ra) : f2mul(way, A[k][n]);
-              dA[k][n] = f2fma(way, d, dA[k][n]);
-            }
-            into[u * S::CC + k] = f2hsum(in);
-            rate[u * S::CC + k] = f2hsum(ra);
-            yd[u * S::CC + k] = f2hsum(ys);
-          }
-          float sums[8] = {db[0].x, db[0].y, db[1].x, db[1].y, dc[0].x, dc[0].y, dc[1].x, dc[1].y};
-          sum_and_deal<8, S::CL, S::SL>(sums, me.lane);
-          // lane cl has sums [cl 8 / CL, ...); more lanes than sums: one each of lanes 0, CL / 8, ...
-          constexpr int GOT = S::CL >= 8 ? 1 : 8 / S::CL, SHARED = S::CL >= 8 ? S::CL / 8 : 1;
-          const int cl = me.lane / S::SL, first = S::CL >= 8 ? cl / SHARED : cl * GOT;
-          if (SHARED == 1 || cl % SHARED == 0) {
-#pragma unroll
-            for (int e0 = 0; e0 < GOT; ++e0) {
-              const int e = first + e0;  // dB of states 4 sl .. 4 sl + 3, then dC of them
-              sm.part[k2][threadIdx.x >> 5][r][(e >= 4 ? NP : 0) + 4 * me.sl + (e & 3)] = sums[e0];
+              for (int n = 0; n < 2; ++n) {
+                decay[k][n] = ex2(f2mul(A[k][n], f2(q.x, q.y)));
+                mid[k][n] = f2mul(f2(q.z, q.w), n ? f2(b.z, b.w) : f2(b.x, b.y));
+                if (!(MARKS && mark >> r0 & 1)) mid[k][n] = f2fma(decay[k][n], before[r0 / 2][k][n], mid[k][n]);
+              }
             }
           }
-        }
-        // a channel's lanes share its sums out: (token, channel) by (token, channel)
-        if constexpr (S::SL == 1) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) sm.res[k2][0][r0 + u][me.ch] = into[u], sm.res[k2][1][r0 + u][me.ch] = rate[u], sm.res[k2][2][r0 + u][me.ch] = yd[u];
-        } else {
-          sum_and_deal<4, S::SL, 1>(into, me.lane);
-          sum_and_deal<4, S::SL, 1>(rate, me.lane);
-          sum_and_deal<4, S::SL, 1>(yd, me.lane);
-          constexpr int GOT = S::SL >= 4 ? 1 : 4 / S::SL, SHARED = S::SL >= 4 ? S::SL / 4 : 1;
-          const int first = S::SL >= 4 ? me.sl / SHARED : me.sl * GOT;
+          for (int u = 1; u >= 0; --u) {
+            const int r = r0 + u;
+            const float4 c = *reinterpret_cast<const float4*>(cp + r * NP), b = *reinterpret_cast<const float4*>(bp + r * NP);
+            const F2 cv[2] = {f2(c.x, c.y), f2(c.z, c.w)}, bv[2] = {f2(b.x, b.y), f2(b.z, b.w)};
+            F2 db[2], dc[2];
+#pragma unroll
+            for (int k = 0; k < S::CC; ++k) {
+              const float4 q = du[r * S::CH + k];
+              const F2 d = f2(q.x, q.y), v = f2(q.z, q.w), gk = gp[r * S::CH + k];
+              F2 in, ra, ys;
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                dh[k][n] = f2fma(gk, cv[n], dh[k][n]);
+                db[n] = k ? f2fma(dh[k][n], v, db[n]) : f2mul(dh[k][n], v);
+                dc[n] = k ? f2fma(gk, h[k][n], dc[n]) : f2mul(gk, h[k][n]);
+                in = n ? f2fma(dh[k][n], bv[n], in) : f2mul(dh[k][n], bv[n]);
+                ys = n ? f2fma(h[k][n], cv[n], ys) : f2mul(h[k][n], cv[n]);
+                h[k][n] = u ? mid[k][n] : before[r0 / 2][k][n];
+                dh[k][n] = f2mul(dh[k][n], u ? ex2(f2mul(A[k][n], d)) : decay[k][n]);
+                F2 way = f2mul(dh[k][n], h[k][n]);
+                if (MARKS && mark >> r & 1) dh[k][n] = way = f2(0.f);
+                ra = n ? f2fma(way, A[k][n], ra) : f2mul(way, A[k][n]);
+                dA[k][n] = f2fma(way, d, dA[k][n]);
+              }
+              into[u * S::CC + k] = f2hsum(in);
+              rate[u * S::CC + k] = f2hsum(ra);
+              yd[u * S::CC + k] = f2hsum(ys);
+            }
+            float sums[8] = {db[0].x, db[0].y, db[1].x, db[1].y, dc[0].x, dc[0].y, dc[1].x, dc[1].y};
+            sum_and_deal<8, S::CL, S::SL>(sums, me.lane);
+            // lane cl has sums [cl 8 / CL, ...); more lanes than sums: one each of lanes 0, CL / 8, ...
+            constexpr int GOT = S::CL >= 8 ? 1 : 8 / S::CL, SHARED = S::CL >= 8 ? S::CL / 8 : 1;
+            const int cl = me.lane / S::SL, first = S::CL >= 8 ? cl / SHARED : cl * GOT;
+            if (SHARED == 1 || cl % SHARED == 0) {
+#pragma unroll
+              for (int e0 = 0; e0 < GOT; ++e0) {
+                const int e = first + e0;  // dB of states 4 sl .. 4 sl + 3, then dC of them
+                sm.part[k2][threadIdx.x >> 5][r][(e >= 4 ? NP : 0) + 4 * me.sl + (e & 3)] = sums[e0];
+              }
+            }
+          }
+          // a channel's lanes share its sums out: (token, channel) by (token, channel)
+          constexpr int DEAL = 2 * S::CC, GOT = S::SL >= DEAL ? 1 : DEAL / S::SL, SHARED = S::SL >= DEAL ? S::SL / DEAL : 1;
+          sum_and_deal<DEAL, S::SL, 1>(into, me.lane);
+          sum_and_deal<DEAL, S::SL, 1>(rate, me.lane);
+          sum_and_deal<DEAL, S::SL, 1>(yd, me.lane);
+          const int first = S::SL >= DEAL ? me.sl / SHARED : me.sl * GOT;
           if (SHARED == 1 || me.sl % SHARED == 0) {
 #pragma unroll
             for (int e0 = 0; e0 < GOT; ++e0) {
-              const int r = r0 + (first + e0) / 2, c = me.ch + (first + e0) % 2;
+              const int r = r0 + (first + e0) / S::CC, c = me.ch + (first + e0) % S::CC;
               sm.res[k2][0][r][c] = into[e0], sm.res[k2][1][r][c] = rate[e0], sm.res[k2][2][r][c] = yd[e0];
             }
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
     }
     me.store(dA, p.part_a + ((at.b * p.nseg + at.seg) * p.C + at.c0) * NP, NP, at.have);
     if (at.seg == 0 && p.gstate != nullptr) me.store(dh, p.gstate + (at.b * p.C + at.c0) * p.N, p.N, at.have);
@@ -238,8 +242,9 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
         gv = f2mul(gv, f2(act_of(zv.x, ACT_SILU), act_of(zv.y, ACT_SILU)));
       }
       const F2 v = f2mul(d, pair_of(&sm.raw[k][3][r][2 * pr]));
-      sm.du[i & 1][r][pr] = make_float4(d.x, v.x, d.y, v.y);
-      *reinterpret_cast<float2*>(&sm.g[i & 1][r][2 * pr]) = gv;
+      sm.du[i & 1][r][2 * pr] = make_float4(d.x, d.x, v.x, v.x);
+      sm.du[i & 1][r][2 * pr + 1] = make_float4(d.y, d.y, v.y, v.y);
+      *reinterpret_cast<float4*>(&sm.g[i & 1][r][2 * pr]) = make_float4(gv.x, gv.x, gv.y, gv.y);
     }
 #pragma unroll
     for (int e = tid; e < 2 * SEL_TILE * NP; e += SEL_THREADS) (&sm.bc[i & 1][0][0][0])[e] = ld_as_float<T>(&sm.raw_bc[k][0][0][0], e);
@@ -249,33 +254,34 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
       first[0] = first[1];
     }
   };
-  auto finish = [&](int i) {
-    const int k = i % SEL_STAGES, k2 = i & 1;
-    const int64_t t0 = at.t_lo + (int64_t)(tiles - 1 - i) * SEL_TILE;
-    const int left = (int)min((int64_t)SEL_TILE, at.t_hi - t0);
+  auto finish = [&](int i, int half) {
+    const int k = i % SEL_STAGES, k2 = half ^ 1, base = half * SEL_HALF;
+    const int64_t t0 = at.t_lo + (int64_t)(tiles - 1 - i) * SEL_TILE + base;
+    const int left = (int)min((int64_t)SEL_HALF, at.t_hi - t0);
     if (pair_have > 0) {
 #pragma unroll 2
-      for (int r = row0; r < SEL_TILE; r += S::ROWS) {
+      for (int r = row0; r < SEL_HALF; r += S::ROWS) {
         if (r >= left) break;
-        const F2 xv = pair_of(&sm.raw[k][3][r][2 * pr]), gv = *reinterpret_cast<const float2*>(&sm.g[k2][r][2 * pr]);
+        const float4 gg = *reinterpret_cast<const float4*>(&sm.g[i & 1][base + r][2 * pr]);
+        const F2 xv = pair_of(&sm.raw[k][3][base + r][2 * pr]), gv = f2(gg.x, gg.z);
         const F2 in = *reinterpret_cast<const float2*>(&sm.res[k2][0][r][2 * pr]);
-        const float4 q = sm.du[k2][r][pr];
+        const F2 q = f2(sm.du[i & 1][base + r][2 * pr].x, sm.du[i & 1][base + r][2 * pr + 1].x);
         const int64_t row = (at.b * p.T + t0 + r) * p.C + at.c0 + 2 * pr;
-        put_pair<T>(static_cast<T*>(p.gx) + row, f2fma(f2(q.x, q.z), in, f2mul(skip, gv)), pair_have, whole);
+        put_pair<T>(static_cast<T*>(p.gx) + row, f2fma(q, in, f2mul(skip, gv)), pair_have, whole);
         F2 dd = f2fma(*reinterpret_cast<const float2*>(&sm.res[k2][1][r][2 * pr]), f2(LN2), f2mul(in, xv));
         if (p.softplus) {
-          const F2 v = f2add(pair_of(&sm.raw[k][0][r][2 * pr]), bias);
+          const F2 v = f2add(pair_of(&sm.raw[k][0][base + r][2 * pr]), bias);
           dd = f2mul(dd, f2(sigmoid_of(v.x), sigmoid_of(v.y)));
         }
         put_pair<T>(static_cast<T*>(p.gdt) + row, dd, pair_have, whole);
         s0 = f2fma(gv, xv, s0);
         s1 = f2add(s1, dd);
         if (p.z != nullptr) {
-          const float2 zv = pair_of(&sm.raw[k][2][r][2 * pr]);
+          const float2 zv = pair_of(&sm.raw[k][2][base + r][2 * pr]);
           F2 slope;
           act_and_slope(zv.x, ACT_SILU, slope.x), act_and_slope(zv.y, ACT_SILU, slope.y);
           const F2 y = f2fma(skip, xv, *reinterpret_cast<const float2*>(&sm.res[k2][2][r][2 * pr]));
-          put_pair<T>(static_cast<T*>(p.gz) + row, f2mul(f2mul(pair_of(&sm.raw[k][1][r][2 * pr]), y), slope), pair_have, whole);
+          put_pair<T>(static_cast<T*>(p.gz) + row, f2mul(f2mul(pair_of(&sm.raw[k][1][base + r][2 * pr]), y), slope), pair_have, whole);
         }
       }
     }
@@ -297,14 +303,18 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
   make_ready(0);
   __syncthreads();
   for (int i = 0; i < tiles; ++i) {
-    if (i > 0) finish(i - 1);
+    // while the second half is scanned
+    if (i > 0) finish(i - 1, 0);
     copy_wait_all();
     helpers_sync();  // the copies of tile i + 1 are everybody's, and nobody reads tile i - 1 any more
     if (i + 2 < tiles) fetch(i + 2);
+    __syncthreads();
+    // while the first half is
+    finish(i, 1);
     if (i + 1 < tiles) make_ready(i + 1);
     __syncthreads();
   }
-  finish(tiles - 1);
+  finish(tiles - 1, 0);
   float* sums = reinterpret_cast<float*>(&sm.du[0][0][0]);  // [2][ROWS][CH]
   helpers_sync();
   sums[row0 * S::CH + 2 * pr] = s0.x;
@@ -391,11 +401,12 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_rev_kernel(const Se
     __syncthreads();
 #pragma unroll 8
     for (int r = SEL_TILE - 1; r >= 0; --r) {
-      const float2 d = grads_of<NP>(reinterpret_cast<const float*>(&sm.d[r][0]), me), g = grads_of<NP>(sm.g[r], me);
+      const float* dp = reinterpret_cast<const float*>(&sm.d[r][0]) + me.ch;
+      const float* gp = sm.g[r] + me.ch;
       const float4 c = *reinterpret_cast<const float4*>(&sm.c[r][4 * me.sl]);
 #pragma unroll
       for (int k = 0; k < S::CC; ++k) {
-        const F2 dk = f2(k ? d.y : d.x), gk = f2(k ? g.y : g.x);
+        const F2 dk = f2(dp[k]), gk = f2(gp[k]);
         dh[k][0] = f2mul(f2fma(gk, f2(c.x, c.y), dh[k][0]), ex2(f2mul(A[k][0], dk)));
         dh[k][1] = f2mul(f2fma(gk, f2(c.z, c.w), dh[k][1]), ex2(f2mul(A[k][1], dk)));
         if (MARKS && mark >> r & 1) dh[k][0] = dh[k][1] = f2(0.f);

@@ -177,7 +177,8 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
 #pragma unroll
         for (int l = 0; l < S::SL; ++l) v = f2add(v, *reinterpret_cast<const float2*>(&sm.y[i & 1][r][2 * (pr * S::SL + l)]));
       } else {
-        v = *reinterpret_cast<const float2*>(&sm.y[i & 1][r][2 * pr]);
+#pragma unroll
+        for (int l = 0; l < S::SL; ++l) v = f2add(v, f2(sm.y[i & 1][r][2 * pr * S::SL + l], sm.y[i & 1][r][(2 * pr + 1) * S::SL + l]));
       }
       v = f2fma(skip, pair_of(&sm.raw[k][0][r][2 * pr]), v);
       if (z != nullptr) {
@@ -294,7 +295,7 @@ int sel_padded(int N) {
   return n;
 }
 SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd) {
-  const int NP = sel_padded(N), CH = NP <= 8 ? 128 : 1024 / NP, each = C / G;
+  const int NP = sel_padded(N), CH = NP == 4 ? 128 : NP == 8 ? 64 : 1024 / NP, each = C / G;
   SelCut k{};
   k.channel_blocks = (each + CH - 1) / CH;
   const int64_t blocks = B * G * k.channel_blocks, tiles = (T + SEL_TILE - 1) / SEL_TILE;

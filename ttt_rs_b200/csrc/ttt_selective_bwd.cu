@@ -4,7 +4,7 @@
 //   dx = d <dh, B> + D g,   dd = <e, A> + <dh, B> x,   dA = sum_t e d,   dB = sum_channels dh d x,   dC = sum_channels g h
 //   ddt = dd / (1 + exp(-dt - bias)),   dz = dout (<C, h> + D x) SiLU'(z)
 // Half a tile of SEL_TILE tokens at a time, from the last: its states again from the saved one before the tile, every second one
-// kept in registers, then the gradients token by token (whole tiles at once: twice the code, whose fetches cost more than the states
+// kept in registers, like all decays, then the gradients token by token (whole tiles at once: twice the code, whose fetches cost more than the states
 // of the first half do once more).  Sums over a channel's states are dealt out over its lanes, sums over channels over the lanes with
 // channels of their own, then over the block's warps through shared memory; the blocks' shares of dB, dC, dA, dD and the bias's
 // gradient go to the workspace and are joined in a fixed order.  Segments: as in the forward, from the last token on.
@@ -85,24 +85,28 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
       for (int half = 1; half >= 0; --half) {
         const int k2 = half ^ 1;  // results alternate
         F2 h[S::CC][2], before[SEL_HALF / 2][S::CC][2];  // the states that the half's tokens 0, 2, 4, 6 find
+        F2 decay[SEL_HALF][S::CC][2];
 #pragma unroll
         for (int k = 0; k < S::CC; ++k) h[k][0] = h0[k][0], h[k][1] = h0[k][1];
         const float4* du = &sm.du[i & 1][0][me.ch];
         const float* bp = &sm.bc[i & 1][1][0][4 * me.sl];
         uint32_t mark = marks;
-        auto step = [&](int r) {
+        auto step = [&](int r, F2 (&a)[S::CC][2]) {
           const float4 b = *reinterpret_cast<const float4*>(bp + r * NP);
 #pragma unroll
           for (int k = 0; k < S::CC; ++k) {
             const float4 q = du[r * S::CH + k];
             if (MARKS && mark >> r & 1) h[k][0] = h[k][1] = f2(0.f);
-            h[k][0] = f2fma(ex2(f2mul(A[k][0], f2(q.x, q.y))), h[k][0], f2mul(f2(q.z, q.w), f2(b.x, b.y)));
-            h[k][1] = f2fma(ex2(f2mul(A[k][1], f2(q.x, q.y))), h[k][1], f2mul(f2(q.z, q.w), f2(b.z, b.w)));
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              a[k][n] = ex2(f2mul(A[k][n], f2(q.x, q.y)));
+              h[k][n] = f2fma(a[k][n], h[k][n], f2mul(f2(q.z, q.w), n ? f2(b.z, b.w) : f2(b.x, b.y)));
+            }
           }
         };
         if (half) {
 #pragma unroll 4
-          for (int r = 0; r < SEL_HALF; ++r) step(r);
+          for (int r = 0; r < SEL_HALF; ++r) step(r, decay[0]);
           du += SEL_HALF * S::CH;
           bp += SEL_HALF * NP;
           mark >>= SEL_HALF;
@@ -115,13 +119,13 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
           if (r % 2 == 0)
 #pragma unroll
             for (int k = 0; k < S::CC; ++k) before[r / 2][k][0] = h[k][0], before[r / 2][k][1] = h[k][1];
-          step(r);
+          step(r, decay[r]);
         }
 #pragma unroll
         for (int r0 = SEL_HALF - 2; r0 >= 0; r0 -= 2) {
           asm volatile("" ::: "memory");
           float into[2 * S::CC], rate[2 * S::CC], yd[2 * S::CC];
-          F2 decay[S::CC][2], mid[S::CC][2];  // of token r0; the state behind it
+          F2 mid[S::CC][2];  // the state behind token r0
           {
             const float4 b = *reinterpret_cast<const float4*>(bp + r0 * NP);
 #pragma unroll
@@ -129,9 +133,8 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
               const float4 q = du[r0 * S::CH + k];
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
-                decay[k][n] = ex2(f2mul(A[k][n], f2(q.x, q.y)));
                 mid[k][n] = f2mul(f2(q.z, q.w), n ? f2(b.z, b.w) : f2(b.x, b.y));
-                if (!(MARKS && mark >> r0 & 1)) mid[k][n] = f2fma(decay[k][n], before[r0 / 2][k][n], mid[k][n]);
+                if (!(MARKS && mark >> r0 & 1)) mid[k][n] = f2fma(decay[r0][k][n], before[r0 / 2][k][n], mid[k][n]);
               }
             }
           }
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
                 in = n ? f2fma(dh[k][n], bv[n], in) : f2mul(dh[k][n], bv[n]);
                 ys = n ? f2fma(h[k][n], cv[n], ys) : f2mul(h[k][n], cv[n]);
                 h[k][n] = u ? mid[k][n] : before[r0 / 2][k][n];
-                dh[k][n] = f2mul(dh[k][n], u ? ex2(f2mul(A[k][n], d)) : decay[k][n]);
+                dh[k][n] = f2mul(dh[k][n], decay[r][k][n]);
                 F2 way = f2mul(dh[k][n], h[k][n]);
                 if (MARKS && mark >> r & 1) dh[k][n] = way = f2(0.f);
                 ra = n ? f2fma(way, A[k][n], ra) : f2mul(way, A[k][n]);

@@ -19,8 +19,8 @@ struct SelBwdSmem {
   using S = SelShape<NP>;
   alignas(16) T raw[SEL_STAGES][4][SEL_TILE][S::CH];    // dt, gradient of y, z, x
   alignas(16) T raw_bc[SEL_STAGES][2][SEL_TILE][NP];    // c, b
-  alignas(16) float4 du[2][SEL_TILE][S::CH];            // step and step x, twice each, as operands of packed operations
-  alignas(16) float2 g[2][SEL_TILE][S::CH];             // gradient of the result before the gate, twice
+  alignas(16) float2 du[2][SEL_TILE][S::CH];            // step, step x
+  alignas(16) float g[2][SEL_TILE][S::CH];              // gradient of the result before the gate
   alignas(16) float bc[2][2][SEL_TILE][NP];             // c, b
   alignas(16) float res[2][3][SEL_HALF][S::PITCH];      // <dh, B>, <e, A log2 e>, <C, h>
   alignas(16) float part[2][SEL_THREADS / 32][SEL_HALF][2 * NP];  // dB, dC
@@ -88,19 +88,28 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
         F2 decay[SEL_HALF][S::CC][2];
 #pragma unroll
         for (int k = 0; k < S::CC; ++k) h[k][0] = h0[k][0], h[k][1] = h0[k][1];
-        const float4* du = &sm.du[i & 1][0][me.ch];
+        const float2* du = &sm.du[i & 1][0][me.ch];
         const float* bp = &sm.bc[i & 1][1][0][4 * me.sl];
         uint32_t mark = marks;
+        auto channels = [&](float2 (&q)[S::CC], const float2* at) {  // of the thread's channels
+          if constexpr (S::CC == 2) {
+            const float4 e = *reinterpret_cast<const float4*>(at);
+            q[0] = make_float2(e.x, e.y), q[1] = make_float2(e.z, e.w);
+          } else {
+            q[0] = *at;
+          }
+        };
         auto step = [&](int r, F2 (&a)[S::CC][2]) {
           const float4 b = *reinterpret_cast<const float4*>(bp + r * NP);
+          float2 q[S::CC];
+          channels(q, du + r * S::CH);
 #pragma unroll
           for (int k = 0; k < S::CC; ++k) {
-            const float4 q = du[r * S::CH + k];
             if (MARKS && mark >> r & 1) h[k][0] = h[k][1] = f2(0.f);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              a[k][n] = ex2(f2mul(A[k][n], f2(q.x, q.y)));
-              h[k][n] = f2fma(a[k][n], h[k][n], f2mul(f2(q.z, q.w), n ? f2(b.z, b.w) : f2(b.x, b.y)));
+              a[k][n] = ex2(f2mul(A[k][n], f2(q[k].x)));
+              h[k][n] = f2fma(a[k][n], h[k][n], f2mul(f2(q[k].y), n ? f2(b.z, b.w) : f2(b.x, b.y)));
             }
           }
         };
@@ -112,7 +121,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
           mark >>= SEL_HALF;
         }
         const float* cp = bp - SEL_TILE * NP;
-        const float2* gp = &sm.g[i & 1][half * SEL_HALF][me.ch];
+        const float* gp = &sm.g[i & 1][half * SEL_HALF][me.ch];
 #pragma unroll
         for (int r = 0; r < SEL_HALF; ++r) {
           if (r % 4 == 0) asm volatile("" ::: "memory");  // (the loads of all tokens at once would not fit in the registers)
@@ -128,12 +137,13 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
           F2 mid[S::CC][2];  // the state behind token r0
           {
             const float4 b = *reinterpret_cast<const float4*>(bp + r0 * NP);
+            float2 q[S::CC];
+            channels(q, du + r0 * S::CH);
 #pragma unroll
             for (int k = 0; k < S::CC; ++k) {
-              const float4 q = du[r0 * S::CH + k];
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
-                mid[k][n] = f2mul(f2(q.z, q.w), n ? f2(b.z, b.w) : f2(b.x, b.y));
+                mid[k][n] = f2mul(f2(q[k].y), n ? f2(b.z, b.w) : f2(b.x, b.y));
                 if (!(MARKS && mark >> r0 & 1)) mid[k][n] = f2fma(decay[r0][k][n], before[r0 / 2][k][n], mid[k][n]);
               }
             }
@@ -143,11 +153,19 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
             const int r = r0 + u;
             const float4 c = *reinterpret_cast<const float4*>(cp + r * NP), b = *reinterpret_cast<const float4*>(bp + r * NP);
             const F2 cv[2] = {f2(c.x, c.y), f2(c.z, c.w)}, bv[2] = {f2(b.x, b.y), f2(b.z, b.w)};
+            float2 q[S::CC];
+            channels(q, du + r * S::CH);
+            float g[S::CC];
+            if constexpr (S::CC == 2) {
+              const float2 e = *reinterpret_cast<const float2*>(gp + r * S::CH);
+              g[0] = e.x, g[1] = e.y;
+            } else {
+              g[0] = gp[r * S::CH];
+            }
             F2 db[2], dc[2];
 #pragma unroll
             for (int k = 0; k < S::CC; ++k) {
-              const float4 q = du[r * S::CH + k];
-              const F2 d = f2(q.x, q.y), v = f2(q.z, q.w), gk = gp[r * S::CH + k];
+              const F2 d = f2(q[k].x), v = f2(q[k].y), gk = f2(g[k]);
               F2 in, ra, ys;
 #pragma unroll
               for (int n = 0; n < 2; ++n) {
@@ -245,9 +263,8 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
         gv = f2mul(gv, f2(act_of(zv.x, ACT_SILU), act_of(zv.y, ACT_SILU)));
       }
       const F2 v = f2mul(d, pair_of(&sm.raw[k][3][r][2 * pr]));
-      sm.du[i & 1][r][2 * pr] = make_float4(d.x, d.x, v.x, v.x);
-      sm.du[i & 1][r][2 * pr + 1] = make_float4(d.y, d.y, v.y, v.y);
-      *reinterpret_cast<float4*>(&sm.g[i & 1][r][2 * pr]) = make_float4(gv.x, gv.x, gv.y, gv.y);
+      *reinterpret_cast<float4*>(&sm.du[i & 1][r][2 * pr]) = make_float4(d.x, v.x, d.y, v.y);
+      *reinterpret_cast<float2*>(&sm.g[i & 1][r][2 * pr]) = gv;
     }
 #pragma unroll
     for (int e = tid; e < 2 * SEL_TILE * NP; e += SEL_THREADS) (&sm.bc[i & 1][0][0][0])[e] = ld_as_float<T>(&sm.raw_bc[k][0][0][0], e);
@@ -265,12 +282,11 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
 #pragma unroll 2
       for (int r = row0; r < SEL_HALF; r += S::ROWS) {
         if (r >= left) break;
-        const float4 gg = *reinterpret_cast<const float4*>(&sm.g[i & 1][base + r][2 * pr]);
-        const F2 xv = pair_of(&sm.raw[k][3][base + r][2 * pr]), gv = f2(gg.x, gg.z);
+        const F2 xv = pair_of(&sm.raw[k][3][base + r][2 * pr]), gv = *reinterpret_cast<const float2*>(&sm.g[i & 1][base + r][2 * pr]);
         const F2 in = *reinterpret_cast<const float2*>(&sm.res[k2][0][r][2 * pr]);
-        const F2 q = f2(sm.du[i & 1][base + r][2 * pr].x, sm.du[i & 1][base + r][2 * pr + 1].x);
+        const float4 q = *reinterpret_cast<const float4*>(&sm.du[i & 1][base + r][2 * pr]);
         const int64_t row = (at.b * p.T + t0 + r) * p.C + at.c0 + 2 * pr;
-        put_pair<T>(static_cast<T*>(p.gx) + row, f2fma(q, in, f2mul(skip, gv)), pair_have, whole);
+        put_pair<T>(static_cast<T*>(p.gx) + row, f2fma(f2(q.x, q.z), in, f2mul(skip, gv)), pair_have, whole);
         F2 dd = f2fma(*reinterpret_cast<const float2*>(&sm.res[k2][1][r][2 * pr]), f2(LN2), f2mul(in, xv));
         if (p.softplus) {
           const F2 v = f2add(pair_of(&sm.raw[k][0][base + r][2 * pr]), bias);

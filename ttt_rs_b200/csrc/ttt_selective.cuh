@@ -29,8 +29,29 @@ struct SelShape {
   static constexpr int CH = WARP_CH * (SEL_THREADS / 32);  // of a block: 128, 64, 64, 32, 16
   static constexpr int PAIRS = CH / 2;
   static constexpr int ROWS = SEL_THREADS / PAIRS;         // tokens that the block's threads cover, pair by pair
-  static constexpr int PITCH = CH + 16;            // floats between tokens of results: two tokens' channels in different banks
+  static constexpr int SHARES = SL * CH;           // floats of a token's results as the scanning lanes have them
 };
+
+// The lanes' shares of a token's results in shared memory: lane sl's of the pair (or, CC = 1, the channel) of channels `e` at e SL + sl
+// pairs (floats), lanes of a pair in an order by which sixteen neighbouring pairs lie in different banks.
+template <int NP>
+__device__ __forceinline__ int share_at(int e, int sl) {
+  using S = SelShape<NP>;
+  if constexpr (S::CC == 1) return e * S::SL + sl;
+  else return 2 * (e * S::SL + (sl ^ (e / (16 / S::SL) & (S::SL - 1))));
+}
+// a pair's sum over its lanes
+template <int NP>
+__device__ __forceinline__ F2 sum_shares(const float* row, int pr) {
+  using S = SelShape<NP>;
+  F2 v = f2(0.f);
+#pragma unroll 4
+  for (int l = 0; l < S::SL; ++l) {
+    if constexpr (S::CC == 2) v = f2add(v, *reinterpret_cast<const float2*>(row + share_at<NP>(pr, l)));
+    else v = f2add(v, f2(row[share_at<NP>(2 * pr, l)], row[share_at<NP>(2 * pr + 1, l)]));
+  }
+  return v;
+}
 
 // log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1].  log(1 + e) / e is a polynomial of degree 8, fitted on [0, 1] for
 // the least largest relative error (3.0e-8): accurate relative to small steps too, which a logarithm of 1 + e is not, and without a

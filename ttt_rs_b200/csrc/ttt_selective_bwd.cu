@@ -22,7 +22,7 @@ struct SelBwdSmem {
   alignas(16) float2 du[2][SEL_TILE][S::CH];            // step, step x
   alignas(16) float g[2][SEL_TILE][S::CH];              // gradient of the result before the gate
   alignas(16) float bc[2][2][SEL_TILE][NP];             // c, b
-  alignas(16) float res[2][3][SEL_HALF][S::PITCH];      // <dh, B>, <e, A log2 e>, <C, h>
+  alignas(16) float res[2][3][SEL_HALF][S::SHARES]; // shares of <dh, B>, <e, A log2 e>, <C, h>, as the scanning lanes lie
   alignas(16) float part[2][SEL_THREADS / 32][SEL_HALF][2 * NP];  // dB, dC
   uint32_t mark[2];
 };
@@ -61,6 +61,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
     // ---- scan
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const SelLane<NP> me;
+    const int my_share = share_at<NP>(me.ch / S::CC, me.sl);
     F2 A[S::CC][2], dh[S::CC][2], dA[S::CC][2];
     me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
 #pragma unroll
@@ -133,7 +134,6 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
 #pragma unroll
         for (int r0 = SEL_HALF - 2; r0 >= 0; r0 -= 2) {
           asm volatile("" ::: "memory");
-          float into[2 * S::CC], rate[2 * S::CC], yd[2 * S::CC];
           F2 mid[S::CC][2];  // the state behind token r0
           {
             const float4 b = *reinterpret_cast<const float4*>(bp + r0 * NP);
@@ -163,6 +163,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
               g[0] = gp[r * S::CH];
             }
             F2 db[2], dc[2];
+            float share[3][S::CC];
 #pragma unroll
             for (int k = 0; k < S::CC; ++k) {
               const F2 d = f2(q[k].x), v = f2(q[k].y), gk = f2(g[k]);
@@ -181,9 +182,14 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
                 ra = n ? f2fma(way, A[k][n], ra) : f2mul(way, A[k][n]);
                 dA[k][n] = f2fma(way, d, dA[k][n]);
               }
-              into[u * S::CC + k] = f2hsum(in);
-              rate[u * S::CC + k] = f2hsum(ra);
-              yd[u * S::CC + k] = f2hsum(ys);
+              share[0][k] = f2hsum(in);
+              share[1][k] = f2hsum(ra);
+              share[2][k] = f2hsum(ys);
+            }
+#pragma unroll
+            for (int m = 0; m < 3; ++m) {
+              if constexpr (S::CC == 2) *reinterpret_cast<float2*>(&sm.res[k2][m][r][my_share]) = make_float2(share[m][0], share[m][1]);
+              else sm.res[k2][m][r][my_share] = share[m][0];
             }
             float sums[8] = {db[0].x, db[0].y, db[1].x, db[1].y, dc[0].x, dc[0].y, dc[1].x, dc[1].y};
             sum_and_deal<8, S::CL, S::SL>(sums, me.lane);
@@ -196,19 +202,6 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
                 const int e = first + e0;  // dB of states 4 sl .. 4 sl + 3, then dC of them
                 sm.part[k2][threadIdx.x >> 5][r][(e >= 4 ? NP : 0) + 4 * me.sl + (e & 3)] = sums[e0];
               }
-            }
-          }
-          // a channel's lanes share its sums out: (token, channel) by (token, channel)
-          constexpr int DEAL = 2 * S::CC, GOT = S::SL >= DEAL ? 1 : DEAL / S::SL, SHARED = S::SL >= DEAL ? S::SL / DEAL : 1;
-          sum_and_deal<DEAL, S::SL, 1>(into, me.lane);
-          sum_and_deal<DEAL, S::SL, 1>(rate, me.lane);
-          sum_and_deal<DEAL, S::SL, 1>(yd, me.lane);
-          const int first = S::SL >= DEAL ? me.sl / SHARED : me.sl * GOT;
-          if (SHARED == 1 || me.sl % SHARED == 0) {
-#pragma unroll
-            for (int e0 = 0; e0 < GOT; ++e0) {
-              const int r = r0 + (first + e0) / S::CC, c = me.ch + (first + e0) % S::CC;
-              sm.res[k2][0][r][c] = into[e0], sm.res[k2][1][r][c] = rate[e0], sm.res[k2][2][r][c] = yd[e0];
             }
           }
         }
@@ -283,11 +276,11 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
       for (int r = row0; r < SEL_HALF; r += S::ROWS) {
         if (r >= left) break;
         const F2 xv = pair_of(&sm.raw[k][3][base + r][2 * pr]), gv = *reinterpret_cast<const float2*>(&sm.g[i & 1][base + r][2 * pr]);
-        const F2 in = *reinterpret_cast<const float2*>(&sm.res[k2][0][r][2 * pr]);
+        const F2 in = sum_shares<NP>(sm.res[k2][0][r], pr);
         const float4 q = *reinterpret_cast<const float4*>(&sm.du[i & 1][base + r][2 * pr]);
         const int64_t row = (at.b * p.T + t0 + r) * p.C + at.c0 + 2 * pr;
         put_pair<T>(static_cast<T*>(p.gx) + row, f2fma(f2(q.x, q.z), in, f2mul(skip, gv)), pair_have, whole);
-        F2 dd = f2fma(*reinterpret_cast<const float2*>(&sm.res[k2][1][r][2 * pr]), f2(LN2), f2mul(in, xv));
+        F2 dd = f2fma(sum_shares<NP>(sm.res[k2][1][r], pr), f2(LN2), f2mul(in, xv));
         if (p.softplus) {
           const F2 v = f2add(pair_of(&sm.raw[k][0][base + r][2 * pr]), bias);
           dd = f2mul(dd, f2(sigmoid_of(v.x), sigmoid_of(v.y)));
@@ -299,7 +292,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
           const float2 zv = pair_of(&sm.raw[k][2][base + r][2 * pr]);
           F2 slope;
           act_and_slope(zv.x, ACT_SILU, slope.x), act_and_slope(zv.y, ACT_SILU, slope.y);
-          const F2 y = f2fma(skip, xv, *reinterpret_cast<const float2*>(&sm.res[k2][2][r][2 * pr]));
+          const F2 y = f2fma(skip, xv, sum_shares<NP>(sm.res[k2][2][r], pr));
           put_pair<T>(static_cast<T*>(p.gz) + row, f2mul(f2mul(pair_of(&sm.raw[k][1][base + r][2 * pr]), y), slope), pair_have, whole);
         }
       }

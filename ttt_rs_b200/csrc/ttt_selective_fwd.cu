@@ -15,7 +15,7 @@ struct SelSmem {
   alignas(16) T raw_bc[SEL_STAGES][FULL ? 2 : 1][SEL_TILE][NP];
   alignas(16) float4 du[2][SEL_TILE][S::PAIRS];             // (step, step x) of two channels
   alignas(16) float bc[2][FULL ? 2 : 1][SEL_TILE][NP];
-  alignas(16) float y[2][FULL ? SEL_TILE : 1][S::SL * S::CH];  // shares of a result, as the scanning lanes lie
+  alignas(16) float y[2][FULL ? SEL_TILE : 1][S::SHARES];  // shares of a result, as the scanning lanes lie
   uint32_t mark[2];                                         // starts of a tile, bit by bit
 };
 
@@ -31,6 +31,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
   if (threadIdx.x < SEL_THREADS) {
     // ---- scan
     const SelLane<NP> me;
+    [[maybe_unused]] const int my_share = share_at<NP>(me.ch / S::CC, me.sl);
     F2 A[S::CC][2], h[S::CC][2];
     me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
 #pragma unroll
@@ -92,9 +93,9 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
           h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
           if constexpr (FULL) part[k] = f2hsum(f2fma(h[k][0], f2(c.x, c.y), f2mul(h[k][1], f2(c.z, c.w))));
         }
-        if constexpr (FULL) {  // [pair][lane of its channels][channel]
-          if constexpr (S::CC == 2) *reinterpret_cast<float2*>(&sm.y[i & 1][r][2 * threadIdx.x]) = make_float2(part[0], part[1]);
-          else sm.y[i & 1][r][threadIdx.x] = part[0];
+        if constexpr (FULL) {
+          if constexpr (S::CC == 2) *reinterpret_cast<float2*>(&sm.y[i & 1][r][my_share]) = make_float2(part[0], part[1]);
+          else sm.y[i & 1][r][my_share] = part[0];
         }
       }
       __syncthreads();
@@ -172,14 +173,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
 #pragma unroll
     for (int r = row0; r < SEL_TILE; r += S::ROWS, y += (int64_t)S::ROWS * p.C) {
       if (r >= left) break;
-      F2 v = f2(0.f);
-      if constexpr (S::CC == 2) {
-#pragma unroll
-        for (int l = 0; l < S::SL; ++l) v = f2add(v, *reinterpret_cast<const float2*>(&sm.y[i & 1][r][2 * (pr * S::SL + l)]));
-      } else {
-#pragma unroll
-        for (int l = 0; l < S::SL; ++l) v = f2add(v, f2(sm.y[i & 1][r][2 * pr * S::SL + l], sm.y[i & 1][r][(2 * pr + 1) * S::SL + l]));
-      }
+      F2 v = sum_shares<NP>(sm.y[i & 1][r], pr);
       v = f2fma(skip, pair_of(&sm.raw[k][0][r][2 * pr]), v);
       if (z != nullptr) {
         const float2 zv = pair_of(&sm.raw[k][Smem::TENSORS - 1][r][2 * pr]);

@@ -101,8 +101,8 @@ extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t cha
   s.need("y", y);
   s.need("state_out", state_out);
   s.align("state", state);
-  const bool vec = s.low % 16 == 0 && channels * es % 16 == 0;
   s.need("weight", weight);
+  const bool vec = s.low % (4 * es) == 0 && channels % 4 == 0;
   s.align("bias", bias);
   if (s.rc != TTT_OK) return s.rc;
   const int64_t held = batch * (taps - 1) * channels * es, n = batch * seq_len * channels * es;
@@ -118,7 +118,7 @@ extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t cha
   p.x = x, p.w = weight, p.bias = bias, p.state = state, p.starts = static_cast<const uint8_t*>(starts);
   p.y = y, p.state_out = state_out;
   p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
-  return launched(ttt::launch_conv(dtype, p, taps, vec, static_cast<cudaStream_t>(stream)), "causal convolution");
+  return launched(ttt::launch_conv(dtype, p, taps, vec, false, static_cast<cudaStream_t>(stream)), "causal convolution");
 }
 
 extern "C" size_t ttt_layer_causal_conv_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype) {
@@ -142,8 +142,8 @@ extern "C" int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, in
   s.align("state", state);
   s.align("grad_state_out", grad_state_out);
   s.align("grad_state", grad_state);
-  const bool vec = s.low % 16 == 0 && channels * es % 16 == 0;
   s.need("weight", weight);
+  const bool vec = s.low % (4 * es) == 0 && channels % 4 == 0;
   s.align("bias", bias);
   s.align("grad_weight", grad_weight);
   s.align("grad_bias", grad_bias);
@@ -156,7 +156,7 @@ extern "C" int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, in
   p.gy = grad_y, p.gstate_out = grad_state_out, p.gx = grad_x, p.gstate = grad_state, p.gw = grad_weight, p.gbias = grad_bias;
   p.partials = sums ? static_cast<float*>(workspace) : nullptr;
   p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
-  return launched(ttt::launch_conv_bwd(dtype, p, taps, vec, static_cast<cudaStream_t>(stream)), "causal convolution backward");
+  return launched(ttt::launch_conv(dtype, p, taps, vec, true, static_cast<cudaStream_t>(stream)), "causal convolution backward");
 }
 
 namespace {
@@ -177,7 +177,6 @@ void norm_dims(ttt::NormParams* p, int64_t B, int64_t T, int64_t C, int G, int a
   p->B = B, p->T = T, p->tokens = B * T, p->C = (int)C, p->G = G, p->c = (int)(C / G), p->act = activation, p->eps = eps;
   p->inv_c = 1.f / (float)p->c;
 }
-bool flat_rows(const int64_t (&s)[2], int64_t B, int64_t T) { return B == 1 || (T > 1 && s[0] == T * s[1]); }
 int norm_width(uintptr_t low, int c, int es) {
   if (low % 16 == 0 && c % (16 / es) == 0) return 16 / es;
   return low % (2 * es) == 0 && c % 2 == 0 ? 2 : 1;
@@ -213,7 +212,6 @@ extern "C" int ttt_layer_group_norm(int64_t batch, int64_t seq_len, int64_t chan
   if ((rc = check_bytes(workspace_bytes, ttt_layer_group_norm_workspace_bytes(batch, seq_len, channels, groups, over, dtype), workspace,
                         "workspace")) != TTT_OK)
     return rc;
-  p.flat = flat_rows(p.xs, batch, seq_len) && (gate == nullptr || flat_rows(p.gates, batch, seq_len));
   p.x = x, p.gate = gate, p.w = weight, p.bias = bias, p.y = y, p.stats = stats, p.moments = static_cast<float*>(workspace);
   return launched(ttt::launch_norm(dtype, p, norm_width(s.low, p.c, es), over == TTT_OVER_SEQUENCE, false, static_cast<cudaStream_t>(stream)),
                   "group norm");
@@ -248,7 +246,6 @@ extern "C" int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int
   if (sums && (rc = check_bytes(workspace_bytes, ttt_layer_group_norm_backward_workspace_bytes(batch, seq_len, channels, groups, over, dtype),
                                 workspace, "workspace")) != TTT_OK)
     return rc;
-  p.flat = flat_rows(p.xs, batch, seq_len) && flat_rows(p.gys, batch, seq_len) && (gate == nullptr || flat_rows(p.gates, batch, seq_len));
   p.x = x, p.gate = gate, p.gy = grad_y, p.w = weight, p.bias = bias, p.stats = const_cast<float*>(stats);
   p.gx = grad_x, p.ggate = grad_gate, p.gw = grad_weight, p.gb = grad_bias;
   p.partials = sums ? static_cast<float*>(workspace) : nullptr;

@@ -504,8 +504,8 @@ struct ConvParams {
   int64_t strips;
 };
 size_t conv_partial_floats(int64_t B, int64_t T, int C, int K);
-cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, bool vec, cudaStream_t st);
-cudaError_t launch_conv_bwd(int dtype, const ConvParams& p, int taps, bool vec, cudaStream_t st);
+// vec: channels are a multiple of 4, and all addresses of 4 channels
+cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, bool vec, bool bwd, cudaStream_t st);
 
 // ---- group norm (ttt_norm.cu): tensors [B,T,C] with contiguous channels ------------------------------------------------------------
 struct NormParams {
@@ -519,7 +519,6 @@ struct NormParams {
   float* sums;                       // set by the launch, like all below G
   int64_t xs[2], gates[2], gys[2];   // strides of batch and token, in elements
   int64_t B, T, tokens;
-  bool flat;                         // rows of x, gate and gy are one token stride apart throughout
   int C, G, c, act;
   float eps, inv_c;
   int lanes, cols, rows, per_block, spans, chunks;

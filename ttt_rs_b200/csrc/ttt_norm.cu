@@ -19,14 +19,46 @@
 namespace ttt {
 
 constexpr int NORM_THREADS = 256;
+constexpr int NORM_FWD_RESIDENT = 4, NORM_BWD_RESIDENT = 2, NORM_SEQ_RESIDENT = 3;  // blocks of 256 threads per SM that registers are bounded for
+constexpr int NORM_BWD_AHEAD = 2;  // tokens on their way at a time
 constexpr int NORM_EACH = 8;  // channels per thread, a token's groups
 constexpr int NORM_WIDE = NORM_TOKEN_CHANNELS / NORM_EACH;  // threads at most, of groups that several warps share
 
-__device__ __forceinline__ int64_t norm_row(const NormParams& p, int64_t token, const int64_t (&s)[2]) {
-  if (p.flat) return token * s[1];
-  const int64_t b = token / p.T;
-  return b * s[0] + (token - b * p.T) * s[1];
+// What a kernel knows of the call when it is built: everything at run time, SiLU without a gate, or a gate with SiLU
+enum : int { NORM_GENERAL = 0, NORM_SILU = 1, NORM_GATED_SILU = 2 };
+template <int MODE>
+__device__ __forceinline__ bool norm_gated(const NormParams& p) {
+  return MODE == NORM_GATED_SILU || (MODE == NORM_GENERAL && p.gate != nullptr);
 }
+template <int MODE>
+__device__ __forceinline__ int norm_act(const NormParams& p) {
+  return MODE == NORM_GENERAL ? p.act : ACT_SILU;
+}
+// A place among the tokens, walked in steps: its offsets in x, the gate and the result's gradient
+struct NormWalk {
+  uint32_t t;  // of its sequence
+  int64_t x, gate, gy;
+  __device__ __forceinline__ NormWalk(const NormParams& p, int64_t token) {
+    const int64_t b = token / p.T;
+    t = (uint32_t)(token - b * p.T);
+    x = b * p.xs[0] + t * p.xs[1];
+    gate = b * p.gates[0] + t * p.gates[1];
+    gy = b * p.gys[0] + t * p.gys[1];
+  }
+  __device__ __forceinline__ void step(const NormParams& p, uint32_t by) {
+    t += by;
+    x += by * p.xs[1];
+    gate += by * p.gates[1];
+    gy += by * p.gys[1];
+    if (t >= (uint32_t)p.T) {
+      const uint32_t rows = t / (uint32_t)p.T;
+      t -= rows * (uint32_t)p.T;
+      x += rows * (p.xs[0] - p.T * p.xs[1]);
+      gate += rows * (p.gates[0] - p.T * p.gates[1]);
+      gy += rows * (p.gys[0] - p.T * p.gys[1]);
+    }
+  }
+};
 
 // sum over the lanes of a group; wide: over its warps too (red: a float per warp, all threads of the block take part)
 template <bool WIDE>
@@ -90,41 +122,44 @@ __device__ __forceinline__ float norm_stats(F2 (&d)[NormLane<T, V>::NV][NormLane
   return rsqrtf(norm_sum<WIDE>(f2hsum(q), p.lanes, red) * p.inv_c + p.eps);
 }
 
-template <typename T, int V, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_token_kernel(const NormParams p) {
+template <typename T, int V, bool WIDE, int MODE>
+__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NORM_FWD_RESIDENT) ttt_norm_token_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   using L = NormLane<T, V>;
-  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE ? 1 : sizeof(T) == 2 ? 4 : 2;
+  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE || V == 1 || sizeof(T) == 4 ? 1 : 2;
   __shared__ float red[32];
   const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
-  const int g = gcol / p.lanes, l = gcol & (p.lanes - 1);
-  const bool live = row < p.rows && g < p.G;
+  const int g = gcol / p.lanes, l = gcol & (p.lanes - 1), act = norm_act<MODE>(p);
+  const bool live = row < p.rows && g < p.G, gated = norm_gated<MODE>(p);
   L me;
   me.set(p, g, l, live);
   const T* x = static_cast<const T*>(p.x) + me.c0;
   const T* gate = static_cast<const T*>(p.gate) + me.c0;
-  T* y = static_cast<T*>(p.y) + me.c0;
-  for (int64_t base = (int64_t)blockIdx.x * p.rows; base < p.tokens; base += (int64_t)gridDim.x * p.rows * AHEAD) {
+  const uint32_t step = gridDim.x * p.rows;
+  int64_t token = (int64_t)blockIdx.x * p.rows + row;
+  T* y = static_cast<T*>(p.y) + token * p.C + me.c0;
+  NormWalk at(p, token);
+  for (int64_t base = (int64_t)blockIdx.x * p.rows; base < p.tokens; base += (int64_t)step * AHEAD) {
     Ch in[AHEAD][NV], gt[AHEAD][NV];
+    bool has[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
-      const bool has = live && t < p.tokens;
-      const int64_t xo = has ? norm_row(p, t, p.xs) : 0, go = has && p.gate != nullptr ? norm_row(p, t, p.gates) : 0;
+      has[u] = live && token < p.tokens;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         in[u][n].zero();
         gt[u][n].zero();
-        if (has && me.at[n] >= 0) {
-          in[u][n].load(x + xo + me.at[n]);
-          if (p.gate != nullptr) gt[u][n].load(gate + go + me.at[n]);
+        if (has[u] && me.at[n] >= 0) {
+          in[u][n].load(x + at.x + me.at[n]);
+          if (gated) gt[u][n].load(gate + at.gate + me.at[n]);
         }
       }
+      token += step;
+      at.step(p, step);
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
-      if (base + (int64_t)u * gridDim.x * p.rows >= p.tokens) break;  // (the whole block)
+      if (u > 0 && base + (int64_t)u * step >= p.tokens) break;  // (the whole block)
       F2 d[NV][P];
 #pragma unroll
       for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
@@ -136,65 +171,67 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_toke
 #pragma unroll
         for (int k = 0; k < P; ++k) {
           const F2 v = f2fma(f2mul(d[n][k], f2(r)), me.w[n][k], me.b[n][k]);
-          if (p.gate != nullptr) d[n][k] = f2mul(v, f2(act_of(e[k].x, p.act), act_of(e[k].y, p.act)));
-          else d[n][k] = f2(act_of(v.x, p.act), act_of(v.y, p.act));
+          if (gated) d[n][k] = f2mul(v, f2(act_of(e[k].x, act), act_of(e[k].y, act)));
+          else d[n][k] = f2(act_of(v.x, act), act_of(v.y, act));
         }
-        if (live && t < p.tokens && me.at[n] >= 0) {
+        if (has[u] && me.at[n] >= 0) {
           Ch out;
           out.pack(d[n]);
-          out.store(y + t * p.C + me.at[n]);
+          out.store(y + me.at[n]);
         }
       }
+      y += (int64_t)step * p.C;
     }
   }
 }
 
-template <typename T, int V, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_token_bwd_kernel(const NormParams p) {
+template <typename T, int V, bool WIDE, int MODE>
+__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NORM_BWD_RESIDENT) ttt_norm_token_bwd_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   using L = NormLane<T, V>;
-  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE ? 1 : sizeof(T) == 2 ? 2 : 1;
+  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE || V == 1 || sizeof(T) == 4 ? 1 : NORM_BWD_AHEAD;
   __shared__ float red[32];
   const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
-  const int g = gcol / p.lanes, l = gcol & (p.lanes - 1);
-  const bool live = row < p.rows && g < p.G;
+  const int g = gcol / p.lanes, l = gcol & (p.lanes - 1), act = norm_act<MODE>(p);
+  const bool live = row < p.rows && g < p.G, gated = norm_gated<MODE>(p);
   L me;
   me.set(p, g, l, live);
   const T* x = static_cast<const T*>(p.x) + me.c0;
   const T* gate = static_cast<const T*>(p.gate) + me.c0;
   const T* gy = static_cast<const T*>(p.gy) + me.c0;
-  T* gx = static_cast<T*>(p.gx) + me.c0;
-  T* ggate = static_cast<T*>(p.ggate) + me.c0;
+  const uint32_t step = gridDim.x * p.rows;
+  int64_t token = (int64_t)blockIdx.x * p.rows + row, to = token * p.C + me.c0;
+  T* gx = static_cast<T*>(p.gx);
+  T* ggate = static_cast<T*>(p.ggate);
+  NormWalk at(p, token);
   F2 dw[NV][P], db[NV][P];
 #pragma unroll
   for (int n = 0; n < NV; ++n)
 #pragma unroll
     for (int k = 0; k < P; ++k) dw[n][k] = db[n][k] = f2(0.f);
-  for (int64_t base = (int64_t)blockIdx.x * p.rows; base < p.tokens; base += (int64_t)gridDim.x * p.rows * AHEAD) {
+  for (int64_t base = (int64_t)blockIdx.x * p.rows; base < p.tokens; base += (int64_t)step * AHEAD) {
     Ch in[AHEAD][NV], gt[AHEAD][NV], gr[AHEAD][NV];
+    bool has[AHEAD];
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
-      const bool has = live && t < p.tokens;
-      const int64_t xo = has ? norm_row(p, t, p.xs) : 0, go = has && p.gate != nullptr ? norm_row(p, t, p.gates) : 0;
-      const int64_t yo = has ? norm_row(p, t, p.gys) : 0;
+      has[u] = live && token < p.tokens;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         in[u][n].zero();
         gt[u][n].zero();
         gr[u][n].zero();
-        if (has && me.at[n] >= 0) {
-          in[u][n].load(x + xo + me.at[n]);
-          gr[u][n].load(gy + yo + me.at[n]);
-          if (p.gate != nullptr) gt[u][n].load(gate + go + me.at[n]);
+        if (has[u] && me.at[n] >= 0) {
+          in[u][n].load(x + at.x + me.at[n]);
+          gr[u][n].load(gy + at.gy + me.at[n]);
+          if (gated) gt[u][n].load(gate + at.gate + me.at[n]);
         }
       }
+      token += step;
+      at.step(p, step);
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int64_t t = base + (int64_t)u * gridDim.x * p.rows + row;
-      if (base + (int64_t)u * gridDim.x * p.rows >= p.tokens) break;  // (the whole block)
-      const bool has = live && t < p.tokens;
+      if (u > 0 && base + (int64_t)u * step >= p.tokens) break;  // (the whole block)
       F2 d[NV][P];
 #pragma unroll
       for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
@@ -210,14 +247,14 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_toke
           d[n][k] = f2mul(d[n][k], f2(r));  // n
           const F2 v = f2fma(d[n][k], me.w[n][k], me.b[n][k]);
           F2 a, slope;
-          if (p.gate != nullptr) {
-            a.x = act_and_slope(e[k].x, p.act, slope.x);
-            a.y = act_and_slope(e[k].y, p.act, slope.y);
+          if (gated) {
+            a.x = act_and_slope(e[k].x, act, slope.x);
+            a.y = act_and_slope(e[k].y, act, slope.y);
             dg[k] = f2mul(f2mul(du[k], v), slope);
             du[k] = f2mul(du[k], a);
           } else {
-            act_and_slope(v.x, p.act, slope.x);
-            act_and_slope(v.y, p.act, slope.y);
+            act_and_slope(v.x, act, slope.x);
+            act_and_slope(v.y, act, slope.y);
             du[k] = f2mul(du[k], slope);
           }
           dw[n][k] = f2fma(du[k], d[n][k], dw[n][k]);
@@ -226,10 +263,10 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_toke
           s1 = f2add(s1, q[n][k]);
           s2 = f2fma(q[n][k], d[n][k], s2);
         }
-        if (p.gate != nullptr && has && me.at[n] >= 0) {
+        if (gated && has[u] && me.at[n] >= 0) {
           Ch out;
           out.pack(dg);
-          out.store(ggate + t * p.C + me.at[n]);
+          out.store(ggate + to + me.at[n]);
         }
       }
       const float m1 = norm_sum<WIDE>(f2hsum(s1), p.lanes, red) * p.inv_c, m2 = norm_sum<WIDE>(f2hsum(s2), p.lanes, red) * p.inv_c;
@@ -237,12 +274,13 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_toke
       for (int n = 0; n < NV; ++n) {
 #pragma unroll
         for (int k = 0; k < P; ++k) q[n][k] = f2mul(f2fma(d[n][k], f2(-m2), f2add(q[n][k], f2(-m1))), f2(r));
-        if (has && me.at[n] >= 0) {
+        if (has[u] && me.at[n] >= 0) {
           Ch out;
           out.pack(q[n]);
-          out.store(gx + t * p.C + me.at[n]);
+          out.store(gx + to + me.at[n]);
         }
       }
+      to += (int64_t)step * p.C;
     }
   }
   if (p.partials == nullptr) return;
@@ -285,17 +323,10 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS) ttt_norm_toke
 
 // rows of partial sums [rows][2][C] -> weight's and bias's gradients, in a fixed order
 template <typename T>
-__global__ void __launch_bounds__(256) ttt_norm_reduce_kernel(const float* partials, int rows, int C, T* gw, T* gb) {
-  __shared__ float part[8][33];
-  const int col = (int)blockIdx.x * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
-  float v = 0.f;
-  if (col < 2 * C)
-    for (int r = share; r < rows; r += 8) v += partials[(int64_t)r * 2 * C + col];
-  part[share][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (share != 0 || col >= 2 * C) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x & 31];
+__global__ void __launch_bounds__(ROWS_THREADS) ttt_norm_reduce_kernel(const float* partials, int rows, int C, T* gw, T* gb) {
+  int64_t col;
+  float v;
+  if (!sum_of_rows(partials, rows, 2 * C, 2 * C, blockIdx.x, &col, &v)) return;
   if (col < C) {
     if (gw != nullptr) st_from_float<T>(gw, col, v);
   } else if (gb != nullptr) {
@@ -358,7 +389,7 @@ struct SeqPlace {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_stats_kernel(const NormParams p) {
+__global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_stats_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   constexpr int P = Ch::P, AHEAD = 4;
   __shared__ float sm[3][NORM_THREADS];
@@ -413,12 +444,14 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_stats_kernel(const 
   }
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_apply_kernel(const NormParams p) {
+template <typename T, int V, int MODE>
+__global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_apply_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   constexpr int P = Ch::P, AHEAD = 4;
   __shared__ float stat[NORM_THREADS][2];
   const SeqPlace at(p, V);
+  const bool gated = norm_gated<MODE>(p);
+  const int act = norm_act<MODE>(p);
   const int lane = threadIdx.x & 31;
   for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
     const float* m = p.moments + (at.b * p.G + at.g0 + k) * p.chunks * p.spans * 3;
@@ -457,7 +490,7 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_apply_kernel(const 
       gt[u].zero();
       if (t + (int64_t)u * p.rows < at.t_hi) {
         in[u].load(x + (t + (int64_t)u * p.rows) * p.xs[1]);
-        if (p.gate != nullptr) gt[u].load(gate + (t + (int64_t)u * p.rows) * p.gates[1]);
+        if (gated) gt[u].load(gate + (t + (int64_t)u * p.rows) * p.gates[1]);
       }
     }
 #pragma unroll
@@ -469,8 +502,8 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_apply_kernel(const 
 #pragma unroll
       for (int k = 0; k < P; ++k) {
         v[k] = f2fma(f2mul(f2add(v[k], f2(-mean)), f2(r)), w[k], b[k]);
-        if (p.gate != nullptr) v[k] = f2mul(v[k], f2(act_of(e[k].x, p.act), act_of(e[k].y, p.act)));
-        else v[k] = f2(act_of(v[k].x, p.act), act_of(v[k].y, p.act));
+        if (gated) v[k] = f2mul(v[k], f2(act_of(e[k].x, act), act_of(e[k].y, act)));
+        else v[k] = f2(act_of(v[k].x, act), act_of(v[k].y, act));
       }
       Ch out;
       out.pack(v);
@@ -481,34 +514,36 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_apply_kernel(const 
 
 // du and n of a thread's channels of one token, and the gate's gradient
 template <int P>
-__device__ __forceinline__ void norm_du(const NormParams& p, F2 (&n)[P], F2 (&du)[P], const F2 (&e)[P], F2 (&dg)[P], float mean, float r,
+__device__ __forceinline__ void norm_du(bool gated, int act, F2 (&n)[P], F2 (&du)[P], const F2 (&e)[P], F2 (&dg)[P], float mean, float r,
                                         const F2 (&w)[P], const F2 (&b)[P]) {
 #pragma unroll
   for (int k = 0; k < P; ++k) {
     n[k] = f2mul(f2add(n[k], f2(-mean)), f2(r));
     const F2 v = f2fma(n[k], w[k], b[k]);
     F2 a, slope;
-    if (p.gate != nullptr) {
-      a.x = act_and_slope(e[k].x, p.act, slope.x);
-      a.y = act_and_slope(e[k].y, p.act, slope.y);
+    if (gated) {
+      a.x = act_and_slope(e[k].x, act, slope.x);
+      a.y = act_and_slope(e[k].y, act, slope.y);
       dg[k] = f2mul(f2mul(du[k], v), slope);
       du[k] = f2mul(du[k], a);
     } else {
-      act_and_slope(v.x, p.act, slope.x);
-      act_and_slope(v.y, p.act, slope.y);
+      act_and_slope(v.x, act, slope.x);
+      act_and_slope(v.y, act, slope.y);
       du[k] = f2mul(du[k], slope);
     }
   }
 }
 
 // APPLY false: every channel's sums of du and du n over the chunk.  true: the gradients of x and the gate.
-template <typename T, int V, bool APPLY>
-__global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_bwd_kernel(const NormParams p) {
+template <typename T, int V, bool APPLY, int MODE>
+__global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_bwd_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   constexpr int P = Ch::P, AHEAD = 2;
   __shared__ float mean_of[NORM_THREADS][2];
   extern __shared__ float norm_smem[];  // APPLY false: [2][rows][cols][V]
   const SeqPlace at(p, V);
+  const bool gated = norm_gated<MODE>(p);
+  const int act = norm_act<MODE>(p);
   if constexpr (APPLY) {  // the groups' means of p and p n, from the channels' sums
     const int lane = threadIdx.x & 31;
     const float inv = 1.f / ((float)p.c * (float)p.T);
@@ -557,7 +592,7 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_bwd_kernel(const No
         if (tu < at.t_hi) {
           in[u].load(x + tu * p.xs[1]);
           gr[u].load(gy + tu * p.gys[1]);
-          if (p.gate != nullptr) gt[u].load(gate + tu * p.gates[1]);
+          if (gated) gt[u].load(gate + tu * p.gates[1]);
         }
       }
 #pragma unroll
@@ -568,14 +603,14 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_bwd_kernel(const No
         in[u].unpack(n);
         gr[u].unpack(du);
         gt[u].unpack(e);
-        norm_du<P>(p, n, du, e, dg, mean, r, w, b);
+        norm_du<P>(gated, act, n, du, e, dg, mean, r, w, b);
         if constexpr (APPLY) {
           Ch out;
 #pragma unroll
           for (int k = 0; k < P; ++k) du[k] = f2mul(f2fma(n[k], f2(-m2), f2fma(du[k], w[k], f2(-m1))), f2(r));
           out.pack(du);
           out.store(gx + tu * p.C);
-          if (p.gate != nullptr) {
+          if (gated) {
             out.pack(dg);
             out.store(ggate + tu * p.C);
           }
@@ -614,18 +649,11 @@ __global__ void __launch_bounds__(NORM_THREADS) ttt_norm_seq_bwd_kernel(const No
 }
 
 // the chunks' sums [B][chunks][2][C] (du n, du) -> [B][2][C] (du, du n)
-__global__ void __launch_bounds__(256) ttt_norm_seq_sums_kernel(const float* partials, float* sums, int chunks, int C, int column_blocks) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(ROWS_THREADS) ttt_norm_seq_sums_kernel(const float* partials, float* sums, int chunks, int C, int column_blocks) {
   const int64_t b = blockIdx.x / column_blocks;
-  const int col = (int)(blockIdx.x - b * column_blocks) * 32 + (threadIdx.x & 31), share = threadIdx.x >> 5;
-  float v = 0.f;
-  if (col < 2 * C)
-    for (int r = share; r < chunks; r += 8) v += partials[(b * chunks + r) * 2 * C + col];
-  part[share][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (share != 0 || col >= 2 * C) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x & 31];
+  int64_t col;
+  float v;
+  if (!sum_of_rows(partials + b * chunks * 2 * C, chunks, 2 * C, 2 * C, blockIdx.x - b * column_blocks, &col, &v)) return;
   sums[b * 2 * C + (col < C ? C + col : col - C)] = v;
 }
 
@@ -646,7 +674,9 @@ static NormCut norm_token_cut(int64_t tokens, int G, int c, bool bwd) {
   k.rows = k.cols < NORM_THREADS ? NORM_THREADS / k.cols : 1;
   k.threads = (k.cols * k.rows + 31) / 32 * 32;
   k.y = (int)((total + k.cols - 1) / k.cols);
-  const int64_t need = (tokens + k.rows - 1) / k.rows, wanted = 148 * (bwd ? 3 : 6) / k.y, most = wanted > 1 ? wanted : 1;
+  const int regs = 65536 / (NORM_THREADS * (bwd ? NORM_BWD_RESIDENT : NORM_FWD_RESIDENT));
+  const int64_t resident = k.threads > NORM_THREADS ? 1 : 65536 / (regs * k.threads);
+  const int64_t need = (tokens + k.rows - 1) / k.rows, wanted = 148 * resident / k.y, most = wanted > 1 ? wanted : 1;
   k.x = need < most ? need : most;
   return k;
 }
@@ -667,7 +697,8 @@ static NormCut norm_seq_cut(int64_t B, int64_t T, int G, int c, int V) {
     k.rows = 1;
     k.y = G * k.spans;
   }
-  int64_t chunks = (148 * 4 + B * k.y - 1) / (B * k.y);
+  int64_t chunks = 148 * NORM_SEQ_RESIDENT / (B * k.y);
+  if (chunks < 1) chunks = 1;
   const int64_t most = (T + 4 * k.rows - 1) / (4 * k.rows);  // (four tokens per thread at least)
   if (chunks > most) chunks = most;
   k.chunk = (T + chunks - 1) / chunks;
@@ -706,27 +737,29 @@ size_t norm_backward_floats(int64_t B, int64_t T, int C, int G, bool sequence, i
 
 template <typename T>
 static cudaError_t reduce(const NormParams& p, int64_t rows, cudaStream_t st) {
-  ttt_norm_reduce_kernel<T><<<(2 * p.C + 31) / 32, 256, 0, st>>>(p.partials, (int)rows, p.C, static_cast<T*>(p.gw), static_cast<T*>(p.gb));
+  ttt_norm_reduce_kernel<T><<<(2 * p.C + 31) / 32, ROWS_THREADS, 0, st>>>(p.partials, (int)rows, p.C, static_cast<T*>(p.gw), static_cast<T*>(p.gb));
+  return cudaGetLastError();
+}
+// (the wide vectors' kernels know a SiLU when they are built; the others, and what is rare, ask at run time)
+template <typename T, int V, bool WIDE>
+static cudaError_t token_mode(const NormParams& p, const NormCut& k, bool bwd, size_t smem, cudaStream_t st) {
+  void (*kernel)(NormParams) = bwd ? ttt_norm_token_bwd_kernel<T, V, WIDE, NORM_GENERAL> : ttt_norm_token_kernel<T, V, WIDE, NORM_GENERAL>;
+  if constexpr (V * sizeof(T) == 16 && !WIDE) {
+    if (p.act == ACT_SILU && p.gate != nullptr) kernel = bwd ? ttt_norm_token_bwd_kernel<T, V, WIDE, NORM_GATED_SILU> : ttt_norm_token_kernel<T, V, WIDE, NORM_GATED_SILU>;
+    else if (p.act == ACT_SILU) kernel = bwd ? ttt_norm_token_bwd_kernel<T, V, WIDE, NORM_SILU> : ttt_norm_token_kernel<T, V, WIDE, NORM_SILU>;
+  }
+  kernel<<<dim3((unsigned)k.x, k.y), k.threads, smem, st>>>(p);
   return cudaGetLastError();
 }
 template <typename T, int V>
 static cudaError_t launch_token(NormParams p, bool bwd, cudaStream_t st) {
   const NormCut k = norm_token_cut(p.tokens, p.G, p.c, bwd);
   p.lanes = k.lanes, p.cols = k.cols, p.rows = k.rows;
-  const dim3 grid((unsigned)k.x, k.y);
-  const bool wide = k.lanes > 32;
-  if (!bwd) {
-    if (wide) ttt_norm_token_kernel<T, V, true><<<grid, k.threads, 0, st>>>(p);
-    else ttt_norm_token_kernel<T, V, false><<<grid, k.threads, 0, st>>>(p);
-    return cudaGetLastError();
-  }
-  const size_t smem = k.rows > 1 ? sizeof(float) * 2 * k.rows * k.cols * NORM_EACH : 0;
-  if (wide) ttt_norm_token_bwd_kernel<T, V, true><<<grid, k.threads, smem, st>>>(p);
-  else ttt_norm_token_bwd_kernel<T, V, false><<<grid, k.threads, smem, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  return e != cudaSuccess || p.partials == nullptr ? e : reduce<T>(p, k.x, st);
+  const size_t smem = bwd && k.rows > 1 ? sizeof(float) * 2 * k.rows * k.cols * NORM_EACH : 0;
+  const cudaError_t e = k.lanes > 32 ? token_mode<T, V, true>(p, k, bwd, smem, st) : token_mode<T, V, false>(p, k, bwd, smem, st);
+  return e != cudaSuccess || !bwd || p.partials == nullptr ? e : reduce<T>(p, k.x, st);
 }
-template <typename T, int V>
+template <typename T, int V, int MODE>
 static cudaError_t launch_seq(NormParams p, bool bwd, cudaStream_t st) {
   const NormCut k = norm_seq_cut(p.B, p.T, p.G, p.c, V);
   p.cols = k.cols, p.rows = k.rows, p.per_block = k.per_block, p.spans = k.spans, p.chunks = k.chunks, p.chunk = k.chunk;
@@ -735,22 +768,26 @@ static cudaError_t launch_seq(NormParams p, bool bwd, cudaStream_t st) {
   if (!bwd) {
     ttt_norm_seq_stats_kernel<T, V><<<grid, NORM_THREADS, 0, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    ttt_norm_seq_apply_kernel<T, V><<<grid, NORM_THREADS, 0, st>>>(p);
+    ttt_norm_seq_apply_kernel<T, V, MODE><<<grid, NORM_THREADS, 0, st>>>(p);
     return cudaGetLastError();
   }
   p.sums = p.partials + (size_t)k.x * 2 * p.C;
-  ttt_norm_seq_bwd_kernel<T, V, false><<<grid, NORM_THREADS, sizeof(float) * 2 * k.rows * k.cols * V, st>>>(p);
+  ttt_norm_seq_bwd_kernel<T, V, false, MODE><<<grid, NORM_THREADS, sizeof(float) * 2 * k.rows * k.cols * V, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int column_blocks = (2 * p.C + 31) / 32;
-  ttt_norm_seq_sums_kernel<<<(unsigned)(p.B * column_blocks), 256, 0, st>>>(p.partials, p.sums, k.chunks, p.C, column_blocks);
+  ttt_norm_seq_sums_kernel<<<(unsigned)(p.B * column_blocks), ROWS_THREADS, 0, st>>>(p.partials, p.sums, k.chunks, p.C, column_blocks);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  ttt_norm_seq_bwd_kernel<T, V, true><<<grid, NORM_THREADS, 0, st>>>(p);
+  ttt_norm_seq_bwd_kernel<T, V, true, MODE><<<grid, NORM_THREADS, 0, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   return p.gw == nullptr && p.gb == nullptr ? cudaSuccess : reduce<T>(p, k.x, st);
 }
 template <typename T, int V>
 static cudaError_t launch_v(const NormParams& p, bool sequence, bool bwd, cudaStream_t st) {
-  return sequence ? launch_seq<T, V>(p, bwd, st) : launch_token<T, V>(p, bwd, st);
+  if (!sequence) return launch_token<T, V>(p, bwd, st);
+  if constexpr (V * sizeof(T) == 16) {
+    if (p.act == ACT_SILU) return p.gate != nullptr ? launch_seq<T, V, NORM_GATED_SILU>(p, bwd, st) : launch_seq<T, V, NORM_SILU>(p, bwd, st);
+  }
+  return launch_seq<T, V, NORM_GENERAL>(p, bwd, st);
 }
 // V: the widest vector that the group's channels and all addresses allow (16 bytes, 2 channels or 1)
 cudaError_t launch_norm(int dtype, const NormParams& p, int V, bool sequence, bool bwd, cudaStream_t st) {

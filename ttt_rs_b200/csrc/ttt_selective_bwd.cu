@@ -456,19 +456,11 @@ __global__ void __launch_bounds__(256) ttt_selective_bc_kernel(const SelParams p
   st_from_float<T>(which ? p.gc : p.gb, ((b * p.T + t) * p.G + g) * p.N + s, v);
 }
 // rows of partial sums [rows][pitch] (row r at r row_pitch) -> out: [n / NP][N] of [n / NP][NP]
-__global__ void __launch_bounds__(256) ttt_selective_rows_kernel(const float* partials, int64_t rows, int64_t row_pitch, int64_t n, int NP, int N,
-                                                                 float* out) {
-  __shared__ float part[8][33];
-  const int64_t col = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-  const int share = threadIdx.x >> 5;
-  float v = 0.f;
-  if (col < n)
-    for (int64_t r = share; r < rows; r += 8) v += partials[r * row_pitch + col];
-  part[share][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (share != 0 || col >= n) return;
-#pragma unroll
-  for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x & 31];
+__global__ void __launch_bounds__(ROWS_THREADS) ttt_selective_rows_kernel(const float* partials, int64_t rows, int64_t row_pitch, int64_t n, int NP, int N,
+                                                                          float* out) {
+  int64_t col;
+  float v;
+  if (!sum_of_rows(partials, rows, row_pitch, n, blockIdx.x, &col, &v)) return;
   const int64_t c = col / NP;
   const int s = (int)(col - c * NP);
   if (s < N) out[c * N + s] = v;
@@ -499,12 +491,12 @@ static cudaError_t run_all(const SelParams& p, cudaStream_t st) {
   ttt_selective_bc_kernel<T><<<(unsigned)((p.B * p.G * p.T * 2 * NP + 255) / 256), 256, 0, st>>>(p, NP, channel_blocks);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   const int64_t n = (int64_t)p.C * NP;
-  ttt_selective_rows_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(p.part_a, rows, n, n, NP, p.N, p.ga);
+  ttt_selective_rows_kernel<<<(unsigned)((n + 31) / 32), ROWS_THREADS, 0, st>>>(p.part_a, rows, n, n, NP, p.N, p.ga);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   for (int m = 0; m < 2; ++m) {
     float* out = m ? p.gbias : p.gd;
     if (out == nullptr) continue;
-    ttt_selective_rows_kernel<<<(p.C + 31) / 32, 256, 0, st>>>(p.part_d + m * p.C, rows, 2 * (int64_t)p.C, p.C, 1, 1, out);
+    ttt_selective_rows_kernel<<<(p.C + 31) / 32, ROWS_THREADS, 0, st>>>(p.part_d + m * p.C, rows, 2 * (int64_t)p.C, p.C, 1, 1, out);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   return cudaSuccess;

@@ -104,4 +104,27 @@ __device__ __forceinline__ float act_and_slope(float v, int act, float& slope) {
   return v;
 }
 
+
+// Sums over rows [rows][pitch] of blocks' shares, in a fixed order: a block of ROWS_THREADS per 32 columns, a warp per 32nd row.  True in
+// the thread that has column *col's sum.
+constexpr int ROWS_THREADS = 1024;
+__device__ __forceinline__ bool sum_of_rows(const float* partials, int64_t rows, int64_t pitch, int64_t columns, int64_t block, int64_t* col, float* sum) {
+  __shared__ float part[ROWS_THREADS / 32][33];
+  const int lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+  *col = block * 32 + lane;
+  float v = 0.f;
+  if (*col < columns) {
+    const float* at = partials + *col;
+#pragma unroll 4
+    for (int64_t r = share; r < rows; r += ROWS_THREADS / 32) v += at[r * pitch];
+  }
+  part[share][lane] = v;
+  __syncthreads();
+  if (share != 0 || *col >= columns) return false;
+#pragma unroll
+  for (int k = 1; k < ROWS_THREADS / 32; ++k) v += part[k][lane];
+  *sum = v;
+  return true;
+}
+
 }  // namespace ttt

@@ -7,7 +7,7 @@
 //
 // Memory-bound.  A thread holds four neighbouring channels (one, where rows are off a vector's address; eight of bf16 took so many
 // registers that a quarter of the threads fitted: 208 us against 131 us forward for 65536 tokens of 1536) and walks a strip of tokens with the last
-// K - 1 inputs in registers, CONV_AHEAD tokens on their way at a time; the tokens before a strip (and behind it, for dx) are read
+// K - 1 inputs in registers, a few tokens on their way at a time; the tokens before a strip (and behind it, for dx) are read
 // again, from L2.  A start empties the registers of the inputs, and the sums of dx know the
 // last start's place.
 #include <type_traits>
@@ -18,8 +18,11 @@
 namespace ttt {
 
 constexpr int CONV_THREADS = 256;
-constexpr int CONV_FWD_RESIDENT = 4, CONV_BWD_RESIDENT = 2;  // blocks per SM that registers are bounded for
-constexpr int CONV_AHEAD = 8, CONV_BWD_AHEAD = 4;            // tokens on their way at a time
+constexpr int CONV_FWD_RESIDENT = 2, CONV_BWD_RESIDENT = 2;  // blocks per SM that registers are bounded for
+template <typename T>
+__host__ __device__ constexpr int conv_ahead(bool bwd) {  // tokens on their way at a time
+  return (sizeof(T) == 2 ? 8 : 4) / (bwd ? 2 : 1);
+}
 
 // V channels of row t of a sequence; rows before the first are the state's, rows from T on zeros
 template <typename T, int V, int K>
@@ -90,7 +93,7 @@ __device__ __forceinline__ void conv_before(F2 (&h)[K - 1][Chan<T, V>::P], int& 
 template <typename T, int V, int K, bool ACT, bool MARKS>
 __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kernel(const ConvParams p) {
   using Ch = Chan<T, V>;
-  constexpr int P = Ch::P;
+  constexpr int P = Ch::P, AHEAD = conv_ahead<T>(false);
   const int lane = threadIdx.x & ((1 << p.lanes_log) - 1), rows = CONV_THREADS >> p.lanes_log;
   const int c = ((int)blockIdx.y * (1 << p.lanes_log) + lane) * V;
   if (c >= p.C) return;
@@ -107,17 +110,17 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
     conv_before<T, V, K, MARKS>(h, last, p, x, state, starts, t0);
     const T* in_at = x + t0 * p.xs[1];
     T* y = static_cast<T*>(p.y) + (b * p.T + t0) * p.C + c;
-    auto some = [&](int at, auto all) {  // CONV_AHEAD tokens, or as many as are left
-      Ch in[CONV_AHEAD];
-      [[maybe_unused]] uint8_t first[CONV_AHEAD];
+    auto some = [&](int at, auto all) {  // AHEAD tokens, or as many as are left
+      Ch in[AHEAD];
+      [[maybe_unused]] uint8_t first[AHEAD];
 #pragma unroll
-      for (int u = 0; u < CONV_AHEAD; ++u)
+      for (int u = 0; u < AHEAD; ++u)
         if (decltype(all)::value || at + u < n) {
           in[u].load(in_at + u * p.xs[1]);
           if constexpr (MARKS) first[u] = starts[t0 + at + u];
         }
 #pragma unroll
-      for (int u = 0; u < CONV_AHEAD; ++u) {
+      for (int u = 0; u < AHEAD; ++u) {
         if (!decltype(all)::value && at + u >= n) break;
         if (MARKS && first[u]) {
 #pragma unroll
@@ -141,11 +144,11 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
         out.pack(v);
         out.store(y + (int64_t)u * p.C);
       }
-      in_at += CONV_AHEAD * p.xs[1];
-      y += (int64_t)CONV_AHEAD * p.C;
+      in_at += AHEAD * p.xs[1];
+      y += (int64_t)AHEAD * p.C;
     };
     int at = 0;
-    for (; at + CONV_AHEAD <= n; at += CONV_AHEAD) some(at, std::true_type{});
+    for (; at + AHEAD <= n; at += AHEAD) some(at, std::true_type{});
     if (at < n) some(at, std::false_type{});
     // The thread of the first tokens, the only one that has read the given state, writes the new one: they may be the same tensor.
     // (Behind a short row a part of the given state is still visible: read it all before writing.)
@@ -174,7 +177,7 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
 template <typename T, int V, int K, bool ACT, bool MARKS>
 __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_kernel(const ConvParams p) {
   using Ch = Chan<T, V>;
-  constexpr int P = Ch::P;
+  constexpr int P = Ch::P, AHEAD = conv_ahead<T>(true);
   const int lanes = 1 << p.lanes_log, rows = CONV_THREADS >> p.lanes_log;
   const int lane = threadIdx.x & (lanes - 1), row = threadIdx.x >> p.lanes_log;
   const int c = ((int)blockIdx.y * lanes + lane) * V;
@@ -207,11 +210,11 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
       const T* in_at = x + t0 * p.xs[1];
       const T* g_at = static_cast<const T*>(p.gy) + b * p.gs[0] + t0 * p.gs[1] + c;
       T* gx = static_cast<T*>(p.gx) + (b * p.T + t0 - (K - 1)) * p.C + c;  // token t completes the gradient of token t - (K - 1)
-      auto some = [&](int at, auto all) {  // CONV_BWD_AHEAD tokens; all: of the strip, each
-        Ch in[CONV_BWD_AHEAD], grad[CONV_BWD_AHEAD];
-        [[maybe_unused]] uint8_t first[CONV_BWD_AHEAD];
+      auto some = [&](int at, auto all) {  // AHEAD tokens; all: of the strip, each
+        Ch in[AHEAD], grad[AHEAD];
+        [[maybe_unused]] uint8_t first[AHEAD];
 #pragma unroll
-        for (int u = 0; u < CONV_BWD_AHEAD; ++u) {
+        for (int u = 0; u < AHEAD; ++u) {
           if (MARKS) first[u] = 0;
           if (decltype(all)::value || at + u < n_read) {
             in[u].load(in_at + u * p.xs[1]);
@@ -223,7 +226,7 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
           }
         }
 #pragma unroll
-        for (int u = 0; u < CONV_BWD_AHEAD; ++u) {
+        for (int u = 0; u < AHEAD; ++u) {
           const int t = at + u;
           if (!decltype(all)::value && t >= n + K - 1) break;
           if (MARKS && first[u]) {
@@ -277,13 +280,13 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
             else if (p.gstate != nullptr) out.store(static_cast<T*>(p.gstate) + (b * (K - 1) + s + K - 1) * p.C + c);
           }
         }
-        in_at += CONV_BWD_AHEAD * p.xs[1];
-        g_at += CONV_BWD_AHEAD * p.gs[1];
-        gx += (int64_t)CONV_BWD_AHEAD * p.C;
+        in_at += AHEAD * p.xs[1];
+        g_at += AHEAD * p.gs[1];
+        gx += (int64_t)AHEAD * p.C;
       };
       int at = 0;
-      for (; at + CONV_BWD_AHEAD <= n; at += CONV_BWD_AHEAD) some(at, std::true_type{});
-      for (; at < n + K - 1; at += CONV_BWD_AHEAD) some(at, std::false_type{});
+      for (; at + AHEAD <= n; at += AHEAD) some(at, std::true_type{});
+      for (; at < n + K - 1; at += AHEAD) some(at, std::false_type{});
     }
   }
   if (p.partials == nullptr) return;

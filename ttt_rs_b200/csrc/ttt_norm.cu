@@ -19,8 +19,7 @@
 namespace ttt {
 
 constexpr int NORM_THREADS = 256;
-constexpr int NORM_FWD_RESIDENT = 4, NORM_BWD_RESIDENT = 2, NORM_SEQ_RESIDENT = 3;  // blocks of 256 threads per SM that registers are bounded for
-constexpr int NORM_BWD_AHEAD = 2;  // tokens on their way at a time
+constexpr int NORM_FWD_RESIDENT = 4, NORM_BWD_RESIDENT = 3, NORM_SEQ_RESIDENT = 3;  // blocks of 256 threads per SM that registers are bounded for
 constexpr int NORM_EACH = 8;  // channels per thread, a token's groups
 constexpr int NORM_WIDE = NORM_TOKEN_CHANNELS / NORM_EACH;  // threads at most, of groups that several warps share
 
@@ -189,7 +188,7 @@ template <typename T, int V, bool WIDE, int MODE>
 __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NORM_BWD_RESIDENT) ttt_norm_token_bwd_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   using L = NormLane<T, V>;
-  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE || V == 1 || sizeof(T) == 4 ? 1 : NORM_BWD_AHEAD;
+  constexpr int NV = L::NV, P = L::P, AHEAD = 1;
   __shared__ float red[32];
   const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
   const int g = gcol / p.lanes, l = gcol & (p.lanes - 1), act = norm_act<MODE>(p);

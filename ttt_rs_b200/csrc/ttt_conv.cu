@@ -7,7 +7,7 @@
 //
 // Memory-bound.  A thread holds four neighbouring channels (one, where rows are off a vector's address; eight of bf16 took so many
 // registers that a quarter of the threads fitted: 208 us against 131 us forward for 65536 tokens of 1536) and walks a strip of tokens with the last
-// K - 1 inputs in registers, a few tokens on their way at a time; the tokens before a strip (and behind it, for dx) are read
+// K - 1 inputs in registers, the next few tokens on their way; the tokens before a strip (and behind it, for dx) are read
 // again, from L2.  A start empties the registers of the inputs, and the sums of dx know the
 // last start's place.
 #include <type_traits>
@@ -21,7 +21,7 @@ constexpr int CONV_THREADS = 256;
 constexpr int CONV_FWD_RESIDENT = 2, CONV_BWD_RESIDENT = 2;  // blocks per SM that registers are bounded for
 template <typename T>
 __host__ __device__ constexpr int conv_ahead(bool bwd) {  // tokens on their way at a time
-  return (sizeof(T) == 2 ? 8 : 4) / (bwd ? 2 : 1);
+  return bwd && sizeof(T) == 4 ? 2 : 4;
 }
 
 // V channels of row t of a sequence; rows before the first are the state's, rows from T on zeros
@@ -110,15 +110,26 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
     conv_before<T, V, K, MARKS>(h, last, p, x, state, starts, t0);
     const T* in_at = x + t0 * p.xs[1];
     T* y = static_cast<T*>(p.y) + (b * p.T + t0) * p.C + c;
+    Ch next[AHEAD];  // the tokens behind those that are worked on: on their way meanwhile
+    [[maybe_unused]] uint8_t next_first[AHEAD];
+    auto fetch = [&](int at) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (at + u < n) {
+          next[u].load(in_at + u * p.xs[1]);
+          if constexpr (MARKS) next_first[u] = starts[t0 + at + u];
+        }
+      in_at += AHEAD * p.xs[1];
+    };
     auto some = [&](int at, auto all) {  // AHEAD tokens, or as many as are left
       Ch in[AHEAD];
       [[maybe_unused]] uint8_t first[AHEAD];
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (decltype(all)::value || at + u < n) {
-          in[u].load(in_at + u * p.xs[1]);
-          if constexpr (MARKS) first[u] = starts[t0 + at + u];
-        }
+      for (int u = 0; u < AHEAD; ++u) {
+        in[u] = next[u];
+        if constexpr (MARKS) first[u] = next_first[u];
+      }
+      fetch(at + AHEAD);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         if (!decltype(all)::value && at + u >= n) break;
@@ -144,9 +155,9 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
         out.pack(v);
         out.store(y + (int64_t)u * p.C);
       }
-      in_at += AHEAD * p.xs[1];
       y += (int64_t)AHEAD * p.C;
     };
+    fetch(0);
     int at = 0;
     for (; at + AHEAD <= n; at += AHEAD) some(at, std::true_type{});
     if (at < n) some(at, std::false_type{});
@@ -210,21 +221,32 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
       const T* in_at = x + t0 * p.xs[1];
       const T* g_at = static_cast<const T*>(p.gy) + b * p.gs[0] + t0 * p.gs[1] + c;
       T* gx = static_cast<T*>(p.gx) + (b * p.T + t0 - (K - 1)) * p.C + c;  // token t completes the gradient of token t - (K - 1)
+      Ch next[AHEAD], next_grad[AHEAD];  // the tokens behind those that are worked on: on their way meanwhile
+      [[maybe_unused]] uint8_t next_first[AHEAD];
+      auto fetch = [&](int at) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          next[u].zero();  // (no gradient: nothing is added)
+          next_grad[u].zero();
+          if constexpr (MARKS) next_first[u] = 0;
+          if (at + u < n_read) {
+            next[u].load(in_at + u * p.xs[1]);
+            next_grad[u].load(g_at + u * p.gs[1]);
+            if constexpr (MARKS) next_first[u] = starts[t0 + at + u];
+          }
+        }
+        in_at += AHEAD * p.xs[1];
+        g_at += AHEAD * p.gs[1];
+      };
       auto some = [&](int at, auto all) {  // AHEAD tokens; all: of the strip, each
         Ch in[AHEAD], grad[AHEAD];
         [[maybe_unused]] uint8_t first[AHEAD];
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-          if (MARKS) first[u] = 0;
-          if (decltype(all)::value || at + u < n_read) {
-            in[u].load(in_at + u * p.xs[1]);
-            grad[u].load(g_at + u * p.gs[1]);
-            if constexpr (MARKS) first[u] = starts[t0 + at + u];
-          } else {  // (no gradient: nothing is added)
-            in[u].zero();
-            grad[u].zero();
-          }
+          in[u] = next[u], grad[u] = next_grad[u];
+          if constexpr (MARKS) first[u] = next_first[u];
         }
+        fetch(at + AHEAD);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           const int t = at + u;
@@ -280,10 +302,9 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
             else if (p.gstate != nullptr) out.store(static_cast<T*>(p.gstate) + (b * (K - 1) + s + K - 1) * p.C + c);
           }
         }
-        in_at += AHEAD * p.xs[1];
-        g_at += AHEAD * p.gs[1];
         gx += (int64_t)AHEAD * p.C;
       };
+      fetch(0);
       int at = 0;
       for (; at + AHEAD <= n; at += AHEAD) some(at, std::true_type{});
       for (; at < n + K - 1; at += AHEAD) some(at, std::false_type{});

@@ -113,13 +113,20 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
     Ch next[AHEAD];  // the tokens behind those that are worked on: on their way meanwhile
     [[maybe_unused]] uint8_t next_first[AHEAD];
     auto fetch = [&](int at) {
+      if (at + AHEAD <= n) {
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (at + u < n) {
-          next[u].load(in_at + u * p.xs[1]);
+        for (int u = 0; u < AHEAD; ++u, in_at += p.xs[1]) {
+          next[u].load(in_at);
           if constexpr (MARKS) next_first[u] = starts[t0 + at + u];
         }
-      in_at += AHEAD * p.xs[1];
+      } else {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u, in_at += p.xs[1])
+          if (at + u < n) {
+            next[u].load(in_at);
+            if constexpr (MARKS) next_first[u] = starts[t0 + at + u];
+          }
+      }
     };
     auto some = [&](int at, auto all) {  // AHEAD tokens, or as many as are left
       Ch in[AHEAD];
@@ -153,9 +160,9 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_FWD_RESIDENT) ttt_conv_kern
         }
         Ch out;
         out.pack(v);
-        out.store(y + (int64_t)u * p.C);
+        out.store(y);
+        y += p.C;
       }
-      y += (int64_t)AHEAD * p.C;
     };
     fetch(0);
     int at = 0;
@@ -224,21 +231,28 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
       Ch next[AHEAD], next_grad[AHEAD];  // the tokens behind those that are worked on: on their way meanwhile
       [[maybe_unused]] uint8_t next_first[AHEAD];
       auto fetch = [&](int at) {
+        if (at + AHEAD <= n_read) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-          next[u].zero();  // (no gradient: nothing is added)
-          next_grad[u].zero();
-          if constexpr (MARKS) next_first[u] = 0;
-          if (at + u < n_read) {
-            next[u].load(in_at + u * p.xs[1]);
-            next_grad[u].load(g_at + u * p.gs[1]);
+          for (int u = 0; u < AHEAD; ++u, in_at += p.xs[1], g_at += p.gs[1]) {
+            next[u].load(in_at);
+            next_grad[u].load(g_at);
             if constexpr (MARKS) next_first[u] = starts[t0 + at + u];
           }
+        } else {
+#pragma unroll
+          for (int u = 0; u < AHEAD; ++u, in_at += p.xs[1], g_at += p.gs[1]) {
+            next[u].zero();  // (no gradient: nothing is added)
+            next_grad[u].zero();
+            if constexpr (MARKS) next_first[u] = 0;
+            if (at + u < n_read) {
+              next[u].load(in_at);
+              next_grad[u].load(g_at);
+              if constexpr (MARKS) next_first[u] = starts[t0 + at + u];
+            }
+          }
         }
-        in_at += AHEAD * p.xs[1];
-        g_at += AHEAD * p.gs[1];
       };
-      auto some = [&](int at, auto all) {  // AHEAD tokens; all: of the strip, each
+      auto some = [&](int at, auto all) {  // AHEAD tokens; all: of the strip, each, and at least K - 1 of it before them
         Ch in[AHEAD], grad[AHEAD];
         [[maybe_unused]] uint8_t first[AHEAD];
 #pragma unroll
@@ -287,8 +301,8 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
             h[K - 2][k] = now[k];
           }
           const int s = t - (K - 1);
-          if (s >= s_lo) {
-            if (gstate_out != nullptr && s >= s_tail && (!MARKS || s >= last)) {
+          if (decltype(all)::value || s >= s_lo) {
+            if (!decltype(all)::value && gstate_out != nullptr && s >= s_tail && (!MARKS || s >= last)) {
               Ch r;
               F2 e[P];
               r.load(gstate_out + (int64_t)(s - s_tail) * p.C);
@@ -298,14 +312,15 @@ __global__ void __launch_bounds__(CONV_THREADS, CONV_BWD_RESIDENT) ttt_conv_bwd_
             }
             Ch out;
             out.pack(whole);
-            if (t0 + s >= 0) out.store(gx + (int64_t)u * p.C);
+            if (decltype(all)::value || t0 + s >= 0) out.store(gx);
             else if (p.gstate != nullptr) out.store(static_cast<T*>(p.gstate) + (b * (K - 1) + s + K - 1) * p.C + c);
           }
+          gx += p.C;
         }
-        gx += (int64_t)AHEAD * p.C;
       };
       fetch(0);
       int at = 0;
+      for (; at < K - 1; at += AHEAD) some(at, std::false_type{});
       for (; at + AHEAD <= n; at += AHEAD) some(at, std::true_type{});
       for (; at < n + K - 1; at += AHEAD) some(at, std::false_type{});
     }

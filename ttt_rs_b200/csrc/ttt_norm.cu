@@ -320,9 +320,9 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NO
         }
 }
 
-// rows of partial sums [rows][2][C] -> weight's and bias's gradients, in a fixed order
+// rows of partial sums [rows][2][C] (of du n and du) -> weight's and bias's gradients, in a fixed order
 template <typename T>
-__global__ void __launch_bounds__(ROWS_THREADS) ttt_norm_reduce_kernel(const float* partials, int rows, int C, T* gw, T* gb) {
+__global__ void __launch_bounds__(ROWS_THREADS) ttt_norm_reduce_kernel(const float* partials, int64_t rows, int C, T* gw, T* gb) {
   int64_t col;
   float v;
   if (!sum_of_rows(partials, rows, 2 * C, 2 * C, blockIdx.x, &col, &v)) return;
@@ -339,25 +339,28 @@ __global__ void __launch_bounds__(ROWS_THREADS) ttt_norm_reduce_kernel(const flo
 struct Moments {
   float n, mean, m2;
   __device__ __forceinline__ void join(float bn, float bmean, float bm2) {
-    const float all = n + bn;
-    if (!(bn > 0.f)) return;
-    const float d = bmean - mean, f = bn / all;
+    const float all = n + bn, d = bmean - mean, f = all > 0.f ? __fdividef(bn, all) : 0.f;
     mean = fmaf(d, f, mean);
     m2 += bm2 + d * d * n * f;
     n = all;
   }
-  __device__ __forceinline__ void join_warp() {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+  __device__ __forceinline__ void join_lanes(int lanes) {  // over a power of two of neighbouring lanes
+    for (int o = 1; o < lanes; o <<= 1) {
       const float bn = __shfl_xor_sync(0xffffffffu, n, o), bm = __shfl_xor_sync(0xffffffffu, mean, o), b2 = __shfl_xor_sync(0xffffffffu, m2, o);
       // (both lanes join in the same order, so that both have the same)
-      Moments lo = (threadIdx.x & o) ? Moments{bn, bm, b2} : *this, hi = (threadIdx.x & o) ? *this : Moments{bn, bm, b2};
-      if (lo.n > 0.f) lo.join(hi.n, hi.mean, hi.m2);
-      else lo = hi;
+      const bool second = (threadIdx.x & o) != 0;
+      Moments lo = second ? Moments{bn, bm, b2} : *this;
+      lo.join(second ? n : bn, second ? mean : bm, second ? m2 : b2);
       *this = lo;
     }
   }
 };
+// threads for each of a block's groups: a power of two, all groups at once
+__device__ __forceinline__ int threads_per_group(int groups) {
+  int w = 32;
+  while (w > 1 && w * groups > NORM_THREADS) w >>= 1;
+  return w;
+}
 
 // Where a block of the sequence kernels stands.  blockIdx.x: row of the batch and chunk of tokens; blockIdx.y: groups, or a part of
 // a group's channels.
@@ -420,26 +423,23 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_
             const F2 d = f2(v[u][k].x - mean, V > 1 ? v[u][k].y - mean : 0.f);
             q = f2fma(d, d, q);
           }
-      if (me.n > 0.f) me.join(n, mean, f2hsum(q));
-      else me = Moments{n, mean, f2hsum(q)};
+      me.join(n, mean, f2hsum(q));
     }
   }
   sm[0][threadIdx.x] = me.n, sm[1][threadIdx.x] = me.mean, sm[2][threadIdx.x] = me.m2;
   __syncthreads();
-  // a warp per group, lanes over its columns and rows
-  const int lane = threadIdx.x & 31, per_group = p.spans == 1 ? p.c / V : p.cols, entries = per_group * p.rows;
-  for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
-    Moments m{0.f, 0.f, 0.f};
-    for (int e = lane; e < entries; e += 32) {
+  const int per_group = p.spans == 1 ? p.c / V : p.cols, entries = per_group * p.rows;
+  const int w = threads_per_group(at.groups), k = threadIdx.x / w, lane = threadIdx.x & (w - 1);
+  Moments m{0.f, 0.f, 0.f};
+  if (k < at.groups)
+    for (int e = lane; e < entries; e += w) {
       const int r = e / per_group, i = r * p.cols + k * per_group + (e - r * per_group);
-      if (m.n > 0.f) m.join(sm[0][i], sm[1][i], sm[2][i]);
-      else m = Moments{sm[0][i], sm[1][i], sm[2][i]};
+      m.join(sm[0][i], sm[1][i], sm[2][i]);
     }
-    m.join_warp();
-    if (lane == 0) {
-      float* out = p.moments + (((at.b * p.G + at.g0 + k) * p.chunks + at.chunk) * p.spans + at.span) * 3;
-      out[0] = m.n, out[1] = m.mean, out[2] = m.m2;
-    }
+  m.join_lanes(w);
+  if (k < at.groups && lane == 0) {
+    float* out = p.moments + (((at.b * p.G + at.g0 + k) * p.chunks + at.chunk) * p.spans + at.span) * 3;
+    out[0] = m.n, out[1] = m.mean, out[2] = m.m2;
   }
 }
 
@@ -451,16 +451,16 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_
   const SeqPlace at(p, V);
   const bool gated = norm_gated<MODE>(p);
   const int act = norm_act<MODE>(p);
-  const int lane = threadIdx.x & 31;
-  for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
-    const float* m = p.moments + (at.b * p.G + at.g0 + k) * p.chunks * p.spans * 3;
+  {
+    const int w = threads_per_group(at.groups), k = threadIdx.x / w, lane = threadIdx.x & (w - 1);
     Moments all{0.f, 0.f, 0.f};
-    for (int e = lane; e < p.chunks * p.spans; e += 32) {
-      if (all.n > 0.f) all.join(m[3 * e], m[3 * e + 1], m[3 * e + 2]);
-      else all = Moments{m[3 * e], m[3 * e + 1], m[3 * e + 2]};
+    if (k < at.groups) {
+      const float* m = p.moments + (at.b * p.G + at.g0 + k) * p.chunks * p.spans * 3;
+#pragma unroll 4
+      for (int e = lane; e < p.chunks * p.spans; e += w) all.join(m[3 * e], m[3 * e + 1], m[3 * e + 2]);
     }
-    all.join_warp();
-    if (lane == 0) {
+    all.join_lanes(w);
+    if (k < at.groups && lane == 0) {
       stat[k][0] = all.mean;
       stat[k][1] = rsqrtf(all.m2 / all.n + p.eps);
       if (p.stats != nullptr && at.chunk == 0 && at.span == 0) {
@@ -544,24 +544,24 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_
   const bool gated = norm_gated<MODE>(p);
   const int act = norm_act<MODE>(p);
   if constexpr (APPLY) {  // the groups' means of p and p n, from the channels' sums
-    const int lane = threadIdx.x & 31;
     const float inv = 1.f / ((float)p.c * (float)p.T);
-    for (int k = threadIdx.x >> 5; k < at.groups; k += NORM_THREADS / 32) {
+    const int w = threads_per_group(at.groups), k = threadIdx.x / w, lane = threadIdx.x & (w - 1);
+    float m1 = 0.f, m2 = 0.f;
+    if (k < at.groups) {
       const int c0 = (at.g0 + k) * p.c;
       const float* s = p.sums + at.b * 2 * p.C + c0;
-      float m1 = 0.f, m2 = 0.f;
-      for (int c = lane; c < p.c; c += 32) {
-        const float w = p.w != nullptr ? ld_as_float<T>(p.w, c0 + c) : 1.f;
-        m1 = fmaf(w, s[c], m1);
-        m2 = fmaf(w, s[p.C + c], m2);
+#pragma unroll 4
+      for (int c = lane; c < p.c; c += w) {
+        const float wt = p.w != nullptr ? ld_as_float<T>(p.w, c0 + c) : 1.f;
+        m2 = fmaf(wt, s[c], m2);
+        m1 = fmaf(wt, s[p.C + c], m1);
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        m1 += __shfl_xor_sync(0xffffffffu, m1, o);
-        m2 += __shfl_xor_sync(0xffffffffu, m2, o);
-      }
-      if (lane == 0) mean_of[k][0] = m1 * inv, mean_of[k][1] = m2 * inv;
     }
+    for (int o = 1; o < w; o <<= 1) {
+      m1 += __shfl_xor_sync(0xffffffffu, m1, o);
+      m2 += __shfl_xor_sync(0xffffffffu, m2, o);
+    }
+    if (k < at.groups && lane == 0) mean_of[k][0] = m1 * inv, mean_of[k][1] = m2 * inv;
     __syncthreads();
   }
   F2 s1[P], s2[P];
@@ -647,13 +647,13 @@ __global__ void __launch_bounds__(NORM_THREADS, NORM_SEQ_RESIDENT) ttt_norm_seq_
   }
 }
 
-// the chunks' sums [B][chunks][2][C] (du n, du) -> [B][2][C] (du, du n)
+// the chunks' sums [B][chunks][2][C] -> [B][2][C]
 __global__ void __launch_bounds__(ROWS_THREADS) ttt_norm_seq_sums_kernel(const float* partials, float* sums, int chunks, int C, int column_blocks) {
   const int64_t b = blockIdx.x / column_blocks;
   int64_t col;
   float v;
   if (!sum_of_rows(partials + b * chunks * 2 * C, chunks, 2 * C, 2 * C, blockIdx.x - b * column_blocks, &col, &v)) return;
-  sums[b * 2 * C + (col < C ? C + col : col - C)] = v;
+  sums[b * 2 * C + col] = v;
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------
@@ -735,8 +735,8 @@ size_t norm_backward_floats(int64_t B, int64_t T, int C, int G, bool sequence, i
 }
 
 template <typename T>
-static cudaError_t reduce(const NormParams& p, int64_t rows, cudaStream_t st) {
-  ttt_norm_reduce_kernel<T><<<(2 * p.C + 31) / 32, ROWS_THREADS, 0, st>>>(p.partials, (int)rows, p.C, static_cast<T*>(p.gw), static_cast<T*>(p.gb));
+static cudaError_t reduce(const NormParams& p, const float* partials, int64_t rows, cudaStream_t st) {
+  ttt_norm_reduce_kernel<T><<<(2 * p.C + 31) / 32, ROWS_THREADS, 0, st>>>(partials, rows, p.C, static_cast<T*>(p.gw), static_cast<T*>(p.gb));
   return cudaGetLastError();
 }
 // (the wide vectors' kernels know a SiLU when they are built; the others, and what is rare, ask at run time)
@@ -756,7 +756,7 @@ static cudaError_t launch_token(NormParams p, bool bwd, cudaStream_t st) {
   p.lanes = k.lanes, p.cols = k.cols, p.rows = k.rows;
   const size_t smem = bwd && k.rows > 1 ? sizeof(float) * 2 * k.rows * k.cols * NORM_EACH : 0;
   const cudaError_t e = k.lanes > 32 ? token_mode<T, V, true>(p, k, bwd, smem, st) : token_mode<T, V, false>(p, k, bwd, smem, st);
-  return e != cudaSuccess || !bwd || p.partials == nullptr ? e : reduce<T>(p, k.x, st);
+  return e != cudaSuccess || !bwd || p.partials == nullptr ? e : reduce<T>(p, p.partials, k.x, st);
 }
 template <typename T, int V, int MODE>
 static cudaError_t launch_seq(NormParams p, bool bwd, cudaStream_t st) {
@@ -778,7 +778,7 @@ static cudaError_t launch_seq(NormParams p, bool bwd, cudaStream_t st) {
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   ttt_norm_seq_bwd_kernel<T, V, true, MODE><<<grid, NORM_THREADS, 0, st>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  return p.gw == nullptr && p.gb == nullptr ? cudaSuccess : reduce<T>(p, k.x, st);
+  return p.gw == nullptr && p.gb == nullptr ? cudaSuccess : reduce<T>(p, p.sums, p.B, st);
 }
 template <typename T, int V>
 static cudaError_t launch_v(const NormParams& p, bool sequence, bool bwd, cudaStream_t st) {

@@ -42,7 +42,7 @@ __device__ __forceinline__ void gradient_behind(F2 (&dh)[SelShape<NP>::CC][2], c
       const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
       const bool cut = sum == INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) dh[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), dh[k][i], own[k][i]);
+      for (int i = 0; i < 2; ++i) dh[k][i] = cut ? own[k][i] : f2fma(decay_of(A[k][i], sum), dh[k][i], own[k][i]);
     }
   }
 }
@@ -86,7 +86,9 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
       for (int half = 1; half >= 0; --half) {
         const int k2 = half ^ 1;  // results alternate
         F2 h[S::CC][2], before[SEL_HALF / 2][S::CC][2];  // the states that the half's tokens 0, 2, 4, 6 find
-        F2 decay[SEL_HALF][S::CC][2];
+        F2 decay[SEL_HALF][S::CC][2], dA_half[S::CC][2];  // (sums of sums: thousands of tokens one by one would lose ten times as much)
+#pragma unroll
+        for (int k = 0; k < S::CC; ++k) dA_half[k][0] = dA_half[k][1] = f2(0.f);
 #pragma unroll
         for (int k = 0; k < S::CC; ++k) h[k][0] = h0[k][0], h[k][1] = h0[k][1];
         const float2* du = &sm.du[i & 1][0][me.ch];
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
             if (MARKS && mark >> r & 1) h[k][0] = h[k][1] = f2(0.f);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              a[k][n] = ex2(f2mul(A[k][n], f2(q[k].x)));
+              a[k][n] = decay_of(A[k][n], q[k].x);
               h[k][n] = f2fma(a[k][n], h[k][n], f2mul(f2(q[k].y), n ? f2(b.z, b.w) : f2(b.x, b.y)));
             }
           }
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
                 F2 way = f2mul(dh[k][n], h[k][n]);
                 if (MARKS && mark >> r & 1) dh[k][n] = way = f2(0.f);
                 ra = n ? f2fma(way, A[k][n], ra) : f2mul(way, A[k][n]);
-                dA[k][n] = f2fma(way, d, dA[k][n]);
+                dA_half[k][n] = f2fma(way, d, dA_half[k][n]);
               }
               share[0][k] = f2hsum(in);
               share[1][k] = f2hsum(ra);
@@ -205,6 +207,8 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
             }
           }
         }
+#pragma unroll
+        for (int k = 0; k < S::CC; ++k) dA[k][0] = f2add(dA[k][0], dA_half[k][0]), dA[k][1] = f2add(dA[k][1], dA_half[k][1]);
         __syncthreads();
       }
     }
@@ -419,8 +423,8 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_rev_kernel(const Se
 #pragma unroll
       for (int k = 0; k < S::CC; ++k) {
         const F2 dk = f2(dp[k]), gk = f2(gp[k]);
-        dh[k][0] = f2mul(f2fma(gk, f2(c.x, c.y), dh[k][0]), ex2(f2mul(A[k][0], dk)));
-        dh[k][1] = f2mul(f2fma(gk, f2(c.z, c.w), dh[k][1]), ex2(f2mul(A[k][1], dk)));
+        dh[k][0] = f2mul(f2fma(gk, f2(c.x, c.y), dh[k][0]), decay_of(A[k][0], dk));
+        dh[k][1] = f2mul(f2fma(gk, f2(c.z, c.w), dh[k][1]), decay_of(A[k][1], dk));
         if (MARKS && mark >> r & 1) dh[k][0] = dh[k][1] = f2(0.f);
       }
     }

@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
           const float sum = me.ch + k < at.have ? p.seg_sum[row + me.ch + k] : 0.f;
           const bool cut = sum == INFINITY;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) h[k][i] = cut ? own[k][i] : f2fma(ex2(f2mul(A[k][i], f2(sum))), h[k][i], own[k][i]);
+          for (int i = 0; i < 2; ++i) h[k][i] = cut ? own[k][i] : f2fma(decay_of(A[k][i], f2(sum)), h[k][i], own[k][i]);
         }
       }
     } else {
@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
 #pragma unroll
         for (int k = 0; k < S::CC; ++k) {
           const F2 d = f2(k ? q.z : q.x), v = f2(k ? q.w : q.y);
-          h[k][0] = f2fma(ex2(f2mul(A[k][0], d)), h[k][0], f2mul(v, f2(b.x, b.y)));
-          h[k][1] = f2fma(ex2(f2mul(A[k][1], d)), h[k][1], f2mul(v, f2(b.z, b.w)));
+          h[k][0] = f2fma(decay_of(A[k][0], d), h[k][0], f2mul(v, f2(b.x, b.y)));
+          h[k][1] = f2fma(decay_of(A[k][1], d), h[k][1], f2mul(v, f2(b.z, b.w)));
           if constexpr (FULL) part[k] = f2hsum(f2fma(h[k][0], f2(c.x, c.y), f2mul(h[k][1], f2(c.z, c.w))));
         }
         if constexpr (FULL) {
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_step_kernel(const S
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      h[k] = fmaf(ex2(a[k] * LOG2E * d), start ? 0.f : h[k], u * bv[k]);
+      h[k] = fmaf(decay_of(f2(a[k] * LOG2E), d).x, start ? 0.f : h[k], u * bv[k]);
       s = fmaf(h[k], cv[k], s);
     }
 #pragma unroll

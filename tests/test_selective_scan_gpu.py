@@ -173,6 +173,17 @@ def test_extreme_steps():
     close(outs[1], want[1], "state", 2 * ELEMENT)
 
 
+def test_rates_that_keep_nothing():
+    """A rate of -inf keeps nothing of a state, in sequences of any length: 0 = exp(-inf) for every step above zero."""
+    ins, _ = make(1, 21, 8, 16, starts=False)
+    ins[2][:, 3] = float("-inf")
+    t = [v.cuda() for v in ins]
+    y, s = scan(tb.selective_scan, t, None)
+    want = scan(O.selective_scan, [v.double() for v in ins], None)
+    close(y, want[0], "y", 2 * ELEMENT)
+    close(s, want[1], "state", 2 * ELEMENT)
+
+
 def test_graph_capture_of_steps_and_training():
     ins, _ = make(4, 1, 64, 16, dtype=torch.bfloat16, starts=False)
     t = [v.cuda() for v in ins]

@@ -171,6 +171,7 @@ int check_norm(int64_t B, int64_t T, int64_t C, int G, int over, int dtype, int 
   if (activation < ttt::ACT_NONE || activation > ttt::ACT_GELU)
     return fail(TTT_ERR_UNSUPPORTED, "unknown activation %d (0: none, 1: SiLU, 2: GELU)", activation);
   if (!(eps >= 0.f)) return fail(TTT_ERR_SHAPE, "epsilon must be >= 0");
+  if (over == TTT_OVER_SEQUENCE && B * C >= (int64_t)1 << 34) return fail(TTT_ERR_SHAPE, "batch*channels must be below 2^34");
   return TTT_OK;
 }
 void norm_dims(ttt::NormParams* p, int64_t B, int64_t T, int64_t C, int G, int activation, float eps) {

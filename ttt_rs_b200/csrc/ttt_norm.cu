@@ -59,21 +59,46 @@ struct NormWalk {
   }
 };
 
-// sum over the lanes of a group; wide: over its warps too (red: a float per warp, all threads of the block take part)
+// Sums over the lanes of a group.  WIDE: over its warps too, through shared memory; all threads of the block take part, and the sums
+// go round four places, so that one barrier each is enough.
 template <bool WIDE>
-__device__ __forceinline__ float norm_sum(float v, int lanes, float* red) {
+struct NormSum;
+template <>
+struct NormSum<false> {
+  __device__ __forceinline__ float operator()(float v, int lanes) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if constexpr (WIDE) {
-    const int warp = threadIdx.x >> 5, first = warp & ~((lanes >> 5) - 1);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    for (int o = 16; o > 0; o >>= 1)
+      if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+};
+template <>
+struct NormSum<true> {
+  float* red;  // [4][warps]
+  int turn = 0;
+  __device__ __forceinline__ float operator()(float v, int lanes) {
+    constexpr int WARPS = NORM_WIDE / 32;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const int warp = threadIdx.x >> 5, warps = lanes >> 5, first = warp & ~(warps - 1);
+    float* at = red + (turn++ & 3) * WARPS;
+    if ((threadIdx.x & 31) == 0) at[warp] = v;
     __syncthreads();
     v = 0.f;
-    for (int k = 0; k < (lanes >> 5); ++k) v += red[first + k];
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k)
+      if (k < warps) v += at[first + k];
+    return v;
   }
-  return v;
+};
+template <bool WIDE>
+__device__ __forceinline__ NormSum<WIDE> norm_sum() {
+  if constexpr (WIDE) {
+    __shared__ float red[4 * NORM_WIDE / 32];
+    return {red};
+  } else {
+    return {};
+  }
 }
 
 template <typename T, int V>
@@ -102,14 +127,14 @@ struct NormLane {  // a thread's channels
 // difference from the mean and 1 / sqrt(var + eps) of a thread's channels (d: the channels on entry)
 template <typename T, int V, bool WIDE>
 __device__ __forceinline__ float norm_stats(F2 (&d)[NormLane<T, V>::NV][NormLane<T, V>::P], const NormLane<T, V>& me, const NormParams& p,
-                                            float* red) {
+                                            NormSum<WIDE>& sum) {
   using L = NormLane<T, V>;
   F2 s = f2(0.f);
 #pragma unroll
   for (int n = 0; n < L::NV; ++n)
 #pragma unroll
     for (int k = 0; k < L::P; ++k) s = f2add(s, d[n][k]);
-  const float mean = norm_sum<WIDE>(f2hsum(s), p.lanes, red) * p.inv_c;
+  const float mean = sum(f2hsum(s), p.lanes) * p.inv_c;
   F2 q = f2(0.f);
 #pragma unroll
   for (int n = 0; n < L::NV; ++n)
@@ -118,15 +143,15 @@ __device__ __forceinline__ float norm_stats(F2 (&d)[NormLane<T, V>::NV][NormLane
       d[n][k] = me.at[n] < 0 ? f2(0.f) : f2(d[n][k].x - mean, V > 1 ? d[n][k].y - mean : 0.f);
       q = f2fma(d[n][k], d[n][k], q);
     }
-  return rsqrtf(norm_sum<WIDE>(f2hsum(q), p.lanes, red) * p.inv_c + p.eps);
+  return rsqrtf(sum(f2hsum(q), p.lanes) * p.inv_c + p.eps);
 }
 
 template <typename T, int V, bool WIDE, int MODE>
-__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NORM_FWD_RESIDENT) ttt_norm_token_kernel(const NormParams p) {
+__global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? NORM_FWD_RESIDENT / 2 : NORM_FWD_RESIDENT) ttt_norm_token_kernel(const NormParams p) {
   using Ch = Chan<T, V>;
   using L = NormLane<T, V>;
-  constexpr int NV = L::NV, P = L::P, AHEAD = WIDE || V == 1 || sizeof(T) == 4 ? 1 : 2;
-  __shared__ float red[32];
+  constexpr int NV = L::NV, P = L::P, AHEAD = V == 1 || sizeof(T) == 4 ? 1 : 2;
+  NormSum<WIDE> sum = norm_sum<WIDE>();
   const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
   const int g = gcol / p.lanes, l = gcol & (p.lanes - 1), act = norm_act<MODE>(p);
   const bool live = row < p.rows && g < p.G, gated = norm_gated<MODE>(p);
@@ -162,7 +187,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NO
       F2 d[NV][P];
 #pragma unroll
       for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
-      const float r = norm_stats<T, V, WIDE>(d, me, p, red);
+      const float r = norm_stats<T, V, WIDE>(d, me, p, sum);
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
         F2 e[P];
@@ -189,7 +214,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NO
   using Ch = Chan<T, V>;
   using L = NormLane<T, V>;
   constexpr int NV = L::NV, P = L::P, AHEAD = 1;
-  __shared__ float red[32];
+  NormSum<WIDE> sum = norm_sum<WIDE>();
   const int row = threadIdx.x / p.cols, col = threadIdx.x - row * p.cols, gcol = (int)blockIdx.y * p.cols + col;
   const int g = gcol / p.lanes, l = gcol & (p.lanes - 1), act = norm_act<MODE>(p);
   const bool live = row < p.rows && g < p.G, gated = norm_gated<MODE>(p);
@@ -234,7 +259,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NO
       F2 d[NV][P];
 #pragma unroll
       for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
-      const float r = norm_stats<T, V, WIDE>(d, me, p, red);
+      const float r = norm_stats<T, V, WIDE>(d, me, p, sum);
       F2 q[NV][P], s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
@@ -268,7 +293,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NO
           out.store(ggate + to + me.at[n]);
         }
       }
-      const float m1 = norm_sum<WIDE>(f2hsum(s1), p.lanes, red) * p.inv_c, m2 = norm_sum<WIDE>(f2hsum(s2), p.lanes, red) * p.inv_c;
+      const float m1 = sum(f2hsum(s1), p.lanes) * p.inv_c, m2 = sum(f2hsum(s2), p.lanes) * p.inv_c;
 #pragma unroll
       for (int n = 0; n < NV; ++n) {
 #pragma unroll
@@ -673,8 +698,9 @@ static NormCut norm_token_cut(int64_t tokens, int G, int c, bool bwd) {
   k.rows = k.cols < NORM_THREADS ? NORM_THREADS / k.cols : 1;
   k.threads = (k.cols * k.rows + 31) / 32 * 32;
   k.y = (int)((total + k.cols - 1) / k.cols);
-  const int regs = 65536 / (NORM_THREADS * (bwd ? NORM_BWD_RESIDENT : NORM_FWD_RESIDENT));
-  const int64_t resident = k.threads > NORM_THREADS ? 1 : 65536 / (regs * k.threads);
+  const bool wide = k.lanes > 32;
+  const int regs = !bwd ? 65536 / (NORM_THREADS * NORM_FWD_RESIDENT) : wide ? 65536 / NORM_WIDE : 65536 / (NORM_THREADS * NORM_BWD_RESIDENT);
+  const int64_t resident = 65536 / (regs * k.threads);
   const int64_t need = (tokens + k.rows - 1) / k.rows, wanted = 148 * resident / k.y, most = wanted > 1 ? wanted : 1;
   k.x = need < most ? need : most;
   return k;

@@ -185,6 +185,15 @@ struct SelLane {
     sl = lane & (S::SL - 1);
     ch = (threadIdx.x >> 5) * S::WARP_CH + (lane / S::SL) * S::CC;
   }
+  // rates, times log2 e; one of -inf as the lowest number, so that a step of zero (behind the last token) keeps what there is
+  __device__ __forceinline__ void load_rates(F2 (&A)[S::CC][2], const float* rows, int n, int have) const {
+    load(A, rows, n, have);
+    auto scaled = [](float a) { return a * LOG2E < -3.4e38f ? -3.4e38f : a * LOG2E; };
+#pragma unroll
+    for (int k = 0; k < S::CC; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) A[k][i] = f2(scaled(A[k][i].x), scaled(A[k][i].y));
+  }
   // row of `n` states (N in memory) of channel c0 + ch + k, zeros beyond
   __device__ __forceinline__ void load(F2 (&v)[S::CC][2], const float* rows, int n, int have) const {
 #pragma unroll

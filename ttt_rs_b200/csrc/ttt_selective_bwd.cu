@@ -63,11 +63,9 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
     const SelLane<NP> me;
     const int my_share = share_at<NP>(me.ch / S::CC, me.sl);
     F2 A[S::CC][2], dh[S::CC][2], dA[S::CC][2];
-    me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
+    me.load_rates(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
 #pragma unroll
-    for (int k = 0; k < S::CC; ++k)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) A[k][i] = f2mul(A[k][i], f2(LOG2E)), dA[k][i] = f2(0.f);
+    for (int k = 0; k < S::CC; ++k) dA[k][0] = dA[k][1] = f2(0.f);
     gradient_behind<NP>(dh, A, me, at, p);
     const float* saved = p.saved + ((at.b * ((p.T + SEL_TILE - 1) / SEL_TILE) + at.t_lo / SEL_TILE + tiles - 1) * p.C + at.c0) * NP;
     F2 next[S::CC][2];
@@ -375,11 +373,9 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_rev_kernel(const Se
   const int64_t t_last = at.t_lo + (at.t_hi - at.t_lo - 1) / SEL_TILE * SEL_TILE;
   fetch(t_last, 0);
   F2 A[S::CC][2], dh[S::CC][2];
-  me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
+  me.load_rates(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
 #pragma unroll
-  for (int k = 0; k < S::CC; ++k)
-#pragma unroll
-    for (int i = 0; i < 2; ++i) A[k][i] = f2mul(A[k][i], f2(LOG2E)), dh[k][i] = f2(0.f);
+  for (int k = 0; k < S::CC; ++k) dh[k][0] = dh[k][1] = f2(0.f);
   const int pr = tid % S::PAIRS, row0 = tid / S::PAIRS, pair_have = at.have - 2 * pr;
   float2 bias = make_float2(0.f, 0.f), sum = make_float2(0.f, 0.f);
   if (p.bias != nullptr) {

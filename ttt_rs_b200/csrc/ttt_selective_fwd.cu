@@ -33,9 +33,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
     const SelLane<NP> me;
     [[maybe_unused]] const int my_share = share_at<NP>(me.ch / S::CC, me.sl);
     F2 A[S::CC][2], h[S::CC][2];
-    me.load(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
-#pragma unroll
-    for (int k = 0; k < S::CC; ++k) A[k][0] = f2mul(A[k][0], f2(LOG2E)), A[k][1] = f2mul(A[k][1], f2(LOG2E));
+    me.load_rates(A, p.A + (int64_t)at.c0 * p.N, p.N, at.have);
     if constexpr (FULL) {
       if (p.nseg == 1) me.load(h, p.state != nullptr ? p.state + (at.b * p.C + at.c0) * p.N : nullptr, p.N, at.have);
       else me.load_padded(h, p.seg_state + ((p.B * p.nseg + at.b) * p.C + at.c0) * NP, at.have);

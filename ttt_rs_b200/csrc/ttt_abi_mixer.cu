@@ -259,8 +259,8 @@ struct SelDims {
   int64_t B, T, C;
   int G, N, dtype;
   int NP, es;
-  ttt::SelCut cut[2];  // forward, backward
-  int64_t tiles, blocks;
+  int64_t tiles;
+  ttt::SelCut cut(bool backward) const { return ttt::sel_cut(B, T, (int)C, G, N, backward); }
 };
 int sel_dims(SelDims* d, int64_t B, int64_t T, int64_t C, int G, int N, int dtype) {
   const int rc = check_sizes(B, T, C, dtype);
@@ -272,9 +272,7 @@ int sel_dims(SelDims* d, int64_t B, int64_t T, int64_t C, int G, int N, int dtyp
   d->B = B, d->T = T, d->C = C, d->G = G, d->N = N, d->dtype = dtype;
   d->NP = ttt::sel_padded(N);
   d->es = dtype == TTT_BF16 ? 2 : 4;
-  for (int k = 0; k < 2; ++k) d->cut[k] = ttt::sel_cut(B, T, (int)C, G, N, k != 0);
   d->tiles = (T + ttt::SEL_TILE - 1) / ttt::SEL_TILE;
-  d->blocks = d->cut[0].channel_blocks;
   return TTT_OK;
 }
 int64_t up4(int64_t n) { return (n + 3) & ~(int64_t)3; }
@@ -283,9 +281,9 @@ int64_t seg_floats(const SelDims& d, const ttt::SelCut& k) {
   return k.nseg == 1 ? 0 : d.B * (k.nseg + 1) * d.C * d.NP + up4(d.B * k.nseg * d.C);
 }
 int64_t saved_floats(const SelDims& d) { return d.B * d.tiles * d.C * d.NP; }
-int64_t backward_floats(const SelDims& d) {
-  const int64_t rows = d.B * d.cut[1].nseg;
-  return d.B * d.G * d.blocks * d.T * 2 * d.NP + rows * d.C * d.NP + up4(rows * 2 * d.C) + seg_floats(d, d.cut[1]);
+int64_t backward_floats(const SelDims& d, const ttt::SelCut& k) {
+  const int64_t rows = d.B * k.nseg;
+  return d.B * d.G * k.channel_blocks * d.T * 2 * d.NP + rows * d.C * d.NP + up4(rows * 2 * d.C) + seg_floats(d, k);
 }
 void set_segments(ttt::SelParams* p, const SelDims& d, const ttt::SelCut& k, float* at) {
   p->nseg = k.nseg, p->seg_tiles = k.seg_tiles;
@@ -358,12 +356,12 @@ extern "C" size_t ttt_linear_selective_saved_bytes(int64_t batch, int64_t seq_le
 extern "C" size_t ttt_linear_selective_forward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,
                                                                int dtype) {
   SelDims d;
-  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * seg_floats(d, d.cut[0]) : 0;
+  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * seg_floats(d, d.cut(false)) : 0;
 }
 extern "C" size_t ttt_linear_selective_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,
                                                                 int dtype) {
   SelDims d;
-  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * backward_floats(d) : 0;
+  return sel_dims(&d, batch, seq_len, channels, groups, states, dtype) == TTT_OK ? sizeof(float) * backward_floats(d, d.cut(true)) : 0;
 }
 
 extern "C" int ttt_linear_selective_forward(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype, int softplus,
@@ -401,9 +399,10 @@ extern "C" int ttt_linear_selective_forward(int64_t batch, int64_t seq_len, int6
   p.y = y, p.state_out = state_out;
   if (saved == nullptr && seq_len <= 16) return launched(ttt::launch_selective_step(dtype, p, static_cast<cudaStream_t>(stream)), "selective step");
   if (saved != nullptr && (rc = check_bytes(saved_bytes, sizeof(float) * saved_floats(d), saved, "saved")) != TTT_OK) return rc;
-  if ((rc = check_bytes(workspace_bytes, sizeof(float) * seg_floats(d, d.cut[0]), workspace, "workspace")) != TTT_OK) return rc;
+  const ttt::SelCut cut = d.cut(false);
+  if ((rc = check_bytes(workspace_bytes, sizeof(float) * seg_floats(d, cut), workspace, "workspace")) != TTT_OK) return rc;
   p.saved = static_cast<float*>(saved);
-  set_segments(&p, d, d.cut[0], static_cast<float*>(workspace));
+  set_segments(&p, d, cut, static_cast<float*>(workspace));
   return launched(ttt::launch_selective(dtype, p, static_cast<cudaStream_t>(stream)), "selective scan");
 }
 
@@ -435,13 +434,14 @@ extern "C" int ttt_linear_selective_backward(int64_t batch, int64_t seq_len, int
     if (q.needed && q.p == nullptr) return fail(TTT_ERR_NULL, "%s is null", q.name);
     if (reinterpret_cast<uintptr_t>(q.p) % q.align != 0) return fail(TTT_ERR_ALIGN, "%s is not aligned to its elements", q.name);
   }
-  if ((rc = check_bytes(workspace_bytes, sizeof(float) * backward_floats(d), workspace, "workspace")) != TTT_OK) return rc;
+  const ttt::SelCut cut = d.cut(true);
+  if ((rc = check_bytes(workspace_bytes, sizeof(float) * backward_floats(d, cut), workspace, "workspace")) != TTT_OK) return rc;
   float* ws = static_cast<float*>(workspace);
-  const int64_t rows = d.B * d.cut[1].nseg;
-  p.part_bc = ws, ws += d.B * d.G * d.blocks * d.T * 2 * d.NP;
+  const int64_t rows = d.B * cut.nseg;
+  p.part_bc = ws, ws += d.B * d.G * cut.channel_blocks * d.T * 2 * d.NP;
   p.part_a = ws, ws += rows * d.C * d.NP;
   p.part_d = ws, ws += up4(rows * 2 * d.C);
-  set_segments(&p, d, d.cut[1], ws);
+  set_segments(&p, d, cut, ws);
   p.softplus = softplus != 0;
   p.saved = static_cast<float*>(const_cast<void*>(saved));
   p.gy = grad_y, p.gstate_out = grad_state_out, p.gx = grad_x, p.gdt = grad_dt, p.gz = grad_z, p.ga = grad_a, p.gb = grad_b, p.gc = grad_c;

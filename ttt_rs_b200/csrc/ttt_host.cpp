@@ -687,12 +687,13 @@ struct Selective {
            m.vector(o[0], at::kFloat) && (!o[1].defined() || (channel_rows(o[1], m.dev, m.dt) && o[1].sizes() == t[0].sizes())) &&
            m.vector(o[2], at::kFloat) && held(o[3]) && m.marks(o[4]);
   }
-  std::vector<int64_t> strides(std::initializer_list<const Tensor*> rows, const Tensor& b, const Tensor& c) const {
-    std::vector<int64_t> s;
+  static std::array<int64_t, 14> strides(std::initializer_list<const Tensor*> rows, const Tensor& b, const Tensor& c) {
+    std::array<int64_t, 14> s{};
+    size_t i = 0;
     for (const Tensor* t : rows)
-      for (int k = 0; k < 2; ++k) s.push_back(t->defined() ? t->stride(k) : 0);
+      for (int k = 0; k < 2; ++k) s[i++] = t->defined() ? t->stride(k) : 0;
     for (const Tensor* t : {&b, &c})
-      for (int k = 0; k < 3; ++k) s.push_back(t->stride(k));
+      for (int k = 0; k < 3; ++k) s[i++] = t->stride(k);
     return s;
   }
   static const float* f32(const Tensor& t) { return static_cast<const float*>(ptr(t)); }

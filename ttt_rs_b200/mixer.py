@@ -13,14 +13,13 @@ from . import _lib
 from ._lib import TttError
 from .fused import _expect
 
-_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
+_CONV_ACTIVATIONS = {None: 0, "silu": 1}
+_NORM_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}
 _OVER = {"token": 0, "sequence": 1}
 
 
-def _activation(name: Optional[str], known) -> int:
-    if name not in known:
-        raise TttError(_lib.TTT_ERR_UNSUPPORTED, f"activation must be one of {known} (got {name!r})")
-    return _ACTIVATIONS[name]
+def _unknown(what: str, name, known) -> TttError:
+    return TttError(_lib.TTT_ERR_UNSUPPORTED, f"{what} must be one of {tuple(known)} (got {name!r})")
 
 
 def _check_rows(name: str, x: torch.Tensor):
@@ -79,7 +78,9 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     is the last K-1 inputs as far as they are visible (zeros elsewhere), in `state_out` where given (it may be `state` itself but share
     nothing with another tensor; not recorded for autograd, and refused where that asks for gradients).  Differentiable with respect to
     x, weight, bias and state, through both results, once and not in forward mode; sums are float32."""
-    act = _activation(activation, (None, "silu"))
+    act = _CONV_ACTIVATIONS.get(activation)
+    if act is None:
+        raise _unknown("activation", activation, _CONV_ACTIVATIONS)
     native = _lib.host().causal_conv(x, weight, bias, state, act, starts, state_out)
     if native is not None:
         return native
@@ -166,10 +167,12 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
     weight + bias (weight, bias [C] of x's type; None: ones, zeros) the result is act(u), or, given a gate [B,T,C], u * act(gate);
     activation None, "silu" or "gelu" (tanh form).  Contiguous [B,T,C].  Differentiable with respect to x, weight, bias and gate, once
     and not in forward mode; statistics and sums are float32, variances are taken from differences."""
-    act = _activation(activation, (None, "silu", "gelu"))
-    if over not in _OVER:
-        raise TttError(_lib.TTT_ERR_UNSUPPORTED, f"over must be one of {tuple(_OVER)} (got {over!r})")
-    native = _lib.host().group_norm(x, groups, weight, bias, gate, act, eps, _OVER[over])
+    act, place = _NORM_ACTIVATIONS.get(activation), _OVER.get(over)
+    if act is None:
+        raise _unknown("activation", activation, _NORM_ACTIVATIONS)
+    if place is None:
+        raise _unknown("over", over, _OVER)
+    native = _lib.host().group_norm(x, groups, weight, bias, gate, act, eps, place)
     if native is not None:
         return native
     _check_rows("x", x)
@@ -181,7 +184,7 @@ def group_norm(x: torch.Tensor, groups: int, weight: Optional[torch.Tensor] = No
             _expect(name, t, (C,), x.dtype, x.device)
     if gate is not None:
         _expect("gate", gate, x.shape, x.dtype, x.device)
-    native = _lib.host().group_norm(_rows(x), groups, _dense(weight), _dense(bias), _rows(gate), act, eps, _OVER[over])
+    native = _lib.host().group_norm(_rows(x), groups, _dense(weight), _dense(bias), _rows(gate), act, eps, place)
     if native is None:
         raise TttError(_lib.TTT_ERR_SHAPE, _lib.last_error() or "unsupported problem for the group norm")
     return native

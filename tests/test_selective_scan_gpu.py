@@ -117,6 +117,17 @@ def test_token_by_token_is_the_sequence(dtype):
     close(state, want[1], "state", 2 * ELEMENT)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,C,N,G", [(64, 640, 16, 1), (64, 640, 10, 5), (40, 256, 64, 1), (160, 1000, 3, 1), (64, 1300, 8, 2), (33, 700, 32, 7)])
+def test_steps_of_many_sequences(B, C, N, G, dtype):
+    """Steps whose threads would not all be resident hold more states each."""
+    ins, marks = make(B, 2, C, N, G, dtype, starts=True)
+    got = scan(tb.selective_scan, [t.cuda() for t in ins], marks.cuda())
+    want = scan(O.selective_scan, [t.double() for t in ins], marks)
+    close(got[0], want[0], "y", 2 * ELEMENT)
+    close(got[1], want[1], "state", 2 * ELEMENT)
+
+
 def test_a_state_in_place_over_segments():
     ins, _ = make(1, 3000, 16, 16, dtype=torch.bfloat16, starts=False)
     t = [v.cuda() for v in ins]

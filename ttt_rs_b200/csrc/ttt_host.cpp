@@ -1541,6 +1541,8 @@ PyObject* py_selective(PyObject*, PyObject* const* args, Py_ssize_t n) {
   NONE_IF(!optional_tensor(args[11], out));
   const int64_t softplus = as_int(args[10]);
   if (PyErr_Occurred()) return nullptr;
+  for (int i = 3; i < 5; ++i)
+    if (t[i].dim() == 3) t[i] = t[i].unsqueeze(2);  // one group
   refuse_tangents({&t[0], &t[1], &t[2], &t[3], &t[4], &o[0], &o[1], &o[2], &o[3], &out});
   Selective call;
   NONE_IF(!call.set(t, o, softplus) || !call.held(out));

@@ -119,9 +119,6 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     even a NaN.  The new state goes to `state_out` where given (it may be `state` itself but share nothing with another tensor; not
     recorded for autograd, and refused where that asks for gradients).  Differentiable with respect to all nine, through both results,
     once and not in forward mode.  Steps, decays, states and sums are float32, and results are rounded to bfloat16 once."""
-    one = isinstance(B, torch.Tensor) and isinstance(C, torch.Tensor) and B.dim() == 3 and C.dim() == 3
-    if one:
-        B, C = B.unsqueeze(2), C.unsqueeze(2)
     native = _lib.host().selective(x, dt, A, B, C, D, z, dt_bias, state, starts, softplus, state_out)
     if native is not None:
         return native
@@ -129,6 +126,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     b, T, ch = x.shape
     dev = x.device
     _expect("dt", dt, x.shape, x.dtype, dev)
+    B, C = (t.unsqueeze(2) if t.dim() == 3 else t for t in (B, C))
     if B.dim() != 4 or ch % max(1, B.shape[2]) or B.numel() == 0:
         raise TttError(_lib.TTT_ERR_SHAPE, f"B must be [batch, seq_len, groups, states] with groups that divide {ch} channels, got {tuple(B.shape)}")
     G, N = B.shape[2:]

@@ -9,10 +9,13 @@
 // Memory-bound.
 //   A token's groups: eight channels per thread, a group to a power of two of lanes (several warps where it has more than 256
 //   channels), everything in registers between one read and one write.  A thread keeps its channels from token to token, so that
-//   weights and their gradients stay in registers; the backward's blocks leave a row of sums each, joined in a fixed order.
+//   weights and their gradients stay in registers; the backward's blocks leave a row of sums each, joined in a fixed order.  bf16, 65536
+//   tokens of 24 heads of 64 channels with gate: 117 us (5.2 TB/s, 0.79 of a copy), gradient 212 us (4.7 TB/s, 0.72; with two tokens at a
+//   time, which two instead of three blocks per SM have room for, 250 us); SiLU known when the kernel is built: 151 and 455 us before that.
+//   One group of 1536 channels: 252 and 533 us, the barriers of the block's sums.
 //   A sequence's groups: a pass for the statistics (backward: for every channel's sums of du and du n) and one that applies them,
 //   which reads x again, from L2 where the tensors fit.  Chunks of tokens leave (mean, sum of squares) pairs that every block of the
-//   second pass joins in the same order.
+//   second pass joins in the same order.  16 x 4096 x 512: 20 + 28 us, gradient 39 + 5 + 38 + 3 us (135 MB in and out 2.8 TB/s forward).
 #include "ttt_kernels.h"
 #include "ttt_vec.cuh"
 

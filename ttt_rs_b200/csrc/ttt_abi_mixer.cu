@@ -87,6 +87,11 @@ int check_conv(int64_t B, int64_t T, int64_t C, int taps, int dtype, int activat
   return TTT_OK;
 }
 
+int conv_width(uintptr_t low, int64_t channels, int es) {
+  if (low % (4 * es) == 0 && channels % 4 == 0) return 4;
+  return es == 2 && low % 4 == 0 && channels % 2 == 0 ? 2 : 1;
+}
+
 }  // namespace
 
 extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype, int activation, const void* x,
@@ -102,7 +107,7 @@ extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t cha
   s.need("state_out", state_out);
   s.align("state", state);
   s.need("weight", weight);
-  const bool vec = s.low % (4 * es) == 0 && channels % 4 == 0;
+  const int width = conv_width(s.low, channels, es);
   s.align("bias", bias);
   if (s.rc != TTT_OK) return s.rc;
   const int64_t held = batch * (taps - 1) * channels * es, n = batch * seq_len * channels * es;
@@ -118,7 +123,7 @@ extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t cha
   p.x = x, p.w = weight, p.bias = bias, p.state = state, p.starts = static_cast<const uint8_t*>(starts);
   p.y = y, p.state_out = state_out;
   p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
-  return launched(ttt::launch_conv(dtype, p, taps, vec, false, static_cast<cudaStream_t>(stream)), "causal convolution");
+  return launched(ttt::launch_conv(dtype, p, taps, width, false, static_cast<cudaStream_t>(stream)), "causal convolution");
 }
 
 extern "C" size_t ttt_layer_causal_conv_backward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype) {
@@ -143,7 +148,7 @@ extern "C" int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, in
   s.align("grad_state_out", grad_state_out);
   s.align("grad_state", grad_state);
   s.need("weight", weight);
-  const bool vec = s.low % (4 * es) == 0 && channels % 4 == 0;
+  const int width = conv_width(s.low, channels, es);
   s.align("bias", bias);
   s.align("grad_weight", grad_weight);
   s.align("grad_bias", grad_bias);
@@ -156,7 +161,7 @@ extern "C" int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, in
   p.gy = grad_y, p.gstate_out = grad_state_out, p.gx = grad_x, p.gstate = grad_state, p.gw = grad_weight, p.gbias = grad_bias;
   p.partials = sums ? static_cast<float*>(workspace) : nullptr;
   p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
-  return launched(ttt::launch_conv(dtype, p, taps, vec, true, static_cast<cudaStream_t>(stream)), "causal convolution backward");
+  return launched(ttt::launch_conv(dtype, p, taps, width, true, static_cast<cudaStream_t>(stream)), "causal convolution backward");
 }
 
 namespace {

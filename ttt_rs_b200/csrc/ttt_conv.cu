@@ -5,8 +5,8 @@
 // is the last K - 1 inputs, as they are visible behind the last token.  With g_t = dy_t act'(v_t):
 //   dx_s = sum_j w_j g_{s+K-1-j} over the tokens that saw s (+ the new state's gradient),  dw_j = sum_t g_t x_{t-K+1+j},  db = sum_t g_t
 //
-// Memory-bound by its bytes, held back by instructions and latency.  A thread holds four neighbouring channels (one, where rows are
-// off a vector's address) and walks a strip of tokens with the last K - 1 inputs in registers and the next few tokens on their way; the
+// Memory-bound by its bytes, held back by instructions and latency.  A thread holds four neighbouring channels (two of bf16, or one,
+// where rows are off a vector's address) and walks a strip of tokens with the last K - 1 inputs in registers and the next few tokens on their way; the
 // tokens before a strip (and behind it, for dx) are read again, from L2.  Whole groups of tokens inside a strip go without checks.  A
 // start empties the registers of the inputs, and the sums of dx know the last start's place; without starts, kernels know of none.
 // bf16, 65536 tokens of 1536 channels, 4 taps, SiLU: 94 us forward (4.3 TB/s, 0.65 of a copy), 167 us backward (3.6 TB/s, 0.55).  Eight
@@ -383,9 +383,9 @@ static ConvCut conv_cut(int64_t B, int64_t T, int C, int V, bool bwd) {
   k.x = need < most ? need : most;
   return k;
 }
-size_t conv_partial_floats(int64_t B, int64_t T, int C, int K) {  // for either width
+size_t conv_partial_floats(int64_t B, int64_t T, int C, int K) {  // for any width
   size_t most = 0;
-  for (int V : {1, 4}) {
+  for (int V : {1, 2, 4}) {
     const size_t n = (size_t)conv_cut(B, T, C, V, true).x * (K + 1) * C;
     if (n > most) most = n;
   }
@@ -422,9 +422,11 @@ static cudaError_t launch_k(const ConvParams& p, int taps, bool bwd, cudaStream_
     default: return launch_kind<T, V, 4>(p, bwd, st);
   }
 }
-cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, bool vec, bool bwd, cudaStream_t st) {
-  if (dtype == 1) return vec ? launch_k<__nv_bfloat16, 4>(p, taps, bwd, st) : launch_k<__nv_bfloat16, 1>(p, taps, bwd, st);
-  return vec ? launch_k<float, 4>(p, taps, bwd, st) : launch_k<float, 1>(p, taps, bwd, st);
+cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, int V, bool bwd, cudaStream_t st) {
+  if (dtype == 1)
+    return V == 4 ? launch_k<__nv_bfloat16, 4>(p, taps, bwd, st) : V == 2 ? launch_k<__nv_bfloat16, 2>(p, taps, bwd, st)
+                                                                          : launch_k<__nv_bfloat16, 1>(p, taps, bwd, st);
+  return V == 4 ? launch_k<float, 4>(p, taps, bwd, st) : launch_k<float, 1>(p, taps, bwd, st);
 }
 
 }  // namespace ttt

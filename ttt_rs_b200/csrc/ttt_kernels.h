@@ -504,8 +504,8 @@ struct ConvParams {
   int64_t strips;
 };
 size_t conv_partial_floats(int64_t B, int64_t T, int C, int K);
-// vec: channels are a multiple of 4, and all addresses of 4 channels
-cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, bool vec, bool bwd, cudaStream_t st);
+// V: channels at a time, 4, 2 (bf16) or 1, of which channels and all addresses are multiples
+cudaError_t launch_conv(int dtype, const ConvParams& p, int taps, int V, bool bwd, cudaStream_t st);
 
 // ---- group norm (ttt_norm.cu): tensors [B,T,C] with contiguous channels ------------------------------------------------------------
 struct NormParams {

@@ -90,8 +90,8 @@ __device__ __forceinline__ void helpers_sync() { asm volatile("bar.sync 1, %0;" 
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // rows [t0, t0 + SEL_TILE) of `have` elements, at most WIDE, into dst [SEL_TILE][WIDE]; zeros beyond T and `have`.  bytes: 16, 4, or an
-// element's size, what addresses, strides and `have` are multiples of.
-template <typename T, int WIDE>
+// element's size, what addresses, strides and `have` are multiples of; by elements, AHEAD are on their way at a time.
+template <typename T, int WIDE, int AHEAD>
 __device__ __forceinline__ void copy_rows(int tid, T* dst, const T* src, int64_t stride, int64_t t0, int64_t t_end, int have, int bytes) {
   constexpr int V16 = 16 / sizeof(T);
   if (WIDE >= V16 && bytes == 16) {
@@ -109,9 +109,18 @@ __device__ __forceinline__ void copy_rows(int tid, T* dst, const T* src, int64_t
       copy_async4(dst + r * WIDE + e, live ? src + (t0 + r) * stride + e : src, live);
     }
   } else {
-    for (int i = tid; i < SEL_TILE * WIDE; i += SEL_THREADS) {
-      const int r = i / WIDE, e = i - r * WIDE;
-      dst[i] = t0 + r < t_end && e < have ? src[(t0 + r) * stride + e] : T(0.f);
+    constexpr int MOST = (SEL_TILE * WIDE + SEL_THREADS - 1) / SEL_THREADS, PER = MOST < AHEAD ? MOST : AHEAD;
+    for (int i0 = tid; i0 < SEL_TILE * WIDE; i0 += PER * SEL_THREADS) {
+      T v[PER];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int i = i0 + k * SEL_THREADS, r = i / WIDE, e = i - r * WIDE;
+        v[k] = T(0.f);
+        if (i < SEL_TILE * WIDE && t0 + r < t_end && e < have) v[k] = src[(t0 + r) * stride + e];
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (i0 + k * SEL_THREADS < SEL_TILE * WIDE) dst[i0 + k * SEL_THREADS] = v[k];
     }
   }
 }

@@ -228,13 +228,13 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
   auto fetch = [&](int i) {
     const int k = i % SEL_STAGES;
     const int64_t t0 = at.t_lo + (int64_t)(tiles - 1 - i) * SEL_TILE;
-    copy_rows<T, S::CH>(tid, &sm.raw[k][0][0][0], static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0, p.ds[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(tid, &sm.raw[k][1][0][0], static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0, p.gs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH, 1>(tid, &sm.raw[k][0][0][0], static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH, 1>(tid, &sm.raw[k][1][0][0], static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0, p.gs[1], t0, at.t_hi, at.have, p.xg);
     if (p.z != nullptr)
-      copy_rows<T, S::CH>(tid, &sm.raw[k][2][0][0], static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0, p.zs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(tid, &sm.raw[k][3][0][0], static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c0, p.xs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, NP>(tid, &sm.raw_bc[k][0][0][0], static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2], p.cs[1], t0, at.t_hi, p.N, p.bg);
-    copy_rows<T, NP>(tid, &sm.raw_bc[k][1][0][0], static_cast<const T*>(p.b) + at.b * p.bs[0] + at.g * p.bs[2], p.bs[1], t0, at.t_hi, p.N, p.bg);
+      copy_rows<T, S::CH, 1>(tid, &sm.raw[k][2][0][0], static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0, p.zs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH, 1>(tid, &sm.raw[k][3][0][0], static_cast<const T*>(p.x) + at.b * p.xs[0] + at.c0, p.xs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP, 1>(tid, &sm.raw_bc[k][0][0][0], static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2], p.cs[1], t0, at.t_hi, p.N, p.bg);
+    copy_rows<T, NP, 1>(tid, &sm.raw_bc[k][1][0][0], static_cast<const T*>(p.b) + at.b * p.bs[0] + at.g * p.bs[2], p.bs[1], t0, at.t_hi, p.N, p.bg);
     copy_commit();
     if constexpr (MARKS) {
       const int64_t t = t0 + (tid & 31);
@@ -370,11 +370,11 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_rev_kernel(const Se
   const SelLane<NP> me;
   const int tid = threadIdx.x;
   auto fetch = [&](int64_t t0, int k) {
-    copy_rows<T, S::CH>(tid, &sm.raw[k][0][0][0], static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0, p.ds[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(tid, &sm.raw[k][1][0][0], static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0, p.gs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH, 1>(tid, &sm.raw[k][0][0][0], static_cast<const T*>(p.dt) + at.b * p.ds[0] + at.c0, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH, 1>(tid, &sm.raw[k][1][0][0], static_cast<const T*>(p.gy) + at.b * p.gs[0] + at.c0, p.gs[1], t0, at.t_hi, at.have, p.xg);
     if (p.z != nullptr)
-      copy_rows<T, S::CH>(tid, &sm.raw[k][2][0][0], static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0, p.zs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, NP>(tid, &sm.raw_c[k][0][0], static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2], p.cs[1], t0, at.t_hi, p.N, p.bg);
+      copy_rows<T, S::CH, 1>(tid, &sm.raw[k][2][0][0], static_cast<const T*>(p.z) + at.b * p.zs[0] + at.c0, p.zs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP, 1>(tid, &sm.raw_c[k][0][0], static_cast<const T*>(p.c) + at.b * p.cs[0] + at.g * p.cs[2], p.cs[1], t0, at.t_hi, p.N, p.bg);
     copy_commit();
   };
   const int64_t t_last = at.t_lo + (at.t_hi - at.t_lo - 1) / SEL_TILE * SEL_TILE;

@@ -122,12 +122,12 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 3) ttt_selective_kernel(const
   auto fetch = [&](int i) {
     const int k = i % SEL_STAGES;
     const int64_t t0 = at.t_lo + (int64_t)i * SEL_TILE;
-    copy_rows<T, S::CH>(tid, &sm.raw[k][0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, S::CH>(tid, &sm.raw[k][1][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
-    copy_rows<T, NP>(tid, &sm.raw_bc[k][0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
+    copy_rows<T, S::CH, 8>(tid, &sm.raw[k][0][0][0], x, p.xs[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, S::CH, 8>(tid, &sm.raw[k][1][0][0], dt, p.ds[1], t0, at.t_hi, at.have, p.xg);
+    copy_rows<T, NP, 8>(tid, &sm.raw_bc[k][0][0][0], bm, p.bs[1], t0, at.t_hi, p.N, p.bg);
     if constexpr (FULL) {
-      if (z != nullptr) copy_rows<T, S::CH>(tid, &sm.raw[k][Smem::TENSORS - 1][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
-      copy_rows<T, NP>(tid, &sm.raw_bc[k][FULL ? 1 : 0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
+      if (z != nullptr) copy_rows<T, S::CH, 8>(tid, &sm.raw[k][Smem::TENSORS - 1][0][0], z, p.zs[1], t0, at.t_hi, at.have, p.xg);
+      copy_rows<T, NP, 8>(tid, &sm.raw_bc[k][FULL ? 1 : 0][0][0], cm, p.cs[1], t0, at.t_hi, p.N, p.bg);
     }
     copy_commit();
     if constexpr (MARKS) {

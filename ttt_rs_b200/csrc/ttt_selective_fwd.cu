@@ -307,19 +307,18 @@ SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd) {
   SelCut k{};
   k.channel_blocks = (each + CH - 1) / CH;
   const int64_t blocks = B * G * k.channel_blocks, tiles = (T + SEL_TILE - 1) / SEL_TILE;
-  const int resident = bwd ? 2 : 4;
-  // As many segments as make the slowest SM's work least: tiles after one another, `resident` blocks of them for the price of about
-  // one and a half; the segments' own states cost about two thirds of the scan itself (backward: a third).
-  double least = 0.0;
-  k.nseg = 1;
-  for (int n = 1; n <= 64 && n <= tiles; ++n) {
-    const int64_t each_tiles = (tiles + n - 1) / n, total = blocks * ((tiles + each_tiles - 1) / each_tiles), per_sm = (total + 147) / 148;
-    const double rounds = (double)(per_sm / resident) * 1.0 + (per_sm % resident ? 0.6 + 0.4 * (per_sm % resident) / resident : 0.0);
-    const double cost = rounds * each_tiles * (n == 1 ? 1.0 : bwd ? 1.33 : 1.67) + (n == 1 ? 0.0 : 4.0 + 0.25 * n);
-    if (n > 1 && cost >= least) continue;
-    least = cost;
-    k.nseg = n;
-  }
+  // Forward: as many segments as blocks are resident (three per SM).  Backward: two rounds of those resident (two per SM), which shares
+  // the last round out; four where a block per SM leaves little idle anyway, and none there with 64 states, whose gradients
+  // carried back cost more.  Segments of two tiles at least, of four beyond 32 of them: a block joins all that are before it.
+  // us, 16 states: 1 x 32768 x 1536: 18 segments 580, 12 623, 24 615, 36 574; backward 24 1373, 12 1439, 32 1517.  2 x 4096 x 1536: 9
+  // segments 161, 6 169, 12 179; backward 12 392, 6 396, 8 441.  4 x 2048 x 2048: 3 segments 201, 1 229, 4 220; backward 9 to 12
+  // 500, 1 550, 4 523.  1 x 512 x 512: 16 segments 21, 8 27; backward 16 46, 8 62.  (64 states, 2 x 2048 x 1024: backward 1 611, 8 654.)
+  int64_t wanted = 444 / blocks;
+  if (bwd) wanted = blocks < 100 ? 592 / blocks : blocks <= 148 && NP < 64 ? 1184 / blocks : 1;
+  int64_t most = tiles / 4 > 32 ? tiles / 4 : 32;
+  if (most > tiles / 2) most = tiles / 2;
+  if (wanted > most) wanted = most;
+  k.nseg = wanted > 1 ? (int)wanted : 1;
   k.seg_tiles = (int)((tiles + k.nseg - 1) / k.nseg);
   k.nseg = (int)((tiles + k.seg_tiles - 1) / k.seg_tiles);
   return k;

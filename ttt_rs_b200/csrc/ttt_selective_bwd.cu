@@ -449,28 +449,42 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_rev_kernel(const Se
 // The blocks' shares of dB and dC, [B][G][blocks][T][2][NP] -> [B][T][G][N] each
 template <typename T>
 __global__ void __launch_bounds__(256) ttt_selective_bc_kernel(const SelParams p, int NP, int blocks) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // (b G + g) T 2 NP + t 2 NP + ...
-  const int64_t per = p.T * 2 * NP;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = p.T * NP / 2;  // four states each: (b G + g) T 2 NP / 4 + ...
   if (i >= p.B * p.G * per) return;
   const int64_t bg = i / per, e = i - bg * per;
-  const float* src = p.part_bc + bg * blocks * per + e;
-  float v = 0.f;
-  for (int k = 0; k < blocks; ++k) v += src[k * per];
-  const int64_t t = e / (2 * NP);
-  const int n = (int)(e - t * 2 * NP), which = n / NP, s = n - which * NP;
-  if (s >= p.N) return;
-  const int64_t b = bg / p.G, g = bg - b * p.G;
-  st_from_float<T>(which ? p.gc : p.gb, ((b * p.T + t) * p.G + g) * p.N + s, v);
+  const float4* src = reinterpret_cast<const float4*>(p.part_bc) + bg * blocks * per + e;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = 0; k < blocks; ++k) {
+    const float4 w = src[k * per];
+    v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
+  }
+  const int64_t t = e / (NP / 2);
+  const int n = 4 * (int)(e - t * (NP / 2)), which = n / NP, s = n - which * NP;
+  const int64_t b = bg / p.G, g = bg - b * p.G, to = ((b * p.T + t) * p.G + g) * p.N + s;
+  void* out = which ? p.gc : p.gb;
+  if (s < p.N) st_from_float<T>(out, to, v.x);
+  if (s + 1 < p.N) st_from_float<T>(out, to + 1, v.y);
+  if (s + 2 < p.N) st_from_float<T>(out, to + 2, v.z);
+  if (s + 3 < p.N) st_from_float<T>(out, to + 3, v.w);
 }
-// rows of partial sums [rows][pitch] (row r at r row_pitch) -> out: [n / NP][N] of [n / NP][NP]
-__global__ void __launch_bounds__(ROWS_THREADS) ttt_selective_rows_kernel(const float* partials, int64_t rows, int64_t row_pitch, int64_t n, int NP, int N,
-                                                                          float* out) {
-  int64_t col;
+// The blocks' rows of sums -> gradients of A (of [C][NP], the first blocks), D and the bias (of [C] each, blocks_c blocks)
+__global__ void __launch_bounds__(ROWS_THREADS) ttt_selective_rows_kernel(const SelParams p, int64_t rows, int NP, int64_t blocks_a, int64_t blocks_c) {
+  int64_t col, block = blockIdx.x;
   float v;
-  if (!sum_of_rows(partials, rows, row_pitch, n, blockIdx.x, &col, &v)) return;
-  const int64_t c = col / NP;
-  const int s = (int)(col - c * NP);
-  if (s < N) out[c * N + s] = v;
+  if (block < blocks_a) {
+    const int64_t n = (int64_t)p.C * NP;
+    if (!sum_of_rows(p.part_a, rows, n, n, block, &col, &v)) return;
+    const int64_t c = col / NP;
+    const int s = (int)(col - c * NP);
+    if (s < p.N) p.ga[c * p.N + s] = v;
+    return;
+  }
+  block -= blocks_a;
+  const bool second = block >= blocks_c;
+  float* out = second ? p.gbias : p.gd;
+  if (out == nullptr) return;  // (the whole block)
+  if (sum_of_rows(p.part_d + (second ? p.C : 0), rows, 2 * (int64_t)p.C, p.C, second ? block - blocks_c : block, &col, &v)) out[col] = v;
 }
 
 template <typename K>
@@ -495,18 +509,12 @@ static cudaError_t run_all(const SelParams& p, cudaStream_t st) {
   if ((e = run(marks ? ttt_selective_bwd_kernel<T, NP, true> : ttt_selective_bwd_kernel<T, NP, false>, sizeof(SelBwdSmem<T, NP>), blocks * p.nseg,
                2 * SEL_THREADS, p, st)) != cudaSuccess)
     return e;
-  ttt_selective_bc_kernel<T><<<(unsigned)((p.B * p.G * p.T * 2 * NP + 255) / 256), 256, 0, st>>>(p, NP, channel_blocks);
+  ttt_selective_bc_kernel<T><<<(unsigned)((p.B * p.G * p.T * NP / 2 + 255) / 256), 256, 0, st>>>(p, NP, channel_blocks);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int64_t n = (int64_t)p.C * NP;
-  ttt_selective_rows_kernel<<<(unsigned)((n + 31) / 32), ROWS_THREADS, 0, st>>>(p.part_a, rows, n, n, NP, p.N, p.ga);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  for (int m = 0; m < 2; ++m) {
-    float* out = m ? p.gbias : p.gd;
-    if (out == nullptr) continue;
-    ttt_selective_rows_kernel<<<(p.C + 31) / 32, ROWS_THREADS, 0, st>>>(p.part_d + m * p.C, rows, 2 * (int64_t)p.C, p.C, 1, 1, out);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  }
-  return cudaSuccess;
+  const int64_t blocks_a = ((int64_t)p.C * NP + 31) / 32, blocks_c = (p.C + 31) / 32;
+  ttt_selective_rows_kernel<<<(unsigned)(blocks_a + (p.gd != nullptr || p.gbias != nullptr ? 2 * blocks_c : 0)), ROWS_THREADS, 0, st>>>(p, rows, NP, blocks_a,
+                                                                                                                                blocks_c);
+  return cudaGetLastError();
 }
 template <typename T>
 static cudaError_t run_np(const SelParams& p, cudaStream_t st) {

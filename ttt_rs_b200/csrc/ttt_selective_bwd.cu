@@ -9,7 +9,7 @@
 // other warps through shared memory; the blocks' shares of dB, dC, dA, dD and the bias's gradient go to the workspace and are joined in
 // a fixed order.  Segments: as in the forward, from the last token on.
 //
-// bf16, 16 x 2048 tokens of 1536 channels, 16 states: 1205 us (+ 22 us for dB and dC over the 24 blocks of channels), from 2349 us with
+// bf16, 16 x 2048 tokens of 1536 channels, 16 states: 1198 us (+ 22 us for dB and dC over the 24 blocks of channels), from 2349 us with
 // all warps doing everything.  Whole tiles at once, twice the code: 1647 us, a quarter of the stalls instruction fetches; halves, which
 // walk the first half's states once more: 1345 us.  Steps and gradients once instead of twice in shared memory, 12 of 50 wavefronts per
 // token: 1329 -> 1243 us.  Registers for three blocks per SM (no decays kept): 1196 us for these 384 blocks, but 399 us instead of 343

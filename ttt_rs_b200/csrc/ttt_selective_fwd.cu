@@ -4,9 +4,9 @@
 // the card: every segment's own state first (from zero, with the sum of its steps, since exp(A sum d) is its whole decay), which the
 // scan's blocks join along the sequence before they begin.  For training the states before every SEL_TILE tokens are kept.
 //
-// bf16, 16 x 2048 tokens of 1536 channels, 16 states: 396 us with the states kept (all eight warps doing everything: 519 us; a quotient
+// bf16, 16 x 2048 tokens of 1536 channels, 16 states: 390 us with the states kept (all eight warps doing everything: 519 us; a quotient
 // in the step's logarithm and range handling in the exponentials: 424 us; shares of y through shuffles: 8 instructions more per token);
-// one sequence of 32768 such tokens: 238 us for the segments' states, 0.8 of what their exponentials allow, and 342 us for the scan.
+// one sequence of 32768 such tokens: 235 us for the segments' states, 0.77 of what their exponentials allow, and 336 us for the scan.
 #include "ttt_selective.cuh"
 
 namespace ttt {

@@ -54,7 +54,8 @@ __device__ __forceinline__ void gradient_behind(F2 (&dh)[SelShape<NP>::CC][2], c
   }
 }
 
-// The launch's 128 registers per thread are shared out: the scanning warps take 176, the others keep 80 (build.py checks the 128).
+// The launch's 128 registers per thread are shared out: the scanning warps take 176, the others keep 80; with MARKS 200 and
+// 56, for 176 spill there (16 x 2048 x 1536, bf16: 1503 us against 1806).  build.py checks the 128.
 // MARKS: there are starts (else the kernel knows none).
 template <typename T, int NP, bool MARKS>
 __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(const SelParams p) {
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
   const int tiles = (int)((at.t_hi - at.t_lo + SEL_TILE - 1) / SEL_TILE);
   if (threadIdx.x < SEL_THREADS) {
     // ---- scan
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MARKS ? 200 : 176));
     const SelLane<NP> me;
     const int my_share = share_at<NP>(me.ch / S::CC, me.sl);
     F2 A[S::CC][2], dh[S::CC][2], dA[S::CC][2];
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
     return;
   }
   // ---- what is done once per token and channel, pair of channels by pair
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MARKS ? 56 : 80));
   const int tid = threadIdx.x - SEL_THREADS, pr = tid % S::PAIRS, row0 = tid / S::PAIRS, pair_have = at.have - 2 * pr;
   bool first[2] = {false, false};  // lane r of a warp: a start at token r of the next tile to be made ready, and of the one behind it
   auto fetch = [&](int i) {
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
   float2 s0 = make_float2(0.f, 0.f), s1 = make_float2(0.f, 0.f);  // of dD and of the bias's gradient
   auto make_ready = [&](int i) {
     const int k = i % SEL_STAGES, left = (int)(at.t_hi - at.t_lo) - (tiles - 1 - i) * SEL_TILE;
-#pragma unroll
+#pragma unroll(MARKS ? 2 : SEL_TILE)
     for (int r = row0; r < SEL_TILE; r += S::ROWS) {
       F2 d = f2add(pair_of(&sm.raw[k][0][r][2 * pr]), bias), gv = pair_of(&sm.raw[k][1][r][2 * pr]);
       if (p.softplus) d = softplus_of(d);
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
     const int64_t t0 = at.t_lo + (int64_t)(tiles - 1 - i) * SEL_TILE + base;
     const int left = (int)min((int64_t)SEL_HALF, at.t_hi - t0);
     if (pair_have > 0) {
-#pragma unroll
+#pragma unroll(MARKS ? 2 : SEL_HALF)
       for (int r = row0; r < SEL_HALF; r += S::ROWS) {
         if (r >= left) break;
         const F2 xv = pair_of(&sm.raw[k][3][base + r][2 * pr]), gv = *reinterpret_cast<const float2*>(&sm.g[i & 1][base + r][2 * pr]);

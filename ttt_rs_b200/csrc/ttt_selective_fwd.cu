@@ -313,8 +313,13 @@ SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd) {
   // us, 16 states: 1 x 32768 x 1536: 18 segments 580, 12 623, 24 615, 36 574; backward 24 1373, 12 1439, 32 1517.  2 x 4096 x 1536: 9
   // segments 161, 6 169, 12 179; backward 12 392, 6 396, 8 441.  4 x 2048 x 2048: 3 segments 201, 1 229, 4 220; backward 9 to 12
   // 500, 1 550, 4 523.  1 x 512 x 512: 16 segments 21, 8 27; backward 16 46, 8 62.  (64 states, 2 x 2048 x 1024: backward 1 611, 8 654.)
-  int64_t wanted = 444 / blocks;
-  if (bwd) wanted = blocks < 100 ? 592 / blocks : blocks <= 148 && NP < 64 ? 1184 / blocks : 1;
+  // Between one block per SM and four thirds of that, three segments both ways: the second round would leave most SMs idle, and two
+  // segments do not mend that.  192 blocks, 1 / 2 / 3 segments: 8 x 2048 x 1536 float32 forward 322 / 387 / 322, backward 1103 / 1010 /
+  // 899; 4 states, 16 x 2048 x 1536 bf16 360 / 440 / 336 and 1280 / 1130 / 1003; 64 states, 2 x 2048 x 1536 backward 1145 / 1018 / 911.
+  // 224 blocks: 285 / 375 / 338 and 795 / 936 / 844.
+  const bool thirds = blocks > 148 && blocks <= 197;
+  int64_t wanted = thirds ? 3 : blocks > 197 ? 1 : 444 / blocks;
+  if (bwd && !thirds) wanted = blocks < 100 ? 592 / blocks : blocks <= 148 && NP < 64 ? 1184 / blocks : 1;
   int64_t most = tiles / 4 > 32 ? tiles / 4 : 32;
   if (most > tiles / 2) most = tiles / 2;
   if (wanted > most) wanted = most;

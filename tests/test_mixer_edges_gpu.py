@@ -1,0 +1,30 @@
+"""Edges of the selective layer's operators: an epsilon of zero."""
+
+import pytest
+import torch
+
+import ttt_rs_b200 as tb
+from mixer_checks import ELEMENT, SUM, close, grads, leaves
+from oracle import mixer_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("gated", [False, True], ids=["plain", "gated"])
+@pytest.mark.parametrize("over", ["token", "sequence"])
+@pytest.mark.parametrize("case", [(3, 29, 4, 16), (1, 5, 2, 33), (2, 7, 3, 6), (1, 3, 2, 520)], ids=str)
+def test_an_epsilon_of_zero(case, over, gated, dtype):
+    """Blocks whose last rows hold no token: 1 / sqrt(0 + 0) of nothing must not reach the sums for weight and bias."""
+    B, T, G, c = case
+    g = torch.Generator().manual_seed(T + c)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    C = G * c
+    ins = [r(B, T, C).to(dtype), (1 + 0.2 * r(C)).to(dtype), (0.3 * r(C)).to(dtype), r(B, T, C).to(dtype) if gated else None]
+    up = r(B, T, C).to(dtype)
+    dev, ref = leaves(ins)
+    call = lambda f, t: f(t[0], G, t[1], t[2], gate=t[3], activation="silu", eps=0.0, over=over)  # noqa: E731
+    y, want = call(tb.group_norm, dev), call(O.group_norm, ref)
+    close(y, want, "y")
+    for a, b, n in zip(grads(y, dev, up.cuda()), grads(want, ref, up.double()), ("x", "weight", "bias", "gate")):
+        close(a, b, n, SUM if n in ("weight", "bias") else 4 * ELEMENT)

@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(WIDE ? NORM_WIDE : NORM_THREADS, WIDE ? 1 : NO
       F2 d[NV][P];
 #pragma unroll
       for (int n = 0; n < NV; ++n) in[u][n].unpack(d[n]);
-      const float r = norm_stats<T, V, WIDE>(d, me, p, sum);
+      const float stat = norm_stats<T, V, WIDE>(d, me, p, sum), r = has[u] ? stat : 0.f;  // (no token: 1 / sqrt(0 + eps) may be infinite)
       F2 q[NV][P], s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
       for (int n = 0; n < NV; ++n) {

@@ -1,4 +1,4 @@
-"""Edges of the selective layer's operators: an epsilon of zero."""
+"""Edges of the selective layer's operators: an epsilon of zero, rates of -inf."""
 
 import pytest
 import torch
@@ -28,3 +28,28 @@ def test_an_epsilon_of_zero(case, over, gated, dtype):
     close(y, want, "y")
     for a, b, n in zip(grads(y, dev, up.cuda()), grads(want, ref, up.double()), ("x", "weight", "bias", "gate")):
         close(a, b, n, SUM if n in ("weight", "bias") else 4 * ELEMENT)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("N", [16, 10])
+@pytest.mark.parametrize("T", [1, 16, 21, 700])
+def test_a_step_of_zero_keeps_a_state_at_any_rate(T, N, dtype):
+    """A rate of -inf keeps nothing over a step above zero and everything over a step of zero, as its limit, the lowest rate, does:
+    in single tokens, in short calls and in long ones."""
+    g = torch.Generator().manual_seed(T + N)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    B, C = 2, 24
+    x, dt = (0.5 * r(B, T, C)).to(dtype), (0.5 * r(B, T, C)).to(dtype)
+    dt[0, :, :8] = -200.0  # (a step of zero in float32)
+    dt[1, T // 2:, 4:] = float("-inf")
+    A = -torch.exp(0.7 * r(C, N))
+    A[:, 3] = float("-inf")
+    Bm, Cm, bias, state = r(B, T, 1, N).to(dtype), r(B, T, 1, N).to(dtype), 0.5 * r(C) - 1.0, r(B, C, N)
+    lowest = A.double().clamp(min=torch.finfo(torch.float32).min)
+    want = O.selective_scan(x.double(), dt.double(), lowest, Bm.double(), Cm.double(), None, None, bias.double(), state.double())
+    t = [v.cuda() for v in (x, dt, A, Bm, Cm)]
+    for recorded in (False, True):  # (recorded for gradients, few tokens are scanned as many are)
+        t[0].requires_grad_(recorded)
+        y, s = tb.selective_scan(*t, dt_bias=bias.cuda(), state=state.cuda())
+        close(y, want[0], "y", 2 * ELEMENT)
+        close(s, want[1], "state", 2 * ELEMENT)

@@ -62,6 +62,10 @@ __device__ __forceinline__ F2 sum_shares(const float* row, int pr) {
 __device__ __forceinline__ F2 decay_of(F2 A, F2 d) { return ex2(f2fma(A, d, f2(2.2e-8f))); }
 __device__ __forceinline__ F2 decay_of(F2 A, float d) { return decay_of(A, f2(d)); }
 
+// A rate times log2 e; one of -inf as the lowest number, so that a step of zero keeps what there is (the limit of ever lower rates, and what
+// the places behind the last token rely on) where 0 times -inf would be a NaN
+__device__ __forceinline__ float rate_of(float a) { return a * LOG2E < -3.4e38f ? -3.4e38f : a * LOG2E; }
+
 // log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in (0, 1].  log(1 + e) / e is a polynomial of degree 8, fitted on [0, 1] for
 // the least largest relative error (3.0e-8): accurate relative to small steps too, which a logarithm of 1 + e is not, and without a
 // quotient, whose place among the exponentials it would take.  Two channels at once; a NaN stays one.
@@ -197,14 +201,13 @@ struct SelLane {
     sl = lane & (S::SL - 1);
     ch = (threadIdx.x >> 5) * S::WARP_CH + (lane / S::SL) * S::CC;
   }
-  // rates, times log2 e; one of -inf as the lowest number, so that a step of zero (behind the last token) keeps what there is
+  // rates, as rate_of gives them
   __device__ __forceinline__ void load_rates(F2 (&A)[S::CC][2], const float* rows, int n, int have) const {
     load(A, rows, n, have);
-    auto scaled = [](float a) { return a * LOG2E < -3.4e38f ? -3.4e38f : a * LOG2E; };
 #pragma unroll
     for (int k = 0; k < S::CC; ++k)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) A[k][i] = f2(scaled(A[k][i].x), scaled(A[k][i].y));
+      for (int i = 0; i < 2; ++i) A[k][i] = f2(rate_of(A[k][i].x), rate_of(A[k][i].y));
   }
   // row of `n` states (N in memory) of channel c0 + ch + k, zeros beyond
   __device__ __forceinline__ void load(F2 (&v)[S::CC][2], const float* rows, int n, int have) const {

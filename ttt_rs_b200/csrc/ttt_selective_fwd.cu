@@ -257,6 +257,8 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_step_kernel(const S
   };
   float a[EACH];
   load(p.A + (int64_t)c * p.N, a);
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) a[k] = rate_of(a[k]);
   const float bias = p.bias != nullptr ? p.bias[c] : 0.f, skip = p.D != nullptr ? p.D[c] : 0.f;
   for (int64_t b = blockIdx.y; b < p.B; b += gridDim.y) {
     float h[EACH];
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(SEL_THREADS) ttt_selective_step_kernel(const S
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < EACH; ++k) {
-        h[k] = fmaf(decay_of(f2(a[k] * LOG2E), d).x, start ? 0.f : h[k], u * bv[k]);
+        h[k] = fmaf(decay_of(f2(a[k]), d).x, start ? 0.f : h[k], u * bv[k]);
         s = fmaf(h[k], cv[k], s);
       }
 #pragma unroll

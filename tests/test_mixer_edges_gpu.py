@@ -1,4 +1,4 @@
-"""Edges of the selective layer's operators: an epsilon of zero, rates of -inf."""
+"""Edges of the selective layer's operators: an epsilon of zero, rates of -inf, steps of zero."""
 
 import pytest
 import torch
@@ -53,3 +53,27 @@ def test_a_step_of_zero_keeps_a_state_at_any_rate(T, N, dtype):
         y, s = tb.selective_scan(*t, dt_bias=bias.cuda(), state=state.cuda())
         close(y, want[0], "y", 2 * ELEMENT)
         close(s, want[1], "state", 2 * ELEMENT)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("N", [16, 10])
+@pytest.mark.parametrize("T", [1, 21, 700])
+def test_gradients_at_steps_of_zero_and_rates_of_minus_infinity(T, N, dtype):
+    """The lowest rate times a state's gradient may be beyond float32, the softplus's slope there is zero: no gradient for the step."""
+    g = torch.Generator().manual_seed(T + N)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    B, C = 2, 24
+    x, dt = (0.5 * r(B, T, C)).to(dtype), (0.5 * r(B, T, C)).to(dtype)
+    dt[0, :, :8] = -200.0
+    dt[1, T // 2:, 4:] = float("-inf")
+    A = -torch.exp(0.7 * r(C, N))
+    A[:, 3] = A[:, 7] = torch.finfo(torch.float32).min
+    ins = [x, dt, A, r(B, T, 1, N).to(dtype), r(B, T, 1, N).to(dtype), None, None, 0.5 * r(C) - 1.0, 8 * r(B, C, N)]
+    dev, ref = leaves(ins)
+    dev[2] = torch.where(ins[2] == ins[2].min(), float("-inf"), ins[2]).cuda().requires_grad_()
+    call = lambda f, t: f(*t[:5], dt_bias=t[7], state=t[8])  # noqa: E731
+    outs, want = call(tb.selective_scan, dev), call(O.selective_scan, ref)
+    up = [r(*w.shape).to(o.dtype) for o, w in zip(outs, want)]
+    got, exp = grads(outs, dev, [8 * u.cuda() for u in up]), grads(want, ref, [8 * u.double() for u in up])
+    for a, b, n in zip(got, exp, ("x", "dt", "A", "B", "C", "dt_bias", "state")):
+        close(a, b, n, SUM)

@@ -470,7 +470,7 @@ int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int64_t channe
  *   strides       of x, dt, z (backward: and grad_y) those of batch and token, then of b and c those of batch, token and group, in
  *                 elements, not negative (null: all contiguous; not read where there is one row, or no z)
  *   a             float32 [channels, states], at most 0 for states that do not grow; -inf keeps nothing of a state, but a step of zero
- *                 keeps all of it at any rate; d_skip, dt_bias float32 [channels] or null (zeros)
+ *                 keeps all of it at any rate (rates below -2^100 / log2(e) count as that); d_skip, dt_bias float32 [channels] or null (zeros)
  *   state         float32 [batch, channels, states] before the first token, or null: zeros
  *   starts        uint8 [batch, seq_len] or null: nonzero: the token finds a state of zero
  *   y             T [batch, seq_len, channels] (out);  state_out  float32 like state (out; it may be state).  Results lie over no other

@@ -293,8 +293,7 @@ __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(c
         F2 dd = f2fma(sum_shares<NP>(sm.res[k2][1][r], pr), f2(LN2), f2mul(in, xv));
         if (p.softplus) {
           const F2 v = f2add(pair_of(&sm.raw[k][0][base + r][2 * pr]), bias);
-          const F2 slope = f2(sigmoid_of(v.x), sigmoid_of(v.y));  // (0: a step of zero, whose rates' products may be beyond float32)
-          dd = f2(slope.x == 0.f ? 0.f : dd.x * slope.x, slope.y == 0.f ? 0.f : dd.y * slope.y);
+          dd = f2mul(dd, f2(sigmoid_of(v.x), sigmoid_of(v.y)));
         }
         put_pair<T>(static_cast<T*>(p.gdt) + row, dd, pair_have, whole);
         s0 = f2fma(gv, xv, s0);

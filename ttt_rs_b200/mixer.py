@@ -114,7 +114,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     gate) [B,T,C], float32 or bfloat16, and B, C [B,T,G,N] or [B,T,N] (one group) of the same type, shared by the C / G neighbouring
     channels of a group: strides that are not negative, with contiguous channels and states (columns of a projection are read where they
     lie).  A [C,N], 1 to 64 states per channel, at most 0 for states that do not grow (-inf keeps nothing of a state, but a step
-    of zero keeps all of it at any rate); D, dt_bias [C] (None: zeros); state [B,C,N], the
+    of zero keeps all of it at any rate; rates below -2^100 / log2(e) count as that); D, dt_bias [C] (None: zeros); state [B,C,N], the
     state before the first token (None: zeros): float32.  softplus=False: d_t = dt_t + dt_bias.  starts [B,T] (bool or uint8): such a token
     finds a state of zero, so that sequences may follow one another in one row, or be padded on the left; nothing before it is seen, not
     even a NaN.  The new state goes to `state_out` where given (it may be `state` itself but share nothing with another tensor; not

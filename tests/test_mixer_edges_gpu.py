@@ -1,4 +1,4 @@
-"""Edges of the selective layer's operators: an epsilon of zero, rates of -inf, steps of zero."""
+"""Edges of the selective layer's operators: an epsilon of zero, rates of -inf, steps of zero, GELU of large numbers."""
 
 import pytest
 import torch
@@ -77,3 +77,26 @@ def test_gradients_at_steps_of_zero_and_rates_of_minus_infinity(T, N, dtype):
     got, exp = grads(outs, dev, [8 * u.cuda() for u in up]), grads(want, ref, [8 * u.double() for u in up])
     for a, b, n in zip(got, exp, ("x", "dt", "A", "B", "C", "dt_bias", "state")):
         close(a, b, n, SUM)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("size", [1e10, 1e20, 3e38])
+@pytest.mark.parametrize("over", ["token", "sequence"])
+def test_gelu_of_large_numbers(over, size, dtype):
+    """GELU's slope is 1 and 0 far from zero, also where the cube, or the square, of its argument is beyond float32."""
+    g = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    B, T, G, C = 2, 9, 2, 32
+    ends = torch.where(torch.arange(C) % 3 == 0, size, torch.where(torch.arange(C) % 3 == 1, -size, 0.5))
+    x, up = r(B, T, C).to(dtype), r(B, T, C).to(dtype)
+    # as the gate: its gradient
+    dev, ref = leaves([x, None, None, ends.expand(B, T, C).contiguous().to(dtype)])
+    call = lambda f, t: f(t[0], G, t[1], t[2], gate=t[3], activation="gelu", eps=1e-3, over=over)  # noqa: E731
+    (got,) = torch.autograd.grad(call(tb.group_norm, dev), dev[3], up.cuda())
+    (exp,) = torch.autograd.grad(call(O.group_norm, ref), ref[3], up.double())
+    close(got, exp, "gate")
+    # as the normed and shifted input: the others' gradients
+    dev, ref = leaves([x, (1 + 0.2 * r(C)).to(dtype), ends.to(dtype), None])
+    got, exp = grads(call(tb.group_norm, dev), dev, up.cuda()), grads(call(O.group_norm, ref), ref, up.double())
+    for a, b, n in zip(got, exp, ("x", "weight", "bias")):
+        close(a, b, n, SUM if n != "x" else 4 * ELEMENT)

@@ -95,9 +95,10 @@ __device__ __forceinline__ float act_and_slope(float v, int act, float& slope) {
     return y;
   }
   if (act == ACT_GELU) {
-    const float vv = v * v, u = 0.7978845608028654f * v * fmaf(0.044715f, vv, 1.f);
-    const float s = sigmoid_of(2.f * u), y = v * s;
-    slope = fmaf(2.f * y * (1.f - s), 0.7978845608028654f * fmaf(3.f * 0.044715f, vv, 1.f), s);
+    const float u = 0.7978845608028654f * v * fmaf(0.044715f * v, v, 1.f), s = sigmoid_of(2.f * u), y = v * s;
+    // s + 2 k y (1 - s) (1 + 3 c v v), from the left: where v v is beyond float32, y (1 - s) is 0 and must meet no infinity
+    const float t = y * (1.f - s);
+    slope = fmaf(6.f * 0.044715f * 0.7978845608028654f, t * v * v, fmaf(2.f * 0.7978845608028654f, t, s));
     return y;
   }
   slope = 1.f;

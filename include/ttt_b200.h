@@ -427,17 +427,23 @@ int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads, const void
  *
  * ttt_layer_causal_conv: y_t = act(bias + sum_j weight_j x_{t-taps+1+j}) channel by channel, taps 2 to 4, activation 0 (none) or 1
  *   (SiLU).  weight T [channels, taps]; bias T [channels] or null; state T [batch, taps-1, channels] or null (zeros): the inputs before
- *   the first token; state_out likewise, the last inputs (it may be state, and lies over no other tensor of the call, as y lies over none
- *   of x and state).  starts uint8 [batch, seq_len] or null: a token with a nonzero start, and those behind it, see no input before it.
+ *   the first token; state_out likewise, the last inputs (it may be state).  starts uint8 [batch, seq_len] or null: a token with a nonzero
+ *   start, and those behind it, see no input before it.
  * ttt_layer_causal_conv_backward: `strides` of x, grad_y; grad_state_out, grad_state T [batch, taps-1, channels] or null; grad_weight,
- *   grad_bias T or null, summed in float32 in a fixed order; with either, the workspace (16-byte aligned).
+ *   grad_bias T or null, summed in float32 in a fixed order; with either, the workspace (16-byte aligned).  grad_state may be state,
+ *   grad_weight weight, grad_bias bias.
  *
  * ttt_layer_group_norm: `groups` groups of neighbouring channels; over 0: of every token (up to 4096 channels per group), 1: of every
  *   sequence (batch row).  u = (x - mean) / sqrt(var + epsilon) * weight + bias; y = act(u) without a gate, u * act(gate) with one;
  *   activation 0, 1 or 2 (GELU, tanh form).  `strides` of x, gate.  weight, bias T [channels] or null (ones, zeros).  stats float32
- *   [batch, groups, 2] (out, over 1 only): for the backward, or null.  Variances come from differences, also across blocks.
+ *   [batch, groups, 2] (out, over 1 only): for the backward, or null.  Variances come from differences, also across blocks.  y may be x or
+ *   gate where that is contiguous.  Over 1, batch*channels < 2^34.
  * ttt_layer_group_norm_backward: `strides` of x, gate, grad_y; grad_gate exactly with a gate; grad_weight, grad_bias T or null, summed in
- *   float32 in a fixed order; workspace where one of them is given, and always over 1.
+ *   float32 in a fixed order; workspace where one of them is given, and always over 1.  grad_x and grad_gate may be x, gate or grad_y
+ *   where that is contiguous, grad_weight weight, grad_bias bias.
+ *
+ * Otherwise results (states, stats and workspaces among them) that share a byte with one another or with another tensor of the call, from
+ * its first byte to its last, are refused (TTT_ERR_SHAPE).
  */
 enum ttt_over { TTT_OVER_TOKEN = 0, TTT_OVER_SEQUENCE = 1 };
 int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t channels, int taps, int dtype, int activation, const void* x,
@@ -473,17 +479,18 @@ int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int64_t channe
  *                 keeps all of it at any rate (rates below -2^100 / log2(e) count as that); d_skip, dt_bias float32 [channels] or null (zeros)
  *   state         float32 [batch, channels, states] before the first token, or null: zeros
  *   starts        uint8 [batch, seq_len] or null: nonzero: the token finds a state of zero
- *   y             T [batch, seq_len, channels] (out);  state_out  float32 like state (out; it may be state).  Results lie over no other
- *                 tensor of the call.
+ *   y             T [batch, seq_len, channels] (out);  state_out  float32 like state (out; it may be state).  Results (saved and the
+ *                 workspace among them) that share a byte with one another or with another tensor of the call are refused.
  *   saved         (out) ttt_linear_selective_saved_bytes bytes for the backward: the states before every 16 tokens, opaque; null for
  *                 inference (1 to 16 tokens then are a decode step: one launch, no workspace)
  *   workspace     ..._forward_workspace_bytes / ..._backward_workspace_bytes, 16-byte aligned; the forward's may be 0 (null then)
- * states 1..64; batch*seq_len, batch*channels < 2^31.  a, state, state_out and their gradients on 16 bytes; all others at any multiple
+ * states 1..64; batch*seq_len, batch*channels < 2^31, batch*seq_len*groups < 2^32.  a, state, state_out and their gradients on 16 bytes; all others at any multiple
  * of an element.  Steps, decays, states and sums are float32; no result depends on the order in which blocks run.
  *
  * ttt_linear_selective_backward: gradients for loss = <grad_y, y> + <grad_state_out, state_out> (grad_state_out null: zero).  grad_x,
  * grad_dt, grad_z (exactly with z) T, contiguous; grad_b, grad_c T [batch, seq_len, groups, states]; grad_a, grad_d, grad_dt_bias,
- * grad_state float32, the last three or null.
+ * grad_state float32, the last three or null.  grad_x, grad_dt and grad_z may be x, dt, z or grad_y, grad_b and grad_c b or c, where those
+ * are contiguous, grad_a a, grad_d d_skip, grad_dt_bias dt_bias; results that lie over a tensor of the call otherwise are refused.
  */
 size_t ttt_linear_selective_saved_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states, int dtype);
 size_t ttt_linear_selective_forward_workspace_bytes(int64_t batch, int64_t seq_len, int64_t channels, int groups, int states,

@@ -2,6 +2,7 @@
 // Argument checks and launches.
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 
 #include "../../include/ttt_b200.h"
 #include "ttt_kernels.h"
@@ -25,6 +26,7 @@ int launched(cudaError_t e, const char* what) {
 }
 
 constexpr int64_t kMostChannels = 1 << 20;
+constexpr int64_t kFarthest = (int64_t)1 << 58;  // elements that one stride reaches: three of them are still an int64 of bytes
 
 int check_sizes(int64_t B, int64_t T, int64_t C, int dtype) {
   if (B <= 0 || T <= 0 || C <= 0) return fail(TTT_ERR_SHAPE, "batch, seq_len and channels must be positive");
@@ -65,16 +67,35 @@ struct Spans {
       out[k] = size[k] == 1 ? 0 : strides != nullptr ? strides[2 * i + k] : dense[k];
       low |= (uintptr_t)(out[k] * es);
       if (rc == TTT_OK && out[k] < 0) rc = fail(TTT_ERR_SHAPE, "the strides of %s must not be negative", name);
-      if (rc == TTT_OK && out[k] > ((int64_t)1 << 60) / size[k]) rc = fail(TTT_ERR_SHAPE, "the strides of %s are out of range", name);
+      if (rc == TTT_OK && out[k] > kFarthest / size[k]) rc = fail(TTT_ERR_SHAPE, "the strides of %s are out of range", name);
     }
   }
   int64_t bytes(const int64_t (&s)[2]) const { return ((B - 1) * s[0] + (T - 1) * s[1] + C) * es; }
+  bool contiguous(const int64_t (&s)[2]) const { return (B == 1 || s[0] == T * C) && (T == 1 || s[1] == C); }
 };
-// A result (contiguous, `size` bytes) must share nothing with another tensor of the call; `same`: it may be that tensor itself
-int check_apart(const char* name, const void* out, int64_t size, const char* other_name, const void* other, int64_t other_size, bool same) {
-  if (out == nullptr || other == nullptr || (same && out == other && size == other_size)) return TTT_OK;
-  const uintptr_t a = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(other);
-  if (a < b + (uintptr_t)other_size && b < a + (uintptr_t)size) return fail(TTT_ERR_SHAPE, "%s lies over %s", name, other_name);
+// Bytes of a tensor of the call, and its kinds, bit by bit
+struct Region {
+  const char* name;
+  const void* p;
+  int64_t bytes;
+  unsigned kinds;
+};
+// Results (contiguous) share nothing with one another, nor with an input, except that a result may be an input, all of it, of one of its
+// kinds: those are read, by the thread that writes in their place or by an earlier launch, before they are written.
+int check_apart(std::initializer_list<Region> results, std::initializer_list<Region> inputs) {
+  auto meet = [](const Region& a, const Region& b) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    return a.p != nullptr && b.p != nullptr && x < y + (uintptr_t)b.bytes && y < x + (uintptr_t)a.bytes;
+  };
+  for (const Region& r : results) {
+    for (const Region& in : inputs)
+      if (meet(r, in) && !((r.kinds & in.kinds) != 0 && r.p == in.p && r.bytes == in.bytes))
+        return fail(TTT_ERR_SHAPE, "%s lies over %s", r.name, in.name);
+    for (const Region& other : results) {
+      if (&other == &r) break;
+      if (meet(r, other)) return fail(TTT_ERR_SHAPE, "%s lies over %s", r.name, other.name);
+    }
+  }
   return TTT_OK;
 }
 
@@ -111,14 +132,9 @@ extern "C" int ttt_layer_causal_conv(int64_t batch, int64_t seq_len, int64_t cha
   s.align("bias", bias);
   if (s.rc != TTT_OK) return s.rc;
   const int64_t held = batch * (taps - 1) * channels * es, n = batch * seq_len * channels * es;
-  if ((rc = check_apart("state_out", state_out, held, "state", state, held, true)) != TTT_OK ||
-      (rc = check_apart("state_out", state_out, held, "x", x, s.bytes(p.xs), false)) != TTT_OK ||
-      (rc = check_apart("state_out", state_out, held, "y", y, n, false)) != TTT_OK ||
-      (rc = check_apart("state_out", state_out, held, "weight", weight, channels * taps * es, false)) != TTT_OK ||
-      (rc = check_apart("state_out", state_out, held, "bias", bias, channels * es, false)) != TTT_OK ||
-      (rc = check_apart("state_out", state_out, held, "starts", starts, batch * seq_len, false)) != TTT_OK ||
-      (rc = check_apart("y", y, n, "x", x, s.bytes(p.xs), false)) != TTT_OK ||
-      (rc = check_apart("y", y, n, "state", state, held, false)) != TTT_OK)
+  if ((rc = check_apart({{"state_out", state_out, held, 1}, {"y", y, n, 0}},
+                        {{"x", x, s.bytes(p.xs), 0}, {"weight", weight, channels * taps * es, 0}, {"bias", bias, channels * es, 0},
+                         {"state", state, held, 1}, {"starts", starts, batch * seq_len, 0}})) != TTT_OK)
     return rc;
   p.x = x, p.w = weight, p.bias = bias, p.state = state, p.starts = static_cast<const uint8_t*>(starts);
   p.y = y, p.state_out = state_out;
@@ -153,13 +169,19 @@ extern "C" int ttt_layer_causal_conv_backward(int64_t batch, int64_t seq_len, in
   s.align("grad_weight", grad_weight);
   s.align("grad_bias", grad_bias);
   if (s.rc != TTT_OK) return s.rc;
-  const bool sums = grad_weight != nullptr || grad_bias != nullptr;
-  if (sums && (rc = check_bytes(workspace_bytes, ttt_layer_causal_conv_backward_workspace_bytes(batch, seq_len, channels, taps, dtype), workspace,
-                                "workspace")) != TTT_OK)
+  const size_t need =
+      grad_weight != nullptr || grad_bias != nullptr ? ttt_layer_causal_conv_backward_workspace_bytes(batch, seq_len, channels, taps, dtype) : 0;
+  if ((rc = check_bytes(workspace_bytes, need, workspace, "workspace")) != TTT_OK) return rc;
+  const int64_t held = batch * (taps - 1) * channels * es, n = batch * seq_len * channels * es, taps_bytes = channels * taps * es;
+  if ((rc = check_apart({{"grad_x", grad_x, n, 0}, {"grad_state", grad_state, held, 1}, {"grad_weight", grad_weight, taps_bytes, 2},
+                         {"grad_bias", grad_bias, channels * es, 4}, {"workspace", need != 0 ? workspace : nullptr, (int64_t)need, 0}},
+                        {{"x", x, s.bytes(p.xs), 0}, {"grad_y", grad_y, s.bytes(p.gs), 0}, {"weight", weight, taps_bytes, 2},
+                         {"bias", bias, channels * es, 4}, {"state", state, held, 1}, {"starts", starts, batch * seq_len, 0},
+                         {"grad_state_out", grad_state_out, held, 0}})) != TTT_OK)
     return rc;
   p.x = x, p.w = weight, p.bias = bias, p.state = state, p.starts = static_cast<const uint8_t*>(starts);
   p.gy = grad_y, p.gstate_out = grad_state_out, p.gx = grad_x, p.gstate = grad_state, p.gw = grad_weight, p.gbias = grad_bias;
-  p.partials = sums ? static_cast<float*>(workspace) : nullptr;
+  p.partials = need != 0 ? static_cast<float*>(workspace) : nullptr;
   p.B = batch, p.T = seq_len, p.C = (int)channels, p.act = activation;
   return launched(ttt::launch_conv(dtype, p, taps, width, true, static_cast<cudaStream_t>(stream)), "causal convolution backward");
 }
@@ -215,11 +237,17 @@ extern "C" int ttt_layer_group_norm(int64_t batch, int64_t seq_len, int64_t chan
   s.align("bias", bias);
   if (s.rc != TTT_OK) return s.rc;
   if ((reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return fail(TTT_ERR_ALIGN, "stats is not aligned to its elements");
-  if ((rc = check_bytes(workspace_bytes, ttt_layer_group_norm_workspace_bytes(batch, seq_len, channels, groups, over, dtype), workspace,
-                        "workspace")) != TTT_OK)
+  const size_t need = ttt_layer_group_norm_workspace_bytes(batch, seq_len, channels, groups, over, dtype);
+  if ((rc = check_bytes(workspace_bytes, need, workspace, "workspace")) != TTT_OK) return rc;
+  const bool sequence = over == TTT_OVER_SEQUENCE;
+  const int64_t n = batch * seq_len * channels * es, wide = channels * es;
+  if ((rc = check_apart({{"y", y, n, 1}, {"stats", sequence ? stats : nullptr, batch * groups * 8, 0},
+                         {"workspace", need != 0 ? workspace : nullptr, (int64_t)need, 0}},
+                        {{"x", x, s.bytes(p.xs), s.contiguous(p.xs)}, {"gate", gate, s.bytes(p.gates), s.contiguous(p.gates)},
+                         {"weight", weight, wide, 0}, {"bias", bias, wide, 0}})) != TTT_OK)
     return rc;
   p.x = x, p.gate = gate, p.w = weight, p.bias = bias, p.y = y, p.stats = stats, p.moments = static_cast<float*>(workspace);
-  return launched(ttt::launch_norm(dtype, p, norm_width(s.low, p.c, es), over == TTT_OVER_SEQUENCE, false, static_cast<cudaStream_t>(stream)),
+  return launched(ttt::launch_norm(dtype, p, norm_width(s.low, p.c, es), sequence, false, static_cast<cudaStream_t>(stream)),
                   "group norm");
 }
 
@@ -248,13 +276,20 @@ extern "C" int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int
   if (s.rc != TTT_OK) return s.rc;
   if (sequence && stats == nullptr) return fail(TTT_ERR_NULL, "stats is null");
   if ((reinterpret_cast<uintptr_t>(stats) & 3u) != 0) return fail(TTT_ERR_ALIGN, "stats is not aligned to its elements");
-  const bool sums = sequence || grad_weight != nullptr || grad_bias != nullptr;
-  if (sums && (rc = check_bytes(workspace_bytes, ttt_layer_group_norm_backward_workspace_bytes(batch, seq_len, channels, groups, over, dtype),
-                                workspace, "workspace")) != TTT_OK)
+  const size_t need = sequence || grad_weight != nullptr || grad_bias != nullptr
+                          ? ttt_layer_group_norm_backward_workspace_bytes(batch, seq_len, channels, groups, over, dtype)
+                          : 0;
+  if ((rc = check_bytes(workspace_bytes, need, workspace, "workspace")) != TTT_OK) return rc;
+  const int64_t n = batch * seq_len * channels * es, wide = channels * es;
+  if ((rc = check_apart({{"grad_x", grad_x, n, 1}, {"grad_gate", gate != nullptr ? grad_gate : nullptr, n, 1}, {"grad_weight", grad_weight, wide, 2},
+                         {"grad_bias", grad_bias, wide, 4}, {"workspace", need != 0 ? workspace : nullptr, (int64_t)need, 0}},
+                        {{"x", x, s.bytes(p.xs), s.contiguous(p.xs)}, {"gate", gate, s.bytes(p.gates), s.contiguous(p.gates)},
+                         {"grad_y", grad_y, s.bytes(p.gys), s.contiguous(p.gys)}, {"weight", weight, wide, 2}, {"bias", bias, wide, 4},
+                         {"stats", sequence ? stats : nullptr, batch * groups * 8, 0}})) != TTT_OK)
     return rc;
   p.x = x, p.gate = gate, p.gy = grad_y, p.w = weight, p.bias = bias, p.stats = const_cast<float*>(stats);
   p.gx = grad_x, p.ggate = grad_gate, p.gw = grad_weight, p.gb = grad_bias;
-  p.partials = sums ? static_cast<float*>(workspace) : nullptr;
+  p.partials = need != 0 ? static_cast<float*>(workspace) : nullptr;
   return launched(ttt::launch_norm(dtype, p, width, sequence, true, static_cast<cudaStream_t>(stream)), "group norm backward");
 }
 
@@ -324,7 +359,7 @@ int sel_inputs(ttt::SelParams* p, const SelDims& d, const void* x, const void* d
     m.rows(names[k], bases[k], two, 0, rows);
     const int64_t group = d.G == 1 ? 0 : at != nullptr ? at[3 * k + 2] : d.N;
     m.low |= (uintptr_t)(group * d.es);
-    if (m.rc == TTT_OK && (group < 0 || group > (int64_t)1 << 40)) m.rc = fail(TTT_ERR_SHAPE, "the strides of %s are out of range", names[k]);
+    if (m.rc == TTT_OK && (group < 0 || group > kFarthest / d.G)) m.rc = fail(TTT_ERR_SHAPE, "the strides of %s are out of range", names[k]);
     (*out[k])[0] = rows[0], (*out[k])[1] = rows[1], (*out[k])[2] = group;
   }
   const int64_t wide = (int64_t)d.N * d.es;
@@ -345,6 +380,11 @@ int sel_inputs(ttt::SelParams* p, const SelDims& d, const void* x, const void* d
   p->starts = static_cast<const uint8_t*>(starts);
   p->B = d.B, p->T = d.T, p->C = (int)d.C, p->G = d.G, p->N = d.N;
   return TTT_OK;
+}
+// bytes that b or c spans
+int64_t states_bytes(const SelDims& d, const int64_t (&s)[3]) { return ((d.B - 1) * s[0] + (d.T - 1) * s[1] + (d.G - 1) * s[2] + d.N) * d.es; }
+bool states_contiguous(const SelDims& d, const int64_t (&s)[3]) {
+  return (d.B == 1 || s[0] == d.T * d.G * d.N) && (d.T == 1 || s[1] == (int64_t)d.G * d.N) && (d.G == 1 || s[2] == d.N);
 }
 int need16(const char* name, const void* p, bool optional) {
   if (p == nullptr && !optional) return fail(TTT_ERR_NULL, "%s is null", name);
@@ -381,31 +421,22 @@ extern "C" int ttt_linear_selective_forward(int64_t batch, int64_t seq_len, int6
       (rc = sel_inputs(&p, d, x, dt, a, b, c, d_skip, z, dt_bias, state, starts, nullptr, false, strides, y, nullptr, nullptr, nullptr)) != TTT_OK ||
       (rc = need16("state_out", state_out, false)) != TTT_OK)
     return rc;
-  const Spans s{d.B, d.T, d.C, d.es};
-  const Spans m{d.B, d.T, d.N, d.es};
-  const int64_t held = d.B * d.C * d.N * 4, n = d.B * d.T * d.C * d.es;
-  const int64_t bb[2] = {p.bs[0], p.bs[1]}, cb[2] = {p.cs[0], p.cs[1]};
-  const struct {
-    const char* name;
-    const void* p;
-    int64_t bytes;
-  } others[] = {{"x", x, s.bytes(p.xs)}, {"dt", dt, s.bytes(p.ds)}, {"z", z, s.bytes(p.zs)}, {"a", a, d.C * d.N * 4}, {"d", d_skip, d.C * 4},
-                {"dt_bias", dt_bias, d.C * 4}, {"b", b, m.bytes(bb) + p.bs[2] * (d.G - 1) * d.es}, {"c", c, m.bytes(cb) + p.cs[2] * (d.G - 1) * d.es},
-                {"starts", starts, d.B * d.T}};
-  for (const auto& o : others) {
-    if ((rc = check_apart("state_out", state_out, held, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
-    if ((rc = check_apart("y", y, n, o.name, o.p, o.bytes, false)) != TTT_OK) return rc;
-  }
-  if ((rc = check_apart("state_out", state_out, held, "y", y, n, false)) != TTT_OK ||
-      (rc = check_apart("state_out", state_out, held, "state", state, held, true)) != TTT_OK ||
-      (rc = check_apart("y", y, n, "state", state, held, false)) != TTT_OK)
-    return rc;
   p.softplus = softplus != 0;
   p.y = y, p.state_out = state_out;
-  if (saved == nullptr && seq_len <= 16) return launched(ttt::launch_selective_step(dtype, p, static_cast<cudaStream_t>(stream)), "selective step");
-  if (saved != nullptr && (rc = check_bytes(saved_bytes, sizeof(float) * saved_floats(d), saved, "saved")) != TTT_OK) return rc;
+  const bool step = saved == nullptr && seq_len <= 16;
   const ttt::SelCut cut = d.cut(false);
-  if ((rc = check_bytes(workspace_bytes, sizeof(float) * seg_floats(d, cut), workspace, "workspace")) != TTT_OK) return rc;
+  const int64_t need = step ? 0 : 4 * seg_floats(d, cut);
+  if (saved != nullptr && (rc = check_bytes(saved_bytes, sizeof(float) * saved_floats(d), saved, "saved")) != TTT_OK) return rc;
+  if ((rc = check_bytes(workspace_bytes, need, workspace, "workspace")) != TTT_OK) return rc;
+  const Spans s{d.B, d.T, d.C, d.es};
+  const int64_t held = d.B * d.C * d.N * 4;
+  if ((rc = check_apart({{"state_out", state_out, held, 1}, {"y", y, d.B * d.T * d.C * d.es, 0}, {"saved", saved, 4 * saved_floats(d), 0},
+                         {"workspace", need != 0 ? workspace : nullptr, need, 0}},
+                        {{"x", x, s.bytes(p.xs), 0}, {"dt", dt, s.bytes(p.ds), 0}, {"z", z, s.bytes(p.zs), 0}, {"a", a, d.C * d.N * 4, 0},
+                         {"b", b, states_bytes(d, p.bs), 0}, {"c", c, states_bytes(d, p.cs), 0}, {"d", d_skip, d.C * 4, 0},
+                         {"dt_bias", dt_bias, d.C * 4, 0}, {"state", state, held, 1}, {"starts", starts, d.B * d.T, 0}})) != TTT_OK)
+    return rc;
+  if (step) return launched(ttt::launch_selective_step(dtype, p, static_cast<cudaStream_t>(stream)), "selective step");
   p.saved = static_cast<float*>(saved);
   set_segments(&p, d, cut, static_cast<float*>(workspace));
   return launched(ttt::launch_selective(dtype, p, static_cast<cudaStream_t>(stream)), "selective scan");
@@ -440,7 +471,20 @@ extern "C" int ttt_linear_selective_backward(int64_t batch, int64_t seq_len, int
     if (reinterpret_cast<uintptr_t>(q.p) % q.align != 0) return fail(TTT_ERR_ALIGN, "%s is not aligned to its elements", q.name);
   }
   const ttt::SelCut cut = d.cut(true);
-  if ((rc = check_bytes(workspace_bytes, sizeof(float) * backward_floats(d, cut), workspace, "workspace")) != TTT_OK) return rc;
+  const int64_t need = 4 * backward_floats(d, cut);
+  if ((rc = check_bytes(workspace_bytes, need, workspace, "workspace")) != TTT_OK) return rc;
+  const Spans s{d.B, d.T, d.C, d.es};
+  const int64_t n = d.B * d.T * d.C * d.es, held = d.B * d.C * d.N * 4, bc = d.B * d.T * d.G * d.N * d.es, wide = d.C * 4, rates = wide * d.N;
+  if ((rc = check_apart({{"grad_x", grad_x, n, 1}, {"grad_dt", grad_dt, n, 1}, {"grad_z", z != nullptr ? grad_z : nullptr, n, 1}, {"grad_a", grad_a, rates, 2},
+                         {"grad_b", grad_b, bc, 4}, {"grad_c", grad_c, bc, 4}, {"grad_d", grad_d, wide, 8}, {"grad_dt_bias", grad_dt_bias, wide, 16},
+                         {"grad_state", grad_state, held, 0}, {"workspace", workspace, need, 0}},
+                        {{"x", x, s.bytes(p.xs), s.contiguous(p.xs)}, {"dt", dt, s.bytes(p.ds), s.contiguous(p.ds)},
+                         {"z", z, s.bytes(p.zs), s.contiguous(p.zs)}, {"grad_y", grad_y, s.bytes(p.gs), s.contiguous(p.gs)}, {"a", a, rates, 2},
+                         {"b", b, states_bytes(d, p.bs), states_contiguous(d, p.bs) ? 4u : 0u},
+                         {"c", c, states_bytes(d, p.cs), states_contiguous(d, p.cs) ? 4u : 0u}, {"d", d_skip, wide, 8},
+                         {"dt_bias", dt_bias, wide, 16}, {"starts", starts, d.B * d.T, 0}, {"saved", saved, 4 * saved_floats(d), 0},
+                         {"grad_state_out", grad_state_out, held, 0}})) != TTT_OK)
+    return rc;
   float* ws = static_cast<float*>(workspace);
   const int64_t rows = d.B * cut.nseg;
   p.part_bc = ws, ws += d.B * d.G * cut.channel_blocks * d.T * 2 * d.NP;

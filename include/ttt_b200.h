@@ -428,10 +428,11 @@ int ttt_layer_qk_norm_rotary_backward(const ttt_dims* d, int k_heads, const void
  * ttt_layer_causal_conv: y_t = act(bias + sum_j weight_j x_{t-taps+1+j}) channel by channel, taps 2 to 4, activation 0 (none) or 1
  *   (SiLU).  weight T [channels, taps]; bias T [channels] or null; state T [batch, taps-1, channels] or null (zeros): the inputs before
  *   the first token; state_out likewise, the last inputs (it may be state).  starts uint8 [batch, seq_len] or null: a token with a nonzero
- *   start, and those behind it, see no input before it.
+ *   start, and those behind it, see no input before it, whatever it is.
  * ttt_layer_causal_conv_backward: `strides` of x, grad_y; grad_state_out, grad_state T [batch, taps-1, channels] or null; grad_weight,
  *   grad_bias T or null, summed in float32 in a fixed order; with either, the workspace (16-byte aligned).  grad_state may be state,
- *   grad_weight weight, grad_bias bias.
+ *   grad_weight weight, grad_bias bias.  (These two sum over all tokens: an input that is not finite reaches them also where a start hides
+ *   it from the tokens whose results are used, 0 times NaN.)
  *
  * ttt_layer_group_norm: `groups` groups of neighbouring channels; over 0: of every token (up to 4096 channels per group), 1: of every
  *   sequence (batch row).  u = (x - mean) / sqrt(var + epsilon) * weight + bias; y = act(u) without a gate, u * act(gate) with one;
@@ -478,7 +479,8 @@ int ttt_layer_group_norm_backward(int64_t batch, int64_t seq_len, int64_t channe
  *   a             float32 [channels, states], at most 0 for states that do not grow; -inf keeps nothing of a state, but a step of zero
  *                 keeps all of it at any rate (rates below -2^100 / log2(e) count as that); d_skip, dt_bias float32 [channels] or null (zeros)
  *   state         float32 [batch, channels, states] before the first token, or null: zeros
- *   starts        uint8 [batch, seq_len] or null: nonzero: the token finds a state of zero
+ *   starts        uint8 [batch, seq_len] or null: nonzero: the token finds a state of zero, whatever came before (gradients that sum over
+ *                 tokens, of a, d_skip and dt_bias, and over channels, of b and c, still have all terms: 0 times NaN is one of them)
  *   y             T [batch, seq_len, channels] (out);  state_out  float32 like state (out; it may be state).  Results (saved and the
  *                 workspace among them) that share a byte with one another or with another tensor of the call are refused.
  *   saved         (out) ttt_linear_selective_saved_bytes bytes for the backward: the states before every 16 tokens, opaque; null for

@@ -5,13 +5,15 @@
 // is the last K - 1 inputs, as they are visible behind the last token.  With g_t = dy_t act'(v_t):
 //   dx_s = sum_j w_j g_{s+K-1-j} over the tokens that saw s (+ the new state's gradient),  dw_j = sum_t g_t x_{t-K+1+j},  db = sum_t g_t
 //
-// Memory-bound by its bytes, held back by instructions and latency.  A thread holds four neighbouring channels (two of bf16, or one,
+// Memory-bound by its bytes, held back by latency with few warps and by instructions.  A thread holds four neighbouring channels (two of bf16, or one,
 // where rows are off a vector's address) and walks a strip of tokens with the last K - 1 inputs in registers and the next few tokens on their way; the
 // tokens before a strip (and behind it, for dx) are read again, from L2.  Whole groups of tokens inside a strip go without checks.  A
 // start empties the registers of the inputs, and the sums of dx know the last start's place; without starts, kernels know of none.
 // bf16, 65536 tokens of 1536 channels, 4 taps, SiLU: 94 us forward (4.3 TB/s, 0.65 of a copy), 167 us backward (3.6 TB/s, 0.55).  Eight
 // channels per thread took so many registers that a quarter of the threads fitted: 208 us forward.  Strips of 64 tokens: 115 us for 100
-// at that stage; without the next tokens on their way 230 us for 207 backward; with checks at every token 207 us for 168.
+// at that stage; without the next tokens on their way 230 us for 207 backward; with checks at every token 207 us for 168.  15 of 64 warps
+// are active, 46 and 53 % of issue slots used; of the 128 registers that two backward blocks leave a thread, 4 taps of bf16 spill: 184 bytes
+// written and 268 read per thread with SiLU (104 / 100 without, 202 / 332 with starts; float32 36 to 84 / 80 to 156; 3 taps 16 / 32).
 #include <type_traits>
 
 #include "ttt_kernels.h"

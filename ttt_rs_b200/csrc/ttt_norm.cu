@@ -8,7 +8,9 @@
 //
 // Memory-bound.
 //   A token's groups: eight channels per thread, a group to a power of two of lanes (several warps where it has more than 256
-//   channels), everything in registers between one read and one write.  A thread keeps its channels from token to token, so that
+//   channels), everything in registers between one read and one write, but for what spills: nothing in the gradient of bf16 vectors with
+//   SiLU, 80 bytes per thread with another activation, 84 of float32 vectors, 128 of float32 pairs, 496 (bf16) and 708 (float32) channel by
+//   channel, whose eight places per thread have a weight, a bias and two sums each.  A thread keeps its channels from token to token, so that
 //   weights and their gradients stay in registers; the backward's blocks leave a row of sums each, joined in a fixed order.  bf16, 65536
 //   tokens of 24 heads of 64 channels with gate: 117 us (5.2 TB/s, 0.79 of a copy), gradient 212 us (4.7 TB/s, 0.72; with two tokens at a
 //   time, which two instead of three blocks per SM have room for, 250 us); SiLU known when the kernel is built: 151 and 455 us before that.

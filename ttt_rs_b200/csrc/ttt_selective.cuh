@@ -6,8 +6,8 @@
 //
 // What bounds it from below is exponentials: one per state, channel and token, 16 per SM and clock, where memory would allow twice as
 // many at N = 16 (16 x 2048 tokens of 1536 channels, 8.05e8 states: 179 us, 224 us with those of steps and gates; 1115 MB of a training
-// step 170 us).  What bounds it now is all of issue slots, exponentials and shared-memory reads together: 76 instructions per token and
-// 16 channels forward (58 % of issue slots, 58 % of exponentials on average, a sixth more on SMs with three blocks of 2.6), 213
+// step 170 us).  What bounds it now is all of issue slots, exponentials and shared-memory reads together: 73 instructions per token and
+// 16 channels forward (57 % of issue slots, 60 % of exponentials on average, a sixth more on SMs with three blocks of 2.6), 214
 // backward.  A thread holds SEL_EACH states of two neighbouring channels (of one where N <= 8); NP / SEL_EACH lanes share a channel.
 // Four warps of a block scan; four others (SEL_THREADS each) do what is done once per token and channel: they copy tiles of SEL_TILE
 // tokens ahead (cp.async), turn them into (step, step times x) pairs in float32 in shared memory a tile before the scan, and write the

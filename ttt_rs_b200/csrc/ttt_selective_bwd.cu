@@ -55,7 +55,8 @@ __device__ __forceinline__ void gradient_behind(F2 (&dh)[SelShape<NP>::CC][2], c
 }
 
 // The launch's 128 registers per thread are shared out: the scanning warps take 176, the others keep 80; with MARKS 200 and
-// 56, for 176 spill there (16 x 2048 x 1536, bf16: 1503 us against 1806).  build.py checks the 128.
+// 56, for 176 spill there (16 x 2048 x 1536, bf16: 1503 us against 1806; without starts 32 and 64 states spill 64 and 32 bytes).
+// build.py checks the 128.
 // MARKS: there are starts (else the kernel knows none).
 template <typename T, int NP, bool MARKS>
 __global__ void __launch_bounds__(2 * SEL_THREADS, 2) ttt_selective_bwd_kernel(const SelParams p) {

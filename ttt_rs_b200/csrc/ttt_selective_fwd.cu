@@ -1,7 +1,8 @@
 // Selective state space scan, forward and decode step (definitions: ttt_selective.cuh).
 //
-// A block of four warps owns 64 channels (N = 16) of a sequence, or of a segment of it.  Segments, where channels are too few to fill
-// the card: every segment's own state first (from zero, with the sum of its steps, since exp(A sum d) is its whole decay), which the
+// A block of eight warps owns 64 channels (N = 16) of one group of a sequence, or of a segment of it; where a group has fewer, the other
+// lanes walk zeros (65536 tokens of 8 groups, 16 states, bf16: 6 channels each 468 us, 64 each 402; training 1531 and 1353).  Segments,
+// where channels are too few to fill the card: every segment's own state first (from zero, with the sum of its steps, since exp(A sum d) is its whole decay), which the
 // scan's blocks join along the sequence before they begin.  For training the states before every SEL_TILE tokens are kept.
 //
 // bf16, 16 x 2048 tokens of 1536 channels, 16 states: 390 us with the states kept (all eight warps doing everything: 519 us; a quotient
@@ -309,16 +310,20 @@ SelCut sel_cut(int64_t B, int64_t T, int C, int G, int N, bool bwd) {
   SelCut k{};
   k.channel_blocks = (each + CH - 1) / CH;
   const int64_t blocks = B * G * k.channel_blocks, tiles = (T + SEL_TILE - 1) / SEL_TILE;
-  // Forward: as many segments as blocks are resident (three per SM).  Backward: two rounds of those resident (two per SM), which shares
-  // the last round out; four where a block per SM leaves little idle anyway, and none there with 64 states, whose gradients
-  // carried back cost more.  Segments of two tiles at least, of four beyond 32 of them: a block joins all that are before it.
+  // Forward: three blocks per SM in all.  Backward: four, which shares the last round of those resident out; eight where a block per SM
+  // leaves little idle anyway, and none there with 64 states, whose gradients carried back cost more.  Segments of two tiles at least, of
+  // four beyond 32 of them: a block joins all that are before it.  The rule does not ask how many blocks are resident.  By their shared
+  // memory that is, forward, three per SM in bf16 with more than 4 states and in float32 with 5 to 8, two in bf16 with up to 4 and in float32
+  // with more than 8, one in float32 with up to 4; backward two with 5 to 8 states and in bf16 with 9 to 32, one otherwise.  Where it is
+  // fewer than three and two, the segments run in more rounds than the sweeps below, of 16 states in bf16, were made for.
   // us, 16 states: 1 x 32768 x 1536: 18 segments 580, 12 623, 24 615, 36 574; backward 24 1373, 12 1439, 32 1517.  2 x 4096 x 1536: 9
   // segments 161, 6 169, 12 179; backward 12 392, 6 396, 8 441.  4 x 2048 x 2048: 3 segments 201, 1 229, 4 220; backward 9 to 12
   // 500, 1 550, 4 523.  1 x 512 x 512: 16 segments 21, 8 27; backward 16 46, 8 62.  (64 states, 2 x 2048 x 1024: backward 1 611, 8 654.)
   // Between one block per SM and four thirds of that, three segments both ways: the second round would leave most SMs idle, and two
   // segments do not mend that.  192 blocks, 1 / 2 / 3 segments: 8 x 2048 x 1536 float32 forward 322 / 387 / 322, backward 1103 / 1010 /
   // 899; 4 states, 16 x 2048 x 1536 bf16 360 / 440 / 336 and 1280 / 1130 / 1003; 64 states, 2 x 2048 x 1536 backward 1145 / 1018 / 911.
-  // 224 blocks: 285 / 375 / 338 and 795 / 936 / 844.
+  // 224 blocks: 285 / 375 / 338 and 795 / 936 / 844.  Not the best there throughout: 160 blocks of 16 states in bf16, three segments 287 and
+  // 666, eight 241 and 593.
   const bool thirds = blocks > 148 && blocks <= 197;
   int64_t wanted = thirds ? 3 : blocks > 197 ? 1 : 444 / blocks;
   if (bwd && !thirds) wanted = blocks < 100 ? 592 / blocks : blocks <= 148 && NP < 64 ? 1184 / blocks : 1;

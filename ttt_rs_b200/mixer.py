@@ -74,7 +74,8 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     tokens, single ones included.  x [B,T,C] (float32 or bfloat16; any strides that are not negative, with contiguous channels: columns
     of a projection are read where they lie), weight [C,K] with 2 to 4 taps, bias [C] (None: none) and state [B,K-1,C], the inputs before
     the first token (None: zeros), of x's type; activation None or "silu".  starts [B,T] (bool or uint8): a token with a start, and
-    those behind it, see nothing before it, so that sequences may follow one another in one row, or be padded on the left.  The new state
+    those behind it, see nothing before it, so that sequences may follow one another in one row, or be padded on the left (where not with
+    finite numbers: the gradients of weight and bias sum over all tokens, and a gradient of zero times a NaN is one).  The new state
     is the last K-1 inputs as far as they are visible (zeros elsewhere), in `state_out` where given (it may be `state` itself but share
     nothing with another tensor; not recorded for autograd, and refused where that asks for gradients).  Differentiable with respect to
     x, weight, bias and state, through both results, once and not in forward mode; sums are float32."""
@@ -117,8 +118,9 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     of zero keeps all of it at any rate; rates below -2^100 / log2(e) count as that); D, dt_bias [C] (None: zeros); state [B,C,N], the
     state before the first token (None: zeros): float32.  softplus=False: d_t = dt_t + dt_bias.  starts [B,T] (bool or uint8): such a token
     finds a state of zero, so that sequences may follow one another in one row, or be padded on the left; nothing before it is seen, not
-    even a NaN.  The new state goes to `state_out` where given (it may be `state` itself but share nothing with another tensor; not
-    recorded for autograd, and refused where that asks for gradients).  Differentiable with respect to all nine, through both results,
+    even a NaN (the gradients of A, D and dt_bias sum over all tokens, though, and those of B and C over a group's channels: a gradient of
+    zero times a NaN is one).  The new state goes to `state_out` where given (contiguous and on 16 bytes; it may be `state` itself but share
+    nothing with another tensor; not recorded for autograd, and refused where that asks for gradients).  Differentiable with respect to all nine, through both results,
     once and not in forward mode.  Steps, decays, states and sums are float32, and results are rounded to bfloat16 once."""
     native = _lib.host().selective(x, dt, A, B, C, D, z, dt_bias, state, starts, softplus, state_out)
     if native is not None:
